@@ -1,0 +1,362 @@
+"""Paged key/value cache in 8 bits: rows quantised as they are written and read back, attention over it.
+
+A page of 16 tokens is a block of bytes per key head: 16 rows of ``D`` key codes (e4m3), 16 rows of value codes, 32 exponents.  A
+row of a token stands for ``code * 2^(byte - 127)``, the exponent being the least one, of -100 to 119, with which the row's largest
+magnitude is at most 448: half the bytes of bf16 and a 64th for ``D`` = 128, every value exactly a bf16 number and off by at most
+2^-4 of itself (2^-10 of 2^exponent where it is smaller than 2^-6 of that).  A row's codes depend on that row alone: neither the
+order nor the portions in which a page is filled change what it holds.
+
+* :func:`write` quantises rows into their slots, :func:`read` gives them back;
+* :func:`decode_attention` is the attention of one query token per sequence (page tables and lengths on the device, as in a captured
+  decode step), :func:`chunk_attention` that of the last tokens of each sequence, causal, by a plan that is made once per step.
+
+CUDA tensors run ``kv_fp8_*.cu``; CPU tensors run the plain PyTorch expressions below (the oracle of the GPU tests).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import Dict, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from ..utils.transfer_stats import to_device
+
+PAGE = 16
+LEAST_EXPONENT, MOST_EXPONENT = -100, 119
+DIMS = (64, 128)
+
+_FN: Dict[str, object] = {}
+
+
+def _fn(name: str):
+    if not _FN:
+        c = ctypes
+        vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
+        _FN["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
+        _FN["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
+        _FN["rows"] = _lib.declare("apb_kv8_rows_attention", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, vp, ll, i, i, i, i, f, vp])
+    return _FN[name]
+
+
+def block_bytes(head_dim: int) -> int:
+    """Bytes of the 16 tokens of a page and key head."""
+    return 2 * PAGE * head_dim + 2 * PAGE
+
+
+class Fp8KVCache:
+    """``data [..., pages, key heads, block]`` uint8: the blocks of one layer, or of all layers in front (:meth:`layer`)."""
+
+    __slots__ = ("data", "head_dim")
+
+    def __init__(self, data: torch.Tensor, head_dim: int):
+        if head_dim not in DIMS:
+            raise ValueError(f"head_dim {head_dim}: the 8-bit cache holds heads of {DIMS[0]} or {DIMS[1]}")
+        if data.dtype != torch.uint8 or data.dim() not in (3, 4) or data.shape[-1] != block_bytes(head_dim):
+            raise ValueError(f"data must be uint8 [(layers,) pages, heads, {block_bytes(head_dim)}], got {data.dtype} {tuple(data.shape)}")
+        if not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError("data must be contiguous and begin on a 16-byte boundary")
+        self.data, self.head_dim = data, head_dim
+
+    @staticmethod
+    def zeros(num_pages: int, num_kv_heads: int, head_dim: int, device="cuda", layers: Optional[int] = None) -> "Fp8KVCache":
+        shape = (num_pages, num_kv_heads, block_bytes(head_dim))
+        return Fp8KVCache(torch.zeros(shape if layers is None else (layers,) + shape, device=device, dtype=torch.uint8), head_dim)
+
+    def layer(self, i: int) -> "Fp8KVCache":
+        return Fp8KVCache(self.data[i], self.head_dim)
+
+    @property
+    def num_pages(self) -> int:
+        return self.data.shape[-3]
+
+    @property
+    def num_kv_heads(self) -> int:
+        return self.data.shape[-2]
+
+    def nbytes(self) -> int:
+        return self.data.numel()
+
+    def parts(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Views: key codes and value codes ``[..., 16, D]``, exponent bytes ``[..., 8, 2, 2]`` (token % 8; key or value; token // 8)."""
+        n = PAGE * self.head_dim
+        k, v = (self.data[..., i * n:(i + 1) * n].unflatten(-1, (PAGE, self.head_dim)) for i in (0, 1))
+        return k, v, self.data[..., 2 * n:].unflatten(-1, (8, 2, 2))
+
+
+def _one_layer(cache: Fp8KVCache) -> torch.Tensor:
+    if cache.data.dim() != 3:
+        raise ValueError("a cache of several layers: take one with .layer(i)")
+    return cache.data
+
+
+def _same_device(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.device != device:
+            raise ValueError(f"{name} lives on {t.device}, not on {device}")
+
+
+def _ints(name: str, t: torch.Tensor, *shape: Optional[int]) -> None:
+    if t.dtype != torch.int32 or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)) \
+            or (t.numel() and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be int32 {[n if n is not None else '*' for n in shape]} with neighbouring elements, got "
+                         f"{t.dtype} {list(t.shape)}")
+
+
+class _On:
+    """Launches go to the tensors' device, whichever is current."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device: torch.device):
+        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+
+
+# --------------------------------------------------------------------------------------------- rows
+def quantise_ref(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``[..., D]`` to codes (uint8) and exponent bytes ``[...]``."""
+    x = x.float()
+    most = torch.nan_to_num(x.abs(), nan=0.0).amax(-1, keepdim=True)
+    mantissa, exponent = torch.frexp(most)                       # 448 = 0.875 * 2^9
+    e = torch.where(most > 0, exponent - 9 + (mantissa > 0.875), LEAST_EXPONENT)
+    e = torch.where(torch.isinf(most), MOST_EXPONENT, e).clamp(LEAST_EXPONENT, MOST_EXPONENT)
+    codes = (x * torch.exp2(-e.float())).clamp(-448, 448).to(torch.float8_e4m3fn)
+    return codes.view(torch.uint8), (e + 127).squeeze(-1).to(torch.uint8)
+
+
+def values_ref(codes: torch.Tensor, byte: torch.Tensor) -> torch.Tensor:
+    """Codes ``[..., D]`` and exponent bytes ``[...]`` to fp32."""
+    return codes.contiguous().view(torch.float8_e4m3fn).float() * torch.exp2(byte.float() - 127)[..., None]
+
+
+def _check_rows(cache: Fp8KVCache, slots: torch.Tensor, distinct: bool = False) -> torch.Tensor:
+    data = _one_layer(cache)
+    _ints("slots", slots, None)
+    from ..utils import checked
+    if checked.active_for(slots):
+        checked.check_range("slots", slots, -(1 << 31), cache.num_pages * PAGE)
+        if distinct:
+            checked.check_distinct("slots", slots)
+    return data
+
+
+def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Fp8KVCache) -> None:
+    """``k``, ``v [T, heads, D]`` (bf16 or fp32; tokens and heads may be strided, as the columns of a projection are) into
+    ``slots [T]`` int32 = page * 16 + token in the page; rows of slots below 0 are left out.  A slot is named once in a call.
+
+    Magnitudes above 448 * 2^119 (2.98e38), infinities among them, become that; what is not a number stays none and leaves the
+    rest of its row alone."""
+    data = _check_rows(cache, slots, distinct=True)
+    T, H, D = slots.shape[0], cache.num_kv_heads, cache.head_dim
+    for name, t in (("k", k), ("v", v)):
+        if t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != k.dtype or tuple(t.shape) != (T, H, D):
+            raise ValueError(f"{name} must be bf16 or fp32 {[T, H, D]}, got {t.dtype} {list(t.shape)}")
+    _same_device(data.device, k=k, v=v, slots=slots)
+    if T == 0:
+        return
+    if not data.is_cuda:
+        ck, cv, ex = cache.parts()
+        at = slots[slots >= 0].long()
+        if at.numel() and int(at.max()) >= cache.num_pages * PAGE:
+            raise ValueError("slots: beyond the cache's pages")
+        page, t = at // PAGE, at % PAGE
+        for w, (codes, x) in enumerate(((ck, k), (cv, v))):
+            c, e = quantise_ref(x[slots >= 0])
+            codes[page, :, t] = c
+            ex[page, :, t % 8, w, t // 8] = e
+        return
+    k, v = _rows_aligned(k), _rows_aligned(v)
+    with _On(data.device):
+        _lib.check(_fn("write")(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(),
+                                data.data_ptr(), T, H, D, cache.num_pages, int(k.dtype == torch.float32), _lib.stream_ptr()),
+                   "kv8_write")
+
+
+def _rows_aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t [T, heads, D]`` itself where its rows are whole and begin on 16-byte boundaries, else a copy."""
+    unit = 16 // t.element_size()
+    if t.stride(2) == 1 and t.stride(0) % unit == 0 and t.stride(1) % unit == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def read(cache: Fp8KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that ``slots [T]`` hold, ``[T, heads, D]`` each, exact in ``dtype`` (bf16 or fp32); zeros for slots below 0."""
+    data = _check_rows(cache, slots)
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"rows are read as bf16 or fp32, not {dtype}")
+    _same_device(data.device, slots=slots)
+    T, H, D = slots.shape[0], cache.num_kv_heads, cache.head_dim
+    if not data.is_cuda:
+        if T and int(slots.max()) >= cache.num_pages * PAGE:
+            raise ValueError("slots: beyond the cache's pages")
+        ck, cv, ex = cache.parts()
+        at = slots.long().clamp_min(0)
+        page, t, keep = at // PAGE, at % PAGE, (slots >= 0)[:, None, None]
+        return tuple(torch.where(keep, values_ref(c[page, :, t], ex[page, :, t % 8, w, t // 8]), 0.0).to(dtype) for w, c in enumerate((ck, cv)))
+    out = torch.empty((2, T, H, D), device=data.device, dtype=dtype)
+    k, v = out[0], out[1]
+    if T:
+        with _On(data.device):
+            _lib.check(_fn("read")(data.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, H, D, cache.num_pages,
+                                   int(dtype == torch.float32), _lib.stream_ptr()), "kv8_read")
+    return k, v
+
+
+# --------------------------------------------------------------------------------------------- attention
+def _check_queries(q: torch.Tensor, cache: Fp8KVCache, out: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    data = _one_layer(cache)
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] == 0 or q.shape[1] % cache.num_kv_heads:
+        raise ValueError(f"q must be bf16 [rows, a multiple of {cache.num_kv_heads} heads, {cache.head_dim}], got {q.dtype} {list(q.shape)}")
+    if out is not None and (out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != q.shape[2]):
+        raise ValueError("out must be bf16 of q's shape with whole rows")
+    _same_device(data.device, q=q, **({} if out is None else {"out": out}))
+    if q.stride(2) != 1 or q.stride(1) != q.shape[2] or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    return q, data
+
+
+def context_ref(cache: Fp8KVCache, pages: torch.Tensor, n: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of the first ``n`` tokens on ``pages``, ``[n, heads, D]`` fp32."""
+    t = torch.arange(n, device=pages.device)
+    return read(cache, (pages.long()[t // PAGE] * PAGE + t % PAGE).to(torch.int32), torch.float32)
+
+
+def attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, last: torch.Tensor, scale: float) -> torch.Tensor:
+    """``q [rows, Hq, D]`` over ``k``, ``v [n, Hkv, D]`` up to token ``last [rows]``; zeros where a row sees nothing."""
+    rep = q.shape[1] // k.shape[1]
+    s = torch.einsum("ihd,thd->hit", q.to(k.dtype), k.repeat_interleave(rep, 1)) * scale
+    seen = torch.arange(k.shape[0], device=q.device) <= last[:, None]
+    s = s.masked_fill(~seen, float("-inf"))
+    p = torch.exp(s - s.amax(-1, keepdim=True).nan_to_num(neginf=0.0)) if k.shape[0] else s
+    total = p.sum(-1)
+    o = torch.einsum("hit,thd->ihd", p, v.repeat_interleave(rep, 1))
+    return o / torch.where(total == 0, 1.0, total).t()[..., None]
+
+
+def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``q [B, Hq, D]`` bf16, one token per sequence, over the first ``lengths [B]`` (int32) tokens on the pages ``page_table
+    [B, max_pages]`` (int32) -> ``[B, Hq, D]`` bf16; zeros for sequences of length 0.  Query head ``h`` reads key head
+    ``h // (Hq // Hkv)``; ``scale``: of the scores, ``D ** -0.5`` if None.  Entries of the table behind a sequence's pages are not looked at."""
+    q, data = _check_queries(q, cache, out)
+    B, Hq, D = q.shape
+    _ints("page_table", page_table, B, None)
+    _ints("lengths", lengths, B)
+    _same_device(data.device, page_table=page_table, lengths=lengths)
+    scale = D ** -0.5 if scale is None else float(scale)
+    from ..utils import checked
+    if checked.active_for(q):
+        checked.check_page_table("page_table", page_table, lengths, cache.num_pages, PAGE)
+    if out is None:
+        out = torch.empty((B, Hq, D), device=q.device, dtype=q.dtype)
+    if B == 0:
+        return out
+    if not data.is_cuda:
+        for b, n in enumerate(lengths.tolist()):
+            k, v = context_ref(cache, page_table[b], n)
+            out[b:b + 1] = attention_ref(q[b:b + 1].float(), k, v, torch.tensor([n - 1]), scale).to(q.dtype)
+        return out
+    with _On(data.device):
+        _lib.check(_fn("rows")(q.data_ptr(), q.stride(0), data.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+                               cache.num_pages, lengths.data_ptr(), None, None, out.data_ptr(), out.stride(0), B, Hq, cache.num_kv_heads, D,
+                               scale, _lib.stream_ptr()), "kv8_rows_attention")
+    return out
+
+
+@dataclass
+class ChunkPlan:
+    """Tables of a step in which every sequence brings some tokens; made on the host once and used by all layers.
+
+    Sequence ``s`` has ``lengths[s]`` tokens in the cache, the last ``new[s]`` of which are its query rows (row ``i`` sees the tokens
+    up to position ``lengths[s] - new[s] + i``; one below 0 sees nothing); the rows of the sequences follow one another."""
+    rows: int
+    new: np.ndarray
+    lengths: np.ndarray
+    pages: List[np.ndarray]
+    heads: int
+    kv_heads: int
+    num_pages: int
+    head_dim: int
+    table: Optional[torch.Tensor] = None
+    d_lengths: Optional[torch.Tensor] = None
+    row_entry: Optional[torch.Tensor] = None
+    row_last: Optional[torch.Tensor] = None
+
+    @staticmethod
+    def build(new: Sequence[int], lengths: Sequence[int], pages, heads: int, cache: Fp8KVCache) -> "ChunkPlan":
+        """``pages``: per sequence its page ids in order (a table's further entries are not looked at)."""
+        new, lengths = np.asarray(new, dtype=np.int64).reshape(-1), np.asarray(lengths, dtype=np.int64).reshape(-1)
+        n = len(new)
+        if len(lengths) != n or len(pages) != n or (new < 0).any() or (lengths < 0).any():
+            raise ValueError("new, lengths and pages describe the same sequences, with counts from 0 on")
+        if heads < 1 or heads % cache.num_kv_heads:
+            raise ValueError(f"{heads} query heads are not a multiple of {cache.num_kv_heads} key heads")
+        need = (lengths + PAGE - 1) // PAGE
+        used = []
+        for s in range(n):
+            p = np.asarray(pages[s]).reshape(-1)[:need[s]]
+            if len(p) < need[s]:
+                raise ValueError(f"sequence {s}: {len(p)} pages do not hold {lengths[s]} tokens")
+            if len(p) and (p.min() < 0 or p.max() >= cache.num_pages):
+                raise ValueError(f"sequence {s}: a page outside the cache's {cache.num_pages}")
+            used.append(p.astype(np.int32))
+        rows = int(new.sum())
+        plan = ChunkPlan(rows, new, lengths, used, heads, cache.num_kv_heads, cache.num_pages, cache.head_dim)
+        if cache.data.is_cuda and rows:
+            wide = max(1, int(need.max()))
+            table = np.zeros((n, wide), dtype=np.int32)
+            for s in range(n):
+                table[s, :need[s]] = used[s]
+            entry = np.repeat(np.arange(n), new)
+            last = np.concatenate([np.arange(l - m, l) for m, l in zip(new, lengths)])
+            flat = np.concatenate([table.reshape(-1), lengths, entry, last]).astype(np.int32)
+            dev = to_device(torch.from_numpy(flat).pin_memory(), cache.data.device)
+            t, plan.d_lengths, plan.row_entry, plan.row_last = dev.split([n * wide, n, rows, rows])
+            plan.table = t.view(n, wide)
+        return plan
+
+
+def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``q [T, Hq, D]`` bf16, the new tokens of the plan's sequences one behind another -> ``[T, Hq, D]`` bf16.  Each row sees the
+    tokens of its sequence up to itself (:class:`ChunkPlan`), rows that see nothing are zeros.  Rows of ``q`` behind the last
+    sequence are padding: they are left as they were in ``out``, zeros without it.  The new tokens' own keys and values are read from the
+    cache: :func:`write` comes first."""
+    q, data = _check_queries(q, cache, out)
+    T, Hq, D = q.shape
+    if (Hq, cache.num_kv_heads, cache.num_pages, D) != (plan.heads, plan.kv_heads, plan.num_pages, plan.head_dim):
+        raise ValueError("the plan was made for other heads or another cache")
+    if T < plan.rows:
+        raise ValueError(f"q has {T} rows, the plan's sequences bring {plan.rows}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if out is None:
+        out = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
+        out[plan.rows:].zero_()
+    if plan.rows == 0:
+        return out
+    if not data.is_cuda:
+        row = 0
+        for m, n, p in zip(plan.new.tolist(), plan.lengths.tolist(), plan.pages):
+            k, v = context_ref(cache, torch.from_numpy(p), n)
+            out[row:row + m] = attention_ref(q[row:row + m].float(), k, v, torch.arange(n - m, n), scale).to(q.dtype)
+            row += m
+        return out
+    _same_device(data.device, plan=plan.table)
+    with _On(data.device):
+        _lib.check(_fn("rows")(q.data_ptr(), q.stride(0), data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.table.shape[1],
+                               cache.num_pages, plan.d_lengths.data_ptr(), plan.row_entry.data_ptr(), plan.row_last.data_ptr(),
+                               out.data_ptr(), out.stride(0), plan.rows, Hq, cache.num_kv_heads, D, scale, _lib.stream_ptr()),
+                   "kv8_rows_attention")
+    return out

@@ -144,6 +144,15 @@ def check_permutation(name: str, table: Any, n: int) -> None:
         raise TableError(f"{name} names {i} {int(seen[i])} times")
 
 
+def check_distinct(name: str, table: Any) -> None:
+    """No entry from 0 on occurs twice."""
+    t = _as_tensor(table).reshape(-1)
+    t = torch.sort(t[t >= 0]).values
+    twice = t[1:] == t[:-1]
+    if bool(twice.any()):
+        raise TableError(f"{name} names {int(t[_first_bad(twice)])} more than once")
+
+
 def check_routing(dst_rank: Any, dst_row: Any, world: int, rows_cap: int, name: str = "routing") -> None:
     """Dispatch entries: rank -1 = dropped; every other entry names a rank of the group and a row of its buffer."""
     r, row = _as_tensor(dst_rank).long(), _as_tensor(dst_row).long()
