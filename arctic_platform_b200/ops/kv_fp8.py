@@ -38,6 +38,7 @@ def _fn(name: str):
         vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
         _FN["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
         _FN["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
+        _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, f, vp])
         _FN["rows"] = _lib.declare("apb_kv8_rows_attention", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, vp, ll, i, i, i, i, f, vp])
     return _FN[name]
 
@@ -57,6 +58,8 @@ class Fp8KVCache:
             raise ValueError(f"head_dim {head_dim}: the 8-bit cache holds heads of {DIMS[0]} or {DIMS[1]}")
         if data.dtype != torch.uint8 or data.dim() not in (3, 4) or data.shape[-1] != block_bytes(head_dim):
             raise ValueError(f"data must be uint8 [(layers,) pages, heads, {block_bytes(head_dim)}], got {data.dtype} {tuple(data.shape)}")
+        if min(data.shape[:-1]) < 1:
+            raise ValueError("a cache has at least one page and head")
         if not data.is_contiguous() or data.data_ptr() % 16:
             raise ValueError("data must be contiguous and begin on a 16-byte boundary")
         self.data, self.head_dim = data, head_dim
@@ -269,9 +272,9 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
             out[b:b + 1] = attention_ref(q[b:b + 1].float(), k, v, torch.tensor([n - 1]), scale).to(q.dtype)
         return out
     with _On(data.device):
-        _lib.check(_fn("rows")(q.data_ptr(), q.stride(0), data.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-                               cache.num_pages, lengths.data_ptr(), None, None, out.data_ptr(), out.stride(0), B, Hq, cache.num_kv_heads, D,
-                               scale, _lib.stream_ptr()), "kv8_rows_attention")
+        _lib.check(_fn("decode")(q.data_ptr(), q.stride(0), data.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+                                 cache.num_pages, lengths.data_ptr(), out.data_ptr(), out.stride(0), B, Hq, cache.num_kv_heads, D, scale,
+                                 _lib.stream_ptr()), "kv8_decode")
     return out
 
 

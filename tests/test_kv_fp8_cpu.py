@@ -117,6 +117,7 @@ def _refusals():
     plan = lambda **a: kv_fp8.ChunkPlan.build(**{**dict(new=[1], lengths=[17], pages=[[0, 1]], heads=4, cache=cache), **a})  # noqa: E731
     return {
         "head size": lambda: kv_fp8.Fp8KVCache.zeros(4, 2, 96, device="cpu"),
+        "no pages": lambda: kv_fp8.Fp8KVCache.zeros(0, 2, 64, device="cpu"),
         "block size": lambda: kv_fp8.Fp8KVCache(torch.zeros(4, 2, 100, dtype=torch.uint8), 64),
         "type of the cache": lambda: kv_fp8.Fp8KVCache(torch.zeros(4, 2, 2080), 64),
         "cache in strides": lambda: kv_fp8.Fp8KVCache(torch.zeros(4, 4, 2080, dtype=torch.uint8)[:, ::2], 64),
