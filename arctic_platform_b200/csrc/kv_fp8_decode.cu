@@ -1,8 +1,8 @@
 // Decode attention (one query token per sequence) over the 8-bit cache (layout: kv_fp8.cuh).
 //
 // Bound by the stream of codes: a page of 16 tokens and one key head is 32 D + 32 bytes that up to 16 query heads share.  A warp walks
-// pages by itself: one TMA copy brings a page's keys and values into its ring of shared memory (swizzled, so that the 16-byte reads
-// below meet no bank twice), the 32 exponents go to registers, a word per lane.
+// pages by itself, two at a time: a TMA copy brings a page's keys and values into its ring of shared memory (swizzled, so that the
+// 16-byte reads below meet no bank twice) while the two before are worked on, the 32 exponents go to registers, a word per lane.
 //
 // Both products run on m16n8k16 MMAs in fp16, transposed: S^T = K Q^T and O^T += V^T W^T.  The 16 rows of a tile are tokens or
 // dimensions, its 8 columns the heads of a group.  Codes become fp16 numbers exactly, by one instruction per pair; which dimension is
@@ -41,7 +41,8 @@ struct Kv8Decode {
 };
 
 constexpr float kKv8Top = 14.f;          // log2 of the largest weight and (about) of the largest query element
-constexpr int kKv8Stages = 4;
+constexpr int kKv8Stages = 2;            // of a warp's ring, two pages each
+constexpr float kKv8None = -1.7e38f;     // a maximum of nothing: finite, so that differences of such are numbers
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -71,7 +72,7 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
 
 template <int D, int H, int WARPS>
 struct Kv8DecodeCfg {
-  static constexpr int kStage = 32 * D;                              // codes of a page
+  static constexpr int kStage = 64 * D;                              // codes of two pages
   static constexpr int kRing = kKv8Stages * kStage;
   static constexpr int kHeads = 8 * H;
   static constexpr int kJoin = (WARPS + 1) * kHeads * (D + 4) * 4;   // the warps' results and the CTA's, in place of the rings
@@ -122,7 +123,7 @@ struct Kv8Heads {
       for (int k = 0; k < 2; ++k) {
         const int e2 = __shfl_sync(0xffffffffu, e, 4 * (2 * c4 + k));
         c[h][k] = scale_log2 * exp2_int(e2);
-        top[h][k] = m[h][k] = -INFINITY;
+        top[h][k] = m[h][k] = kKv8None;
         l[h][k] = 0.f;
       }
 #pragma unroll
@@ -130,54 +131,76 @@ struct Kv8Heads {
     }
   }
 
-  // A page's codes at `stage`, its exponents of tokens g and g + 8 in `ex` (255: no such page); `left` of its tokens count.
-  __device__ __forceinline__ void page(uint32_t stage, uint32_t ex, int left, int lane) {
+  // The codes of two pages at `stage`, their exponents of tokens g and g + 8 in `ex` (255: no such page); `left` of their tokens
+  // count.  Two at a time: the chains of one hide those of the other, and what is done once per maximum is done half as often.
+  __device__ __forceinline__ void pages(uint32_t stage, const uint32_t (&ex)[2], int left, int lane) {
     const int g = lane >> 2, c4 = lane & 3;
-    float s[H][4];
+    float s[2][H][4];
 #pragma unroll
-    for (int h = 0; h < H; ++h) s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
+    for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+      for (int h = 0; h < H; ++h) s[pg][h][0] = s[pg][h][1] = s[pg][h][2] = s[pg][h][3] = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
       const int chunk = D == 128 ? (2 * c4 + i) ^ g : c4 ^ (g >> 1);
-      const uint4 lo = lds128(stage + g * D + chunk * 16), hi = lds128(stage + (g + 8) * D + chunk * 16);
-      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+      uint4 lo[2], hi[2];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t a0, a1, a2, a3;
-        e4m3x4_to_f16(wl[w], a0, a2);
-        e4m3x4_to_f16(wh[w], a1, a3);
-#pragma unroll
-        for (int h = 0; h < H; ++h) mma_f16(s[h], a0, a1, a2, a3, qb[h][4 * i + w][0], qb[h][4 * i + w][1]);
+      for (int pg = 0; pg < 2; ++pg) {
+        lo[pg] = lds128(stage + pg * 32 * D + g * D + chunk * 16);
+        hi[pg] = lds128(stage + pg * 32 * D + (g + 8) * D + chunk * 16);
       }
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
+          const uint32_t wl = w == 0 ? lo[pg].x : w == 1 ? lo[pg].y : w == 2 ? lo[pg].z : lo[pg].w;
+          const uint32_t wh = w == 0 ? hi[pg].x : w == 1 ? hi[pg].y : w == 2 ? hi[pg].z : hi[pg].w;
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_to_f16(wl, a0, a2);
+          e4m3x4_to_f16(wh, a1, a3);
+#pragma unroll
+          for (int h = 0; h < H; ++h) mma_f16(s[pg][h], a0, a1, a2, a3, qb[h][4 * i + w][0], qb[h][4 * i + w][1]);
+        }
     }
-    const uint32_t k0 = ex & 255, k1 = (ex >> 8) & 255, v0 = (ex >> 16) & 255, v1 = ex >> 24;
-    const bool in0 = g < left && k0 != 255, in1 = g + 8 < left && k1 != 255;
-    const float f0 = __uint_as_float(k0 << 23), f1 = __uint_as_float(k1 << 23);
-    const float y0 = static_cast<float>(static_cast<int>(v0) - 127), y1 = static_cast<float>(static_cast<int>(v1) - 127);
-    uint32_t pb[H][2];
+    // tokens g, g + 8 of the first page and of the second
+    float f[4], y[4];
+    bool in[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t k = (ex[t >> 1] >> (8 * (t & 1))) & 255, v = (ex[t >> 1] >> (16 + 8 * (t & 1))) & 255;
+      in[t] = g + 8 * t < left && k != 255;
+      f[t] = __uint_as_float(k << 23);
+      y[t] = static_cast<float>(static_cast<int>(v) - 127);
+    }
+    uint32_t pb[2][H][2];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      float w[4], grown[2];
+      float w[2][4], grown[2];
       bool grew = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float s0 = in0 ? s[h][e] * (f0 * c[h][e]) : -INFINITY, s1 = in1 ? s[h][2 + e] * (f1 * c[h][e]) : -INFINITY;
-        const float m_new = fmaxf(m[h][e], fmaxf(s0, s1)), m_use = m_new == -INFINITY ? 0.f : m_new;
-        l[h][e] = l[h][e] * ex2(m[h][e] - m_use) + (ex2(s0 - m_use) + ex2(s1 - m_use));
+        float x[4], sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = in[t] ? s[t >> 1][h][2 * (t & 1) + e] * (f[t] * c[h][e]) : -INFINITY;
+        const float m_new = fmaxf(fmaxf(m[h][e], fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sum += ex2(x[t] - m_new);
+        l[h][e] = l[h][e] * ex2(m[h][e] - m_new) + sum;
         m[h][e] = m_new;
-        float mx = fmaxf(s0 + y0, s1 + y1);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] += y[t];
+        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
         grown[e] = fmaxf(top[h][e], mx);
         grew |= grown[e] > top[h][e];
-        const float use = (grown[e] == -INFINITY ? 0.f : grown[e]) - kKv8Top;
-        w[e] = ex2(s0 + y0 - use);
-        w[2 + e] = ex2(s1 + y1 - use);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w[e][t] = ex2(x[t] - (grown[e] - kKv8Top));
       }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float alpha = top[h][e] == -INFINITY ? 0.f : ex2(top[h][e] - grown[e]);
+          const float alpha = ex2(top[h][e] - grown[e]);
           top[h][e] = grown[e];
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
@@ -186,40 +209,44 @@ struct Kv8Heads {
           }
         }
       }
-      pb[h][0] = transpose_8x8(pack_f16x2(w[0], w[1]));
-      pb[h][1] = transpose_8x8(pack_f16x2(w[2], w[3]));
-    }
-    // values of tokens 2 c4, 2 c4 + 1 and the same + 8
-    constexpr int W = D / 32;             // words of a lane's dimensions
-    uint32_t x[4][W];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int t = 2 * c4 + (k & 1) + 8 * (k >> 1);
-      if constexpr (D == 128) {
-        const uint4 r = lds128(stage + (16 + t) * D + ((g ^ (t & 7)) << 4));
-        x[k][0] = r.x, x[k][1] = r.y, x[k][2] = r.z, x[k][3] = r.w;
-      } else {
-        const uint2 r = lds64(stage + (16 + t) * D + (((g >> 1) ^ ((t >> 1) & 3)) << 4) + (g & 1) * 8);
-        x[k][0] = r.x, x[k][1] = r.y;
+      for (int t = 0; t < 4; ++t) pb[t >> 1][h][t & 1] = transpose_8x8(pack_f16x2(w[0][t], w[1][t]));
+    }
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg) {
+      // values of tokens 2 c4, 2 c4 + 1 and the same + 8
+      constexpr int W = D / 32;             // words of a lane's dimensions
+      uint32_t x[4][W];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = 2 * c4 + (k & 1) + 8 * (k >> 1);
+        const uint32_t row = stage + pg * 32 * D + (16 + t) * D;
+        if constexpr (D == 128) {
+          const uint4 r = lds128(row + ((g ^ (t & 7)) << 4));
+          x[k][0] = r.x, x[k][1] = r.y, x[k][2] = r.z, x[k][3] = r.w;
+        } else {
+          const uint2 r = lds64(row + (((g >> 1) ^ ((t >> 1) & 3)) << 4) + (g & 1) * 8);
+          x[k][0] = r.x, x[k][1] = r.y;
+        }
       }
-    }
-    if (left < kKv8Page) {                // what lies behind the last token may be anything, and 0 times no number is none
+      if (left < 32) {                // what lies behind the last token may be anything, and 0 times no number is none
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (2 * c4 + (k & 1) + 8 * (k >> 1) >= left)
+        for (int k = 0; k < 4; ++k)
+          if (16 * pg + 2 * c4 + (k & 1) + 8 * (k >> 1) >= left)
 #pragma unroll
-          for (int w = 0; w < W; ++w) x[k][w] = 0u;
-    }
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t a0, a1, a2, a3;
-        e4m3x4_to_f16(__byte_perm(x[0][w], x[1][w], u ? 0x7362 : 0x5140), a0, a1);
-        e4m3x4_to_f16(__byte_perm(x[2][w], x[3][w], u ? 0x7362 : 0x5140), a2, a3);
-#pragma unroll
-        for (int h = 0; h < H; ++h) mma_f16(o[h][2 * w + u], a0, a1, a2, a3, pb[h][0], pb[h][1]);
+            for (int w = 0; w < W; ++w) x[k][w] = 0u;
       }
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_to_f16(__byte_perm(x[0][w], x[1][w], u ? 0x7362 : 0x5140), a0, a1);
+          e4m3x4_to_f16(__byte_perm(x[2][w], x[3][w], u ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+          for (int h = 0; h < H; ++h) mma_f16(o[h][2 * w + u], a0, a1, a2, a3, pb[pg][h][0], pb[pg][h][1]);
+        }
+    }
   }
 
   // sums of a head over its lanes; m and l are then the same in all of them
@@ -231,13 +258,60 @@ struct Kv8Heads {
         float mx = m[h][e];
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-        float sum = m[h][e] == -INFINITY ? 0.f : l[h][e] * ex2(m[h][e] - mx);
-        if (l[h][e] != l[h][e]) sum = l[h][e];         // a score that is no number leaves the maximum alone
+        float sum = l[h][e] * ex2(m[h][e] - mx);
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
         m[h][e] = mx;
         l[h][e] = sum;
       }
+  }
+};
+
+// From numerators in units of 2^(M - 14) and a sum in units of 2^m to results.
+struct Kv8Final {
+  float f, inv;
+  __device__ __forceinline__ Kv8Final(float top, float m, float l) {
+    const bool some = l != 0.f;
+    inv = some ? 1.f / l : 0.f;
+    f = some ? exp2f((top - m - kKv8Top) * 0.5f) : 0.f;       // half of it: values may be far from 1
+  }
+  __device__ __forceinline__ float operator()(float o) const { return inv == 0.f ? 0.f : o * inv * f * f; }
+};
+
+// A warp's ring: copies of two pages each under way while the two before are worked on.
+template <int D>
+struct Kv8Copies {
+  const CUtensorMap* map;
+  const Kv8Decode& p;
+  uint8_t* ring;
+  uint64_t* full;
+  int lane;
+  __device__ __forceinline__ int checked(int id) const {
+    if (static_cast<unsigned>(id) < static_cast<unsigned>(p.pages)) return id;
+    if (p.status) atomicCAS(p.status, 0, kBadTable);
+    return -1;
+  }
+  // copy number j, of pages id0 and (two) id1; `ex`: this lane's exponents, 255s where there is no page
+  __device__ __forceinline__ void ask(int j, int id0, int id1, bool two, int kvh, uint32_t (&ex)[2]) const {
+    const int block0 = id0 * p.Hkv + kvh, block1 = id1 * p.Hkv + kvh, behind = p.pages * p.Hkv;       // behind the cache are zeros
+    if (lane == 0) {
+      uint64_t* bar = &full[j % kKv8Stages];
+      mbar_expect_tx(bar, (two ? 2 : 1) * 32 * D);
+      tma_load_3d(ring + j % kKv8Stages * 64 * D, map, bar, 0, 0, id0 < 0 ? behind : block0);
+      if (two) tma_load_3d(ring + j % kKv8Stages * 64 * D + 32 * D, map, bar, 0, 0, id1 < 0 ? behind : block1);
+    }
+    const uint8_t* at = p.data + 2 * Kv8<D>::kHalf + (lane & 28);
+    ex[0] = id0 < 0 ? ~0u : __ldcg(reinterpret_cast<const uint32_t*>(at + static_cast<long long>(block0) * Kv8<D>::kBlock));
+    ex[1] = !two || id1 < 0 ? ~0u : __ldcg(reinterpret_cast<const uint32_t*>(at + static_cast<long long>(block1) * Kv8<D>::kBlock));
+  }
+  __device__ __forceinline__ bool wait(int j) const {
+    return __all_sync(0xffffffffu, mbar_wait(&full[j % kKv8Stages], (j / kKv8Stages) & 1, p.status, kTimeoutFull));
+  }
+  __device__ __forceinline__ uint32_t stage(int j) const { return smem_u32(ring) + j % kKv8Stages * 64 * D; }
+  __device__ __forceinline__ void give_up() const {       // copies that are late may still write to the ring
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 100000ull) {
+    }
   }
 };
 
@@ -266,57 +340,35 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
     if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kBadTable);
     len = p.max_pages * kKv8Page;
   }
-  const int n_pages = (max(len, 0) + kKv8Page - 1) / kKv8Page;
-  const int per = (n_pages + p.splits - 1) / p.splits, p0 = split * per, p1 = min(n_pages, p0 + per);
-  const int first = p0 + warp, n = (p1 - first + WARPS - 1) / WARPS;      // pages first, first + WARPS, ... (n <= 0: none)
+  const int n_pages = (max(len, 0) + kKv8Page - 1) / kKv8Page, pairs = (n_pages + 1) / 2;
+  const int per = (pairs + p.splits - 1) / p.splits, p0 = split * per, p1 = min(pairs, p0 + per);
+  const int first = p0 + warp, n = (p1 - first + WARPS - 1) / WARPS;      // pairs of pages first, first + WARPS, ... (n <= 0: none)
   const int* table = p.table + b * p.ld_table;
-  const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing;
-  const int blocks = p.pages * p.Hkv;
-
-  int ids = 0;                              // of pages [j & ~31, + 32) of the walk, a lane each
-  auto load_ids = [&](int j) {
-    ids = j + lane < n ? table[first + (j + lane) * WARPS] : 0;
-    if (static_cast<unsigned>(ids) >= static_cast<unsigned>(p.pages)) {
-      if (p.status) atomicCAS(p.status, 0, kBadTable);
-      ids = -1;
-    }
-  };
-  // asks for page j; returns this lane's exponents
+  Kv8Copies<D> copies{&map, p, smem + warp * Cfg::kRing, full, lane};
+  int ids = 0;                              // of pairs [j & ~15, + 16) of the walk, two lanes each
+  uint32_t next[2] = {~0u, ~0u};
   auto issue = [&](int j) {
-    if ((j & 31) == 0) load_ids(j);
-    const int id = __shfl_sync(0xffffffffu, ids, j & 31);
-    if (j >= n) return 0u;
-    const int block = id < 0 ? blocks : id * p.Hkv + kvh;       // a place behind the cache reads as zeros
-    if (lane == 0) {
-      uint64_t* bar = &full[j % kKv8Stages];
-      mbar_expect_tx(bar, Cfg::kStage);
-      tma_load_3d(smem + warp * Cfg::kRing + j % kKv8Stages * Cfg::kStage, &map, bar, 0, 0, block);
+    if ((j & 15) == 0) {
+      const int at = 2 * (first + (j + (lane >> 1)) * WARPS) + (lane & 1);
+      ids = copies.checked(j + (lane >> 1) < n && at < n_pages ? table[at] : 0);
     }
-    return id < 0 ? 0xFFFFFFFFu
-                  : __ldcg(reinterpret_cast<const uint32_t*>(p.data + static_cast<long long>(block) * Kv8<D>::kBlock + 2 * Kv8<D>::kHalf) + (lane >> 2));
+    const int id0 = __shfl_sync(0xffffffffu, ids, 2 * (j & 15)), id1 = __shfl_sync(0xffffffffu, ids, 2 * (j & 15) + 1);
+    if (j < n) copies.ask(j, id0, id1, 2 * (first + j * WARPS) + 1 < n_pages, kvh, next);
   };
   Kv8Heads<D, H> acc;
-  uint32_t ex[kKv8Stages - 1];
-#pragma unroll
-  for (int j = 0; j < kKv8Stages - 1; ++j) ex[j] = issue(j);
+  issue(0);
   acc.start(p.q + b * p.ldq + head0 * D, heads, p.scale_log2, lane);
   bool ok = true;
 #pragma unroll 1
   for (int j = 0; j < n; ++j) {
-    const uint32_t now = ex[0];
-#pragma unroll
-    for (int i = 0; i + 1 < kKv8Stages - 1; ++i) ex[i] = ex[i + 1];
-    ex[kKv8Stages - 2] = issue(j + kKv8Stages - 1);
-    ok = __all_sync(0xffffffffu, mbar_wait(&full[j % kKv8Stages], (j / kKv8Stages) & 1, p.status, kTimeoutFull));
+    const uint32_t ex[2] = {next[0], next[1]};
+    issue(j + 1);
+    ok = copies.wait(j);
     if (!ok) break;
-    acc.page(ring + j % kKv8Stages * Cfg::kStage, now, len - (first + j * WARPS) * kKv8Page, lane);
+    acc.pages(copies.stage(j), ex, len - 2 * (first + j * WARPS) * kKv8Page, lane);
     __syncwarp();
   }
-  if (!ok) {
-    const uint64_t t0 = global_timer_ns();
-    while (global_timer_ns() - t0 < 100000ull) {
-    }
-  }
+  if (!ok) copies.give_up();
   acc.finish();
 
   // the warps of the CTA, then the CTAs of the cluster
@@ -344,22 +396,19 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
   __syncthreads();
   // joins `parts` results of one head and dimension, in the order of their places
   auto join = [&](int parts, auto top_of, auto m_of, auto l_of, auto o_of, float& top, float& m, float& l, float& o) {
-    top = m = -INFINITY;
+    top = m = kKv8None;
     for (int k = 0; k < parts; ++k) top = fmaxf(top, top_of(k)), m = fmaxf(m, m_of(k));
     l = o = 0.f;
     for (int k = 0; k < parts; ++k) {
       const float lk = l_of(k);
       if (lk == 0.f) continue;                               // nothing seen
       const float mk = m_of(k), tk = top_of(k);
-      l += lk * (mk == -INFINITY ? 1.f : ex2(mk - m));
-      o += o_of(k) * (tk == -INFINITY ? 1.f : ex2(tk - top));
+      l += lk * ex2(mk - m);
+      o += o_of(k) * ex2(tk - top);
     }
   };
   auto finished = [&](int head, int d, float top, float m, float l, float o) {
-    // 2^(top - m) may be far from 1 where the values are: half of it at a time
-    const float f = l == 0.f ? 0.f : exp2f((top - m - kKv8Top) * 0.5f);
-    const float v = l == 0.f ? 0.f : o / l * f * f;
-    p.out[b * p.ldo + (head0 + head) * D + d] = __float2bfloat16(m == -INFINITY && l != 0.f ? l : v);
+    p.out[b * p.ldo + (head0 + head) * D + d] = __float2bfloat16(Kv8Final(top, m, l)(o));
   };
   for (int i = threadIdx.x; i < heads * D; i += 32 * WARPS) {
     const int head = i / D, d = i % D;
@@ -423,7 +472,7 @@ using namespace apb;
 int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* table, long long ld_table, int max_pages, int pages,
                    const int* lengths, void* out, long long ldo, int B, int Hq, int Hkv, int D, float scale, cudaStream_t s) {
   if (B <= 0) return 0;
-  if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || pages < 0 || max_pages < 0 || static_cast<long long>(pages) * Hkv >= (1ll << 31) - 1 ||
+  if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || pages < 1 || max_pages < 0 || static_cast<long long>(pages) * Hkv >= (1ll << 31) - 1 ||
       ldq % 8 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(data) % 16)
     return kBadArgument;
   const int R = Hq / Hkv, H = R > 8 ? 2 : 1, groups = (R + 8 * H - 1) / (8 * H);
