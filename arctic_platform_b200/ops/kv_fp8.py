@@ -39,7 +39,7 @@ def _fn(name: str):
         _FN["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
         _FN["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
         _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, f, vp])
-        _FN["rows"] = _lib.declare("apb_kv8_rows_attention", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, vp, ll, i, i, i, i, f, vp])
+        _FN["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, i, vp, i, i, vp, vp, ll, i, i, i, i, f, vp])
     return _FN[name]
 
 
@@ -278,6 +278,25 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
     return out
 
 
+def _work(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: int) -> Tuple[np.ndarray, np.ndarray, int]:
+    """Items, joins and scratch tiles (``csrc/runtime_kv8.cpp``)."""
+    fn = _lib.rt_lib().apb_rt_kv8_plan
+    c = ctypes
+    fn.argtypes, fn.restype = [c.c_void_p, c.c_void_p, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_void_p, c.c_int64, c.c_void_p, c.c_int64,
+                               c.c_void_p], c.c_int32
+    new, lengths = np.ascontiguousarray(new, dtype=np.int32), np.ascontiguousarray(lengths, dtype=np.int32)
+    counts = np.zeros(3, dtype=np.int64)
+    items, joins = np.empty((0, 12), dtype=np.int32), np.empty((0, 8), dtype=np.int32)
+    for _ in range(2):
+        if fn(new.ctypes.data, lengths.ctypes.data, len(new), heads, kv_heads, sms, items.ctypes.data, len(items), joins.ctypes.data,
+              len(joins), counts.ctypes.data) != 0:
+            raise ValueError("chunk plan: sizes out of range")
+        if len(items) == counts[0]:
+            break
+        items, joins = np.empty((int(counts[0]), 12), dtype=np.int32), np.empty((int(counts[1]), 8), dtype=np.int32)
+    return items, joins, int(counts[2])
+
+
 @dataclass
 class ChunkPlan:
     """Tables of a step in which every sequence brings some tokens; made on the host once and used by all layers.
@@ -292,10 +311,10 @@ class ChunkPlan:
     kv_heads: int
     num_pages: int
     head_dim: int
-    table: Optional[torch.Tensor] = None
-    d_lengths: Optional[torch.Tensor] = None
-    row_entry: Optional[torch.Tensor] = None
-    row_last: Optional[torch.Tensor] = None
+    table: Optional[torch.Tensor] = None             # on the cache's device: pages, work items, joins of items cut along the keys
+    items: Optional[torch.Tensor] = None
+    joins: Optional[torch.Tensor] = None
+    part_tiles: int = 0                              # tiles of 128 rows of scratch
 
     @staticmethod
     def build(new: Sequence[int], lengths: Sequence[int], pages, heads: int, cache: Fp8KVCache) -> "ChunkPlan":
@@ -306,6 +325,8 @@ class ChunkPlan:
             raise ValueError("new, lengths and pages describe the same sequences, with counts from 0 on")
         if heads < 1 or heads % cache.num_kv_heads:
             raise ValueError(f"{heads} query heads are not a multiple of {cache.num_kv_heads} key heads")
+        if new.sum() >= 1 << 31 or (n and lengths.max() >= 1 << 31):
+            raise ValueError("more rows or tokens than 2^31")
         need = (lengths + PAGE - 1) // PAGE
         used = []
         for s in range(n):
@@ -318,16 +339,15 @@ class ChunkPlan:
         rows = int(new.sum())
         plan = ChunkPlan(rows, new, lengths, used, heads, cache.num_kv_heads, cache.num_pages, cache.head_dim)
         if cache.data.is_cuda and rows:
-            wide = max(1, int(need.max()))
-            table = np.zeros((n, wide), dtype=np.int32)
+            sms = torch.cuda.get_device_properties(cache.data.device).multi_processor_count
+            items, joins, plan.part_tiles = _work(new, lengths, heads, cache.num_kv_heads, sms)
+            table = np.zeros((n, max(1, int(need.max()))), dtype=np.int32)
             for s in range(n):
                 table[s, :need[s]] = used[s]
-            entry = np.repeat(np.arange(n), new)
-            last = np.concatenate([np.arange(l - m, l) for m, l in zip(new, lengths)])
-            flat = np.concatenate([table.reshape(-1), lengths, entry, last]).astype(np.int32)
-            dev = to_device(torch.from_numpy(flat).pin_memory(), cache.data.device)
-            t, plan.d_lengths, plan.row_entry, plan.row_last = dev.split([n * wide, n, rows, rows])
-            plan.table = t.view(n, wide)
+            flat = torch.from_numpy(np.concatenate([items.reshape(-1), joins.reshape(-1), table.reshape(-1)])).pin_memory()
+            dev = to_device(flat, cache.data.device)
+            plan.items, plan.joins, plan.table = (t.view(a.shape) for t, a in zip(dev.split([items.size, joins.size, table.size]),
+                                                                                (items, joins, table)))
         return plan
 
 
@@ -336,7 +356,7 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
     """``q [T, Hq, D]`` bf16, the new tokens of the plan's sequences one behind another -> ``[T, Hq, D]`` bf16.  Each row sees the
     tokens of its sequence up to itself (:class:`ChunkPlan`), rows that see nothing are zeros.  Rows of ``q`` behind the last
     sequence are padding: they are left as they were in ``out``, zeros without it.  The new tokens' own keys and values are read from the
-    cache: :func:`write` comes first."""
+    cache: :func:`write` comes first.  Values whose tokens' exponents lie more than 100 below the largest of their sequence lose bits."""
     q, data = _check_queries(q, cache, out)
     T, Hq, D = q.shape
     if (Hq, cache.num_kv_heads, cache.num_pages, D) != (plan.heads, plan.kv_heads, plan.num_pages, plan.head_dim):
@@ -346,7 +366,8 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
     scale = D ** -0.5 if scale is None else float(scale)
     if out is None:
         out = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
-        out[plan.rows:].zero_()
+        if T > plan.rows:
+            out[plan.rows:].zero_()
     if plan.rows == 0:
         return out
     if not data.is_cuda:
@@ -356,10 +377,15 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
             out[row:row + m] = attention_ref(q[row:row + m].float(), k, v, torch.arange(n - m, n), scale).to(q.dtype)
             row += m
         return out
-    _same_device(data.device, plan=plan.table)
+    if plan.items is None or plan.items.device != data.device:
+        raise ValueError(f"the plan was not made for a cache on {data.device}")
+    if out.stride(0) % 8 or out.data_ptr() % 16:             # rows off the 16-byte boundaries: by way of a copy
+        out[:plan.rows].copy_(chunk_attention(q, cache, plan, scale)[:plan.rows])
+        return out
     with _On(data.device):
-        _lib.check(_fn("rows")(q.data_ptr(), q.stride(0), data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.table.shape[1],
-                               cache.num_pages, plan.d_lengths.data_ptr(), plan.row_entry.data_ptr(), plan.row_last.data_ptr(),
-                               out.data_ptr(), out.stride(0), plan.rows, Hq, cache.num_kv_heads, D, scale, _lib.stream_ptr()),
-                   "kv8_rows_attention")
+        scratch = torch.empty(plan.part_tiles * 128 * (D + 2), device=q.device, dtype=torch.float32) if plan.part_tiles else None
+        _lib.check(_fn("chunk")(q.data_ptr(), q.stride(0), data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
+                                plan.items.shape[0], plan.joins.data_ptr(), plan.joins.shape[0], plan.part_tiles,
+                                None if scratch is None else scratch.data_ptr(), out.data_ptr(), out.stride(0), T, Hq, cache.num_kv_heads, D,
+                                scale, _lib.stream_ptr()), "kv8_chunk")
     return out
