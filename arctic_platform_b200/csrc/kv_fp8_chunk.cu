@@ -43,8 +43,11 @@ struct Kv8Chunk {
   int* status;
 };
 
-constexpr int kKcThreads = 384;
-constexpr int kKcRegsIssue = 56, kKcRegsSoftmax = 224;     // 56 + 2 * 224 = 3 * 168
+// Four warpgroups: issue, codes to tiles, two of softmax.  Registers move between them: 40 + 72 + 2 * 200 = 4 * 128, what the block was
+// launched with.
+constexpr int kKcThreads = 512;
+constexpr int kKcConvert = 4;               // warps that turn codes into tiles
+constexpr int kKcRegsIssue = 40, kKcRegsConvert = 72, kKcRegsSoftmax = 200;
 constexpr int kKcBlock = 128;
 constexpr int kKcStages = 2, kKcMeta = 4;
 
@@ -95,10 +98,10 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
   if (threadIdx.x == 0) {
     for (int s = 0; s < kKcStages; ++s) {
       mbar_init(&st_full[s], 1);
-      mbar_init(&st_empty[s], 2);
+      mbar_init(&st_empty[s], kKcConvert);
     }
     for (int s = 0; s < kRing; ++s) {
-      mbar_init(&kv_full[s], 2);
+      mbar_init(&kv_full[s], kKcConvert);
       mbar_init(&kv_empty[s], 1);
     }
     mbar_init(q_full, 1);
@@ -256,9 +259,12 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
           }
         }
       }
-    } else {
+    }
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKcRegsConvert));
+    {
       // ---------------------------------------------------------------- codes to tiles
-      const int half = warp - 2;
+      const int part = warp - 4;
       constexpr int kUnits = D / 16;         // of 16 codes in a row
       bool ok = true;
       int st = 0, slot = 0;
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
           kmax = __reduce_max_sync(0xffffffffu, kmax);
           vmax = __reduce_max_sync(0xffffffffu, vmax);
           if (j == 0 || vmax > vref + 7) vref = vmax;       // factors up to 2^127 do without a new one
-          if (half == 0 && lane == 0) meta[n_blocks % kKcMeta] = make_int2(kmax - 127, vref - 127);
+          if (part == 0 && lane == 0) meta[n_blocks % kKcMeta] = make_int2(kmax - 127, vref - 127);
           ++n_blocks;
 #pragma unroll 1
           for (int which = 0; which < 2 && ok; ++which) {
@@ -292,27 +298,38 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
             const uint32_t sign = which ? 0u : p.key_sign;
             ok = wait(&kv_empty[slot], phase ^ 1, kTimeoutEmpty);
             if (!ok) break;
-            uint8_t* tile = smem_kv + slot * Cfg::kTile;
-            const int c = lane % kUnits, u0 = 2 * (c & 3) + (c >> 2);       // the upper half of a row takes its units the other way around:
-            const uint32_t col = (c >> 2) * 16384;                          // no bank is met twice
-#pragma unroll 2
-            for (int i = 0; i < 2 * kUnits; ++i) {
-              const int t = (i * 64 + half * 32 + lane) / kUnits;
-              const uint8_t* block = stage + (t >> 4) * Kv8<D>::kBlock;
-              uint4 w = *reinterpret_cast<const uint4*>(block + which * Kv8<D>::kHalf + (t & 15) * D + c * 16);
-              const int e = block[2 * Kv8<D>::kHalf + kv8_exponent_at(t & 15, which)];
-              uint32_t f = static_cast<uint32_t>(max(127 + 120 + e - ref, 0)) << 7;
-              f = f << 16 | f | sign;
-              if (t >= valid) w = make_uint4(0, 0, 0, 0), f = 0;
-              uint4 a, b;
-              e4m3x4_to_bf16(w.x, f, a.x, a.y);
-              e4m3x4_to_bf16(w.y, f, a.z, a.w);
-              e4m3x4_to_bf16(w.z, f, b.x, b.y);
-              e4m3x4_to_bf16(w.w, f, b.z, b.w);
-              uint8_t* row = tile + col + t * 128;
-              const bool swap = c >> 2;
-              *reinterpret_cast<uint4*>(row + ((u0 ^ (t & 7)) << 4)) = swap ? b : a;
-              *reinterpret_cast<uint4*>(row + (((u0 ^ 1) ^ (t & 7)) << 4)) = swap ? a : b;
+            // A lane has the same 16 columns of every second or fourth token ...; the upper half of a row takes its two units the other
+            // way around, so that no bank is met twice.
+            const int c = lane % kUnits, u0 = 2 * (c & 3) + (c >> 2), t0 = (part * 32 + lane) / kUnits;
+            constexpr int kStep = 32 * kKcConvert / kUnits, kAt = 4;           // tokens between a lane's, of them at a time
+            const bool swap = c >> 2;
+            const uint32_t tile = smem_u32(smem_kv) + slot * Cfg::kTile + (c >> 2) * 16384;
+            const uint32_t codes = smem_u32(stage) + which * Kv8<D>::kHalf + c * 16, exps = smem_u32(stage) + 2 * Kv8<D>::kHalf;
+#pragma unroll 1
+            for (int i = 0; i < 128 / kStep; i += kAt) {
+              uint4 w[kAt];
+              int e[kAt];
+#pragma unroll
+              for (int k = 0; k < kAt; ++k) {
+                const int t = t0 + (i + k) * kStep;
+                w[k] = lds128(codes + (t >> 4) * Kv8<D>::kBlock + (t & 15) * D);
+                e[k] = lds8(exps + (t >> 4) * Kv8<D>::kBlock + kv8_exponent_at(t & 15, which));
+              }
+#pragma unroll
+              for (int k = 0; k < kAt; ++k) {
+                const int t = t0 + (i + k) * kStep;
+                uint32_t f = static_cast<uint32_t>(max(127 + 120 + e[k] - ref, 0)) << 7;
+                f = f << 16 | f | sign;
+                if (t >= valid) w[k] = make_uint4(0, 0, 0, 0), f = 0;
+                uint4 a, b;
+                e4m3x4_to_bf16(swap ? w[k].z : w[k].x, f, a.x, a.y);
+                e4m3x4_to_bf16(swap ? w[k].w : w[k].y, f, a.z, a.w);
+                e4m3x4_to_bf16(swap ? w[k].x : w[k].z, f, b.x, b.y);
+                e4m3x4_to_bf16(swap ? w[k].y : w[k].w, f, b.z, b.w);
+                const uint32_t row = tile + t * 128, u = (u0 ^ (t & 7)) << 4;
+                sts128(row + u, a);
+                sts128(row + (u ^ 16), b);
+              }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -328,7 +345,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
   } else {
     // ------------------------------------------------------------------ softmax groups
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKcRegsSoftmax));
-    const int g = (warp >> 2) - 1, quarter = warp & 3, row = quarter * 32 + lane;
+    const int g = (warp >> 2) - 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem_base + lane_off + g * 128, t_o = tmem_base + lane_off + 256 + g * 128;
     const int row_token = g * p.tp + row / p.hp, row_head = row % p.hp;
