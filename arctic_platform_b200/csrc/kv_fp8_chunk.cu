@@ -43,11 +43,11 @@ struct Kv8Chunk {
   int* status;
 };
 
-// Four warpgroups: issue, codes to tiles, two of softmax.  Registers move between them: 40 + 72 + 2 * 200 = 4 * 128, what the block was
+// Four warpgroups: issue, codes to tiles, two of softmax.  Registers move between them: 80 + 96 + 2 * 168 = 4 * 128, what the block was
 // launched with.
 constexpr int kKcThreads = 512;
 constexpr int kKcConvert = 4;               // warps that turn codes into tiles
-constexpr int kKcRegsIssue = 40, kKcRegsConvert = 72, kKcRegsSoftmax = 200;
+constexpr int kKcRegsIssue = 80, kKcRegsConvert = 96, kKcRegsSoftmax = 168;
 constexpr int kKcBlock = 128;
 constexpr int kKcStages = 2, kKcMeta = 4;
 
@@ -371,20 +371,28 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         const float c1 = fmaxf(p.scale_log2 * exp2_int(ref.x), 1.2e-38f);
         const uint64_t c2 = xtc_pair(c1, c1);
         const int limit = seen - j * kKcBlock;
-        uint32_t v[4][32];
+        const bool masked = __any_sync(0xffffffffu, limit < kKcBlock);
+        // twice through the scores, 32 columns at a time and the next ones on their way: all 128 in registers spilled
+        uint32_t v[2][32];
+        auto mask = [&](int c, uint32_t (&x)[32]) {
+          if (masked) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, v[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_wait(v[c]);
-        if (__any_sync(0xffffffffu, limit < kKcBlock)) {
-#pragma unroll
-          for (int c = 0; c < kKcBlock; ++c)
-            if (c >= limit) v[c / 32][c % 32] = 0xff800000u;
-        }
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= limit) x[i] = 0xff800000u;
+          }
+        };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld_32x32(t_s, v[0]);
+        tmem_ld_wait(v[0]);
 #pragma unroll
-        for (int c = 0; c < kKcBlock; c += 2)
-          mx[(c >> 1) & 3] = fmaxf(fmaxf(mx[(c >> 1) & 3], __uint_as_float(v[c / 32][c % 32])), __uint_as_float(v[c / 32][c % 32 + 1]));
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_32x32(t_s + ((c + 1) & 3) * 32, v[(c + 1) & 1]);
+          mask(c, v[c & 1]);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            mx[(i >> 1) & 3] = fmaxf(fmaxf(mx[(i >> 1) & 3], __uint_as_float(v[c & 1][i])), __uint_as_float(v[c & 1][i + 1]));
+          tmem_ld_wait(v[(c + 1) & 1]);
+        }
         const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1);
         if (j == 0) ev = ref.y;
         if (__any_sync(0xffffffffu, m_new > m_run) || ev != ref.y) {
@@ -417,15 +425,18 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          if (c < 3) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
+          mask(c, v[c & 1]);
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float2 f = xtc_unpair(xtc_fma2(xtc_pair(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), c2, nm2));
+            float2 f = xtc_unpair(xtc_fma2(xtc_pair(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), c2, nm2));
             f.x = xtc_ex2(f.x);
             f.y = xtc_ex2(f.y);
             sum[i & 1] = xtc_add2(sum[i & 1], xtc_pair(f.x, f.y));
             pk[i] = pack_bf16x2(f.x, f.y);
           }
+          if (c < 3) tmem_ld_wait(v[(c + 1) & 1]);
           tmem_st_32x16(t_s + c * 16, pk);
         }
         tmem_st_wait();
