@@ -51,12 +51,12 @@ constexpr int kKcRegsIssue = 80, kKcRegsConvert = 96, kKcRegsSoftmax = 168;
 constexpr int kKcBlock = 128;
 constexpr int kKcStages = 2, kKcMeta = 4;
 
-template <int D>
+template <int D, bool DUAL>
 struct Kv8ChunkCfg {
   static constexpr int kTile = 128 * D * 2;
-  static constexpr int kRing = 3;
+  static constexpr int kQ = DUAL ? 1 : 2, kRing = DUAL ? 4 : 3;      // tiles
   static constexpr int kStage = 8 * Kv8<D>::kBlock;
-  static constexpr int kSmem = (2 + kRing) * kTile + kKcStages * kStage + 256 + 1024;
+  static constexpr int kSmem = (kQ + kRing) * kTile + kKcStages * kStage + 256 + (DUAL ? 1024 : 0) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
 };
 
@@ -73,14 +73,15 @@ __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t factor, uint
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(factor));
 }
 
-template <int D>
+// DUAL: items of one tile each; the two softmax groups take every second block of it and join what they have at the item's end.
+template <int D, bool DUAL>
 __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_constant__ CUtensorMap tma_q, const Kv8Chunk p) {
-  using Cfg = Kv8ChunkCfg<D>;
+  using Cfg = Kv8ChunkCfg<D, DUAL>;
   constexpr int kRing = Cfg::kRing, kChunks = D / 64;
   extern __shared__ uint8_t kc_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kc_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_q = smem;
-  uint8_t* smem_kv = smem + 2 * Cfg::kTile;
+  uint8_t* smem_kv = smem + Cfg::kQ * Cfg::kTile;
   uint8_t* smem_st = smem_kv + kRing * Cfg::kTile;
   uint64_t* st_full = reinterpret_cast<uint64_t*>(smem_st + kKcStages * Cfg::kStage);
   uint64_t* st_empty = st_full + kKcStages;
@@ -91,8 +92,11 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
   uint64_t* s_full = q_empty + 1;      // [2]
   uint64_t* p_full = s_full + 2;       // [2]
   uint64_t* o_full = p_full + 2;       // [2] once per item
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* pair = o_full + 2;         // DUAL: both softmax groups
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pair + 1);
   int2* meta = reinterpret_cast<int2*>(tmem_holder + 2);      // [kKcMeta] reference exponents of a block's keys and values
+  float* other = reinterpret_cast<float*>(st_full) + 64;      // [2][128] DUAL: a number per row and group
+  int* other_ev = reinterpret_cast<int*>(meta + kKcMeta);     // [2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -111,6 +115,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
       mbar_init(&p_full[g], 128);
       mbar_init(&o_full[g], 1);
     }
+    mbar_init(pair, 256);
     mbar_fence_init();
     tma_prefetch_desc(&tma_q);
   }
@@ -119,7 +124,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
     tmem_relinquish();
   }
   // rows that no query fills stay zeros
-  for (int i = threadIdx.x; i < 2 * Cfg::kTile / 16; i += kKcThreads) reinterpret_cast<uint4*>(smem_q)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < Cfg::kQ * Cfg::kTile / 16; i += kKcThreads) reinterpret_cast<uint4*>(smem_q)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
@@ -155,7 +160,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         if (at < 0) continue;
         const Kv8Item w = p.items[at];
         if (w.blocks == 0) continue;
-        const int tiles = w.tokens > p.tp ? 2 : 1, pages = (w.len + kKv8Page - 1) / kKv8Page;
+        const int tiles = !DUAL && w.tokens > p.tp ? 2 : 1, pages = (w.len + kKv8Page - 1) / kKv8Page;
         const int* table = p.table + w.seq * p.ld_table;
         auto page_of = [&](int j) {        // of block j, a lane each
           const int i = (w.block0 + j) * 8 + lane;
@@ -197,10 +202,10 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
       const uint64_t desc_q = umma_smem_desc(smem_u32(smem_q), 0, 1024), desc_k = umma_smem_desc(smem_u32(smem_kv), 0, 1024);
       const uint64_t desc_v = umma_smem_desc(smem_u32(smem_kv), 16384, 1024);
       constexpr uint32_t kT = Cfg::kTile >> 4;
-      auto issue_s = [&](uint32_t g, uint32_t slot) {
+      auto issue_s = [&](uint32_t g, uint32_t slot, uint32_t q) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_bf16_ss(tmem_base + g * 128, desc_q + g * kT + (k / 4) * 1024 + (k % 4) * 2, desc_k + slot * kT + (k / 4) * 1024 + (k % 4) * 2,
+          umma_bf16_ss(tmem_base + g * 128, desc_q + q * kT + (k / 4) * 1024 + (k % 4) * 2, desc_k + slot * kT + (k / 4) * 1024 + (k % 4) * 2,
                        idesc_s, k > 0 ? 1u : 0u);
         tc_commit(&s_full[g]);
       };
@@ -217,17 +222,49 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         return r;
       };
       bool ok = true;
+      uint32_t tile = 0;               // DUAL: number of the item's first tile
       for (int round = 0; round < rounds && ok; ++round) {
         const int at = item_at(round);
         if (at < 0) continue;
-        const int blocks = p.items[at].blocks, tiles = p.items[at].tokens > p.tp ? 2 : 1;
+        const int blocks = p.items[at].blocks, tiles = !DUAL && p.items[at].tokens > p.tp ? 2 : 1;
         if (blocks == 0) continue;
+        if constexpr (DUAL) {
+          auto wait_tile = [&](uint32_t t) { return wait(&kv_full[t % kRing], (t / kRing) & 1, kTimeoutFull); };
+          auto scores = [&](int j) {   // of block j, when its keys are there
+            const uint32_t t = tile + 2 * j;
+            if (!wait_tile(t)) return false;
+            if (elect_one()) {
+              issue_s(j & 1, t % kRing, 0);
+              tc_commit(&kv_empty[t % kRing]);
+              if (j + 1 == blocks) tc_commit(q_empty);
+            }
+            __syncwarp();
+            return true;
+          };
+          ok = wait(q_full, n_q & 1, kTimeoutFull) && scores(0) && (blocks == 1 || scores(1));
+          ++n_q;
+          for (int j = 0; j < blocks && ok; ++j) {
+            const uint32_t g = j & 1, t = tile + 2 * j + 1;
+            ok = wait_tile(t) && wait(&p_full[g], done[g] & 1, kTimeoutTmemEmpty);
+            if (!ok) break;
+            ++done[g];
+            if (elect_one()) {
+              issue_o(g, t % kRing, j < 2);
+              tc_commit(&kv_empty[t % kRing]);
+              if (j + 2 >= blocks) tc_commit(&o_full[g]);
+            }
+            __syncwarp();
+            if (j + 2 < blocks) ok = scores(j + 2);
+          }
+          tile += 2 * blocks;
+          continue;
+        }
         int sk = slot;
         ok = wait(q_full, n_q & 1, kTimeoutFull) && wait_slot();
         if (!ok) break;
         ++n_q;
         if (elect_one()) {
-          for (int g = 0; g < tiles; ++g) issue_s(g, sk);
+          for (int g = 0; g < tiles; ++g) issue_s(g, sk, g);
           tc_commit(&kv_empty[sk]);
           if (blocks == 1) tc_commit(q_empty);
         }
@@ -246,7 +283,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
             if (elect_one()) {
               issue_o(g, sv, j == 0);
               if (more)
-                issue_s(g, sk);      // over P, which the product above reads first: the tensor core keeps the order of issue
+                issue_s(g, sk, g);      // over P, which the product above reads first: the tensor core keeps the order of issue
               else
                 tc_commit(&o_full[g]);
               if (g == tiles - 1) {
@@ -348,14 +385,19 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
     const int g = (warp >> 2) - 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem_base + lane_off + g * 128, t_o = tmem_base + lane_off + 256 + g * 128;
-    const int row_token = g * p.tp + row / p.hp, row_head = row % p.hp;
-    uint32_t blocks_seen = 0, blocks_all = 0, items = 0;
+    const int row_token = (DUAL ? 0 : g * p.tp) + row / p.hp, row_head = row % p.hp;
+    uint32_t blocks_seen = 0, blocks_all = 0, items = 0, met = 0;
     bool ok = true;
+    auto meet = [&]() {                // the other group
+      tc_fence_before();
+      mbar_arrive(pair);
+      return wait(pair, met++ & 1, kTimeoutTmemFull);
+    };
     for (int round = 0; round < rounds && ok; ++round) {
       const int at = item_at(round);
       if (at < 0) continue;
       const Kv8Item w = p.items[at];
-      if (g > 0 && w.tokens <= p.tp) {
+      if (!DUAL && g > 0 && w.tokens <= p.tp) {
         blocks_all += w.blocks;
         continue;
       }
@@ -363,11 +405,13 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
       float m_run = -INFINITY;
       uint64_t l2 = 0;
       int ev = 0;
-      for (int j = 0; j < w.blocks; ++j) {
+      const int mine_n = DUAL ? (w.blocks + 1 - g) / 2 : w.blocks;          // blocks of this group
+      for (int k = 0; k < mine_n; ++k) {
+        const int j = DUAL ? 2 * k + g : k;
         ok = wait(&s_full[g], blocks_seen & 1, kTimeoutTmemFull);
         if (!ok) break;
         ++blocks_seen;
-        const int2 ref = meta[blocks_all++ % kKcMeta];
+        const int2 ref = meta[(blocks_all + j) % kKcMeta];
         const float c1 = fmaxf(p.scale_log2 * exp2_int(ref.x), 1.2e-38f);
         const uint64_t c2 = xtc_pair(c1, c1);
         const int limit = seen - j * kKcBlock;
@@ -394,9 +438,9 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
           tmem_ld_wait(v[(c + 1) & 1]);
         }
         const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1);
-        if (j == 0) ev = ref.y;
+        if (k == 0) ev = ref.y;
         if (__any_sync(0xffffffffu, m_new > m_run) || ev != ref.y) {
-          if (j > 0) {           // O holds the blocks before this one: their product was issued ahead of this S
+          if (k > 0) {           // O holds the blocks before this one: their product was issued ahead of this S
             const float alpha = m_run == -INFINITY ? 0.f : xtc_ex2(m_run - m_new);
             l2 = xtc_mul2(l2, xtc_pair(alpha, alpha));
             const float ao = alpha * exp2_int(max(ev - ref.y, -126));
@@ -444,28 +488,56 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         mbar_arrive(&p_full[g]);
         l2 = xtc_add2(l2, xtc_add2(sum[0], sum[1]));
       }
+      blocks_all += w.blocks;
       if (!ok) break;
-      if (w.blocks > 0) {
+      if (mine_n > 0) {
         ok = wait(&o_full[g], items & 1, kTimeoutTmemFull);
         if (!ok) break;
         ++items;
       }
       const float2 lp = xtc_unpair(l2);
-      const float l = lp.x + lp.y, inv = l == 0.f ? 0.f : 1.f / l, unit = exp2_int(ev);
+      float l = lp.x + lp.y;
+      // output = (own O * f0 + the other group's O * f1): DUAL, a half of the columns each
+      float f0 = l == 0.f ? 0.f : exp2_int(ev) / l, f1 = 0.f;
+      if constexpr (DUAL) {
+        auto pass = [&](float x) {       // this row's number of the other group
+          other[g * 128 + row] = x;
+          ok = ok && meet();
+          const float y = other[(1 - g) * 128 + row];
+          ok = ok && meet();
+          return y;
+        };
+        if (row == 0) other_ev[g] = ev;
+        const float m1 = pass(m_run), l1 = pass(l);
+        if (!ok) break;
+        const float m = fmaxf(m_run, m1), a0 = l == 0.f ? 0.f : xtc_ex2(m_run - m), a1 = l1 == 0.f ? 0.f : xtc_ex2(m1 - m);
+        const int ev1 = other_ev[1 - g];
+        l = l * a0 + l1 * a1;
+        m_run = m;
+        f0 = a0 == 0.f ? 0.f : a0 * exp2_int(ev) / l;
+        f1 = a1 == 0.f ? 0.f : a1 * exp2_int(ev1) / l;
+      }
       const bool mine = row < p.hp * p.tp && row_token < w.tokens && row_head < w.heads;
       __nv_bfloat16* dst = p.out + (static_cast<long long>(w.row0) + row_token) * p.ldo + (w.head0 + row_head) * D;
-      const long long part = (static_cast<long long>(w.part) + g) * 128 + row;
+      const long long part = (static_cast<long long>(w.part) + (DUAL ? 0 : g)) * 128 + row;
+      constexpr int kPer = DUAL ? D / 64 : D / 32;           // runs of 32 columns per group
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = DUAL ? g * kPer : 0; c < (DUAL ? (g + 1) * kPer : kPer); ++c) {
         uint32_t r[32];
-        if (w.blocks > 0) {
+        float f[32];
+        if (mine_n > 0) {
           tmem_ld_32x32(t_o + c * 32, r);
           tmem_ld_wait(r);
         }
-        if (mine) {
-          float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = l == 0.f ? 0.f : __uint_as_float(r[i]) * inv * unit;
+        for (int i = 0; i < 32; ++i) f[i] = f0 == 0.f ? 0.f : __uint_as_float(r[i]) * f0;
+        if (DUAL && (g == 0 ? w.blocks > 1 : w.blocks > 0)) {          // the other group has some
+          tmem_ld_32x32(t_o + (g == 0 ? 128 : -128) + c * 32, r);
+          tmem_ld_wait(r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] += f1 == 0.f ? 0.f : __uint_as_float(r[i]) * f1;
+        }
+        if (mine) {
           if (w.part < 0) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -479,8 +551,9 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
           }
         }
       }
-      if (w.part >= 0 && mine) *reinterpret_cast<float2*>(p.part_s + part * 2) = make_float2(m_run, l);
+      if (w.part >= 0 && mine && (!DUAL || g == 0)) *reinterpret_cast<float2*>(p.part_s + part * 2) = make_float2(m_run, l);
       tc_fence_before();
+      if (DUAL && !(ok = meet())) break;          // the next item's products write over both groups' O
     }
   }
 
@@ -530,18 +603,18 @@ __global__ void __launch_bounds__(128) kv8_chunk_join_kernel(const Kv8Chunk p, c
   for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
 }
 
-template <int D>
+template <int D, bool DUAL>
 static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, const Kv8ChunkJoin* joins, int n_joins, cudaStream_t s) {
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(kv8_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8ChunkCfg<D>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kv8_chunk_kernel<D, DUAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8ChunkCfg<D, DUAL>::kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev & 63] = true;
   }
   const int grid = p.n_items < sm_count() ? p.n_items : sm_count();
-  kv8_chunk_kernel<D><<<grid, kKcThreads, Kv8ChunkCfg<D>::kSmem, s>>>(tq, p);
+  kv8_chunk_kernel<D, DUAL><<<grid, kKcThreads, Kv8ChunkCfg<D, DUAL>::kSmem, s>>>(tq, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || n_joins == 0) return static_cast<int>(e);
   kv8_chunk_join_kernel<D><<<dim3(n_joins, (p.hp * p.tp + 3) / 4), 128, 0, s>>>(p, joins);
@@ -553,10 +626,10 @@ static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, const Kv8C
 extern "C" {
 using namespace apb;
 
-// q [T, Hq, D], out [T, Hq, D] (rows on 16-byte boundaries); items [n][12], joins [n][8] and their sizes as apb_rt_kv8_plan makes
+// q [T, Hq, D], out [T, Hq, D] (rows on 16-byte boundaries); one_tile: no item has two tiles; items [n][12], joins [n][8] and their sizes as apb_rt_kv8_plan makes
 // them; scratch: part_tiles * 128 * (D + 2) floats.
 int apb_kv8_chunk(const void* q, long long ldq, const void* data, const int* table, long long ld_table, const int* items, int n_items,
-                  const int* joins, int n_joins, int part_tiles, void* scratch, void* out, long long ldo, int T, int Hq, int Hkv, int D,
+                  const int* joins, int n_joins, int part_tiles, int one_tile, void* scratch, void* out, long long ldo, int T, int Hq, int Hkv, int D,
                   float scale, cudaStream_t s) {
   if (n_items <= 0) return 0;
   if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || ldq % 8 || ldo % 8 || reinterpret_cast<uintptr_t>(q) % 16 ||
@@ -574,6 +647,7 @@ int apb_kv8_chunk(const void* q, long long ldq, const void* data, const int* tab
                 static_cast<__nv_bfloat16*>(out), ldo, part_o, part_o + static_cast<long long>(part_tiles) * 128 * D, Hkv, hp, tp,
                 fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, status_device_ptr()};
   const Kv8ChunkJoin* j = reinterpret_cast<const Kv8ChunkJoin*>(joins);
-  return D == 128 ? launch_kv8_chunk<128>(tq, p, j, n_joins, s) : launch_kv8_chunk<64>(tq, p, j, n_joins, s);
+  if (one_tile) return D == 128 ? launch_kv8_chunk<128, true>(tq, p, j, n_joins, s) : launch_kv8_chunk<64, true>(tq, p, j, n_joins, s);
+  return D == 128 ? launch_kv8_chunk<128, false>(tq, p, j, n_joins, s) : launch_kv8_chunk<64, false>(tq, p, j, n_joins, s);
 }
 }

@@ -39,7 +39,7 @@ def _fn(name: str):
         _FN["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
         _FN["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
         _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, f, vp])
-        _FN["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, i, vp, i, i, vp, vp, ll, i, i, i, i, f, vp])
+        _FN["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, i, vp, i, i, i, vp, vp, ll, i, i, i, i, f, vp])
     return _FN[name]
 
 
@@ -315,6 +315,7 @@ class ChunkPlan:
     items: Optional[torch.Tensor] = None
     joins: Optional[torch.Tensor] = None
     part_tiles: int = 0                              # tiles of 128 rows of scratch
+    one_tile: bool = False                           # no item has a second tile
 
     @staticmethod
     def build(new: Sequence[int], lengths: Sequence[int], pages, heads: int, cache: Fp8KVCache) -> "ChunkPlan":
@@ -341,6 +342,7 @@ class ChunkPlan:
         if cache.data.is_cuda and rows:
             sms = torch.cuda.get_device_properties(cache.data.device).multi_processor_count
             items, joins, plan.part_tiles = _work(new, lengths, heads, cache.num_kv_heads, sms)
+            plan.one_tile = int(new.max()) <= 128 // min(128, heads // cache.num_kv_heads)
             table = np.zeros((n, max(1, int(need.max()))), dtype=np.int32)
             for s in range(n):
                 table[s, :need[s]] = used[s]
@@ -385,7 +387,7 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
     with _On(data.device):
         scratch = torch.empty(plan.part_tiles * 128 * (D + 2), device=q.device, dtype=torch.float32) if plan.part_tiles else None
         _lib.check(_fn("chunk")(q.data_ptr(), q.stride(0), data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
-                                plan.items.shape[0], plan.joins.data_ptr(), plan.joins.shape[0], plan.part_tiles,
+                                plan.items.shape[0], plan.joins.data_ptr(), plan.joins.shape[0], plan.part_tiles, int(plan.one_tile),
                                 None if scratch is None else scratch.data_ptr(), out.data_ptr(), out.stride(0), T, Hq, cache.num_kv_heads, D,
                                 scale, _lib.stream_ptr()), "kv8_chunk")
     return out
