@@ -28,8 +28,8 @@ struct Kv8Item {
   int pad;
 };
 struct Kv8Chunk {
-  const Kv8Item* items;
-  int n_items;
+  const Kv8Item* items;    // of CTA c: [first[c], first[c + 1])
+  const int* first;
   const uint8_t* data;
   const int* table;        // [sequences, ...]
   long long ld_table;
@@ -131,11 +131,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
-  const int rounds = (p.n_items + gridDim.x - 1) / gridDim.x;
-  auto item_at = [&](int round) {
-    const int i = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    return i < p.n_items ? i : -1;
-  };
+  const int item0 = p.first[blockIdx.x], item1 = p.first[blockIdx.x + 1];
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {      // of a whole warp
     const bool r = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code));
     tc_fence_after();
@@ -148,6 +144,85 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
     }
   };
 
+  auto convert = [&]() {
+    // ---------------------------------------------------------------- codes to tiles
+    const int part = warp - 4;
+    constexpr int kUnits = D / 16;         // of 16 codes in a row
+    bool ok = true;
+    int st = 0, slot = 0;
+    uint32_t st_phase = 0, phase = 0, n_blocks = 0;
+    for (int at = item0; at < item1 && ok; ++at) {
+      const int blocks = p.items[at].blocks, left0 = p.items[at].len - p.items[at].block0 * kKcBlock;
+      int vref = 0;
+      for (int j = 0; j < blocks && ok; ++j) {
+        ok = wait(&st_full[st], st_phase, kTimeoutFull);
+        if (!ok) break;
+        const int valid = min(kKcBlock, left0 - j * kKcBlock);
+        const uint8_t* stage = smem_st + st * Cfg::kStage;
+        int kmax = 0, vmax = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int word = lane + 32 * i, t = (word >> 3) * kKv8Page + (word & 7);
+          const uint32_t e = *reinterpret_cast<const uint32_t*>(stage + (word >> 3) * Kv8<D>::kBlock + 2 * Kv8<D>::kHalf + (word & 7) * 4);
+          if (t < valid) kmax = max(kmax, static_cast<int>(e & 255)), vmax = max(vmax, static_cast<int>(e >> 16 & 255));
+          if (t + 8 < valid) kmax = max(kmax, static_cast<int>(e >> 8 & 255)), vmax = max(vmax, static_cast<int>(e >> 24));
+        }
+        kmax = __reduce_max_sync(0xffffffffu, kmax);
+        vmax = __reduce_max_sync(0xffffffffu, vmax);
+        if (j == 0 || vmax > vref + 7) vref = vmax;       // factors up to 2^127 do without a new one
+        if (part == 0 && lane == 0) meta[n_blocks % kKcMeta] = make_int2(kmax - 127, vref - 127);
+        ++n_blocks;
+#pragma unroll 1
+        for (int which = 0; which < 2 && ok; ++which) {
+          const int ref = which ? vref : kmax;
+          const uint32_t sign = which ? 0u : p.key_sign;
+          ok = wait(&kv_empty[slot], phase ^ 1, kTimeoutEmpty);
+          if (!ok) break;
+          // A lane has the same 16 columns of every kStep-th token; the upper half of a row takes its two units the other
+          // way around, so that no bank is met twice.
+          const int c = lane % kUnits, u0 = 2 * (c & 3) + (c >> 2), t0 = (part * 32 + lane) / kUnits;
+          constexpr int kStep = 32 * kKcConvert / kUnits, kAt = 4;           // tokens between a lane's, of them at a time
+          const bool swap = c >> 2, ragged = valid < kKcBlock;
+          const uint32_t tile = smem_u32(smem_kv) + slot * Cfg::kTile + (c >> 2) * 16384;
+          const uint32_t codes = smem_u32(stage) + which * Kv8<D>::kHalf + c * 16, exps = smem_u32(stage) + 2 * Kv8<D>::kHalf;
+#pragma unroll 1
+          for (int i = t0; i < 128; i += kStep * kAt) {
+            uint4 w[kAt];
+            int e[kAt];
+#pragma unroll
+            for (int k = 0; k < kAt; ++k) {
+              const int t = i + k * kStep;
+              w[k] = lds128(codes + (t >> 4) * Kv8<D>::kBlock + (t & 15) * D);
+              e[k] = lds8(exps + (t >> 4) * Kv8<D>::kBlock + kv8_exponent_at(t & 15, which));
+            }
+#pragma unroll
+            for (int k = 0; k < kAt; ++k) {
+              const int t = i + k * kStep;
+              uint32_t f = static_cast<uint32_t>(max(127 + 120 + e[k] - ref, 0)) << 7;
+              f = f << 16 | f | sign;
+              if (ragged && t >= valid) w[k] = make_uint4(0, 0, 0, 0), f = 0;
+              uint4 a, b;
+              e4m3x4_to_bf16(swap ? w[k].z : w[k].x, f, a.x, a.y);
+              e4m3x4_to_bf16(swap ? w[k].w : w[k].y, f, a.z, a.w);
+              e4m3x4_to_bf16(swap ? w[k].x : w[k].z, f, b.x, b.y);
+              e4m3x4_to_bf16(swap ? w[k].y : w[k].w, f, b.z, b.w);
+              const uint32_t row = tile + t * 128, u = (u0 ^ (t & 7)) << 4;
+              sts128(row + u, a);
+              sts128(row + (u ^ 16), b);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[slot]);
+          next(slot, phase, kRing);
+        }
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(&st_empty[st]);
+        next(st, st_phase, kKcStages);
+      }
+    }
+  };
+
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKcRegsIssue));
     if (warp == 0) {
@@ -155,9 +230,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
       bool ok = true;
       int slot = 0;
       uint32_t phase = 0, n_q = 0;
-      for (int round = 0; round < rounds && ok; ++round) {
-        const int at = item_at(round);
-        if (at < 0) continue;
+      for (int at = item0; at < item1 && ok; ++at) {
         const Kv8Item w = p.items[at];
         if (w.blocks == 0) continue;
         const int tiles = !DUAL && w.tokens > p.tp ? 2 : 1, pages = (w.len + kKv8Page - 1) / kKv8Page;
@@ -223,9 +296,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
       };
       bool ok = true;
       uint32_t tile = 0;               // DUAL: number of the item's first tile
-      for (int round = 0; round < rounds && ok; ++round) {
-        const int at = item_at(round);
-        if (at < 0) continue;
+      for (int at = item0; at < item1 && ok; ++at) {
         const int blocks = p.items[at].blocks, tiles = !DUAL && p.items[at].tokens > p.tp ? 2 : 1;
         if (blocks == 0) continue;
         if constexpr (DUAL) {
@@ -299,86 +370,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
     }
   } else if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKcRegsConvert));
-    {
-      // ---------------------------------------------------------------- codes to tiles
-      const int part = warp - 4;
-      constexpr int kUnits = D / 16;         // of 16 codes in a row
-      bool ok = true;
-      int st = 0, slot = 0;
-      uint32_t st_phase = 0, phase = 0, n_blocks = 0;
-      for (int round = 0; round < rounds && ok; ++round) {
-        const int at = item_at(round);
-        if (at < 0) continue;
-        const int blocks = p.items[at].blocks, left0 = p.items[at].len - p.items[at].block0 * kKcBlock;
-        int vref = 0;
-        for (int j = 0; j < blocks && ok; ++j) {
-          ok = wait(&st_full[st], st_phase, kTimeoutFull);
-          if (!ok) break;
-          const int valid = min(kKcBlock, left0 - j * kKcBlock);
-          const uint8_t* stage = smem_st + st * Cfg::kStage;
-          int kmax = 0, vmax = 0;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int word = lane + 32 * i, t = (word >> 3) * kKv8Page + (word & 7);
-            const uint32_t e = *reinterpret_cast<const uint32_t*>(stage + (word >> 3) * Kv8<D>::kBlock + 2 * Kv8<D>::kHalf + (word & 7) * 4);
-            if (t < valid) kmax = max(kmax, static_cast<int>(e & 255)), vmax = max(vmax, static_cast<int>(e >> 16 & 255));
-            if (t + 8 < valid) kmax = max(kmax, static_cast<int>(e >> 8 & 255)), vmax = max(vmax, static_cast<int>(e >> 24));
-          }
-          kmax = __reduce_max_sync(0xffffffffu, kmax);
-          vmax = __reduce_max_sync(0xffffffffu, vmax);
-          if (j == 0 || vmax > vref + 7) vref = vmax;       // factors up to 2^127 do without a new one
-          if (part == 0 && lane == 0) meta[n_blocks % kKcMeta] = make_int2(kmax - 127, vref - 127);
-          ++n_blocks;
-#pragma unroll 1
-          for (int which = 0; which < 2 && ok; ++which) {
-            const int ref = which ? vref : kmax;
-            const uint32_t sign = which ? 0u : p.key_sign;
-            ok = wait(&kv_empty[slot], phase ^ 1, kTimeoutEmpty);
-            if (!ok) break;
-            // A lane has the same 16 columns of every second or fourth token ...; the upper half of a row takes its two units the other
-            // way around, so that no bank is met twice.
-            const int c = lane % kUnits, u0 = 2 * (c & 3) + (c >> 2), t0 = (part * 32 + lane) / kUnits;
-            constexpr int kStep = 32 * kKcConvert / kUnits, kAt = 4;           // tokens between a lane's, of them at a time
-            const bool swap = c >> 2;
-            const uint32_t tile = smem_u32(smem_kv) + slot * Cfg::kTile + (c >> 2) * 16384;
-            const uint32_t codes = smem_u32(stage) + which * Kv8<D>::kHalf + c * 16, exps = smem_u32(stage) + 2 * Kv8<D>::kHalf;
-#pragma unroll 1
-            for (int i = 0; i < 128 / kStep; i += kAt) {
-              uint4 w[kAt];
-              int e[kAt];
-#pragma unroll
-              for (int k = 0; k < kAt; ++k) {
-                const int t = t0 + (i + k) * kStep;
-                w[k] = lds128(codes + (t >> 4) * Kv8<D>::kBlock + (t & 15) * D);
-                e[k] = lds8(exps + (t >> 4) * Kv8<D>::kBlock + kv8_exponent_at(t & 15, which));
-              }
-#pragma unroll
-              for (int k = 0; k < kAt; ++k) {
-                const int t = t0 + (i + k) * kStep;
-                uint32_t f = static_cast<uint32_t>(max(127 + 120 + e[k] - ref, 0)) << 7;
-                f = f << 16 | f | sign;
-                if (t >= valid) w[k] = make_uint4(0, 0, 0, 0), f = 0;
-                uint4 a, b;
-                e4m3x4_to_bf16(swap ? w[k].z : w[k].x, f, a.x, a.y);
-                e4m3x4_to_bf16(swap ? w[k].w : w[k].y, f, a.z, a.w);
-                e4m3x4_to_bf16(swap ? w[k].x : w[k].z, f, b.x, b.y);
-                e4m3x4_to_bf16(swap ? w[k].y : w[k].w, f, b.z, b.w);
-                const uint32_t row = tile + t * 128, u = (u0 ^ (t & 7)) << 4;
-                sts128(row + u, a);
-                sts128(row + (u ^ 16), b);
-              }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&kv_full[slot]);
-            next(slot, phase, kRing);
-          }
-          if (!ok) break;
-          if (lane == 0) mbar_arrive(&st_empty[st]);
-          next(st, st_phase, kKcStages);
-        }
-      }
-    }
+    convert();
   } else {
     // ------------------------------------------------------------------ softmax groups
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKcRegsSoftmax));
@@ -393,9 +385,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
       mbar_arrive(pair);
       return wait(pair, met++ & 1, kTimeoutTmemFull);
     };
-    for (int round = 0; round < rounds && ok; ++round) {
-      const int at = item_at(round);
-      if (at < 0) continue;
+    for (int at = item0; at < item1 && ok; ++at) {
       const Kv8Item w = p.items[at];
       if (!DUAL && g > 0 && w.tokens <= p.tp) {
         blocks_all += w.blocks;
@@ -604,7 +594,7 @@ __global__ void __launch_bounds__(128) kv8_chunk_join_kernel(const Kv8Chunk p, c
 }
 
 template <int D, bool DUAL>
-static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, const Kv8ChunkJoin* joins, int n_joins, cudaStream_t s) {
+static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, int grid, const Kv8ChunkJoin* joins, int n_joins, cudaStream_t s) {
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -613,8 +603,7 @@ static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, const Kv8C
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev & 63] = true;
   }
-  const int grid = p.n_items < sm_count() ? p.n_items : sm_count();
-  kv8_chunk_kernel<D, DUAL><<<grid, kKcThreads, Kv8ChunkCfg<D, DUAL>::kSmem, s>>>(tq, p);
+    kv8_chunk_kernel<D, DUAL><<<grid, kKcThreads, Kv8ChunkCfg<D, DUAL>::kSmem, s>>>(tq, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || n_joins == 0) return static_cast<int>(e);
   kv8_chunk_join_kernel<D><<<dim3(n_joins, (p.hp * p.tp + 3) / 4), 128, 0, s>>>(p, joins);
@@ -626,12 +615,12 @@ static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, const Kv8C
 extern "C" {
 using namespace apb;
 
-// q [T, Hq, D], out [T, Hq, D] (rows on 16-byte boundaries); one_tile: no item has two tiles; items [n][12], joins [n][8] and their sizes as apb_rt_kv8_plan makes
+// q [T, Hq, D], out [T, Hq, D] (rows on 16-byte boundaries); one_tile: no item has two tiles; items [..][12], first [ctas + 1], joins [n_joins][8] as apb_rt_kv8_plan makes
 // them; scratch: part_tiles * 128 * (D + 2) floats.
-int apb_kv8_chunk(const void* q, long long ldq, const void* data, const int* table, long long ld_table, const int* items, int n_items,
-                  const int* joins, int n_joins, int part_tiles, int one_tile, void* scratch, void* out, long long ldo, int T, int Hq, int Hkv, int D,
+int apb_kv8_chunk(const void* q, long long ldq, const void* data, const int* table, long long ld_table, const int* items, const int* first,
+                  int ctas, const int* joins, int n_joins, int part_tiles, int one_tile, void* scratch, void* out, long long ldo, int T, int Hq, int Hkv, int D,
                   float scale, cudaStream_t s) {
-  if (n_items <= 0) return 0;
+  if (ctas <= 0) return 0;
   if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || ldq % 8 || ldo % 8 || reinterpret_cast<uintptr_t>(q) % 16 ||
       reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(data) % 16 || reinterpret_cast<uintptr_t>(items) % 16)
     return kBadArgument;
@@ -643,11 +632,11 @@ int apb_kv8_chunk(const void* q, long long ldq, const void* data, const int* tab
   const int rc = make_tmap_nd(&tq, q, 2, 3, dims, strides, box);
   if (rc) return 1000 + rc;
   float* part_o = static_cast<float*>(scratch);
-  Kv8Chunk p = {reinterpret_cast<const Kv8Item*>(items), n_items, static_cast<const uint8_t*>(data), table, ld_table,
+  Kv8Chunk p = {reinterpret_cast<const Kv8Item*>(items), first, static_cast<const uint8_t*>(data), table, ld_table,
                 static_cast<__nv_bfloat16*>(out), ldo, part_o, part_o + static_cast<long long>(part_tiles) * 128 * D, Hkv, hp, tp,
                 fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, status_device_ptr()};
   const Kv8ChunkJoin* j = reinterpret_cast<const Kv8ChunkJoin*>(joins);
-  if (one_tile) return D == 128 ? launch_kv8_chunk<128, true>(tq, p, j, n_joins, s) : launch_kv8_chunk<64, true>(tq, p, j, n_joins, s);
-  return D == 128 ? launch_kv8_chunk<128, false>(tq, p, j, n_joins, s) : launch_kv8_chunk<64, false>(tq, p, j, n_joins, s);
+  if (one_tile) return D == 128 ? launch_kv8_chunk<128, true>(tq, p, ctas, j, n_joins, s) : launch_kv8_chunk<64, true>(tq, p, ctas, j, n_joins, s);
+  return D == 128 ? launch_kv8_chunk<128, false>(tq, p, ctas, j, n_joins, s) : launch_kv8_chunk<64, false>(tq, p, ctas, j, n_joins, s);
 }
 }

@@ -39,7 +39,7 @@ def _fn(name: str):
         _FN["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
         _FN["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
         _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, f, vp])
-        _FN["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, i, vp, i, i, i, vp, vp, ll, i, i, i, i, f, vp])
+        _FN["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, vp, i, vp, i, i, i, vp, vp, ll, i, i, i, i, f, vp])
     return _FN[name]
 
 
@@ -278,23 +278,34 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
     return out
 
 
-def _work(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: int) -> Tuple[np.ndarray, np.ndarray, int]:
-    """Items, joins and scratch tiles (``csrc/runtime_kv8.cpp``)."""
+@dataclass
+class _Work:
+    """What the CTAs of chunk attention do (``csrc/runtime_kv8.cpp``): items, where each CTA's begin, joins of items cut along the keys."""
+    items: np.ndarray
+    first: np.ndarray
+    joins: np.ndarray
+    part_tiles: int           # tiles of 128 rows of scratch
+    ctas: int
+    one_tile: bool            # no item has a second tile
+
+
+def _work(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: int) -> _Work:
     fn = _lib.rt_lib().apb_rt_kv8_plan
     c = ctypes
-    fn.argtypes, fn.restype = [c.c_void_p, c.c_void_p, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_void_p, c.c_int64, c.c_void_p, c.c_int64,
-                               c.c_void_p], c.c_int32
+    fn.argtypes, fn.restype = [c.c_void_p, c.c_void_p, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_void_p, c.c_int64, c.c_void_p,
+                               c.c_void_p, c.c_int64, c.c_void_p], c.c_int32
     new, lengths = np.ascontiguousarray(new, dtype=np.int32), np.ascontiguousarray(lengths, dtype=np.int32)
-    counts = np.zeros(3, dtype=np.int64)
+    counts, first = np.zeros(5, dtype=np.int64), np.zeros(sms + 1, dtype=np.int32)
+    # as many items as tiles hold tokens, and a few more that a border cuts: the first call says how many it is
     items, joins = np.empty((0, 12), dtype=np.int32), np.empty((0, 8), dtype=np.int32)
     for _ in range(2):
-        if fn(new.ctypes.data, lengths.ctypes.data, len(new), heads, kv_heads, sms, items.ctypes.data, len(items), joins.ctypes.data,
-              len(joins), counts.ctypes.data) != 0:
+        if fn(new.ctypes.data, lengths.ctypes.data, len(new), heads, kv_heads, sms, items.ctypes.data, len(items), first.ctypes.data,
+              joins.ctypes.data, len(joins), counts.ctypes.data) != 0:
             raise ValueError("chunk plan: sizes out of range")
-        if len(items) == counts[0]:
+        if len(items) >= counts[0] and len(joins) >= counts[1]:
             break
         items, joins = np.empty((int(counts[0]), 12), dtype=np.int32), np.empty((int(counts[1]), 8), dtype=np.int32)
-    return items, joins, int(counts[2])
+    return _Work(items, first[:int(counts[3]) + 1], joins, int(counts[2]), int(counts[3]), bool(counts[4]))
 
 
 @dataclass
@@ -311,11 +322,11 @@ class ChunkPlan:
     kv_heads: int
     num_pages: int
     head_dim: int
-    table: Optional[torch.Tensor] = None             # on the cache's device: pages, work items, joins of items cut along the keys
+    work: Optional[_Work] = None
+    table: Optional[torch.Tensor] = None             # on the cache's device: pages, and the work's tables
     items: Optional[torch.Tensor] = None
+    first: Optional[torch.Tensor] = None
     joins: Optional[torch.Tensor] = None
-    part_tiles: int = 0                              # tiles of 128 rows of scratch
-    one_tile: bool = False                           # no item has a second tile
 
     @staticmethod
     def build(new: Sequence[int], lengths: Sequence[int], pages, heads: int, cache: Fp8KVCache) -> "ChunkPlan":
@@ -341,15 +352,14 @@ class ChunkPlan:
         plan = ChunkPlan(rows, new, lengths, used, heads, cache.num_kv_heads, cache.num_pages, cache.head_dim)
         if cache.data.is_cuda and rows:
             sms = torch.cuda.get_device_properties(cache.data.device).multi_processor_count
-            items, joins, plan.part_tiles = _work(new, lengths, heads, cache.num_kv_heads, sms)
-            plan.one_tile = int(new.max()) <= 128 // min(128, heads // cache.num_kv_heads)
+            plan.work = w = _work(new, lengths, heads, cache.num_kv_heads, sms)
             table = np.zeros((n, max(1, int(need.max()))), dtype=np.int32)
             for s in range(n):
                 table[s, :need[s]] = used[s]
-            flat = torch.from_numpy(np.concatenate([items.reshape(-1), joins.reshape(-1), table.reshape(-1)])).pin_memory()
-            dev = to_device(flat, cache.data.device)
-            plan.items, plan.joins, plan.table = (t.view(a.shape) for t, a in zip(dev.split([items.size, joins.size, table.size]),
-                                                                                (items, joins, table)))
+            parts = (w.items, w.joins, w.first, table)
+            flat = torch.from_numpy(np.concatenate([a.reshape(-1) for a in parts])).pin_memory()
+            dev = to_device(flat, cache.data.device).split([a.size for a in parts])
+            plan.items, plan.joins, plan.first, plan.table = (t.view(a.shape) for t, a in zip(dev, parts))
         return plan
 
 
@@ -385,9 +395,10 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
         out[:plan.rows].copy_(chunk_attention(q, cache, plan, scale)[:plan.rows])
         return out
     with _On(data.device):
-        scratch = torch.empty(plan.part_tiles * 128 * (D + 2), device=q.device, dtype=torch.float32) if plan.part_tiles else None
+        w = plan.work
+        scratch = torch.empty(w.part_tiles * 128 * (D + 2), device=q.device, dtype=torch.float32) if w.part_tiles else None
         _lib.check(_fn("chunk")(q.data_ptr(), q.stride(0), data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
-                                plan.items.shape[0], plan.joins.data_ptr(), plan.joins.shape[0], plan.part_tiles, int(plan.one_tile),
+                                plan.first.data_ptr(), w.ctas, plan.joins.data_ptr(), len(w.joins), w.part_tiles, int(w.one_tile),
                                 None if scratch is None else scratch.data_ptr(), out.data_ptr(), out.stride(0), T, Hq, cache.num_kv_heads, D,
                                 scale, _lib.stream_ptr()), "kv8_chunk")
     return out
