@@ -2,7 +2,8 @@
 //
 // Both are bound by memory: a row of D values moves 2 D (4 D from fp32) + D + 1 bytes on its way in, D + 1 + 2 D on its way out.
 // D / 8 lanes share a row, eight neighbouring values each, so that 16-byte accesses to the values and 8-byte ones to the codes cover
-// whole sectors; the largest magnitude of a row is found by shuffles among them, and nothing is read twice.
+// whole sectors; the largest magnitude of a row is found by shuffles among them, and nothing is read twice.  (Lanes that walked over
+// rows one at a time kept too little on its way, and a 64-bit division per row: 2.9 TB/s in, 4.1 out.)
 #include <cuda_fp16.h>
 
 #include "host_utils.cuh"
@@ -53,80 +54,113 @@ __device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// rows in the order token, keys or values, head
+// A warp has kAtOnce runs of rows of one token, 32 / kLanes rows each: all of their loads are on their way before the first is used.
+constexpr int kAtOnce = 4;
+template <int D>
+struct RowsWalk {
+  static constexpr int kLanes = D / 8, kRows = 32 / kLanes, kPerWarp = kRows * kAtOnce;
+  int t, row0, part;        // token, first row of this lane's of its 2 H, eight values of it
+  __device__ __forceinline__ bool start(const Kv8Rows& p, int warps_per_token) {
+    const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    t = w / warps_per_token;
+    row0 = (w - t * warps_per_token) * kPerWarp + lane / kLanes;
+    part = lane % kLanes;
+    return t < p.T;
+  }
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv8_write_kernel(const Kv8Rows p) {
+__global__ void __launch_bounds__(256) kv8_write_kernel(const Kv8Rows p, int warps_per_token) {
   pdl_entry();
-  constexpr int kLanes = D / 8;
-  const int part = threadIdx.x % kLanes;
-  const long long rows = 2ll * p.T * p.H, step = static_cast<long long>(gridDim.x) * (256 / kLanes);
-  for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / kLanes; i - threadIdx.x / kLanes < rows; i += step) {
-    const bool there = i < rows;               // all lanes of a warp stay for its shuffles
-    const int t = there ? static_cast<int>(i / (2 * p.H)) : 0;
-    const int w = there ? static_cast<int>(i % (2 * p.H)) : 0;
-    const int which = w >= p.H, h = w - which * p.H;
-    const int slot = there ? p.slots[t] : -1;
-    float v[8];
-    load8(static_cast<const T*>(p.x[which]) + t * p.ld[which] + h * p.lh[which] + part * 8, v);
+  using Walk = RowsWalk<D>;
+  Walk at;
+  if (!at.start(p, warps_per_token)) return;
+  const int slot = p.slots[at.t];
+  float v[kAtOnce][8];
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    const int row = min(at.row0 + i * Walk::kRows, 2 * p.H - 1), which = row >= p.H, h = row - which * p.H;      // all lanes stay for the shuffles
+    load8(static_cast<const T*>(p.x[which]) + at.t * p.ld[which] + h * p.lh[which] + at.part * 8, v[i]);
+  }
+  if (slot < 0) return;
+  if (slot >= p.slots_end) {
+    if (p.status) atomicCAS(p.status, 0, kBadTable);
+    return;
+  }
+  const int token = slot % kKv8Page;
+  uint8_t* page = p.data + static_cast<long long>(slot / kKv8Page) * p.H * Kv8<D>::kBlock;
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    const int row = at.row0 + i * Walk::kRows, which = row >= p.H, h = row - which * p.H;
     float most = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(v[k]));
+    for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(v[i][k]));
 #pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (slot < 0) continue;
-    if (slot >= p.slots_end) {
-      if (p.status) atomicCAS(p.status, 0, kBadTable);
-      continue;
-    }
+    for (int o = 1; o < Walk::kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (row >= 2 * p.H) continue;
     const int e = kv8_exponent(most);
     const float f = exp2_int(-e);
     uint16_t c[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) c[k] = e4m3_pair(v[2 * k] * f, v[2 * k + 1] * f);
-    const int token = slot % kKv8Page;
-    uint8_t* block = p.data + (static_cast<long long>(slot / kKv8Page) * p.H + h) * Kv8<D>::kBlock;
-    *reinterpret_cast<uint2*>(block + which * Kv8<D>::kHalf + token * D + part * 8) =
+    for (int k = 0; k < 4; ++k) c[k] = e4m3_pair(v[i][2 * k] * f, v[i][2 * k + 1] * f);
+    uint8_t* block = page + h * Kv8<D>::kBlock;
+    *reinterpret_cast<uint2*>(block + which * Kv8<D>::kHalf + token * D + at.part * 8) =
         make_uint2(c[0] | static_cast<uint32_t>(c[1]) << 16, c[2] | static_cast<uint32_t>(c[3]) << 16);
-    if (part == 0) block[2 * Kv8<D>::kHalf + kv8_exponent_at(token, which)] = static_cast<uint8_t>(e + 127);
+    if (at.part == 0) block[2 * Kv8<D>::kHalf + kv8_exponent_at(token, which)] = static_cast<uint8_t>(e + 127);
   }
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Rows p, T* out_k, T* out_v) {
+__global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Rows p, int warps_per_token, T* out_k, T* out_v) {
   pdl_entry();
-  constexpr int kLanes = D / 8;
-  const int part = threadIdx.x % kLanes;
-  const long long rows = 2ll * p.T * p.H, step = static_cast<long long>(gridDim.x) * (256 / kLanes);
-  for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / kLanes; i < rows; i += step) {
-    const int t = static_cast<int>(i / (2 * p.H)), w = static_cast<int>(i % (2 * p.H));
-    const int which = w >= p.H, h = w - which * p.H;
-    const int slot = p.slots[t];
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (slot >= p.slots_end) {
-      if (p.status) atomicCAS(p.status, 0, kBadTable);
-    } else if (slot >= 0) {
-      const int token = slot % kKv8Page;
-      const uint8_t* block = p.data + (static_cast<long long>(slot / kKv8Page) * p.H + h) * Kv8<D>::kBlock;
-      const uint2 c = *reinterpret_cast<const uint2*>(block + which * Kv8<D>::kHalf + token * D + part * 8);
-      const float f = exp2f(static_cast<float>(block[2 * Kv8<D>::kHalf + kv8_exponent_at(token, which)]) - 127.f);
-      const uint16_t pair[4] = {static_cast<uint16_t>(c.x), static_cast<uint16_t>(c.x >> 16), static_cast<uint16_t>(c.y),
-                                static_cast<uint16_t>(c.y >> 16)};
+  using Walk = RowsWalk<D>;
+  Walk at;
+  if (!at.start(p, warps_per_token)) return;
+  int slot = p.slots[at.t];
+  if (slot >= p.slots_end) {
+    if (p.status) atomicCAS(p.status, 0, kBadTable);
+    slot = -1;
+  }
+  const int token = slot % kKv8Page;
+  const uint8_t* page = p.data + static_cast<long long>(slot / kKv8Page) * p.H * Kv8<D>::kBlock;
+  uint2 c[kAtOnce];
+  int e[kAtOnce];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t x = e4m3_to_f16x2(pair[k]);
-        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x));
-        v[2 * k] = y.x * f;
-        v[2 * k + 1] = y.y * f;
-      }
+  for (int i = 0; i < kAtOnce; ++i) {
+    const int row = at.row0 + i * Walk::kRows, which = row >= p.H, h = row - which * p.H;
+    const uint8_t* block = page + h * Kv8<D>::kBlock;
+    c[i] = make_uint2(0, 0);
+    e[i] = 0;
+    if (row < 2 * p.H && slot >= 0) {
+      c[i] = *reinterpret_cast<const uint2*>(block + which * Kv8<D>::kHalf + token * D + at.part * 8);
+      e[i] = block[2 * Kv8<D>::kHalf + kv8_exponent_at(token, which)];
     }
-    store8((which ? out_v : out_k) + (static_cast<long long>(t) * p.H + h) * D + part * 8, v);
+  }
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    const int row = at.row0 + i * Walk::kRows, which = row >= p.H, h = row - which * p.H;
+    if (row >= 2 * p.H) break;
+    const float f = exp2f(static_cast<float>(e[i]) - 127.f);
+    const uint16_t pair[4] = {static_cast<uint16_t>(c[i].x), static_cast<uint16_t>(c[i].x >> 16), static_cast<uint16_t>(c[i].y),
+                              static_cast<uint16_t>(c[i].y >> 16)};
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t x = e4m3_to_f16x2(pair[k]);
+      const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x));
+      v[2 * k] = y.x * f;
+      v[2 * k + 1] = y.y * f;
+    }
+    store8((which ? out_v : out_k) + (static_cast<long long>(at.t) * p.H + h) * D + at.part * 8, v);
   }
 }
 
-template <typename K, typename... Args>
-static int launch_rows(K kernel, const Kv8Rows& p, int D, cudaStream_t s, Args... args) {
-  const long long blocks = (2ll * p.T * p.H * (D / 8) + 255) / 256, most = sm_count() * 8;
-  return static_cast<int>(launch_kernel(kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, s, p, args...));
+template <int D, typename K, typename... Args>
+static int launch_rows(K kernel, const Kv8Rows& p, cudaStream_t s, Args... args) {
+  const int per_token = (2 * p.H + RowsWalk<D>::kPerWarp - 1) / RowsWalk<D>::kPerWarp;
+  const long long blocks = (static_cast<long long>(p.T) * per_token + 7) / 8;
+  if (blocks * 8 >= 1ll << 31) return kBadArgument;
+  return static_cast<int>(launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, p, per_token, args...));
 }
 
 }  // namespace apb
@@ -145,8 +179,8 @@ int apb_kv8_write(const void* k, long long ldk, long long lhk, const void* v, lo
       reinterpret_cast<uintptr_t>(data) % 16)
     return kBadArgument;
   Kv8Rows p = {{k, v}, {ldk, ldv}, {lhk, lhv}, slots, static_cast<uint8_t*>(data), T, H, pages * kKv8Page, status_device_ptr()};
-  if (dtype == 0) return D == 128 ? launch_rows(kv8_write_kernel<__nv_bfloat16, 128>, p, D, s) : launch_rows(kv8_write_kernel<__nv_bfloat16, 64>, p, D, s);
-  return D == 128 ? launch_rows(kv8_write_kernel<float, 128>, p, D, s) : launch_rows(kv8_write_kernel<float, 64>, p, D, s);
+  if (dtype == 0) return D == 128 ? launch_rows<128>(kv8_write_kernel<__nv_bfloat16, 128>, p, s) : launch_rows<64>(kv8_write_kernel<__nv_bfloat16, 64>, p, s);
+  return D == 128 ? launch_rows<128>(kv8_write_kernel<float, 128>, p, s) : launch_rows<64>(kv8_write_kernel<float, 64>, p, s);
 }
 
 // out_k, out_v: [T, H, D] of bf16 (dtype 0) or fp32 (1); zeros where slots[t] is below 0.
@@ -164,9 +198,9 @@ int apb_kv8_read(const void* data, const int* slots, void* out_k, void* out_v, i
   p.status = status_device_ptr();
   if (dtype == 0) {
     auto *ok = static_cast<__nv_bfloat16*>(out_k), *ov = static_cast<__nv_bfloat16*>(out_v);
-    return D == 128 ? launch_rows(kv8_read_kernel<__nv_bfloat16, 128>, p, D, s, ok, ov) : launch_rows(kv8_read_kernel<__nv_bfloat16, 64>, p, D, s, ok, ov);
+    return D == 128 ? launch_rows<128>(kv8_read_kernel<__nv_bfloat16, 128>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<__nv_bfloat16, 64>, p, s, ok, ov);
   }
   auto *ok = static_cast<float*>(out_k), *ov = static_cast<float*>(out_v);
-  return D == 128 ? launch_rows(kv8_read_kernel<float, 128>, p, D, s, ok, ov) : launch_rows(kv8_read_kernel<float, 64>, p, D, s, ok, ov);
+  return D == 128 ? launch_rows<128>(kv8_read_kernel<float, 128>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<float, 64>, p, s, ok, ov);
 }
 }

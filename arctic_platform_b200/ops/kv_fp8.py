@@ -15,7 +15,6 @@ CUDA tensors run ``kv_fp8_*.cu``; CPU tensors run the plain PyTorch expressions 
 from __future__ import annotations
 
 import ctypes
-import math
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -23,6 +22,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from ..utils import checked
 from ..utils.transfer_stats import to_device
 
 PAGE = 16
@@ -51,7 +51,7 @@ def block_bytes(head_dim: int) -> int:
 class Fp8KVCache:
     """``data [..., pages, key heads, block]`` uint8: the blocks of one layer, or of all layers in front (:meth:`layer`)."""
 
-    __slots__ = ("data", "head_dim")
+    __slots__ = ("data", "head_dim", "num_pages", "num_kv_heads", "one_layer", "index")
 
     def __init__(self, data: torch.Tensor, head_dim: int):
         if head_dim not in DIMS:
@@ -63,6 +63,8 @@ class Fp8KVCache:
         if not data.is_contiguous() or data.data_ptr() % 16:
             raise ValueError("data must be contiguous and begin on a 16-byte boundary")
         self.data, self.head_dim = data, head_dim
+        # plain numbers: a decode step asks for them in every layer
+        self.num_pages, self.num_kv_heads, self.one_layer, self.index = data.shape[-3], data.shape[-2], data.dim() == 3, data.get_device()
 
     @staticmethod
     def zeros(num_pages: int, num_kv_heads: int, head_dim: int, device="cuda", layers: Optional[int] = None) -> "Fp8KVCache":
@@ -71,14 +73,6 @@ class Fp8KVCache:
 
     def layer(self, i: int) -> "Fp8KVCache":
         return Fp8KVCache(self.data[i], self.head_dim)
-
-    @property
-    def num_pages(self) -> int:
-        return self.data.shape[-3]
-
-    @property
-    def num_kv_heads(self) -> int:
-        return self.data.shape[-2]
 
     def nbytes(self) -> int:
         return self.data.numel()
@@ -90,40 +84,18 @@ class Fp8KVCache:
         return k, v, self.data[..., 2 * n:].unflatten(-1, (8, 2, 2))
 
 
-def _one_layer(cache: Fp8KVCache) -> torch.Tensor:
-    if cache.data.dim() != 3:
+def _refuse(cache: Fp8KVCache, **tensors) -> None:
+    """Says what is wrong with where the tensors are."""
+    if not cache.one_layer:
         raise ValueError("a cache of several layers: take one with .layer(i)")
-    return cache.data
-
-
-def _same_device(device, **tensors) -> None:
     for name, t in tensors.items():
-        if t.device != device:
-            raise ValueError(f"{name} lives on {t.device}, not on {device}")
+        if t.get_device() != cache.index:
+            raise ValueError(f"{name} lives on {t.device}, not on {cache.data.device}")
 
 
-def _ints(name: str, t: torch.Tensor, *shape: Optional[int]) -> None:
-    if t.dtype != torch.int32 or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)) \
-            or (t.numel() and t.stride(-1) != 1):
-        raise ValueError(f"{name} must be int32 {[n if n is not None else '*' for n in shape]} with neighbouring elements, got "
-                         f"{t.dtype} {list(t.shape)}")
-
-
-class _On:
-    """Launches go to the tensors' device, whichever is current."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
+def _elsewhere(cache: Fp8KVCache) -> bool:
+    """The cache is on another GPU than the current one."""
+    return cache.index != torch._C._cuda_getDevice()
 
 
 # --------------------------------------------------------------------------------------------- rows
@@ -143,15 +115,15 @@ def values_ref(codes: torch.Tensor, byte: torch.Tensor) -> torch.Tensor:
     return codes.contiguous().view(torch.float8_e4m3fn).float() * torch.exp2(byte.float() - 127)[..., None]
 
 
-def _check_rows(cache: Fp8KVCache, slots: torch.Tensor, distinct: bool = False) -> torch.Tensor:
-    data = _one_layer(cache)
-    _ints("slots", slots, None)
-    from ..utils import checked
-    if checked.active_for(slots):
+def _check_slots(cache: Fp8KVCache, slots: torch.Tensor, distinct: bool) -> None:
+    if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError(f"slots must be int32 [rows] with neighbouring elements, got {slots.dtype} {list(slots.shape)}")
+    if not cache.one_layer or slots.get_device() != cache.index:
+        _refuse(cache, slots=slots)
+    if checked.enabled() and checked.active_for(slots):
         checked.check_range("slots", slots, -(1 << 31), cache.num_pages * PAGE)
         if distinct:
             checked.check_distinct("slots", slots)
-    return data
 
 
 def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Fp8KVCache) -> None:
@@ -160,15 +132,17 @@ def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Fp8KVCac
 
     Magnitudes above 448 * 2^119 (2.98e38), infinities among them, become that; what is not a number stays none and leaves the
     rest of its row alone."""
-    data = _check_rows(cache, slots, distinct=True)
-    T, H, D = slots.shape[0], cache.num_kv_heads, cache.head_dim
+    _check_slots(cache, slots, True)
+    data, shape, dt = cache.data, (slots.shape[0], cache.num_kv_heads, cache.head_dim), k.dtype
     for name, t in (("k", k), ("v", v)):
-        if t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != k.dtype or tuple(t.shape) != (T, H, D):
-            raise ValueError(f"{name} must be bf16 or fp32 {[T, H, D]}, got {t.dtype} {list(t.shape)}")
-    _same_device(data.device, k=k, v=v, slots=slots)
+        if t.dtype is not dt or t.shape != shape or (dt is not torch.bfloat16 and dt is not torch.float32):
+            raise ValueError(f"{name} must be bf16 or fp32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+        if t.get_device() != cache.index:
+            _refuse(cache, **{name: t})
+    T, H, D = shape
     if T == 0:
         return
-    if not data.is_cuda:
+    if cache.index < 0:
         ck, cv, ex = cache.parts()
         at = slots[slots >= 0].long()
         if at.numel() and int(at.max()) >= cache.num_pages * PAGE:
@@ -179,55 +153,64 @@ def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Fp8KVCac
             codes[page, :, t] = c
             ex[page, :, t % 8, w, t // 8] = e
         return
-    k, v = _rows_aligned(k), _rows_aligned(v)
-    with _On(data.device):
-        _lib.check(_fn("write")(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(),
-                                data.data_ptr(), T, H, D, cache.num_pages, int(k.dtype == torch.float32), _lib.stream_ptr()),
-                   "kv8_write")
+    if _elsewhere(cache):
+        with torch.cuda.device(cache.index):
+            return write(k, v, slots, cache)
+    k, k0, k1 = _rows_aligned(k)
+    v, v0, v1 = _rows_aligned(v)
+    _lib.check(_fn("write")(k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, slots.data_ptr(), data.data_ptr(), T, H, D, cache.num_pages,
+                            dt is torch.float32, _lib.stream_ptr()), "kv8_write")
 
 
-def _rows_aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t [T, heads, D]`` itself where its rows are whole and begin on 16-byte boundaries, else a copy."""
-    unit = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % unit == 0 and t.stride(1) % unit == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _rows_aligned(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """``t [T, heads, D]`` itself where its rows are whole and begin on 16-byte boundaries, else a copy; its strides."""
+    a, b, c = t.stride()
+    if c != 1 or (a | b) % (16 // t.element_size()) or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        a, b, _ = t.stride()
+    return t, a, b
 
 
 def read(cache: Fp8KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that ``slots [T]`` hold, ``[T, heads, D]`` each, exact in ``dtype`` (bf16 or fp32); zeros for slots below 0."""
-    data = _check_rows(cache, slots)
-    if dtype not in (torch.bfloat16, torch.float32):
+    _check_slots(cache, slots, False)
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise ValueError(f"rows are read as bf16 or fp32, not {dtype}")
-    _same_device(data.device, slots=slots)
-    T, H, D = slots.shape[0], cache.num_kv_heads, cache.head_dim
-    if not data.is_cuda:
+    data, T, H, D = cache.data, slots.shape[0], cache.num_kv_heads, cache.head_dim
+    if cache.index < 0:
         if T and int(slots.max()) >= cache.num_pages * PAGE:
             raise ValueError("slots: beyond the cache's pages")
         ck, cv, ex = cache.parts()
         at = slots.long().clamp_min(0)
         page, t, keep = at // PAGE, at % PAGE, (slots >= 0)[:, None, None]
         return tuple(torch.where(keep, values_ref(c[page, :, t], ex[page, :, t % 8, w, t // 8]), 0.0).to(dtype) for w, c in enumerate((ck, cv)))
-    out = torch.empty((2, T, H, D), device=data.device, dtype=dtype)
-    k, v = out[0], out[1]
+    if _elsewhere(cache):
+        with torch.cuda.device(cache.index):
+            return read(cache, slots, dtype)
+    k, v = torch.empty((2, T, H, D), device=data.device, dtype=dtype).unbind()
     if T:
-        with _On(data.device):
-            _lib.check(_fn("read")(data.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, H, D, cache.num_pages,
-                                   int(dtype == torch.float32), _lib.stream_ptr()), "kv8_read")
+        _lib.check(_fn("read")(data.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, H, D, cache.num_pages,
+                               dtype is torch.float32, _lib.stream_ptr()), "kv8_read")
     return k, v
 
 
 # --------------------------------------------------------------------------------------------- attention
-def _check_queries(q: torch.Tensor, cache: Fp8KVCache, out: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-    data = _one_layer(cache)
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] == 0 or q.shape[1] % cache.num_kv_heads:
+def _check_queries(q: torch.Tensor, cache: Fp8KVCache, out: Optional[torch.Tensor]) -> Tuple[torch.Tensor, int]:
+    """The queries, copied where their rows are not whole or off the 16-byte boundaries; the distance of their rows."""
+    if q.dtype is not torch.bfloat16 or q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] == 0 or q.shape[1] % cache.num_kv_heads:
         raise ValueError(f"q must be bf16 [rows, a multiple of {cache.num_kv_heads} heads, {cache.head_dim}], got {q.dtype} {list(q.shape)}")
-    if out is not None and (out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != q.shape[2]):
-        raise ValueError("out must be bf16 of q's shape with whole rows")
-    _same_device(data.device, q=q, **({} if out is None else {"out": out}))
-    if q.stride(2) != 1 or q.stride(1) != q.shape[2] or q.stride(0) % 8 or q.data_ptr() % 16:
+    if not cache.one_layer or q.get_device() != cache.index:
+        _refuse(cache, q=q)
+    a, b, c = q.stride()
+    if out is not None:
+        if out.dtype is not torch.bfloat16 or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != cache.head_dim:
+            raise ValueError("out must be bf16 of q's shape with whole rows")
+        if out.get_device() != cache.index:
+            _refuse(cache, out=out)
+    if c != 1 or b != cache.head_dim or a % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    return q, data
+        a = q.stride(0)
+    return q, a
 
 
 def context_ref(cache: Fp8KVCache, pages: torch.Tensor, n: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -253,28 +236,31 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
     """``q [B, Hq, D]`` bf16, one token per sequence, over the first ``lengths [B]`` (int32) tokens on the pages ``page_table
     [B, max_pages]`` (int32) -> ``[B, Hq, D]`` bf16; zeros for sequences of length 0.  Query head ``h`` reads key head
     ``h // (Hq // Hkv)``; ``scale``: of the scores, ``D ** -0.5`` if None.  Entries of the table behind a sequence's pages are not looked at."""
-    q, data = _check_queries(q, cache, out)
+    q, ldq = _check_queries(q, cache, out)
     B, Hq, D = q.shape
-    _ints("page_table", page_table, B, None)
-    _ints("lengths", lengths, B)
-    _same_device(data.device, page_table=page_table, lengths=lengths)
-    scale = D ** -0.5 if scale is None else float(scale)
-    from ..utils import checked
-    if checked.active_for(q):
+    for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
+        if t.dtype is not torch.int32 or t.dim() != dims or t.shape[0] != B or (t.stride(dims - 1) != 1 and t.numel()):
+            raise ValueError(f"{name} must be int32 {'[%d, pages]' % B if dims == 2 else [B]} with neighbouring elements, got {t.dtype} {list(t.shape)}")
+        if t.get_device() != cache.index:
+            _refuse(cache, **{name: t})
+    data, scale = cache.data, D ** -0.5 if scale is None else float(scale)
+    if checked.enabled() and checked.active_for(q):
         checked.check_page_table("page_table", page_table, lengths, cache.num_pages, PAGE)
     if out is None:
-        out = torch.empty((B, Hq, D), device=q.device, dtype=q.dtype)
+        out = torch.empty((B, Hq, D), device=data.device, dtype=torch.bfloat16)
     if B == 0:
         return out
-    if not data.is_cuda:
+    if cache.index < 0:
         for b, n in enumerate(lengths.tolist()):
             k, v = context_ref(cache, page_table[b], n)
             out[b:b + 1] = attention_ref(q[b:b + 1].float(), k, v, torch.tensor([n - 1]), scale).to(q.dtype)
         return out
-    with _On(data.device):
-        _lib.check(_fn("decode")(q.data_ptr(), q.stride(0), data.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-                                 cache.num_pages, lengths.data_ptr(), out.data_ptr(), out.stride(0), B, Hq, cache.num_kv_heads, D, scale,
-                                 _lib.stream_ptr()), "kv8_decode")
+    if _elsewhere(cache):
+        with torch.cuda.device(cache.index):
+            return decode_attention(q, cache, page_table, lengths, scale, out)
+    _lib.check(_fn("decode")(q.data_ptr(), ldq, data.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+                             cache.num_pages, lengths.data_ptr(), out.data_ptr(), out.stride(0), B, Hq, cache.num_kv_heads, D, scale,
+                             _lib.stream_ptr()), "kv8_decode")
     return out
 
 
@@ -350,7 +336,7 @@ class ChunkPlan:
             used.append(p.astype(np.int32))
         rows = int(new.sum())
         plan = ChunkPlan(rows, new, lengths, used, heads, cache.num_kv_heads, cache.num_pages, cache.head_dim)
-        if cache.data.is_cuda and rows:
+        if cache.index >= 0 and rows:
             sms = torch.cuda.get_device_properties(cache.data.device).multi_processor_count
             plan.work = w = _work(new, lengths, heads, cache.num_kv_heads, sms)
             table = np.zeros((n, max(1, int(need.max()))), dtype=np.int32)
@@ -369,7 +355,8 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
     tokens of its sequence up to itself (:class:`ChunkPlan`), rows that see nothing are zeros.  Rows of ``q`` behind the last
     sequence are padding: they are left as they were in ``out``, zeros without it.  The new tokens' own keys and values are read from the
     cache: :func:`write` comes first.  Values whose tokens' exponents lie more than 100 below the largest of their sequence lose bits."""
-    q, data = _check_queries(q, cache, out)
+    q, ldq = _check_queries(q, cache, out)
+    data = cache.data
     T, Hq, D = q.shape
     if (Hq, cache.num_kv_heads, cache.num_pages, D) != (plan.heads, plan.kv_heads, plan.num_pages, plan.head_dim):
         raise ValueError("the plan was made for other heads or another cache")
@@ -377,28 +364,29 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
         raise ValueError(f"q has {T} rows, the plan's sequences bring {plan.rows}")
     scale = D ** -0.5 if scale is None else float(scale)
     if out is None:
-        out = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
+        out = torch.empty((T, Hq, D), device=data.device, dtype=torch.bfloat16)
         if T > plan.rows:
             out[plan.rows:].zero_()
     if plan.rows == 0:
         return out
-    if not data.is_cuda:
+    if cache.index < 0:
         row = 0
         for m, n, p in zip(plan.new.tolist(), plan.lengths.tolist(), plan.pages):
             k, v = context_ref(cache, torch.from_numpy(p), n)
             out[row:row + m] = attention_ref(q[row:row + m].float(), k, v, torch.arange(n - m, n), scale).to(q.dtype)
             row += m
         return out
-    if plan.items is None or plan.items.device != data.device:
+    if plan.items is None or plan.items.get_device() != cache.index:
         raise ValueError(f"the plan was not made for a cache on {data.device}")
     if out.stride(0) % 8 or out.data_ptr() % 16:             # rows off the 16-byte boundaries: by way of a copy
         out[:plan.rows].copy_(chunk_attention(q, cache, plan, scale)[:plan.rows])
         return out
-    with _On(data.device):
-        w = plan.work
-        scratch = torch.empty(w.part_tiles * 128 * (D + 2), device=q.device, dtype=torch.float32) if w.part_tiles else None
-        _lib.check(_fn("chunk")(q.data_ptr(), q.stride(0), data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
-                                plan.first.data_ptr(), w.ctas, plan.joins.data_ptr(), len(w.joins), w.part_tiles, int(w.one_tile),
-                                None if scratch is None else scratch.data_ptr(), out.data_ptr(), out.stride(0), T, Hq, cache.num_kv_heads, D,
-                                scale, _lib.stream_ptr()), "kv8_chunk")
+    if _elsewhere(cache):
+        with torch.cuda.device(cache.index):
+            return chunk_attention(q, cache, plan, scale, out)
+    w = plan.work
+    scratch = torch.empty(w.part_tiles * 128 * (D + 2), device=data.device, dtype=torch.float32).data_ptr() if w.part_tiles else None
+    _lib.check(_fn("chunk")(q.data_ptr(), ldq, data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
+                            plan.first.data_ptr(), w.ctas, plan.joins.data_ptr(), len(w.joins), w.part_tiles, w.one_tile, scratch,
+                            out.data_ptr(), out.stride(0), T, Hq, cache.num_kv_heads, D, scale, _lib.stream_ptr()), "kv8_chunk")
     return out
