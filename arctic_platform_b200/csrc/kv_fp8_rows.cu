@@ -12,8 +12,8 @@
 namespace apb {
 
 struct Kv8Rows {
-  const void* x[2];        // keys and values: [T, H, D] with the given strides in elements
-  long long ld[2], lh[2];
+  const void *k, *v;       // [T, H, D] with the given strides in elements
+  long long ldk, lhk, ldv, lhv;
   const int* slots;        // page * 16 + token in the page; below 0: none
   uint8_t* data;           // [pages, H, block]
   int T, H;
@@ -21,26 +21,31 @@ struct Kv8Rows {
   int* status;
 };
 
+// Eight neighbouring values as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 r = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+struct Eight {
+  uint4 r[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t w[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float4 r = reinterpret_cast<const float4*>(p)[i];
-    v[4 * i] = r.x, v[4 * i + 1] = r.y, v[4 * i + 2] = r.z, v[4 * i + 3] = r.w;
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v[4 * i] = __uint_as_float(r[i].x), v[4 * i + 1] = __uint_as_float(r[i].y);
+        v[4 * i + 2] = __uint_as_float(r[i].z), v[4 * i + 3] = __uint_as_float(r[i].w);
+      }
+    }
   }
-}
+};
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]);
 template <>
@@ -54,113 +59,118 @@ __device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// A warp has kAtOnce runs of rows of one token, 32 / kLanes rows each: all of their loads are on their way before the first is used.
-constexpr int kAtOnce = 4;
-template <int D>
+// A warp takes the same 32 / kLanes rows of AT tokens behind one another, all of their loads on the way before the first is used: tokens
+// that lie in one page share its exponents' sector.  AT = 4 moves the most; where there are fewer runs than fill the GPU, AT = 1 is
+// sooner done (a step of 128 tokens: 2.0 us instead of 2.8).
+template <int D, int AT>
 struct RowsWalk {
-  static constexpr int kLanes = D / 8, kRows = 32 / kLanes, kPerWarp = kRows * kAtOnce;
-  int t, row0, part;        // token, first row of this lane's of its 2 H, eight values of it
-  __device__ __forceinline__ bool start(const Kv8Rows& p, int warps_per_token) {
+  static constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+  int t, row, part;         // first token, this lane's row of the 2 H, eight values of it
+  bool there;
+  __device__ __forceinline__ RowsWalk(const Kv8Rows& p, int per_token) {
     const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    t = w / warps_per_token;
-    row0 = (w - t * warps_per_token) * kPerWarp + lane / kLanes;
+    t = w / per_token;
+    row = (w - t * per_token) * kRows + lane / kLanes;
+    there = row < 2 * p.H;
+    t *= AT;
     part = lane % kLanes;
-    return t < p.T;
   }
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv8_write_kernel(const Kv8Rows p, int warps_per_token) {
+template <typename T, int D, int AT>
+__global__ void __launch_bounds__(256) kv8_write_kernel(const Kv8Rows p, int per_token) {
   pdl_entry();
-  using Walk = RowsWalk<D>;
-  Walk at;
-  if (!at.start(p, warps_per_token)) return;
-  const int slot = p.slots[at.t];
-  float v[kAtOnce][8];
+  const RowsWalk<D, AT> at(p, per_token);
+  if (at.t >= p.T) return;
+  const int row = min(at.row, 2 * p.H - 1), which = row >= p.H, h = row - which * p.H;      // all lanes stay for the shuffles
+  const T* from = static_cast<const T*>(which ? p.v : p.k) + h * (which ? p.lhv : p.lhk) + at.part * 8;
+  const long long ld = which ? p.ldv : p.ldk;
+  int slot[AT];
+  Eight<T> x[AT];
 #pragma unroll
-  for (int i = 0; i < kAtOnce; ++i) {
-    const int row = min(at.row0 + i * Walk::kRows, 2 * p.H - 1), which = row >= p.H, h = row - which * p.H;      // all lanes stay for the shuffles
-    load8(static_cast<const T*>(p.x[which]) + at.t * p.ld[which] + h * p.lh[which] + at.part * 8, v[i]);
+  for (int i = 0; i < AT; ++i) {
+    const int t = min(at.t + i, p.T - 1);
+    slot[i] = at.t + i < p.T ? p.slots[t] : -1;
+    x[i].load(from + t * ld);
   }
-  if (slot < 0) return;
-  if (slot >= p.slots_end) {
-    if (p.status) atomicCAS(p.status, 0, kBadTable);
-    return;
-  }
-  const int token = slot % kKv8Page;
-  uint8_t* page = p.data + static_cast<long long>(slot / kKv8Page) * p.H * Kv8<D>::kBlock;
+  uint8_t* const to = p.data + static_cast<long long>(h) * Kv8<D>::kBlock;
 #pragma unroll
-  for (int i = 0; i < kAtOnce; ++i) {
-    const int row = at.row0 + i * Walk::kRows, which = row >= p.H, h = row - which * p.H;
-    float most = 0.f;
+  for (int i = 0; i < AT; ++i) {
+    float v[8], most = 0.f;
+    x[i].get(v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(v[i][k]));
+    for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(v[k]));
 #pragma unroll
-    for (int o = 1; o < Walk::kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (row >= 2 * p.H) continue;
-    const int e = kv8_exponent(most);
+    for (int o = 1; o < RowsWalk<D, AT>::kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (!at.there || slot[i] < 0) continue;
+    if (slot[i] >= p.slots_end) {
+      if (p.status) atomicCAS(p.status, 0, kBadTable);
+      continue;
+    }
+    const int e = kv8_exponent(most), token = slot[i] % kKv8Page;
     const float f = exp2_int(-e);
     uint16_t c[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) c[k] = e4m3_pair(v[i][2 * k] * f, v[i][2 * k + 1] * f);
-    uint8_t* block = page + h * Kv8<D>::kBlock;
+    for (int k = 0; k < 4; ++k) c[k] = e4m3_pair(v[2 * k] * f, v[2 * k + 1] * f);
+    uint8_t* block = to + static_cast<long long>(slot[i] / kKv8Page) * p.H * Kv8<D>::kBlock;
     *reinterpret_cast<uint2*>(block + which * Kv8<D>::kHalf + token * D + at.part * 8) =
         make_uint2(c[0] | static_cast<uint32_t>(c[1]) << 16, c[2] | static_cast<uint32_t>(c[3]) << 16);
     if (at.part == 0) block[2 * Kv8<D>::kHalf + kv8_exponent_at(token, which)] = static_cast<uint8_t>(e + 127);
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Rows p, int warps_per_token, T* out_k, T* out_v) {
+template <typename T, int D, int AT>
+__global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Rows p, int per_token, T* out_k, T* out_v) {
   pdl_entry();
-  using Walk = RowsWalk<D>;
-  Walk at;
-  if (!at.start(p, warps_per_token)) return;
-  int slot = p.slots[at.t];
-  if (slot >= p.slots_end) {
-    if (p.status) atomicCAS(p.status, 0, kBadTable);
-    slot = -1;
-  }
-  const int token = slot % kKv8Page;
-  const uint8_t* page = p.data + static_cast<long long>(slot / kKv8Page) * p.H * Kv8<D>::kBlock;
-  uint2 c[kAtOnce];
-  int e[kAtOnce];
+  const RowsWalk<D, AT> at(p, per_token);
+  if (at.t >= p.T || !at.there) return;
+  const int which = at.row >= p.H, h = at.row - which * p.H;
+  const uint8_t* const from = p.data + static_cast<long long>(h) * Kv8<D>::kBlock;
+  int slot[AT], e[AT];
+  uint2 c[AT];
 #pragma unroll
-  for (int i = 0; i < kAtOnce; ++i) {
-    const int row = at.row0 + i * Walk::kRows, which = row >= p.H, h = row - which * p.H;
-    const uint8_t* block = page + h * Kv8<D>::kBlock;
+  for (int i = 0; i < AT; ++i) slot[i] = at.t + i < p.T ? p.slots[at.t + i] : -1;
+#pragma unroll
+  for (int i = 0; i < AT; ++i) {
     c[i] = make_uint2(0, 0);
     e[i] = 0;
-    if (row < 2 * p.H && slot >= 0) {
+    if (slot[i] >= p.slots_end) {
+      if (p.status) atomicCAS(p.status, 0, kBadTable);
+    } else if (slot[i] >= 0) {
+      const int token = slot[i] % kKv8Page;
+      const uint8_t* block = from + static_cast<long long>(slot[i] / kKv8Page) * p.H * Kv8<D>::kBlock;
       c[i] = *reinterpret_cast<const uint2*>(block + which * Kv8<D>::kHalf + token * D + at.part * 8);
       e[i] = block[2 * Kv8<D>::kHalf + kv8_exponent_at(token, which)];
     }
   }
 #pragma unroll
-  for (int i = 0; i < kAtOnce; ++i) {
-    const int row = at.row0 + i * Walk::kRows, which = row >= p.H, h = row - which * p.H;
-    if (row >= 2 * p.H) break;
+  for (int i = 0; i < AT; ++i) {
+    if (at.t + i >= p.T) break;
     const float f = exp2f(static_cast<float>(e[i]) - 127.f);
     const uint16_t pair[4] = {static_cast<uint16_t>(c[i].x), static_cast<uint16_t>(c[i].x >> 16), static_cast<uint16_t>(c[i].y),
                               static_cast<uint16_t>(c[i].y >> 16)};
     float v[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint32_t x = e4m3_to_f16x2(pair[k]);
-      const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x));
-      v[2 * k] = y.x * f;
-      v[2 * k + 1] = y.y * f;
+      const uint32_t y = e4m3_to_f16x2(pair[k]);
+      const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&y));
+      v[2 * k] = z.x * f;
+      v[2 * k + 1] = z.y * f;
     }
-    store8((which ? out_v : out_k) + (static_cast<long long>(at.t) * p.H + h) * D + at.part * 8, v);
+    store8((which ? out_v : out_k) + (static_cast<long long>(at.t + i) * p.H + h) * D + at.part * 8, v);
   }
 }
 
-template <int D, typename K, typename... Args>
-static int launch_rows(K kernel, const Kv8Rows& p, cudaStream_t s, Args... args) {
-  const int per_token = (2 * p.H + RowsWalk<D>::kPerWarp - 1) / RowsWalk<D>::kPerWarp;
-  const long long blocks = (static_cast<long long>(p.T) * per_token + 7) / 8;
-  if (blocks * 8 >= 1ll << 31) return kBadArgument;
-  return static_cast<int>(launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, p, per_token, args...));
+// kernel<AT> for the AT that fits
+template <int D, typename K4, typename K1, typename... Args>
+static int launch_rows(K4 four, K1 one, const Kv8Rows& p, cudaStream_t s, Args... args) {
+  const int per_token = (2 * p.H + RowsWalk<D, 1>::kRows - 1) / RowsWalk<D, 1>::kRows;
+  const bool few = static_cast<long long>(p.T) * per_token <= sm_count() * 32ll;
+  const long long warps = (static_cast<long long>(p.T) + 3) / (few ? 1 : 4) * per_token;
+  if (warps >= 1ll << 31) return kBadArgument;
+  const dim3 grid(static_cast<unsigned>((warps + 7) / 8));
+  return static_cast<int>(few ? launch_kernel(one, grid, dim3(256), 0, s, p, per_token, args...)
+                              : launch_kernel(four, grid, dim3(256), 0, s, p, per_token, args...));
 }
 
 }  // namespace apb
@@ -178,9 +188,9 @@ int apb_kv8_write(const void* k, long long ldk, long long lhk, const void* v, lo
       ldv % unit || lhv % unit || reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16 ||
       reinterpret_cast<uintptr_t>(data) % 16)
     return kBadArgument;
-  Kv8Rows p = {{k, v}, {ldk, ldv}, {lhk, lhv}, slots, static_cast<uint8_t*>(data), T, H, pages * kKv8Page, status_device_ptr()};
-  if (dtype == 0) return D == 128 ? launch_rows<128>(kv8_write_kernel<__nv_bfloat16, 128>, p, s) : launch_rows<64>(kv8_write_kernel<__nv_bfloat16, 64>, p, s);
-  return D == 128 ? launch_rows<128>(kv8_write_kernel<float, 128>, p, s) : launch_rows<64>(kv8_write_kernel<float, 64>, p, s);
+  Kv8Rows p = {k, v, ldk, lhk, ldv, lhv, slots, static_cast<uint8_t*>(data), T, H, pages * kKv8Page, status_device_ptr()};
+  if (dtype == 0) return D == 128 ? launch_rows<128>(kv8_write_kernel<__nv_bfloat16, 128, 4>, kv8_write_kernel<__nv_bfloat16, 128, 1>, p, s) : launch_rows<64>(kv8_write_kernel<__nv_bfloat16, 64, 4>, kv8_write_kernel<__nv_bfloat16, 64, 1>, p, s);
+  return D == 128 ? launch_rows<128>(kv8_write_kernel<float, 128, 4>, kv8_write_kernel<float, 128, 1>, p, s) : launch_rows<64>(kv8_write_kernel<float, 64, 4>, kv8_write_kernel<float, 64, 1>, p, s);
 }
 
 // out_k, out_v: [T, H, D] of bf16 (dtype 0) or fp32 (1); zeros where slots[t] is below 0.
@@ -198,9 +208,9 @@ int apb_kv8_read(const void* data, const int* slots, void* out_k, void* out_v, i
   p.status = status_device_ptr();
   if (dtype == 0) {
     auto *ok = static_cast<__nv_bfloat16*>(out_k), *ov = static_cast<__nv_bfloat16*>(out_v);
-    return D == 128 ? launch_rows<128>(kv8_read_kernel<__nv_bfloat16, 128>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<__nv_bfloat16, 64>, p, s, ok, ov);
+    return D == 128 ? launch_rows<128>(kv8_read_kernel<__nv_bfloat16, 128, 4>, kv8_read_kernel<__nv_bfloat16, 128, 1>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<__nv_bfloat16, 64, 4>, kv8_read_kernel<__nv_bfloat16, 64, 1>, p, s, ok, ov);
   }
   auto *ok = static_cast<float*>(out_k), *ov = static_cast<float*>(out_v);
-  return D == 128 ? launch_rows<128>(kv8_read_kernel<float, 128>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<float, 64>, p, s, ok, ov);
+  return D == 128 ? launch_rows<128>(kv8_read_kernel<float, 128, 4>, kv8_read_kernel<float, 128, 1>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<float, 64, 4>, kv8_read_kernel<float, 64, 1>, p, s, ok, ov);
 }
 }
