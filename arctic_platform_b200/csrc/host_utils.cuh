@@ -38,7 +38,25 @@ inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// The same with thread-block clusters of `cluster` CTAs along x (1: none); the grid is a multiple of it.
+// A kernel that always may start (set-up, loads of arguments) while its predecessor still runs: its first access to anything that the
+// predecessor writes, or reads and it writes, comes behind pdl_wait().
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_kernel_after(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                       Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// launch_kernel with thread-block clusters of `cluster` CTAs along x (1: none); the grid is a multiple of it.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_kernel_clusters(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster,
                                           cudaStream_t stream, Args... args) {

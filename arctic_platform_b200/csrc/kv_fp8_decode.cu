@@ -426,6 +426,282 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
   }
 }
 
+// All pages of all sequences in one row, cut into equal shares: a CTA walks its share through whichever units (sequence, key head, group
+// of query heads) it meets, its warps take the pairs of pages of a unit in turn, and the copies of the next unit's pages are on
+// their way while this one's results are joined.  A unit that lies in one share is finished there; of one that crosses borders every share
+// leaves its part, and kv8_join_kernel joins them.
+struct Kv8Parts {
+  float *o, *s;               // [CTAs][2] rows: of the unit that began in front of the share, of one that goes on behind it; a row is
+                              // [8 H][D] numerators, [8 H][4]: M, m, l
+  int4* crossing;             // the unit that begins in a CTA and goes on behind it: sequence, unit of it, CTAs (0: none), the first of
+                              // them; by CTA, or by unit where there are fewer of those
+  bool by_unit;
+  int least;                  // pages of a share at least
+};
+constexpr int kKv8Warps = 4;
+
+template <int D, int H>
+struct Kv8StreamCfg {
+  static constexpr int kRing = kKv8Stages * 64 * D;
+  static constexpr int kJoin = kKv8Warps * 4 * (D + 4) * 4;          // four heads of every warp
+  static constexpr int kSmem = kKv8Warps * kRing + kJoin + kKv8Warps * kKv8Stages * 8 + 64 + 1024;
+};
+
+// Parts of a head added up, V dimensions a lane.
+template <int V>
+struct Kv8Joined {
+  float top = kKv8None, m = kKv8None, l = 0.f, o[V] = {};
+  __device__ __forceinline__ void add(const float4& s, const float (&v)[V]) {
+    const float t1 = fmaxf(top, s.x), m1 = fmaxf(m, s.y), fo = ex2(top - t1), gn = ex2(s.x - t1);
+    l = l * ex2(m - m1) + s.z * ex2(s.y - m1);
+#pragma unroll
+    for (int x = 0; x < V; ++x) o[x] = o[x] * fo + v[x] * gn;
+    top = t1, m = m1;
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* out) const {
+    const Kv8Final fin(top, m, l);
+#pragma unroll
+    for (int x = 0; x < V; x += 2) *reinterpret_cast<uint32_t*>(out + x) = pack_bf16x2(fin(o[x]), fin(o[x + 1]));
+  }
+};
+template <int V>
+__device__ __forceinline__ void kv8_load_part(const float* o, const float* sums, bool there, float4& s, float (&v)[V]) {
+  s = make_float4(kKv8None, kKv8None, 0.f, 0.f);
+#pragma unroll
+  for (int x = 0; x < V; ++x) v[x] = 0.f;
+  if (!there) return;
+  s = __ldcg(reinterpret_cast<const float4*>(sums));
+#pragma unroll
+  for (int x = 0; x < V; x += 2) {
+    const float2 y = __ldcg(reinterpret_cast<const float2*>(o + x));
+    v[x] = y.x, v[x + 1] = y.y;
+  }
+}
+
+template <int D, int H>
+__global__ void __launch_bounds__(32 * kKv8Warps, H == 1 ? 3 : 2)
+kv8_decode_stream_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p, const Kv8Parts parts) {
+  using Cfg = Kv8StreamCfg<D, H>;
+  constexpr int kHeads = 8 * H, kThreads = 32 * kKv8Warps;
+  extern __shared__ uint8_t kv8_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv8_smem) + 1023) & ~uintptr_t(1023));
+  float* jo = reinterpret_cast<float*>(smem + kKv8Warps * Cfg::kRing);          // [warps][4][D]
+  float* js = jo + kKv8Warps * 4 * D;                                           // [warps][4][4]: M, m, l
+  uint64_t* bars = reinterpret_cast<uint64_t*>(js + kKv8Warps * 4 * 4);
+  int* found = reinterpret_cast<int*>(bars + kKv8Warps * kKv8Stages);           // sequence that the share begins in, pages in front of it; sums of the warps
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int R = p.Hq / p.Hkv, U = p.Hkv * p.groups;
+  uint64_t* full = bars + warp * kKv8Stages;
+  if (lane == 0) {
+    for (int s = 0; s < kKv8Stages; ++s) mbar_init(&full[s], 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&map);
+  }
+  pdl_entry();
+
+  auto tokens_of = [&](int b) { return min(max(p.lengths[b], 0), p.max_pages * kKv8Page); };
+  auto pages_of = [&](int b) { return (tokens_of(b) + kKv8Page - 1) / kKv8Page; };
+  int from, to, share;        // this share; pages of all but the last ones
+  {
+    const int per = (p.B + kThreads - 1) / kThreads, b0 = min(p.B, static_cast<int>(threadIdx.x) * per), b1 = min(p.B, b0 + per);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) {
+      mine += pages_of(b);
+      if (p.lengths[b] > p.max_pages * kKv8Page && p.status) atomicCAS(p.status, 0, kBadTable);
+    }
+    int end = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += t;
+    }
+    if (lane == 31) found[2 + warp] = end;
+    __syncthreads();
+    int at = end - mine, total = 0;
+#pragma unroll
+    for (int k = 0; k < kKv8Warps; ++k) {
+      if (k < warp) at += found[2 + k];
+      total += found[2 + k];
+    }
+    total *= U;
+    constexpr int kRound = 2 * kKv8Warps;            // pages that the warps take at a time
+    const int even = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    share = (max(parts.least, even) + kRound - 1) / kRound * kRound;
+    from = min(total, static_cast<int>(blockIdx.x) * share);
+    to = min(total, from + share);
+    if (from < to && at * U <= from && from < (at + mine) * U) {
+      int b = b0;
+      for (;; ++b) {
+        const int np = pages_of(b);
+        if (from < (at + np) * U) break;
+        at += np;
+      }
+      found[0] = b;
+      found[1] = at;
+    }
+    if (threadIdx.x == 0 && !parts.by_unit) parts.crossing[blockIdx.x] = make_int4(0, 0, 0, 0);
+    for (int b = blockIdx.x; b < p.B; b += gridDim.x)       // sequences without tokens
+      if (pages_of(b) == 0) {
+        for (int i = threadIdx.x; i < p.Hq * D; i += kThreads) p.out[b * p.ldo + i] = __float2bfloat16(0.f);
+        if (parts.by_unit)
+          for (int i = threadIdx.x; i < U; i += kThreads) parts.crossing[b * U + i] = make_int4(0, 0, 0, 0);
+      }
+    __syncthreads();
+    if (from == to) return;
+  }
+  // where a walk through the share is: pages [j, end) of unit u of sequence b, which has np pages; `left` pages of the share from j on
+  struct Cursor {
+    int b, u, j, np, left;
+    __device__ __forceinline__ int pages() const { return min(np - j, left); }
+  };
+  Cursor c;
+  c.b = found[0];
+  c.np = pages_of(c.b);
+  {
+    const int in = from - found[1] * U;
+    c.u = in / c.np;
+    c.j = in - c.u * c.np;
+    c.left = to - from;
+  }
+  auto next_unit = [&](Cursor& x) {           // there is one: pages of the share are left
+    x.left -= x.pages();
+    x.j = 0;
+    if (x.left > 0 && ++x.u == U) {
+      x.u = 0;
+      do ++x.b;
+      while ((x.np = pages_of(x.b)) == 0);
+    }
+  };
+  Kv8Copies<D> copies{&map, p, smem + warp * Cfg::kRing, full, lane};
+  Cursor f = c;               // of the copies
+  int pair = warp, ids_at = -64, ids = 0, asked = 0;      // pair of f's pages; ids: of pairs [ids_at, + 64) by fours, two lanes each
+  uint32_t next[2] = {~0u, ~0u};
+  auto issue = [&]() {
+    while (f.left > 0 && 2 * pair >= f.pages()) {
+      next_unit(f);
+      pair = warp;
+      ids_at = -64;
+    }
+    if (f.left <= 0) return;
+    const int n = f.pages();
+    if (pair >= ids_at + 64) {
+      ids_at = pair;
+      const int at = 2 * (pair + (lane >> 1) * kKv8Warps) + (lane & 1);
+      ids = copies.checked(at < n ? p.table[f.b * p.ld_table + f.j + at] : 0);
+    }
+    const int i = (pair - ids_at) / kKv8Warps * 2, id0 = __shfl_sync(0xffffffffu, ids, i), id1 = __shfl_sync(0xffffffffu, ids, i + 1);
+    copies.ask(asked++, id0, id1, 2 * pair + 1 < n, f.u / p.groups, next);
+    pair += kKv8Warps;
+  };
+  issue();
+  Kv8Heads<D, H> acc;
+  bool ok = true;
+  int copy = 0, at = from;
+  while (c.left > 0) {
+    const int n = c.pages(), pairs = (n + 1) / 2, len = tokens_of(c.b);
+    const int group = c.u % p.groups, head0 = c.u / p.groups * R + group * kHeads, heads = min(kHeads, R - group * kHeads);
+    acc.start(p.q + c.b * p.ldq + head0 * D, heads, p.scale_log2, lane);
+#pragma unroll 1
+    for (int k = warp; k < pairs && ok; k += kKv8Warps, ++copy) {
+      const uint32_t ex[2] = {next[0], next[1]};
+      issue();
+      ok = copies.wait(copy);
+      if (!ok) break;
+      acc.pages(copies.stage(copy), ex, min(len - (c.j + 2 * k) * kKv8Page, (n - 2 * k) * kKv8Page), lane);
+      __syncwarp();
+    }
+    acc.finish();
+    const bool whole = n == c.np;
+    const long long row0 = (static_cast<long long>(blockIdx.x) * 2 + (at - c.j < from ? 0 : 1)) * kHeads;
+    // the warps' results, four heads at a time
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll 1
+    for (int h4 = 8 * h; h4 < min(heads, 8 * h + 8); h4 += 4) {
+      constexpr int N = D / 8;
+      if ((lane & 3) / 2 == h4 / 4 % 2) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = warp * 4 + 2 * (lane & 1) + e;
+          float* dst = jo + row * D + (lane >> 2) * N;
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(acc.o[h][i][e], acc.o[h][i][2 + e]);
+          if (lane < 4) *reinterpret_cast<float4*>(js + row * 4) = make_float4(acc.top[h][e], acc.m[h][e], acc.l[h][e], 0.f);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = threadIdx.x; i < 4 * D; i += kThreads) {
+        const int head = h4 + i / D, d = i % D;
+        if (head >= heads) break;
+        Kv8Joined<1> sum;
+#pragma unroll
+        for (int k = 0; k < kKv8Warps; ++k) {
+          const float v[1] = {jo[k * 4 * D + i]};
+          sum.add(*reinterpret_cast<const float4*>(js + (k * 4 + i / D) * 4), v);
+        }
+        if (whole) {
+          p.out[c.b * p.ldo + (head0 + head) * D + d] = __float2bfloat16(Kv8Final(sum.top, sum.m, sum.l)(sum.o[0]));
+        } else {
+          parts.o[(row0 + head) * D + d] = sum.o[0];
+          if (d == 0) *reinterpret_cast<float4*>(parts.s + (row0 + head) * 4) = make_float4(sum.top, sum.m, sum.l, 0.f);
+        }
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x == 0 && c.j == 0) {
+      const int ctas = (at + c.np - 1) / share - static_cast<int>(blockIdx.x) + 1;
+      if (parts.by_unit || ctas > 1)
+        parts.crossing[parts.by_unit ? c.b * U + c.u : blockIdx.x] = make_int4(c.b, c.u, ctas > 1 ? ctas : 0, blockIdx.x);
+    }
+    at += n;
+    next_unit(c);
+  }
+  if (!ok) copies.give_up();
+}
+
+// Joins the parts of the units that cross borders between CTAs; KB parts are loaded at a time.  WARPS > 1: a CTA per unit and head, its
+// warps take the parts in turn and one joins theirs; else a warp per head.
+template <int D, int H, int WARPS, int KB>
+__global__ void __launch_bounds__(32 * (WARPS > 1 ? WARPS : 16)) kv8_join_kernel(const Kv8Decode p, const Kv8Parts parts) {
+  pdl_wait();
+  constexpr int kHeads = 8 * H, V = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 unit = __ldcg(parts.crossing + blockIdx.x);
+  const int n = unit.z, R = p.Hq / p.Hkv, group = unit.y % p.groups, heads = min(kHeads, R - group * kHeads);
+  const int head = WARPS > 1 ? blockIdx.y : warp, first = WARPS > 1 ? warp : 0;
+  if (n == 0 || head >= heads) return;
+  Kv8Joined<V> sum;
+  for (int k0 = first; k0 < n; k0 += WARPS * KB) {
+    float4 s[KB];
+    float v[KB][V];
+#pragma unroll
+    for (int i = 0; i < KB; ++i) {
+      const int k = k0 + WARPS * i;
+      const long long row = ((static_cast<long long>(unit.w) + k) * 2 + (k == 0)) * kHeads + head;
+      kv8_load_part<V>(parts.o + row * D + lane * V, parts.s + row * 4, k < n, s[i], v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < KB; ++i) sum.add(s[i], v[i]);
+  }
+  if constexpr (WARPS > 1) {
+    __shared__ float so[WARPS][D];
+    __shared__ float4 ss[WARPS];
+#pragma unroll
+    for (int x = 0; x < V; ++x) so[warp][lane * V + x] = sum.o[x];
+    if (lane == 0) ss[warp] = make_float4(sum.top, sum.m, sum.l, 0.f);
+    __syncthreads();
+    if (warp) return;
+    for (int k = 1; k < WARPS; ++k) {
+      float v[V];
+#pragma unroll
+      for (int x = 0; x < V; ++x) v[x] = so[k][lane * V + x];
+      sum.add(ss[k], v);
+    }
+  }
+  sum.store(p.out + unit.x * p.ldo + (unit.y / p.groups * R + group * kHeads + head) * D + lane * V);
+}
+
 // [blocks][32 rows of D codes]: what lies behind a block's codes is passed over
 static int kv8_map(CUtensorMap* map, const void* data, int D, long long blocks) {
   EncodeTiledFn fn = encode_tiled_fn();
@@ -453,27 +729,84 @@ static int launch_kv8_decode(const CUtensorMap& map, const Kv8Decode& p, cudaStr
                                                  p.splits, s, map, p));
 }
 
+// CTAs that a unit is cut into, of 8 pages at least, as long as all have a place
+static int kv8_splits(long long units, int longest) {
+  int splits = 1;
+  while (splits < 8 && units * splits * 2 <= 3 * sm_count() && splits * 8 < longest) splits *= 2;
+  return splits;
+}
+static int kv8_stream_ctas(int H) { return sm_count() * (H == 1 ? 3 : 2); }
+
+template <int D, int H>
+static int launch_kv8_stream(const CUtensorMap& map, const Kv8Decode& p, const Kv8Parts& parts, cudaStream_t s) {
+  constexpr int smem = Kv8StreamCfg<D, H>::kSmem;
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!configured[dev & 63]) {
+    cudaError_t e = cudaFuncSetAttribute(kv8_decode_stream_kernel<D, H>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    configured[dev & 63] = true;
+  }
+  const int ctas = kv8_stream_ctas(H);
+  const int rc = static_cast<int>(launch_kernel(kv8_decode_stream_kernel<D, H>, dim3(ctas), dim3(32 * kKv8Warps), smem, s, map, p, parts));
+  if (rc) return rc;
+  const int heads = p.Hq / p.Hkv < 8 * H ? p.Hq / p.Hkv : 8 * H, units = p.B * p.Hkv * p.groups;
+  if (parts.by_unit)          // parts of a unit: more than one on the mean
+    return static_cast<int>(launch_kernel_after(kv8_join_kernel<D, H, 8, 8>, dim3(units, heads), dim3(256), 0, s, p, parts));
+  return static_cast<int>(launch_kernel_after(kv8_join_kernel<D, H, 1, 2>, dim3(ctas), dim3(32 * heads), 0, s, p, parts));
+}
+
 }  // namespace apb
 
 extern "C" {
 using namespace apb;
 
+// Bytes of scratch that apb_kv8_decode should get for sequences of up to `longest` pages; 0: none, a cluster per unit is sooner done.
+//
+// Times are counted in rounds, in which the four warps of a CTA take two pages each: a CTA of a unit walks its part of the longest sequence
+// while others idle or wait for a place (a quarter of a walk where CTAs go in more than one wave and lengths differ); even shares
+// cost all pages over all places and about 6 rounds for finding them, for the parts and for the join.  Measured, unit / shares, 32 / 8
+// heads: 41 x 500..1500 tokens 22 / 28 us, 128 x 333..1000 41 / 49, 1 x 6000 11.6 / 13.0, 4 x 4000..12000 21.6 / 23.8; 1 x 36864 40.5 /
+// 21.5, 16 x 4000..12000 57 / 54, 64 x 1667..5000 93 / 83; 32 / 4 heads, 2 x 36864 42 / 23.
+long long apb_kv8_decode_scratch(int B, int longest, int Hq, int Hkv, int D) {
+  const int R = Hq / Hkv, H = R > 8 ? 2 : 1, places = kv8_stream_ctas(H);
+  const double units = static_cast<double>(B) * Hkv * ((R + 8 * H - 1) / (8 * H));
+  const int splits = kv8_splits(static_cast<long long>(units), longest);
+  const double walk = longest / (8.0 * splits), waves = units * splits / places;
+  const double unit = walk * (waves > 1 ? waves + 0.25 : 1.0), shares = units * longest / (8.0 * places) + 6.0;
+  return unit <= shares ? 0 : static_cast<long long>(places) * (2 * 8 * H * (D + 4) * 4 + 16);
+}
+
+// scratch: null, or what apb_kv8_decode_scratch says
 int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* table, long long ld_table, int max_pages, int pages,
-                   const int* lengths, void* out, long long ldo, int B, int Hq, int Hkv, int D, float scale, cudaStream_t s) {
+                   const int* lengths, void* out, long long ldo, int B, int longest, int Hq, int Hkv, int D, float scale, void* scratch, cudaStream_t s) {
   if (B <= 0) return 0;
   if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || pages < 1 || max_pages < 0 || static_cast<long long>(pages) * Hkv >= (1ll << 31) - 1 ||
-      ldq % 8 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(data) % 16)
+      ldq % 8 || ldo % 2 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 4 || reinterpret_cast<uintptr_t>(data) % 16 ||
+      reinterpret_cast<uintptr_t>(scratch) % 16)
     return kBadArgument;
   const int R = Hq / Hkv, H = R > 8 ? 2 : 1, groups = (R + 8 * H - 1) / (8 * H);
   const long long units = static_cast<long long>(B) * Hkv * groups;
-  int splits = 1;
-  while (splits < 8 && units * splits * 2 <= 3 * sm_count() && splits * 8 < max_pages) splits *= 2;
-  if (units * splits >= (1ll << 31)) return kBadArgument;
   CUtensorMap map;
   const int rc = kv8_map(&map, data, D, static_cast<long long>(pages) * Hkv);
   if (rc) return 1000 + rc;
-  const Kv8Decode p = {static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const uint8_t*>(data), table, ld_table, max_pages, pages, lengths,
-                       static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, groups, splits, scale * 1.4426950408889634f, status_device_ptr()};
+  Kv8Decode p = {static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const uint8_t*>(data), table, ld_table, max_pages, pages, lengths,
+                 static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, groups, 1, scale * 1.4426950408889634f, status_device_ptr()};
+  if (scratch) {
+    if (units * max_pages >= (1ll << 30)) return kBadArgument;
+    const long long rows = static_cast<long long>(kv8_stream_ctas(H)) * 2 * 8 * H;
+    Kv8Parts parts;
+    parts.o = static_cast<float*>(scratch);
+    parts.s = parts.o + rows * D;
+    parts.crossing = reinterpret_cast<int4*>(parts.s + rows * 4);
+    parts.by_unit = units * 4 <= kv8_stream_ctas(H);
+    parts.least = 2 * kKv8Warps;
+    if (D == 128) return H == 1 ? launch_kv8_stream<128, 1>(map, p, parts, s) : launch_kv8_stream<128, 2>(map, p, parts, s);
+    return H == 1 ? launch_kv8_stream<64, 1>(map, p, parts, s) : launch_kv8_stream<64, 2>(map, p, parts, s);
+  }
+  p.splits = kv8_splits(units, longest);
+  if (units * p.splits >= (1ll << 31)) return kBadArgument;
   if (D == 128) return H == 1 ? launch_kv8_decode<128, 1, 4>(map, p, s) : launch_kv8_decode<128, 2, 4>(map, p, s);
   return H == 1 ? launch_kv8_decode<64, 1, 4>(map, p, s) : launch_kv8_decode<64, 2, 4>(map, p, s);
 }

@@ -38,7 +38,8 @@ def _fn(name: str):
         vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
         _FN["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
         _FN["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
-        _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, f, vp])
+        _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, i, f, vp, vp])
+        _FN["scratch"] = _lib.declare("apb_kv8_decode_scratch", [i, i, i, i, i], ll)
         _FN["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, vp, i, vp, i, i, i, vp, vp, ll, i, i, i, i, f, vp])
     return _FN[name]
 
@@ -232,10 +233,13 @@ def attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, last: torch
 
 
 def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None,
-                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     out: Optional[torch.Tensor] = None, longest: Optional[int] = None) -> torch.Tensor:
     """``q [B, Hq, D]`` bf16, one token per sequence, over the first ``lengths [B]`` (int32) tokens on the pages ``page_table
     [B, max_pages]`` (int32) -> ``[B, Hq, D]`` bf16; zeros for sequences of length 0.  Query head ``h`` reads key head
-    ``h // (Hq // Hkv)``; ``scale``: of the scores, ``D ** -0.5`` if None.  Entries of the table behind a sequence's pages are not looked at."""
+    ``h // (Hq // Hkv)``; ``scale``: of the scores, ``D ** -0.5`` if None.  Entries of the table behind a sequence's pages are not looked at.
+
+    ``longest``: about how long the longest sequence is or will be, where the table is much wider than that; the kernel is chosen by it,
+    the result does not depend on it but for last bits."""
     q, ldq = _check_queries(q, cache, out)
     B, Hq, D = q.shape
     for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
@@ -257,9 +261,15 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
         return out
     if _elsewhere(cache):
         with torch.cuda.device(cache.index):
-            return decode_attention(q, cache, page_table, lengths, scale, out)
-    _lib.check(_fn("decode")(q.data_ptr(), ldq, data.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-                             cache.num_pages, lengths.data_ptr(), out.data_ptr(), out.stride(0), B, Hq, cache.num_kv_heads, D, scale,
+            return decode_attention(q, cache, page_table, lengths, scale, out, longest)
+    if out.stride(0) % 8 or out.data_ptr() % 16:             # rows off the 16-byte boundaries: by way of a copy
+        return out.copy_(decode_attention(q, cache, page_table, lengths, scale, None, longest))
+    wide = page_table.shape[1]
+    pages = wide if longest is None else min(wide, (longest + PAGE - 1) // PAGE)
+    need = _fn("scratch")(B, pages, Hq, cache.num_kv_heads, D)
+    scratch = torch.empty(need, device=data.device, dtype=torch.uint8).data_ptr() if need else None
+    _lib.check(_fn("decode")(q.data_ptr(), ldq, data.data_ptr(), page_table.data_ptr(), page_table.stride(0), wide, cache.num_pages,
+                             lengths.data_ptr(), out.data_ptr(), out.stride(0), B, pages, Hq, cache.num_kv_heads, D, scale, scratch,
                              _lib.stream_ptr()), "kv8_decode")
     return out
 

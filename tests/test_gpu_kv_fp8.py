@@ -163,6 +163,24 @@ def test_decode_sizes(B, length, Hq, H, D):
     _close(kv_fp8.decode_attention(q, cache, table, n), *_want(q, cache, table, n))
 
 
+@pytest.mark.parametrize("longest", [None, 0, 20000, 1 << 30])
+@pytest.mark.parametrize("Hq,H,D", [(8, 2, 128), (12, 1, 128), (4, 4, 64)])
+def test_decode_of_one_long_among_short_ones(Hq, H, D, longest):
+    """Whatever the hint about lengths says: shares of pages that many short sequences fill, and one sequence over many shares."""
+    lengths = [1, 0, 17, 5] * 20 + [0, 0, 20000, 3] + [40] * 9 + [0]
+    cache, table, n, _ = _filled(lengths, H, D, seed=2)
+    wide = torch.cat([table, torch.full((len(lengths), 900), -3, device="cuda", dtype=torch.int32)], 1)
+    q = torch.randn((len(lengths), Hq, D), device="cuda", generator=_gen(2)).bfloat16()
+    want = _want(q, cache, table, n)
+    out = torch.full_like(q, 7.0)
+    for t in (table, wide):
+        _close(kv_fp8.decode_attention(q, cache, t, n, out=out, longest=longest), *want)
+    assert not out[n == 0].any()
+    again = kv_fp8.decode_attention(q, cache, wide, n, longest=longest)
+    assert torch.equal(again, out)
+    _lib.check_status("decode")
+
+
 @pytest.mark.parametrize("case", ["large", "small", "values of unlike size", "one huge value nobody sees", "steep", "negative scale", "zero scale"])
 def test_decode_numbers(case):
     H, D, n = 2, 128, 300
