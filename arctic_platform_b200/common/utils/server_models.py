@@ -101,7 +101,7 @@ def parse_arctic_inference_rollout(ai_cfg: Optional[dict]) -> Dict[str, Any]:
 
 
 _SAMPLER_KEYS = {"max_model_len", "max_num_seqs", "kv_cache_tokens", "tensor_parallel_size", "gpu_memory_utilization",
-                 "enable_sleep_mode", "eos_token_id", "dtype", "seed"}
+                 "enable_sleep_mode", "eos_token_id", "dtype", "seed", "kv_cache_dtype"}
 
 
 def build_model_config(model_name: str, vllm_config: Optional[dict], ai_cfg: Optional[dict] = None) -> Dict[str, Any]:

@@ -161,6 +161,97 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Rows p, int per_
   }
 }
 
+// Behind the split-K qkv projection of a decode step: sums [B, (Hq + 2 H) D] in fp32 (cleared as they are read), RMSNorm and rotate-half
+// RoPE of q and k per head, q to bf16, k and v rounded to bf16 and into their slots, as decode_qkv_post_kernel and kv8_write_kernel
+// would leave them.  One warp per token and head; bound by launch and latency.
+struct Kv8QkvPost {
+  float* acc;
+  long long ld_acc;
+  const __nv_bfloat16 *wq, *wk;      // null: no norm
+  const float *cos_t, *sin_t;        // [positions, D / 2]
+  const int *pos, *slots;
+  __nv_bfloat16* q_out;              // [B, Hq, D]
+  uint8_t* data;
+  int B, Hq, H, slots_end;
+  float eps;
+  int* status;
+};
+template <int D>
+__global__ void __launch_bounds__(256) kv8_qkv_post_kernel(const Kv8QkvPost p) {
+  pdl_entry();
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 31, heads = p.Hq + 2 * p.H, w = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (w >= p.B * heads) return;
+  const int t = w / heads, h = w - t * heads;
+  float* src = p.acc + t * p.ld_acc + static_cast<long long>(h) * D;
+  float a[E], b[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    a[j] = src[lane * E + j];
+    b[j] = src[D / 2 + lane * E + j];
+    src[lane * E + j] = 0.f;
+    src[D / 2 + lane * E + j] = 0.f;
+  }
+  const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.H;
+  const int slot = p.slots[t];
+  if (!is_v) {
+    const __nv_bfloat16* weight = is_q ? p.wq : p.wk;
+    if (weight) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) ss += a[j] * a[j] + b[j] * b[j];
+      const float rstd = rsqrtf(warp_sum(ss) / D + p.eps);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        a[j] *= rstd * __bfloat162float(weight[lane * E + j]);
+        b[j] *= rstd * __bfloat162float(weight[D / 2 + lane * E + j]);
+      }
+    }
+    const long long at = static_cast<long long>(p.pos[t]) * (D / 2) + lane * E;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float c = p.cos_t[at + j], s = p.sin_t[at + j], x = a[j] * c - b[j] * s;
+      b[j] = b[j] * c + a[j] * s;
+      a[j] = x;
+    }
+  }
+  if (is_q) {
+    __nv_bfloat16* dst = p.q_out + (static_cast<long long>(t) * p.Hq + h) * D;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      dst[lane * E + j] = __float2bfloat16(a[j]);
+      dst[D / 2 + lane * E + j] = __float2bfloat16(b[j]);
+    }
+    return;
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    a[j] = __bfloat162float(__float2bfloat16(a[j]));
+    b[j] = __bfloat162float(__float2bfloat16(b[j]));
+    most = fmaxf(most, fmaxf(fabsf(a[j]), fabsf(b[j])));
+  }
+  most = warp_max(most);
+  if (slot < 0) return;
+  if (slot >= p.slots_end) {
+    if (p.status) atomicCAS(p.status, 0, kBadTable);
+    return;
+  }
+  const int e = kv8_exponent(most), token = slot % kKv8Page;
+  const float f = exp2_int(-e);
+  uint8_t* block = p.data + (static_cast<long long>(slot / kKv8Page) * p.H + (h - p.Hq - (is_v ? p.H : 0))) * Kv8<D>::kBlock;
+  uint8_t* row = block + is_v * Kv8<D>::kHalf + token * D;
+  if constexpr (E == 2) {
+    *reinterpret_cast<uint16_t*>(row + lane * 2) = e4m3_pair(a[0] * f, a[1] * f);
+    *reinterpret_cast<uint16_t*>(row + D / 2 + lane * 2) = e4m3_pair(b[0] * f, b[1] * f);
+  } else {
+    const uint16_t c = e4m3_pair(a[0] * f, b[0] * f);
+    row[lane] = static_cast<uint8_t>(c);
+    row[D / 2 + lane] = static_cast<uint8_t>(c >> 8);
+  }
+  if (lane == 0) block[2 * Kv8<D>::kHalf + kv8_exponent_at(token, is_v)] = static_cast<uint8_t>(e + 127);
+}
+
 // kernel<AT> for the AT that fits
 template <int D, typename K4, typename K1, typename... Args>
 static int launch_rows(K4 four, K1 one, const Kv8Rows& p, cudaStream_t s, Args... args) {
@@ -212,5 +303,17 @@ int apb_kv8_read(const void* data, const int* slots, void* out_k, void* out_v, i
   }
   auto *ok = static_cast<float*>(out_k), *ov = static_cast<float*>(out_v);
   return D == 128 ? launch_rows<128>(kv8_read_kernel<float, 128, 4>, kv8_read_kernel<float, 128, 1>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<float, 64, 4>, kv8_read_kernel<float, 64, 1>, p, s, ok, ov);
+}
+
+// acc [B, (Hq + 2 H) D] fp32, left as zeros; wq, wk [D] bf16 or null; cos, sin [positions, D / 2]; q_out [B, Hq, D] bf16.
+int apb_kv8_qkv_post(float* acc, long long ld_acc, const void* wq, const void* wk, const float* cos_t, const float* sin_t, const int* pos,
+                     const int* slots, void* q_out, void* data, int B, int Hq, int H, int D, int pages, float eps, cudaStream_t s) {
+  if (B <= 0) return 0;
+  if ((D != 64 && D != 128) || H < 1 || Hq < 1 || pages < 0 || pages > (1 << 27) || reinterpret_cast<uintptr_t>(data) % 16) return kBadArgument;
+  const Kv8QkvPost p = {acc, ld_acc, static_cast<const __nv_bfloat16*>(wq), static_cast<const __nv_bfloat16*>(wk), cos_t, sin_t, pos, slots,
+                        static_cast<__nv_bfloat16*>(q_out), static_cast<uint8_t*>(data), B, Hq, H, pages * kKv8Page, eps, status_device_ptr()};
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(B) * (Hq + 2 * H) + 7) / 8));
+  return static_cast<int>(D == 128 ? launch_kernel(kv8_qkv_post_kernel<128>, grid, dim3(256), 0, s, p)
+                                   : launch_kernel(kv8_qkv_post_kernel<64>, grid, dim3(256), 0, s, p));
 }
 }

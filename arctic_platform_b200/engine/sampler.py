@@ -16,7 +16,10 @@ engine for the same contract -- ``generate(prompts, sampling_params)`` returning
   start with the same tokens share a HEADER node (found at admission from the token ids, page aligned,
   prefilled and stored once), the rollouts of one prompt share the PROMPT node, and every sequence owns
   its private pages; each node is attended once per step by all sequences below it and the levels are
-  merged by log-sum-exp.
+  merged by log-sum-exp;
+* with ``kv_cache_dtype="fp8"`` keys and values are held in 8 bits (``ops/kv_fp8.py``): half the memory and half the bytes that decode
+  attention reads.  Prompts attend to their own keys in bf16; every decode step reads each sequence's whole context by itself
+  (pages of a prompt are still shared by its rollouts, headers are not looked for).
 
 Pages for a sequence's maximum length are reserved at admission, which keeps the decode loop free
 of host-side allocation.
@@ -34,7 +37,7 @@ import torch
 
 from ..models.config import DecoderConfig
 from ..models.decoder import DecoderLM
-from ..ops import _lib, gemm, norm
+from ..ops import _lib, gemm, kv_fp8, norm
 from ..ops.attention import AttnLayout, attention_fwd_cuda
 from ..utils.transfer_stats import to_device, to_host
 
@@ -81,6 +84,15 @@ class SamplingParams:
                 import logging
                 logging.getLogger(__name__).warning("sampling parameter %s=%r is not supported and is ignored", k, v)
         return sp
+
+
+def kv_cache_in_fp8(kv_cache_dtype: Optional[str]) -> bool:
+    """Whether this ``kv_cache_dtype`` asks for the 8-bit cache (``auto``, ``bfloat16`` and None: that of the model)."""
+    if kv_cache_dtype in (None, "", "auto", "bfloat16", "bf16"):
+        return False
+    if kv_cache_dtype in ("fp8", "fp8_e4m3"):
+        return True
+    raise ValueError(f"unsupported kv_cache_dtype {kv_cache_dtype!r} ('auto', 'bfloat16', 'fp8' or 'fp8_e4m3')")
 
 
 _I32P = ctypes.POINTER(ctypes.c_int32)
@@ -240,8 +252,13 @@ class SamplerEngine:
                  kv_cache_tokens: int = 1 << 20, max_batch: int = 256, max_seq_len: int = 8192,
                  cascade: bool = True, sync_interval: int = 16, use_cuda_graph: bool = True, seed: int = 0,
                  eos_token_id: Optional[int] = None, prefix_on_tensor_cores: bool = True, split_k: bool = True,
-                 quantization: Optional[str] = None, tp_group=None):
+                 quantization: Optional[str] = None, tp_group=None, kv_cache_dtype: Optional[str] = None):
         self.device = torch.device(device)
+        self.kv_fp8 = kv_cache_in_fp8(kv_cache_dtype)
+        if self.kv_fp8 and tp_group is not None:
+            raise NotImplementedError("tensor-parallel replicas hold their keys and values in bf16 (kv_cache_dtype 'auto')")
+        if self.kv_fp8 and cfg.head_dim not in kv_fp8.DIMS:
+            raise ValueError(f"kv_cache_dtype 'fp8' serves head sizes {kv_fp8.DIMS}, not {cfg.head_dim}")
         # tensor-parallel replica: this engine is ONE rank of ``tp`` and holds the heads / columns of its shard
         # (``vllm_config.tensor_parallel_size`` in the reference, arctic_platform/common/ray_server.py:375-404)
         self.tp_group = tp_group
@@ -302,10 +319,15 @@ class SamplerEngine:
     # ------------------------------------------------------------------ memory
     def _alloc_cache(self) -> None:
         c = self.cfg
-        shape = (c.num_layers, self.num_pages, c.num_kv_heads, PAGE, c.head_dim)
-        # zero-filled: the unwritten tail of a last page is multiplied by probability 0 and must be finite
-        self.kcache = torch.zeros(shape, device=self.device, dtype=torch.bfloat16)
-        self.vcache = torch.zeros(shape, device=self.device, dtype=torch.bfloat16)
+        if self.kv_fp8:
+            whole = kv_fp8.Fp8KVCache.zeros(self.num_pages, c.num_kv_heads, c.head_dim, self.device, layers=c.num_layers)
+            self.kcache = self.vcache = whole.data            # keys and values of a page lie in one block
+            self._kv8 = [whole.layer(li) for li in range(c.num_layers)]
+        else:
+            shape = (c.num_layers, self.num_pages, c.num_kv_heads, PAGE, c.head_dim)
+            # zero-filled: the unwritten tail of a last page is multiplied by probability 0 and must be finite
+            self.kcache = torch.zeros(shape, device=self.device, dtype=torch.bfloat16)
+            self.vcache = torch.zeros(shape, device=self.device, dtype=torch.bfloat16)
         if self.device.type == "cuda":
             from ..utils import memory_budget
             memory_budget.set_kv_resident(self.device, self.kv_bytes())
@@ -342,6 +364,8 @@ class SamplerEngine:
         self.d_g_pages = self.d_forest[B + 4 * N:].view(N, self.max_pages)
         self.n_levels = 1            # shared levels in use: 1 = prompt nodes only, 2 = header + prompt nodes
         self.forest_stats = {"shared_tokens": 0, "covered_tokens": 0}
+        self._bound = np.zeros(B, dtype=np.int64)    # tokens that a slot's sequence comes to at most
+        self._longest = 0            # 8-bit cache: bound on them all, by which decode attention is chosen
         self._one_launch = True      # decode attention of dense models over shared prompts: one launch or three
         self._own = np.zeros(B, dtype=np.int32)      # tokens on a slot's own pages, the one being fed included (as d_priv_len),
         self._left = np.zeros(B, dtype=np.int32)     # and steps that it has before it at most
@@ -382,7 +406,7 @@ class SamplerEngine:
         self.d_x = torch.empty((B, c.hidden_size), device=dev, dtype=torch.bfloat16)   # its embedding row
 
     def kv_bytes(self) -> int:
-        return 2 * self.kcache.numel() * 2
+        return self.kcache.numel() if self.kv_fp8 else 2 * self.kcache.numel() * 2
 
     # ------------------------------------------------------------------ layers (no autograd)
     @torch.no_grad()
@@ -396,9 +420,7 @@ class SamplerEngine:
         qkv = gemm.matmul_nt(h, blk.wqkv)
         q, k, v = norm.qknorm_rope(qkv, blk.q_norm, blk.k_norm, *self.model.rope(self.device), positions, c.num_heads,
                                    c.num_kv_heads, c.head_dim, c.rms_norm_eps)
-        _lib.check(_fn("kvw")(_lib.ptr(k), k.stride(0), _lib.ptr(v), v.stride(0), _lib.ptr(slots),
-                              _lib.ptr(self.kcache[li]), _lib.ptr(self.vcache[li]), k.shape[0], c.num_kv_heads,
-                              c.head_dim, _lib.stream_ptr()), "kv_cache_write")
+        self._write_kv(li, k, v, slots)
         a = attn_fn(li, q, k, v)
         if rows is not None:
             a, stream = a.index_select(0, rows), stream.index_select(0, rows)
@@ -410,6 +432,16 @@ class SamplerEngine:
             _, act = gemm.gate_up_swiglu(h2, blk.wgu, keep_gu=False)
             d = self._tp_sum(gemm.matmul_nt(act, blk.wdown))
         return d, stream
+
+    def _write_kv(self, li: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Keys and values ``[T, key heads, D]`` into their cache slots."""
+        if self.kv_fp8:
+            kv_fp8.write(k, v, slots, self._kv8[li])
+            return
+        c = self.cfg
+        _lib.check(_fn("kvw")(_lib.ptr(k), k.stride(0), _lib.ptr(v), v.stride(0), _lib.ptr(slots),
+                              _lib.ptr(self.kcache[li]), _lib.ptr(self.vcache[li]), k.shape[0], c.num_kv_heads,
+                              c.head_dim, _lib.stream_ptr()), "kv_cache_write")
 
     def _tp_sum(self, t: torch.Tensor) -> torch.Tensor:
         """Prefill under tensor parallelism: the row-parallel projections' partial results are summed over the
@@ -444,9 +476,7 @@ class SamplerEngine:
         qkv = fp8_linear(h, *w["wqkv"])
         q, k, v = norm.qknorm_rope(qkv, blk.q_norm, blk.k_norm, *self.model.rope(self.device), positions, c.num_heads,
                                    c.num_kv_heads, c.head_dim, c.rms_norm_eps)
-        _lib.check(_fn("kvw")(_lib.ptr(k), k.stride(0), _lib.ptr(v), v.stride(0), _lib.ptr(slots),
-                              _lib.ptr(self.kcache[li]), _lib.ptr(self.vcache[li]), k.shape[0], c.num_kv_heads,
-                              c.head_dim, _lib.stream_ptr()), "kv_cache_write")
+        self._write_kv(li, k, v, slots)
         a = attn_fn(li, q, k, v)
         if rows is not None:
             a, stream = a.index_select(0, rows), stream.index_select(0, rows)
@@ -460,6 +490,9 @@ class SamplerEngine:
     def _decode_attention(self, li: int, q: torch.Tensor, B: int) -> torch.Tensor:
         c = self.cfg
         scale = 1.0 / math.sqrt(c.head_dim)
+        if self.kv_fp8:
+            return kv_fp8.decode_attention(q.view(B, c.num_heads, c.head_dim), self._kv8[li], self.d_page_table[:B], self.d_len[:B], scale,
+                                           longest=self._longest)
         kc, vc = self.kcache[li], self.vcache[li]
         out = torch.empty((B, c.num_heads, c.head_dim), device=self.device, dtype=torch.bfloat16)
         seq_splits = self._seq_splits(B)
@@ -508,6 +541,8 @@ class SamplerEngine:
     def _choose_attention(self, B: int) -> None:
         """One launch or three until sequences join again, by the lengths that the host knows now and the steps that may follow."""
         self._one_launch = True
+        if self.kv_fp8:              # in powers of two: few graphs
+            self._longest = 1 << int(max(1, self._bound[:B].max()) - 1).bit_length()
         if self.cfg.is_moe or not self._cascade_on() or self.n_groups <= 0:
             return
         nodes = self._group_bucket()
@@ -525,7 +560,7 @@ class SamplerEngine:
         128.  Other shapes decode every sequence over its whole page table."""
         c = self.cfg
         R = c.num_heads // c.num_kv_heads
-        return bool(self.cascade and self.prefix_on_tensor_cores and c.head_dim == 128 and 128 % R == 0)
+        return bool(self.cascade and self.prefix_on_tensor_cores and not self.kv_fp8 and c.head_dim == 128 and 128 % R == 0)
 
     def _max_rows(self) -> int:
         """Sequences per shared-node tile (their query heads of one KV head fill at most 128 rows)."""
@@ -653,20 +688,22 @@ class SamplerEngine:
             if sq > 1:
                 # split-K qkv into fp32 sums, then one kernel: q/k norm + RoPE, q to bf16, k and v into the cache
                 gemm.gemm_raw(h, blk.wqkv, acc_qkv, M=B, N=c.qkv_size, K=H, epi=gemm.EPI_F32_ATOMIC, splits=sq, bn=128)
-                q = torch.empty((B, c.num_heads, c.head_dim), device=self.device, dtype=torch.bfloat16)
-                cos_t, sin_t = self.model.rope(self.device)
-                _lib.check(_fn("qkv_post")(_lib.ptr(acc_qkv), acc_qkv.stride(0), _lib.ptr(blk.q_norm), _lib.ptr(blk.k_norm),
-                                           _lib.ptr(cos_t), _lib.ptr(sin_t), _lib.ptr(positions), _lib.ptr(slots),
-                                           _lib.ptr(q), _lib.ptr(self.kcache[li]), _lib.ptr(self.vcache[li]), B,
-                                           c.num_heads, c.num_kv_heads, c.head_dim, c.rms_norm_eps, _lib.stream_ptr()),
-                           "decode_qkv_post")
+                if self.kv_fp8:
+                    q = kv_fp8.norm_rope_write(acc_qkv, blk.q_norm, blk.k_norm, self.model.rope(self.device), positions, slots, self._kv8[li],
+                                               c.num_heads, c.rms_norm_eps)
+                else:
+                    q = torch.empty((B, c.num_heads, c.head_dim), device=self.device, dtype=torch.bfloat16)
+                    cos_t, sin_t = self.model.rope(self.device)
+                    _lib.check(_fn("qkv_post")(_lib.ptr(acc_qkv), acc_qkv.stride(0), _lib.ptr(blk.q_norm), _lib.ptr(blk.k_norm),
+                                               _lib.ptr(cos_t), _lib.ptr(sin_t), _lib.ptr(positions), _lib.ptr(slots),
+                                               _lib.ptr(q), _lib.ptr(self.kcache[li]), _lib.ptr(self.vcache[li]), B,
+                                               c.num_heads, c.num_kv_heads, c.head_dim, c.rms_norm_eps, _lib.stream_ptr()),
+                               "decode_qkv_post")
             else:
                 qkv = gemm.matmul_nt(h, blk.wqkv)
                 q, k, v = norm.qknorm_rope(qkv, blk.q_norm, blk.k_norm, *self.model.rope(self.device), positions,
                                            c.num_heads, c.num_kv_heads, c.head_dim, c.rms_norm_eps)
-                _lib.check(_fn("kvw")(_lib.ptr(k), k.stride(0), _lib.ptr(v), v.stride(0), _lib.ptr(slots),
-                                      _lib.ptr(self.kcache[li]), _lib.ptr(self.vcache[li]), B, c.num_kv_heads,
-                                      c.head_dim, _lib.stream_ptr()), "kv_cache_write")
+                self._write_kv(li, k, v, slots)
             a = self._decode_attention(li, q, B).reshape(B, -1)
             gemm.gemm_raw(a, blk.wo, acc_o, M=B, N=H, K=c.q_size, epi=gemm.EPI_F32_ATOMIC, splits=so, bn=128)
             h2, stream = self._norm_f32(acc_o, blk.ln2, stream)
@@ -743,7 +780,7 @@ class SamplerEngine:
                 self._decode_step(B)
             return
         nodes = self._group_bucket() if self._cascade_on() else 0
-        key = (B, nodes, self.n_levels, self._filter_on, nodes == 0 or self._one_launch)
+        key = (B, nodes, self.n_levels, self._filter_on, nodes == 0 or self._one_launch, self._longest)
         g = self._graphs.get(key)
         if g is None:
             # the first steps run eagerly (kernel attribute set-up, device binding, allocator warm-up)
@@ -777,6 +814,7 @@ class SamplerEngine:
         if getattr(self, "d_arrived", None) is not None:
             self.d_arrived.zero_()         # a call that an error ended may have left arrivals behind
         self._own[:] = 0
+        self._bound[:] = 0
         prompts_np = [np.asarray(p, dtype=np.int64) for p in prompts]
         for p in prompts_np:
             if len(p) == 0:
@@ -895,7 +933,7 @@ class SamplerEngine:
             retired = bool(done_slots)
             if done_slots:
                 done_t = self._upload(np.asarray(done_slots, dtype=np.int64))
-                self._own[done_slots] = 0
+                self._own[done_slots] = self._bound[done_slots] = 0
                 freed: List[np.ndarray] = []
                 nout = to_host(self.d_out_idx[:B, 0]).numpy()
                 toks = to_host(self.d_out_tokens[:B]).numpy()
@@ -1069,6 +1107,7 @@ class SamplerEngine:
                 checked.check_page_table("page_table", pt, plen + sh - 1, self.num_pages, PAGE)
                 checked.check_page_table("priv_table", pv, plen - 1, self.num_pages, PAGE)
             self._own[slots], self._left[slots] = plen, sp.max_tokens - 1
+            self._bound[slots] = plen + sh + sp.max_tokens
             longs = self._upload(np.asarray(rows + slots + src + dst, dtype=np.int64))
             rows_t, st, src_t, dst_t = longs.split([n, n, len(src), len(src)])
             ints = self._upload(np.concatenate([pt.reshape(-1), pv.reshape(-1), plen, sh,
@@ -1117,7 +1156,8 @@ class SamplerEngine:
     def _copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Copies KV pages (a prompt's partial last page to every rollout) in all layers."""
         self.kcache[:, dst] = self.kcache[:, src]
-        self.vcache[:, dst] = self.vcache[:, src]
+        if not self.kv_fp8:
+            self.vcache[:, dst] = self.vcache[:, src]
 
     def _fork_slots(self, forks: List[Tuple[int, List[int]]]) -> None:
         """``(slot, other slots)``: the others continue from the state the first one's prompt left.  Nothing to do
@@ -1224,6 +1264,7 @@ class SamplerEngine:
             self._parked_graphs = None
         self._graphs = {}
         self.kcache = self.vcache = None
+        self._kv8 = []
         if self.device.type == "cuda":
             from ..utils import memory_budget
             memory_budget.set_kv_resident(self.device, 0)

@@ -176,7 +176,8 @@ class EngineWorker:
                 kv_cache_tokens=int(vc.get("kv_cache_tokens", 1 << 20)), max_batch=int(vc.get("max_num_seqs", 256)),
                 max_seq_len=int(vc.get("max_model_len", 8192)),
                 cascade=bool((job_config.get("arctic_inference_config") or {}).get("zorro_inference", {}).get("enable", True)),
-                seed=seed, eos_token_id=vc.get("eos_token_id"), quantization=vc.get("quantization"))
+                seed=seed, eos_token_id=vc.get("eos_token_id"), quantization=vc.get("quantization"),
+                **self._kv_cache_dtype(SamplerEngine, vc))
             if vc.get("enable_return_routed_experts"):
                 self.sampler.always_return_routing = True
             return True
@@ -230,6 +231,18 @@ class EngineWorker:
                         prefetch=int(opts.get("prefetch", 2)))
         return True
 
+    @staticmethod
+    def _kv_cache_dtype(engine, vllm_config: Dict[str, Any]) -> Dict[str, Any]:
+        """``kv_cache_dtype`` for the engine that has it; of the others a request for 8 bits is reported and they keep the model's type."""
+        from .sampler import SamplerEngine, kv_cache_in_fp8
+        asked = vllm_config.get("kv_cache_dtype")
+        if engine is SamplerEngine:
+            return {"kv_cache_dtype": asked}
+        if kv_cache_in_fp8(asked):
+            import logging
+            logging.getLogger(__name__).warning("kv_cache_dtype=%r: %s holds keys and values in the model's type", asked, engine.__name__)
+        return {}
+
     def _initialize_tp_sampler(self, job_config, model, tp: int, dtype, seed) -> bool:
         """A sampling replica over ``tp`` consecutive ranks of the job: every rank keeps a head / column shard of the
         decoder (``parallel/tp_sampler.py``) and all ranks of a replica are called together."""
@@ -245,6 +258,7 @@ class EngineWorker:
         paged = (self.device.type == "cuda" and not self.model_cfg.is_moe and self.model_cfg.layer_types is None
                  and self.model_cfg.head_dim == 128 and not vc.get("enable_return_routed_experts")
                  and vc.get("tp_engine", "paged") == "paged")
+        self._kv_cache_dtype(TensorParallelSampler, vc)          # neither engine of these replicas has it
         if paged:
             # dense decoders on GPUs: the paged CUDA engine with head shards of the KV cache and the fused
             # GEMM -> reduce-scatter / norm -> all-gather kernels in its decode loop

@@ -43,6 +43,7 @@ def main():
     ap.add_argument("--max-tokens", type=int, default=256)
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--no-cascade", action="store_true")
+    ap.add_argument("--kv-cache-dtype", default="auto", help="auto | fp8")
     ap.add_argument("--repeat", type=int, default=2)
     args = ap.parse_args()
     cfg = PRESETS[args.model]
@@ -62,7 +63,7 @@ def main():
     eng = SamplerEngine(cfg, "cuda", model=model, tp_group=group,
                         kv_cache_tokens=args.prompts * (args.prompt_len + 64) + B * (args.max_tokens + 64) + 4096,
                         max_batch=max(8, B), max_seq_len=args.prompt_len + args.max_tokens + 16,
-                        cascade=not args.no_cascade, use_cuda_graph=not args.no_graph)
+                        cascade=not args.no_cascade, use_cuda_graph=not args.no_graph, kv_cache_dtype=args.kv_cache_dtype)
     g = torch.Generator().manual_seed(0)
     res = {}
     for it in range(args.repeat):
@@ -85,7 +86,7 @@ def main():
     _lib.check_status("bench_decode")
     if rank == 0:
         print(json.dumps({"model": args.model, "layers": cfg.num_layers, "batch": B, "prompt_len": args.prompt_len,
-                          "max_tokens": args.max_tokens, "graph": not args.no_graph, "cascade": not args.no_cascade,
+                          "max_tokens": args.max_tokens, "graph": not args.no_graph, "cascade": not args.no_cascade, "kv_cache_dtype": args.kv_cache_dtype,
                           "tensor_parallel": world, "tp_step": os.environ.get("APB_TP_DECODE", "fused") if world > 1 else None,
                           **res}), flush=True)
     if world > 1:

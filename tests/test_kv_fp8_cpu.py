@@ -191,3 +191,19 @@ def test_plan_of_nothing():
     kv_fp8.write(torch.zeros(0, 2, 64), torch.zeros(0, 2, 64), torch.zeros(0, dtype=torch.int32), cache)
     assert kv_fp8.read(cache, torch.zeros(0, dtype=torch.int32))[0].shape == (0, 2, 64)
     assert np.array_equal(plan.new, [])
+
+
+def test_names_of_cache_types():
+    from arctic_platform_b200.engine.sampler import kv_cache_in_fp8
+    assert [kv_cache_in_fp8(n) for n in (None, "", "auto", "bfloat16", "fp8", "fp8_e4m3")] == [False] * 4 + [True] * 2
+    with pytest.raises(ValueError):
+        kv_cache_in_fp8("int8")
+
+
+def test_engines_without_it_say_so(caplog):
+    from arctic_platform_b200.engine.reference_sampler import ReferenceSampler
+    from arctic_platform_b200.engine.sampler import SamplerEngine
+    from arctic_platform_b200.engine.worker import EngineWorker
+    assert EngineWorker._kv_cache_dtype(SamplerEngine, {"kv_cache_dtype": "fp8"}) == {"kv_cache_dtype": "fp8"}
+    assert EngineWorker._kv_cache_dtype(ReferenceSampler, {"kv_cache_dtype": "auto"}) == {} and not caplog.records
+    assert EngineWorker._kv_cache_dtype(ReferenceSampler, {"kv_cache_dtype": "fp8"}) == {} and "ReferenceSampler" in caplog.text
