@@ -1,18 +1,29 @@
 // Attention of chunks of query tokens over the 8-bit cache (layout: kv_fp8.cuh) on tcgen05 tensor cores.
 //
 // A tile holds 128 rows: the query heads of one key head for 128 / heads neighbouring tokens, so that short chunks fill it too.  A CTA
-// walks work items of one or two such tiles over a range of 128-token blocks: S = Q K^T and O += P V by 128 x 128 MMAs, S and O in
-// tensor memory, P over S, one softmax warpgroup per tile, as in attention_fwd.cu.
+// (or a pair of them) walks work items of one or two such tiles over a range of 128-token blocks: S = Q K^T and O += P V by MMAs of 128 x
+// 128 per CTA, S and O in tensor memory, P over S, one softmax warpgroup per tile, one thread per row.
 //
 // Keys and values are bf16 operands here: kind::f16 wants both sides in 16 bits, and queries and weights do not fit 8.  Pages come by
-// bulk copies into a staging ring as they lie in the cache; two warps turn them into swizzled bf16 tiles, which serves both query
-// tiles.  A code becomes a bf16 number by moving its bits (exponents off by 120), two at a time, and one multiplication by a power of
-// two, which also brings in its token's exponent relative to a reference: for keys the block's largest exponent, which the softmax
-// multiplies by, for values one that moves only when a block's is larger by 2^8 or more, and O with it.  Nothing is rounded: 2^-120
-// of the reference is far below what counts (tokens more than 2^100 smaller than the largest of their sequence lose bits).
+// bulk copies into a staging ring as they lie in the cache; one or two warpgroups turn them into swizzled bf16 tiles.  A code becomes
+// a bf16 number by moving its bits (exponents off by 120), two at a time, and one multiplication by a power of two, which also brings
+// in its token's exponent relative to a reference: for keys the block's largest exponent, which the softmax multiplies by, for values
+// one that moves only when a block's is larger by 2^8 or more, and O with it.  Nothing is rounded: 2^-120 of the reference is far below
+// what counts (tokens more than 2^100 smaller than the largest of their sequence lose bits).
+//
+// What bounds it.  A block of two tiles is 2050 clocks of MMAs, 2050 of exponentials, 3000 of turning codes into tiles, and the three
+// wait for one another.  Hence the pair: its MMAs of 256 rows take half of the keys and half of the values' columns from either CTA, so
+// that each turns half of the codes.  And weights are taken relative to a reference that stays while they fit (the softmax below), in one
+// pass over the scores.  Both together took 512 new tokens of a 16896-token conversation (32/8 heads of 128) from 181 to 146 us, 960
+// TFLOP/s; 16 prompts' 397 to 324 (one CTA per item with this softmax: 168 and 355).  S in halves of 64 columns with buffers of their
+// own, so that the tensor core need not wait for the softmax, was slower (158: an MMA of 64 columns takes 0.7 of one of 128).
+// Short chunks (5 draft tokens: 27 us where the bytes take 4.8) have one tile of 20 rows, for which all codes are turned into tiles: two
+// warpgroups do that there (one: 31).
 //
 // Items over long contexts are cut along the keys where there are too few to fill the GPU (csrc/runtime_kv8.cpp); their parts are
 // joined by kv8_chunk_join_kernel.
+#include <type_traits>
+
 #include "attention_common.cuh"
 #include "host_utils.cuh"
 #include "kv_fp8.cuh"
@@ -43,20 +54,27 @@ struct Kv8Chunk {
   int* status;
 };
 
-// Four warpgroups: issue, codes to tiles, two of softmax.  Registers move between them: 80 + 96 + 2 * 168 = 4 * 128, what the block was
-// launched with.
-constexpr int kKcThreads = 512;
-constexpr int kKcConvert = 4;               // warps that turn codes into tiles
-constexpr int kKcRegsIssue = 80, kKcRegsConvert = 96, kKcRegsSoftmax = 168;
+constexpr float kKcRoom = 1.1e12f;          // 2^40: what a row's weights of a block may sum up to
 constexpr int kKcBlock = 128;
 constexpr int kKcStages = 2, kKcMeta = 4;
 
-template <int D, bool DUAL>
+// kTwo: a CTA per item of one or two tiles.
+// kDual: items of one tile each; the two softmax groups take every second block of it and join what they have at the item's end.
+// kPair: two CTAs per item, whose tiles have 256 rows, 128 for each; a CTA makes the half of the keys and the half of the values'
+// columns that its partner's tensor core then reads as well.
+enum Kv8ChunkForm : int { kTwo, kDual, kPair };
+
+template <int D, int FORM>
 struct Kv8ChunkCfg {
-  static constexpr int kTile = 128 * D * 2;
-  static constexpr int kQ = DUAL ? 1 : 2, kRing = DUAL ? 4 : 3;      // tiles
+  static constexpr int kTile = 128 * D * 2, kKv = FORM == kPair ? kTile / 2 : kTile;            // bytes of a tile of queries, of the ring
+  static constexpr int kQ = FORM == kDual ? 1 : 2, kRing = FORM == kTwo ? 3 : FORM == kDual ? 4 : 6;      // tiles
+  // Warpgroups: issue, one or two that turn codes into tiles, one of softmax per tile.  Registers move between them; their sum is what
+  // the block was launched with.
+  static constexpr int kConvert = FORM == kDual ? 8 : 4, kThreads = 128 + 32 * kConvert + 256;         // warps that turn codes into tiles
+  static constexpr int kRegsIssue = FORM == kDual ? 56 : 80, kRegsConvert = FORM == kDual ? 72 : 96, kRegsSoftmax = FORM == kDual ? 136 : 168;
+  static_assert(kRegsIssue * 128 + kRegsConvert * 32 * kConvert + kRegsSoftmax * 256 <= (FORM == kDual ? 96 : 128) * kThreads, "registers");
   static constexpr int kStage = 8 * Kv8<D>::kBlock;
-  static constexpr int kSmem = (kQ + kRing) * kTile + kKcStages * kStage + 256 + (DUAL ? 1024 : 0) + 1024;
+  static constexpr int kSmem = kQ * kTile + kRing * kKv + kKcStages * kStage + 2048 + 384;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
 };
 
@@ -65,73 +83,144 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// Four codes times 2^-120 as bf16 pairs, each times its factor
+// A load whose bytes are counted on a barrier that may live in the partner CTA.
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void umma_bf16_ts_pair(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on the barrier at this place in both CTAs once every MMA issued so far is done.
+__device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+// Four codes times 2^-120 as bf16 pairs, each times its factor: in their order, or (cheaper by three instructions of eight that move
+// bits) the even ones first, where that can be put right later.
+template <bool ORDERED>
 __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t factor, uint32_t& lo, uint32_t& hi) {
-  const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
-  const uint32_t x = (a & 0x80008000u) | ((a >> 4) & 0x07F007F0u), y = (b & 0x80008000u) | ((b >> 4) & 0x07F007F0u);
+  uint32_t x, y;
+  if constexpr (ORDERED) {
+    const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
+    x = (a & 0x80008000u) | ((a >> 4) & 0x07F007F0u);
+    y = (b & 0x80008000u) | ((b >> 4) & 0x07F007F0u);
+  } else {
+    x = ((w * 256u) & 0x80008000u) | ((w * 16u) & 0x07F007F0u);
+    y = (w & 0x80008000u) | ((w >> 4) & 0x07F007F0u);
+  }
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(factor));
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(factor));
 }
 
-// DUAL: items of one tile each; the two softmax groups take every second block of it and join what they have at the item's end.
-template <int D, bool DUAL>
-__global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_constant__ CUtensorMap tma_q, const Kv8Chunk p) {
-  using Cfg = Kv8ChunkCfg<D, DUAL>;
+template <int D, int FORM>
+__global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
+    kv8_chunk_kernel(const __grid_constant__ CUtensorMap tma_q, const Kv8Chunk p) {
+  using Cfg = Kv8ChunkCfg<D, FORM>;
+  constexpr bool DUAL = FORM == kDual, PAIR = FORM == kPair;
+  constexpr int kConvert = Cfg::kConvert;
+  constexpr int kCtas = PAIR ? 2 : 1;
+  // Parts of a block's columns that softmax threads hand over one by one, so that the values' product of one runs beside the softmax of
+  // the next.  One where that is no gain: kDual's groups wait for tiles, and kPair's CTAs would have to meet twice as often.
+  constexpr int kHalves = FORM == kTwo ? 2 : 1, kCols = kKcBlock / kHalves;
   constexpr int kRing = Cfg::kRing, kChunks = D / 64;
-  extern __shared__ uint8_t kc_smem[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kc_smem) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t kc_smem[];
+  uint8_t* smem = kc_smem;
+  pdl_entry();
+  if (smem_u32(smem) & 1023) {             // the tiles' swizzle goes by the address
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kBadArgument);
+    return;
+  }
   uint8_t* smem_q = smem;
   uint8_t* smem_kv = smem + Cfg::kQ * Cfg::kTile;
-  uint8_t* smem_st = smem_kv + kRing * Cfg::kTile;
-  uint64_t* st_full = reinterpret_cast<uint64_t*>(smem_st + kKcStages * Cfg::kStage);
+  uint8_t* smem_st = smem_kv + kRing * Cfg::kKv;
+  uint8_t* smem_x = smem_st + kKcStages * Cfg::kStage;        // [2] 1 KB through which the softmax threads of a group pass numbers of rows
+  uint64_t* st_full = reinterpret_cast<uint64_t*>(smem_x + 2048);
   uint64_t* st_empty = st_full + kKcStages;
   uint64_t* kv_full = st_empty + kKcStages;
   uint64_t* kv_empty = kv_full + kRing;
   uint64_t* q_full = kv_empty + kRing;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;      // [2]
-  uint64_t* p_full = s_full + 2;       // [2]
-  uint64_t* o_full = p_full + 2;       // [2] once per item
-  uint64_t* pair = o_full + 2;         // DUAL: both softmax groups
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pair + 1);
-  int2* meta = reinterpret_cast<int2*>(tmem_holder + 2);      // [kKcMeta] reference exponents of a block's keys and values
-  float* other = reinterpret_cast<float*>(st_full) + 64;      // [2][128] DUAL: a number per row and group
-  int* other_ev = reinterpret_cast<int*>(meta + kKcMeta);     // [2]
+  uint64_t* p_full = s_full + 2;       // [2][2] of the halves
+  uint64_t* o_full = p_full + 4;       // [2][2] after a half's product, but for the last one's only at the end of an item
+  uint64_t* meet = o_full + 4;         // [4] kDual: the two warps of 32 rows
+  int2* meta = reinterpret_cast<int2*>(meet + 4);             // [kKcMeta] reference exponents of a block's keys and values
+  int* other_ev = reinterpret_cast<int*>(meta + kKcMeta);     // [2][4] kDual: what a group's O is in units of, for 32 rows each
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(other_ev + 8);
+  static_assert((2 * kKcStages + 2 * kRing + 2 + 10 + 4) * 8 + kKcMeta * 8 + 36 <= 384, "barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = PAIR ? cluster_cta_rank() : 0;          // 0 issues the products of both
   if (threadIdx.x == 0) {
     for (int s = 0; s < kKcStages; ++s) {
       mbar_init(&st_full[s], 1);
-      mbar_init(&st_empty[s], kKcConvert);
+      mbar_init(&st_empty[s], kConvert);
     }
     for (int s = 0; s < kRing; ++s) {
-      mbar_init(&kv_full[s], kKcConvert);
+      mbar_init(&kv_full[s], kCtas * kConvert);
       mbar_init(&kv_empty[s], 1);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     for (int g = 0; g < 2; ++g) {
       mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[g], 128);
-      mbar_init(&o_full[g], 1);
+      mbar_init(&p_full[g * 2], kCtas * 4);
+      mbar_init(&p_full[g * 2 + 1], kCtas * 4);
+      mbar_init(&o_full[g * 2], 1);
+      mbar_init(&o_full[g * 2 + 1], 1);
     }
-    mbar_init(pair, 256);
+    for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
     mbar_fence_init();
     tma_prefetch_desc(&tma_q);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_holder, 512);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_holder, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_holder, 512);
+      tmem_relinquish();
+    }
   }
   // rows that no query fills stay zeros
-  for (int i = threadIdx.x; i < Cfg::kQ * Cfg::kTile / 16; i += kKcThreads) reinterpret_cast<uint4*>(smem_q)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < Cfg::kQ * Cfg::kTile / 16; i += Cfg::kThreads) reinterpret_cast<uint4*>(smem_q)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();                // both CTAs' barriers are there before anybody signals the partner
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
-  const int item0 = p.first[blockIdx.x], item1 = p.first[blockIdx.x + 1];
+  const int item0 = p.first[blockIdx.x / kCtas], item1 = p.first[blockIdx.x / kCtas + 1];
+  // To the CTA that issues.  What it tells of is tiles in shared memory (behind a proxy fence) or weights in tensor memory (behind
+  // tcgen05's): released at the cluster's scope besides, an arrival took 1000 clocks.
+  auto arrive_issuer = [&](uint64_t* bar) {
+    if constexpr (PAIR)
+      mbar_arrive_remote(map_to_cta(smem_u32(bar), 0));
+    else
+      mbar_arrive(bar);
+  };
+  auto commit = [&](uint64_t* bar) {
+    if constexpr (PAIR)
+      tc_commit_both(bar);
+    else
+      tc_commit(bar);
+  };
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {      // of a whole warp
     const bool r = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code));
     tc_fence_after();
@@ -147,7 +236,6 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
   auto convert = [&]() {
     // ---------------------------------------------------------------- codes to tiles
     const int part = warp - 4;
-    constexpr int kUnits = D / 16;         // of 16 codes in a row
     bool ok = true;
     int st = 0, slot = 0;
     uint32_t st_phase = 0, phase = 0, n_blocks = 0;
@@ -172,50 +260,58 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         if (j == 0 || vmax > vref + 7) vref = vmax;       // factors up to 2^127 do without a new one
         if (part == 0 && lane == 0) meta[n_blocks % kKcMeta] = make_int2(kmax - 127, vref - 127);
         ++n_blocks;
-#pragma unroll 1
-        for (int which = 0; which < 2 && ok; ++which) {
-          const int ref = which ? vref : kmax;
-          const uint32_t sign = which ? 0u : p.key_sign;
+        const bool ragged = valid < kKcBlock;
+        auto tile = [&](auto value) {
+          constexpr int kValue = decltype(value)::value;
           ok = wait(&kv_empty[slot], phase ^ 1, kTimeoutEmpty);
-          if (!ok) break;
-          // A lane has the same 16 columns of every kStep-th token; the upper half of a row takes its two units the other
-          // way around, so that no bank is met twice.
-          const int c = lane % kUnits, u0 = 2 * (c & 3) + (c >> 2), t0 = (part * 32 + lane) / kUnits;
-          constexpr int kStep = 32 * kKcConvert / kUnits, kAt = 4;           // tokens between a lane's, of them at a time
-          const bool swap = c >> 2, ragged = valid < kKcBlock;
-          const uint32_t tile = smem_u32(smem_kv) + slot * Cfg::kTile + (c >> 2) * 16384;
-          const uint32_t codes = smem_u32(stage) + which * Kv8<D>::kHalf + c * 16, exps = smem_u32(stage) + 2 * Kv8<D>::kHalf;
-#pragma unroll 1
-          for (int i = t0; i < 128; i += kStep * kAt) {
-            uint4 w[kAt];
-            int e[kAt];
+          if (!ok) return;
+          // A lane has the same 16 columns of some tokens.  Eight neighbouring lanes read eight places of 16 bytes that lie in different
+          // banks, and so do the two they write to: one token's whole row, half of them with their two units the other way around, or
+          // (PAIR's values, half a row) those of a token and of another two pages on.
+          constexpr bool kHalfRow = PAIR && kValue;
+          constexpr int kUnits = (kHalfRow ? D / 2 : D) / 16, kRows = PAIR && !kValue ? 64 : 128;           // units of a row; tokens
+          constexpr int kAt = kRows * kUnits / (32 * kConvert);
+          const int c = kHalfRow ? lane & 3 : lane % kUnits;
+          const int t0 = kHalfRow ? (lane >> 2 & 1) * 32 + part * 4 + (lane >> 3) : (part * 32 + lane) / kUnits;
+          const bool swap = kHalfRow ? lane >> 2 & 1 : c >> 2;
+          const int u0 = kHalfRow ? 2 * c + swap : 2 * (c & 3) + swap;
+          // tokens from a lane's first to its k-th
+          auto after = [](int k) { return kHalfRow ? (k * 4 * kConvert & 31) + 64 * (k * 4 * kConvert >> 5) : k * (32 * kConvert / kUnits); };
+          static_assert(kHalfRow || 32 * kConvert / kUnits % 16 == 0, "a lane's tokens have the same place in their pages");
+          const int t_half = PAIR && !kValue ? static_cast<int>(cta) * 64 : 0;       // the first token of the tile
+          const uint32_t page0 = smem_u32(stage) + ((t0 + t_half) >> 4) * Kv8<D>::kBlock;
+          const uint32_t codes = page0 + kValue * Kv8<D>::kHalf + (t0 & 15) * D + c * 16 + (kHalfRow ? cta * (D / 2) : 0);
+          const uint32_t exps = page0 + 2 * Kv8<D>::kHalf + kv8_exponent_at(t0 & 15, kValue);
+          const uint32_t to = smem_u32(smem_kv) + slot * Cfg::kKv + (c >> 2) * kRows * 128 + t0 * 128, u = (u0 ^ (t0 & 7)) << 4;
+          const uint32_t sign = kValue ? 0u : p.key_sign;
+          const int up = 127 + 120 - (kValue ? vref : kmax);
+          uint4 w[kAt];
+          int e[kAt];
 #pragma unroll
-            for (int k = 0; k < kAt; ++k) {
-              const int t = i + k * kStep;
-              w[k] = lds128(codes + (t >> 4) * Kv8<D>::kBlock + (t & 15) * D);
-              e[k] = lds8(exps + (t >> 4) * Kv8<D>::kBlock + kv8_exponent_at(t & 15, which));
-            }
+          for (int k = 0; k < kAt; ++k) {
+            w[k] = lds128(codes + after(k) / 16 * Kv8<D>::kBlock);
+            e[k] = lds8(exps + after(k) / 16 * Kv8<D>::kBlock);
+          }
 #pragma unroll
-            for (int k = 0; k < kAt; ++k) {
-              const int t = i + k * kStep;
-              uint32_t f = static_cast<uint32_t>(max(127 + 120 + e[k] - ref, 0)) << 7;
-              f = f << 16 | f | sign;
-              if (ragged && t >= valid) w[k] = make_uint4(0, 0, 0, 0), f = 0;
-              uint4 a, b;
-              e4m3x4_to_bf16(swap ? w[k].z : w[k].x, f, a.x, a.y);
-              e4m3x4_to_bf16(swap ? w[k].w : w[k].y, f, a.z, a.w);
-              e4m3x4_to_bf16(swap ? w[k].x : w[k].z, f, b.x, b.y);
-              e4m3x4_to_bf16(swap ? w[k].y : w[k].w, f, b.z, b.w);
-              const uint32_t row = tile + t * 128, u = (u0 ^ (t & 7)) << 4;
-              sts128(row + u, a);
-              sts128(row + (u ^ 16), b);
-            }
+          for (int k = 0; k < kAt; ++k) {
+            uint32_t f = static_cast<uint32_t>(max(e[k] + up, 0)) * 0x00800080u + sign;      // two exponents
+            if (ragged && t_half + t0 + after(k) >= valid) w[k] = make_uint4(0, 0, 0, 0), f = 0;
+            uint4 a, b;
+            constexpr bool kOrdered = !kValue;
+            e4m3x4_to_bf16<kOrdered>(swap ? w[k].z : w[k].x, f, a.x, a.y);
+            e4m3x4_to_bf16<kOrdered>(swap ? w[k].w : w[k].y, f, a.z, a.w);
+            e4m3x4_to_bf16<kOrdered>(swap ? w[k].x : w[k].z, f, b.x, b.y);
+            e4m3x4_to_bf16<kOrdered>(swap ? w[k].y : w[k].w, f, b.z, b.w);
+            sts128(to + after(k) * 128 + u, a);
+            sts128(to + after(k) * 128 + (u ^ 16), b);
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&kv_full[slot]);
+          if (lane == 0) arrive_issuer(&kv_full[slot]);
           next(slot, phase, kRing);
-        }
+        };
+        tile(std::integral_constant<int, 0>());
+        if (ok) tile(std::integral_constant<int, 1>());
         if (!ok) break;
         if (lane == 0) mbar_arrive(&st_empty[st]);
         next(st, st_phase, kKcStages);
@@ -224,7 +320,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKcRegsIssue));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsIssue));
     if (warp == 0) {
       // ---------------------------------------------------------------- copies
       bool ok = true;
@@ -233,7 +329,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
       for (int at = item0; at < item1 && ok; ++at) {
         const Kv8Item w = p.items[at];
         if (w.blocks == 0) continue;
-        const int tiles = !DUAL && w.tokens > p.tp ? 2 : 1, pages = (w.len + kKv8Page - 1) / kKv8Page;
+        const int tiles = !DUAL && w.tokens > kCtas * p.tp ? 2 : 1, pages = (w.len + kKv8Page - 1) / kKv8Page;
         const int* table = p.table + w.seq * p.ld_table;
         auto page_of = [&](int j) {        // of block j, a lane each
           const int i = (w.block0 + j) * 8 + lane;
@@ -244,10 +340,17 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         if (!ok) break;
         ++n_q;
         if (lane == 0) {
-          mbar_expect_tx(q_full, tiles * kChunks * 128 * p.hp * p.tp);
+          if (cta == 0) mbar_expect_tx(q_full, kCtas * tiles * kChunks * 128 * p.hp * p.tp);
+          const uint32_t bar = PAIR ? map_to_cta(smem_u32(q_full), 0) : 0;
           for (int g = 0; g < tiles; ++g)
-            for (int c = 0; c < kChunks; ++c)
-              tma_load_3d(smem_q + g * Cfg::kTile + c * 16384, &tma_q, q_full, c * 64, w.head0, w.row0 + g * p.tp);
+            for (int c = 0; c < kChunks; ++c) {
+              uint8_t* to = smem_q + g * Cfg::kTile + c * 16384;
+              const int row = w.row0 + (g * kCtas + static_cast<int>(cta)) * p.tp;
+              if constexpr (PAIR)
+                tma_load_3d_pair(to, &tma_q, bar, c * 64, w.head0, row);
+              else
+                tma_load_3d(to, &tma_q, q_full, c * 64, w.head0, row);
+            }
         }
         for (int j = 0; j < w.blocks; ++j) {
           const int id_next = page_of(j + 1);
@@ -269,23 +372,36 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         while (global_timer_ns() - t0 < 100000ull) {
         }
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 && cta == 0) {
       // ---------------------------------------------------------------- products (one elected lane issues)
-      const uint32_t idesc_s = umma_idesc_bf16(128, kKcBlock, 0, 0), idesc_o = umma_idesc_bf16(128, D, 0, 1);
+      const uint32_t idesc_s = umma_idesc_bf16(kCtas * 128, kKcBlock, 0, 0), idesc_o = umma_idesc_bf16(kCtas * 128, D, 0, 1);
       const uint64_t desc_q = umma_smem_desc(smem_u32(smem_q), 0, 1024), desc_k = umma_smem_desc(smem_u32(smem_kv), 0, 1024);
       const uint64_t desc_v = umma_smem_desc(smem_u32(smem_kv), 16384, 1024);
-      constexpr uint32_t kT = Cfg::kTile >> 4;
+      constexpr uint32_t kT = Cfg::kTile >> 4, kKvT = Cfg::kKv >> 4;
       auto issue_s = [&](uint32_t g, uint32_t slot, uint32_t q) {
+        const uint32_t d = tmem_base + g * 128;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_bf16_ss(tmem_base + g * 128, desc_q + q * kT + (k / 4) * 1024 + (k % 4) * 2, desc_k + slot * kT + (k / 4) * 1024 + (k % 4) * 2,
-                       idesc_s, k > 0 ? 1u : 0u);
-        tc_commit(&s_full[g]);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t a = desc_q + q * kT + (k / 4) * 1024 + (k % 4) * 2;
+          const uint64_t b = desc_k + slot * kKvT + (k / 4) * (1024 / kCtas) + (k % 4) * 2;
+          if constexpr (PAIR)
+            umma_bf16_ss_pair(d, a, b, idesc_s, k > 0 ? 1u : 0u);
+          else
+            umma_bf16_ss(d, a, b, idesc_s, k > 0 ? 1u : 0u);
+        }
+        commit(&s_full[g]);
       };
-      auto issue_o = [&](uint32_t g, uint32_t slot, bool first) {
+      // the h-th part of the block's columns
+      auto issue_o = [&](uint32_t g, uint32_t h, uint32_t slot, bool first) {
 #pragma unroll
-        for (int k = 0; k < kKcBlock / 16; ++k)
-          umma_bf16_ts(tmem_base + 256 + g * 128, tmem_base + g * 128 + k * 8, desc_v + slot * kT + k * 128, idesc_o, (!first || k > 0) ? 1u : 0u);
+        for (int k = 0; k < kCols / 16; ++k) {
+          const uint32_t d = tmem_base + 256 + g * 128, a = tmem_base + g * 128 + h * 32 + k * 8;
+          const uint64_t b = desc_v + slot * kKvT + (h * 4 + k) * 128;
+          if constexpr (PAIR)
+            umma_bf16_ts_pair(d, a, b, idesc_o, (!first || k > 0) ? 1u : 0u);
+          else
+            umma_bf16_ts(d, a, b, idesc_o, (!first || k > 0) ? 1u : 0u);
+        }
       };
       int slot = 0;
       uint32_t phase = 0, n_q = 0, done[2] = {0, 0};
@@ -295,9 +411,9 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         return r;
       };
       bool ok = true;
-      uint32_t tile = 0;               // DUAL: number of the item's first tile
+      uint32_t tile = 0;               // kDual: number of the item's first tile
       for (int at = item0; at < item1 && ok; ++at) {
-        const int blocks = p.items[at].blocks, tiles = !DUAL && p.items[at].tokens > p.tp ? 2 : 1;
+        const int blocks = p.items[at].blocks, tiles = !DUAL && p.items[at].tokens > kCtas * p.tp ? 2 : 1;
         if (blocks == 0) continue;
         if constexpr (DUAL) {
           auto wait_tile = [&](uint32_t t) { return wait(&kv_full[t % kRing], (t / kRing) & 1, kTimeoutFull); };
@@ -306,8 +422,8 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
             if (!wait_tile(t)) return false;
             if (elect_one()) {
               issue_s(j & 1, t % kRing, 0);
-              tc_commit(&kv_empty[t % kRing]);
-              if (j + 1 == blocks) tc_commit(q_empty);
+              commit(&kv_empty[t % kRing]);
+              if (j + 1 == blocks) commit(q_empty);
             }
             __syncwarp();
             return true;
@@ -316,13 +432,13 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
           ++n_q;
           for (int j = 0; j < blocks && ok; ++j) {
             const uint32_t g = j & 1, t = tile + 2 * j + 1;
-            ok = wait_tile(t) && wait(&p_full[g], done[g] & 1, kTimeoutTmemEmpty);
+            ok = wait_tile(t) && wait(&p_full[g * 2], done[g] & 1, kTimeoutTmemEmpty);
             if (!ok) break;
             ++done[g];
             if (elect_one()) {
-              issue_o(g, t % kRing, j < 2);
-              tc_commit(&kv_empty[t % kRing]);
-              if (j + 2 >= blocks) tc_commit(&o_full[g]);
+              issue_o(g, 0, t % kRing, j < 2);
+              commit(&kv_empty[t % kRing]);
+              if (j + 2 >= blocks) commit(&o_full[g * 2]);
             }
             __syncwarp();
             if (j + 2 < blocks) ok = scores(j + 2);
@@ -336,8 +452,8 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
         ++n_q;
         if (elect_one()) {
           for (int g = 0; g < tiles; ++g) issue_s(g, sk, g);
-          tc_commit(&kv_empty[sk]);
-          if (blocks == 1) tc_commit(q_empty);
+          commit(&kv_empty[sk]);
+          if (blocks == 1) commit(q_empty);
         }
         __syncwarp();
         for (int j = 0; j < blocks && ok; ++j) {
@@ -345,213 +461,267 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv8_chunk_kernel(const __grid_c
           const int sv = slot;
           ok = wait_slot();
           sk = slot;
-          if (ok && more) ok = wait_slot();
-          if (!ok) break;
-          for (int g = 0; g < tiles && ok; ++g) {
-            ok = wait(&p_full[g], done[g] & 1, kTimeoutTmemEmpty);
+          if constexpr (kHalves == 1) {
+            if (ok && more) ok = wait_slot();          // ahead of the weights, not between them and their product
             if (!ok) break;
-            ++done[g];
-            if (elect_one()) {
-              issue_o(g, sv, j == 0);
-              if (more)
-                issue_s(g, sk, g);      // over P, which the product above reads first: the tensor core keeps the order of issue
-              else
-                tc_commit(&o_full[g]);
-              if (g == tiles - 1) {
-                tc_commit(&kv_empty[sv]);
-                if (more) tc_commit(&kv_empty[sk]);
-                if (j + 2 == blocks) tc_commit(q_empty);
+            for (int g = 0; g < tiles && ok; ++g) {
+              ok = wait(&p_full[g * 2], done[g] & 1, kTimeoutTmemEmpty);
+              if (!ok) break;
+              ++done[g];
+              if (elect_one()) {
+                issue_o(g, 0, sv, j == 0);
+                if (more)
+                  issue_s(g, sk, g);      // over P, which the product above reads first: the tensor core keeps the order of issue
+                else
+                  commit(&o_full[g * 2]);
+                if (g == tiles - 1) {
+                  commit(&kv_empty[sv]);
+                  if (more) commit(&kv_empty[sk]);
+                  if (j + 2 == blocks) commit(q_empty);
+                }
+              }
+              __syncwarp();
+            }
+          } else {
+            for (int g = 0; g < tiles && ok; ++g) {
+              for (int h = 0; h < 2 && ok; ++h) {
+                ok = wait(&p_full[g * 2 + h], done[g] >> 1 & 1, kTimeoutTmemEmpty);
+                if (!ok) break;
+                ++done[g];
+                if (elect_one()) {
+                  issue_o(g, h, sv, j == 0 && h == 0);
+                  commit(&o_full[g * 2 + h]);
+                  if (h == 1 && g == tiles - 1) commit(&kv_empty[sv]);
+                }
+                __syncwarp();
+                if (!more || h == 0) continue;
+                if (g == 0 && !(ok = wait_slot())) break;
+                if (elect_one()) {
+                  issue_s(g, sk, g);
+                  if (g == tiles - 1) {
+                    commit(&kv_empty[sk]);
+                    if (j + 2 == blocks) commit(q_empty);
+                  }
+                }
+                __syncwarp();
               }
             }
-            __syncwarp();
           }
         }
       }
     }
-  } else if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKcRegsConvert));
+  } else if (warp < 4 + kConvert) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsConvert));
     convert();
   } else {
     // ------------------------------------------------------------------ softmax groups
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKcRegsSoftmax));
-    const int g = (warp >> 2) - 2, quarter = warp & 3, row = quarter * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoftmax));
+    const int g = (warp - 4 - kConvert) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_s = tmem_base + lane_off + g * 128, t_o = tmem_base + lane_off + 256 + g * 128;
-    const int row_token = (DUAL ? 0 : g * p.tp) + row / p.hp, row_head = row % p.hp;
-    uint32_t blocks_seen = 0, blocks_all = 0, items = 0, met = 0;
+    const uint32_t t_s0 = tmem_base + lane_off + g * 128;        // scores; weights go over the first half of them
+    const uint32_t t_o = tmem_base + lane_off + 256 + g * 128;
+    const int row_token = (DUAL ? 0 : (g * kCtas + static_cast<int>(cta)) * p.tp) + row / p.hp, row_head = row % p.hp;
+    uint32_t parts_seen = 0, blocks_all = 0, items = 0, met = 0;
     bool ok = true;
-    auto meet = [&]() {                // the other group
+    auto meet_other = [&]() {
       tc_fence_before();
-      mbar_arrive(pair);
-      return wait(pair, met++ & 1, kTimeoutTmemFull);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&meet[quarter]);
+      return wait(&meet[quarter], met++ & 1, kTimeoutTmemFull);
     };
     for (int at = item0; at < item1 && ok; ++at) {
       const Kv8Item w = p.items[at];
-      if (!DUAL && g > 0 && w.tokens <= p.tp) {
+      if (!DUAL && g > 0 && w.tokens <= kCtas * p.tp) {
         blocks_all += w.blocks;
         continue;
       }
       const int seen = min(w.len, w.pos0 + row_token + 1) - w.block0 * kKcBlock;      // tokens of the range that the row sees (or more)
-      float m_run = -INFINITY;
+      float m_ref = -INFINITY;             // what weights are relative to: a score of the row not far below its largest
       uint64_t l2 = 0;
       int ev = 0;
-      const int mine_n = DUAL ? (w.blocks + 1 - g) / 2 : w.blocks;          // blocks of this group
+      const int mine_n = DUAL ? (w.blocks + 1 - g) / 2 : kHalves * w.blocks;          // this group's parts of blocks
       for (int k = 0; k < mine_n; ++k) {
-        const int j = DUAL ? 2 * k + g : k;
-        ok = wait(&s_full[g], blocks_seen & 1, kTimeoutTmemFull);
+        const int j = DUAL ? 2 * k + g : k / kHalves, h = k % kHalves;
+        const uint32_t t_s = t_s0 + h * 64;
+        if (h == 0) ok = wait(&s_full[g], parts_seen / kHalves & 1, kTimeoutTmemFull);
         if (!ok) break;
-        ++blocks_seen;
+        ++parts_seen;
         const int2 ref = meta[(blocks_all + j) % kKcMeta];
         const float c1 = fmaxf(p.scale_log2 * exp2_int(ref.x), 1.2e-38f);
         const uint64_t c2 = xtc_pair(c1, c1);
-        const int limit = seen - j * kKcBlock;
-        const bool masked = __any_sync(0xffffffffu, limit < kKcBlock);
-        // twice through the scores, 32 columns at a time and the next ones on their way: all 128 in registers spilled
-        uint32_t v[2][32];
-        auto mask = [&](int c, uint32_t (&x)[32]) {
+        const int limit = seen - j * kKcBlock - h * 64;
+        const bool masked = __any_sync(0xffffffffu, limit < kCols);
+        if (k == 0) ev = ref.y;
+        float alpha = 1.f;
+        auto mask = [&](int c, uint32_t (&x)[16]) {
           if (masked) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= limit) x[i] = 0xff800000u;
+            for (int i = 0; i < 16; ++i)
+              if (c * 16 + i >= limit) x[i] = 0xff800000u;
           }
         };
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_ld_32x32(t_s, v[0]);
-        tmem_ld_wait(v[0]);
+        // Once through the scores, 16 columns at a time and the next ones on their way.  The reference stays while weights fit in: any will
+        // do as long as nothing overflows, and bf16 has the range.  Where a block's sum passes 2^40 its weights are taken again, with
+        // the row's maximum as the reference (scores that spread by 130 nats, so that most blocks of some row do: 4.0 us a block for 2.4).
+        constexpr int kRuns = kCols / 16;
+        uint32_t pk[kCols / 2];
+        uint64_t sum = 0;
+        bool anew = __any_sync(0xffffffffu, m_ref == -INFINITY && limit > 0);
+#pragma unroll 1
+        for (int turn = 0; turn < 2; ++turn) {
+          uint32_t v[2][16];
+          tmem_ld_32x16(t_s, v[0]);
+          tmem_ld_wait(v[0]);
+          if (anew) {
+            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld_32x32(t_s + ((c + 1) & 3) * 32, v[(c + 1) & 1]);
-          mask(c, v[c & 1]);
+            for (int c = 0; c < kRuns; ++c) {
+              tmem_ld_32x16(t_s + (c + 1) % kRuns * 16, v[(c + 1) & 1]);
+              mask(c, v[c & 1]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            mx[(i >> 1) & 3] = fmaxf(fmaxf(mx[(i >> 1) & 3], __uint_as_float(v[c & 1][i])), __uint_as_float(v[c & 1][i + 1]));
-          tmem_ld_wait(v[(c + 1) & 1]);
-        }
-        const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1);
-        if (k == 0) ev = ref.y;
-        if (__any_sync(0xffffffffu, m_new > m_run) || ev != ref.y) {
-          if (k > 0) {           // O holds the blocks before this one: their product was issued ahead of this S
-            const float alpha = m_run == -INFINITY ? 0.f : xtc_ex2(m_run - m_new);
-            l2 = xtc_mul2(l2, xtc_pair(alpha, alpha));
-            const float ao = alpha * exp2_int(max(ev - ref.y, -126));
-            const uint64_t a2 = xtc_pair(ao, ao);
-            uint32_t r[2][16];
-            tmem_ld_32x16(t_o, r[0]);
-            tmem_ld_wait(r[0]);
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              if (c + 1 < D / 16) tmem_ld_32x16(t_o + (c + 1) * 16, r[(c + 1) & 1]);
-#pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                const float2 f = xtc_unpair(xtc_mul2(xtc_pair(__uint_as_float(r[c & 1][i]), __uint_as_float(r[c & 1][i + 1])), a2));
-                r[c & 1][i] = __float_as_uint(f.x);
-                r[c & 1][i + 1] = __float_as_uint(f.y);
-              }
-              tmem_st_32x16(t_o + c * 16, r[c & 1]);
-              if (c + 1 < D / 16) tmem_ld_wait(r[(c + 1) & 1]);
+              for (int i = 0; i < 16; i += 2)
+                mx[(i >> 1) & 1] = fmaxf(fmaxf(mx[(i >> 1) & 1], __uint_as_float(v[c & 1][i])), __uint_as_float(v[c & 1][i + 1]));
+              tmem_ld_wait(v[(c + 1) & 1]);
             }
+            const float m_new = fmaxf(m_ref, fmaxf(mx[0], mx[1]) * c1);
+            alpha = m_ref == -INFINITY ? 0.f : xtc_ex2(m_ref - m_new);
+            m_ref = m_new;
           }
-          m_run = m_new;
-          ev = ref.y;
-        }
-        const float m_use = m_run == -INFINITY ? 0.f : m_run;
-        const uint64_t nm2 = xtc_pair(-m_use, -m_use);
-        uint64_t sum[2] = {0, 0};
+          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+          const uint64_t nm2 = xtc_pair(-m_use, -m_use);
+          uint64_t part[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c < 3) tmem_ld_32x32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
-          mask(c, v[c & 1]);
-          uint32_t pk[16];
+          for (int c = 0; c < kRuns; ++c) {
+            if (c + 1 < kRuns) tmem_ld_32x16(t_s + (c + 1) * 16, v[(c + 1) & 1]);
+            mask(c, v[c & 1]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 f = xtc_unpair(xtc_fma2(xtc_pair(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), c2, nm2));
-            f.x = xtc_ex2(f.x);
-            f.y = xtc_ex2(f.y);
-            sum[i & 1] = xtc_add2(sum[i & 1], xtc_pair(f.x, f.y));
-            pk[i] = pack_bf16x2(f.x, f.y);
+            for (int i = 0; i < 8; ++i) {
+              float2 f = xtc_unpair(xtc_fma2(xtc_pair(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), c2, nm2));
+              f.x = xtc_ex2(f.x);
+              f.y = xtc_ex2(f.y);
+              part[i & 1] = xtc_add2(part[i & 1], xtc_pair(f.x, f.y));
+              pk[c * 8 + i] = pack_bf16x2(f.x, f.y);
+            }
+            if (c + 1 < kRuns) tmem_ld_wait(v[(c + 1) & 1]);
           }
-          if (c < 3) tmem_ld_wait(v[(c + 1) & 1]);
-          tmem_st_32x16(t_s + c * 16, pk);
+          sum = xtc_add2(part[0], part[1]);
+          const float2 f = xtc_unpair(sum);
+          if (anew || !__any_sync(0xffffffffu, !(f.x + f.y <= kKcRoom))) break;
+          anew = true;
         }
+        if (k > 0 && (anew || ev != ref.y)) {
+          // O with what came before: issued ahead of this S, but for the product of the block's first half
+          if (h == 1 && !(ok = wait(&o_full[g * 2], (parts_seen - 1) / kHalves & 1, kTimeoutTmemFull))) break;
+          l2 = xtc_mul2(l2, xtc_pair(alpha, alpha));
+          const float ao = alpha * exp2_int(max(ev - ref.y, -126));
+          const uint64_t a2 = xtc_pair(ao, ao);
+          uint32_t r[16];
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            tmem_ld_32x16(t_o + c * 16, r);
+            tmem_ld_wait(r);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float2 f = xtc_unpair(xtc_mul2(xtc_pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), a2));
+              r[i] = __float_as_uint(f.x);
+              r[i + 1] = __float_as_uint(f.y);
+            }
+            tmem_st_32x16(t_o + c * 16, r);
+          }
+        }
+        ev = ref.y;
+#pragma unroll
+        for (int c = 0; c < kCols / 64; ++c) tmem_st_32x32(t_s0 + h * 32 + c * 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + c * 32));
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_full[g]);
-        l2 = xtc_add2(l2, xtc_add2(sum[0], sum[1]));
+        __syncwarp();
+        if (lane == 0) arrive_issuer(&p_full[g * 2 + h]);
+        l2 = xtc_add2(l2, sum);
       }
       blocks_all += w.blocks;
       if (!ok) break;
       if (mine_n > 0) {
-        ok = wait(&o_full[g], items & 1, kTimeoutTmemFull);
+        ok = wait(&o_full[g * 2 + kHalves - 1], (kHalves == 1 ? items : (parts_seen - 1) >> 1) & 1, kTimeoutTmemFull);
         if (!ok) break;
         ++items;
       }
+      // output = own O * f0 * 2^ev + the other group's O * f1 * 2^ev1; kDual: half of the columns per group
       const float2 lp = xtc_unpair(l2);
       float l = lp.x + lp.y;
-      // output = (own O * f0 + the other group's O * f1): DUAL, a half of the columns each
-      float f0 = l == 0.f ? 0.f : exp2_int(ev) / l, f1 = 0.f;
+      float f0 = l == 0.f ? 0.f : 1.f / l, f1 = 0.f;
+      const float e0 = exp2_int(ev);
+      float e1 = 0.f;
+      constexpr int kOut = DUAL ? D / 2 : D;
+      const int col0 = DUAL ? g * kOut : 0;
       if constexpr (DUAL) {
-        auto pass = [&](float x) {       // this row's number of the other group
-          other[g * 128 + row] = x;
-          ok = ok && meet();
-          const float y = other[(1 - g) * 128 + row];
-          ok = ok && meet();
-          return y;
-        };
-        if (row == 0) other_ev[g] = ev;
-        const float m1 = pass(m_run), l1 = pass(l);
+        float* y = reinterpret_cast<float*>(smem_x) + row;            // [2] groups of [128] references and [128] sums
+        y[g * 256] = m_ref;
+        y[g * 256 + 128] = l;
+        if (lane == 0) other_ev[g * 4 + quarter] = ev;
+        ok = meet_other();
         if (!ok) break;
-        const float m = fmaxf(m_run, m1), a0 = l == 0.f ? 0.f : xtc_ex2(m_run - m), a1 = l1 == 0.f ? 0.f : xtc_ex2(m1 - m);
-        const int ev1 = other_ev[1 - g];
-        l = l * a0 + l1 * a1;
-        m_run = m;
-        f0 = a0 == 0.f ? 0.f : a0 * exp2_int(ev) / l;
-        f1 = a1 == 0.f ? 0.f : a1 * exp2_int(ev1) / l;
+        const float m1 = y[(1 - g) * 256], l1 = y[(1 - g) * 256 + 128];
+        const float m = fmaxf(m_ref, m1), a0 = l == 0.f ? 0.f : xtc_ex2(m_ref - m), a1 = l1 == 0.f ? 0.f : xtc_ex2(m1 - m);
+        l = g == 0 ? l * a0 + l1 * a1 : l1 * a1 + l * a0;
+        m_ref = m;
+        f0 = a0 == 0.f ? 0.f : a0 / l;
+        f1 = a1 == 0.f ? 0.f : a1 / l;
+        e1 = exp2_int(other_ev[(1 - g) * 4 + quarter]);
       }
       const bool mine = row < p.hp * p.tp && row_token < w.tokens && row_head < w.heads;
       __nv_bfloat16* dst = p.out + (static_cast<long long>(w.row0) + row_token) * p.ldo + (w.head0 + row_head) * D;
-      const long long part = (static_cast<long long>(w.part) + (DUAL ? 0 : g)) * 128 + row;
-      constexpr int kPer = DUAL ? D / 64 : D / 32;           // runs of 32 columns per group
+      const long long part = (static_cast<long long>(w.part) + (DUAL ? 0 : g * kCtas + static_cast<int>(cta))) * 128 + row;
 #pragma unroll 1
-      for (int c = DUAL ? g * kPer : 0; c < (DUAL ? (g + 1) * kPer : kPer); ++c) {
-        uint32_t r[32];
-        float f[32];
+      for (int c = col0; c < col0 + kOut; c += 16) {
+        uint32_t r[16];
+        float f[16];
         if (mine_n > 0) {
-          tmem_ld_32x32(t_o + c * 32, r);
+          tmem_ld_32x16(t_o + c, r);
           tmem_ld_wait(r);
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = f0 == 0.f ? 0.f : __uint_as_float(r[i]) * f0;
+        for (int i = 0; i < 16; ++i) f[i] = f0 == 0.f ? 0.f : __uint_as_float(r[i]) * f0 * e0;
         if (DUAL && (g == 0 ? w.blocks > 1 : w.blocks > 0)) {          // the other group has some
-          tmem_ld_32x32(t_o + (g == 0 ? 128 : -128) + c * 32, r);
+          tmem_ld_32x16(t_o + (g == 0 ? 128 : -128) + c, r);
           tmem_ld_wait(r);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] += f1 == 0.f ? 0.f : __uint_as_float(r[i]) * f1;
+          for (int i = 0; i < 16; ++i) f[i] += f1 == 0.f ? 0.f : __uint_as_float(r[i]) * f1 * e1;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {          // values' columns have the even ones of four in front
+          const float odd = f[i + 2];
+          f[i + 2] = f[i + 1];
+          f[i + 1] = odd;
         }
         if (mine) {
           if (w.part < 0) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) =
+            for (int q = 0; q < 2; ++q)
+              *reinterpret_cast<uint4*>(dst + c + q * 8) =
                   make_uint4(pack_bf16x2(f[q * 8], f[q * 8 + 1]), pack_bf16x2(f[q * 8 + 2], f[q * 8 + 3]), pack_bf16x2(f[q * 8 + 4], f[q * 8 + 5]),
                              pack_bf16x2(f[q * 8 + 6], f[q * 8 + 7]));
           } else {
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<float4*>(p.part_o + part * D + c * 32 + q * 4) = make_float4(f[q * 4], f[q * 4 + 1], f[q * 4 + 2], f[q * 4 + 3]);
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<float4*>(p.part_o + part * D + c + q * 4) = make_float4(f[q * 4], f[q * 4 + 1], f[q * 4 + 2], f[q * 4 + 3]);
           }
         }
       }
-      if (w.part >= 0 && mine && (!DUAL || g == 0)) *reinterpret_cast<float2*>(p.part_s + part * 2) = make_float2(m_run, l);
+      if (w.part >= 0 && mine && (!DUAL || g == 0)) *reinterpret_cast<float2*>(p.part_s + part * 2) = make_float2(m_ref, l);
       tc_fence_before();
-      if (DUAL && !(ok = meet())) break;          // the next item's products write over both groups' O
+      if (DUAL && !(ok = meet_other())) break;          // the next item's products write over both groups' O
     }
   }
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();                // nobody's memory is still a target of the partner
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem_base, 512);
+    else
+      tmem_dealloc(tmem_base, 512);
   }
 }
 
@@ -593,18 +763,19 @@ __global__ void __launch_bounds__(128) kv8_chunk_join_kernel(const Kv8Chunk p, c
   for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
 }
 
-template <int D, bool DUAL>
-static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, int grid, const Kv8ChunkJoin* joins, int n_joins, cudaStream_t s) {
+template <int D, int FORM>
+static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, int workers, const Kv8ChunkJoin* joins, int n_joins, cudaStream_t s) {
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(kv8_chunk_kernel<D, DUAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8ChunkCfg<D, DUAL>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kv8_chunk_kernel<D, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8ChunkCfg<D, FORM>::kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev & 63] = true;
   }
-    kv8_chunk_kernel<D, DUAL><<<grid, kKcThreads, Kv8ChunkCfg<D, DUAL>::kSmem, s>>>(tq, p);
-  cudaError_t e = cudaGetLastError();
+  constexpr int kCtas = FORM == kPair ? 2 : 1;
+  using Cfg = Kv8ChunkCfg<D, FORM>;
+  cudaError_t e = launch_kernel_clusters(kv8_chunk_kernel<D, FORM>, dim3(workers * kCtas), dim3(Cfg::kThreads), Cfg::kSmem, kCtas, s, tq, p);
   if (e != cudaSuccess || n_joins == 0) return static_cast<int>(e);
   kv8_chunk_join_kernel<D><<<dim3(n_joins, (p.hp * p.tp + 3) / 4), 128, 0, s>>>(p, joins);
   return static_cast<int>(cudaGetLastError());
@@ -615,12 +786,13 @@ static int launch_kv8_chunk(const CUtensorMap& tq, const Kv8Chunk& p, int grid, 
 extern "C" {
 using namespace apb;
 
-// q [T, Hq, D], out [T, Hq, D] (rows on 16-byte boundaries); one_tile: no item has two tiles; items [..][12], first [ctas + 1], joins [n_joins][8] as apb_rt_kv8_plan makes
-// them; scratch: part_tiles * 128 * (D + 2) floats.
+// q [T, Hq, D], out [T, Hq, D] (rows on 16-byte boundaries); items [..][12], first [workers + 1], joins [n_joins][8] and the form of the
+// workers (CTAs or pairs) as apb_rt_kv8_plan makes them; scratch: part_tiles * 128 * (D + 2) floats.
 int apb_kv8_chunk(const void* q, long long ldq, const void* data, const int* table, long long ld_table, const int* items, const int* first,
-                  int ctas, const int* joins, int n_joins, int part_tiles, int one_tile, void* scratch, void* out, long long ldo, int T, int Hq, int Hkv, int D,
-                  float scale, cudaStream_t s) {
-  if (ctas <= 0) return 0;
+                  int workers, const int* joins, int n_joins, int part_tiles, int form, void* scratch, void* out, long long ldo, int T,
+                  int Hq, int Hkv, int D, float scale, cudaStream_t s) {
+  if (workers <= 0) return 0;
+  if (form < kTwo || form > kPair || (form == kPair && D != 128)) return kBadArgument;
   if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || ldq % 8 || ldo % 8 || reinterpret_cast<uintptr_t>(q) % 16 ||
       reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(data) % 16 || reinterpret_cast<uintptr_t>(items) % 16)
     return kBadArgument;
@@ -636,7 +808,10 @@ int apb_kv8_chunk(const void* q, long long ldq, const void* data, const int* tab
                 static_cast<__nv_bfloat16*>(out), ldo, part_o, part_o + static_cast<long long>(part_tiles) * 128 * D, Hkv, hp, tp,
                 fabsf(scale) * 1.4426950408889634f, scale < 0.f ? 0x80008000u : 0u, status_device_ptr()};
   const Kv8ChunkJoin* j = reinterpret_cast<const Kv8ChunkJoin*>(joins);
-  if (one_tile) return D == 128 ? launch_kv8_chunk<128, true>(tq, p, ctas, j, n_joins, s) : launch_kv8_chunk<64, true>(tq, p, ctas, j, n_joins, s);
-  return D == 128 ? launch_kv8_chunk<128, false>(tq, p, ctas, j, n_joins, s) : launch_kv8_chunk<64, false>(tq, p, ctas, j, n_joins, s);
+  if (D == 64 && form == kDual) return launch_kv8_chunk<64, kDual>(tq, p, workers, j, n_joins, s);
+  if (D == 64) return launch_kv8_chunk<64, kTwo>(tq, p, workers, j, n_joins, s);
+  if (form == kPair) return launch_kv8_chunk<128, kPair>(tq, p, workers, j, n_joins, s);
+  if (form == kDual) return launch_kv8_chunk<128, kDual>(tq, p, workers, j, n_joins, s);
+  return launch_kv8_chunk<128, kTwo>(tq, p, workers, j, n_joins, s);
 }
 }

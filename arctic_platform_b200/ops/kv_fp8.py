@@ -312,27 +312,31 @@ class _Work:
     first: np.ndarray
     joins: np.ndarray
     part_tiles: int           # tiles of 128 rows of scratch
-    ctas: int
-    one_tile: bool            # no item has a second tile
+    ctas: int                 # or pairs of them
+    form: int                 # how items are taken: one or two tiles, one, one or two of 256 rows by two CTAs
+
+    @property
+    def one_tile(self) -> bool:
+        return self.form == 1
 
 
-def _work(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: int) -> _Work:
+def _work(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: int, head_dim: int = 64, form: int = -1) -> _Work:
     fn = _lib.rt_lib().apb_rt_kv8_plan
     c = ctypes
-    fn.argtypes, fn.restype = [c.c_void_p, c.c_void_p, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_void_p, c.c_int64, c.c_void_p,
+    fn.argtypes, fn.restype = [c.c_void_p, c.c_void_p, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_int32, c.c_void_p, c.c_int64, c.c_void_p,
                                c.c_void_p, c.c_int64, c.c_void_p], c.c_int32
     new, lengths = np.ascontiguousarray(new, dtype=np.int32), np.ascontiguousarray(lengths, dtype=np.int32)
     counts, first = np.zeros(5, dtype=np.int64), np.zeros(sms + 1, dtype=np.int32)
-    # as many items as tiles hold tokens, and a few more that a border cuts: the first call says how many it is
+    # the first call says how many there are
     items, joins = np.empty((0, 12), dtype=np.int32), np.empty((0, 8), dtype=np.int32)
     for _ in range(2):
-        if fn(new.ctypes.data, lengths.ctypes.data, len(new), heads, kv_heads, sms, items.ctypes.data, len(items), first.ctypes.data,
+        if fn(new.ctypes.data, lengths.ctypes.data, len(new), heads, kv_heads, head_dim, sms, form, items.ctypes.data, len(items), first.ctypes.data,
               joins.ctypes.data, len(joins), counts.ctypes.data) != 0:
             raise ValueError("chunk plan: sizes out of range")
         if len(items) >= counts[0] and len(joins) >= counts[1]:
             break
         items, joins = np.empty((int(counts[0]), 12), dtype=np.int32), np.empty((int(counts[1]), 8), dtype=np.int32)
-    return _Work(items, first[:int(counts[3]) + 1], joins, int(counts[2]), int(counts[3]), bool(counts[4]))
+    return _Work(items, first[:int(counts[3]) + 1], joins, int(counts[2]), int(counts[3]), int(counts[4]))
 
 
 @dataclass
@@ -379,7 +383,7 @@ class ChunkPlan:
         plan = ChunkPlan(rows, new, lengths, used, heads, cache.num_kv_heads, cache.num_pages, cache.head_dim)
         if cache.index >= 0 and rows:
             sms = torch.cuda.get_device_properties(cache.data.device).multi_processor_count
-            plan.work = w = _work(new, lengths, heads, cache.num_kv_heads, sms)
+            plan.work = w = _work(new, lengths, heads, cache.num_kv_heads, sms, cache.head_dim)
             table = np.zeros((n, max(1, int(need.max()))), dtype=np.int32)
             for s in range(n):
                 table[s, :need[s]] = used[s]
@@ -428,6 +432,6 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
     w = plan.work
     scratch = torch.empty(w.part_tiles * 128 * (D + 2), device=data.device, dtype=torch.float32).data_ptr() if w.part_tiles else None
     _lib.check(_fn("chunk")(q.data_ptr(), ldq, data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
-                            plan.first.data_ptr(), w.ctas, plan.joins.data_ptr(), len(w.joins), w.part_tiles, w.one_tile, scratch,
+                            plan.first.data_ptr(), w.ctas, plan.joins.data_ptr(), len(w.joins), w.part_tiles, w.form, scratch,
                             out.data_ptr(), out.stride(0), T, Hq, cache.num_kv_heads, D, scale, _lib.stream_ptr()), "kv8_chunk")
     return out

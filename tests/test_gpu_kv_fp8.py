@@ -321,6 +321,67 @@ def test_padding_rows_of_a_chunk_are_left():
     assert torch.equal(wide[:37, 8:16], out[:37]) and (wide[:, :8] == 3).all() and (wide[37:] == 3).all()
 
 
+def _plan(monkeypatch, form, new, lengths, table, Hq, cache):
+    """With items taken in this form (csrc/runtime_kv8.cpp), whichever is sooner done."""
+    work, number = kv_fp8._work, {"ctas": 0, "one tile": 1, "pairs": 2}[form]
+    monkeypatch.setattr(kv_fp8, "_work", lambda *a: work(*a, form=number))
+    plan = kv_fp8.ChunkPlan.build(new, lengths, table.cpu().numpy(), Hq, cache)
+    assert plan.work.form == number
+    return plan
+
+
+@pytest.mark.parametrize("form", ["ctas", "pairs"])
+@pytest.mark.parametrize("new,lengths,Hq,H", [([512], [5000], 32, 8), ([700, 1, 33], [700, 9000, 40], 16, 8), ([1300] * 3, [1300, 1290, 2000], 5, 1),
+                                              ([150, 20], [150, 3000], 130, 1), ([65] * 90, [65 + 17 * i for i in range(90)], 64, 4)])
+def test_long_chunks_by_ctas_and_by_pairs(monkeypatch, form, new, lengths, Hq, H):
+    """Rows that see nothing (a length below the new tokens), tiles that no token fills, more heads than a tile has rows."""
+    cache, table, n, _ = _filled(lengths, H, 128, seed=4)
+    q = torch.randn((sum(new), Hq, 128), device="cuda", generator=_gen(5)).bfloat16()
+    plan = _plan(monkeypatch, form, new, lengths, table, Hq, cache)
+    _close(kv_fp8.chunk_attention(q, cache, plan), *_want(q, cache, table, n, new), BF16)
+    _lib.check_status("chunk")
+
+
+@pytest.mark.parametrize("form,new,D", [("one tile", 9, 64), ("one tile", 9, 128), ("ctas", 500, 64), ("ctas", 1500, 128), ("pairs", 1500, 128)])
+def test_scores_that_grow_by_leaps(monkeypatch, form, new, D):
+    """What a chunk's weights are relative to moves only when they pass 2^40: here the scores leap along the sequence, by little and by a
+    lot, at the borders of blocks, inside of them and from one half of a block to the next, up and down again, and by head."""
+    length, H, R = 2100, 2, 4
+    g = _gen(6)
+    base = torch.randn((H, D), device="cuda", generator=g)
+    base /= base.square().sum(-1, keepdim=True).sqrt()
+    height = torch.zeros(length, device="cuda")
+    for at, to in ((0, 1.0), (40, 20.0), (100, 45.0), (128, 60.0), (200, 130.0), (256, 125.0), (320, 250.0), (600, 0.0), (1024, 290.0), (1100, -300.0),
+                   (1536, 400.0), (2064, 560.0)):
+        height[at:] = to
+    k = base * height[:, None, None] + 0.3 * torch.randn((length, H, D), device="cuda", generator=g)
+    v = torch.randn((length, H, D), device="cuda", generator=g) * torch.exp(torch.randn((length, H, 1), device="cuda", generator=g))
+    cache = kv_fp8.Fp8KVCache.zeros((length + 15) // 16, H, D)
+    table = torch.randperm(cache.num_pages, device="cuda", generator=g).to(torch.int32)[None]
+    t = torch.arange(length, device="cuda")
+    kv_fp8.write(k, v, (table[0].long()[t // 16] * 16 + t % 16).to(torch.int32), cache)
+    q = (base.repeat_interleave(R, 0) * torch.linspace(-0.5, 1.0, H * R, device="cuda")[:, None] * D ** 0.5 * 0.7
+         + 0.2 * torch.randn((new, H * R, D), device="cuda", generator=g)).bfloat16()
+    n = torch.tensor([length], device="cuda", dtype=torch.int32)
+    plan = _plan(monkeypatch, form, [new], [length], table, H * R, cache)
+    want, size = _want(q, cache, table, n, [new])
+    # scores of up to 400: eight sums in fp32 that a product of 16 terms each is added to, off by 2^-23 of it at most, leave weights off by
+    # 8 * 2^-23 * 400 = 2^-11.3 more, and their sum likewise; (2^-8 + 2^-12) * 0.25 is above 2 * 2^-11.3 + 2^-14
+    _close(kv_fp8.chunk_attention(q, cache, plan), want, size * 1.25, BF16)
+    _lib.check_status("chunk")
+
+
+@pytest.mark.parametrize("Hq,H,D,new", [(130, 1, 64, 2), (200, 1, 128, 3), (256, 2, 128, 1), (384, 1, 64, 40)])
+def test_more_heads_than_a_tile_has_rows(Hq, H, D, new):
+    lengths = [700, 33]
+    cache, table, n, _ = _filled(lengths, H, D, seed=7)
+    q = torch.randn((2 * new, Hq, D), device="cuda", generator=_gen(8)).bfloat16()
+    plan = kv_fp8.ChunkPlan.build([new] * 2, lengths, table.cpu().numpy(), Hq, cache)
+    _close(kv_fp8.chunk_attention(q, cache, plan), *_want(q, cache, table, n, [new] * 2), BF16)
+    q = q[:2]
+    _close(kv_fp8.decode_attention(q, cache, table, n), *_want(q, cache, table, n))
+
+
 # --------------------------------------------------------------------------------------------- together
 def test_a_sequence_step_by_step():
     """A prompt in chunks, then token after token: written, attended to, read back."""

@@ -55,3 +55,38 @@ def test_shares_of_a_long_conversation_are_even():
     w = _work(np.array([512]), np.array([16896]), 32, 8, 148)
     load = [w.items[a:b, 9].sum() for a, b in zip(w.first, w.first[1:])]
     assert len(load) == 148 and max(load) <= 1.2 * sum(load) / 148
+
+
+@pytest.mark.parametrize("sms", [2, 5, 148])
+def test_pairs_see_every_block_once(sms):
+    """Pairs of CTAs take tiles of twice the tokens; the joins leave out tiles that no token fills."""
+    seen = 0
+    for new, lengths, Hq, H in [*CASES, *_random()]:
+        hp = min(Hq // H, 128)
+        tp = 128 // hp
+        assert (_work(np.array(new), np.array(lengths), Hq, H, sms, 128).form == 1) == all(m <= tp for m in new)
+        if all(m <= tp for m in new):
+            continue
+        w = _work(np.array(new), np.array(lengths), Hq, H, sms, 128, form=2)
+        assert w.form == 2
+        seen += 1
+        assert w.ctas <= sms // 2 and len(w.first) == w.ctas + 1 and w.first[-1] == len(w.items) and (np.diff(w.first) >= 0).all()
+        ranges, scratch, filled = {}, set(), set()
+        for row0, tokens, s, kvh, head0, heads, pos0, length, b0, blocks, part, _ in w.items.tolist():
+            assert 0 < tokens <= 4 * tp
+            ranges.setdefault((row0, tokens, head0, heads), []).append((b0, blocks, part, max(0, min(length, pos0 + tokens))))
+            for g in range(4 if tokens > 2 * tp else 2) if part >= 0 else ():
+                assert part + g < w.part_tiles and part + g not in scratch
+                scratch.add(part + g)
+                if g * tp < tokens:
+                    filled.add(part + g)
+        assert sum(tokens * heads for _, tokens, _, heads in ranges) == sum(new) * Hq
+        for pieces in ranges.values():
+            at = 0
+            for b0, blocks, part, _ in sorted(pieces):
+                assert b0 == at and (part >= 0) == (len(pieces) > 1)
+                at += blocks
+            assert at == -(-pieces[0][3] // 128)
+        joined = [part + k * step for _, _, _, _, part, parts, step, _ in w.joins.tolist() for k in range(parts)]
+        assert sorted(joined) == sorted(filled) and len(scratch) == w.part_tiles
+    assert seen > 3
