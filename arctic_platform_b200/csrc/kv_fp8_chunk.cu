@@ -18,7 +18,7 @@
 // TFLOP/s; 16 prompts' 397 to 324 (one CTA per item with this softmax: 168 and 355).  S in halves of 64 columns with buffers of their
 // own, so that the tensor core need not wait for the softmax, was slower (158: an MMA of 64 columns takes 0.7 of one of 128).
 // Short chunks (5 draft tokens: 27 us where the bytes take 4.8) have one tile of 20 rows, for which all codes are turned into tiles: two
-// warpgroups do that there (one: 31).
+// warpgroups do that there (one: 31).  Of up to 16 rows most go the way of decode attention instead (apb_kv8_few).
 //
 // Items over long contexts are cut along the keys where there are too few to fill the GPU (csrc/runtime_kv8.cpp); their parts are
 // joined by kv8_chunk_join_kernel.
@@ -536,6 +536,9 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
         continue;
       }
       const int seen = min(w.len, w.pos0 + row_token + 1) - w.block0 * kKcBlock;      // tokens of the range that the row sees (or more)
+      auto asked_for = [&]() { return row < p.hp * p.tp && row_token < w.tokens && row_head < w.heads; };
+      // rows that nobody asked for: whatever their weights are, nothing is stored (of two tiles few are such, and the test costs them 2%)
+      const bool idle = DUAL && !__any_sync(0xffffffffu, asked_for());
       float m_ref = -INFINITY;             // what weights are relative to: a score of the row not far below its largest
       uint64_t l2 = 0;
       int ev = 0;
@@ -546,6 +549,12 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
         if (h == 0) ok = wait(&s_full[g], parts_seen / kHalves & 1, kTimeoutTmemFull);
         if (!ok) break;
         ++parts_seen;
+        if (idle) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_issuer(&p_full[g * 2 + h]);
+          continue;
+        }
         const int2 ref = meta[(blocks_all + j) % kKcMeta];
         const float c1 = fmaxf(p.scale_log2 * exp2_int(ref.x), 1.2e-38f);
         const uint64_t c2 = xtc_pair(c1, c1);
@@ -668,11 +677,11 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
         f1 = a1 == 0.f ? 0.f : a1 / l;
         e1 = exp2_int(other_ev[(1 - g) * 4 + quarter]);
       }
-      const bool mine = row < p.hp * p.tp && row_token < w.tokens && row_head < w.heads;
+      const bool mine = asked_for();
       __nv_bfloat16* dst = p.out + (static_cast<long long>(w.row0) + row_token) * p.ldo + (w.head0 + row_head) * D;
       const long long part = (static_cast<long long>(w.part) + (DUAL ? 0 : g * kCtas + static_cast<int>(cta))) * 128 + row;
 #pragma unroll 1
-      for (int c = col0; c < col0 + kOut; c += 16) {
+      for (int c = col0; c < (idle ? col0 : col0 + kOut); c += 16) {
         uint32_t r[16];
         float f[16];
         if (mine_n > 0) {

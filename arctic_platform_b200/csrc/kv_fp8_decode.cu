@@ -1,4 +1,4 @@
-// Decode attention (one query token per sequence) over the 8-bit cache (layout: kv_fp8.cuh).
+// Decode attention (one query token per sequence, or few of them: apb_kv8_few) over the 8-bit cache (layout: kv_fp8.cuh).
 //
 // Bound by the stream of codes: a page of 16 tokens and one key head is 32 D + 32 bytes that up to 16 query heads share.  A warp walks
 // pages by itself, two at a time: a TMA copy brings a page's keys and values into its ring of shared memory (swizzled, so that the
@@ -34,10 +34,11 @@ struct Kv8Decode {
   __nv_bfloat16* out;
   long long ldo;
   int B, Hq, Hkv;
-  int groups;                // of 8 H query heads per key head
+  int groups;                // of 8 H query heads (ROWS: heads of some tokens) per key head
   int splits;                // parts of a sequence: CTAs of a cluster
   float scale_log2;
   int* status;
+  const int* starts;         // ROWS [B + 1]: where the query tokens of a sequence begin in q and out
 };
 
 constexpr float kKv8Top = 14.f;          // log2 of the largest weight and (about) of the largest query element
@@ -71,7 +72,8 @@ struct Kv8DecodeCfg {
 
 // What a warp has of its heads: a lane has heads 2 (lane % 4) and the next of every group of 8, of them the dimensions
 // D/8 (lane / 4) + [0, D/8) and the softmax sums of tokens lane / 4 and lane / 4 + 8 of its pages.
-template <int D, int H>
+// ROWS: heads of several tokens, which differ in how many of the sequence's last tokens they do not see.
+template <int D, int H, bool ROWS = false>
 struct Kv8Heads {
   static constexpr int KS = D / 16;       // k steps of the first product, tiles of 16 dimensions of the second
   uint32_t qb[H][KS][2];
@@ -79,8 +81,11 @@ struct Kv8Heads {
   float o[H][KS][4];
   float top[H][2];                        // M
   float m[H][2], l[H][2];
+  int unseen[ROWS ? H : 1][2];
 
-  __device__ __forceinline__ void start(const __nv_bfloat16* q, int heads, float scale_log2, int lane) {
+  // q_of(head): where its query is
+  template <typename Q>
+  __device__ __forceinline__ void start(Q q_of, int heads, float scale_log2, int lane) {
     const int g = lane >> 2, c4 = lane & 3;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
@@ -89,7 +94,7 @@ struct Kv8Heads {
 #pragma unroll
       for (int i = 0; i < KS / 2; ++i) {
         uint4 r = make_uint4(0, 0, 0, 0);
-        if (head < heads) r = *reinterpret_cast<const uint4*>(q + head * D + c4 * (D / 4) + i * 8);
+        if (head < heads) r = *reinterpret_cast<const uint4*>(q_of(head) + c4 * (D / 4) + i * 8);
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -170,7 +175,8 @@ struct Kv8Heads {
       for (int e = 0; e < 2; ++e) {
         float x[4], sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = in[t] ? s[t >> 1][h][2 * (t & 1) + e] * (f[t] * c[h][e]) : -INFINITY;
+        for (int t = 0; t < 4; ++t)
+          x[t] = in[t] && (!ROWS || g + 8 * t < left - unseen[h][e]) ? s[t >> 1][h][2 * (t & 1) + e] * (f[t] * c[h][e]) : -INFINITY;
         const float m_new = fmaxf(fmaxf(m[h][e], fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
 #pragma unroll
         for (int t = 0; t < 4; ++t) sum += ex2(x[t] - m_new);
@@ -304,7 +310,7 @@ struct Kv8Copies {
   }
 };
 
-template <int D, int H, int WARPS>
+template <int D, int H, int WARPS, bool ROWS>
 __global__ void __launch_bounds__(32 * WARPS)
 kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
   using Cfg = Kv8DecodeCfg<D, H, WARPS>;
@@ -314,7 +320,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
   const int group = unit % p.groups, kvh = unit / p.groups % p.Hkv, b = unit / p.groups / p.Hkv;
-  const int R = p.Hq / p.Hkv, head0 = kvh * R + group * Cfg::kHeads, heads = min(Cfg::kHeads, R - group * Cfg::kHeads);
+  const int R = p.Hq / p.Hkv;
   uint64_t* full = bars + warp * kKv8Stages;
   if (lane == 0) {
     for (int s = 0; s < kKv8Stages; ++s) mbar_init(&full[s], 1);
@@ -324,6 +330,15 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
   __syncwarp();
   pdl_entry();
 
+  const int token0 = ROWS ? p.starts[b] : b, tokens = ROWS ? p.starts[b + 1] - token0 : 1;
+  const int heads = min(Cfg::kHeads, tokens * R - group * Cfg::kHeads);
+  if (heads <= 0) return;
+  // of a head of the group: its token of the sequence's, its place among the key head's
+  auto token_of = [&](int head) { return ROWS ? (group * Cfg::kHeads + head) / R : 0; };
+  auto row_of = [&](int head, long long ld) {
+    const int t = token_of(head);
+    return (token0 + t) * ld + (kvh * R + group * Cfg::kHeads + head - t * R) * D;
+  };
   int len = p.lengths[b];
   if (len > p.max_pages * kKv8Page) {
     if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kBadTable);
@@ -344,9 +359,15 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
     const int id0 = __shfl_sync(0xffffffffu, ids, 2 * (j & 15)), id1 = __shfl_sync(0xffffffffu, ids, 2 * (j & 15) + 1);
     if (j < n) copies.ask(j, id0, id1, 2 * (first + j * WARPS) + 1 < n_pages, kvh, next);
   };
-  Kv8Heads<D, H> acc;
+  Kv8Heads<D, H, ROWS> acc;
   issue(0);
-  acc.start(p.q + b * p.ldq + head0 * D, heads, p.scale_log2, lane);
+  acc.start([&](int head) { return p.q + row_of(head, p.ldq); }, heads, p.scale_log2, lane);
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) acc.unseen[h][e] = tokens - 1 - token_of(min(8 * h + 2 * (lane & 3) + e, heads - 1));
+  }
   bool ok = true;
 #pragma unroll 1
   for (int j = 0; j < n; ++j) {
@@ -397,7 +418,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
     }
   };
   auto finished = [&](int head, int d, float top, float m, float l, float o) {
-    p.out[b * p.ldo + (head0 + head) * D + d] = __float2bfloat16(Kv8Final(top, m, l)(o));
+    p.out[row_of(head, p.ldo) + d] = __float2bfloat16(Kv8Final(top, m, l)(o));
   };
   for (int i = threadIdx.x; i < heads * D; i += 32 * WARPS) {
     const int head = i / D, d = i % D;
@@ -600,7 +621,7 @@ kv8_decode_stream_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decod
   while (c.left > 0) {
     const int n = c.pages(), pairs = (n + 1) / 2, len = tokens_of(c.b);
     const int group = c.u % p.groups, head0 = c.u / p.groups * R + group * kHeads, heads = min(kHeads, R - group * kHeads);
-    acc.start(p.q + c.b * p.ldq + head0 * D, heads, p.scale_log2, lane);
+    acc.start([&](int head) { return p.q + c.b * p.ldq + (head0 + head) * D; }, heads, p.scale_log2, lane);
 #pragma unroll 1
     for (int k = warp; k < pairs && ok; k += kKv8Warps, ++copy) {
       const uint32_t ex[2] = {next[0], next[1]};
@@ -714,18 +735,18 @@ static int kv8_map(CUtensorMap* map, const void* data, int D, long long blocks) 
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE));
 }
 
-template <int D, int H, int WARPS>
+template <int D, int H, int WARPS, bool ROWS = false>
 static int launch_kv8_decode(const CUtensorMap& map, const Kv8Decode& p, cudaStream_t s) {
   constexpr int smem = Kv8DecodeCfg<D, H, WARPS>::kSmem;
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(kv8_decode_kernel<D, H, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(kv8_decode_kernel<D, H, WARPS, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev & 63] = true;
   }
-  return static_cast<int>(launch_kernel_clusters(kv8_decode_kernel<D, H, WARPS>, dim3(p.B * p.Hkv * p.groups * p.splits), dim3(32 * WARPS), smem,
+  return static_cast<int>(launch_kernel_clusters(kv8_decode_kernel<D, H, WARPS, ROWS>, dim3(p.B * p.Hkv * p.groups * p.splits), dim3(32 * WARPS), smem,
                                                  p.splits, s, map, p));
 }
 
@@ -792,7 +813,7 @@ int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* ta
   const int rc = kv8_map(&map, data, D, static_cast<long long>(pages) * Hkv);
   if (rc) return 1000 + rc;
   Kv8Decode p = {static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const uint8_t*>(data), table, ld_table, max_pages, pages, lengths,
-                 static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, groups, 1, scale * 1.4426950408889634f, status_device_ptr()};
+                 static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, groups, 1, scale * 1.4426950408889634f, status_device_ptr(), nullptr};
   if (scratch) {
     if (units * max_pages >= (1ll << 30)) return kBadArgument;
     const long long rows = static_cast<long long>(kv8_stream_ctas(H)) * 2 * 8 * H;
@@ -809,5 +830,27 @@ int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* ta
   if (units * p.splits >= (1ll << 31)) return kBadArgument;
   if (D == 128) return H == 1 ? launch_kv8_decode<128, 1, 4>(map, p, s) : launch_kv8_decode<128, 2, 4>(map, p, s);
   return H == 1 ? launch_kv8_decode<64, 1, 4>(map, p, s) : launch_kv8_decode<64, 2, 4>(map, p, s);
+}
+
+// Attention of few query tokens of each sequence, causal, 16 of them times the query heads of a key head at most: sequence b has those from
+// starts[b] to starts[b + 1], at the end of its lengths[b] tokens, `most` at most; q, out [rows, Hq, D].  A unit's rows are then heads of
+// several tokens.  (A third group of 8 rows was slower than 128-row tiles: 20 rows, 16 x 1500 tokens 33 us against 27.)
+int apb_kv8_few(const void* q, long long ldq, const void* data, const int* table, long long ld_table, int max_pages, int pages, const int* lengths,
+                const int* starts, void* out, long long ldo, int B, int most, int longest, int Hq, int Hkv, int D, float scale, cudaStream_t s) {
+  if (B <= 0 || most <= 0) return 0;
+  if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || pages < 1 || max_pages < 0 || static_cast<long long>(pages) * Hkv >= (1ll << 31) - 1 ||
+      ldq % 8 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(data) % 16)
+    return kBadArgument;
+  const long long rows = static_cast<long long>(most) * (Hq / Hkv), units = static_cast<long long>(B) * Hkv;
+  if (rows > 16) return kBadArgument;
+  CUtensorMap map;
+  const int rc = kv8_map(&map, data, D, static_cast<long long>(pages) * Hkv);
+  if (rc) return 1000 + rc;
+  Kv8Decode p = {static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const uint8_t*>(data), table, ld_table, max_pages, pages, lengths,
+                 static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, 1, kv8_splits(units, longest),
+                 scale * 1.4426950408889634f, status_device_ptr(), starts};
+  if (units * p.splits >= (1ll << 31)) return kBadArgument;
+  if (D == 128) return rows <= 8 ? launch_kv8_decode<128, 1, 4, true>(map, p, s) : launch_kv8_decode<128, 2, 4, true>(map, p, s);
+  return rows <= 8 ? launch_kv8_decode<64, 1, 4, true>(map, p, s) : launch_kv8_decode<64, 2, 4, true>(map, p, s);
 }
 }

@@ -42,6 +42,7 @@ def _fn(name: str):
         _FN["qkv"] = _lib.declare("apb_kv8_qkv_post", [vp, ll] + [vp] * 8 + [i, i, i, i, i, f, vp])
         _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, i, f, vp, vp])
         _FN["scratch"] = _lib.declare("apb_kv8_decode_scratch", [i, i, i, i, i], ll)
+        _FN["few"] = _lib.declare("apb_kv8_few", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, ll, i, i, i, i, i, i, f, vp])
         _FN["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, vp, i, vp, i, i, i, vp, vp, ll, i, i, i, i, f, vp])
     return _FN[name]
 
@@ -339,6 +340,14 @@ def _work(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: 
     return _Work(items, first[:int(counts[3]) + 1], joins, int(counts[2]), int(counts[3]), int(counts[4]))
 
 
+def _few(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: int) -> bool:
+    """Whether the tokens are so few that they go the way of decode attention."""
+    fn = _lib.rt_lib().apb_rt_kv8_few
+    fn.argtypes, fn.restype = [ctypes.c_void_p] * 2 + [ctypes.c_int32] * 4, ctypes.c_int32
+    new, lengths = np.ascontiguousarray(new, dtype=np.int32), np.ascontiguousarray(lengths, dtype=np.int32)
+    return bool(fn(new.ctypes.data, lengths.ctypes.data, len(new), heads, kv_heads, sms))
+
+
 @dataclass
 class ChunkPlan:
     """Tables of a step in which every sequence brings some tokens; made on the host once and used by all layers.
@@ -353,11 +362,12 @@ class ChunkPlan:
     kv_heads: int
     num_pages: int
     head_dim: int
-    work: Optional[_Work] = None
+    work: Optional[_Work] = None                     # None: few tokens of each sequence, the way of decode attention
     table: Optional[torch.Tensor] = None             # on the cache's device: pages, and the work's tables
     items: Optional[torch.Tensor] = None
     first: Optional[torch.Tensor] = None
     joins: Optional[torch.Tensor] = None
+    tokens: Optional[torch.Tensor] = None            # lengths [n], where the sequences' rows begin [n + 1]
 
     @staticmethod
     def build(new: Sequence[int], lengths: Sequence[int], pages, heads: int, cache: Fp8KVCache) -> "ChunkPlan":
@@ -383,14 +393,20 @@ class ChunkPlan:
         plan = ChunkPlan(rows, new, lengths, used, heads, cache.num_kv_heads, cache.num_pages, cache.head_dim)
         if cache.index >= 0 and rows:
             sms = torch.cuda.get_device_properties(cache.data.device).multi_processor_count
-            plan.work = w = _work(new, lengths, heads, cache.num_kv_heads, sms, cache.head_dim)
+            sizes = (new, lengths, heads, cache.num_kv_heads, sms)
+            if not _few(*sizes):
+                plan.work = w = _work(*sizes, cache.head_dim)
             table = np.zeros((n, max(1, int(need.max()))), dtype=np.int32)
             for s in range(n):
                 table[s, :need[s]] = used[s]
-            parts = (w.items, w.joins, w.first, table)
+            tokens = np.concatenate([lengths, [0], np.cumsum(new)]).astype(np.int32)
+            parts = (table, tokens) if plan.work is None else (w.items, w.joins, w.first, table)
             flat = torch.from_numpy(np.concatenate([a.reshape(-1) for a in parts])).pin_memory()
-            dev = to_device(flat, cache.data.device).split([a.size for a in parts])
-            plan.items, plan.joins, plan.first, plan.table = (t.view(a.shape) for t, a in zip(dev, parts))
+            dev = [t.view(a.shape) for t, a in zip(to_device(flat, cache.data.device).split([a.size for a in parts]), parts)]
+            if plan.work is None:
+                plan.table, plan.tokens = dev
+            else:
+                plan.items, plan.joins, plan.first, plan.table = dev
         return plan
 
 
@@ -421,7 +437,7 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
             out[row:row + m] = attention_ref(q[row:row + m].float(), k, v, torch.arange(n - m, n), scale).to(q.dtype)
             row += m
         return out
-    if plan.items is None or plan.items.get_device() != cache.index:
+    if plan.table is None or plan.table.get_device() != cache.index:
         raise ValueError(f"the plan was not made for a cache on {data.device}")
     if out.stride(0) % 8 or out.data_ptr() % 16:             # rows off the 16-byte boundaries: by way of a copy
         out[:plan.rows].copy_(chunk_attention(q, cache, plan, scale)[:plan.rows])
@@ -430,6 +446,13 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
         with torch.cuda.device(cache.index):
             return chunk_attention(q, cache, plan, scale, out)
     w = plan.work
+    if w is None:
+        n = len(plan.new)
+        _lib.check(_fn("few")(q.data_ptr(), ldq, data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.table.shape[1],
+                              cache.num_pages, plan.tokens.data_ptr(), plan.tokens[n:].data_ptr(), out.data_ptr(), out.stride(0), n,
+                              int(plan.new.max()), int((plan.lengths.max() + PAGE - 1) // PAGE), Hq, cache.num_kv_heads, D, scale,
+                              _lib.stream_ptr()), "kv8_few")
+        return out
     scratch = torch.empty(w.part_tiles * 128 * (D + 2), device=data.device, dtype=torch.float32).data_ptr() if w.part_tiles else None
     _lib.check(_fn("chunk")(q.data_ptr(), ldq, data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
                             plan.first.data_ptr(), w.ctas, plan.joins.data_ptr(), len(w.joins), w.part_tiles, w.form, scratch,

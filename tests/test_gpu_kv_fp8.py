@@ -322,11 +322,12 @@ def test_padding_rows_of_a_chunk_are_left():
 
 
 def _plan(monkeypatch, form, new, lengths, table, Hq, cache):
-    """With items taken in this form (csrc/runtime_kv8.cpp), whichever is sooner done."""
-    work, number = kv_fp8._work, {"ctas": 0, "one tile": 1, "pairs": 2}[form]
+    """With items taken in this form (csrc/runtime_kv8.cpp), whichever is sooner done; "few": without items."""
+    work, number = kv_fp8._work, {"ctas": 0, "one tile": 1, "pairs": 2, "few": None}[form]
     monkeypatch.setattr(kv_fp8, "_work", lambda *a: work(*a, form=number))
+    monkeypatch.setattr(kv_fp8, "_few", lambda *a: form == "few")
     plan = kv_fp8.ChunkPlan.build(new, lengths, table.cpu().numpy(), Hq, cache)
-    assert plan.work.form == number
+    assert (plan.work is None) if form == "few" else plan.work.form == number
     return plan
 
 
@@ -342,7 +343,7 @@ def test_long_chunks_by_ctas_and_by_pairs(monkeypatch, form, new, lengths, Hq, H
     _lib.check_status("chunk")
 
 
-@pytest.mark.parametrize("form,new,D", [("one tile", 9, 64), ("one tile", 9, 128), ("ctas", 500, 64), ("ctas", 1500, 128), ("pairs", 1500, 128)])
+@pytest.mark.parametrize("form,new,D", [("few", 4, 64), ("few", 2, 128), ("one tile", 9, 64), ("one tile", 9, 128), ("ctas", 500, 64), ("ctas", 1500, 128), ("pairs", 1500, 128)])
 def test_scores_that_grow_by_leaps(monkeypatch, form, new, D):
     """What a chunk's weights are relative to moves only when they pass 2^40: here the scores leap along the sequence, by little and by a
     lot, at the borders of blocks, inside of them and from one half of a block to the next, up and down again, and by head."""
@@ -369,6 +370,22 @@ def test_scores_that_grow_by_leaps(monkeypatch, form, new, D):
     # 8 * 2^-23 * 400 = 2^-11.3 more, and their sum likewise; (2^-8 + 2^-12) * 0.25 is above 2 * 2^-11.3 + 2^-14
     _close(kv_fp8.chunk_attention(q, cache, plan), want, size * 1.25, BF16)
     _lib.check_status("chunk")
+
+
+@pytest.mark.parametrize("Hq,H,D,new", [(8, 2, 64, 2), (32, 8, 128, 2), (32, 8, 128, 4), (3, 3, 128, 8), (5, 1, 128, 3), (16, 1, 64, 1), (7, 1, 128, 1),
+                                        (12, 4, 64, 5)])
+@pytest.mark.parametrize("lengths", [[1], [40, 0, 129, 3, 16, 17], [9000, 31, 2], [300 + 7 * i for i in range(70)]])
+def test_few_tokens_of_each_sequence(monkeypatch, Hq, H, D, new, lengths):
+    """Causal among themselves, with sequences that bring none, that bring less than others, or more than they have."""
+    cache, table, n, _ = _filled(lengths, H, D, seed=Hq)
+    news = [new if i % 3 != 2 else i % 2 * (new - 1) for i in range(len(lengths))]
+    q = torch.randn((sum(news) + 3, Hq, D), device="cuda", generator=_gen(5)).bfloat16()
+    plan = _plan(monkeypatch, "few", news, lengths, table, Hq, cache)
+    out = torch.full_like(q, 3.0)
+    kv_fp8.chunk_attention(q, cache, plan, out=out)
+    _close(out[:-3], *_want(q[:-3], cache, table, n, news))
+    assert (out[-3:] == 3).all()
+    _lib.check_status("few")
 
 
 @pytest.mark.parametrize("Hq,H,D,new", [(130, 1, 64, 2), (200, 1, 128, 3), (256, 2, 128, 1), (384, 1, 64, 40)])
