@@ -18,7 +18,7 @@
 // TFLOP/s; 16 prompts' 397 to 324 (one CTA per item with this softmax: 168 and 355).  S in halves of 64 columns with buffers of their
 // own, so that the tensor core need not wait for the softmax, was slower (158: an MMA of 64 columns takes 0.7 of one of 128).
 // Short chunks (5 draft tokens: 27 us where the bytes take 4.8) have one tile of 20 rows, for which all codes are turned into tiles: two
-// warpgroups do that there (one: 31).  Of up to 16 rows most go the way of decode attention instead (apb_kv8_few).
+// warpgroups do that there (one: 31), 2000 clocks a block.  Of up to 16 rows most go the way of decode attention instead (apb_kv8_few).
 //
 // Items over long contexts are cut along the keys where there are too few to fill the GPU (csrc/runtime_kv8.cpp); their parts are
 // joined by kv8_chunk_join_kernel.
@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
   constexpr int kConvert = Cfg::kConvert;
   constexpr int kCtas = PAIR ? 2 : 1;
   // Parts of a block's columns that softmax threads hand over one by one, so that the values' product of one runs beside the softmax of
-  // the next.  One where that is no gain: kDual's groups wait for tiles, and kPair's CTAs would have to meet twice as often.
-  constexpr int kHalves = FORM == kTwo ? 2 : 1, kCols = kKcBlock / kHalves;
+  // the next.  One for kPair, whose CTAs would have to meet twice as often: 169 us for 146.
+  constexpr int kHalves = PAIR ? 1 : 2, kCols = kKcBlock / kHalves;
   constexpr int kRing = Cfg::kRing, kChunks = D / 64;
   extern __shared__ __align__(1024) uint8_t kc_smem[];
   uint8_t* smem = kc_smem;
@@ -432,15 +432,19 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
           ++n_q;
           for (int j = 0; j < blocks && ok; ++j) {
             const uint32_t g = j & 1, t = tile + 2 * j + 1;
-            ok = wait_tile(t) && wait(&p_full[g * 2], done[g] & 1, kTimeoutTmemEmpty);
-            if (!ok) break;
-            ++done[g];
-            if (elect_one()) {
-              issue_o(g, 0, t % kRing, j < 2);
-              commit(&kv_empty[t % kRing]);
-              if (j + 2 >= blocks) commit(&o_full[g * 2]);
+            ok = wait_tile(t);
+            for (int h = 0; h < 2 && ok; ++h) {
+              ok = wait(&p_full[g * 2 + h], done[g] >> 1 & 1, kTimeoutTmemEmpty);
+              if (!ok) break;
+              ++done[g];
+              if (elect_one()) {
+                issue_o(g, h, t % kRing, j < 2 && h == 0);
+                commit(&o_full[g * 2 + h]);
+                if (h == 1) commit(&kv_empty[t % kRing]);
+              }
+              __syncwarp();
             }
-            __syncwarp();
+            if (!ok) break;
             if (j + 2 < blocks) ok = scores(j + 2);
           }
           tile += 2 * blocks;
@@ -542,9 +546,9 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
       float m_ref = -INFINITY;             // what weights are relative to: a score of the row not far below its largest
       uint64_t l2 = 0;
       int ev = 0;
-      const int mine_n = DUAL ? (w.blocks + 1 - g) / 2 : kHalves * w.blocks;          // this group's parts of blocks
+      const int mine_n = kHalves * (DUAL ? (w.blocks + 1 - g) / 2 : w.blocks);          // this group's parts of blocks
       for (int k = 0; k < mine_n; ++k) {
-        const int j = DUAL ? 2 * k + g : k / kHalves, h = k % kHalves;
+        const int j = DUAL ? k / kHalves * 2 + g : k / kHalves, h = k % kHalves;
         const uint32_t t_s = t_s0 + h * 64;
         if (h == 0) ok = wait(&s_full[g], parts_seen / kHalves & 1, kTimeoutTmemFull);
         if (!ok) break;
