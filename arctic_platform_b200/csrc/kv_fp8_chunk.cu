@@ -11,12 +11,14 @@
 // one that moves only when a block's is larger by 2^8 or more, and O with it.  Nothing is rounded: 2^-120 of the reference is far below
 // what counts (tokens more than 2^100 smaller than the largest of their sequence lose bits).
 //
-// What bounds it.  A block of two tiles is 2050 clocks of MMAs, 2050 of exponentials, 3000 of turning codes into tiles, and the three
-// wait for one another.  Hence the pair: its MMAs of 256 rows take half of the keys and half of the values' columns from either CTA, so
-// that each turns half of the codes.  And weights are taken relative to a reference that stays while they fit (the softmax below), in one
-// pass over the scores.  Both together took 512 new tokens of a 16896-token conversation (32/8 heads of 128) from 181 to 146 us, 960
-// TFLOP/s; 16 prompts' 397 to 324 (one CTA per item with this softmax: 168 and 355).  S in halves of 64 columns with buffers of their
-// own, so that the tensor core need not wait for the softmax, was slower (158: an MMA of 64 columns takes 0.7 of one of 128).
+// What bounds it.  A block of two tiles is 2050 clocks of MMAs and 2050 of exponentials, of which a warp by itself gets half the rate,
+// beside turning codes into tiles (3000 by one warpgroup), and the three wait for one another.  Hence the pair: its MMAs of 256 rows take
+// half of the keys and half of the values' columns from either CTA, so that each turns half of the codes.  And weights are taken
+// relative to a reference that stays while they fit (the softmax below), in one pass over the scores.  Both together took 512 new tokens
+// of a 16896-token conversation (32/8 heads of 128) from 181 to 156 us, 897 TFLOP/s; 16 prompts' 397 to 346 (one CTA per item with this
+// softmax: 170 and 357).  The chain of a tile is what is left: 2300 clocks of softmax, 260 until the issuing warp knows, 1470 until the
+// next scores.  S in halves of 64 columns with buffers of their own was slower (an MMA of 64 columns takes 0.7 of one of 128), and so
+// were two threads per row (171 us: they have to agree on the reference).  Looking for codes that are no numbers costs 10 of the 156 us.
 // Short chunks (5 draft tokens: 27 us where the bytes take 4.8) have one tile of 20 rows, for which all codes are turned into tiles: two
 // warpgroups do that there (one: 31), 2000 clocks a block.  Of up to 16 rows most go the way of decode attention instead (apb_kv8_few).
 //
@@ -70,9 +72,9 @@ struct Kv8ChunkCfg {
   static constexpr int kQ = FORM == kDual ? 1 : 2, kRing = FORM == kTwo ? 3 : FORM == kDual ? 4 : 6;      // tiles
   // Warpgroups: issue, one or two that turn codes into tiles, one of softmax per tile.  Registers move between them; their sum is what
   // the block was launched with.
-  static constexpr int kConvert = FORM == kDual ? 8 : 4, kThreads = 128 + 32 * kConvert + 256;         // warps that turn codes into tiles
-  static constexpr int kRegsIssue = FORM == kDual ? 56 : 80, kRegsConvert = FORM == kDual ? 72 : 96, kRegsSoftmax = FORM == kDual ? 136 : 168;
-  static_assert(kRegsIssue * 128 + kRegsConvert * 32 * kConvert + kRegsSoftmax * 256 <= (FORM == kDual ? 96 : 128) * kThreads, "registers");
+  static constexpr int kConvert = FORM != kTwo ? 8 : 4, kThreads = 128 + 32 * kConvert + 256;         // warps that turn codes into tiles
+  static constexpr int kRegsIssue = FORM != kTwo ? 56 : 80, kRegsConvert = FORM != kTwo ? 72 : 96, kRegsSoftmax = FORM != kTwo ? 136 : 168;
+  static_assert(kRegsIssue * 128 + kRegsConvert * 32 * kConvert + kRegsSoftmax * 256 <= (FORM != kTwo ? 96 : 128) * kThreads, "registers");
   static constexpr int kStage = 8 * Kv8<D>::kBlock;
   static constexpr int kSmem = kQ * kTile + kRing * kKv + kKcStages * kStage + 2048 + 384;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
@@ -110,21 +112,22 @@ __device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
                "h"(static_cast<uint16_t>(3))
                : "memory");
 }
-// Four codes times 2^-120 as bf16 pairs, each times its factor: in their order, or (cheaper by three instructions of eight that move
-// bits) the even ones first, where that can be put right later.
-template <bool ORDERED>
+// Four codes times 2^-120 as bf16 pairs, times their factor: a byte with its sign eight times in front of it, moved by four bits, has sign,
+// exponent and mantissa in their places.
 __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t factor, uint32_t& lo, uint32_t& hi) {
   uint32_t x, y;
-  if constexpr (ORDERED) {
-    const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
-    x = (a & 0x80008000u) | ((a >> 4) & 0x07F007F0u);
-    y = (b & 0x80008000u) | ((b >> 4) & 0x07F007F0u);
-  } else {
-    x = ((w * 256u) & 0x80008000u) | ((w * 16u) & 0x07F007F0u);
-    y = (w & 0x80008000u) | ((w >> 4) & 0x07F007F0u);
-  }
+  asm("prmt.b32 %0, %1, 0, 0x9180;" : "=r"(x) : "r"(w));
+  asm("prmt.b32 %0, %1, 0, 0xB3A2;" : "=r"(y) : "r"(w));
+  x = (x * 16u) & 0x87F087F0u;
+  y = (y * 16u) & 0x87F087F0u;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(factor));
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(factor));
+}
+// Puts no numbers where codes are none.
+__device__ __forceinline__ void e4m3x4_nan(uint32_t w, uint32_t& lo, uint32_t& hi) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if ((w >> (8 * i) & 0x7F) == 0x7F) (i < 2 ? lo : hi) |= i & 1 ? 0x7FC00000u : 0x7FC0u;
 }
 
 template <int D, int FORM>
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
   constexpr int kConvert = Cfg::kConvert;
   constexpr int kCtas = PAIR ? 2 : 1;
   // Parts of a block's columns that softmax threads hand over one by one, so that the values' product of one runs beside the softmax of
-  // the next.  One for kPair, whose CTAs would have to meet twice as often: 169 us for 146.
+  // the next.  One for kPair, whose CTAs would have to meet twice as often: 169 us for 146 without the look for numbers.
   constexpr int kHalves = PAIR ? 1 : 2, kCols = kKcBlock / kHalves;
   constexpr int kRing = Cfg::kRing, kChunks = D / 64;
   extern __shared__ __align__(1024) uint8_t kc_smem[];
@@ -292,18 +295,33 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
             w[k] = lds128(codes + after(k) / 16 * Kv8<D>::kBlock);
             e[k] = lds8(exps + after(k) / 16 * Kv8<D>::kBlock);
           }
-#pragma unroll
-          for (int k = 0; k < kAt; ++k) {
-            uint32_t f = static_cast<uint32_t>(max(e[k] + up, 0)) * 0x00800080u + sign;      // two exponents
-            if (ragged && t_half + t0 + after(k) >= valid) w[k] = make_uint4(0, 0, 0, 0), f = 0;
+          uint32_t none_of = 0;          // the top bit of a byte: some code there was no number
+          auto turn = [&](uint4 r, int exponent, int later, bool none) {
+            uint32_t f = static_cast<uint32_t>(max(exponent + up, 0)) * 0x00800080u + sign;      // two exponents
+            if (ragged && t_half + t0 + later >= valid) r = make_uint4(0, 0, 0, 0), f = 0;
+            none_of |= ((r.x & 0x7F7F7F7Fu) + 0x01010101u) | ((r.y & 0x7F7F7F7Fu) + 0x01010101u);
+            none_of |= ((r.z & 0x7F7F7F7Fu) + 0x01010101u) | ((r.w & 0x7F7F7F7Fu) + 0x01010101u);
+            if (swap) r = make_uint4(r.z, r.w, r.x, r.y);
             uint4 a, b;
-            constexpr bool kOrdered = !kValue;
-            e4m3x4_to_bf16<kOrdered>(swap ? w[k].z : w[k].x, f, a.x, a.y);
-            e4m3x4_to_bf16<kOrdered>(swap ? w[k].w : w[k].y, f, a.z, a.w);
-            e4m3x4_to_bf16<kOrdered>(swap ? w[k].x : w[k].z, f, b.x, b.y);
-            e4m3x4_to_bf16<kOrdered>(swap ? w[k].y : w[k].w, f, b.z, b.w);
-            sts128(to + after(k) * 128 + u, a);
-            sts128(to + after(k) * 128 + (u ^ 16), b);
+            e4m3x4_to_bf16(r.x, f, a.x, a.y);
+            e4m3x4_to_bf16(r.y, f, a.z, a.w);
+            e4m3x4_to_bf16(r.z, f, b.x, b.y);
+            e4m3x4_to_bf16(r.w, f, b.z, b.w);
+            if (none) {
+              e4m3x4_nan(r.x, a.x, a.y);
+              e4m3x4_nan(r.y, a.z, a.w);
+              e4m3x4_nan(r.z, b.x, b.y);
+              e4m3x4_nan(r.w, b.z, b.w);
+            }
+            sts128(to + later * 128 + u, a);
+            sts128(to + later * 128 + (u ^ 16), b);
+          };
+#pragma unroll
+          for (int k = 0; k < kAt; ++k) turn(w[k], e[k], after(k), false);
+          if (none_of & 0x80808080u) {          // hardly ever: once more
+#pragma unroll 1
+            for (int k = 0; k < kAt; ++k)
+              turn(lds128(codes + after(k) / 16 * Kv8<D>::kBlock), lds8(exps + after(k) / 16 * Kv8<D>::kBlock), after(k), true);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -699,12 +717,6 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
           tmem_ld_wait(r);
 #pragma unroll
           for (int i = 0; i < 16; ++i) f[i] += f1 == 0.f ? 0.f : __uint_as_float(r[i]) * f1 * e1;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {          // values' columns have the even ones of four in front
-          const float odd = f[i + 2];
-          f[i + 2] = f[i + 1];
-          f[i + 1] = odd;
         }
         if (mine) {
           if (w.part < 0) {

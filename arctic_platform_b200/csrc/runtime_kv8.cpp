@@ -20,7 +20,7 @@ enum Form : int { kTwo, kDual, kPair };
 struct Cost {
   double two, one, item;
 };
-constexpr Cost kCost[3] = {{2.6, 2.2, 6.0}, {1.7, 1.7, 5.0}, {2.2, 2.05, 7.0}};
+constexpr Cost kCost[3] = {{2.6, 2.2, 6.0}, {1.7, 1.7, 5.0}, {2.4, 2.2, 7.0}};
 constexpr double kPart = 1.5, kJoin = 4.0;          // what a part takes longer than an item; the join of the parts
 constexpr int kLeast = 2;          // blocks of a part
 

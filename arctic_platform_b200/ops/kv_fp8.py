@@ -415,7 +415,9 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
     """``q [T, Hq, D]`` bf16, the new tokens of the plan's sequences one behind another -> ``[T, Hq, D]`` bf16.  Each row sees the
     tokens of its sequence up to itself (:class:`ChunkPlan`), rows that see nothing are zeros.  Rows of ``q`` behind the last
     sequence are padding: they are left as they were in ``out``, zeros without it.  The new tokens' own keys and values are read from the
-    cache: :func:`write` comes first.  Values whose tokens' exponents lie more than 100 below the largest of their sequence lose bits."""
+    cache: :func:`write` comes first.  Values whose tokens' exponents lie more than 100 below the largest of their sequence lose bits.
+    A key that is no number reaches the rows that see it, such a value that column of its sequence's rows, those in front of it too.  A
+    captured call reads the plan's tables when it is replayed: the plan has to live as long."""
     q, ldq = _check_queries(q, cache, out)
     data = cache.data
     T, Hq, D = q.shape

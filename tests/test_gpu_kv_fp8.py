@@ -372,6 +372,79 @@ def test_scores_that_grow_by_leaps(monkeypatch, form, new, D):
     _lib.check_status("chunk")
 
 
+@pytest.mark.parametrize("case", ["large", "small", "values of unlike size", "one huge value nobody sees", "steep", "negative scale", "zero scale",
+                                  "nothing but one token"])
+@pytest.mark.parametrize("form,new,D", [("few", 2, 128), ("one tile", 9, 64), ("one tile", 9, 128), ("ctas", 150, 64), ("ctas", 150, 128), ("pairs", 150, 128)])
+def test_numbers_of_chunks(monkeypatch, form, new, D, case):
+    H, R, n = 2, 4, 420
+    cache, table, lengths, slots = _filled([n], H, D, seed=3)
+    g = _gen(10)
+    k, v = (torch.randn((n, H, D), device="cuda", generator=g) for _ in range(2))
+    q = torch.randn((new, H * R, D), device="cuda", generator=g)
+    scale = D ** -0.5
+    if case == "large":
+        k, v, q = k * 1e15, v * 1e30, q * 1e-15
+    elif case == "small":
+        k, v, q = k * 1e-12, v * 1e-22, q * 1e12
+    elif case == "values of unlike size":
+        v = v * torch.exp(12 * torch.randn((n, H, 1), device="cuda", generator=g))
+    elif case == "one huge value nobody sees":
+        q[:, :, 0], k[:, :, 0] = 30.0, 0.0
+        k[77, :, 0] = -400.0
+        v[77] = 1e20                            # 2^66, 2^67 of the others
+    elif case == "steep":
+        q = q * 40
+    elif case == "negative scale":
+        scale = -0.3
+    elif case == "zero scale":
+        scale = 0.0
+    else:
+        k, v = k * 0, v * 0
+        v[5] = 1.0
+    kv_fp8.write(k, v, slots, cache)
+    q = q.bfloat16()
+    plan = _plan(monkeypatch, form, [new], [n], table, H * R, cache)
+    k, v = kv_fp8.read(cache, slots, torch.float32)
+    want, size = _attend(q, k, v, torch.arange(n - new, n, device="cuda"), scale)
+    if case in ("steep", "values of unlike size"):
+        size = size * 1.25                     # scores of up to 400, as below
+    _close(kv_fp8.chunk_attention(q, cache, plan, scale), want, size, FP16 if form == "few" else BF16)
+
+
+@pytest.mark.parametrize("form,new,D", [("few", 2, 128), ("one tile", 9, 64), ("one tile", 9, 128), ("ctas", 150, 64), ("ctas", 150, 128), ("pairs", 150, 128)])
+def test_numbers_that_are_none_in_a_chunk(monkeypatch, form, new, D):
+    """A key that is none reaches the rows that see it, of its sequence and head; a value its column of them at least."""
+    H, R = 2, 4
+    lengths = [400, 300]
+    cache, table, n, slots = _filled(lengths, H, D, seed=5)
+    q = torch.randn((2 * new, H * R, D), device="cuda", generator=_gen(1)).bfloat16()
+    plan = _plan(monkeypatch, form, [new] * 2, lengths, table, H * R, cache)
+    k, v = kv_fp8.read(cache, slots, torch.float32)
+    kv_fp8.write(k, v, slots, cache)                # a row whose largest was rounded down may get the next exponent, and the same numbers
+    want = kv_fp8.chunk_attention(q, cache, plan)
+    for token, column in ((10, 3), (200, D - 1), (400 - new + new // 2, 17), (399, 0)):
+        bad = k.clone()
+        bad[token, 1, column] = -math.nan
+        kv_fp8.write(bad, v, slots, cache)
+        got = kv_fp8.chunk_attention(q, cache, plan)
+        sees = torch.arange(400 - new, 400, device="cuda") >= token
+        assert torch.isnan(got[:new, R:][sees]).all()
+        if not sees.all():             # the others may share a warp with rows that see it, and take another reference
+            exact, size = _attend(q[:new], k[:400], v[:400], torch.arange(400 - new, 400, device="cuda"), D ** -0.5)
+            _close(got[:new, R:][~sees], exact[:, R:][~sees], size[:, R:][~sees], FP16 if form == "few" else BF16)
+        got[:new, R:] = want[:new, R:]
+        assert torch.equal(got, want)
+        bad = v.clone()
+        bad[token, 1, column] = math.nan
+        kv_fp8.write(k, bad, slots, cache)
+        got = kv_fp8.chunk_attention(q, cache, plan)
+        assert torch.isnan(got[:new, R:, column][sees]).all()
+        got[:new, R:, column] = want[:new, R:, column]
+        assert torch.equal(got, want)
+    cache.data[int(table[0, 0]), 1, 3 * D] = 0xFF            # as other writers have them
+    assert torch.isnan(kv_fp8.chunk_attention(q, cache, plan)[:new, R:]).all()
+
+
 @pytest.mark.parametrize("Hq,H,D,new", [(8, 2, 64, 2), (32, 8, 128, 2), (32, 8, 128, 4), (3, 3, 128, 8), (5, 1, 128, 3), (16, 1, 64, 1), (7, 1, 128, 1),
                                         (12, 4, 64, 5)])
 @pytest.mark.parametrize("lengths", [[1], [40, 0, 129, 3, 16, 17], [9000, 31, 2], [300 + 7 * i for i in range(70)]])
