@@ -299,10 +299,10 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
     wide = page_table.shape[1]
     pages = wide if longest is None else min(wide, (longest + PAGE - 1) // PAGE)
     need = _fn("scratch")(B, pages, Hq, cache.num_kv_heads, D)
-    scratch = torch.empty(need, device=data.device, dtype=torch.uint8).data_ptr() if need else None
+    scratch = torch.empty(need, device=data.device, dtype=torch.uint8) if need else None          # kept until the launch has been made
     _lib.check(_fn("decode")(q.data_ptr(), ldq, data.data_ptr(), page_table.data_ptr(), page_table.stride(0), wide, cache.num_pages,
-                             lengths.data_ptr(), out.data_ptr(), out.stride(0), B, pages, Hq, cache.num_kv_heads, D, scale, scratch,
-                             _lib.stream_ptr()), "kv8_decode")
+                             lengths.data_ptr(), out.data_ptr(), out.stride(0), B, pages, Hq, cache.num_kv_heads, D, scale,
+                             _lib.ptr(scratch), _lib.stream_ptr()), "kv8_decode")
     return out
 
 
@@ -455,8 +455,8 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
                               int(plan.new.max()), int((plan.lengths.max() + PAGE - 1) // PAGE), Hq, cache.num_kv_heads, D, scale,
                               _lib.stream_ptr()), "kv8_few")
         return out
-    scratch = torch.empty(w.part_tiles * 128 * (D + 2), device=data.device, dtype=torch.float32).data_ptr() if w.part_tiles else None
+    scratch = torch.empty(w.part_tiles * 128 * (D + 2), device=data.device, dtype=torch.float32) if w.part_tiles else None
     _lib.check(_fn("chunk")(q.data_ptr(), ldq, data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
-                            plan.first.data_ptr(), w.ctas, plan.joins.data_ptr(), len(w.joins), w.part_tiles, w.form, scratch,
+                            plan.first.data_ptr(), w.ctas, plan.joins.data_ptr(), len(w.joins), w.part_tiles, w.form, _lib.ptr(scratch),
                             out.data_ptr(), out.stride(0), T, Hq, cache.num_kv_heads, D, scale, _lib.stream_ptr()), "kv8_chunk")
     return out

@@ -536,6 +536,66 @@ def test_two_graphs_and_two_streams(what):
     assert torch.equal(again[0][0], want[0][0])
 
 
+@pytest.mark.parametrize("form,new,lengths", [("few", 2, [900, 65, 17]), ("one tile", 9, [9000, 65, 17]), ("ctas", 300, [9000, 600, 300]),
+                                              ("pairs", 300, [9000, 600, 300]), ("pairs", 40, [40] * 30)])
+def test_chunks_captured_and_on_two_streams(monkeypatch, form, new, lengths):
+    """Every form, replayed beside another graph and beside itself on a second stream, gives the bits of an eager call; a cache of
+    another layer takes the same plan."""
+    H, Hq, D = 2, 8, 128
+    cache, table, n, _ = _filled(lengths, H, D, seed=9)
+    other = kv_fp8.Fp8KVCache(cache.data.clone(), D)
+    plan = _plan(monkeypatch, form, [new] * len(lengths), lengths, table, Hq, cache)
+    qs = [torch.randn((new * len(lengths), Hq, D), device="cuda", generator=_gen(i)).bfloat16() for i in range(2)]
+    want = [kv_fp8.chunk_attention(q, cache, plan).clone() for q in qs]
+    _close(want[0], *_want(qs[0], cache, table, n, [new] * len(lengths)), FP16 if form == "few" else BF16)
+    graphs, outs = [], []
+    for q, c in zip(qs, (cache, other)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(kv_fp8.chunk_attention(q, c, plan))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+            again = kv_fp8.chunk_attention(qs[0], other, plan)
+        more = kv_fp8.chunk_attention(qs[1], cache, plan)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        assert torch.equal(again, want[0]) and torch.equal(more, want[1])
+    in_place = qs[0].clone()
+    kv_fp8.chunk_attention(in_place, cache, plan, out=in_place)
+    assert torch.equal(in_place, want[0])
+    _lib.check_status("chunk")
+
+
+@pytest.mark.parametrize("what", ["decode", "chunk"])
+def test_scratch_is_kept_until_the_launch_is_made(monkeypatch, what):
+    """Another thread that allocates on the same stream meanwhile gets other memory."""
+    H, Hq, D, lengths = 2, 8, 128, [20000, 3]
+    cache, table, n, _ = _filled(lengths, H, D, seed=9)
+    q = torch.randn((8, Hq, D), device="cuda", generator=_gen(0)).bfloat16()
+    plan = _plan(monkeypatch, "one tile", [4, 4], lengths, table, Hq, cache)
+    assert plan.work.part_tiles
+    call = (lambda: kv_fp8.decode_attention(q[:2], cache, table, n)) if what == "decode" else (lambda: kv_fp8.chunk_attention(q, cache, plan))
+    want = call().clone()
+    size = kv_fp8._fn("scratch")(2, table.shape[1], Hq, H, D) if what == "decode" else plan.work.part_tiles * 128 * (D + 2) * 4
+    assert size
+    fn, others = kv_fp8._fn(what), []
+
+    def interrupted(*args):
+        others.append(torch.empty(size, device="cuda", dtype=torch.uint8))
+        assert others[-1].data_ptr() not in [getattr(a, "value", a) for a in args]
+        return fn(*args)
+
+    monkeypatch.setitem(kv_fp8._FN, what, interrupted)
+    assert torch.equal(call(), want) and len(others) == 1
+
+
 def test_offsets_behind_two_to_the_31():
     H, D = 8, 128
     pages = (1 << 31) // (H * kv_fp8.block_bytes(D)) + 50
