@@ -175,6 +175,11 @@ def _rows_aligned(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
     return t, a, b
 
 
+def _rows(T: int, H: int, D: int, like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """New rows ``[T, H, D]`` on the device of ``like`` (with the strides named: 0.8 us of host time less than ``torch.empty``)."""
+    return torch.empty_strided((T, H, D), (H * D, D, 1), device=like.device, dtype=dtype)
+
+
 def read(cache: Fp8KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that ``slots [T]`` hold, ``[T, heads, D]`` each, exact in ``dtype`` (bf16 or fp32); zeros for slots below 0."""
     _check_slots(cache, slots, False)
@@ -191,7 +196,7 @@ def read(cache: Fp8KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bflo
     if _elsewhere(cache):
         with torch.cuda.device(cache.index):
             return read(cache, slots, dtype)
-    k, v = torch.empty((2, T, H, D), device=data.device, dtype=dtype).unbind()
+    k, v = _rows(T, H, D, data, dtype), _rows(T, H, D, data, dtype)
     if T:
         _lib.check(_fn("read")(data.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, H, D, cache.num_pages,
                                dtype is torch.float32, _lib.stream_ptr()), "kv8_read")
@@ -264,6 +269,15 @@ def attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, last: torch
     return o / torch.where(total == 0, 1.0, total).t()[..., None]
 
 
+def _refuse_tables(cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.Tensor, B: int) -> None:
+    """Says what is wrong with a batch's tables."""
+    for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
+        if t.dtype is not torch.int32 or t.dim() != dims or t.shape[0] != B or (t.stride(dims - 1) != 1 and t.numel()):
+            raise ValueError(f"{name} must be int32 {'[%d, pages]' % B if dims == 2 else [B]} with neighbouring elements, got {t.dtype} {list(t.shape)}")
+        if t.get_device() != cache.index:
+            _refuse(cache, **{name: t})
+
+
 def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None, longest: Optional[int] = None) -> torch.Tensor:
     """``q [B, Hq, D]`` bf16, one token per sequence, over the first ``lengths [B]`` (int32) tokens on the pages ``page_table
@@ -274,19 +288,19 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
     the result does not depend on it but for last bits."""
     q, ldq = _check_queries(q, cache, out)
     B, Hq, D = q.shape
-    for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
-        if t.dtype is not torch.int32 or t.dim() != dims or t.shape[0] != B or (t.stride(dims - 1) != 1 and t.numel()):
-            raise ValueError(f"{name} must be int32 {'[%d, pages]' % B if dims == 2 else [B]} with neighbouring elements, got {t.dtype} {list(t.shape)}")
-        if t.get_device() != cache.index:
-            _refuse(cache, **{name: t})
+    index = cache.index
+    if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B or (page_table.stride(1) != 1 and page_table.numel())
+            or lengths.dtype is not torch.int32 or lengths.shape != (B,) or (lengths.stride(0) != 1 and B)
+            or page_table.get_device() != index or lengths.get_device() != index):
+        _refuse_tables(cache, page_table, lengths, B)
     data, scale = cache.data, D ** -0.5 if scale is None else float(scale)
     if checked.enabled() and checked.active_for(q):
         checked.check_page_table("page_table", page_table, lengths, cache.num_pages, PAGE)
     if out is None:
-        out = torch.empty((B, Hq, D), device=data.device, dtype=torch.bfloat16)
+        out = _rows(B, Hq, D, data, torch.bfloat16)
     if B == 0:
         return out
-    if cache.index < 0:
+    if index < 0:
         for b, n in enumerate(lengths.tolist()):
             k, v = context_ref(cache, page_table[b], n)
             out[b:b + 1] = attention_ref(q[b:b + 1].float(), k, v, torch.tensor([n - 1]), scale).to(q.dtype)
@@ -367,7 +381,8 @@ class ChunkPlan:
     items: Optional[torch.Tensor] = None
     first: Optional[torch.Tensor] = None
     joins: Optional[torch.Tensor] = None
-    tokens: Optional[torch.Tensor] = None            # lengths [n], where the sequences' rows begin [n + 1]
+    # without work: the lengths [n], where the sequences' rows begin [n + 1], the most new tokens and pages of a sequence
+    few: Optional[Tuple[torch.Tensor, torch.Tensor, int, int]] = None
 
     @staticmethod
     def build(new: Sequence[int], lengths: Sequence[int], pages, heads: int, cache: Fp8KVCache) -> "ChunkPlan":
@@ -399,12 +414,14 @@ class ChunkPlan:
             table = np.zeros((n, max(1, int(need.max()))), dtype=np.int32)
             for s in range(n):
                 table[s, :need[s]] = used[s]
-            tokens = np.concatenate([lengths, [0], np.cumsum(new)]).astype(np.int32)
-            parts = (table, tokens) if plan.work is None else (w.items, w.joins, w.first, table)
+            if plan.work is None:
+                parts = (table, lengths.astype(np.int32), np.concatenate([[0], np.cumsum(new)]).astype(np.int32))
+            else:
+                parts = (w.items, w.joins, w.first, table)
             flat = torch.from_numpy(np.concatenate([a.reshape(-1) for a in parts])).pin_memory()
             dev = [t.view(a.shape) for t, a in zip(to_device(flat, cache.data.device).split([a.size for a in parts]), parts)]
             if plan.work is None:
-                plan.table, plan.tokens = dev
+                plan.table, plan.few = dev[0], (dev[1], dev[2], int(new.max()), int(need.max()))
             else:
                 plan.items, plan.joins, plan.first, plan.table = dev
         return plan
@@ -427,7 +444,7 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
         raise ValueError(f"q has {T} rows, the plan's sequences bring {plan.rows}")
     scale = D ** -0.5 if scale is None else float(scale)
     if out is None:
-        out = torch.empty((T, Hq, D), device=data.device, dtype=torch.bfloat16)
+        out = _rows(T, Hq, D, data, torch.bfloat16)
         if T > plan.rows:
             out[plan.rows:].zero_()
     if plan.rows == 0:
@@ -449,11 +466,10 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
             return chunk_attention(q, cache, plan, scale, out)
     w = plan.work
     if w is None:
-        n = len(plan.new)
-        _lib.check(_fn("few")(q.data_ptr(), ldq, data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.table.shape[1],
-                              cache.num_pages, plan.tokens.data_ptr(), plan.tokens[n:].data_ptr(), out.data_ptr(), out.stride(0), n,
-                              int(plan.new.max()), int((plan.lengths.max() + PAGE - 1) // PAGE), Hq, cache.num_kv_heads, D, scale,
-                              _lib.stream_ptr()), "kv8_few")
+        table, (lengths, starts, most, longest) = plan.table, plan.few
+        _lib.check(_fn("few")(q.data_ptr(), ldq, data.data_ptr(), table.data_ptr(), table.stride(0), table.shape[1], cache.num_pages,
+                              lengths.data_ptr(), starts.data_ptr(), out.data_ptr(), out.stride(0), table.shape[0], most, longest, Hq,
+                              cache.num_kv_heads, D, scale, _lib.stream_ptr()), "kv8_few")
         return out
     scratch = torch.empty(w.part_tiles * 128 * (D + 2), device=data.device, dtype=torch.float32) if w.part_tiles else None
     _lib.check(_fn("chunk")(q.data_ptr(), ldq, data.data_ptr(), plan.table.data_ptr(), plan.table.stride(0), plan.items.data_ptr(),
