@@ -138,15 +138,17 @@ def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Fp8KVCac
     rest of its row alone."""
     _check_slots(cache, slots, True)
     data, shape, dt = cache.data, (slots.shape[0], cache.num_kv_heads, cache.head_dim), k.dtype
-    for name, t in (("k", k), ("v", v)):
-        if t.dtype is not dt or t.shape != shape or (dt is not torch.bfloat16 and dt is not torch.float32):
-            raise ValueError(f"{name} must be bf16 or fp32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-        if t.get_device() != cache.index:
-            _refuse(cache, **{name: t})
+    index = cache.index
+    if (v.dtype is not dt or (dt is not torch.bfloat16 and dt is not torch.float32) or k.shape != shape or v.shape != shape
+            or k.get_device() != index or v.get_device() != index):
+        for name, t in (("k", k), ("v", v)):
+            if t.dtype is not dt or t.shape != shape or (dt is not torch.bfloat16 and dt is not torch.float32):
+                raise ValueError(f"{name} must be bf16 or fp32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+        _refuse(cache, k=k, v=v)
     T, H, D = shape
     if T == 0:
         return
-    if cache.index < 0:
+    if index < 0:
         ck, cv, ex = cache.parts()
         at = slots[slots >= 0].long()
         if at.numel() and int(at.max()) >= cache.num_pages * PAGE:
@@ -235,7 +237,8 @@ def norm_rope_write(acc: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: O
 # --------------------------------------------------------------------------------------------- attention
 def _check_queries(q: torch.Tensor, cache: Fp8KVCache, out: Optional[torch.Tensor]) -> Tuple[torch.Tensor, int]:
     """The queries, copied where their rows are not whole or off the 16-byte boundaries; the distance of their rows."""
-    if q.dtype is not torch.bfloat16 or q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] == 0 or q.shape[1] % cache.num_kv_heads:
+    _, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+    if q.dtype is not torch.bfloat16 or dim != cache.head_dim or heads == 0 or heads % cache.num_kv_heads:
         raise ValueError(f"q must be bf16 [rows, a multiple of {cache.num_kv_heads} heads, {cache.head_dim}], got {q.dtype} {list(q.shape)}")
     if not cache.one_layer or q.get_device() != cache.index:
         _refuse(cache, q=q)
@@ -245,7 +248,7 @@ def _check_queries(q: torch.Tensor, cache: Fp8KVCache, out: Optional[torch.Tenso
             raise ValueError("out must be bf16 of q's shape with whole rows")
         if out.get_device() != cache.index:
             _refuse(cache, out=out)
-    if c != 1 or b != cache.head_dim or a % 8 or q.data_ptr() % 16:
+    if c != 1 or b != dim or a % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         a = q.stride(0)
     return q, a
