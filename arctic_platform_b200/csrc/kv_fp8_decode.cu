@@ -12,9 +12,9 @@
 // fp16 holds codes, but not their scales: those stay outside the products.  Queries are scaled by a power of two per head so that the
 // largest is about 2^14 (what fp16 drops is below 2^-38 of it); a score is (product) * 2^(key exponent) * constant.  A value's
 // exponent belongs to its weight: with y = score + value exponent, weights are 2^(y - M + 14) against the running maximum M of y, not
-// of the scores, so that the largest weight is always 2^14 and what falls out of fp16's range is below 2^-38 of the largest term.  They are rounded to
-// 11 bits.  The sum of the softmax runs beside it in fp32 against the maximum of the scores, by lane: only M has to be common to
-// the lanes of a head while the walk lasts.
+// of the scores, so that the largest weight is always 2^14 and what falls out of fp16's range is below 2^-38 of the largest term.  They
+// are rounded to 11 bits.  The sum of the softmax runs beside it in fp32 against the maximum of the scores, by lane: only M has to be
+// common to the lanes of a head while the walk lasts.
 //
 // Measured: 128 sequences of 1365 to 4096 tokens, 32 / 8 heads of 128, 127 us (5.6 TB/s, 0.85 of a copy; the copies alone take 113); 2 of
 // 36864, 32 / 4 heads, 22.9; 41 of 500 to 1500, 16 / 8 heads, 22.5; one of 384, 6.2.
@@ -512,7 +512,8 @@ kv8_decode_stream_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decod
   float* jo = reinterpret_cast<float*>(smem + kKv8Warps * Cfg::kRing);          // [warps][4][D]
   float* js = jo + kKv8Warps * 4 * D;                                           // [warps][4][4]: M, m, l
   uint64_t* bars = reinterpret_cast<uint64_t*>(js + kKv8Warps * 4 * 4);
-  int* found = reinterpret_cast<int*>(bars + kKv8Warps * kKv8Stages);           // sequence that the share begins in, pages in front of it; sums of the warps
+  // sequence that the share begins in, pages in front of it; sums of the warps
+  int* found = reinterpret_cast<int*>(bars + kKv8Warps * kKv8Stages);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int R = p.Hq / p.Hkv, U = p.Hkv * p.groups;
   uint64_t* full = bars + warp * kKv8Stages;
@@ -804,7 +805,8 @@ long long apb_kv8_decode_scratch(int B, int longest, int Hq, int Hkv, int D) {
 
 // scratch: null, or what apb_kv8_decode_scratch says
 int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* table, long long ld_table, int max_pages, int pages,
-                   const int* lengths, void* out, long long ldo, int B, int longest, int Hq, int Hkv, int D, float scale, void* scratch, cudaStream_t s) {
+                   const int* lengths, void* out, long long ldo, int B, int longest, int Hq, int Hkv, int D, float scale,
+                   void* scratch, cudaStream_t s) {
   if (B <= 0) return 0;
   if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || pages < 1 || max_pages < 0 || static_cast<long long>(pages) * Hkv >= (1ll << 31) - 1 ||
       ldq % 8 || ldo % 2 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 4 || reinterpret_cast<uintptr_t>(data) % 16 ||

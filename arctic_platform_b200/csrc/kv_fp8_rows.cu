@@ -281,8 +281,12 @@ int apb_kv8_write(const void* k, long long ldk, long long lhk, const void* v, lo
       reinterpret_cast<uintptr_t>(data) % 16)
     return kBadArgument;
   Kv8Rows p = {k, v, ldk, lhk, ldv, lhv, slots, static_cast<uint8_t*>(data), T, H, pages * kKv8Page, status_device_ptr()};
-  if (dtype == 0) return D == 128 ? launch_rows<128>(kv8_write_kernel<__nv_bfloat16, 128, 4>, kv8_write_kernel<__nv_bfloat16, 128, 1>, p, s) : launch_rows<64>(kv8_write_kernel<__nv_bfloat16, 64, 4>, kv8_write_kernel<__nv_bfloat16, 64, 1>, p, s);
-  return D == 128 ? launch_rows<128>(kv8_write_kernel<float, 128, 4>, kv8_write_kernel<float, 128, 1>, p, s) : launch_rows<64>(kv8_write_kernel<float, 64, 4>, kv8_write_kernel<float, 64, 1>, p, s);
+  using bf16 = __nv_bfloat16;
+  if (dtype == 0)
+    return D == 128 ? launch_rows<128>(kv8_write_kernel<bf16, 128, 4>, kv8_write_kernel<bf16, 128, 1>, p, s)
+                    : launch_rows<64>(kv8_write_kernel<bf16, 64, 4>, kv8_write_kernel<bf16, 64, 1>, p, s);
+  return D == 128 ? launch_rows<128>(kv8_write_kernel<float, 128, 4>, kv8_write_kernel<float, 128, 1>, p, s)
+                  : launch_rows<64>(kv8_write_kernel<float, 64, 4>, kv8_write_kernel<float, 64, 1>, p, s);
 }
 
 // out_k, out_v: [T, H, D] of bf16 (dtype 0) or fp32 (1); zeros where slots[t] is below 0.
@@ -299,11 +303,14 @@ int apb_kv8_read(const void* data, const int* slots, void* out_k, void* out_v, i
   p.slots_end = pages * kKv8Page;
   p.status = status_device_ptr();
   if (dtype == 0) {
-    auto *ok = static_cast<__nv_bfloat16*>(out_k), *ov = static_cast<__nv_bfloat16*>(out_v);
-    return D == 128 ? launch_rows<128>(kv8_read_kernel<__nv_bfloat16, 128, 4>, kv8_read_kernel<__nv_bfloat16, 128, 1>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<__nv_bfloat16, 64, 4>, kv8_read_kernel<__nv_bfloat16, 64, 1>, p, s, ok, ov);
+    using bf16 = __nv_bfloat16;
+    auto *ok = static_cast<bf16*>(out_k), *ov = static_cast<bf16*>(out_v);
+    return D == 128 ? launch_rows<128>(kv8_read_kernel<bf16, 128, 4>, kv8_read_kernel<bf16, 128, 1>, p, s, ok, ov)
+                    : launch_rows<64>(kv8_read_kernel<bf16, 64, 4>, kv8_read_kernel<bf16, 64, 1>, p, s, ok, ov);
   }
   auto *ok = static_cast<float*>(out_k), *ov = static_cast<float*>(out_v);
-  return D == 128 ? launch_rows<128>(kv8_read_kernel<float, 128, 4>, kv8_read_kernel<float, 128, 1>, p, s, ok, ov) : launch_rows<64>(kv8_read_kernel<float, 64, 4>, kv8_read_kernel<float, 64, 1>, p, s, ok, ov);
+  return D == 128 ? launch_rows<128>(kv8_read_kernel<float, 128, 4>, kv8_read_kernel<float, 128, 1>, p, s, ok, ov)
+                  : launch_rows<64>(kv8_read_kernel<float, 64, 4>, kv8_read_kernel<float, 64, 1>, p, s, ok, ov);
 }
 
 // acc [B, (Hq + 2 H) D] fp32, left as zeros; wq, wk [D] bf16 or null; cos, sin [positions, D / 2]; q_out [B, Hq, D] bf16.

@@ -276,7 +276,8 @@ def _refuse_tables(cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.T
     """Says what is wrong with a batch's tables."""
     for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
         if t.dtype is not torch.int32 or t.dim() != dims or t.shape[0] != B or (t.stride(dims - 1) != 1 and t.numel()):
-            raise ValueError(f"{name} must be int32 {'[%d, pages]' % B if dims == 2 else [B]} with neighbouring elements, got {t.dtype} {list(t.shape)}")
+            shape = f"[{B}, pages]" if dims == 2 else [B]
+            raise ValueError(f"{name} must be int32 {shape} with neighbouring elements, got {t.dtype} {list(t.shape)}")
         if t.get_device() != cache.index:
             _refuse(cache, **{name: t})
 
@@ -292,7 +293,8 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
     q, ldq = _check_queries(q, cache, out)
     B, Hq, D = q.shape
     index = cache.index
-    if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B or (page_table.stride(1) != 1 and page_table.numel())
+    if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B
+            or (page_table.stride(1) != 1 and page_table.numel())
             or lengths.dtype is not torch.int32 or lengths.shape != (B,) or (lengths.stride(0) != 1 and B)
             or page_table.get_device() != index or lengths.get_device() != index):
         _refuse_tables(cache, page_table, lengths, B)
