@@ -4,7 +4,7 @@
 // D / 8 lanes share a row, eight neighbouring values each, so that 16-byte accesses to the values and 8-byte ones to the codes cover
 // whole sectors; the largest magnitude of a row is found by shuffles among them, and nothing is read twice.  (Lanes that walked over
 // rows one at a time kept too little on its way, and a 64-bit division per row: 2.9 TB/s in, 4.1 out.)  Measured, 8 heads of 128, bf16:
-// 16384 tokens 20 us in (5.1 TB/s), 16 out; 36864 tokens of 4 heads 20.2 us out (5.6 TB/s, 0.86 of a copy; issue slots are 76 % busy).
+// 16384 tokens 36 us in and out (4.7 TB/s); 36864 tokens of 4 heads 20.2 us out (5.6 TB/s, 0.86 of a copy; issue slots are 76 % busy).
 #include <cuda_fp16.h>
 
 #include "host_utils.cuh"
