@@ -173,7 +173,7 @@ struct Kv8QkvPost {
   const int *pos, *slots;
   __nv_bfloat16* q_out;              // [B, Hq, D]
   uint8_t* data;
-  int B, Hq, H, slots_end;
+  int B, Hq, H, slots_end, positions;      // positions: rows of cos and sin
   float eps;
   int* status;
 };
@@ -194,8 +194,14 @@ __global__ void __launch_bounds__(256) kv8_qkv_post_kernel(const Kv8QkvPost p) {
     src[D / 2 + lane * E + j] = 0.f;
   }
   const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.H;
-  const int slot = p.slots[t];
-  if (!is_v) {
+  const int pos = p.pos[t];
+  const bool lost = static_cast<unsigned>(pos) >= static_cast<unsigned>(p.positions);      // the tables have no such row
+  const int slot = lost ? -1 : p.slots[t];
+  if (lost) {
+    if (p.status) atomicCAS(p.status, 0, kBadTable);
+#pragma unroll
+    for (int j = 0; j < E; ++j) a[j] = b[j] = 0.f;
+  } else if (!is_v) {
     const __nv_bfloat16* weight = is_q ? p.wq : p.wk;
     if (weight) {
       float ss = 0.f;
@@ -208,7 +214,7 @@ __global__ void __launch_bounds__(256) kv8_qkv_post_kernel(const Kv8QkvPost p) {
         b[j] *= rstd * __bfloat162float(weight[D / 2 + lane * E + j]);
       }
     }
-    const long long at = static_cast<long long>(p.pos[t]) * (D / 2) + lane * E;
+    const long long at = static_cast<long long>(pos) * (D / 2) + lane * E;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const float c = p.cos_t[at + j], s = p.sin_t[at + j], x = a[j] * c - b[j] * s;
@@ -315,11 +321,14 @@ int apb_kv8_read(const void* data, const int* slots, void* out_k, void* out_v, i
 
 // acc [B, (Hq + 2 H) D] fp32, left as zeros; wq, wk [D] bf16 or null; cos, sin [positions, D / 2]; q_out [B, Hq, D] bf16.
 int apb_kv8_qkv_post(float* acc, long long ld_acc, const void* wq, const void* wk, const float* cos_t, const float* sin_t, const int* pos,
-                     const int* slots, void* q_out, void* data, int B, int Hq, int H, int D, int pages, float eps, cudaStream_t s) {
+                     const int* slots, void* q_out, void* data, int B, int Hq, int H, int D, int pages, int positions, float eps,
+                     cudaStream_t s) {
   if (B <= 0) return 0;
-  if ((D != 64 && D != 128) || H < 1 || Hq < 1 || pages < 0 || pages > (1 << 27) || reinterpret_cast<uintptr_t>(data) % 16) return kBadArgument;
+  if ((D != 64 && D != 128) || H < 1 || Hq < 1 || positions < 0 || pages < 0 || pages > (1 << 27) || reinterpret_cast<uintptr_t>(data) % 16)
+    return kBadArgument;
   const Kv8QkvPost p = {acc, ld_acc, static_cast<const __nv_bfloat16*>(wq), static_cast<const __nv_bfloat16*>(wk), cos_t, sin_t, pos, slots,
-                        static_cast<__nv_bfloat16*>(q_out), static_cast<uint8_t*>(data), B, Hq, H, pages * kKv8Page, eps, status_device_ptr()};
+                        static_cast<__nv_bfloat16*>(q_out), static_cast<uint8_t*>(data), B, Hq, H, pages * kKv8Page, positions, eps,
+                        status_device_ptr()};
   const dim3 grid(static_cast<unsigned>((static_cast<long long>(B) * (Hq + 2 * H) + 7) / 8));
   return static_cast<int>(D == 128 ? launch_kernel(kv8_qkv_post_kernel<128>, grid, dim3(256), 0, s, p)
                                    : launch_kernel(kv8_qkv_post_kernel<64>, grid, dim3(256), 0, s, p));

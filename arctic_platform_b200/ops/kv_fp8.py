@@ -39,7 +39,7 @@ def _fn(name: str):
         vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
         _FN["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
         _FN["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
-        _FN["qkv"] = _lib.declare("apb_kv8_qkv_post", [vp, ll] + [vp] * 8 + [i, i, i, i, i, f, vp])
+        _FN["qkv"] = _lib.declare("apb_kv8_qkv_post", [vp, ll] + [vp] * 8 + [i, i, i, i, i, i, f, vp])
         _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, i, f, vp, vp])
         _FN["scratch"] = _lib.declare("apb_kv8_decode_scratch", [i, i, i, i, i], ll)
         _FN["few"] = _lib.declare("apb_kv8_few", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, ll, i, i, i, i, i, i, f, vp])
@@ -209,28 +209,35 @@ def norm_rope_write(acc: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: O
                     positions: torch.Tensor, slots: torch.Tensor, cache: Fp8KVCache, heads: int, eps: float) -> torch.Tensor:
     """A decode step behind its qkv projection (CUDA only): ``acc [B, (heads + 2 * key heads) * D]`` fp32 sums, left as zeros for the next
     ones to be added to; RMSNorm per head (weights ``[D]`` bf16, or None) and rotate-half RoPE (``cos, sin [positions, D / 2]`` fp32) of
-    q and k at ``positions [B]`` int32.  Returns q ``[B, heads, D]`` bf16; k and v are rounded to bf16 and written as :func:`write` does."""
+    q and k at ``positions [B]`` int32.  Returns q ``[B, heads, D]`` bf16; k and v are rounded to bf16 and written as :func:`write` does.
+    A position that the tables do not have is reported (:func:`_lib.check_status`): its q is zeros, its k and v are not written."""
     _check_slots(cache, slots, True)
     data, B, H, D = cache.data, slots.shape[0], cache.num_kv_heads, cache.head_dim
-    if acc.dtype is not torch.float32 or acc.shape != (B, (heads + 2 * H) * D) or acc.stride(1) != 1:
-        raise ValueError(f"acc must be fp32 {[B, (heads + 2 * H) * D]} with whole rows, got {acc.dtype} {list(acc.shape)}")
+    width = (heads + 2 * H) * D
+    if heads < 1 or acc.dtype is not torch.float32 or acc.shape != (B, width) or acc.stride(1) != 1 or (B > 1 and acc.stride(0) < width):
+        raise ValueError(f"acc must be fp32 {[B, width]} with whole rows of their own, got {acc.dtype} {list(acc.shape)}")
     if positions.dtype is not torch.int32 or positions.shape != slots.shape or not positions.is_contiguous():
         raise ValueError("positions must be int32, one per row")
     cos, sin = rope
-    for name, t, dt, last in (("cos", cos, torch.float32, D // 2), ("sin", sin, torch.float32, D // 2), ("q_norm", q_norm, torch.bfloat16, D),
-                              ("k_norm", k_norm, torch.bfloat16, D)):
-        if t is not None and (t.dtype is not dt or t.shape[-1] != last or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {dt} with rows of {last}")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype is not torch.float32 or t.dim() != 2 or t.shape != (cos.shape[0], D // 2) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous fp32 [positions, {D // 2}], as many as the other one, got {t.dtype} {list(t.shape)}")
+    norms = {name: t for name, t in (("q_norm", q_norm), ("k_norm", k_norm)) if t is not None}
+    for name, t in norms.items():
+        if t.dtype is not torch.bfloat16 or t.shape != (D,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous bf16 [{D}], got {t.dtype} {list(t.shape)}")
+    _refuse(cache, acc=acc, positions=positions, cos=cos, sin=sin, **norms)
     if cache.index < 0:
         raise ValueError("norm_rope_write runs on a GPU")
-    _refuse(cache, acc=acc, positions=positions, cos=cos, sin=sin)
+    if checked.enabled() and checked.active_for(positions):
+        checked.check_range("positions", positions, 0, cos.shape[0])
     if _elsewhere(cache):
         with torch.cuda.device(cache.index):
             return norm_rope_write(acc, q_norm, k_norm, rope, positions, slots, cache, heads, eps)
     q = torch.empty((B, heads, D), device=data.device, dtype=torch.bfloat16)
     _lib.check(_fn("qkv")(acc.data_ptr(), acc.stride(0), _lib.ptr(q_norm), _lib.ptr(k_norm), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
-                          slots.data_ptr(), q.data_ptr(), data.data_ptr(), B, heads, H, D, cache.num_pages, float(eps), _lib.stream_ptr()),
-               "kv8_qkv_post")
+                          slots.data_ptr(), q.data_ptr(), data.data_ptr(), B, heads, H, D, cache.num_pages, cos.shape[0], float(eps),
+                          _lib.stream_ptr()), "kv8_qkv_post")
     return q
 
 

@@ -1,0 +1,49 @@
+"""The 8-bit cache on the GPU, at the limits of what its operators take."""
+import pytest
+import torch
+
+from arctic_platform_b200.ops import _lib, kv_fp8
+from arctic_platform_b200.utils import checked
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_position_behind_the_tables_is_left_out_and_reported(D):
+    B, Hq, H = 5, 4, 2
+    g = _gen(D)
+    sums = torch.randn((B, (Hq + 2 * H) * D), device="cuda", generator=g)
+    w = torch.randn(D, device="cuda", generator=g).bfloat16()
+    angle = torch.randn((9, D // 2), device="cuda", generator=g)
+    rope = angle.cos().contiguous(), angle.sin().contiguous()
+    slots = torch.arange(B, device="cuda", dtype=torch.int32)
+    pos = torch.tensor([3, 9, 8, -1, 0], device="cuda", dtype=torch.int32)
+    good = torch.tensor([True, False, True, False, True], device="cuda")
+    want = kv_fp8.Fp8KVCache.zeros(1, H, D)
+    q_want = kv_fp8.norm_rope_write(sums.clone(), w, w, rope, pos.clamp(0, 8), torch.where(good, slots, -1), want, Hq, 1e-6)
+    checked.force(False)
+    try:
+        got, acc = kv_fp8.Fp8KVCache.zeros(1, H, D), sums.clone()
+        q = kv_fp8.norm_rope_write(acc, w, w, rope, pos, slots, got, Hq, 1e-6)
+        with pytest.raises(_lib.KernelError, match="203"):
+            _lib.check_status("step")
+        checked.force(True)
+        with pytest.raises(checked.TableError, match="positions"):
+            kv_fp8.norm_rope_write(sums.clone(), w, w, rope, pos, slots, got, Hq, 1e-6)
+    finally:
+        checked.force(None)
+    assert torch.equal(got.data, want.data) and torch.equal(q[good], q_want[good]) and not q[~good].any() and not acc.any()
+
+
+def test_weights_on_the_host_are_refused():
+    sums = torch.zeros((1, 4 * 64), device="cuda")
+    w = torch.ones(64).bfloat16()
+    rope = torch.ones((2, 32), device="cuda"), torch.zeros((2, 32), device="cuda")
+    at = torch.zeros(1, device="cuda", dtype=torch.int32)
+    for q_norm, k_norm in ((w, None), (None, w), (w.cuda(), w)):
+        with pytest.raises(ValueError, match="_norm lives on cpu"):
+            kv_fp8.norm_rope_write(sums, q_norm, k_norm, rope, at, at, kv_fp8.Fp8KVCache.zeros(1, 1, 64), 2, 1e-6)
