@@ -336,6 +336,12 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
         next(st, st_phase, kKcStages);
       }
     }
+    // Commits arrive by themselves, in pairs from the partner's tensor core too: the block does not leave before the last ones have, those
+    // of every tile that is still in the ring (a slot that was never taken counts as given back).
+    for (int i = 0; i < kRing && ok; ++i) {
+      ok = wait(&kv_empty[slot], phase ^ 1, kTimeoutEmpty);
+      next(slot, phase, kRing);
+    }
   };
 
   if (warp < 4) {
@@ -386,6 +392,7 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
           next(slot, phase, kKcStages);
         }
       }
+      if (ok) ok = wait(q_empty, (n_q & 1) ^ 1, kTimeoutEmpty);          // the last commit, as with the ring's
       if (!ok) {
         const uint64_t t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 100000ull) {
@@ -741,6 +748,8 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
       tc_fence_before();
       if (DUAL && !(ok = meet_other())) break;          // the next item's products write over both groups' O
     }
+    // the last commit that no reference asked for
+    if (kHalves == 2 && ok && parts_seen > 0) wait(&o_full[g * 2], (parts_seen / 2 - 1) & 1, kTimeoutTmemFull);
   }
 
   tc_fence_before();
