@@ -94,8 +94,10 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+// An arrival at a barrier of either CTA that orders no accesses to shared memory: for what lies in tensor memory, which tcgen05's fences
+// order with it.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void umma_bf16_ts_pair(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -165,8 +167,9 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
   uint64_t* meet = o_full + 4;         // [4] kDual: the two warps of 32 rows
   int2* meta = reinterpret_cast<int2*>(meet + 4);             // [kKcMeta] reference exponents of a block's keys and values
   int* other_ev = reinterpret_cast<int*>(meta + kKcMeta);     // [2][4] kDual: what a group's O is in units of, for 32 rows each
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(other_ev + 8);
-  static_assert((2 * kKcStages + 2 * kRing + 2 + 10 + 4) * 8 + kKcMeta * 8 + 36 <= 384, "barriers");
+  uint64_t* kv_made = reinterpret_cast<uint64_t*>(other_ev + 8);      // kPair: [kRing] this CTA's part of a tile
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(kv_made + (PAIR ? kRing : 0));
+  static_assert((2 * kKcStages + (PAIR ? 3 : 2) * kRing + 2 + 10 + 4) * 8 + kKcMeta * 8 + 36 <= 384, "barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t cta = PAIR ? cluster_cta_rank() : 0;          // 0 issues the products of both
@@ -176,8 +179,9 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
       mbar_init(&st_empty[s], kConvert);
     }
     for (int s = 0; s < kRing; ++s) {
-      mbar_init(&kv_full[s], kCtas * kConvert);
+      mbar_init(&kv_full[s], PAIR ? kCtas : kConvert);
       mbar_init(&kv_empty[s], 1);
+      if constexpr (PAIR) mbar_init(&kv_made[s], kConvert);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -211,11 +215,10 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
   const uint32_t tmem_base = *tmem_holder;
 
   const int item0 = p.first[blockIdx.x / kCtas], item1 = p.first[blockIdx.x / kCtas + 1];
-  // To the CTA that issues.  What it tells of is tiles in shared memory (behind a proxy fence) or weights in tensor memory (behind
-  // tcgen05's): released at the cluster's scope besides, an arrival took 1000 clocks.
+  // To the warp that issues: weights are in tensor memory, scores may be written over.
   auto arrive_issuer = [&](uint64_t* bar) {
     if constexpr (PAIR)
-      mbar_arrive_remote(map_to_cta(smem_u32(bar), 0));
+      mbar_arrive_relaxed(map_to_cta(smem_u32(bar), 0));
     else
       mbar_arrive(bar);
   };
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
       tc_commit(bar);
   };
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {      // of a whole warp
-    const bool r = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code));
+    const bool r = __all_sync(0xffffffffu, mbar_wait<PAIR>(bar, parity, p.status, code));
     tc_fence_after();
     return r;
   };
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) arrive_issuer(&kv_full[slot]);
+          if (lane == 0) mbar_arrive(PAIR ? &kv_made[slot] : &kv_full[slot]);
           next(slot, phase, kRing);
         };
         tile(std::integral_constant<int, 0>());
@@ -538,6 +541,20 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
             }
           }
         }
+      }
+    } else if (PAIR && warp == 2) {
+      // ---------------------------------------------------------------- tiles made, to the CTA that issues
+      // Tiles are stores to shared memory that the products of another CTA's thread read: they have to be released at the cluster's scope.
+      // By the warps that make them that takes 1000 clocks a tile, for their own stores to settle (202 us for 148, 512 tokens behind 16384);
+      // a warp that has none passes on what it has acquired.
+      int tiles = 0;
+      for (int at = item0; at < item1; ++at) tiles += 2 * p.items[at].blocks;
+      int slot = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < tiles; ++i) {
+        if (!wait(&kv_made[slot], phase, kTimeoutFull)) break;
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&kv_full[slot]), 0));
+        next(slot, phase, kRing);
       }
     }
   } else if (warp < 4 + kConvert) {
