@@ -819,8 +819,7 @@ int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* ta
   if (rc) return 1000 + rc;
   Kv8Decode p = {static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const uint8_t*>(data), table, ld_table, max_pages, pages, lengths,
                  static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, groups, 1, scale * 1.4426950408889634f, status_device_ptr(), nullptr};
-  if (scratch) {
-    if (units * max_pages >= (1ll << 30)) return kBadArgument;
+  if (scratch && units * max_pages < (1ll << 30)) {          // shares count pages in 32 bits, of as many as a table could name
     const long long rows = static_cast<long long>(kv8_stream_ctas(H)) * 2 * 8 * H;
     Kv8Parts parts;
     parts.o = static_cast<float*>(scratch);

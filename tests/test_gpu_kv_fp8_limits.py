@@ -4,6 +4,7 @@ import torch
 
 from arctic_platform_b200.ops import _lib, kv_fp8
 from arctic_platform_b200.utils import checked
+from tests.test_gpu_kv_fp8 import _close, _filled, _want
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,19 @@ def test_weights_on_the_host_are_refused():
     for q_norm, k_norm in ((w, None), (None, w), (w.cuda(), w)):
         with pytest.raises(ValueError, match="_norm lives on cpu"):
             kv_fp8.norm_rope_write(sums, q_norm, k_norm, rope, at, at, kv_fp8.Fp8KVCache.zeros(1, 1, 64), 2, 1e-6)
+
+
+def test_a_table_far_wider_than_its_sequences():
+    """More places in the table than shares of pages count; the sequences' lengths decide, not the table's width."""
+    H, Hq, D, B, wide = 8, 32, 128, 16, 1 << 23
+    cache, table, n, _ = _filled([300], H, D)
+    table = torch.cat([table, torch.full((1, wide - table.shape[1]), -1, device="cuda", dtype=torch.int32)], 1).expand(B, -1)
+    n = torch.arange(1, 301, 19, device="cuda", dtype=torch.int32)
+    assert len(n) == B and kv_fp8._fn("scratch")(B, 5000 // 16, Hq, H, D) > 0
+    q = torch.randn((B, Hq, D), device="cuda", generator=_gen(1)).bfloat16()
+    checked.force(False)
+    try:
+        _close(kv_fp8.decode_attention(q, cache, table, n, longest=5000), *_want(q, cache, table, n))
+    finally:
+        checked.force(None)
+    _lib.check_status("decode")
