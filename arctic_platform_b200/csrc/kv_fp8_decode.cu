@@ -754,6 +754,9 @@ static int launch_kv8_decode(const CUtensorMap& map, const Kv8Decode& p, cudaStr
                                                  p.splits, s, map, p));
 }
 
+// Places of a table that count: as many as a sequence of up to 2^31 tokens has, so that their tokens fit 32 bits.
+static int table_width(int max_pages) { return max_pages < (1 << 27) ? max_pages : (1 << 27) - 1; }
+
 // CTAs that a unit is cut into, of 8 pages at least, as long as all have a place
 static int kv8_splits(long long units, int longest) {
   int splits = 1;
@@ -812,6 +815,7 @@ int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* ta
       ldq % 8 || ldo % 2 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 4 || reinterpret_cast<uintptr_t>(data) % 16 ||
       reinterpret_cast<uintptr_t>(scratch) % 16)
     return kBadArgument;
+  max_pages = table_width(max_pages);
   const int R = Hq / Hkv, H = R > 8 ? 2 : 1, groups = (R + 8 * H - 1) / (8 * H);
   const long long units = static_cast<long long>(B) * Hkv * groups;
   CUtensorMap map;
@@ -847,6 +851,7 @@ int apb_kv8_few(const void* q, long long ldq, const void* data, const int* table
     return kBadArgument;
   const long long rows = static_cast<long long>(most) * (Hq / Hkv), units = static_cast<long long>(B) * Hkv;
   if (rows > 16) return kBadArgument;
+  max_pages = table_width(max_pages);
   CUtensorMap map;
   const int rc = kv8_map(&map, data, D, static_cast<long long>(pages) * Hkv);
   if (rc) return 1000 + rc;

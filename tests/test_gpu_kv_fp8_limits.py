@@ -64,3 +64,16 @@ def test_a_table_far_wider_than_its_sequences():
     finally:
         checked.force(None)
     _lib.check_status("decode")
+
+
+def test_a_table_of_as_many_places_as_there_are_tokens_in_32_bits():
+    cache, table, n, _ = _filled([300], 1, 64)
+    wide = torch.cat([table[0], torch.full(((1 << 27) - table.shape[1],), -1, device="cuda", dtype=torch.int32)])[None]
+    q = torch.randn((1, 4, 64), device="cuda", generator=_gen(1)).bfloat16()
+    checked.force(False)
+    try:
+        for longest in (300, None):
+            _close(kv_fp8.decode_attention(q, cache, wide, n, longest=longest), *_want(q, cache, table, n))
+    finally:
+        checked.force(None)
+    _lib.check_status("decode")
