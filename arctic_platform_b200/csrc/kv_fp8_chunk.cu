@@ -7,7 +7,7 @@
 // Keys and values are bf16 operands here: kind::f16 wants both sides in 16 bits, and queries and weights do not fit 8.  Pages come by
 // bulk copies into a staging ring as they lie in the cache; one or two warpgroups turn them into swizzled bf16 tiles.  A code becomes
 // a bf16 number by moving its bits (exponents off by 120), two at a time, and one multiplication by a power of two, which also brings
-// in its token's exponent relative to a reference: for keys the block's largest exponent, which the softmax multiplies by, for values
+// in its token's exponent relative to a reference: for keys the block's largest exponent (and 16), which the softmax multiplies by, for values
 // one that moves only when a block's is larger by 2^8 or more, and O with it.  Nothing is rounded: 2^-120 of the reference is far below
 // what counts (tokens more than 2^100 smaller than the largest of their sequence lose bits).
 //
@@ -243,6 +243,10 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
   auto convert = [&]() {
     // ---------------------------------------------------------------- codes to tiles
     const int part = warp - 4;
+    // Keys' exponents are taken relative to 16 above their largest: they are at most 2^-7 then, and 128 products with queries of any size
+    // fit fp32.  Less where the reference times the scale would come near the end of fp32: queries for which the rest matters have scores
+    // behind that end.
+    const int most_ref = min(111, 110 + 127 - static_cast<int>(__float_as_uint(p.scale_log2) >> 23));
     bool ok = true;
     int st = 0, slot = 0;
     uint32_t st_phase = 0, phase = 0, n_blocks = 0;
@@ -265,7 +269,8 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
         kmax = __reduce_max_sync(0xffffffffu, kmax);
         vmax = __reduce_max_sync(0xffffffffu, vmax);
         if (j == 0 || vmax > vref + 7) vref = vmax;       // factors up to 2^127 do without a new one
-        if (part == 0 && lane == 0) meta[n_blocks % kKcMeta] = make_int2(kmax - 127, vref - 127);
+        const int kref = kmax + min(max(most_ref + 127 - kmax, 0), 16);
+        if (part == 0 && lane == 0) meta[n_blocks % kKcMeta] = make_int2(kref - 127, vref - 127);
         ++n_blocks;
         const bool ragged = valid < kKcBlock;
         auto tile = [&](auto value) {
@@ -291,7 +296,7 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
           const uint32_t exps = page0 + 2 * Kv8<D>::kHalf + kv8_exponent_at(t0 & 15, kValue);
           const uint32_t to = smem_u32(smem_kv) + slot * Cfg::kKv + (c >> 2) * kRows * 128 + t0 * 128, u = (u0 ^ (t0 & 7)) << 4;
           const uint32_t sign = kValue ? 0u : p.key_sign;
-          const int up = 127 + 120 - (kValue ? vref : kmax);
+          const int up = 127 + 120 - (kValue ? vref : kref);
           uint4 w[kAt];
           int e[kAt];
 #pragma unroll

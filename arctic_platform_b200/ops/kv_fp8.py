@@ -9,7 +9,8 @@ order nor the portions in which a page is filled change what it holds.
 * :func:`write` quantises rows into their slots, :func:`read` gives them back; :func:`norm_rope_write` does it behind the projection of a
   decode step;
 * :func:`decode_attention` is the attention of one query token per sequence (page tables and lengths on the device, as in a captured
-  decode step), :func:`chunk_attention` that of the last tokens of each sequence, causal, by a plan that is made once per step.
+  decode step), :func:`chunk_attention` that of the last tokens of each sequence, causal, by a plan that is made once per step.  Scores are
+  fp32 numbers: a query's largest magnitude times that of a key has to be below 2e38.
 
 CUDA tensors run ``kv_fp8_*.cu``; CPU tensors run the plain PyTorch expressions below (the oracle of the GPU tests).
 """

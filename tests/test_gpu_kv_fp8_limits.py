@@ -4,7 +4,7 @@ import torch
 
 from arctic_platform_b200.ops import _lib, kv_fp8
 from arctic_platform_b200.utils import checked
-from tests.test_gpu_kv_fp8 import _close, _filled, _want
+from tests.test_gpu_kv_fp8 import BF16, FP16, _attend, _close, _filled, _plan, _want
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,23 @@ def test_a_table_of_as_many_places_as_there_are_tokens_in_32_bits():
     finally:
         checked.force(None)
     _lib.check_status("decode")
+
+
+@pytest.mark.parametrize("size", [(1e36, 1e-28), (1e-28, 1e36), (3e-37, 1e30)])
+@pytest.mark.parametrize("form,new,D", [("few", 2, 128), ("one tile", 9, 64), ("one tile", 9, 128), ("ctas", 150, 64), ("ctas", 150, 128), ("pairs", 150, 128)])
+def test_queries_and_keys_of_any_size(monkeypatch, form, new, D, size):
+    """Far apart, with a scale that brings their products back.  Queries and keys round as any others do: the tolerance is the usual one."""
+    H, R, n = 2, 4, 420
+    cache, table, lengths, slots = _filled([n], H, D, seed=3)
+    g = _gen(10)
+    k, v = (torch.randn((n, H, D), device="cuda", generator=g) for _ in range(2))
+    q = torch.randn((new, H * R, D), device="cuda", generator=g)
+    scale = D ** -0.5 / (size[0] * size[1])
+    q = (q * size[0]).bfloat16()
+    kv_fp8.write(k * size[1], v, slots, cache)
+    plan = _plan(monkeypatch, form, [new], [n], table, H * R, cache)
+    k, v = kv_fp8.read(cache, slots, torch.float32)
+    want, most = _attend(q, k, v, torch.arange(n - new, n, device="cuda"), scale)
+    _close(kv_fp8.chunk_attention(q, cache, plan, scale), want, most, FP16 if form == "few" else BF16)
+    _close(kv_fp8.decode_attention(q[-1:], cache, table, lengths, scale), want[-1:], most[-1:])
+    _lib.check_status("chunk")
