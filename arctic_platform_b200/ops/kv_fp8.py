@@ -244,21 +244,23 @@ def norm_rope_write(acc: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: O
 
 # --------------------------------------------------------------------------------------------- attention
 def _check_queries(q: torch.Tensor, cache: Fp8KVCache, out: Optional[torch.Tensor]) -> Tuple[torch.Tensor, int]:
-    """The queries, copied where their rows are not whole or off the 16-byte boundaries; the distance of their rows."""
-    _, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+    """The queries, copied where their rows are not whole, off the 16-byte boundaries or one over another (a tensor map wants strides that
+    grow); the distance of their rows."""
+    rows, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
     if q.dtype is not torch.bfloat16 or dim != cache.head_dim or heads == 0 or heads % cache.num_kv_heads:
         raise ValueError(f"q must be bf16 [rows, a multiple of {cache.num_kv_heads} heads, {cache.head_dim}], got {q.dtype} {list(q.shape)}")
     if not cache.one_layer or q.get_device() != cache.index:
         _refuse(cache, q=q)
     a, b, c = q.stride()
     if out is not None:
-        if out.dtype is not torch.bfloat16 or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != cache.head_dim:
-            raise ValueError("out must be bf16 of q's shape with whole rows")
+        if (out.dtype is not torch.bfloat16 or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != dim
+                or (rows > 1 and out.stride(0) < heads * dim)):
+            raise ValueError("out must be bf16 of q's shape with whole rows of their own")
         if out.get_device() != cache.index:
             _refuse(cache, out=out)
-    if c != 1 or b != dim or a % 8 or q.data_ptr() % 16:
+    if c != 1 or b != dim or a % 8 or a < heads * dim or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-        a = q.stride(0)
+        a = heads * dim
     return q, a
 
 

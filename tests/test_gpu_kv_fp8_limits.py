@@ -97,3 +97,14 @@ def test_queries_and_keys_of_any_size(monkeypatch, form, new, D, size):
     _close(kv_fp8.chunk_attention(q, cache, plan, scale), want, most, FP16 if form == "few" else BF16)
     _close(kv_fp8.decode_attention(q[-1:], cache, table, lengths, scale), want[-1:], most[-1:])
     _lib.check_status("chunk")
+
+
+@pytest.mark.parametrize("form,new", [("few", 2), ("one tile", 9), ("ctas", 300), ("pairs", 300)])
+def test_one_query_for_all_tokens(monkeypatch, form, new):
+    H, Hq, D = 2, 8, 128
+    cache, table, n, _ = _filled([400, 330], H, D)
+    plan = _plan(monkeypatch, form, [new] * 2, [400, 330], table, Hq, cache)
+    q = torch.randn((1, Hq, D), device="cuda", generator=_gen(2)).bfloat16().expand(2 * new, -1, -1)
+    want = kv_fp8.chunk_attention(q.contiguous(), cache, plan)
+    assert torch.equal(kv_fp8.chunk_attention(q, cache, plan), want)
+    assert torch.equal(kv_fp8.decode_attention(q[:2], cache, table, n), kv_fp8.decode_attention(q[:2].contiguous(), cache, table, n))

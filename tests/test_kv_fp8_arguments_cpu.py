@@ -36,3 +36,26 @@ def test_a_step_asks_where_each_of_its_tensors_lives(monkeypatch):
     with pytest.raises(ValueError, match="runs on a GPU"):
         kv_fp8.norm_rope_write(**_step())
     assert seen >= {"acc", "positions", "cos", "sin", "q_norm", "k_norm"}
+
+
+def test_queries_that_share_their_memory_get_rows_of_their_own():
+    cache = kv_fp8.Fp8KVCache.zeros(4, H, D, device="cpu")
+    one = torch.randn(1, HEADS, D).bfloat16()
+    q, distance = kv_fp8._check_queries(one.expand(5, -1, -1), cache, None)
+    assert distance == q.stride(0) == HEADS * D and torch.equal(q, one.expand(5, -1, -1))
+    over = torch.zeros(5 * 8 + HEADS * D).bfloat16().as_strided((5, HEADS, D), (8, D, 1))
+    assert kv_fp8._check_queries(over, cache, None)[1] == HEADS * D
+    wide = torch.zeros(5, 3 * HEADS, D).bfloat16()[:, HEADS:2 * HEADS]
+    assert kv_fp8._check_queries(wide, cache, None)[0] is wide                # rows of their own stay where they are
+
+
+@pytest.mark.parametrize("what", ["decode", "chunk"])
+def test_outputs_over_one_another_are_refused(what):
+    cache = kv_fp8.Fp8KVCache.zeros(4, H, D, device="cpu")
+    q, table, n = torch.zeros(B, HEADS, D).bfloat16(), torch.zeros(B, 1, dtype=torch.int32), torch.ones(B, dtype=torch.int32)
+    plan = kv_fp8.ChunkPlan.build([1] * B, [1] * B, table.numpy(), HEADS, cache)
+    for out in (q[:1].clone().expand(B, -1, -1), torch.zeros(2 * 64 + HEADS * D).bfloat16().as_strided((B, HEADS, D), (64, D, 1))):
+        with pytest.raises(ValueError, match="out must"):
+            kv_fp8.decode_attention(q, cache, table, n, out=out) if what == "decode" else kv_fp8.chunk_attention(q, cache, plan, out=out)
+    one = q[:1].clone().expand(B, -1, -1)[:1]                                    # a single row has no neighbour
+    kv_fp8.decode_attention(q[:1], cache, table[:1], n[:1], out=one)
