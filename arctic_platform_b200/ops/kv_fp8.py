@@ -36,15 +36,16 @@ _FN: Dict[str, object] = {}
 
 def _fn(name: str):
     if not _FN:
-        c = ctypes
+        c, fns = ctypes, {}
         vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
-        _FN["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
-        _FN["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
-        _FN["qkv"] = _lib.declare("apb_kv8_qkv_post", [vp, ll] + [vp] * 8 + [i, i, i, i, i, i, f, vp])
-        _FN["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, i, f, vp, vp])
-        _FN["scratch"] = _lib.declare("apb_kv8_decode_scratch", [i, i, i, i, i], ll)
-        _FN["few"] = _lib.declare("apb_kv8_few", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, ll, i, i, i, i, i, i, f, vp])
-        _FN["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, vp, i, vp, i, i, i, vp, vp, ll, i, i, i, i, f, vp])
+        fns["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
+        fns["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
+        fns["qkv"] = _lib.declare("apb_kv8_qkv_post", [vp, ll] + [vp] * 8 + [i, i, i, i, i, i, f, vp])
+        fns["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, i, f, vp, vp])
+        fns["scratch"] = _lib.declare("apb_kv8_decode_scratch", [i, i, i, i, i], ll)
+        fns["few"] = _lib.declare("apb_kv8_few", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, ll, i, i, i, i, i, i, f, vp])
+        fns["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, vp, i, vp, i, i, i, vp, vp, ll, i, i, i, i, f, vp])
+        _FN.update(fns)              # in one step: another thread may be looking
     return _FN[name]
 
 

@@ -1,4 +1,6 @@
 """Arguments of the 8-bit cache's operators that a kernel would take on trust: what is refused on the host, without a GPU."""
+import threading
+
 import pytest
 import torch
 
@@ -59,3 +61,26 @@ def test_outputs_over_one_another_are_refused(what):
             kv_fp8.decode_attention(q, cache, table, n, out=out) if what == "decode" else kv_fp8.chunk_attention(q, cache, plan, out=out)
     one = q[:1].clone().expand(B, -1, -1)[:1]                                    # a single row has no neighbour
     kv_fp8.decode_attention(q[:1], cache, table[:1], n[:1], out=one)
+
+
+def test_two_threads_may_make_the_first_call(monkeypatch):
+    """The table of the kernels' entry points is there as a whole or not at all."""
+    monkeypatch.setattr(kv_fp8, "_FN", {})
+    half_way, go_on = threading.Event(), threading.Event()
+
+    def declare(name, *types):
+        if threading.current_thread() is first and name == "apb_kv8_read":
+            half_way.set()
+            go_on.wait(10)
+        return name
+
+    monkeypatch.setattr(kv_fp8._lib, "declare", declare)
+    first = threading.Thread(target=lambda: kv_fp8._fn("write"))
+    first.start()
+    try:
+        assert half_way.wait(10)
+        assert kv_fp8._fn("chunk") == "apb_kv8_chunk"
+    finally:
+        go_on.set()
+        first.join()
+    assert kv_fp8._fn("write") == "apb_kv8_write"
