@@ -30,15 +30,9 @@ class TableError(ValueError):
 _forced: Optional[bool] = None
 
 
-# what lies under os.environ, by bytes: a look into it costs a fifth of os.environ.get, which every call of an operator would pay
-_environ = getattr(os.environ, "_data", None) if os.name == "posix" else None
-
-
 def enabled() -> bool:
     if _forced is not None:
         return _forced
-    if isinstance(_environ, dict):
-        return _environ.get(b"APB_DEBUG_CHECKS", b"0") not in (b"0", b"", b"false", b"False")
     return os.environ.get("APB_DEBUG_CHECKS", "0") not in ("0", "", "false", "False")
 
 
