@@ -42,6 +42,8 @@ struct Kv8Decode {
   float scale_log2;
   int* status;
   const int* starts;         // ROWS [B + 1]: where the query tokens of a sequence begin in q and out
+  const int* active;         // null, or [B]: sequences that are taken as empty where it is not above 0
+  __device__ __forceinline__ int length(int b) const { return active && active[b] <= 0 ? 0 : lengths[b]; }
 };
 
 constexpr float kKv8Top = 14.f;          // log2 of the largest weight and (about) of the largest query element
@@ -342,7 +344,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decode p) {
     const int t = token_of(head);
     return (token0 + t) * ld + (kvh * R + group * Cfg::kHeads + head - t * R) * D;
   };
-  int len = p.lengths[b];
+  int len = p.length(b);
   if (len > p.max_pages * kKv8Page) {
     if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kBadTable);
     len = p.max_pages * kKv8Page;
@@ -524,7 +526,7 @@ kv8_decode_stream_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decod
   }
   pdl_entry();
 
-  auto tokens_of = [&](int b) { return min(max(p.lengths[b], 0), p.max_pages * kKv8Page); };
+  auto tokens_of = [&](int b) { return min(max(p.length(b), 0), p.max_pages * kKv8Page); };
   auto pages_of = [&](int b) { return (tokens_of(b) + kKv8Page - 1) / kKv8Page; };
   int from, to, share;        // this share; pages of all but the last ones
   {
@@ -532,7 +534,7 @@ kv8_decode_stream_kernel(const __grid_constant__ CUtensorMap map, const Kv8Decod
     int mine = 0;
     for (int b = b0; b < b1; ++b) {
       mine += pages_of(b);
-      if (p.lengths[b] > p.max_pages * kKv8Page && p.status) atomicCAS(p.status, 0, kBadTable);
+      if (p.length(b) > p.max_pages * kKv8Page && p.status) atomicCAS(p.status, 0, kBadTable);
     }
     int end = mine;
 #pragma unroll
@@ -806,9 +808,9 @@ long long apb_kv8_decode_scratch(int B, int longest, int Hq, int Hkv, int D) {
   return unit <= shares ? 0 : static_cast<long long>(places) * (2 * 8 * H * (D + 4) * 4 + 16);
 }
 
-// scratch: null, or what apb_kv8_decode_scratch says
+// scratch: null, or what apb_kv8_decode_scratch says; active: null, or [B], sequences without are taken as empty
 int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* table, long long ld_table, int max_pages, int pages,
-                   const int* lengths, void* out, long long ldo, int B, int longest, int Hq, int Hkv, int D, float scale,
+                   const int* lengths, const int* active, void* out, long long ldo, int B, int longest, int Hq, int Hkv, int D, float scale,
                    void* scratch, cudaStream_t s) {
   if (B <= 0) return 0;
   if ((D != 64 && D != 128) || Hkv < 1 || Hq % Hkv || pages < 1 || max_pages < 0 || static_cast<long long>(pages) * Hkv >= (1ll << 31) - 1 ||
@@ -822,7 +824,8 @@ int apb_kv8_decode(const void* q, long long ldq, const void* data, const int* ta
   const int rc = kv8_map(&map, data, D, static_cast<long long>(pages) * Hkv);
   if (rc) return 1000 + rc;
   Kv8Decode p = {static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const uint8_t*>(data), table, ld_table, max_pages, pages, lengths,
-                 static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, groups, 1, scale * 1.4426950408889634f, status_device_ptr(), nullptr};
+                 static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, groups, 1, scale * 1.4426950408889634f, status_device_ptr(), nullptr,
+                 active};
   if (scratch && units * max_pages < (1ll << 30)) {          // shares count pages in 32 bits, of as many as a table could name
     const long long rows = static_cast<long long>(kv8_stream_ctas(H)) * 2 * 8 * H;
     Kv8Parts parts;
@@ -857,7 +860,7 @@ int apb_kv8_few(const void* q, long long ldq, const void* data, const int* table
   if (rc) return 1000 + rc;
   Kv8Decode p = {static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const uint8_t*>(data), table, ld_table, max_pages, pages, lengths,
                  static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, 1, kv8_splits(units, longest),
-                 scale * 1.4426950408889634f, status_device_ptr(), starts};
+                 scale * 1.4426950408889634f, status_device_ptr(), starts, nullptr};
   if (units * p.splits >= (1ll << 31)) return kBadArgument;
   if (D == 128) return rows <= 8 ? launch_kv8_decode<128, 1, 4, true>(map, p, s) : launch_kv8_decode<128, 2, 4, true>(map, p, s);
   return rows <= 8 ? launch_kv8_decode<64, 1, 4, true>(map, p, s) : launch_kv8_decode<64, 2, 4, true>(map, p, s);

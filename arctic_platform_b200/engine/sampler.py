@@ -492,7 +492,7 @@ class SamplerEngine:
         scale = 1.0 / math.sqrt(c.head_dim)
         if self.kv_fp8:
             return kv_fp8.decode_attention(q.view(B, c.num_heads, c.head_dim), self._kv8[li], self.d_page_table[:B], self.d_len[:B], scale,
-                                           longest=self._longest)
+                                           longest=self._longest, active=self.d_active[:B])
         kc, vc = self.kcache[li], self.vcache[li]
         out = torch.empty((B, c.num_heads, c.head_dim), device=self.device, dtype=torch.bfloat16)
         seq_splits = self._seq_splits(B)

@@ -41,7 +41,7 @@ def _fn(name: str):
         fns["write"] = _lib.declare("apb_kv8_write", [vp, ll, ll, vp, ll, ll, vp, vp, i, i, i, i, i, vp])
         fns["read"] = _lib.declare("apb_kv8_read", [vp, vp, vp, vp, i, i, i, i, i, vp])
         fns["qkv"] = _lib.declare("apb_kv8_qkv_post", [vp, ll] + [vp] * 8 + [i, i, i, i, i, i, f, vp])
-        fns["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, ll, i, i, i, i, i, f, vp, vp])
+        fns["decode"] = _lib.declare("apb_kv8_decode", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, ll, i, i, i, i, i, f, vp, vp])
         fns["scratch"] = _lib.declare("apb_kv8_decode_scratch", [i, i, i, i, i], ll)
         fns["few"] = _lib.declare("apb_kv8_few", [vp, ll, vp, vp, ll, i, i, vp, vp, vp, ll, i, i, i, i, i, i, f, vp])
         fns["chunk"] = _lib.declare("apb_kv8_chunk", [vp, ll, vp, vp, ll, vp, vp, i, vp, i, i, i, vp, vp, ll, i, i, i, i, f, vp])
@@ -283,9 +283,9 @@ def attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, last: torch
     return o / torch.where(total == 0, 1.0, total).t()[..., None]
 
 
-def _refuse_tables(cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.Tensor, B: int) -> None:
+def _refuse_tables(cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.Tensor, B: int, what: str = "lengths") -> None:
     """Says what is wrong with a batch's tables."""
-    for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
+    for name, t, dims in (("page_table", page_table, 2), (what, lengths, 1)):
         if t.dtype is not torch.int32 or t.dim() != dims or t.shape[0] != B or (t.stride(dims - 1) != 1 and t.numel()):
             shape = f"[{B}, pages]" if dims == 2 else [B]
             raise ValueError(f"{name} must be int32 {shape} with neighbouring elements, got {t.dtype} {list(t.shape)}")
@@ -294,13 +294,14 @@ def _refuse_tables(cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.T
 
 
 def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None,
-                     out: Optional[torch.Tensor] = None, longest: Optional[int] = None) -> torch.Tensor:
+                     out: Optional[torch.Tensor] = None, longest: Optional[int] = None, active: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``q [B, Hq, D]`` bf16, one token per sequence, over the first ``lengths [B]`` (int32) tokens on the pages ``page_table
     [B, max_pages]`` (int32) -> ``[B, Hq, D]`` bf16; zeros for sequences of length 0.  Query head ``h`` reads key head
     ``h // (Hq // Hkv)``; ``scale``: of the scores, ``D ** -0.5`` if None.  Entries of the table behind a sequence's pages are not looked at.
 
     ``longest``: about how long the longest sequence is or will be, where the table is much wider than that; the kernel is chosen by it,
-    the result does not depend on it but for last bits."""
+    the result does not depend on it but for last bits.  ``active [B]`` int32: sequences where it is not above 0 are taken as empty, whatever
+    their length says."""
     q, ldq = _check_queries(q, cache, out)
     B, Hq, D = q.shape
     index = cache.index
@@ -309,29 +310,32 @@ def decode_attention(q: torch.Tensor, cache: Fp8KVCache, page_table: torch.Tenso
             or lengths.dtype is not torch.int32 or lengths.shape != (B,) or (lengths.stride(0) != 1 and B)
             or page_table.get_device() != index or lengths.get_device() != index):
         _refuse_tables(cache, page_table, lengths, B)
+    if active is not None and (active.dtype is not torch.int32 or active.shape != (B,) or (active.stride(0) != 1 and B)
+                               or active.get_device() != index):
+        _refuse_tables(cache, page_table, active, B, "active")
     data, scale = cache.data, D ** -0.5 if scale is None else float(scale)
     if checked.enabled() and checked.active_for(q):
-        checked.check_page_table("page_table", page_table, lengths, cache.num_pages, PAGE)
+        checked.check_page_table("page_table", page_table, lengths if active is None else lengths * (active > 0), cache.num_pages, PAGE)
     if out is None:
         out = _rows(B, Hq, D, data, torch.bfloat16)
     if B == 0:
         return out
     if index < 0:
-        for b, n in enumerate(lengths.tolist()):
+        for b, n in enumerate((lengths if active is None else lengths * (active > 0)).tolist()):
             k, v = context_ref(cache, page_table[b], n)
             out[b:b + 1] = attention_ref(q[b:b + 1].float(), k, v, torch.tensor([n - 1]), scale).to(q.dtype)
         return out
     if _elsewhere(cache):
         with torch.cuda.device(cache.index):
-            return decode_attention(q, cache, page_table, lengths, scale, out, longest)
+            return decode_attention(q, cache, page_table, lengths, scale, out, longest, active)
     if out.stride(0) % 8 or out.data_ptr() % 16:             # rows off the 16-byte boundaries: by way of a copy
-        return out.copy_(decode_attention(q, cache, page_table, lengths, scale, None, longest))
+        return out.copy_(decode_attention(q, cache, page_table, lengths, scale, None, longest, active))
     wide = page_table.shape[1]
     pages = wide if longest is None else min(wide, (longest + PAGE - 1) // PAGE)
     need = _fn("scratch")(B, pages, Hq, cache.num_kv_heads, D)
     scratch = torch.empty(need, device=data.device, dtype=torch.uint8) if need else None          # kept until the launch has been made
     _lib.check(_fn("decode")(q.data_ptr(), ldq, data.data_ptr(), page_table.data_ptr(), page_table.stride(0), wide, cache.num_pages,
-                             lengths.data_ptr(), out.data_ptr(), out.stride(0), B, pages, Hq, cache.num_kv_heads, D, scale,
+                             lengths.data_ptr(), _lib.ptr(active), out.data_ptr(), out.stride(0), B, pages, Hq, cache.num_kv_heads, D, scale,
                              _lib.ptr(scratch), _lib.stream_ptr()), "kv8_decode")
     return out
 

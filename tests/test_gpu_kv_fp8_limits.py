@@ -108,3 +108,26 @@ def test_one_query_for_all_tokens(monkeypatch, form, new):
     want = kv_fp8.chunk_attention(q.contiguous(), cache, plan)
     assert torch.equal(kv_fp8.chunk_attention(q, cache, plan), want)
     assert torch.equal(kv_fp8.decode_attention(q[:2], cache, table, n), kv_fp8.decode_attention(q[:2].contiguous(), cache, table, n))
+
+
+@pytest.mark.parametrize("longest", [None, 20000])
+@pytest.mark.parametrize("Hq,H,D", [(8, 2, 128), (12, 1, 128), (4, 4, 64)])
+def test_sequences_that_are_not_active_give_zeros(Hq, H, D, longest):
+    """Both kernels, captured: what is active is read when the call is replayed."""
+    lengths = [40, 0, 700, 3000, 16, 1] * 3
+    cache, table, n, _ = _filled(lengths, H, D, seed=2)
+    q = torch.randn((len(lengths), Hq, D), device="cuda", generator=_gen(2)).bfloat16()
+    active = torch.ones_like(n)
+    kv_fp8.decode_attention(q, cache, table, n, longest=longest, active=active)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kv_fp8.decode_attention(q, cache, table, n, longest=longest, active=active)
+    for pattern in ([1] * 18, [0, 1, 1, 0, 1, 1] * 3, [-1] * 18, [0] * 9 + [1] * 9):
+        active.copy_(torch.tensor(pattern))
+        graph.replay()
+        seen = n * (active > 0)
+        _close(out, *_want(q, cache, table, seen))
+        assert not out[seen == 0].any()
+        assert torch.equal(kv_fp8.decode_attention(q, cache, table, n, longest=longest, active=active), out)
+        assert torch.equal(kv_fp8.decode_attention(q, cache, table, seen, longest=longest), out)
+    _lib.check_status("decode")

@@ -84,3 +84,17 @@ def test_two_threads_may_make_the_first_call(monkeypatch):
         go_on.set()
         first.join()
     assert kv_fp8._fn("write") == "apb_kv8_write"
+
+
+def test_sequences_that_are_not_active_are_empty():
+    cache = kv_fp8.Fp8KVCache.zeros(4, H, D, device="cpu")
+    g = torch.Generator().manual_seed(0)
+    kv_fp8.write(*(torch.randn(40, H, D, generator=g) for _ in range(2)), torch.arange(40, dtype=torch.int32), cache)
+    q = torch.randn(B, HEADS, D, generator=g).bfloat16()
+    table, n = torch.arange(3, dtype=torch.int32).expand(B, 3), torch.tensor([40, 33, 7], dtype=torch.int32)
+    active = torch.tensor([1, 0, 2], dtype=torch.int32)
+    want = kv_fp8.decode_attention(q, cache, table, n * (active > 0))
+    assert torch.equal(kv_fp8.decode_attention(q, cache, table, n, active=active), want) and not want[1].any() and want[0].any()
+    for bad in (active.long(), active[:2], active.expand(B, B), torch.zeros(2 * B, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="active must"):
+            kv_fp8.decode_attention(q, cache, table, n, active=bad)
