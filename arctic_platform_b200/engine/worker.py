@@ -177,7 +177,7 @@ class EngineWorker:
                 max_seq_len=int(vc.get("max_model_len", 8192)),
                 cascade=bool((job_config.get("arctic_inference_config") or {}).get("zorro_inference", {}).get("enable", True)),
                 seed=seed, eos_token_id=vc.get("eos_token_id"), quantization=vc.get("quantization"),
-                **self._kv_cache_dtype(SamplerEngine, vc))
+                **self._kv_cache_dtype(SamplerEngine, vc, None if scorer else self.model_cfg.head_dim))
             if vc.get("enable_return_routed_experts"):
                 self.sampler.always_return_routing = True
             return True
@@ -232,16 +232,29 @@ class EngineWorker:
         return True
 
     @staticmethod
-    def _kv_cache_dtype(engine, vllm_config: Dict[str, Any]) -> Dict[str, Any]:
-        """``kv_cache_dtype`` for the engine that has it; of the others a request for 8 bits is reported and they keep the model's type."""
+    def _kv_cache_dtype(engine, vllm_config: Dict[str, Any], head_dim: Optional[int] = 128) -> Dict[str, Any]:
+        """``kv_cache_dtype`` for the engine that has it.  What cannot be served (another engine, another type, heads of another size) is
+        reported, and keys and values keep the model's type: configs that name it for other servers load here.  ``head_dim`` None: an engine
+        that only scores and stores next to nothing."""
+        from ..ops.kv_fp8 import DIMS
         from .sampler import SamplerEngine, kv_cache_in_fp8
         asked = vllm_config.get("kv_cache_dtype")
-        if engine is SamplerEngine:
+        plain = {"kv_cache_dtype": None} if engine is SamplerEngine else {}
+        why = None
+        try:
+            if not kv_cache_in_fp8(asked) or head_dim is None:
+                return plain
+            if engine is not SamplerEngine:
+                why = f"{engine.__name__} has no 8-bit cache"
+            elif head_dim not in DIMS:
+                why = f"the 8-bit cache holds heads of {DIMS[0]} or {DIMS[1]}, not {head_dim}"
+        except ValueError as e:
+            why = str(e)
+        if why is None:
             return {"kv_cache_dtype": asked}
-        if kv_cache_in_fp8(asked):
-            import logging
-            logging.getLogger(__name__).warning("kv_cache_dtype=%r: %s holds keys and values in the model's type", asked, engine.__name__)
-        return {}
+        import logging
+        logging.getLogger(__name__).warning("kv_cache_dtype=%r: %s; keys and values are held in the model's type", asked, why)
+        return plain
 
     def _initialize_tp_sampler(self, job_config, model, tp: int, dtype, seed) -> bool:
         """A sampling replica over ``tp`` consecutive ranks of the job: every rank keeps a head / column shard of the

@@ -98,3 +98,28 @@ def test_sequences_that_are_not_active_are_empty():
     for bad in (active.long(), active[:2], active.expand(B, B), torch.zeros(2 * B, dtype=torch.int32)[::2]):
         with pytest.raises(ValueError, match="active must"):
             kv_fp8.decode_attention(q, cache, table, n, active=bad)
+
+
+@pytest.mark.parametrize("asked,head_dim,served,reported", [
+    ("fp8", 128, "fp8", False), ("fp8_e4m3", 64, "fp8_e4m3", False), ("auto", 256, None, False), (None, 256, None, False), ("bfloat16", 128, None, False),
+    ("fp8_e5m2", 128, None, True), ("int8", 64, None, True), ("fp8", 256, None, True), ("fp8", 96, None, True), ("fp8", None, None, False)])
+def test_cache_types_that_are_not_served_are_reported(caplog, asked, head_dim, served, reported):
+    from arctic_platform_b200.engine.hybrid_sampler import HybridSampler
+    from arctic_platform_b200.engine.sampler import SamplerEngine
+    from arctic_platform_b200.engine.worker import EngineWorker
+    assert EngineWorker._kv_cache_dtype(SamplerEngine, {"kv_cache_dtype": asked}, head_dim) == {"kv_cache_dtype": served}
+    assert bool(caplog.records) == reported and all(repr(asked) in r.getMessage() for r in caplog.records)
+    caplog.clear()
+    assert EngineWorker._kv_cache_dtype(HybridSampler, {"kv_cache_dtype": asked}, head_dim) == {}
+    assert bool(caplog.records) == (reported or served is not None)
+
+
+@pytest.mark.parametrize("asked", ["fp8", "fp8_e5m2", "nonsense"])
+def test_a_job_whose_cache_type_is_not_served_runs(asked, caplog):
+    from arctic_platform_b200.rl import ArcticRLClientConfig, create_arctic_rl_client
+    client = create_arctic_rl_client(ArcticRLClientConfig(
+        comm_protocol="local", model_name="qwen3-tiny", training_gpus=1, sampling_gpus=1, colocate=True,
+        ds_config={"optimizer": {"params": {"lr": 1e-4}}}, vllm_config={"max_num_seqs": 4, "max_model_len": 64, "kv_cache_dtype": asked}))
+    client.call("sync_weights")
+    out = client.call("generate", [[1, 2, 3]], {"n": 1, "temperature": 0.0, "max_tokens": 2, "ignore_eos": True})
+    assert len(out[0]["token_ids"]) == 2 and repr(asked) in caplog.text
