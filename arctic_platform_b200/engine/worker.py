@@ -161,6 +161,7 @@ class EngineWorker:
             spec = self._speculative_setup(job_config, vc, dtype, seed) if not scorer else None
             if spec is not None:
                 from .speculative import SpeculativeSampler
+                self._kv_cache_dtype(SpeculativeSampler, vc)          # it has none
                 self.sampler = SpeculativeSampler(self.model_cfg, self.device, model=m, draft_model=spec["draft"],
                                                   num_speculative_tokens=spec["k"],
                                                   max_seq_len=int(vc.get("max_model_len", 8192)), seed=seed,
@@ -252,8 +253,7 @@ class EngineWorker:
             why = str(e)
         if why is None:
             return {"kv_cache_dtype": asked}
-        import logging
-        logging.getLogger(__name__).warning("kv_cache_dtype=%r: %s; keys and values are held in the model's type", asked, why)
+        logger.warning("kv_cache_dtype=%r: %s; keys and values are held in the model's type", asked, why)
         return plain
 
     def _initialize_tp_sampler(self, job_config, model, tp: int, dtype, seed) -> bool:

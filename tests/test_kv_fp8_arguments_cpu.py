@@ -123,3 +123,13 @@ def test_a_job_whose_cache_type_is_not_served_runs(asked, caplog):
     client.call("sync_weights")
     out = client.call("generate", [[1, 2, 3]], {"n": 1, "temperature": 0.0, "max_tokens": 2, "ignore_eos": True})
     assert len(out[0]["token_ids"]) == 2 and repr(asked) in caplog.text
+
+
+def test_a_draft_models_engine_says_that_it_has_no_8_bit_cache(caplog):
+    from arctic_platform_b200.rl import ArcticRLClientConfig, create_arctic_rl_client
+    client = create_arctic_rl_client(ArcticRLClientConfig(
+        comm_protocol="local", model_name="qwen3-tiny", training_gpus=1, sampling_gpus=1, colocate=True,
+        ds_config={"optimizer": {"params": {"lr": 1e-4}}}, vllm_config={"max_num_seqs": 4, "max_model_len": 64, "kv_cache_dtype": "fp8"},
+        arctic_inference_config={"speculative_decoding": {"model": "qwen3-tiny", "num_speculative_tokens": 2}}))
+    assert len(client.call("generate", [[1, 2, 3]], {"n": 1, "temperature": 0.0, "max_tokens": 2, "ignore_eos": True})[0]["token_ids"]) == 2
+    assert "SpeculativeSampler" in caplog.text and "'fp8'" in caplog.text
