@@ -759,10 +759,12 @@ static int launch_kv8_decode(const CUtensorMap& map, const Kv8Decode& p, cudaStr
 // Places of a table that count: as many as a sequence of up to 2^31 tokens has, so that their tokens fit 32 bits.
 static int table_width(int max_pages) { return max_pages < (1 << 27) ? max_pages : (1 << 27) - 1; }
 
-// CTAs that a unit is cut into, of 8 pages at least, as long as all have a place
-static int kv8_splits(long long units, int longest) {
+// CTAs that a unit is cut into, of more than 4 pages, as long as all have a place.  An SM holds 3 (registers), 2 of heads of 128 with rows of
+// several tokens in two groups.  Those in a second wave cost most of a walk: 10 x 4 tokens behind 1500, 32 / 8 heads of 128, 40 us as 320 CTAs
+// and 32 as 160; 20 x 4 56 and 36.
+static int kv8_splits(long long units, int longest, int places = 3) {
   int splits = 1;
-  while (splits < 8 && units * splits * 2 <= 3 * sm_count() && splits * 8 < longest) splits *= 2;
+  while (splits < 8 && units * splits * 2 <= places * sm_count() && splits * 8 < longest) splits *= 2;
   return splits;
 }
 static int kv8_stream_ctas(int H) { return sm_count() * (H == 1 ? 3 : 2); }
@@ -859,7 +861,7 @@ int apb_kv8_few(const void* q, long long ldq, const void* data, const int* table
   const int rc = kv8_map(&map, data, D, static_cast<long long>(pages) * Hkv);
   if (rc) return 1000 + rc;
   Kv8Decode p = {static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const uint8_t*>(data), table, ld_table, max_pages, pages, lengths,
-                 static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, 1, kv8_splits(units, longest),
+                 static_cast<__nv_bfloat16*>(out), ldo, B, Hq, Hkv, 1, kv8_splits(units, longest, rows > 8 && D == 128 ? 2 : 3),
                  scale * 1.4426950408889634f, status_device_ptr(), starts, nullptr};
   if (units * p.splits >= (1ll << 31)) return kBadArgument;
   if (D == 128) return rows <= 8 ? launch_kv8_decode<128, 1, 4, true>(map, p, s) : launch_kv8_decode<128, 2, 4, true>(map, p, s);

@@ -127,13 +127,14 @@ Deal deal(Form form, const int32_t* new_tokens, const int32_t* lengths, int n, i
 // Estimated time of apb_kv8_few, in microseconds: rounds in which the four warps of a CTA take two pages each, in waves where CTAs do not
 // all have a place, and what it takes besides.  Measured, few / items of one tile, 32 / 8 heads of 128: 8 rows 1 x 300 tokens 9 / 13 us, 16 x
 // 1500 18 / 27, 128 x 6000 207 / 417, 1 x 30000 37 / 34; 16 rows 16 x 300 19 / 13, 4 x 6000 23 / 26, 16 x 6000 55 / 68, 1 x 30000 48 / 35.
-double few_time(const int32_t* lengths, int n, int rows, int Hkv, int sms) {
+double few_time(const int32_t* lengths, int n, int rows, int Hkv, int D, int sms) {
   int64_t longest = 0;
   for (int s = 0; s < n; ++s) longest = std::max<int64_t>(longest, (lengths[s] + 15) / 16);
   const int64_t units = static_cast<int64_t>(n) * Hkv;
+  const int places = rows > 8 && D == 128 ? 2 : 3;          // CTAs of an SM, as kv8_splits has them
   int64_t splits = 1;
-  while (splits < 8 && units * splits * 2 <= 3 * sms && splits * 8 < longest) splits *= 2;
-  const double waves = units * splits / (static_cast<double>(sms) * (rows > 8 ? 2 : 3));
+  while (splits < 8 && units * splits * 2 <= places * sms && splits * 8 < longest) splits *= 2;
+  const double waves = units * splits / (static_cast<double>(sms) * places);
   return (rows > 8 ? 12.0 : 7.0) + (longest / (8.0 * splits)) * (waves > 1 ? waves + 0.25 : 1.0) * (rows > 8 ? 1.5 : 1.2);
 }
 }  // namespace
@@ -141,13 +142,13 @@ double few_time(const int32_t* lengths, int n, int rows, int Hkv, int sms) {
 extern "C" {
 
 // 1 where attention of few tokens of each sequence is sooner done without items, the way of decode attention (apb_kv8_few).
-int32_t apb_rt_kv8_few(const int32_t* new_tokens, const int32_t* lengths, int32_t n, int32_t Hq, int32_t Hkv, int32_t sms) {
+int32_t apb_rt_kv8_few(const int32_t* new_tokens, const int32_t* lengths, int32_t n, int32_t Hq, int32_t Hkv, int32_t D, int32_t sms) {
   if (n < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || sms < 1) return 0;
   const int R = Hq / Hkv;
   for (int s = 0; s < n; ++s)
     if (static_cast<int64_t>(new_tokens[s]) * R > 16) return 0;
   const int rows = n ? *std::max_element(new_tokens, new_tokens + n) * R : 0;
-  return few_time(lengths, n, rows, Hkv, sms) < deal(kDual, new_tokens, lengths, n, R, Hkv, sms).time;
+  return few_time(lengths, n, rows, Hkv, D, sms) < deal(kDual, new_tokens, lengths, n, R, Hkv, sms).time;
 }
 
 // new_tokens, lengths [n]; form: -1 the one that is sooner done (kDual where no sequence has two tiles, whatever is asked for); items [..][12],

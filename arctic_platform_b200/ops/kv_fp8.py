@@ -374,12 +374,12 @@ def _work(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: 
     return _Work(items, first[:int(counts[3]) + 1], joins, int(counts[2]), int(counts[3]), int(counts[4]))
 
 
-def _few(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: int) -> bool:
+def _few(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: int, head_dim: int = 128) -> bool:
     """Whether the tokens are so few that they go the way of decode attention."""
     fn = _lib.rt_lib().apb_rt_kv8_few
-    fn.argtypes, fn.restype = [ctypes.c_void_p] * 2 + [ctypes.c_int32] * 4, ctypes.c_int32
+    fn.argtypes, fn.restype = [ctypes.c_void_p] * 2 + [ctypes.c_int32] * 5, ctypes.c_int32
     new, lengths = np.ascontiguousarray(new, dtype=np.int32), np.ascontiguousarray(lengths, dtype=np.int32)
-    return bool(fn(new.ctypes.data, lengths.ctypes.data, len(new), heads, kv_heads, sms))
+    return bool(fn(new.ctypes.data, lengths.ctypes.data, len(new), heads, kv_heads, head_dim, sms))
 
 
 @dataclass
@@ -429,7 +429,7 @@ class ChunkPlan:
         if cache.index >= 0 and rows:
             sms = torch.cuda.get_device_properties(cache.data.device).multi_processor_count
             sizes = (new, lengths, heads, cache.num_kv_heads, sms)
-            if not _few(*sizes):
+            if not _few(*sizes, cache.head_dim):
                 plan.work = w = _work(*sizes, cache.head_dim)
             table = np.zeros((n, max(1, int(need.max()))), dtype=np.int32)
             for s in range(n):
