@@ -131,3 +131,30 @@ def test_sequences_that_are_not_active_give_zeros(Hq, H, D, longest):
         assert torch.equal(kv_fp8.decode_attention(q, cache, table, n, longest=longest, active=active), out)
         assert torch.equal(kv_fp8.decode_attention(q, cache, table, seen, longest=longest), out)
     _lib.check_status("decode")
+
+
+@pytest.mark.parametrize("T", [3, 5000])
+def test_rows_beside_slots_behind_the_cache_are_written(T):
+    """A row that cannot be written takes none with it: the others are in the cache as the plain expression has them."""
+    H, D = 2, 64
+    g = _gen(T)
+    k, v = (torch.randn((T, H, D), device="cuda", generator=g) for _ in range(2))
+    cache, host = kv_fp8.Fp8KVCache.zeros(T // 16 + 2, H, D), kv_fp8.Fp8KVCache.zeros(T // 16 + 2, H, D, device="cpu")
+    slots = torch.randperm(cache.num_pages * 16, device="cuda", generator=g)[:T].to(torch.int32)
+    bad = slots.clone()
+    bad[1::3] = torch.tensor([cache.num_pages * 16, (1 << 31) - 1], device="cuda", dtype=torch.int32).repeat(T)[:len(bad[1::3])]
+    there = torch.where(bad < cache.num_pages * 16, bad, -1)
+    kv_fp8.write(k.cpu(), v.cpu(), there.cpu(), host)
+    checked.force(False)
+    try:
+        kv_fp8.write(k, v, bad, cache)
+        with pytest.raises(_lib.KernelError, match="203"):
+            _lib.check_status("write")
+        rows = kv_fp8.read(cache, bad, torch.float32)
+        with pytest.raises(_lib.KernelError, match="203"):
+            _lib.check_status("read")
+    finally:
+        checked.force(None)
+    assert torch.equal(cache.data.cpu(), host.data) and host.data.any()
+    for x, y in zip(rows, kv_fp8.read(host, there.cpu(), torch.float32)):
+        assert torch.equal(x.cpu(), y)
