@@ -240,6 +240,12 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
     }
   };
 
+  // Commits arrive by themselves, in pairs from the partner's tensor core too: the block does not leave before the last ones have, those of
+  // every tile that is still in the ring (a slot that was never taken counts as given back).
+  auto ring_given_back = [&](int slot, uint32_t phase) {
+    for (int i = 0; i < kRing && wait(&kv_empty[slot], phase ^ 1, kTimeoutEmpty); ++i) next(slot, phase, kRing);
+  };
+
   auto convert = [&]() {
     // ---------------------------------------------------------------- codes to tiles
     const int part = warp - 4;
@@ -344,12 +350,7 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
         next(st, st_phase, kKcStages);
       }
     }
-    // Commits arrive by themselves, in pairs from the partner's tensor core too: the block does not leave before the last ones have, those
-    // of every tile that is still in the ring (a slot that was never taken counts as given back).
-    for (int i = 0; i < kRing && ok; ++i) {
-      ok = wait(&kv_empty[slot], phase ^ 1, kTimeoutEmpty);
-      next(slot, phase, kRing);
-    }
+    if (!PAIR && ok) ring_given_back(slot, phase);
   };
 
   if (warp < 4) {
@@ -556,11 +557,14 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
       for (int at = item0; at < item1; ++at) tiles += 2 * p.items[at].blocks;
       int slot = 0;
       uint32_t phase = 0;
-      for (int i = 0; i < tiles; ++i) {
-        if (!wait(&kv_made[slot], phase, kTimeoutFull)) break;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        ok = wait(&kv_made[slot], phase, kTimeoutFull);
+        if (!ok) break;
         if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&kv_full[slot]), 0));
         next(slot, phase, kRing);
       }
+      if (ok) ring_given_back(slot, phase);
     }
   } else if (warp < 4 + kConvert) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsConvert));
