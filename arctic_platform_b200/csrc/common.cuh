@@ -148,8 +148,9 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 // 2-D tiled load global -> shared of this CTA, completion on `bar`.  No
-// multicast qualifier is used anywhere in this package.  x is the innermost
-// (contiguous) coordinate and must make a 16-byte aligned start.
+// load of this package has a multicast qualifier (arrivals of tcgen05.commit
+// do).  x is the innermost (contiguous) coordinate and must make a 16-byte
+// aligned start.
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x,
                                             int y) {
   asm volatile(

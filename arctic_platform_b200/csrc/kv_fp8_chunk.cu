@@ -15,12 +15,12 @@
 // beside turning codes into tiles (3000 by one warpgroup), and the three wait for one another.  Hence the pair: its MMAs of 256 rows take
 // half of the keys and half of the values' columns from either CTA, so that each turns half of the codes.  And weights are taken
 // relative to a reference that stays while they fit (the softmax below), in one pass over the scores.  Both together took 512 new tokens
-// of a 16896-token conversation (32/8 heads of 128) from 181 to 156 us, 897 TFLOP/s; four prompts of up to 4096 tokens from 397 to 346
-// (one CTA per item with this softmax: 170 and 357).  The chain of a tile is what is left: 2300 clocks of softmax, 260 until the issuing
-// warp knows, 1470 until the next scores.  S in halves of 64 columns with buffers of their own was slower (an MMA of 64 columns takes 0.7
-// of one of 128), and so were two threads per row (171 us: they have to agree on the reference).  Looking for codes that are no numbers
-// costs 10 of the 156 us.
-// Short chunks (5 draft tokens: 27 us where the bytes take 4.8) have one tile of 20 rows, for which all codes are turned into tiles: two
+// of a 16896-token conversation (32/8 heads of 128) from 181 to 164 us, 851 TFLOP/s (one CTA per item with this softmax: 179); four prompts
+// of up to 4096 tokens from 397 to 357.  (156 and 347 before the pair's tiles were released at the cluster's scope, see the warp that
+// does it.)  The chain of a tile is what is left: 2300 clocks of softmax, 260 until the issuing warp knows, 1470 until the next scores.  S in
+// halves of 64 columns with buffers of their own was slower (an MMA of 64 columns takes 0.7 of one of 128), and so were two threads per
+// row (they have to agree on the reference: 171 us where this form took 148).  Looking for codes that are no numbers costs 10 us.
+// Short chunks (5 draft tokens: 28 us where the bytes take 4.8) have one tile of 20 rows, for which all codes are turned into tiles: two
 // warpgroups do that there (one: 31), 2000 clocks a block.  Of up to 16 rows most go the way of decode attention instead (apb_kv8_few).
 //
 // Items over long contexts are cut along the keys where there are too few to fill the GPU (csrc/runtime_kv8.cpp); their parts are
@@ -551,8 +551,8 @@ __global__ void __launch_bounds__(Kv8ChunkCfg<D, FORM>::kThreads, 1)
     } else if (PAIR && warp == 2) {
       // ---------------------------------------------------------------- tiles made, to the CTA that issues
       // Tiles are stores to shared memory that the products of another CTA's thread read: they have to be released at the cluster's scope.
-      // By the warps that make them that takes 1000 clocks a tile, for their own stores to settle (202 us for 148, 512 tokens behind 16384);
-      // a warp that has none passes on what it has acquired.
+      // By the warps that make them that takes 1000 clocks a tile, for their own stores to settle (512 tokens behind 16384: 202 us where no
+      // release took 148); a warp that has none passes on what it has acquired (164 where none took 156).
       int tiles = 0;
       for (int at = item0; at < item1; ++at) tiles += 2 * p.items[at].blocks;
       int slot = 0;

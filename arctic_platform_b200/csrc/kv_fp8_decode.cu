@@ -17,7 +17,7 @@
 // common to the lanes of a head while the walk lasts.
 //
 // Measured: 128 sequences of 1365 to 4096 tokens, 32 / 8 heads of 128, 127 us (5.6 TB/s, 0.85 of a copy; the copies alone take 113); 2 of
-// 36864, 32 / 4 heads, 22.9; 41 of 500 to 1500, 16 / 8 heads, 22.5; one of 384, 6.2.
+// 36864, 32 / 4 heads, 23.2; 41 of 500 to 1500, 16 / 8 heads, 22.7; one of 384, 6.3.
 #include <cuda_fp16.h>
 
 #include "host_utils.cuh"

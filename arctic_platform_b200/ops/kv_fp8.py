@@ -2,7 +2,7 @@
 
 A page of 16 tokens is a block of bytes per key head: 16 rows of ``D`` key codes (e4m3), 16 rows of value codes, 32 exponents.  A
 row of a token stands for ``code * 2^(byte - 127)``, the exponent being the least one, of -100 to 119, with which the row's largest
-magnitude is at most 448: half the bytes of bf16 and a 64th for ``D`` = 128, every value exactly a bf16 number and off by at most
+magnitude is at most 448: half the bytes of bf16 and a 128th of those for ``D`` = 128, every value exactly a bf16 number and off by at most
 2^-4 of itself (2^-10 of 2^exponent where it is smaller than 2^-6 of that).  A row's codes depend on that row alone: neither the
 order nor the portions in which a page is filled change what it holds.
 
@@ -384,7 +384,8 @@ def _few(new: np.ndarray, lengths: np.ndarray, heads: int, kv_heads: int, sms: i
 
 @dataclass
 class ChunkPlan:
-    """Tables of a step in which every sequence brings some tokens; made on the host once and used by all layers.
+    """Tables of a step in which every sequence brings some tokens; made on the host once and used by all layers.  They go to the cache's
+    device on the current stream.
 
     Sequence ``s`` has ``lengths[s]`` tokens in the cache, the last ``new[s]`` of which are its query rows (row ``i`` sees the tokens
     up to position ``lengths[s] - new[s] + i``; one below 0 sees nothing); the rows of the sequences follow one another."""
