@@ -178,7 +178,8 @@ class EngineWorker:
                 max_seq_len=int(vc.get("max_model_len", 8192)),
                 cascade=bool((job_config.get("arctic_inference_config") or {}).get("zorro_inference", {}).get("enable", True)),
                 seed=seed, eos_token_id=vc.get("eos_token_id"), quantization=vc.get("quantization"),
-                **self._kv_cache_dtype(SamplerEngine, vc, None if scorer else self.model_cfg.head_dim))
+                # (not every family has a head size; those that have none have engines of their own)
+                **self._kv_cache_dtype(SamplerEngine, vc, None if scorer else getattr(self.model_cfg, "head_dim", 0)))
             if vc.get("enable_return_routed_experts"):
                 self.sampler.always_return_routing = True
             return True
