@@ -196,9 +196,9 @@ __global__ void __launch_bounds__(256) kv8_qkv_post_kernel(const Kv8QkvPost p) {
   const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.H;
   const int pos = p.pos[t];
   const bool lost = static_cast<unsigned>(pos) >= static_cast<unsigned>(p.positions);      // the tables have no such row
-  const int slot = lost ? -1 : p.slots[t];
+  const int to = p.slots[t], slot = lost ? -1 : to;
   if (lost) {
-    if (p.status) atomicCAS(p.status, 0, kBadTable);
+    if (to >= 0 && p.status) atomicCAS(p.status, 0, kBadTable);          // of an idle row any position will do
 #pragma unroll
     for (int j = 0; j < E; ++j) a[j] = b[j] = 0.f;
   } else if (!is_v) {

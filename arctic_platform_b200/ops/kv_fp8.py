@@ -212,7 +212,8 @@ def norm_rope_write(acc: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: O
     """A decode step behind its qkv projection (CUDA only): ``acc [B, (heads + 2 * key heads) * D]`` fp32 sums, left as zeros for the next
     ones to be added to; RMSNorm per head (weights ``[D]`` bf16, or None) and rotate-half RoPE (``cos, sin [positions, D / 2]`` fp32) of
     q and k at ``positions [B]`` int32.  Returns q ``[B, heads, D]`` bf16; k and v are rounded to bf16 and written as :func:`write` does.
-    A position that the tables do not have is reported (:func:`_lib.check_status`): its q is zeros, its k and v are not written."""
+    A position that the tables do not have gives zeros for q, and k and v are not written; it is reported (:func:`_lib.check_status`) where the
+    row has a slot."""
     _check_slots(cache, slots, True)
     data, B, H, D = cache.data, slots.shape[0], cache.num_kv_heads, cache.head_dim
     width = (heads + 2 * H) * D
@@ -232,7 +233,7 @@ def norm_rope_write(acc: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: O
     if cache.index < 0:
         raise ValueError("norm_rope_write runs on a GPU")
     if checked.enabled() and checked.active_for(positions):
-        checked.check_range("positions", positions, 0, cos.shape[0])
+        checked.check_range("positions", positions, 0, cos.shape[0], where=slots >= 0)
     if _elsewhere(cache):
         with torch.cuda.device(cache.index):
             return norm_rope_write(acc, q_norm, k_norm, rope, positions, slots, cache, heads, eps)
@@ -453,7 +454,8 @@ def chunk_attention(q: torch.Tensor, cache: Fp8KVCache, plan: ChunkPlan, scale: 
     """``q [T, Hq, D]`` bf16, the new tokens of the plan's sequences one behind another -> ``[T, Hq, D]`` bf16.  Each row sees the
     tokens of its sequence up to itself (:class:`ChunkPlan`), rows that see nothing are zeros.  Rows of ``q`` behind the last
     sequence are padding: they are left as they were in ``out``, zeros without it.  The new tokens' own keys and values are read from the
-    cache: :func:`write` comes first.  Values whose tokens' exponents lie more than 100 below the largest of their sequence lose bits.
+    cache: :func:`write` comes first.  Rows of the cache whose exponents lie more than 100 below the largest of their sequence (values) or of
+    their 128 tokens (keys) lose bits.
     A key that is no number reaches the rows that see it, such a value that column of its sequence's rows, those in front of it too.  A
     captured call reads the plan's tables when it is replayed: the plan has to live as long."""
     q, ldq = _check_queries(q, cache, out)

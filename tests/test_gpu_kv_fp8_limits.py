@@ -158,3 +158,22 @@ def test_rows_beside_slots_behind_the_cache_are_written(T):
     assert torch.equal(cache.data.cpu(), host.data) and host.data.any()
     for x, y in zip(rows, kv_fp8.read(host, there.cpu(), torch.float32)):
         assert torch.equal(x.cpu(), y)
+
+
+@pytest.mark.parametrize("check", [False, True])
+def test_an_idle_row_may_have_any_position(check):
+    B, Hq, H, D = 3, 4, 2, 64
+    g = _gen(1)
+    sums = torch.randn((B, (Hq + 2 * H) * D), device="cuda", generator=g)
+    angle = torch.randn((9, D // 2), device="cuda", generator=g)
+    rope = angle.cos().contiguous(), angle.sin().contiguous()
+    slots = torch.tensor([4, -1, -1], device="cuda", dtype=torch.int32)
+    caches = [kv_fp8.Fp8KVCache.zeros(1, H, D) for _ in range(2)]
+    checked.force(check)
+    try:
+        a, b = (kv_fp8.norm_rope_write(sums.clone(), None, None, rope, torch.tensor(p, device="cuda", dtype=torch.int32), slots, c, Hq, 1e-6)
+                for p, c in (([8, 9, -5], caches[0]), ([8, 0, 0], caches[1])))
+    finally:
+        checked.force(None)
+    _lib.check_status("step")
+    assert torch.equal(a[0], b[0]) and not a[1:].any() and torch.equal(caches[0].data, caches[1].data) and caches[0].data.any()
