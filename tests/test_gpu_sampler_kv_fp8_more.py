@@ -48,7 +48,7 @@ def _force(eng, tokens):
 
 
 @pytest.mark.parametrize("preset,quantization", [("qwen3-tiny-d128", None), ("qwen3-moe-tiny", None), ("tiny-fp8", "fp8")])
-def test_every_step_of_rollouts_that_are_fed_the_same_tokens(preset, quantization):
+def test_every_step_of_rollouts_that_are_fed_the_same_tokens(monkeypatch, preset, quantization):
     """An engine on the 8-bit cache beside one that holds the same numbers in bf16, past several borders of pages.
 
     The first layer's keys and values depend on the fed tokens alone: what the cache holds of them is equal to the last bit, for every slot of
@@ -60,7 +60,7 @@ def test_every_step_of_rollouts_that_are_fed_the_same_tokens(preset, quantizatio
     from arctic_platform_b200.models import config
     from arctic_platform_b200.ops import _lib, kv_fp8
     if preset == "tiny-fp8":
-        config.PRESETS.setdefault(preset, dataclasses.replace(config.PRESETS["qwen3-tiny-d128"], intermediate_size=768, name=preset))
+        monkeypatch.setitem(config.PRESETS, preset, dataclasses.replace(config.PRESETS["qwen3-tiny-d128"], intermediate_size=768, name=preset))
     kw = {"use_cuda_graph": False, "split_k": False, "quantization": quantization}
     model, eng = _engine(preset, kv_cache_dtype="fp8", **kw)
     _, other = _engine(preset, model=model, cascade=False, **kw)
