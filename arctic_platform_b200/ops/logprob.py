@@ -11,6 +11,9 @@ Triton cross-entropy (arctic_platform/common/utils/tiled_logits.py:74-139), chun
 (``:178-237``) and a recompute-in-backward autograd function (``:240-378``).
 
 CPU tensors use the chunked fp32 expression below (the oracle for the GPU tests).
+
+``top_logprobs(logits, k)`` gives the ``k`` most likely tokens of rows of logits in one pass over them (``csrc/top_logprobs.cu``): what scoring
+with ``top_k`` answers and what a teacher hands to :mod:`.distill`.
 """
 from __future__ import annotations
 
@@ -166,3 +169,71 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
     it_s = 1.0 if it_t is not None else float(inv_temperature)
     lp, ent, _ = _LmHeadLogprobFn.apply(hidden, weight, labels, it_t, it_s, with_entropy, bwd_chunk)
     return lp, (ent if with_entropy else None)
+
+
+# ----------------------------------------------------------------------------- the most likely tokens
+MOST_TOP = 1024                                          # tokens of a row that one pass finds
+_TOP_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_TOP = None
+
+
+def _top_fn():
+    global _TOP
+    if _TOP is None:
+        c = ctypes
+        _TOP = _lib.declare("apb_top_logprobs", [c.c_void_p, c.c_int, c.c_longlong, c.c_void_p, c.c_float, c.c_int, c.c_int, c.c_int, c.c_void_p,
+                                                 c.c_void_p, c.c_void_p, c.c_void_p])
+    return _TOP
+
+
+def top_logprobs_ref(logits, k: int, inv_temperature=1.0, dtype: torch.dtype = torch.float32):
+    """:func:`top_logprobs` as an expression in ``dtype``."""
+    z = logits.to(dtype)
+    z = torch.where(torch.isnan(z), float("-inf"), z)
+    z, ids = torch.sort(z, dim=-1, descending=True, stable=True)
+    it = inv_temperature.to(dtype)[:, None] if torch.is_tensor(inv_temperature) else float(inv_temperature)
+    x = torch.where(z == z[:, :1], 0.0, (z - torch.where(torch.isneginf(z[:, :1]), 0.0, z[:, :1])) * it)
+    x = torch.where(torch.isneginf(z), float("-inf"), x)
+    lse = torch.logsumexp(x, -1, keepdim=True)
+    lp = torch.where(torch.isneginf(lse), float("-inf"), x - lse)
+    named = lp[:, :k].exp().sum(-1)                      # next to a logarithm of 1 its difference from 1 says more
+    rest = torch.logsumexp(lp[:, k:], -1) if k < z.shape[1] else torch.full_like(named, float("-inf"))
+    rest = torch.where((named < 0.5) & ~torch.isneginf(lse[:, 0]), torch.log1p(-named), rest)
+    return lp[:, :k].float(), ids[:, :k].to(torch.int32), rest.float()
+
+
+@torch.no_grad()
+def top_logprobs(logits: torch.Tensor, k: int, inv_temperature=1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``logits [N, V]`` (fp32, bf16 or fp16; rows may be strided) -> ``(logprobs [N, k] fp32, ids [N, k] int32, rest [N] fp32)``: of
+    ``softmax(logits * inv_temperature)`` the ``k`` most likely tokens, best first and the lowest index first where logits are equal, and the log
+    of the mass of all others (``-inf`` for ``k = V``).  ``inv_temperature``: a positive number, or one per row.  Logits that are
+    not numbers count as ``-inf``; a row without any above that has log-probabilities and rest of ``-inf``.  On a GPU ``k`` is at
+    most 1024."""
+    if logits.dim() != 2 or logits.dtype not in _TOP_TYPES:
+        raise ValueError(f"logits must be fp32, bf16 or fp16 [N, V], got {logits.dtype} {list(logits.shape)}")
+    N, V = logits.shape
+    k = int(k)
+    if not 1 <= k <= V:
+        raise ValueError(f"k = {k} of {V} tokens")
+    if torch.is_tensor(inv_temperature):
+        if inv_temperature.shape != (N,) or inv_temperature.device != logits.device:
+            raise ValueError(f"inv_temperature must be a number or [{N}] on {logits.device}")
+    elif not float(inv_temperature) > 0:
+        raise ValueError(f"inv_temperature must be positive, got {inv_temperature}")
+    if not logits.is_cuda:
+        return top_logprobs_ref(logits, k, inv_temperature)
+    if k > MOST_TOP:
+        raise ValueError(f"k = {k}: at most {MOST_TOP} on a GPU")
+    if logits.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(logits.device):
+            return top_logprobs(logits, k, inv_temperature)
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    per_row = inv_temperature.to(torch.float32).contiguous() if torch.is_tensor(inv_temperature) else None
+    lp = torch.empty((N, k), device=logits.device, dtype=torch.float32)
+    ids = torch.empty((N, k), device=logits.device, dtype=torch.int32)
+    rest = torch.empty(N, device=logits.device, dtype=torch.float32)
+    _lib.check(_top_fn()(logits.data_ptr(), _TOP_TYPES[logits.dtype], logits.stride(0), _lib.ptr(per_row),
+                         1.0 if per_row is not None else float(inv_temperature), N, V, k, lp.data_ptr(), ids.data_ptr(), rest.data_ptr(),
+                         _lib.stream_ptr()), "apb_top_logprobs")
+    return lp, ids, rest
