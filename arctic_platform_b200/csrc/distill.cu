@@ -1,0 +1,313 @@
+// Distillation from a teacher's most likely tokens through the lm head, around the two vocabulary products of the log-prob head.
+//
+// A row names K tokens with the teacher's log-probabilities lq, and may give the log of the mass of all other tokens, lqr.  With the
+// student's p = softmax(z), z = hidden @ weight^T * scale, and its mass pr of the tokens not named, over the K (+ 1) classes
+//   F = sum q (lq - lp) (+ qr (lqr - lpr)),   R = sum p (lp - lq) (+ pr (lpr - lqr)),   value = (1 - mix) F + mix R.
+// With Q = sum q (+ qr) and E = sum p (lp - lq + 1) (+ pr (lpr - lqr + 1)):
+//   d value / d z_v = (1 - mix) (p_v Q - q_v) + mix p_v (lp_v - lq_v + 1 - E)     for a named token,
+//                   = p_v c,  c = (1 - mix) (Q - qr / pr) + mix (lpr - lqr + 1 - E)  for any other (without the class of the others
+//                                                                                  qr / pr = 0 and lpr - lqr + 1 = 0).
+// So the rows' gradient is dense only as a multiple of p, which is what the log-prob head's backward epilogue writes; the K named places
+// (and the label's) are put over it afterwards.
+//
+//   named    one CTA per row: the row's names in rising order for the product's epilogue; logits of the named tokens and the label as
+//            dot products in fp32.  An entry below 0 or beyond the vocabulary names nothing, a token named again counts once, by
+//            its first entry.
+//   product  CTA pairs (gemm_tcgen05_2cta.cu), records of every 128 columns without the named ones
+//   combine  one warp per row: statistics, value, log-prob and entropy of the label's distribution, c and the named places' gradients
+//   rows     the coefficient of p that the backward product takes; places  the named places and the label's over its output
+//
+// Why the named logits are dot products of their own instead of columns taken out of the product's tiles: the tensor cores round their
+// running sums toward zero, 1e-6 of a logit at 2560 terms, all to one side; here a lane adds every 256th term and the warp joins.  The named
+// tokens carry nearly all of the mass, so values and log-probs are off by a quarter of what they were with all logits from the tiles.
+#include "common.cuh"
+#include "gemm_common.cuh"
+#include "host_utils.cuh"
+
+namespace apb {
+
+constexpr int kMostNamed = 256;
+constexpr int kNoName = 0x7fffffff;
+
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]));
+    const float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[i]));
+    s = fmaf(f.x, g.x, s);
+    s = fmaf(f.y, g.y, s);
+  }
+  return s;
+}
+
+// names [N, K] as given; sorted [N, K]; logit [N, K + 1]: of every entry (-inf where it names nothing), then of the label.
+__global__ void __launch_bounds__(256)
+distill_named_kernel(const __nv_bfloat16* __restrict__ hidden, long long ldh, const __nv_bfloat16* __restrict__ weight, long long ldw,
+                     const int* __restrict__ names, const int* __restrict__ labels, const float* __restrict__ row_scale, float scale, int K,
+                     int V, int H, int* __restrict__ sorted, float* __restrict__ logit) {
+  __shared__ int name[kMostNamed];
+  __shared__ int kept[kMostNamed];
+  const long long row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < K) {
+    const int id = names[row * K + tid];
+    name[tid] = id >= 0 && id < V ? id : kNoName;
+  }
+  __syncthreads();
+  if (tid < K) {
+    int id = name[tid];
+    for (int j = 0; j < tid; ++j)
+      if (name[j] == id) id = kNoName;
+    kept[tid] = id;
+  }
+  __syncthreads();
+  if (tid < K) {
+    const int id = kept[tid];
+    int rank = 0;
+    for (int j = 0; j < K; ++j) rank += kept[j] < id || (kept[j] == id && j < tid);
+    sorted[row * K + rank] = id;
+  }
+  const float rs = scale * (row_scale ? row_scale[row] : 1.f);
+  const uint4* h = reinterpret_cast<const uint4*>(hidden + row * ldh);
+  const int chunks = H / 8;
+  for (int k = warp; k <= K; k += 8) {
+    const int id = k < K ? kept[k] : labels[row];
+    float s = 0.f;
+    const bool there = id >= 0 && id < V;
+    if (there) {
+      const uint4* w = reinterpret_cast<const uint4*>(weight + static_cast<long long>(id) * ldw);
+      for (int c = lane; c < chunks; c += 32) s = dot8(h[c], w[c], s);
+      s = warp_sum(s);
+    }
+    if (lane == 0) logit[row * (K + 1) + k] = there ? s * rs : -INFINITY;
+  }
+}
+
+struct DistillRows {
+  const float4* partial;     // [N][tiles] records of the columns not named
+  const float* logit;        // [N, K + 1]
+  const float* teacher;      // [N, K] log-probabilities
+  const float* rest;         // [N] log of the others' mass, or null
+  float* value;              // [N]
+  float* lp;
+  float* ent;
+  float* lse;
+  float* others;             // c: d value / d z of a token not named is this times its probability
+  float* named_grad;         // [N, K] d value / d z of the named ones
+  int tiles, K, N;
+  float mix;
+};
+
+// x * y, 0 where x is: a class without mass adds nothing, whatever its logarithm is
+__device__ __forceinline__ float mass_times(float x, float y) { return x > 0.f ? x * y : 0.f; }
+
+__global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows a) {
+  const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (row >= a.N) return;
+  const float4* pr = a.partial + static_cast<long long>(row) * a.tiles;
+  const float* zk = a.logit + static_cast<long long>(row) * (a.K + 1);
+  const float* lq = a.teacher + static_cast<long long>(row) * a.K;
+  float m = -INFINITY, s = 0.f, e = 0.f;                // of the tokens not named
+  for (int t = lane; t < a.tiles; t += 32) {
+    const float4 v = pr[t];
+    const float mn = fmaxf(m, v.x);
+    const float c0 = m == -INFINITY ? 0.f : __expf(m - mn), c1 = v.x == -INFINITY ? 0.f : __expf(v.x - mn);
+    s = s * c0 + v.y * c1;
+    e = e * c0 + v.z * c1;
+    m = mn;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o), e2 = __shfl_xor_sync(0xffffffffu, e, o);
+    const float mn = fmaxf(m, m2);
+    const float c0 = m == -INFINITY ? 0.f : __expf(m - mn), c1 = m2 == -INFINITY ? 0.f : __expf(m2 - mn);
+    s = s * c0 + s2 * c1;
+    e = e * c0 + e2 * c1;
+    m = mn;
+  }
+  float top = m;
+  for (int k = lane; k < a.K; k += 32) top = fmaxf(top, zk[k]);
+  top = warp_max(top);
+  float st = 0.f, et = 0.f;
+  for (int k = lane; k < a.K; k += 32) {
+    const float z = zk[k];
+    if (z == -INFINITY) continue;
+    const float x = expf(z - top);
+    st += x;
+    et += x * z;
+  }
+  st = warp_sum(st);
+  et = warp_sum(et);
+  const float shift = m == -INFINITY ? 0.f : expf(m - top);
+  const float sum = st + s * shift;
+  const float lse = top + logf(sum);
+  const float ent = lse - (et + e * shift) / sum;
+  // classes
+  const bool bucket = a.rest != nullptr;
+  const float lpr = s > 0.f ? m + logf(s) - lse : -INFINITY, pr_ = expf(lpr);
+  const float lqr = bucket ? a.rest[row] : -INFINITY, qr = expf(lqr);
+  float F = 0.f, R = 0.f, Q = 0.f, E = 0.f;
+  for (int k = lane; k < a.K; k += 32) {
+    const float z = zk[k];
+    if (z == -INFINITY) continue;
+    const float lp = z - lse, l = lq[k], q = expf(l);
+    F += mass_times(q, l - lp);
+    Q += q;
+    if (a.mix != 0.f) {
+      const float p = expf(lp);
+      R += mass_times(p, lp - l);
+      E += mass_times(p, lp - l + 1.f);
+    }
+  }
+  F = warp_sum(F);
+  Q = warp_sum(Q);
+  R = warp_sum(R);
+  E = warp_sum(E);
+  float c = 0.f;
+  if (bucket) {
+    F += mass_times(qr, lqr - lpr);
+    Q += qr;
+    // below the least normal number (87 below the largest logit) the others' probabilities are zeros to the product's epilogue as well
+    c = pr_ >= 1.18e-38f ? -(1.f - a.mix) * (qr / pr_) : 0.f;
+    if (a.mix != 0.f) {
+      R += mass_times(pr_, lpr - lqr);
+      E += mass_times(pr_, lpr - lqr + 1.f);
+      if (pr_ > 0.f) c += a.mix * (lpr - lqr + 1.f);
+    }
+  }
+  c += (1.f - a.mix) * Q;
+  if (a.mix != 0.f) c -= a.mix * E;
+  for (int k = lane; k < a.K; k += 32) {
+    const float z = zk[k];
+    float g = 0.f;
+    if (z != -INFINITY) {
+      const float lp = z - lse, p = expf(lp), l = lq[k];
+      g = (1.f - a.mix) * (p * Q - expf(l));
+      if (a.mix != 0.f) g += a.mix * mass_times(p, lp - l + 1.f - E);
+    }
+    a.named_grad[static_cast<long long>(row) * a.K + k] = g;
+  }
+  if (lane == 0) {
+    a.value[row] = a.mix == 0.f ? F : (1.f - a.mix) * F + a.mix * R;
+    a.lp[row] = zk[a.K] - lse;
+    a.ent[row] = ent;
+    a.lse[row] = lse;
+    a.others[row] = c;
+  }
+}
+
+// The upstream gradient of a log-prob that would give every token not named what it gets: minus the coefficient of its probability.
+__global__ void __launch_bounds__(256)
+distill_rows_kernel(const float* __restrict__ g_value, const float* __restrict__ g_lp, const float* __restrict__ others, int N,
+                    float* __restrict__ out, int* __restrict__ no_label) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= N) return;
+  const float g = g_value[i];
+  out[i] = (g_lp ? g_lp[i] : 0.f) - (g == 0.f ? 0.f : g * others[i]);
+  no_label[i] = -1;
+}
+
+// One warp per row: the places of the named tokens, and the label's, in d(logits) [N, V] bf16.
+__global__ void __launch_bounds__(256)
+distill_places_kernel(const int* __restrict__ names, const int* __restrict__ labels, const float* __restrict__ logit,
+                      const float* __restrict__ named_grad, const float* __restrict__ others, const float* __restrict__ lse,
+                      const float* __restrict__ ent, const float* __restrict__ g_value, const float* __restrict__ g_lp,
+                      const float* __restrict__ g_ent, const float* __restrict__ row_scale, float scale, int K, int V, int N,
+                      __nv_bfloat16* __restrict__ d, long long ldd) {
+  const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (row >= N) return;
+  const float* zk = logit + static_cast<long long>(row) * (K + 1);
+  const int label = labels[row];
+  const float rs = scale * (row_scale ? row_scale[row] : 1.f);
+  const float gv = g_value[row], gl = g_lp ? g_lp[row] : 0.f, ge = g_ent ? g_ent[row] : 0.f, l = lse[row], en = ent[row];
+  __nv_bfloat16* to = d + row * ldd;
+  bool label_named = false;
+  for (int k = lane; k < K; k += 32) {
+    if (zk[k] == -INFINITY) continue;
+    const int id = names[static_cast<long long>(row) * K + k];
+    const float lp = zk[k] - l, p = expf(lp);
+    float g = (gv == 0.f ? 0.f : gv * named_grad[static_cast<long long>(row) * K + k]) - gl * p - ge * mass_times(p, lp + en);
+    if (id == label) {
+      g += gl;
+      label_named = true;
+    }
+    to[id] = __float2bfloat16_rn(g * rs);
+  }
+  label_named = __any_sync(0xffffffffu, label_named);
+  if (lane == 0 && !label_named && label >= 0 && label < V) {
+    const float lp = zk[K] - l, p = expf(lp);
+    to[label] = __float2bfloat16_rn(((gv == 0.f ? 0.f : gv * others[row] * p) - gl * p - ge * mass_times(p, lp + en) + gl) * rs);
+  }
+}
+
+int launch_gemm_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& p, cudaStream_t stream);
+
+}  // namespace apb
+
+extern "C" {
+
+// hidden [N, H] and weight [V, H] bf16 (H, V and the strides multiples of 8, 16-byte aligned), labels [N], names [N, K] int32 (K <= 256),
+// teacher [N, K] fp32, rest [N] fp32 or null, row_scale [N] or null (then `scale` alone).  Scratch: sorted [N, K] int32, partial
+// [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1], named_grad [N, K], others, lse, ent [N].
+int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* labels, const int* names, const float* teacher,
+                           const float* rest, const float* row_scale, float* partial, int* sorted, float* logit, float* value, float* lp,
+                           float* ent, float* lse, float* others, float* named_grad, int N, int V, int H, int K, long long ldh,
+                           long long ldw, float scale, float mix, cudaStream_t stream) {
+  using namespace apb;
+  if (N <= 0) return 0;
+  if (!hidden || !weight || !labels || !partial || !value || !lp || !ent || !lse || !others || !logit || K < 0 || K > kMostNamed ||
+      (K > 0 && (!names || !teacher || !sorted || !named_grad)) || V <= 0 || H <= 0 || (H % 8) || (V % 8) || (ldh % 8) || (ldw % 8) ||
+      ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15))
+    return kBadArgument;
+  distill_named_kernel<<<N, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(hidden), ldh, static_cast<const __nv_bfloat16*>(weight),
+                                              ldw, names, labels, row_scale, scale, K, V, H, sorted, logit);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  CUtensorMap ta, tb;
+  int rc = make_tmap_2d(&ta, hidden, 2, N, H, ldh, 64, 128);
+  if (rc) return 1000 + rc;
+  rc = make_tmap_2d(&tb, weight, 2, V, H, ldw, 64, 128);
+  if (rc) return 2000 + rc;
+  GemmParams p{};
+  p.M = N;
+  p.N = V;
+  p.K = H;
+  p.epi = kEpiRestPartial;
+  p.splits = 1;
+  p.alpha = scale;
+  p.row_scale = row_scale;
+  p.partial = partial;
+  p.named = sorted;
+  p.n_named = K;
+  p.status = status_device_ptr();
+  rc = launch_gemm_pair(ta, tb, p, stream);
+  if (rc) return rc;
+  DistillRows a{reinterpret_cast<const float4*>(partial), logit, teacher, rest, value, lp, ent, lse, others, named_grad, (V + 127) / 128, K, N,
+                mix};
+  distill_combine_kernel<<<(N + 7) / 8, 256, 0, stream>>>(a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// glp [N] fp32 and no_label [N] int32: what apb_lmhead_dlogits takes in place of the log-prob's upstream gradient and the labels.
+int apb_distill_rows(const float* g_value, const float* g_lp, const float* others, int N, float* glp, int* no_label, cudaStream_t stream) {
+  using namespace apb;
+  if (N <= 0) return 0;
+  if (!g_value || !others || !glp || !no_label) return kBadArgument;
+  distill_rows_kernel<<<(N + 255) / 256, 256, 0, stream>>>(g_value, g_lp, others, N, glp, no_label);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// The named tokens' places and the label's of d [N, V] bf16 (row stride ldd); arguments as kept by the forward pass.
+int apb_distill_places(const int* names, const int* labels, const float* logit, const float* named_grad, const float* others, const float* lse,
+                       const float* ent, const float* g_value, const float* g_lp, const float* g_ent, const float* row_scale, float scale,
+                       int K, int V, int N, void* d, long long ldd, cudaStream_t stream) {
+  using namespace apb;
+  if (N <= 0) return 0;
+  if (!labels || !logit || !others || !lse || !ent || !g_value || !d || K < 0 || K > kMostNamed || (K > 0 && (!names || !named_grad)))
+    return kBadArgument;
+  distill_places_kernel<<<(N + 7) / 8, 256, 0, stream>>>(names, labels, logit, named_grad, others, lse, ent, g_value, g_lp, g_ent, row_scale,
+                                                         scale, K, V, N, static_cast<__nv_bfloat16*>(d), ldd);
+  return static_cast<int>(cudaGetLastError());
+}
+}

@@ -68,7 +68,7 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar_cluster_addr) {
 
 // What a variant of the kernel does with its accumulators.  A kernel holds one of them: with all in one kernel the unrolled code of
 // the untaken ones pushed the taken one out of the instruction cache (gate/up of 18432 tokens: 2.6 ms against 0.9).
-enum PairEpi : int { kPairBf16, kPairF32, kPairSwiGLU, kPairGeGLU, kPairClampGLU, kPairPartial, kPairDlogits };
+enum PairEpi : int { kPairBf16, kPairF32, kPairSwiGLU, kPairGeGLU, kPairClampGLU, kPairPartial, kPairDlogits, kPairRest };
 
 // 128 accumulator columns from `nb` on of the rows [row0, row0 + 32), this lane's row in `acc`.  Columns and rows outside the
 // output are clipped by the tensor maps; a box that would begin outside is not sent.
@@ -79,6 +79,8 @@ __device__ __forceinline__ void pair_epilogue(const GemmParams& p, const CUtenso
   const bool row_ok = row < p.M;
   if constexpr (EPI == kPairPartial) {
     lmhead_partial_128(p, row, row_ok, acc, nb);
+  } else if constexpr (EPI == kPairRest) {
+    lmhead_rest_128(p, row, row_ok, acc, nb);
   } else if constexpr (EPI == kPairF32) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -462,6 +464,7 @@ static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
     case kEpiClampGLU: return launch_pair_as<NT, kPairClampGLU>(ta, tb, tc, tc2, p, s);
     case kEpiLogprobPartial: return launch_pair_as<NT, kPairPartial>(ta, tb, tc, tc2, p, s);
     case kEpiDlogits: return launch_pair_as<NT, kPairDlogits>(ta, tb, tc, tc2, p, s);
+    case kEpiRestPartial: return launch_pair_as<NT, kPairRest>(ta, tb, tc, tc2, p, s);
     default: return kBadArgument;
   }
 }

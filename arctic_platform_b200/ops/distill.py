@@ -1,0 +1,206 @@
+"""Distillation from a teacher's most likely tokens, through the lm head and without a ``[N, V]`` logits tensor.
+
+``lm_head_distill(hidden, weight, labels, teacher_ids, teacher_logprobs, teacher_rest)`` compares, per row, the student's distribution
+``softmax(hidden @ weight^T * inv_temperature)`` with a teacher's, of which the log-probabilities of ``K`` tokens are known and, with
+``teacher_rest``, the log of the mass of all others, which then are one class more (:func:`~.logprob.top_logprobs` gives the three).  Over
+these classes, q the teacher's masses and p the student's, the divergence is ``(1 - reverse) KL(q, p) + reverse KL(p, q)``; without
+``teacher_rest`` both sums run over the named tokens alone (p stays normalised over the whole vocabulary).
+
+On CUDA the vocabulary product runs on tcgen05 CTA pairs with an epilogue that reduces every 128 columns to records without the named
+tokens, whose logits are fp32 dot products (``csrc/distill.cu``); the backward pass forms d(logits) in bf16 a chunk of rows at a time and feeds
+two products, as :func:`~.logprob.lm_head_logprobs` does.  CPU tensors use the fp32 expression below (the oracle of the GPU tests).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Dict, Optional, Tuple
+
+import torch
+
+from . import _lib, gemm
+from .logprob import _BWD_BUDGET, _BWD_ROWS, _bwd_rows
+from ..utils import memory_budget
+
+MOST_NAMED = 256        # tokens that a row may name
+
+_FN: Dict[str, object] = {}
+
+
+def _fn(name: str):
+    if not _FN:
+        c, fns = ctypes, {}
+        vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
+        fns["fwd"] = _lib.declare("apb_lmhead_distill_fwd", [vp] * 16 + [i, i, i, i, ll, ll, f, f, vp])
+        fns["rows"] = _lib.declare("apb_distill_rows", [vp, vp, vp, i, vp, vp, vp])
+        fns["places"] = _lib.declare("apb_distill_places", [vp] * 11 + [f, i, i, i, vp, ll, vp])
+        fns["dlogits"] = _lib.declare("apb_lmhead_dlogits", [vp] * 9 + [i, i, i, ll, ll, ll, f, vp])
+        _FN.update(fns)              # in one step: another thread may be looking
+    return _FN[name]
+
+
+def first_entries(ids: torch.Tensor, vocab: int) -> torch.Tensor:
+    """Which entries of ``ids [N, K]`` count: those that name a token of the vocabulary, of a token named again the first one."""
+    there = (ids >= 0) & (ids < vocab)
+    again = (ids[:, :, None] == ids[:, None, :]).tril(-1).any(-1)
+    return there & ~again
+
+
+def _times(x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+    """``x y``; 0, also in its gradients, where ``x`` is: a class without mass adds nothing, whatever its logarithm is."""
+    return torch.where(x > 0, x * torch.where(x > 0, y, 0.0), 0.0)
+
+
+def distill_ref(hidden, weight, labels, teacher_ids, teacher_logprobs, teacher_rest=None, inv_temperature=1.0, reverse: float = 0.0,
+                with_entropy: bool = True, dtype: torch.dtype = torch.float32):
+    """Differentiable expression of :func:`lm_head_distill` in ``dtype``."""
+    V = weight.shape[0]
+    it = inv_temperature.to(dtype)[:, None] if torch.is_tensor(inv_temperature) else float(inv_temperature)
+    z = (hidden.to(dtype) @ weight.to(dtype).t()) * it
+    log_p = torch.log_softmax(z, -1)
+    counts = first_entries(teacher_ids, V)
+    ids = torch.where(counts, teacher_ids, 0).long()
+    lq = torch.where(counts, teacher_logprobs.detach().to(dtype), 0.0)
+    q = torch.where(counts, lq.exp(), 0.0)
+    lp = torch.where(counts, log_p.gather(1, ids), 0.0)
+    p = torch.where(counts, lp.exp(), 0.0)
+    value = (1 - reverse) * _times(q, lq - lp).sum(-1)
+    if reverse:
+        value = value + reverse * _times(p, lp - lq).sum(-1)
+    if teacher_rest is not None:
+        lqr = teacher_rest.detach().to(dtype)
+        named = torch.zeros(z.shape, dtype=torch.bool, device=z.device)
+        rows = torch.arange(z.shape[0], device=z.device)[:, None].expand_as(ids)
+        named[rows[counts], ids[counts]] = True
+        left = ~named.all(-1)
+        lpr = torch.logsumexp(torch.where(named & left[:, None], float("-inf"), log_p), -1)
+        value = value + (1 - reverse) * _times(lqr.exp(), lqr - torch.where(left, lpr, float("-inf")))
+        if reverse:
+            value = value + reverse * _times(torch.where(left, lpr.exp(), 0.0), lpr - lqr)
+    lab = labels.long()
+    logprob = log_p.gather(1, lab[:, None]).squeeze(-1)
+    entropy = -(log_p.exp() * log_p).sum(-1) if with_entropy else None
+    return value, logprob, entropy
+
+
+class _LmHeadDistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, ids, teacher, rest, inv_temp_t, inv_temp_s, reverse, with_entropy, bwd_chunk):
+        N, H = hidden.shape
+        V, K = weight.shape[0], ids.shape[1]
+        f32 = dict(device=hidden.device, dtype=torch.float32)
+        partial = torch.empty((N, (V + 127) // 128, 4), **f32)
+        in_order = torch.empty((N, K), device=hidden.device, dtype=torch.int32)
+        logit, named = torch.empty((N, K + 1), **f32), torch.empty((N, K), **f32)
+        value, lp, ent, lse, others = torch.empty((5, N), **f32).unbind(0)
+        _lib.check(_fn("fwd")(_lib.ptr(hidden), _lib.ptr(weight), _lib.ptr(labels), _lib.ptr(ids), _lib.ptr(teacher), _lib.ptr(rest),
+                              _lib.ptr(inv_temp_t), _lib.ptr(partial), _lib.ptr(in_order), _lib.ptr(logit), _lib.ptr(value), _lib.ptr(lp),
+                              _lib.ptr(ent), _lib.ptr(lse), _lib.ptr(others), _lib.ptr(named), N, V, H, K, hidden.stride(0), weight.stride(0),
+                              inv_temp_s, reverse, _lib.stream_ptr()), "apb_lmhead_distill_fwd")
+        ctx.save_for_backward(hidden, weight, labels, ids, inv_temp_t, logit, named, others, lse, ent)
+        ctx.inv_temp_s, ctx.with_entropy, ctx.bwd_chunk = inv_temp_s, with_entropy, bwd_chunk
+        ctx.set_materialize_grads(False)
+        return value, lp, (ent if with_entropy else lp.new_zeros(0))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_value, g_lp, g_ent):
+        hidden, weight, labels, ids, it, logit, named, others, lse, ent = ctx.saved_tensors
+        N, H = hidden.shape
+        V, K = weight.shape[0], ids.shape[1]
+        dev = hidden.device
+        with torch.cuda.device(dev):
+            whole = lambda g: None if g is None else g.float().contiguous()                  # noqa: E731
+            g_value = torch.zeros(N, device=dev) if g_value is None else whole(g_value)
+            g_lp, g_ent = whole(g_lp), whole(g_ent) if ctx.with_entropy else None
+            glp = torch.empty(N, device=dev, dtype=torch.float32)
+            no_label = torch.empty(N, device=dev, dtype=torch.int32)
+            _lib.check(_fn("rows")(_lib.ptr(g_value), _lib.ptr(g_lp), _lib.ptr(others), N, _lib.ptr(glp), _lib.ptr(no_label),
+                                   _lib.stream_ptr()), "apb_distill_rows")
+            d_hidden = torch.empty((N, H), device=dev, dtype=hidden.dtype)
+            acc = getattr(weight, "grad_f32", None)
+            chunk = ctx.bwd_chunk
+            if chunk is None:
+                chunk = _bwd_rows(N, V, memory_budget.spare_bytes(dev, _BWD_BUDGET) if N > _BWD_ROWS else 0)
+            want_h, want_w = ctx.needs_input_grad[:2]
+            dw32 = None if not want_w else acc if acc is not None else torch.zeros((V, H), device=dev, dtype=torch.float32)
+            buf_rows = min(chunk, N) if ctx.bwd_chunk or N <= _BWD_ROWS else -(-chunk // _BWD_ROWS) * _BWD_ROWS
+            buf = torch.empty((buf_rows, V), device=dev, dtype=torch.bfloat16)
+            for s in range(0, N, chunk):
+                n = min(chunk, N - s)
+                rows = slice(s, s + n)
+                part = lambda t: _lib.ptr(None if t is None else t[rows])                     # noqa: E731
+                h, dl = hidden[rows], buf[:n]
+                _lib.check(_fn("dlogits")(_lib.ptr(h), _lib.ptr(weight), part(no_label), part(it), part(lse), part(ent), part(glp),
+                                          part(g_ent), _lib.ptr(dl), n, V, H, h.stride(0), weight.stride(0), dl.stride(0), ctx.inv_temp_s,
+                                          _lib.stream_ptr()), "apb_lmhead_dlogits")
+                _lib.check(_fn("places")(part(ids), part(labels), part(logit), part(named), part(others), part(lse), part(ent),
+                                         part(g_value), part(g_lp), part(g_ent), part(it), ctx.inv_temp_s, K, V, n, _lib.ptr(dl),
+                                         dl.stride(0), _lib.stream_ptr()), "apb_distill_places")
+                if not want_h:
+                    pass
+                elif -(-n // 256) * -(-H // 256) < torch.cuda.get_device_properties(dev).multi_processor_count // 2:
+                    # fewer tiles than CTA pairs: the vocabulary is cut into parts that add up in fp32, as in lm_head_logprobs
+                    total = torch.zeros((n, H), device=dev, dtype=torch.float32)
+                    gemm.gemm_raw(dl, weight, total, M=n, N=H, K=V, b_mn=True, epi=gemm.EPI_F32_ACCUM)
+                    d_hidden[rows].copy_(total)
+                else:
+                    gemm.matmul_nn(dl, weight, out=d_hidden[rows])
+                if want_w:
+                    gemm.matmul_tn(dl, h, out=dw32, accumulate=True)
+            dw = None if acc is not None or not want_w else dw32.to(weight.dtype)
+        return d_hidden if want_h else None, dw, None, None, None, None, None, None, None, None, None
+
+
+def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, teacher_ids: torch.Tensor,
+                    teacher_logprobs: torch.Tensor, teacher_rest: Optional[torch.Tensor] = None, inv_temperature=1.0,
+                    reverse: float = 0.0, with_entropy: bool = True, bwd_chunk: Optional[int] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """``hidden [N, H]``, ``weight [V, H]``, ``labels [N]``, ``teacher_ids [N, K]`` (integers), ``teacher_logprobs [N, K]``,
+    ``teacher_rest [N]`` or None -> ``(divergence [N], logprob [N], entropy [N] or None)``, fp32, all three differentiable in ``hidden`` and
+    ``weight`` (the teacher's numbers get no gradient).  ``logprob`` and ``entropy`` are those of :func:`~.logprob.lm_head_logprobs`.
+
+    An entry of ``teacher_ids`` outside the vocabulary (-1 by custom) names nothing; a token named again in a row counts once, by its
+    first entry.  A row that names nothing has divergence 0 without ``teacher_rest``.  A class that the teacher gives no mass (a
+    log-probability of ``-inf``) makes the reverse divergence infinite.  ``inv_temperature`` is a float or a per-row tensor ``[N]``.
+    On CUDA: bf16 hidden states and weights, H and V multiples of 8, K at most 256."""
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"hidden {list(hidden.shape)} and weight {list(weight.shape)} must be [N, H] and [V, H]")
+    N, H = hidden.shape
+    V = weight.shape[0]
+    if teacher_ids.dim() != 2 or teacher_ids.shape[0] != N or teacher_logprobs.shape != teacher_ids.shape:
+        raise ValueError(f"teacher_ids {list(teacher_ids.shape)} and teacher_logprobs {list(teacher_logprobs.shape)} must be [{N}, K] both")
+    if teacher_ids.dtype not in (torch.int32, torch.int64) or not teacher_logprobs.is_floating_point():
+        raise ValueError(f"teacher_ids must be int32 or int64, teacher_logprobs floating: {teacher_ids.dtype}, {teacher_logprobs.dtype}")
+    for name, t in (("labels", labels), ("teacher_rest", teacher_rest), ("inv_temperature", inv_temperature)):
+        if torch.is_tensor(t) and t.shape != (N,):
+            raise ValueError(f"{name} must be [{N}], got {list(t.shape)}")
+    if not 0.0 <= float(reverse) <= 1.0:
+        raise ValueError(f"reverse must lie between 0 (teacher to student) and 1 (student to teacher), got {reverse}")
+    tensors = {"weight": weight, "labels": labels, "teacher_ids": teacher_ids, "teacher_logprobs": teacher_logprobs,
+               "teacher_rest": teacher_rest, "inv_temperature": inv_temperature}
+    for name, t in tensors.items():
+        if torch.is_tensor(t) and t.device != hidden.device:
+            raise ValueError(f"{name} lives on {t.device}, hidden on {hidden.device}")
+    if not hidden.is_cuda:
+        return distill_ref(hidden, weight, labels, teacher_ids, teacher_logprobs, teacher_rest, inv_temperature, float(reverse), with_entropy)
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise ValueError(f"hidden and weight must be bf16 on a GPU, got {hidden.dtype} and {weight.dtype}")
+    if H % 8 or V % 8 or V == 0 or H == 0 or teacher_ids.shape[1] > MOST_NAMED:
+        raise ValueError(f"H = {H} and V = {V} must be multiples of 8, K = {teacher_ids.shape[1]} at most {MOST_NAMED}")
+    if N == 0:
+        # connected to its inputs, so that a shard without rows still has a gradient of zeros
+        z = (hidden.sum() + weight[:0].sum()) * 0.0 + hidden.new_zeros(0, dtype=torch.float32)
+        return z, z, (z if with_entropy else None)
+    with torch.cuda.device(hidden.device):
+        row16 = lambda t: t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 else t.contiguous()   # noqa: E731
+        whole = lambda t, dtype: t.detach().to(dtype).contiguous()                           # noqa: E731
+        it_t = whole(inv_temperature, torch.float32) if torch.is_tensor(inv_temperature) else None
+        if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.data_ptr() % 16:
+            raise ValueError("weight must have whole rows on 16-byte boundaries")
+        if teacher_ids.dtype == torch.int64:         # before 32 bits cut them
+            teacher_ids = torch.where((teacher_ids < 0) | (teacher_ids >= V), -1, teacher_ids)
+        value, lp, ent = _LmHeadDistillFn.apply(
+            row16(hidden), weight, whole(labels, torch.int32), whole(teacher_ids, torch.int32), whole(teacher_logprobs, torch.float32),
+            None if teacher_rest is None else whole(teacher_rest, torch.float32), it_t, 1.0 if it_t is not None else float(inv_temperature),
+            float(reverse), with_entropy, bwd_chunk)
+    return value, lp, (ent if with_entropy else None)
