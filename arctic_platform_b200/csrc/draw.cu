@@ -3,23 +3,26 @@
 //
 // Mathematics.  Every restriction keeps the logits from a threshold on, so a row comes down to one threshold: the top_k-th largest
 // logit; the least logit with exp((l - max) / T) >= min_p; the least logit of which the strictly larger ones hold less than top_p of what
-// stayed so far.  Masses are exp((l - max) / T) in 64 bits, rounded to whole multiples of 2^-45: sums of whole numbers do not depend on
-// their order, and a draw next to a border comes out as it does in 64-bit arithmetic (fp32 masses put one draw of some hundred, from
-// flat rows of 151936, on the neighbour's side).
+// stayed so far.  Masses and their sums are 64-bit numbers: fp32 ones put one draw of some hundred, from flat rows of 151936, on the
+// neighbour's side of a border.  Nothing is added by floating atomics, so that the same numbers give the same token every time.
 //
-// Layout.  A cluster of CTAs per row, each with a part of it in shared memory, so that the row is read from global memory once and walked
-// several times.  A threshold is found by histograms of 256 classes (an eighth of a nat each, then the bytes of the logit's order) that all CTAs of the
-// cluster read from one another, until few elements are left in the class that holds it.
+// Layout.  One CTA of 32 warps a row, or a cluster of 2, 4 or 8 where the rows leave SMs idle.  One walk reads a part from global memory, finds the
+// largest logit and adds up the masses (of exp(l / T) itself: 64-bit numbers have the range, so nothing waits for the largest); a warp has a
+// contiguous range, so that a draw from the whole distribution is then a search in 32 sums, in the 32 of that range and in some
+// hundred elements.  A part that fits shared memory is kept there for further walks, a longer one is read again from L2.  A threshold is found
+// by histograms that the CTAs of a cluster read from one another.
 #include "common.cuh"
 #include "host_utils.cuh"
 
 namespace apb {
 
-constexpr int kDrawThreads = 512;
+constexpr int kDrawThreads = 1024;
 constexpr int kDrawWarps = kDrawThreads / 32;
-constexpr int kDrawClasses = 256;
+constexpr int kDrawClasses = kDrawThreads;
 constexpr int kDrawFew = 256;             // elements of a class that are compared with one another
-constexpr int kDrawMaxPart = 48 * 1024;   // elements of a row in one CTA's shared memory
+constexpr int kDrawKept = 24 * 1024;      // elements of a part that is kept in shared memory
+constexpr int kDrawBytes = 160 * 1024;    // shared memory for the part and for the lists of elements that a nucleus can reach
+constexpr int kDrawMost = 3 << 17;        // elements of a row: units of 2^-45 of their masses add up in 64 bits, limbs of 12 bits in 32
 
 struct DrawArgs {
   const void* logits;
@@ -34,7 +37,7 @@ struct DrawArgs {
   const int* step;
   uint32_t seed;
   int u64;
-  int V, parts, per;
+  int V, parts, per, room;    // per: elements of a part; room: of a warp's list
   int* tokens;
   float* logprobs;
 };
@@ -62,11 +65,6 @@ __device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t a) {
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ unsigned long long warp_sum_u64(unsigned long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 __device__ __forceinline__ unsigned long long warp_scan_u64(unsigned long long v, int lane) {     // sum up to and with this lane
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -76,278 +74,473 @@ __device__ __forceinline__ unsigned long long warp_scan_u64(unsigned long long v
   return v;
 }
 
+// One value of every warp of the row: lane w of v[p] has that of warp w of part p (`none` behind the last part).
+__device__ __forceinline__ void row_f32(const float (&own)[kDrawWarps], int parts, int lane, float none, float (&v)[8]) {
+#pragma unroll
+  for (int p = 0; p < 8; ++p) v[p] = p < parts ? ld_cluster_f32(map_to_cta(smem_u32(&own[lane]), p)) : none;
+}
+__device__ __forceinline__ float row_max(const float (&own)[kDrawWarps], int parts, int lane) {
+  float v[8];
+  row_f32(own, parts, lane, -INFINITY, v);
+  return warp_max(fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]))));
+}
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_scan_f64(double v, int lane) {      // sum up to and with this lane
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+__device__ __forceinline__ double row_sum(const double (&own)[kDrawWarps], int parts, int lane) {
+  double v[8], s = 0;
+#pragma unroll
+  for (int p = 0; p < 8; ++p) v[p] = p < parts ? __longlong_as_double(ld_cluster_u64(map_to_cta(smem_u32(&own[lane]), p))) : 0.0;
+#pragma unroll
+  for (int p = 0; p < 8; ++p) s += v[p];
+  return warp_sum_f64(s);
+}
+__device__ __forceinline__ int row_min(const int (&own)[kDrawWarps], int parts, int lane) {
+  int s = 0x7fffffff;
+#pragma unroll
+  for (int p = 0; p < 8; ++p)
+    if (p < parts) s = min(s, static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&own[lane]), p))));
+  return __reduce_min_sync(0xffffffffu, s);
+}
+__device__ __forceinline__ void row_sync(int parts) {       // the CTAs of a row; what they wrote to their shared memory is there
+  if (parts > 1) cluster_sync_all();
+  else __syncthreads();
+}
+
+// exp2(x / 1024) of a 64-bit number, x from -2^20 to 2^20: x split into a whole number, whose power is a table's and an exponent, and a rest of at
+// most 1/2, whose power is its series to the second term (the third is below 7e-12 of the result, of either sign).  The high word of a table's
+// entry is less by its index at the place from which the shifted whole number carries into the exponent, so that one addition sets both.
+// 6 operations in 64 bits with the addition of the result to a sum: the library's exp2 and a sum of whole numbers took three times as long.
+struct DrawPower {
+  double y, power;                        // the result is their product
+};
+__device__ __forceinline__ DrawPower draw_power(double l, double scale, const double* table) {      // x = l scale
+  constexpr double kShift = 6755399441055744.0;                    // 1.5 2^52: adding it leaves the nearest whole number in the low bits
+  constexpr double kA = 0.69314718055994530942 / 1024;
+  const double t = fma(l, scale, kShift);
+  const int k = __double2loint(t);
+  const double r = fma(l, scale, kShift - t);
+  const double e = table[k & 1023];
+  return {fma(r, fma(r, kA * kA / 2, kA), 1.0), __hiloint2double(__double2hiint(e) + (k << 10), __double2loint(e))};
+}
+
 template <typename T>
 __device__ __forceinline__ float draw_logit(T x) {
   const float z = static_cast<float>(x);
   return z == z ? z : -INFINITY;          // what is not a number is never drawn
 }
 
-// z[shift + i] = element begin + i of the row, i < n; returns this thread's largest.  The shift puts 16-byte words of the row on 16-byte
-// words of the buffer.
-template <typename T>
-__device__ __forceinline__ float draw_load(const T* __restrict__ src, int n, float* buffer, int& shift) {
-  constexpr int kVec = 16 / sizeof(T);
-  const int ahead = static_cast<int>((-(reinterpret_cast<uintptr_t>(src)) & 15) / sizeof(T));
-  const int head = min(ahead, n), words = (n - head) / kVec, tail = head + words * kVec;
-  shift = (4 - head % 4) % 4;
-  float* z = buffer + shift;
-  float m = -INFINITY;
-  if (static_cast<int>(threadIdx.x) < head) {
-    z[threadIdx.x] = draw_logit(src[threadIdx.x]);
-    m = z[threadIdx.x];
-  }
-  const uint4* s4 = reinterpret_cast<const uint4*>(src + head);
-#pragma unroll 4
-  for (int w = threadIdx.x; w < words; w += kDrawThreads) {
-    const uint4 raw = s4[w];
-    const T* x = reinterpret_cast<const T*>(&raw);
-    float4* to = reinterpret_cast<float4*>(z + head + w * kVec);
+struct DrawShared {
+  double table[1024];                       // 2^(j / 1024), the high word less by j << 10
+  uint32_t hist[2][5][kDrawClasses];        // of the classes: limbs of the masses, elements (one copy is read while the next is filled)
+  float list[2][kDrawFew];                  // this CTA's elements of the class that holds a threshold (by rank, by mass)
+  float all[kDrawFew];                      // the row's
+  unsigned long long weight[kDrawFew];
+  double warp_mass[2][kDrawWarps], sub[kDrawWarps], before;
+  unsigned long long scan[kDrawWarps], above;
+  float warp_f[2][kDrawWarps];
+  int warp_i[kDrawWarps];
+  int list_n[2], chosen, in_class, owner;
+};
+
+constexpr int kDrawShared = (sizeof(DrawShared) + 15) / 16 * 16;
+static_assert(kDrawShared + kDrawBytes <= 227 * 1024, "shared memory of one CTA");
+
+// This CTA's part of a row: `n` elements from `src` on, KEPT: in shared memory, element i at z[i].  16-byte words of the row: the first
+// one begins at element `head`.
+template <typename T, bool KEPT>
+struct DrawRow {
+  static constexpr int kVec = 16 / sizeof(T);
+  const T* src;
+  float* z;
+  int n, parts, head, words;
+  float m, cut;        // cut: below it a mass is nothing
+  double scale;        // 1024 log2(e) / T
+  const double* table;
+  bool flat;           // the largest logit is infinite: equal ones stand for 0, all others for -inf
+
+  __device__ __forceinline__ float seen(float l) const { return flat ? (l == INFINITY ? 0.f : -INFINITY) : l; }
+  __device__ __forceinline__ float at(int i) const { return seen(KEPT ? z[i] : draw_logit(src[i])); }
+  __device__ __forceinline__ void word(int w, float (&l)[kVec]) const {
+    if constexpr (KEPT) {
+      const float4* f = reinterpret_cast<const float4*>(z + head + w * kVec);
 #pragma unroll
-    for (int j = 0; j < kVec; j += 4) {
-      const float4 f = make_float4(draw_logit(x[j]), draw_logit(x[j + 1]), draw_logit(x[j + 2]), draw_logit(x[j + 3]));
-      to[j / 4] = f;
-      m = fmaxf(fmaxf(m, fmaxf(f.x, f.y)), fmaxf(f.z, f.w));
+      for (int j = 0; j < kVec; j += 4) {
+        const float4 v = f[j / 4];
+        l[j] = v.x;
+        l[j + 1] = v.y;
+        l[j + 2] = v.z;
+        l[j + 3] = v.w;
+      }
+    } else {
+      const uint4 raw = reinterpret_cast<const uint4*>(src + head)[w];
+      const T* x = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) l[j] = draw_logit(x[j]);
     }
   }
-  for (int i = tail + threadIdx.x; i < n; i += kDrawThreads) {
-    z[i] = draw_logit(src[i]);
-    m = fmaxf(m, z[i]);
+  // Elements of a warp: whole words, the first warp's range begins with the elements in front of them, the last one's ends with those behind.
+  __device__ __forceinline__ int per_warp() const { return (words + kDrawWarps - 1) / kDrawWarps; }
+  __device__ __forceinline__ int from(int warp) const { return warp == 0 ? 0 : head + min(warp * per_warp(), words) * kVec; }
+  __device__ __forceinline__ int to(int warp) const { return warp == kDrawWarps - 1 ? n : head + min((warp + 1) * per_warp(), words) * kVec; }
+  // f(logit) over the elements of this warp, a lane's share each; returns their number.  Two words at a time, whose chains of operations
+  // overlap.
+  template <typename F>
+  __device__ __forceinline__ int walk(int warp, int lane, F f) const {
+    int taken = 0;
+    auto one = [&](int w) {
+      float l[kVec];
+      word(w, l);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) f(seen(l[j]));
+      taken += kVec;
+    };
+    const int w1 = min((warp + 1) * per_warp(), words);
+    int w = min(warp * per_warp(), words) + lane;
+    for (; w + 32 < w1; w += 64) {
+      float l[2][kVec];
+      word(w, l[0]);
+      word(w + 32, l[1]);
+#pragma unroll
+      for (int j = 0; j < 2 * kVec; ++j) f(seen(l[j / kVec][j % kVec]));
+      taken += 2 * kVec;
+    }
+    if (w < w1) one(w);
+    const int tail = head + words * kVec;
+    if (warp == 0 && lane < head) {
+      f(at(lane));
+      ++taken;
+    }
+    if (warp == kDrawWarps - 1 && tail + lane < n) {
+      f(at(tail + lane));
+      ++taken;
+    }
+    return taken;
   }
-  return m;
-}
 
-struct DrawShared {
-  uint32_t hist[2][4][kDrawClasses];        // three 16-bit limbs of the masses, counts (two copies: one is read while the next is filled)
-  float list[kDrawFew];                     // this CTA's elements of the class
-  float all[kDrawFew];                      // the cluster's
-  unsigned long long weight[kDrawFew];
-  unsigned long long warp_mass[kDrawWarps];
-  unsigned long long above, total;
-  float warp_f[kDrawWarps];
-  int warp_i[kDrawWarps];
-  float part_max, part_sum, threshold;
-  int part_first, list_n, chosen, in_class, owner;
-  unsigned long long before;
+  // f(logits, which of them are there) over the elements of this warp, all lanes in step
+  template <typename F>
+  __device__ __forceinline__ void walk_batches(int warp, int lane, F f) const {
+    const int w0 = min(warp * per_warp(), words), w1 = min((warp + 1) * per_warp(), words);
+    float l[2 * kVec];
+    for (int w = w0 + lane; w - lane < w1; w += 64) {
+      uint32_t there = 0;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float x[kVec];
+        const bool on = w + 32 * q < w1;
+        if (on) word(w + 32 * q, x);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) l[q * kVec + j] = on ? seen(x[j]) : -INFINITY;
+        if (on) there |= ((1u << kVec) - 1u) << (q * kVec);
+      }
+      f(l, there);
+    }
+    const int tail = head + words * kVec;
+    const int edge = warp == 0 && lane < head ? lane : warp == kDrawWarps - 1 && tail + lane < n ? tail + lane : -1;
+    if ((warp == 0 && head > 0) || (warp == kDrawWarps - 1 && tail < n)) {
+      l[0] = edge >= 0 ? at(edge) : -INFINITY;
+      f(l, edge >= 0 ? 1u : 0u);
+    }
+  }
+
+  // exp((l - m) / T)
+  __device__ __forceinline__ double mass(float l) const {
+    const DrawPower q = draw_power(static_cast<double>(fmaxf(l, cut)) - static_cast<double>(m), scale, table);
+    return l >= cut ? q.y * q.power : 0.0;
+  }
+  // the same in whole units of 2^-45
+  __device__ __forceinline__ unsigned long long units(float l) const {
+    return static_cast<unsigned long long>(__double_as_longlong(fma(mass(l), 0x1p45, 4503599627370496.0))) - 0x4330000000000000ull;
+  }
 };
 
-struct DrawRow {
-  const float* z;      // this CTA's part
-  int n, parts, part;
-  float m, inv_t;
-  double scale;        // log2(e) / T
-
-  // mass in units of 2^-45; rounded to nearest: rounding down would take 2^-46 from every token of the tail, to one side
-  __device__ __forceinline__ unsigned long long mass(float l) const {
-    if (l == m) return 1ull << 45;
-    const double x = (static_cast<double>(l) - static_cast<double>(m)) * scale;
-    if (!(x > -47.0)) return 0ull;
-    return static_cast<unsigned long long>(__double2ll_rn(exp2(x + 45.0)));
-  }
-  __device__ __forceinline__ int first_class(float l) const {
-    if (l == m) return 0;
-    return static_cast<int>(fminf((m - l) * inv_t * 8.f, static_cast<float>(kDrawClasses - 1)));
-  }
-};
-
-// The threshold of a restriction on the elements >= floor: the least logit of which the strictly larger ones count less than `target`
-// (MASS: weigh less than `share` / 2^64 of all).  The same in every CTA of the cluster.
-template <bool MASS>
-__device__ float draw_threshold(const DrawRow& r, DrawShared& sh, float floor, unsigned long long target, unsigned long long share, int& round) {
+// The threshold of a restriction on the elements that each(f) gives f, a warp's share to each warp (all that can matter of them): the least logit of
+// which the strictly larger ones count (MASS: weigh) less than `target`.  The same in every CTA of the row.  At most one call by count and one
+// by mass.
+template <bool MASS, typename Row, typename Each>
+__device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, float per_class, unsigned long long target, int& round) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // Classes of a level: 1024 equal steps down from the largest logit (the last takes what is left), 1024 steps of that class, then the bytes
+  // of the logits' order, the highest first.
   unsigned long long above = 0;             // of the elements in higher classes
   uint32_t prefix = 0;
-  int first = 0;
-  for (int level = 0; level < 5; ++level, ++round) {
-    const int shift = 32 - 8 * level;       // level 1: the highest byte
+  int first = 0, second = 0;
+  for (int level = 0; level < 6; ++level, ++round) {
+    const int shift = 40 - 8 * level;       // level 2: the highest byte
+    // whether an element belongs to the classes chosen so far; its class of this level
+    auto in_chosen = [&](float l, int& c) {
+      const float x = l == r.m ? 0.f : (r.m - l) * per_class;
+      c = static_cast<int>(fminf(x, kDrawClasses - 1.f));
+      if (level == 0) return true;
+      if (c != first) return false;
+      c = static_cast<int>(fminf((x - static_cast<float>(first)) * kDrawClasses, kDrawClasses - 1.f));
+      if (level == 1) return true;
+      if (c != second) return false;
+      const uint32_t key = draw_key(l);
+      c = 255 - static_cast<int>((key >> shift) & 255u);
+      return level == 2 || (key >> (shift + 8)) == prefix;
+    };
     uint32_t(*h)[kDrawClasses] = sh.hist[round & 1];
-    for (int i = tid; i < 4 * kDrawClasses; i += kDrawThreads) (&h[0][0])[i] = 0;
+#pragma unroll
+    for (int q = MASS ? 0 : 4; q < 5; ++q) h[q][tid] = 0;
     __syncthreads();
-    for (int i = tid; i < r.n; i += kDrawThreads) {
-      const float l = r.z[i];
-      if (!(l >= floor)) continue;
-      int c = r.first_class(l);
-      if (level > 0) {
-        if (c != first) continue;
-        const uint32_t key = draw_key(l);
-        if (level > 1 && (key >> (shift + 8)) != prefix) continue;
-        c = 255 - static_cast<int>((key >> shift) & 255u);
-      }
-      atomicAdd(&h[3][c], 1u);
+    each([&](float l) {
+      int c;
+      if (!in_chosen(l, c)) return;
+      atomicAdd(&h[4][c], 1u);
       if (MASS) {
-        const unsigned long long w = r.mass(l);          // at most 2^45; a class has at most 2^16 elements of this CTA
-        if (w & 0xffffu) atomicAdd(&h[0][c], static_cast<uint32_t>(w & 0xffffu));
-        if ((w >> 16) & 0xffffu) atomicAdd(&h[1][c], static_cast<uint32_t>((w >> 16) & 0xffffu));
-        if (w >> 32) atomicAdd(&h[2][c], static_cast<uint32_t>(w >> 32));
+        // at most 2^45 in limbs of 12 bits, whose sums over a row's elements fit 32 bits: additions of 32 bits are carried out by shared
+        // memory, those of 64 are a loop of comparisons
+        const unsigned long long w = r.units(l);
+        const uint32_t low = static_cast<uint32_t>(w), high = static_cast<uint32_t>(w >> 24);
+        atomicAdd(&h[0][c], low & 0xfffu);
+        if ((low >> 12) & 0xfffu) atomicAdd(&h[1][c], (low >> 12) & 0xfffu);
+        if (high & 0xfffu) atomicAdd(&h[2][c], high & 0xfffu);
+        if (high >> 12) atomicAdd(&h[3][c], high >> 12);
       }
-    }
-    cluster_sync_all();
-    if (warp < 8) {
+    });
+    row_sync(r.parts);
+    {
       // one class a thread; then a scan from the highest on
+      uint32_t elements = 0;
       unsigned long long v = 0;
-      uint32_t count = 0;
-      for (int p = 0; p < r.parts; ++p) {
-        const uint32_t at = map_to_cta(smem_u32(&h[0][tid]), p);
-        count += ld_cluster_u32(at + 3 * kDrawClasses * 4);
-        if (MASS)
-          v += ld_cluster_u32(at) + (static_cast<unsigned long long>(ld_cluster_u32(at + kDrawClasses * 4)) << 16) +
-               (static_cast<unsigned long long>(ld_cluster_u32(at + 2 * kDrawClasses * 4)) << 32);
+#pragma unroll
+      for (int q = MASS ? 0 : 4; q < 5; ++q) {
+        uint32_t x[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) x[p] = p < r.parts ? ld_cluster_u32(map_to_cta(smem_u32(&h[q][tid]), p)) : 0u;
+        unsigned long long wide = 0;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) wide += x[p];
+        if (q == 4) elements = static_cast<uint32_t>(wide);
+        else v += wide << (12 * q);
       }
-      if (!MASS) v = count;
+      if (!MASS) v = elements;
       const unsigned long long upto = warp_scan_u64(v, lane);
-      if (lane == 31) sh.warp_mass[warp] = upto;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      unsigned long long lower = above;
-      for (int w = 0; w < warp; ++w) lower += sh.warp_mass[w];
-      if (MASS && level == 0) {
-        unsigned long long total = 0;
-        for (int w = 0; w < 8; ++w) total += sh.warp_mass[w];
-        // larger < p total, in whole numbers: larger < ceil(p total); the largest always stay
-        target = max(1ull, __umul64hi(share, total) + (share * total != 0ull ? 1ull : 0ull));
-        if (tid == 0) sh.total = target;
-      }
-      const unsigned long long before = lower + upto - v;
+      if (lane == 31) sh.scan[warp] = upto;
+      if (tid == 0) sh.list_n[MASS] = 0;
+      __syncthreads();
+      const unsigned long long warps = warp_scan_u64(sh.scan[lane], lane);
+      unsigned long long before = __shfl_sync(0xffffffffu, warps, (warp - 1) & 31);
+      before = above + (warp ? before : 0ull) + upto - v;
       if (before < target && before + v >= target) {
         sh.chosen = tid;
-        sh.in_class = static_cast<int>(count);
+        sh.in_class = static_cast<int>(elements);
         sh.above = before;
       }
     }
     __syncthreads();
-    if (MASS && level == 0) target = sh.total;
     above = sh.above;
     const int chosen = sh.chosen, few = sh.in_class;
-    if (level == 0)
-      first = chosen;
-    else
-      prefix = level == 1 ? 255u - chosen : prefix << 8 | (255u - chosen);
-    __syncthreads();                          // what was read here is written again
-    if (level == 4) {                         // all bytes: one value
+    if (level == 5) {                         // all bytes: one value
+      __syncthreads();
       ++round;
-      return draw_unkey(prefix);
+      return draw_unkey(prefix << 8 | (255u - chosen));
     }
     if (few <= kDrawFew) {
-      if (tid == 0) sh.list_n = 0;
-      __syncthreads();
-      for (int i = tid; i < r.n; i += kDrawThreads) {
-        const float l = r.z[i];
-        if (!(l >= floor) || r.first_class(l) != first) continue;
-        if (level > 0 && (draw_key(l) >> shift) != prefix) continue;
-        sh.list[atomicAdd(&sh.list_n, 1)] = l;
-      }
-      cluster_sync_all();
+      each([&](float l) {
+        int c;
+        if (in_chosen(l, c) && c == chosen) sh.list[MASS][atomicAdd(&sh.list_n[MASS], 1)] = l;
+      });
+      row_sync(r.parts);
       // the parts' lists one behind another: a warp per part
       if (warp < r.parts) {
-        int at = 0;
-        for (int p = 0; p < warp; ++p) at += static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&sh.list_n), p)));
-        const int n = static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&sh.list_n), warp)));
-        for (int i = lane; i < n; i += 32) {
-          const float l = ld_cluster_f32(map_to_cta(smem_u32(&sh.list[i]), warp));
-          sh.all[at + i] = l;
-          if (MASS) sh.weight[at + i] = r.mass(l);
+        const int ns = lane < r.parts ? static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&sh.list_n[MASS]), lane))) : 0;
+        const int to = __reduce_add_sync(0xffffffffu, lane < warp ? ns : 0), have = __shfl_sync(0xffffffffu, ns, warp);
+        for (int i = lane; i < have; i += 32) {
+          const float l = ld_cluster_f32(map_to_cta(smem_u32(&sh.list[MASS][i]), warp));
+          sh.all[to + i] = l;
+          if (MASS) sh.weight[to + i] = r.units(l);
         }
       }
       __syncthreads();
+      // a group of 4 lanes an element: what is strictly larger, each lane a quarter of the list
       float least = INFINITY;
-      if (tid < few) {
-        const float l = sh.all[tid];
-        unsigned long long larger = above;
-        for (int j = 0; j < few; ++j)
-          if (sh.all[j] > l) larger += MASS ? sh.weight[j] : 1ull;
-        if (larger < target) least = l;
-      }
+      const int e = tid >> 2;
+      unsigned long long larger = 0;
+      const float l = e < few ? sh.all[e] : INFINITY;
+      for (int j = tid & 3; j < few; j += 4)
+        if (sh.all[j] > l) larger += MASS ? sh.weight[j] : 1ull;
+      larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+      larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+      if (e < few && above + larger < target) least = l;
       least = -warp_max(-least);
-      if (lane == 0) sh.warp_f[warp] = least;
+      if (lane == 0) sh.warp_f[1][warp] = least;
       __syncthreads();
-      for (int w = 0; w < kDrawWarps; ++w) least = fminf(least, sh.warp_f[w]);
-      __syncthreads();
-      cluster_sync_all();                     // the lists may be written again
+      least = -warp_max(-sh.warp_f[1][lane]);
       ++round;
       return least;
     }
+    if (level == 0)
+      first = chosen;
+    else if (level == 1)
+      second = chosen;
+    else
+      prefix = level == 2 ? 255u - chosen : prefix << 8 | (255u - chosen);
+    __syncthreads();                          // what was read here is written again
   }
-  return floor;
+  return -INFINITY;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kDrawThreads) draw_kernel(const DrawArgs a) {
+template <typename T, bool KEPT>
+__global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a) {
   pdl_entry();
-  extern __shared__ __align__(16) float draw_buffer[];
-  __shared__ DrawShared sh;
+  extern __shared__ __align__(16) unsigned char draw_smem[];
+  DrawShared& sh = *reinterpret_cast<DrawShared*>(draw_smem);
+  float* const draw_buffer = reinterpret_cast<float*>(draw_smem + kDrawShared);
+  using Row = DrawRow<T, KEPT>;
   const int b = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int begin = min(part * a.per, a.V), n = min(a.V - begin, a.per);
-  const T* src = static_cast<const T*>(a.logits) + b * a.ld + begin;
-  int shift;
-  float m = draw_load(src, n, draw_buffer, shift);
-  const float* z = draw_buffer + shift;
-  m = warp_max(m);
-  if (lane == 0) sh.warp_f[warp] = m;
-  __syncthreads();
-  for (int w = 0; w < kDrawWarps; ++w) m = fmaxf(m, sh.warp_f[w]);
-  if (tid == 0) sh.part_max = m;
-  cluster_sync_all();
-  for (int p = 0; p < a.parts; ++p) m = fmaxf(m, ld_cluster_f32(map_to_cta(smem_u32(&sh.part_max), p)));
+  Row r;
+  r.src = static_cast<const T*>(a.logits) + b * a.ld + begin;
+  r.n = n;
+  r.parts = a.parts;
+  r.head = min(static_cast<int>((-(reinterpret_cast<uintptr_t>(r.src)) & 15) / sizeof(T)), n);
+  r.words = (n - r.head) / Row::kVec;
+  r.table = sh.table;
+  r.flat = false;
+  r.z = draw_buffer + (4 - r.head % 4) % 4;           // words of the row on words of the buffer
+  float* const heavy = draw_buffer + (KEPT ? a.per + 4 : 0) + warp * a.room;
 
+  {
+    const double e = exp2(tid / 1024.0);
+    sh.table[tid] = __hiloint2double(__double2hiint(e) - (tid << 10), __double2loint(e));
+  }
   const float temperature = a.temperature ? a.temperature[b] : a.temperature_all;
   const bool greedy = !(temperature > 0.f);
-  const float t = greedy ? 1.f : temperature;
-  DrawRow r{z, n, a.parts, part, m, 1.f / t, 1.4426950408889634 / static_cast<double>(t)};
+  const float t = greedy ? 1.f : fminf(temperature, 1e30f);
+  r.scale = 1024 * 1.4426950408889634 / static_cast<double>(t);
+  __syncthreads();
+
+  // the first walk: the largest logit, masses exp(l / T) of this warp's range; KEPT: the part into shared memory
+  const float reach_of = 693.f * t;                     // 2^1000: what lies further from 0 is taken as that, and seen by the largest
+  float m = -INFINITY;
+  double mine = 0.0, mine2 = 0.0;
+  {
+    auto take = [&](float l, double& s) {
+      m = fmaxf(m, l);
+      const DrawPower q = draw_power(static_cast<double>(fminf(fmaxf(l, -reach_of), reach_of)), r.scale, sh.table);
+      s = fma(q.y, q.power, s);
+    };
+    const int tail = r.head + r.words * Row::kVec;
+    const int edge = warp == 0 && lane < r.head ? lane : warp == kDrawWarps - 1 && tail + lane < n ? tail + lane : -1;
+    if (edge >= 0) {
+      const float l = draw_logit(r.src[edge]);
+      if (KEPT) r.z[edge] = l;
+      take(l, mine);
+    }
+    const uint4* s4 = reinterpret_cast<const uint4*>(r.src + r.head);
+    const int w1 = min((warp + 1) * r.per_warp(), r.words);
+    // four words in flight while the four before them are added up
+    constexpr int kAhead = 4;
+    uint4 next[kAhead];
+    int w = min(warp * r.per_warp(), r.words) + lane;
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (w + 32 * q < w1) next[q] = s4[w + 32 * q];
+    for (; w < w1; w += 32 * kAhead) {
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int at = w + 32 * q;
+        if (at >= w1) break;
+        const uint4 raw = next[q];
+        if (at + 32 * kAhead < w1) next[q] = s4[at + 32 * kAhead];
+        const T* x = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int j = 0; j < Row::kVec; j += 4) {
+          const float4 f = make_float4(draw_logit(x[j]), draw_logit(x[j + 1]), draw_logit(x[j + 2]), draw_logit(x[j + 3]));
+          if (KEPT) reinterpret_cast<float4*>(r.z + r.head + at * Row::kVec)[j / 4] = f;
+          take(f.x, mine);
+          take(f.y, mine2);
+          take(f.z, mine);
+          take(f.w, mine2);
+        }
+      }
+    }
+  }
+  m = warp_max(m);
+  mine = warp_sum_f64(mine + mine2);
+  if (lane == 0) {
+    sh.warp_f[0][warp] = m;
+    sh.warp_mass[0][warp] = mine;
+  }
+  row_sync(a.parts);
+  m = row_max(sh.warp_f[0], a.parts, lane);
   if (m == -INFINITY) {                      // nothing to draw from
     if (part == 0 && tid == 0) {
       a.tokens[b] = 0;
       a.logprobs[b] = -INFINITY;
     }
-    cluster_sync_all();
+    row_sync(a.parts);
     return;
   }
-  // denominator of the unrestricted row
-  float sum = 0.f;
-  int first = 0x7fffffff;
-  for (int i = tid; i < n; i += kDrawThreads) {
-    const float l = z[i];
-    sum += l == m ? 1.f : __expf((l - m) * r.inv_t);
-    if (l == m) first = min(first, begin + i);
-  }
-  sum = warp_sum(sum);
-  first = __reduce_min_sync(0xffffffffu, first);
-  __syncthreads();
-  if (lane == 0) {
-    sh.warp_f[warp] = sum;
-    sh.warp_i[warp] = first;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kDrawWarps; ++w) {
-      sum += sh.warp_f[w];
-      first = min(first, sh.warp_i[w]);
-    }
-    sh.part_sum = sum;
-    sh.part_first = first;
-  }
-  __syncthreads();
-  auto whole_sum = [&]() {
-    float s = 0.f;
-    for (int p = 0; p < a.parts; ++p) s += ld_cluster_f32(map_to_cta(smem_u32(&sh.part_sum), p));
-    return s;
+  r.flat = m == INFINITY;
+  // the first walk's sums say nothing where the largest logit lies near or beyond what they tell apart
+  const bool redo = !(fabsf(m) <= 600.f * t);
+  if (r.flat) m = 0.f;
+  const float inv_t = 1.f / t;
+  r.m = m;
+  r.cut = m - 70.f * t;
+  const int k = a.top_k ? a.top_k[b] : a.top_k_all;
+  const float mp = fminf(a.min_p ? a.min_p[b] : a.min_p_all, 1.f);
+  const float p = a.top_p ? a.top_p[b] : a.top_p_all;
+  const bool by_rank = k > 0 && k < a.V, by_share = mp > 0.f, by_mass = p < 1.f;
+  // exp((l - m) / T) of this warp's elements >= bound
+  auto weigh = [&](float bound, int slot) {
+    double s0 = 0.0;
+    r.walk(warp, lane, [&](float l) {
+      if (l >= bound) s0 += r.mass(l);
+    });
+    s0 = warp_sum_f64(s0);
+    if (lane == 0) sh.warp_mass[slot][warp] = s0;
   };
+  int slot = 0;                               // of warp_mass: the other one may still be read
+  double factor = 1.0;                        // from the sums' unit to the largest's mass
+  if (redo) {
+    weigh(-INFINITY, slot = 1);
+    row_sync(a.parts);
+  } else {
+    const DrawPower q = draw_power(-static_cast<double>(m), r.scale, sh.table);
+    factor = q.y * q.power;
+  }
+  const double all_mass = row_sum(sh.warp_mass[slot], a.parts, lane) * factor;        // of the unrestricted row
   if (greedy) {
-    cluster_sync_all();
-    if (part == 0 && tid == 0) {
-      for (int p = 0; p < a.parts; ++p) first = min(first, static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&sh.part_first), p))));
-      a.tokens[b] = first;
-      a.logprobs[b] = -logf(whole_sum());
+    int first = 0x7fffffff;
+    const int hi = r.to(warp);
+    for (int i = r.from(warp) + lane; i < hi; i += 32)
+      if (r.at(i) == m) first = min(first, begin + i);
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) sh.warp_i[warp] = first;
+    row_sync(a.parts);
+    if (part == 0 && warp == 0) {
+      first = row_min(sh.warp_i, a.parts, lane);
+      if (lane == 0) {
+        a.tokens[b] = first;
+        a.logprobs[b] = static_cast<float>(-log(all_mass));
+      }
     }
-    cluster_sync_all();
+    row_sync(a.parts);
     return;
   }
 
   // what stays: logits >= threshold
   float threshold = -INFINITY;
   int round = 0;
-  const int k = a.top_k ? a.top_k[b] : a.top_k_all;
-  if (k > 0 && k < a.V) threshold = draw_threshold<false>(r, sh, -INFINITY, static_cast<unsigned long long>(k), 0ull, round);
-  const float mp = fminf(a.min_p ? a.min_p[b] : a.min_p_all, 1.f);
-  if (mp > 0.f && m < INFINITY) {
+  if (by_rank)
+    threshold = draw_threshold<false>(r, sh, [&](auto f) { r.walk(warp, lane, f); }, 32.f * inv_t, static_cast<unsigned long long>(k), round);
+  if (by_share) {
     // the least fp32 number l with (l - m) / T >= log(min_p), in 64 bits; from a rounded guess it is a step or two
     const double need = log(static_cast<double>(mp)) * static_cast<double>(t);
     auto stays = [&](float l) { return static_cast<double>(l) - static_cast<double>(m) >= need; };
@@ -356,105 +549,196 @@ __global__ void __launch_bounds__(kDrawThreads) draw_kernel(const DrawArgs a) {
     for (int i = 0; i < 4 && l > -INFINITY && stays(draw_unkey(draw_key(l) - 1u)); ++i) l = draw_unkey(draw_key(l) - 1u);
     threshold = fmaxf(threshold, fminf(l, m));
   }
-  const float p = a.top_p ? a.top_p[b] : a.top_p_all;
-  if (p < 1.f) {
-    const unsigned long long share = p > 0.f ? static_cast<unsigned long long>(static_cast<double>(p) * 18446744073709551616.0) : 0ull;
-    threshold = fmaxf(threshold, draw_threshold<true>(r, sh, threshold, 0ull, share, round));
+  if (by_mass) {
+    double total = all_mass;
+    if (by_rank || by_share) {
+      weigh(threshold, slot ^= 1);
+      row_sync(a.parts);
+      total = row_sum(sh.warp_mass[slot], a.parts, lane);
+    }
+    // larger < p total; in units, whose sums over the elements are off by less than the least step of p
+    const double share = p > 0.f ? static_cast<double>(p) * total : 0.0;
+    const unsigned long long target = max(1ull, static_cast<unsigned long long>(ceil(share * 0x1p45)));
+    // Elements below the V-th part of what the nucleus leaves out weigh less than that together: they are outside of it.  What is above goes
+    // into a list (of 151936 logits some hundreds to some ten thousands), and only its elements are sorted into classes.
+    const double least = (total - share) / static_cast<double>(a.V) * 0x1p45 - 1.0;
+    float reach = threshold;
+    if (least > 0.0) {
+      // lower by more than the roundings of masses, of l and of its fp32 number
+      const double under = log(least * 0x1p-45) - 1e-5;
+      reach = fmaxf(reach, static_cast<float>(static_cast<double>(m) + static_cast<double>(t) * under) - 1e-6f * fabsf(m));
+    }
+    // this warp's, in a list of its own
+    int have = 0;
+    r.walk_batches(warp, lane, [&](const float (&l)[2 * Row::kVec], uint32_t there) {
+      uint32_t in = 0;
+#pragma unroll
+      for (int j = 0; j < 2 * Row::kVec; ++j)
+        if (((there >> j) & 1u) && l[j] >= reach) in |= 1u << j;
+      if (!__any_sync(0xffffffffu, in != 0)) return;
+      const int count = __popc(in);
+      int to = count;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, to, o);
+        if (lane >= o) to += v;
+      }
+      const int more = __shfl_sync(0xffffffffu, to, 31);
+      to += have - count;
+      have += more;
+#pragma unroll
+      for (int j = 0; j < 2 * Row::kVec; ++j)
+        if ((in >> j) & 1u) {
+          if (to < a.room) heavy[to] = l[j];
+          ++to;
+        }
+    });
+    __syncwarp();
+    const bool listed = have <= a.room;
+    auto each = [&](auto f) {
+      if (!listed) {
+        r.walk(warp, lane, [&](float l) {
+          if (l >= reach) f(l);
+        });
+        return;
+      }
+      int i = lane;
+      for (; i + 32 < have; i += 64) {
+        const float l0 = heavy[i], l1 = heavy[i + 32];
+        f(l0);
+        f(l1);
+      }
+      if (i < have) f(heavy[i]);
+    };
+    const float per_class = reach > -INFINITY && reach < m ? fminf((kDrawClasses - 0.1f) / (m - reach), 1e30f) : 32.f * inv_t;
+    threshold = fmaxf(threshold, draw_threshold<true>(r, sh, each, per_class, target, round));
+    double s0 = 0.0;
+    each([&](float l) {
+      if (l >= threshold) s0 += r.mass(l);
+    });
+    s0 = warp_sum_f64(s0);
+    slot ^= 1;
+    if (lane == 0) sh.warp_mass[slot][warp] = s0;
   }
 
-  // masses of what stays, in whole ranges of a warp
-  const int range = (n + kDrawWarps * 32 - 1) / (kDrawWarps * 32) * 32;
-  const int lo = min(warp * range, n), hi = min(lo + range, n);
-  unsigned long long mine = 0;
-  for (int i = lo + lane; i < hi; i += 32)
-    if (z[i] >= threshold) mine += r.mass(z[i]);
-  mine = warp_sum_u64(mine);
-  if (lane == 0) sh.warp_mass[warp] = mine;
-  cluster_sync_all();
+  // masses of what stays
+  if (by_rank || by_share || by_mass) {
+    if (!by_mass) weigh(threshold, slot ^= 1);
+    factor = 1.0;
+    row_sync(a.parts);
+  }
   if (warp == 0) {
-    // 16 ranges of up to 8 parts, four a lane
-    unsigned long long v[4], total = 0;
+    // 32 ranges of up to 8 parts, eight a lane; a target that roundings put behind the last of their sums lies in the last that has mass
+    double v[8], total = 0.0;
+    const int q = lane / 4;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int q = lane * 4 + j;
-      v[j] = q / kDrawWarps < a.parts ? ld_cluster_u64(map_to_cta(smem_u32(&sh.warp_mass[q % kDrawWarps]), q / kDrawWarps)) : 0ull;
-      total += v[j];
-    }
-    const unsigned long long upto = warp_scan_u64(total, lane);
-    const unsigned long long all = __shfl_sync(0xffffffffu, upto, 31);
-    unsigned long long u;
+    for (int j = 0; j < 8; ++j)        // relative to the largest's
+      v[j] = q < a.parts ? __longlong_as_double(ld_cluster_u64(map_to_cta(smem_u32(&sh.warp_mass[slot][lane % 4 * 8 + j]), q))) * factor : 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) total += v[j];
+    const double upto = warp_scan_f64(total, lane);
+    double u;
     if (a.u == nullptr) {
       const uint32_t step = a.step ? static_cast<uint32_t>(*a.step) : 0u;
       const uint32_t base = draw_hash(a.seed ^ (step * 0x9E3779B9u)) ^ draw_hash(static_cast<uint32_t>(b) * 0x85ebca6bU + 1u);
-      u = static_cast<unsigned long long>(draw_hash(base + 0x9E3779B9u)) << 32 | draw_hash(base ^ 0x85ebca6bU);
+      u = (static_cast<double>(draw_hash(base + 0x9E3779B9u)) + static_cast<double>(draw_hash(base ^ 0x85ebca6bU)) * 0x1p-32) * 0x1p-32;
     } else {
-      const double x = a.u64 ? static_cast<const double*>(a.u)[b] : static_cast<double>(static_cast<const float*>(a.u)[b]);
-      // 1 and above, and what is not a number, stand for the last number below 1
-      u = x < 1.0 ? (x > 0.0 ? static_cast<unsigned long long>(x * 18446744073709551616.0) : 0ull) : ~0ull;
+      u = a.u64 ? static_cast<const double*>(a.u)[b] : static_cast<double>(static_cast<const float*>(a.u)[b]);
     }
-    const unsigned long long target = __umul64hi(u, all);       // floor(u all) < all
-    unsigned long long before = upto - total;
-    if (before <= target && target < upto) {
-      int j = 0;
+    // 1 and above, and what is not a number, stand for the largest number below 1
+    u = u < 1.0 ? fmax(u, 0.0) : 1.0 - 0x1p-52;
+    const double target = u * __shfl_sync(0xffffffffu, upto, 31);
+    // a range of less than 2^-80 has only elements that a mass is not formed of (below e^-70 of the largest), or none
+    const unsigned behind = __ballot_sync(0xffffffffu, total > 0x1p-80 && target < upto), some = __ballot_sync(0xffffffffu, total > 0x1p-80);
+    const int owner = behind ? __ffs(behind) - 1 : 31 - __clz(some);
+    double before = __shfl_up_sync(0xffffffffu, upto, 1);
+    if (lane == 0) before = 0.0;
+    if (lane == owner) {
+      int range = 0;
+      double begins = before;
+      bool found = false;
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (j == i && target >= before + v[i]) {
-          before += v[i];
-          j = i + 1;
+      for (int j = 0; j < 8; ++j) {
+        if (!found && v[j] > 0x1p-80) {
+          range = j;
+          begins = before;
         }
-      sh.owner = lane * 4 + j;
-      sh.before = target - before;            // within the range
+        before += v[j];
+        found = found || (v[j] > 0x1p-80 && target < before);
+      }
+      sh.owner = lane * 8 + range;
+      sh.before = target - begins;            // within the range
     }
   }
   __syncthreads();
-  if (sh.owner / kDrawWarps == part && sh.owner % kDrawWarps == warp) {
-    const unsigned long long target = sh.before;
-    // runs of the range, one a lane; then the run element by element
-    const int run = (hi - lo + 31) / 32, r0 = min(lo + lane * run, hi), r1 = min(r0 + run, hi);
-    unsigned long long s = 0;
-    for (int i = r0; i < r1; ++i)
-      if (z[i] >= threshold) s += r.mass(z[i]);
-    const unsigned long long upto = warp_scan_u64(s, lane);
-    const int at = __ffs(__ballot_sync(0xffffffffu, target < upto)) - 1;
-    unsigned long long before = __shfl_sync(0xffffffffu, upto - s, at);
-    const int e0 = __shfl_sync(0xffffffffu, r0, at), e1 = __shfl_sync(0xffffffffu, r1, at);
-    for (int i0 = e0; i0 < e1; i0 += 32) {
-      const int i = i0 + lane;
-      const unsigned long long w = i < e1 && z[i] >= threshold ? r.mass(z[i]) : 0ull;
-      const unsigned long long sum_w = before + warp_scan_u64(w, lane);
-      const unsigned hit = __ballot_sync(0xffffffffu, target < sum_w);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          a.tokens[b] = begin + i;
-          const double x = z[i] == m ? 0.0 : (static_cast<double>(z[i]) - static_cast<double>(m)) / static_cast<double>(t);
-          a.logprobs[b] = static_cast<float>(x - static_cast<double>(logf(whole_sum())));
+  if (sh.owner / kDrawWarps == part) {
+    // the range again, in 32 runs; then the run element by element
+    const double target = sh.before;
+    const int lo = r.from(sh.owner % kDrawWarps), hi = r.to(sh.owner % kDrawWarps), run = (hi - lo + kDrawWarps - 1) / kDrawWarps;
+    const int r0 = min(lo + warp * run, hi), r1 = min(r0 + run, hi);
+    double s = 0.0;
+    for (int i = r0 + lane; i < r1; i += 32) {
+      const float l = r.at(i);
+      if (l >= threshold) s += r.mass(l);
+    }
+    s = warp_sum_f64(s);
+    if (lane == 0) sh.sub[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+      const double mass = sh.sub[lane], upto = warp_scan_f64(mass, lane);
+      const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0), behind = __ballot_sync(0xffffffffu, mass > 0.0 && target < upto);
+      const int at = behind ? __ffs(behind) - 1 : 31 - __clz(some);
+      double before = __shfl_sync(0xffffffffu, upto - mass, at);
+      const int e0 = min(lo + at * run, hi), e1 = min(e0 + run, hi);
+      int drawn = -1;                         // the first behind which the target does not lie, or the last with any mass
+      for (int i0 = e0; i0 < e1; i0 += 32) {
+        const int i = i0 + lane;
+        const float l = i < e1 ? r.at(i) : -INFINITY;
+        const double w = i < e1 && l >= threshold ? r.mass(l) : 0.0;
+        const double upto_w = before + warp_scan_f64(w, lane);
+        const unsigned held = __ballot_sync(0xffffffffu, w > 0.0), hit = __ballot_sync(0xffffffffu, w > 0.0 && target < upto_w);
+        if (hit) {
+          drawn = i0 + __ffs(hit) - 1;
+          break;
         }
-        break;
+        if (held) drawn = i0 + 31 - __clz(held);
+        before = __shfl_sync(0xffffffffu, upto_w, 31);
       }
-      before = __shfl_sync(0xffffffffu, sum_w, 31);
+      if (lane == 0) {
+        const float l = r.at(drawn);
+        a.tokens[b] = begin + drawn;
+        a.logprobs[b] = static_cast<float>((static_cast<double>(l) - static_cast<double>(m)) / static_cast<double>(t) - log(all_mass));
+      }
     }
   }
-  cluster_sync_all();                         // nobody leaves while its shared memory may be read
+  row_sync(a.parts);                          // nobody leaves while its shared memory may be read
 }
 
-template <typename T>
-static int launch_draw(DrawArgs a, int B, cudaStream_t s) {
-  // parts of about 19000 elements, two CTAs of which an SM holds; more parts where rows are too few for the GPU
-  int parts = 1;
-  while (parts < 8 && ((a.V + parts - 1) / parts > 20480 || (static_cast<long long>(B) * parts * 2 <= 2 * sm_count() && a.V / parts > 4096))) parts *= 2;
-  a.parts = parts;
-  a.per = ((a.V + parts - 1) / parts + 7) / 8 * 8;
-  if (a.per > kDrawMaxPart) return kBadArgument;
-  const size_t smem = (static_cast<size_t>(a.per) + 4) * sizeof(float);
+template <typename T, bool KEPT>
+static int launch_draw_as(const DrawArgs& a, int B, cudaStream_t s) {
   static int allowed[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!allowed[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kDrawMaxPart + 4) * 4);
+    const cudaError_t e = cudaFuncSetAttribute(draw_kernel<T, KEPT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kDrawShared + kDrawBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
     allowed[dev & 63] = 1;
   }
-  return static_cast<int>(launch_kernel_clusters(draw_kernel<T>, dim3(static_cast<unsigned>(B) * parts), dim3(kDrawThreads), smem, parts, s, a));
+  return static_cast<int>(launch_kernel_clusters(draw_kernel<T, KEPT>, dim3(static_cast<unsigned>(B) * a.parts), dim3(kDrawThreads),
+                                                 kDrawShared + kDrawBytes, a.parts, s, a));
+}
+
+template <typename T>
+static int launch_draw(DrawArgs a, int B, cudaStream_t s) {
+  // as many parts as leave every CTA an SM of its own, of no fewer than 4096 elements
+  int parts = 1;
+  while (parts < 8 && static_cast<long long>(B) * parts * 2 <= sm_count() && a.V / parts > 8192) parts *= 2;
+  a.parts = parts;
+  a.per = ((a.V + parts - 1) / parts + 7) / 8 * 8;
+  const bool kept = a.per <= kDrawKept;
+  a.room = (kDrawBytes / 4 - (kept ? a.per + 4 : 0)) / kDrawWarps;
+  return kept ? launch_draw_as<T, true>(a, B, s) : launch_draw_as<T, false>(a, B, s);
 }
 
 }  // namespace apb
@@ -463,15 +747,15 @@ extern "C" {
 
 // logits [B, V], row stride ld: type 0 fp32, 1 bf16, 2 fp16.  Of each setting a tensor [B] (fp32, top_k int32) or null and one number
 // for all rows: temperature (<= 0: the first of the largest logits), top_k (<= 0: off), top_p (>= 1: off), min_p (<= 0: off).  u [B] in
-// [0, 1): fp32, or fp64 with u64; null: a hash of seed, *step (null: 0) and the row.  tokens [B] int32, logprobs [B] fp32.  V up to 8 * 49152.
+// [0, 1): fp32, or fp64 with u64; null: a hash of seed, *step (null: 0) and the row.  tokens [B] int32, logprobs [B] fp32.  V up to 393216.
 int apb_draw(const void* logits, int type, long long ld, const float* temperature, float temperature_all, const int* top_k, int top_k_all,
              const float* top_p, float top_p_all, const float* min_p, float min_p_all, const void* u, int u64, unsigned seed, const int* step,
              int B, int V, int* tokens, float* logprobs, cudaStream_t s) {
   using namespace apb;
   if (B <= 0) return 0;
-  if (!logits || !tokens || !logprobs || V < 1 || V > 8 * kDrawMaxPart || type < 0 || type > 2) return kBadArgument;
+  if (!logits || !tokens || !logprobs || V < 1 || V > kDrawMost || type < 0 || type > 2) return kBadArgument;
   DrawArgs a{logits, ld, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all,
-             u, step, static_cast<uint32_t>(seed), u64, V, 1, 0, tokens, logprobs};
+             u, step, static_cast<uint32_t>(seed), u64, V, 1, 0, 0, tokens, logprobs};
   if (type == 0) return launch_draw<float>(a, B, s);
   if (type == 1) return launch_draw<__nv_bfloat16>(a, B, s);
   return launch_draw<__half>(a, B, s);

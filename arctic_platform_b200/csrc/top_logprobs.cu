@@ -2,9 +2,10 @@
 // the mass of all other tokens.
 //
 // Mathematics.  One pass.  A candidate is a logit's order and its index in one 64-bit number, larger for larger logits and, of equal ones, for
-// the lower index, so that the k largest numbers are the answer.  A buffer takes what is above the k-th largest number seen when it was
-// last sorted; what falls out of it, or never was above that, can no longer be among the k and adds exp(l) to the sum of the others.  That sum
-// is therefore formed from them alone: one minus the named tokens' share would keep nothing of it where they hold all but a little.
+// the lower index, so that the k largest numbers are the answer.  A buffer takes what is above a number that k candidates are known to reach
+// (first the k-th largest of the threads' largest ones, then the k-th of the buffer whenever it is sorted); what falls out of the
+// buffer, or never was above that number, can no longer be among the k and adds exp(l) to the sum of the others.  That sum is therefore
+// formed from them alone: one minus the named tokens' share would keep nothing of it where they hold all but a little.
 //
 // Layout.  One CTA walks a row, or each CTA of a cluster a part of it where rows are few, and the first one sorts what the others kept.
 #include "common.cuh"
@@ -12,9 +13,9 @@
 
 namespace apb {
 
-constexpr int kTopThreads = 1024;
-constexpr int kTopRoom = 2048;            // candidates that the buffer holds
+constexpr int kTopThreads = 512;
 constexpr int kTopMost = 1024;            // k
+constexpr float kTopLog2e = 1.44269504088896340736f;
 
 struct TopArgs {
   const void* logits;
@@ -31,103 +32,125 @@ __device__ __forceinline__ uint32_t top_key(float z) {
   const uint32_t u = __float_as_uint(z);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float top_value(unsigned long long c) {
-  const uint32_t k = static_cast<uint32_t>(c >> 32);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
+__device__ __forceinline__ float top_unkey(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+__device__ __forceinline__ float top_value(unsigned long long c) { return top_unkey(static_cast<uint32_t>(c >> 32)); }
 __device__ __forceinline__ unsigned long long top_candidate(float z, int i) {
   return static_cast<unsigned long long>(top_key(z)) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
 }
 
-// Sum of exp((l - m) scale) against a running maximum.
-struct TopSum {
-  float m = -INFINITY, s = 0.f;
-  __device__ __forceinline__ void add(float z) {
-    if (z > m) {
-      s = (m == -INFINITY ? 0.f : s * __expf(m - z)) + 1.f;
-      m = z;
-    } else if (z > -INFINITY) {
-      s += z == m ? 1.f : __expf(z - m);
-    }
-  }
-  __device__ __forceinline__ void join(float m2, float s2) {
-    const float mn = fmaxf(m, m2);
-    if (mn == -INFINITY) return;
-    s = (m == mn ? s : s * __expf(m - mn)) + (m2 == mn ? s2 : s2 * __expf(m2 - mn));
-    m = mn;
-  }
-};
-
-// The buffer in falling order (all threads).
-__device__ void top_sort(unsigned long long* buf) {
-  for (int size = 2; size <= kTopRoom; size <<= 1)
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      __syncthreads();
-      const int i = 2 * threadIdx.x - (threadIdx.x & (stride - 1)), j = i + stride;
-      const unsigned long long a = buf[i], b = buf[j];
-      if ((a < b) == ((i & size) == 0)) {
-        buf[i] = b;
-        buf[j] = a;
+// The first `size` (a power of 2 from 64 on) entries of the buffer in falling order (all threads).  Pairs at most 32 apart lie in 64 entries
+// that one warp walks: between those steps the warp alone waits.
+__device__ void top_sort(unsigned long long* buf, int size) {
+  __syncthreads();
+  for (int run = 2; run <= size; run <<= 1)
+    for (int stride = run >> 1; stride > 0; stride >>= 1) {
+      for (int t = threadIdx.x; t < size / 2; t += kTopThreads) {
+        const int i = 2 * t - (t & (stride - 1)), j = i + stride;
+        const unsigned long long a = buf[i], b = buf[j];
+        if ((a < b) == ((i & run) == 0)) {
+          buf[i] = b;
+          buf[j] = a;
+        }
       }
+      // the next step's pairs: of half the distance, or the widest of the next run
+      const int next = stride > 1 ? stride >> 1 : run;
+      if (stride > 32 || next > 32) __syncthreads();
+      else __syncwarp();
     }
   __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kTopThreads) top_kernel(const TopArgs a) {
+// 2^((z - ref) scale2), z <= ref: the difference first, as a product of a large logit would lose the digits that tell it from its neighbours.
+__device__ __forceinline__ float top_mass(float z, float ref, float scale2) { return z == ref ? 1.f : exp2f((z - ref) * scale2); }
+
+// Sum of the others' masses against a reference that moves up: the value of `least`, which none of them is above.
+struct TopSum {
+  float scale2, ref = -INFINITY, s = 0.f;
+  __device__ __forceinline__ void add(float z) { s += top_mass(z, ref, scale2); }
+  __device__ __forceinline__ void move(float to) {           // to >= ref
+    s = s == 0.f ? 0.f : s * top_mass(ref, to, scale2);
+    ref = to;
+  }
+};
+
+template <typename T, int ROOM>
+__global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   pdl_entry();
-  __shared__ unsigned long long buf[kTopRoom];
-  __shared__ float warp_m[32], warp_s[32], part_m, part_s;
+  __shared__ unsigned long long buf[ROOM];
+  __shared__ float warp_s[kTopThreads / 32], part_ref, part_s, shared_log;
   __shared__ int held, part_held;
   constexpr int kVec = 16 / sizeof(T);
   constexpr int kAtOnce = 8;              // elements of a thread between two looks at the buffer
+  constexpr int kWords = kAtOnce / kVec;
+  constexpr int kWarps = kTopThreads / 32;
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int begin = min(part * a.per, a.V), n = min(a.V - begin, a.per), k = a.k;
   const T* src = static_cast<const T*>(a.logits) + row * a.ld + begin;
-  const float scale = a.scale * (a.row_scale ? a.row_scale[row] : 1.f);
-  TopSum sum;
-  unsigned long long least = 0;           // the k-th largest when the buffer was last sorted; everything is above 0
+  const float scale2 = a.scale * (a.row_scale ? a.row_scale[row] : 1.f) * kTopLog2e;
+  TopSum sum{scale2};
+  unsigned long long least = 0;           // candidates above this may be among the k: at least k are, or the buffer has taken all
+  float least_z = -INFINITY;
+  int least_i = 0x7fffffff;
+  const int crowd = max(ROOM / 2, 2 * k); // held entries from which on sorting pays: a higher `least`
   if (tid == 0) held = 0;
   __syncthreads();
 
+  auto set_least = [&](unsigned long long c) {
+    least = c;
+    least_z = c ? top_value(c) : -INFINITY;
+    least_i = c ? static_cast<int>(0xffffffffu - static_cast<uint32_t>(c)) : 0x7fffffff;
+    sum.move(least_z);
+  };
+  // candidate(z, at) > least without forming it (-inf included: nothing is below it, and indices are below least_i before it is set)
+  auto above = [&](float z, int at) { return z > least_z || (z == least_z && at < least_i); };
+  auto sort_size = [](int have) { return have <= 64 ? 64 : 1 << (32 - __clz(have - 1)); };
   // sorts, keeps the k largest and counts the others into the sum
   auto squeeze = [&](int have) {
-    for (int i = have + tid; i < kTopRoom; i += kTopThreads) buf[i] = 0;
-    top_sort(buf);
-    for (int i = k + tid; i < have; i += kTopThreads) sum.add(top_value(buf[i]) * scale);
+    const int size = sort_size(have);
+    for (int i = have + tid; i < size; i += kTopThreads) buf[i] = 0;
+    top_sort(buf, size);
+    if (have >= k) set_least(buf[k - 1]);
+    for (int i = k + tid; i < have; i += kTopThreads)
+      if (top_value(buf[i]) > -INFINITY) sum.add(top_value(buf[i]));
     __syncthreads();
     if (tid == 0) held = min(have, k);
-    least = have >= k ? buf[k - 1] : 0;
     __syncthreads();
   };
   // the elements of one step: what is not above `least` into the sum, the others into the buffer
-  auto take = [&](const float (&z)[kAtOnce], const int (&at)[kAtOnce], uint32_t there) {
+  auto take = [&](const float (&z)[kAtOnce], int at0, uint32_t there) {
     uint32_t waiting = 0;
+    auto at = [&](int j) { return at0 + (j / kVec) * kTopThreads * kVec + j % kVec; };
+    auto sieve = [&](uint32_t in) {
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j)
-      if ((there >> j) & 1u) {
-        if (top_candidate(z[j], at[j]) > least) waiting |= 1u << j;
-        else sum.add(z[j] * scale);
+      for (int j = 0; j < kAtOnce; ++j) {
+        const bool on = (in >> j) & 1u, up = on && above(z[j], at(j));
+        if (up) waiting |= 1u << j;
+        if (on && !up && z[j] > -INFINITY) sum.add(z[j]);
       }
+    };
+    sieve(there);
     for (;;) {
       uint32_t left = 0;
+      bool full = false;
+      while (waiting) {
+        const int j = __ffs(waiting) - 1;
+        waiting &= waiting - 1;
+        float zj = z[0];
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j)
-        if ((waiting >> j) & 1u) {
-          const int slot = atomicAdd(&held, 1);
-          if (slot < kTopRoom) buf[slot] = top_candidate(z[j], at[j]);
-          else left |= 1u << j;
-        }
+        for (int i = 1; i < kAtOnce; ++i)
+          if (i == j) zj = z[i];
+        const int slot = atomicAdd(&held, 1);
+        if (slot < ROOM) buf[slot] = top_candidate(zj, at(j));
+        else left |= 1u << j;
+        full |= slot >= crowd;
+      }
+      if (!__syncthreads_or(left != 0 || full)) break;
+      const int have = min(held, ROOM);
+      __syncthreads();
+      squeeze(have);
       if (!__syncthreads_or(left != 0)) break;
-      squeeze(kTopRoom);
-      waiting = 0;
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j)
-        if ((left >> j) & 1u) {
-          if (top_candidate(z[j], at[j]) > least) waiting |= 1u << j;
-          else sum.add(z[j] * scale);
-        }
+      sieve(left);
     }
   };
   auto number = [](T x) {
@@ -138,76 +161,78 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const TopArgs a) {
   const int ahead = static_cast<int>((-(reinterpret_cast<uintptr_t>(src)) & 15) / sizeof(T));
   const int head = min(ahead, n), words = (n - head) / kVec, tail = head + words * kVec;
   const uint4* s4 = reinterpret_cast<const uint4*>(src + head);
-  constexpr int kWords = kAtOnce / kVec;
-  for (int w0 = 0; w0 < words; w0 += kWords * kTopThreads) {
-    float z[kAtOnce];
-    int at[kAtOnce];
-    uint32_t there = 0;
-    uint4 raw[kWords];
+  auto fetch = [&](uint4 (&raw)[kWords], int w0) {
 #pragma unroll
     for (int q = 0; q < kWords; ++q) {
       const int w = w0 + q * kTopThreads + tid;
-      raw[q] = w < words ? s4[w] : make_uint4(0, 0, 0, 0);
-      if (w < words) there |= ((1u << kVec) - 1u) << (q * kVec);
+      raw[q] = w < words ? __ldcs(s4 + w) : make_uint4(0, 0, 0, 0);
     }
+  };
+  uint4 next[kWords];
+  fetch(next, 0);
+  for (int w0 = 0; w0 < words; w0 += kWords * kTopThreads) {
+    float z[kAtOnce];
+    uint32_t there = 0;
 #pragma unroll
     for (int q = 0; q < kWords; ++q) {
-      const T* x = reinterpret_cast<const T*>(&raw[q]);
+      const T* x = reinterpret_cast<const T*>(&next[q]);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        z[q * kVec + j] = number(x[j]);
-        at[q * kVec + j] = begin + head + (w0 + q * kTopThreads + tid) * kVec + j;
-      }
+      for (int j = 0; j < kVec; ++j) z[q * kVec + j] = number(x[j]);
+      if (w0 + q * kTopThreads + tid < words) there |= ((1u << kVec) - 1u) << (q * kVec);
     }
-    take(z, at, there);
+    fetch(next, w0 + kWords * kTopThreads);
+    const int at0 = begin + head + (w0 + tid) * kVec;
+    if (w0 == 0 && k <= kTopThreads && words > kTopThreads) {
+      // k threads' largest elements: so many candidates reach the k-th of them.  Every thread has at least its first word.
+      unsigned long long best = 0;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const unsigned long long c = top_candidate(z[j], at0 + (j / kVec) * kTopThreads * kVec + j % kVec);
+        if (((there >> j) & 1u) && c > best) best = c;
+      }
+      buf[tid] = best;
+      top_sort(buf, kTopThreads);
+      set_least(buf[k - 1] - 1);
+      __syncthreads();
+    }
+    take(z, at0, there);
   }
   {
     // in front of the first and behind the last whole word: at most 14 elements
     float z[kAtOnce];
-    int at[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      z[j] = 0.f;
-      at[j] = 0;
-    }
+    for (int j = 0; j < kAtOnce; ++j) z[j] = 0.f;
     const int i = tid < head ? tid : tail + tid - head;
-    const bool one = i < n;
-    if (one) {
-      z[0] = number(src[i]);
-      at[0] = begin + i;
-    }
-    take(z, at, one ? 1u : 0u);
+    if (i < n) z[0] = number(src[i]);
+    take(z, begin + i, i < n ? 1u : 0u);
   }
-  squeeze(min(held, kTopRoom));
+  {
+    const int have = min(held, ROOM);
+    __syncthreads();
+    squeeze(have);
+  }
 
-  // the parts' candidates into the first one's buffer
-  float m = warp_max(sum.m);
-  float s = sum.m == -INFINITY ? 0.f : sum.s * __expf(sum.m - m);
-  s = warp_sum(s);
-  if (lane == 0) {
-    warp_m[warp] = m;
-    warp_s[warp] = s;
-  }
-  __syncthreads();
+  // the sum over the CTA; the reference is the same in all threads
+  auto join = [&]() {
+    float s = warp_sum(sum.s);
+    if (lane == 0) warp_s[warp] = s;
+    __syncthreads();
+    s = 0.f;
+    for (int w = 0; w < kWarps; ++w) s += warp_s[w];
+    __syncthreads();
+    return s;
+  };
+  float others = join();
   if (a.parts > 1) {
-    if (warp == 0) {
-      const float wm = warp_m[lane], mm = warp_max(wm);
-      const float ss = warp_sum(wm == -INFINITY ? 0.f : warp_s[lane] * __expf(wm - mm));
-      if (lane == 0) {
-        part_m = mm;
-        part_s = ss;
-        part_held = held;
-      }
+    if (tid == 0) {
+      part_ref = sum.ref;
+      part_s = others;
+      part_held = held;
     }
     cluster_sync_all();
     if (part == 0) {
       int have = held;
-      sum.m = -INFINITY;
-      sum.s = 0.f;
-      for (int p = 0; p < a.parts; ++p) {
-        if (tid == 0)
-          sum.join(ld_cluster_f32(map_to_cta(smem_u32(&part_m), p)), ld_cluster_f32(map_to_cta(smem_u32(&part_s), p)));
-        if (p == 0) continue;
+      for (int p = 1; p < a.parts; ++p) {
         int other;
         asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(other) : "r"(map_to_cta(smem_u32(&part_held), p)) : "memory");
         for (int i = tid; i < other; i += kTopThreads) {
@@ -215,68 +240,81 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const TopArgs a) {
           asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(c) : "r"(map_to_cta(smem_u32(&buf[i]), p)) : "memory");
           buf[have + i] = c;
         }
-        have += other;                    // parts * k <= kTopRoom
+        have += other;                    // parts * k <= ROOM
       }
+      sum.s = 0.f;
       __syncthreads();
-      squeeze(have);
-      m = warp_max(sum.m);
-      s = warp_sum(sum.m == -INFINITY ? 0.f : sum.s * __expf(sum.m - m));
-      if (lane == 0) {
-        warp_m[warp] = m;
-        warp_s[warp] = s;
+      squeeze(have);                      // at least k are there: none of the parts' references is above the new one
+      others = join();
+      for (int p = 0; p < a.parts; ++p) {
+        const float ref = ld_cluster_f32(map_to_cta(smem_u32(&part_ref), p)), s = ld_cluster_f32(map_to_cta(smem_u32(&part_s), p));
+        if (s > 0.f) others += s * top_mass(ref, sum.ref, scale2);
       }
-      __syncthreads();
     }
     cluster_sync_all();                   // nobody leaves while its buffer may be read
     if (part != 0) return;
   }
 
   // denominator: the others and the k
-  const float top = top_value(buf[0]) * scale;
-  __shared__ float named_sum;
-  __syncthreads();
-  float others_m = -INFINITY, others = 0.f;
-  if (warp == 0) {
-    const float wm = warp_m[lane];
-    others_m = warp_max(wm);
-    others = warp_sum(wm == -INFINITY ? 0.f : warp_s[lane] * __expf(wm - others_m));
+  const float top = top_value(buf[0]);
+  const float scale = a.scale * (a.row_scale ? a.row_scale[row] : 1.f);
+  float log_others = -INFINITY;           // against `top`
+  if (others > 1e-25f) {
+    log_others = (sum.ref == top ? 0.f : (sum.ref - top) * scale) + logf(others);
+  } else if (k < a.V && least_z > -INFINITY) {
+    // all of them so far below the k-th (57 nats) that their masses against it are lost: the row again, against their largest
+    const T* all = static_cast<const T*>(a.logits) + row * a.ld;
+    const unsigned long long last = buf[k - 1];
+    float most = -INFINITY;
+    for (int i = tid; i < a.V; i += kTopThreads) {
+      const float z = number(all[i]);
+      if (top_candidate(z, i) < last) most = fmaxf(most, z);
+    }
+    most = warp_max(most);
+    if (lane == 0) warp_s[warp] = most;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, warp_s[w]);
+    __syncthreads();
+    sum.s = 0.f;
+    for (int i = tid; i < a.V; i += kTopThreads) {
+      const float z = number(all[i]);
+      if (z > -INFINITY && top_candidate(z, i) < last) sum.s += top_mass(z, most, scale2);
+    }
+    others = join();
+    if (others > 0.f) log_others = (most - top) * scale + logf(others);
   }
   float named = 0.f;
-  for (int i = tid; i < k; i += kTopThreads) {
-    const float z = top_value(buf[i]) * scale;
-    named += z == top ? 1.f : expf(z - top);
-  }
-  named = warp_sum(named);
-  __syncthreads();
-  if (lane == 0) warp_s[warp] = named;
-  __syncthreads();
-  if (warp == 0) {
-    named = warp_sum(warp_s[lane]);
-    const float log_others = others_m == -INFINITY ? -INFINITY : others_m - top + logf(others);     // also where the share itself is 0
+  for (int i = tid; i < k; i += kTopThreads) named += top_mass(top_value(buf[i]), top, scale2);
+  sum.s = named;
+  named = join();
+  if (tid == 0) {
     others = expf(log_others);
-    if (lane == 0) {
-      const float log_all = logf(named + others);
-      named_sum = log_all;
-      // near 1 the logarithm of the others' share is that of one minus the named tokens'
-      a.rest[row] = top == -INFINITY ? -INFINITY : named < others ? log1pf(-named / (named + others)) : log_others - log_all;
-    }
+    const float log_all = logf(named + others);
+    shared_log = log_all;
+    // near 1 the logarithm of the others' share is that of one minus the named tokens'
+    a.rest[row] = top == -INFINITY ? -INFINITY : named < others ? log1pf(-named / (named + others)) : log_others - log_all;
   }
   __syncthreads();
   for (int i = tid; i < k; i += kTopThreads) {
-    const float z = top_value(buf[i]) * scale;
+    const float z = top_value(buf[i]);
     a.ids[static_cast<long long>(row) * k + i] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(buf[i]));
-    a.logprobs[static_cast<long long>(row) * k + i] = top == -INFINITY ? -INFINITY : (z == top ? 0.f : z - top) - named_sum;
+    a.logprobs[static_cast<long long>(row) * k + i] = top == -INFINITY ? -INFINITY : (z == top ? 0.f : (z - top) * scale) - shared_log;
   }
 }
 
-template <typename T>
+template <typename T, int ROOM>
 static int launch_top(TopArgs a, int N, cudaStream_t s) {
   // parts of a row where the GPU has room for more CTAs than rows (two a SM), as long as their candidates fit the first one's buffer
   int parts = 1;
-  while (parts < 8 && static_cast<long long>(N) * parts * 2 <= 2 * sm_count() && a.V / parts > 8192 && 2 * parts * a.k <= kTopRoom) parts *= 2;
+  while (parts < 8 && static_cast<long long>(N) * parts * 2 <= 2 * sm_count() && a.V / parts > 8192 && 2 * parts * a.k <= ROOM) parts *= 2;
   a.parts = parts;
   a.per = ((a.V + parts - 1) / parts + 7) / 8 * 8;
-  return static_cast<int>(launch_kernel_clusters(top_kernel<T>, dim3(static_cast<unsigned>(N) * parts), dim3(kTopThreads), 0, parts, s, a));
+  return static_cast<int>(launch_kernel_clusters(top_kernel<T, ROOM>, dim3(static_cast<unsigned>(N) * parts), dim3(kTopThreads), 0, parts, s, a));
+}
+
+template <typename T>
+static int launch_top_of(const TopArgs& a, int N, cudaStream_t s) {
+  return a.k <= 256 ? launch_top<T, 1024>(a, N, s) : launch_top<T, 2048>(a, N, s);
 }
 
 }  // namespace apb
@@ -291,8 +329,8 @@ int apb_top_logprobs(const void* logits, int type, long long ld, const float* ro
   if (N <= 0) return 0;
   if (!logits || !logprobs || !ids || !rest || V < 1 || k < 1 || k > V || k > kTopMost || type < 0 || type > 2) return kBadArgument;
   TopArgs a{logits, ld, row_scale, scale, V, k, 1, 0, logprobs, ids, rest};
-  if (type == 0) return launch_top<float>(a, N, s);
-  if (type == 1) return launch_top<__nv_bfloat16>(a, N, s);
-  return launch_top<__half>(a, N, s);
+  if (type == 0) return launch_top_of<float>(a, N, s);
+  if (type == 1) return launch_top_of<__nv_bfloat16>(a, N, s);
+  return launch_top_of<__half>(a, N, s);
 }
 }

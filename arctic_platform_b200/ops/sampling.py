@@ -8,8 +8,7 @@
   times all of it; at ``T <= 0`` the first of the largest logits, whatever the other settings are;
 * its log-probability is that of ``softmax(l / T)`` without restrictions (of ``softmax(l)`` at ``T <= 0``), as a policy's gradient wants it.
 
-The order of the restrictions is that of ``engine/reference_sampler.py``.  Masses are summed in 64 bits: the same numbers give the
-same token, whatever the batch around a row.  CUDA tensors run ``csrc/draw.cu``, CPU tensors the expression below (the oracle of the GPU tests).
+The order of the restrictions is that of ``engine/reference_sampler.py``.  Masses are 64-bit numbers.  CUDA tensors run ``csrc/draw.cu``, CPU tensors the expression below (the oracle of the GPU tests).
 """
 from __future__ import annotations
 
@@ -20,7 +19,7 @@ import torch
 
 from . import _lib
 
-MOST_VOCABULARY = 8 * 49152
+MOST_VOCABULARY = 3 << 17
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FN = None
 
@@ -76,10 +75,9 @@ def sample_ref(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
     stays = (larger < p * run[:, -1:]) | ~(p < 1) | (value == -most)
     mass = torch.where(torch.zeros_like(keep).scatter(1, rank, stays), mass, 0.0)
     run = mass.cumsum(-1)
-    u = uniforms.double()[:, None]
-    token = (run <= torch.where(u > 0, u, 0.0) * run[:, -1:]).sum(-1)
-    token = torch.minimum(token, torch.where(mass > 0, at, 0).amax(-1))            # u of 1 and above
-    token = torch.where(torch.isnan(uniforms), torch.where(mass > 0, at, 0).amax(-1), token)
+    u = torch.where(uniforms < 1, uniforms.double().clamp_min(0.0), 1 - 2.0 ** -52)[:, None]
+    token = (run <= u * run[:, -1:]).sum(-1)
+    token = torch.minimum(token, torch.where(mass > 0, at, 0).amax(-1))
     token = torch.where(greedy[:, 0], torch.where(z == most, at, V).amin(-1), token)
     logprob = x.gather(1, token[:, None])[:, 0] - full.sum(-1).log()
     nothing = torch.isinf(most[:, 0]) & (most[:, 0] < 0)
@@ -97,7 +95,7 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Setting = 
     ``[B]`` that take the result.
 
     Logits that are not numbers are never drawn; in a row without any above ``-inf`` token 0 comes out, with log-probability ``-inf``.
-    A uniform of 1 or more, or that is not a number, draws the last token that stayed."""
+    A uniform below 0 counts as 0, one of 1 or more, or that is not a number, as the largest number below 1."""
     if logits.dim() != 2 or logits.dtype not in _TYPES or logits.shape[1] < 1:
         raise ValueError(f"logits must be fp32, bf16 or fp16 [B, V], got {logits.dtype} {list(logits.shape)}")
     B, V = logits.shape
