@@ -18,10 +18,15 @@ namespace apb {
 
 constexpr int kDrawThreads = 1024;
 constexpr int kDrawWarps = kDrawThreads / 32;
-constexpr int kDrawClasses = kDrawThreads;
+constexpr int kDrawClasses = 2048;
+constexpr int kDrawPer = kDrawClasses / kDrawThreads;      // classes of a thread
+constexpr int kDrawLanes = kDrawThreads / 256;             // threads that compare one element with its class
+constexpr int kDrawRanges = kDrawWarps / 4;                // ranges of a lane, of those of 8 parts
+constexpr int kDrawBatch = 8;              // elements of a lane in flight in the first walk
+constexpr int kDrawGroup = 4;             // elements of a lane side by side in later ones: longer code does not fit the instruction cache
 constexpr int kDrawFew = 256;             // elements of a class that are compared with one another
 constexpr int kDrawKept = 24 * 1024;      // elements of a part that is kept in shared memory
-constexpr int kDrawBytes = 160 * 1024;    // shared memory for the part and for the lists of elements that a nucleus can reach
+constexpr int kDrawBytes = 176 * 1024;    // shared memory for the part and for the lists of elements that a nucleus can reach
 constexpr int kDrawMost = 3 << 17;        // elements of a row: units of 2^-45 of their masses add up in 64 bits, limbs of 12 bits in 32
 
 struct DrawArgs {
@@ -37,7 +42,7 @@ struct DrawArgs {
   const int* step;
   uint32_t seed;
   int u64;
-  int V, parts, per, room;    // per: elements of a part; room: of a warp's list
+  int V, parts, per, room;    // per: elements of a part; room: of a lane's list
   int* tokens;
   float* logprobs;
 };
@@ -77,7 +82,7 @@ __device__ __forceinline__ unsigned long long warp_scan_u64(unsigned long long v
 // One value of every warp of the row: lane w of v[p] has that of warp w of part p (`none` behind the last part).
 __device__ __forceinline__ void row_f32(const float (&own)[kDrawWarps], int parts, int lane, float none, float (&v)[8]) {
 #pragma unroll
-  for (int p = 0; p < 8; ++p) v[p] = p < parts ? ld_cluster_f32(map_to_cta(smem_u32(&own[lane]), p)) : none;
+  for (int p = 0; p < 8; ++p) v[p] = p < parts && lane < kDrawWarps ? ld_cluster_f32(map_to_cta(smem_u32(&own[lane]), p)) : none;
 }
 __device__ __forceinline__ float row_max(const float (&own)[kDrawWarps], int parts, int lane) {
   float v[8];
@@ -100,7 +105,8 @@ __device__ __forceinline__ double warp_scan_f64(double v, int lane) {      // su
 __device__ __forceinline__ double row_sum(const double (&own)[kDrawWarps], int parts, int lane) {
   double v[8], s = 0;
 #pragma unroll
-  for (int p = 0; p < 8; ++p) v[p] = p < parts ? __longlong_as_double(ld_cluster_u64(map_to_cta(smem_u32(&own[lane]), p))) : 0.0;
+  for (int p = 0; p < 8; ++p)
+    v[p] = p < parts && lane < kDrawWarps ? __longlong_as_double(ld_cluster_u64(map_to_cta(smem_u32(&own[lane]), p))) : 0.0;
 #pragma unroll
   for (int p = 0; p < 8; ++p) s += v[p];
   return warp_sum_f64(s);
@@ -109,7 +115,7 @@ __device__ __forceinline__ int row_min(const int (&own)[kDrawWarps], int parts, 
   int s = 0x7fffffff;
 #pragma unroll
   for (int p = 0; p < 8; ++p)
-    if (p < parts) s = min(s, static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&own[lane]), p))));
+    if (p < parts && lane < kDrawWarps) s = min(s, static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&own[lane]), p))));
   return __reduce_min_sync(0xffffffffu, s);
 }
 __device__ __forceinline__ void row_sync(int parts) {       // the CTAs of a row; what they wrote to their shared memory is there
@@ -117,21 +123,23 @@ __device__ __forceinline__ void row_sync(int parts) {       // the CTAs of a row
   else __syncthreads();
 }
 
-// exp2(x / 1024) of a 64-bit number, x from -2^20 to 2^20: x split into a whole number, whose power is a table's and an exponent, and a rest of at
-// most 1/2, whose power is its series to the second term (the third is below 7e-12 of the result, of either sign).  The high word of a table's
-// entry is less by its index at the place from which the shifted whole number carries into the exponent, so that one addition sets both.
-// 6 operations in 64 bits with the addition of the result to a sum: the library's exp2 and a sum of whole numbers took three times as long.
+// exp2(x / 64) of a 64-bit number, x from -2^16 to 2^16: x split into a whole number, whose power is a table's and an exponent, and a rest of at
+// most 1/2, whose power is its series to the third term (the fourth is below 4e-11 of the result).  The high word of a table's entry is less by
+// its index at the place from which the shifted whole number carries into the exponent, so that one addition sets both.  7 operations in 64
+// bits with the addition of the result to a sum.  The table has a copy for every two lanes: 1024 entries and a term less, one copy, cost
+// 6 passes through shared memory a load where this has 2 (the walk of a row of 151936 by one CTA 21 us).
 struct DrawPower {
   double y, power;                        // the result is their product
 };
-__device__ __forceinline__ DrawPower draw_power(double l, double scale, const double* table) {      // x = l scale
+__device__ __forceinline__ DrawPower draw_power(double l, double scale, const double* table) {      // x = l scale; table: this lane's
   constexpr double kShift = 6755399441055744.0;                    // 1.5 2^52: adding it leaves the nearest whole number in the low bits
-  constexpr double kA = 0.69314718055994530942 / 1024;
+  constexpr double kA = 0.69314718055994530942 / 64;
   const double t = fma(l, scale, kShift);
   const int k = __double2loint(t);
   const double r = fma(l, scale, kShift - t);
-  const double e = table[k & 1023];
-  return {fma(r, fma(r, kA * kA / 2, kA), 1.0), __hiloint2double(__double2hiint(e) + (k << 10), __double2loint(e))};
+  const double e = table[(k & 63) << 4];
+  return {fma(r, fma(r, fma(r, kA * kA * kA / 6, kA * kA / 2), kA), 1.0),
+          __hiloint2double(__double2hiint(e) + (k << 14), __double2loint(e))};
 }
 
 template <typename T>
@@ -141,8 +149,8 @@ __device__ __forceinline__ float draw_logit(T x) {
 }
 
 struct DrawShared {
-  double table[1024];                       // 2^(j / 1024), the high word less by j << 10
-  uint32_t hist[2][5][kDrawClasses];        // of the classes: limbs of the masses, elements (one copy is read while the next is filled)
+  double table[64][16];                     // 2^(j / 64), the high word less by j << 14; a copy for every two lanes: their own banks
+  uint32_t hist[4][kDrawClasses];           // of the classes: limbs of the masses, or elements
   float list[2][kDrawFew];                  // this CTA's elements of the class that holds a threshold (by rank, by mass)
   float all[kDrawFew];                      // the row's
   unsigned long long weight[kDrawFew];
@@ -150,7 +158,7 @@ struct DrawShared {
   unsigned long long scan[kDrawWarps], above;
   float warp_f[2][kDrawWarps];
   int warp_i[kDrawWarps];
-  int list_n[2], chosen, in_class, owner;
+  int list_n[2], limb[2], warp_n[kDrawWarps], chosen, owner;
 };
 
 constexpr int kDrawShared = (sizeof(DrawShared) + 15) / 16 * 16;
@@ -165,7 +173,7 @@ struct DrawRow {
   float* z;
   int n, parts, head, words;
   float m, cut;        // cut: below it a mass is nothing
-  double scale;        // 1024 log2(e) / T
+  double scale;        // 64 log2(e) / T
   const double* table;
   bool flat;           // the largest logit is infinite: equal ones stand for 0, all others for -inf
 
@@ -193,64 +201,40 @@ struct DrawRow {
   __device__ __forceinline__ int per_warp() const { return (words + kDrawWarps - 1) / kDrawWarps; }
   __device__ __forceinline__ int from(int warp) const { return warp == 0 ? 0 : head + min(warp * per_warp(), words) * kVec; }
   __device__ __forceinline__ int to(int warp) const { return warp == kDrawWarps - 1 ? n : head + min((warp + 1) * per_warp(), words) * kVec; }
-  // f(logit) over the elements of this warp, a lane's share each; returns their number.  Two words at a time, whose chains of operations
-  // overlap.
+  // f(logits) over the elements of this warp, kDrawGroup of a lane at a time, two words on their way meanwhile; places behind the last hold
+  // `none`
   template <typename F>
-  __device__ __forceinline__ int walk(int warp, int lane, F f) const {
-    int taken = 0;
-    auto one = [&](int w) {
-      float l[kVec];
-      word(w, l);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) f(seen(l[j]));
-      taken += kVec;
-    };
+  __device__ __forceinline__ void walk(int warp, int lane, float none, F f) const {
     const int w1 = min((warp + 1) * per_warp(), words);
     int w = min(warp * per_warp(), words) + lane;
-    for (; w + 32 < w1; w += 64) {
-      float l[2][kVec];
-      word(w, l[0]);
-      word(w + 32, l[1]);
+    float next[2][kVec];
+    if (w < w1) word(w, next[0]);
+    if (w + 32 < w1) word(w + 32, next[1]);
+#pragma unroll 1
+    for (; w < w1; w += 32) {
+      float x[kVec];
 #pragma unroll
-      for (int j = 0; j < 2 * kVec; ++j) f(seen(l[j / kVec][j % kVec]));
-      taken += 2 * kVec;
-    }
-    if (w < w1) one(w);
-    const int tail = head + words * kVec;
-    if (warp == 0 && lane < head) {
-      f(at(lane));
-      ++taken;
-    }
-    if (warp == kDrawWarps - 1 && tail + lane < n) {
-      f(at(tail + lane));
-      ++taken;
-    }
-    return taken;
-  }
-
-  // f(logits, which of them are there) over the elements of this warp, all lanes in step
-  template <typename F>
-  __device__ __forceinline__ void walk_batches(int warp, int lane, F f) const {
-    const int w0 = min(warp * per_warp(), words), w1 = min((warp + 1) * per_warp(), words);
-    float l[2 * kVec];
-    for (int w = w0 + lane; w - lane < w1; w += 64) {
-      uint32_t there = 0;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        float x[kVec];
-        const bool on = w + 32 * q < w1;
-        if (on) word(w + 32 * q, x);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) l[q * kVec + j] = on ? seen(x[j]) : -INFINITY;
-        if (on) there |= ((1u << kVec) - 1u) << (q * kVec);
+      for (int j = 0; j < kVec; ++j) {
+        x[j] = next[0][j];
+        next[0][j] = next[1][j];
       }
-      f(l, there);
+      if (w + 64 < w1) word(w + 64, next[1]);
+#pragma unroll
+      for (int g = 0; g < kVec; g += kDrawGroup) {
+        float l[kDrawGroup];
+#pragma unroll
+        for (int j = 0; j < kDrawGroup; ++j) l[j] = seen(x[g + j]);
+        f(l);
+      }
     }
     const int tail = head + words * kVec;
     const int edge = warp == 0 && lane < head ? lane : warp == kDrawWarps - 1 && tail + lane < n ? tail + lane : -1;
-    if ((warp == 0 && head > 0) || (warp == kDrawWarps - 1 && tail < n)) {
-      l[0] = edge >= 0 ? at(edge) : -INFINITY;
-      f(l, edge >= 0 ? 1u : 0u);
+    if (edge >= 0) {
+      float l[kDrawGroup];
+      l[0] = at(edge);
+#pragma unroll
+      for (int j = 1; j < kDrawGroup; ++j) l[j] = none;
+      f(l);
     }
   }
 
@@ -258,6 +242,17 @@ struct DrawRow {
   __device__ __forceinline__ double mass(float l) const {
     const DrawPower q = draw_power(static_cast<double>(fmaxf(l, cut)) - static_cast<double>(m), scale, table);
     return l >= cut ? q.y * q.power : 0.0;
+  }
+  // of those >= bound, together
+  __device__ __forceinline__ double masses(const float (&l)[kDrawGroup], float bound) const {
+    double s[2] = {0.0, 0.0};
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < kDrawGroup; ++j) any |= l[j] >= bound;
+    if (!any) return 0.0;
+#pragma unroll
+    for (int j = 0; j < kDrawGroup; ++j) s[j & 1] += l[j] >= bound ? mass(l[j]) : 0.0;
+    return s[0] + s[1];
   }
   // the same in whole units of 2^-45
   __device__ __forceinline__ unsigned long long units(float l) const {
@@ -269,14 +264,18 @@ struct DrawRow {
 // which the strictly larger ones count (MASS: weigh) less than `target`.  The same in every CTA of the row.  At most one call by count and one
 // by mass.
 template <bool MASS, typename Row, typename Each>
-__device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, float per_class, unsigned long long target, int& round) {
+__device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int elements, float per_class, unsigned long long target) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // Classes of a level: 1024 equal steps down from the largest logit (the last takes what is left), 1024 steps of that class, then the bytes
+  // Sums of limbs over `elements` elements of this CTA have to fit 32 bits: additions of 32 bits are carried out by shared memory, those of 64
+  // are a loop of comparisons.
+  const int limb = elements <= 65536 ? 16 : 13;
+  if (tid == 0) sh.limb[MASS] = limb;
+  // Classes of a level: 2048 equal steps down from the largest logit (the last takes what is left), 2048 steps of that class, then the bytes
   // of the logits' order, the highest first.
   unsigned long long above = 0;             // of the elements in higher classes
   uint32_t prefix = 0;
   int first = 0, second = 0;
-  for (int level = 0; level < 6; ++level, ++round) {
+  for (int level = 0; level < 6; ++level) {
     const int shift = 40 - 8 * level;       // level 2: the highest byte
     // whether an element belongs to the classes chosen so far; its class of this level
     auto in_chosen = [&](float l, int& c) {
@@ -291,72 +290,99 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, float p
       c = 255 - static_cast<int>((key >> shift) & 255u);
       return level == 2 || (key >> (shift + 8)) == prefix;
     };
-    uint32_t(*h)[kDrawClasses] = sh.hist[round & 1];
+    uint32_t(*h)[kDrawClasses] = sh.hist;   // the others have read it when they come to the row's wait behind
 #pragma unroll
-    for (int q = MASS ? 0 : 4; q < 5; ++q) h[q][tid] = 0;
+    for (int q = 0; q < (MASS ? 4 : 1); ++q)
+#pragma unroll
+      for (int i = 0; i < kDrawPer; ++i) h[q][tid + i * kDrawThreads] = 0;
     __syncthreads();
-    each([&](float l) {
-      int c;
-      if (!in_chosen(l, c)) return;
-      atomicAdd(&h[4][c], 1u);
-      if (MASS) {
-        // at most 2^45 in limbs of 12 bits, whose sums over a row's elements fit 32 bits: additions of 32 bits are carried out by shared
-        // memory, those of 64 are a loop of comparisons
-        const unsigned long long w = r.units(l);
-        const uint32_t low = static_cast<uint32_t>(w), high = static_cast<uint32_t>(w >> 24);
-        atomicAdd(&h[0][c], low & 0xfffu);
-        if ((low >> 12) & 0xfffu) atomicAdd(&h[1][c], (low >> 12) & 0xfffu);
-        if (high & 0xfffu) atomicAdd(&h[2][c], high & 0xfffu);
-        if (high >> 12) atomicAdd(&h[3][c], high >> 12);
+    each([&](const float (&l)[kDrawGroup]) {
+      int c[kDrawGroup];
+      bool in[kDrawGroup];
+#pragma unroll
+      for (int j = 0; j < kDrawGroup; ++j) in[j] = in_chosen(l[j], c[j]) && l[j] == l[j];
+      if (!MASS) {
+#pragma unroll
+        for (int j = 0; j < kDrawGroup; ++j)
+          if (in[j]) atomicAdd(&h[0][c[j]], 1u);
+        return;
+      }
+      unsigned long long w[kDrawGroup];
+#pragma unroll
+      for (int j = 0; j < kDrawGroup; ++j) w[j] = r.units(l[j]);       // at most 2^45: 3 limbs of 16 bits, 4 of 13
+#pragma unroll
+      for (int j = 0; j < kDrawGroup; ++j) {
+        if (!in[j]) continue;
+        const uint32_t mask = (1u << limb) - 1u;
+        atomicAdd(&h[0][c[j]], static_cast<uint32_t>(w[j]) & mask);
+        atomicAdd(&h[1][c[j]], static_cast<uint32_t>(w[j] >> limb) & mask);
+        const uint32_t rest = static_cast<uint32_t>(w[j] >> (2 * limb));         // most have no more
+        if (rest) {
+          atomicAdd(&h[2][c[j]], rest & mask);
+          if (rest >> limb) atomicAdd(&h[3][c[j]], rest >> limb);
+        }
       }
     });
     row_sync(r.parts);
     {
-      // one class a thread; then a scan from the highest on
-      uint32_t elements = 0;
-      unsigned long long v = 0;
+      // neighbouring classes to a thread; then a scan from the highest on
+      int limbs[8];
 #pragma unroll
-      for (int q = MASS ? 0 : 4; q < 5; ++q) {
-        uint32_t x[8];
+      for (int p = 0; p < 8; ++p) limbs[p] = MASS && p < r.parts ? static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&sh.limb[MASS]), p))) : 0;
+      unsigned long long v[kDrawPer] = {}, own = 0;
 #pragma unroll
-        for (int p = 0; p < 8; ++p) x[p] = p < r.parts ? ld_cluster_u32(map_to_cta(smem_u32(&h[q][tid]), p)) : 0u;
-        unsigned long long wide = 0;
+      for (int q = 0; q < (MASS ? 4 : 1); ++q)
 #pragma unroll
-        for (int p = 0; p < 8; ++p) wide += x[p];
-        if (q == 4) elements = static_cast<uint32_t>(wide);
-        else v += wide << (12 * q);
-      }
-      if (!MASS) v = elements;
-      const unsigned long long upto = warp_scan_u64(v, lane);
+        for (int p = 0; p < 8; ++p)
+          if (p < r.parts) {
+            const uint32_t from = map_to_cta(smem_u32(&h[q][kDrawPer * tid]), p);
+#pragma unroll
+            for (int i = 0; i < kDrawPer; i += 2) {
+              const unsigned long long x = ld_cluster_u64(from + 4 * i);
+              v[i] += (x & 0xffffffffull) << (q * limbs[p]);
+              v[i + 1] += (x >> 32) << (q * limbs[p]);
+            }
+          }
+#pragma unroll
+      for (int i = 0; i < kDrawPer; ++i) own += v[i];
+      const unsigned long long upto = warp_scan_u64(own, lane);
       if (lane == 31) sh.scan[warp] = upto;
       if (tid == 0) sh.list_n[MASS] = 0;
       __syncthreads();
-      const unsigned long long warps = warp_scan_u64(sh.scan[lane], lane);
-      unsigned long long before = __shfl_sync(0xffffffffu, warps, (warp - 1) & 31);
-      before = above + (warp ? before : 0ull) + upto - v;
-      if (before < target && before + v >= target) {
-        sh.chosen = tid;
-        sh.in_class = static_cast<int>(elements);
-        sh.above = before;
+      unsigned long long before = above + upto - own;
+      for (int w = 0; w < warp; ++w) before += sh.scan[w];
+#pragma unroll
+      for (int i = 0; i < kDrawPer; ++i) {
+        if (before < target && before + v[i] >= target) {
+          sh.chosen = kDrawPer * tid + i;
+          sh.above = before;
+        }
+        before += v[i];
       }
     }
     __syncthreads();
     above = sh.above;
-    const int chosen = sh.chosen, few = sh.in_class;
+    const int chosen = sh.chosen;
     if (level == 5) {                         // all bytes: one value
-      __syncthreads();
-      ++round;
+      row_sync(r.parts);
       return draw_unkey(prefix << 8 | (255u - chosen));
     }
-    if (few <= kDrawFew) {
-      each([&](float l) {
+    each([&](const float (&l)[kDrawGroup]) {
+#pragma unroll
+      for (int j = 0; j < kDrawGroup; ++j) {
         int c;
-        if (in_chosen(l, c) && c == chosen) sh.list[MASS][atomicAdd(&sh.list_n[MASS], 1)] = l;
-      });
-      row_sync(r.parts);
+        if (l[j] == l[j] && in_chosen(l[j], c) && c == chosen) {
+          const int to = atomicAdd(&sh.list_n[MASS], 1);
+          if (to < kDrawFew) sh.list[MASS][to] = l[j];
+        }
+      }
+    });
+    row_sync(r.parts);
+    const int ns = lane < r.parts ? static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&sh.list_n[MASS]), lane))) : 0;
+    const int few = __reduce_add_sync(0xffffffffu, ns);
+    if (few <= kDrawFew) {
       // the parts' lists one behind another: a warp per part
       if (warp < r.parts) {
-        const int ns = lane < r.parts ? static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&sh.list_n[MASS]), lane))) : 0;
         const int to = __reduce_add_sync(0xffffffffu, lane < warp ? ns : 0), have = __shfl_sync(0xffffffffu, ns, warp);
         for (int i = lane; i < have; i += 32) {
           const float l = ld_cluster_f32(map_to_cta(smem_u32(&sh.list[MASS][i]), warp));
@@ -365,21 +391,20 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, float p
         }
       }
       __syncthreads();
-      // a group of 4 lanes an element: what is strictly larger, each lane a quarter of the list
+      // some lanes an element: what is strictly larger, each lane in its share of the list
       float least = INFINITY;
-      const int e = tid >> 2;
+      const int e = tid / kDrawLanes;
       unsigned long long larger = 0;
       const float l = e < few ? sh.all[e] : INFINITY;
-      for (int j = tid & 3; j < few; j += 4)
+      for (int j = tid % kDrawLanes; j < few; j += kDrawLanes)
         if (sh.all[j] > l) larger += MASS ? sh.weight[j] : 1ull;
-      larger += __shfl_xor_sync(0xffffffffu, larger, 1);
-      larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+#pragma unroll
+      for (int o = 1; o < kDrawLanes; o <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
       if (e < few && above + larger < target) least = l;
       least = -warp_max(-least);
       if (lane == 0) sh.warp_f[1][warp] = least;
       __syncthreads();
-      least = -warp_max(-sh.warp_f[1][lane]);
-      ++round;
+      least = -warp_max(-sh.warp_f[1][lane % kDrawWarps]);
       return least;
     }
     if (level == 0)
@@ -388,7 +413,7 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, float p
       second = chosen;
     else
       prefix = level == 2 ? 255u - chosen : prefix << 8 | (255u - chosen);
-    __syncthreads();                          // what was read here is written again
+    row_sync(r.parts);                        // what was read here is written again
   }
   return -INFINITY;
 }
@@ -409,69 +434,82 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
   r.parts = a.parts;
   r.head = min(static_cast<int>((-(reinterpret_cast<uintptr_t>(r.src)) & 15) / sizeof(T)), n);
   r.words = (n - r.head) / Row::kVec;
-  r.table = sh.table;
+  r.table = &sh.table[0][lane & 15];
   r.flat = false;
   r.z = draw_buffer + (4 - r.head % 4) % 4;           // words of the row on words of the buffer
-  float* const heavy = draw_buffer + (KEPT ? a.per + 4 : 0) + warp * a.room;
+  float* const heavy = draw_buffer + (KEPT ? a.per + 4 : 0) + warp * 32 * a.room;
 
-  {
-    const double e = exp2(tid / 1024.0);
-    sh.table[tid] = __hiloint2double(__double2hiint(e) - (tid << 10), __double2loint(e));
+  for (int i = tid; i < 1024; i += kDrawThreads) {
+    const double e = exp2((i >> 4) / 64.0);
+    sh.table[i >> 4][i & 15] = __hiloint2double(__double2hiint(e) - ((i >> 4) << 14), __double2loint(e));
   }
   const float temperature = a.temperature ? a.temperature[b] : a.temperature_all;
   const bool greedy = !(temperature > 0.f);
   const float t = greedy ? 1.f : fminf(temperature, 1e30f);
-  r.scale = 1024 * 1.4426950408889634 / static_cast<double>(t);
+  r.scale = 64 * 1.4426950408889634 / static_cast<double>(t);
   __syncthreads();
 
   // the first walk: the largest logit, masses exp(l / T) of this warp's range; KEPT: the part into shared memory
-  const float reach_of = 693.f * t;                     // 2^1000: what lies further from 0 is taken as that, and seen by the largest
+  // 2^-1000: what lies below is taken as that, as what is no number is; what lies too far above 0 is seen by the largest, and its sums are not used
+  const float reach_of = 693.f * t;
   float m = -INFINITY;
-  double mine = 0.0, mine2 = 0.0;
+  double mine = 0.0;
   {
-    auto take = [&](float l, double& s) {
-      m = fmaxf(m, l);
-      const DrawPower q = draw_power(static_cast<double>(fminf(fmaxf(l, -reach_of), reach_of)), r.scale, sh.table);
-      s = fma(q.y, q.power, s);
+    // the stages of all elements of a batch side by side: an operation in 64 bits has its result some ten times later than one in 32
+    auto take = [&](const float (&l)[kDrawBatch]) {
+      double sum[2] = {0.0, 0.0};
+#pragma unroll
+      for (int j = 0; j < kDrawBatch; ++j) {
+        m = fmaxf(m, l[j]);
+        const DrawPower q = draw_power(static_cast<double>(fmaxf(l[j], -reach_of)), r.scale, r.table);
+        sum[j & 1] = fma(q.y, q.power, sum[j & 1]);
+      }
+      mine += sum[0] + sum[1];
     };
     const int tail = r.head + r.words * Row::kVec;
     const int edge = warp == 0 && lane < r.head ? lane : warp == kDrawWarps - 1 && tail + lane < n ? tail + lane : -1;
     if (edge >= 0) {
       const float l = draw_logit(r.src[edge]);
       if (KEPT) r.z[edge] = l;
-      take(l, mine);
+      m = fmaxf(m, l);
+      const DrawPower q = draw_power(static_cast<double>(fmaxf(l, -reach_of)), r.scale, r.table);
+      mine += q.y * q.power;
     }
     const uint4* s4 = reinterpret_cast<const uint4*>(r.src + r.head);
     const int w1 = min((warp + 1) * r.per_warp(), r.words);
-    // four words in flight while the four before them are added up
-    constexpr int kAhead = 4;
-    uint4 next[kAhead];
+    constexpr int kWords = kDrawBatch / Row::kVec;
+    uint4 next[kWords];                       // of the batch after this one
     int w = min(warp * r.per_warp(), r.words) + lane;
+    auto fetch = [&](int at) {
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q)
-      if (w + 32 * q < w1) next[q] = s4[w + 32 * q];
-    for (; w < w1; w += 32 * kAhead) {
+      for (int q = 0; q < kWords; ++q)
+        if (at + 32 * q < w1) next[q] = s4[at + 32 * q];
+    };
+    fetch(w);
+    for (; w < w1; w += 32 * kWords) {
+      float l[kDrawBatch];
 #pragma unroll
-      for (int q = 0; q < kAhead; ++q) {
-        const int at = w + 32 * q;
-        if (at >= w1) break;
-        const uint4 raw = next[q];
-        if (at + 32 * kAhead < w1) next[q] = s4[at + 32 * kAhead];
-        const T* x = reinterpret_cast<const T*>(&raw);
+      for (int q = 0; q < kWords; ++q) {
+        const bool on = w + 32 * q < w1;
+        const T* x = reinterpret_cast<const T*>(&next[q]);
 #pragma unroll
         for (int j = 0; j < Row::kVec; j += 4) {
-          const float4 f = make_float4(draw_logit(x[j]), draw_logit(x[j + 1]), draw_logit(x[j + 2]), draw_logit(x[j + 3]));
-          if (KEPT) reinterpret_cast<float4*>(r.z + r.head + at * Row::kVec)[j / 4] = f;
-          take(f.x, mine);
-          take(f.y, mine2);
-          take(f.z, mine);
-          take(f.w, mine2);
+          float4 f = make_float4(static_cast<float>(x[j]), static_cast<float>(x[j + 1]), static_cast<float>(x[j + 2]), static_cast<float>(x[j + 3]));
+          if (KEPT && on)
+            reinterpret_cast<float4*>(r.z + r.head + (w + 32 * q) * Row::kVec)[j / 4] = make_float4(draw_logit(f.x), draw_logit(f.y), draw_logit(f.z), draw_logit(f.w));
+          if (!on) f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          l[q * Row::kVec + j] = f.x;
+          l[q * Row::kVec + j + 1] = f.y;
+          l[q * Row::kVec + j + 2] = f.z;
+          l[q * Row::kVec + j + 3] = f.w;
         }
       }
+      fetch(w + 32 * kWords);
+      take(l);
     }
   }
   m = warp_max(m);
-  mine = warp_sum_f64(mine + mine2);
+  mine = warp_sum_f64(mine);
   if (lane == 0) {
     sh.warp_f[0][warp] = m;
     sh.warp_mass[0][warp] = mine;
@@ -500,9 +538,7 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
   // exp((l - m) / T) of this warp's elements >= bound
   auto weigh = [&](float bound, int slot) {
     double s0 = 0.0;
-    r.walk(warp, lane, [&](float l) {
-      if (l >= bound) s0 += r.mass(l);
-    });
+    r.walk(warp, lane, NAN, [&](const float (&l)[kDrawGroup]) { s0 += r.masses(l, bound); });
     s0 = warp_sum_f64(s0);
     if (lane == 0) sh.warp_mass[slot][warp] = s0;
   };
@@ -512,7 +548,7 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
     weigh(-INFINITY, slot = 1);
     row_sync(a.parts);
   } else {
-    const DrawPower q = draw_power(-static_cast<double>(m), r.scale, sh.table);
+    const DrawPower q = draw_power(-static_cast<double>(m), r.scale, r.table);
     factor = q.y * q.power;
   }
   const double all_mass = row_sum(sh.warp_mass[slot], a.parts, lane) * factor;        // of the unrestricted row
@@ -537,9 +573,8 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
 
   // what stays: logits >= threshold
   float threshold = -INFINITY;
-  int round = 0;
   if (by_rank)
-    threshold = draw_threshold<false>(r, sh, [&](auto f) { r.walk(warp, lane, f); }, 32.f * inv_t, static_cast<unsigned long long>(k), round);
+    threshold = draw_threshold<false>(r, sh, [&](auto f) { r.walk(warp, lane, NAN, f); }, n, 64.f * inv_t, static_cast<unsigned long long>(k));
   if (by_share) {
     // the least fp32 number l with (l - m) / T >= log(min_p), in 64 bits; from a rounded guess it is a step or two
     const double need = log(static_cast<double>(mp)) * static_cast<double>(t);
@@ -568,54 +603,42 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
       const double under = log(least * 0x1p-45) - 1e-5;
       reach = fmaxf(reach, static_cast<float>(static_cast<double>(m) + static_cast<double>(t) * under) - 1e-6f * fabsf(m));
     }
-    // this warp's, in a list of its own
+    // each lane's, in a column of its own of the warp's list
     int have = 0;
-    r.walk_batches(warp, lane, [&](const float (&l)[2 * Row::kVec], uint32_t there) {
-      uint32_t in = 0;
+    r.walk(warp, lane, NAN, [&](const float (&l)[kDrawGroup]) {
 #pragma unroll
-      for (int j = 0; j < 2 * Row::kVec; ++j)
-        if (((there >> j) & 1u) && l[j] >= reach) in |= 1u << j;
-      if (!__any_sync(0xffffffffu, in != 0)) return;
-      const int count = __popc(in);
-      int to = count;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, to, o);
-        if (lane >= o) to += v;
-      }
-      const int more = __shfl_sync(0xffffffffu, to, 31);
-      to += have - count;
-      have += more;
-#pragma unroll
-      for (int j = 0; j < 2 * Row::kVec; ++j)
-        if ((in >> j) & 1u) {
-          if (to < a.room) heavy[to] = l[j];
-          ++to;
+      for (int j = 0; j < kDrawGroup; ++j)
+        if (l[j] >= reach) {
+          if (have < a.room) heavy[have * 32 + lane] = l[j];
+          ++have;
         }
     });
-    __syncwarp();
-    const bool listed = have <= a.room;
+    const int most = __reduce_max_sync(0xffffffffu, have), together = __reduce_add_sync(0xffffffffu, have);
+    if (lane == 0) sh.warp_n[warp] = together;
+    __syncthreads();
+    const int elements = __reduce_add_sync(0xffffffffu, lane < kDrawWarps ? sh.warp_n[lane] : 0);
+    const bool listed = most <= a.room;       // else the warp's range takes the list's place
     auto each = [&](auto f) {
       if (!listed) {
-        r.walk(warp, lane, [&](float l) {
-          if (l >= reach) f(l);
+        r.walk(warp, lane, NAN, [&](float (&l)[kDrawGroup]) {
+#pragma unroll
+          for (int j = 0; j < kDrawGroup; ++j) l[j] = l[j] >= reach ? l[j] : NAN;
+          f(l);
         });
         return;
       }
-      int i = lane;
-      for (; i + 32 < have; i += 64) {
-        const float l0 = heavy[i], l1 = heavy[i + 32];
-        f(l0);
-        f(l1);
+#pragma unroll 1
+      for (int i = 0; i < most; i += kDrawGroup) {
+        float l[kDrawGroup];
+#pragma unroll
+        for (int j = 0; j < kDrawGroup; ++j) l[j] = i + j < have ? heavy[(i + j) * 32 + lane] : NAN;
+        f(l);
       }
-      if (i < have) f(heavy[i]);
     };
-    const float per_class = reach > -INFINITY && reach < m ? fminf((kDrawClasses - 0.1f) / (m - reach), 1e30f) : 32.f * inv_t;
-    threshold = fmaxf(threshold, draw_threshold<true>(r, sh, each, per_class, target, round));
+    const float per_class = reach > -INFINITY && reach < m ? fminf((kDrawClasses - 0.1f) / (m - reach), 1e30f) : 64.f * inv_t;
+    threshold = fmaxf(threshold, draw_threshold<true>(r, sh, each, elements, per_class, target));
     double s0 = 0.0;
-    each([&](float l) {
-      if (l >= threshold) s0 += r.mass(l);
-    });
+    each([&](const float (&l)[kDrawGroup]) { s0 += r.masses(l, threshold); });
     s0 = warp_sum_f64(s0);
     slot ^= 1;
     if (lane == 0) sh.warp_mass[slot][warp] = s0;
@@ -628,14 +651,14 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
     row_sync(a.parts);
   }
   if (warp == 0) {
-    // 32 ranges of up to 8 parts, eight a lane; a target that roundings put behind the last of their sums lies in the last that has mass
-    double v[8], total = 0.0;
+    // the ranges of up to 8 parts, some a lane; a target that roundings put behind the last of their sums lies in the last that has mass
+    double v[kDrawRanges], total = 0.0;
     const int q = lane / 4;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)        // relative to the largest's
-      v[j] = q < a.parts ? __longlong_as_double(ld_cluster_u64(map_to_cta(smem_u32(&sh.warp_mass[slot][lane % 4 * 8 + j]), q))) * factor : 0.0;
+    for (int j = 0; j < kDrawRanges; ++j)        // relative to the largest's
+      v[j] = q < a.parts ? __longlong_as_double(ld_cluster_u64(map_to_cta(smem_u32(&sh.warp_mass[slot][lane % 4 * kDrawRanges + j]), q))) * factor : 0.0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) total += v[j];
+    for (int j = 0; j < kDrawRanges; ++j) total += v[j];
     const double upto = warp_scan_f64(total, lane);
     double u;
     if (a.u == nullptr) {
@@ -658,7 +681,7 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
       double begins = before;
       bool found = false;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < kDrawRanges; ++j) {
         if (!found && v[j] > 0x1p-80) {
           range = j;
           begins = before;
@@ -666,48 +689,63 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
         before += v[j];
         found = found || (v[j] > 0x1p-80 && target < before);
       }
-      sh.owner = lane * 8 + range;
+      sh.owner = lane * kDrawRanges + range;
       sh.before = target - begins;            // within the range
     }
   }
   __syncthreads();
   if (sh.owner / kDrawWarps == part) {
-    // the range again, in 32 runs; then the run element by element
+    // the range again, a run to each warp; then the run element by element
     const double target = sh.before;
     const int lo = r.from(sh.owner % kDrawWarps), hi = r.to(sh.owner % kDrawWarps), run = (hi - lo + kDrawWarps - 1) / kDrawWarps;
     const int r0 = min(lo + warp * run, hi), r1 = min(r0 + run, hi);
-    double s = 0.0;
-    for (int i = r0 + lane; i < r1; i += 32) {
-      const float l = r.at(i);
-      if (l >= threshold) s += r.mass(l);
+    // of a run up to 256 elements stay in registers: their loads go out together, and the search takes them from there
+    constexpr int kHeld = 8;
+    float l[kHeld];
+    double w[kHeld], s = 0.0;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) l[j] = r0 + 32 * j + lane < r1 ? r.at(r0 + 32 * j + lane) : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      w[j] = r0 + 32 * j < r1 && l[j] >= threshold ? r.mass(l[j]) : 0.0;
+      s += w[j];
+    }
+    for (int i = r0 + 32 * kHeld + lane; i < r1; i += 32) {
+      const float x = r.at(i);
+      if (x >= threshold) s += r.mass(x);
     }
     s = warp_sum_f64(s);
     if (lane == 0) sh.sub[warp] = s;
     __syncthreads();
-    if (warp == 0) {
-      const double mass = sh.sub[lane], upto = warp_scan_f64(mass, lane);
-      const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0), behind = __ballot_sync(0xffffffffu, mass > 0.0 && target < upto);
-      const int at = behind ? __ffs(behind) - 1 : 31 - __clz(some);
-      double before = __shfl_sync(0xffffffffu, upto - mass, at);
-      const int e0 = min(lo + at * run, hi), e1 = min(e0 + run, hi);
+    const double mass = lane < kDrawWarps ? sh.sub[lane] : 0.0, upto = warp_scan_f64(mass, lane);
+    const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0), behind = __ballot_sync(0xffffffffu, mass > 0.0 && target < upto);
+    const int at = behind ? __ffs(behind) - 1 : 31 - __clz(some);
+    double before = __shfl_sync(0xffffffffu, upto - mass, at);
+    if (warp == at) {
       int drawn = -1;                         // the first behind which the target does not lie, or the last with any mass
-      for (int i0 = e0; i0 < e1; i0 += 32) {
-        const int i = i0 + lane;
-        const float l = i < e1 ? r.at(i) : -INFINITY;
-        const double w = i < e1 && l >= threshold ? r.mass(l) : 0.0;
-        const double upto_w = before + warp_scan_f64(w, lane);
-        const unsigned held = __ballot_sync(0xffffffffu, w > 0.0), hit = __ballot_sync(0xffffffffu, w > 0.0 && target < upto_w);
+      auto search = [&](int i0, double x) {
+        const double upto_x = before + warp_scan_f64(x, lane);
+        const unsigned held = __ballot_sync(0xffffffffu, x > 0.0), hit = __ballot_sync(0xffffffffu, x > 0.0 && target < upto_x);
         if (hit) {
           drawn = i0 + __ffs(hit) - 1;
-          break;
+          return true;
         }
         if (held) drawn = i0 + 31 - __clz(held);
-        before = __shfl_sync(0xffffffffu, upto_w, 31);
+        before = __shfl_sync(0xffffffffu, upto_x, 31);
+        return false;
+      };
+      bool found = false;
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j)
+        if (!found && r0 + 32 * j < r1) found = search(r0 + 32 * j, w[j]);
+      for (int i0 = r0 + 32 * kHeld; i0 < r1 && !found; i0 += 32) {
+        const float x = i0 + lane < r1 ? r.at(i0 + lane) : -INFINITY;
+        found = search(i0, i0 + lane < r1 && x >= threshold ? r.mass(x) : 0.0);
       }
       if (lane == 0) {
-        const float l = r.at(drawn);
+        const float x = r.at(drawn);
         a.tokens[b] = begin + drawn;
-        a.logprobs[b] = static_cast<float>((static_cast<double>(l) - static_cast<double>(m)) / static_cast<double>(t) - log(all_mass));
+        a.logprobs[b] = static_cast<float>((static_cast<double>(x) - static_cast<double>(m)) / static_cast<double>(t) - log(all_mass));
       }
     }
   }
@@ -737,7 +775,7 @@ static int launch_draw(DrawArgs a, int B, cudaStream_t s) {
   a.parts = parts;
   a.per = ((a.V + parts - 1) / parts + 7) / 8 * 8;
   const bool kept = a.per <= kDrawKept;
-  a.room = (kDrawBytes / 4 - (kept ? a.per + 4 : 0)) / kDrawWarps;
+  a.room = (kDrawBytes / 4 - (kept ? a.per + 4 : 0)) / kDrawThreads;
   return kept ? launch_draw_as<T, true>(a, B, s) : launch_draw_as<T, false>(a, B, s);
 }
 
