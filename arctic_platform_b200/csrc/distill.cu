@@ -203,7 +203,7 @@ distill_rows_kernel(const float* __restrict__ g_value, const float* __restrict__
                     float* __restrict__ out, int* __restrict__ no_label) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= N) return;
-  const float g = g_value[i];
+  const float g = g_value ? g_value[i] : 0.f;
   out[i] = (g_lp ? g_lp[i] : 0.f) - (g == 0.f ? 0.f : g * others[i]);
   no_label[i] = -1;
 }
@@ -220,7 +220,7 @@ distill_places_kernel(const int* __restrict__ names, const int* __restrict__ lab
   const float* zk = logit + static_cast<long long>(row) * (K + 1);
   const int label = labels[row];
   const float rs = scale * (row_scale ? row_scale[row] : 1.f);
-  const float gv = g_value[row], gl = g_lp ? g_lp[row] : 0.f, ge = g_ent ? g_ent[row] : 0.f, l = lse[row], en = ent[row];
+  const float gv = g_value ? g_value[row] : 0.f, gl = g_lp ? g_lp[row] : 0.f, ge = g_ent ? g_ent[row] : 0.f, l = lse[row], en = ent[row];
   __nv_bfloat16* to = d + row * ldd;
   bool label_named = false;
   for (int k = lane; k < K; k += 32) {
@@ -246,6 +246,10 @@ int launch_gemm_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GemmPar
 }  // namespace apb
 
 extern "C" {
+
+int apb_lmhead_dlogits(const void* hidden, const void* weight, const int* labels, const float* row_scale, const float* lse, const float* ent,
+                       const float* g_lp, const float* g_ent, void* dlogits, int M, int V, int H, long long ldh, long long ldw, long long ldd,
+                       float scale, cudaStream_t stream);
 
 // hidden [N, H] and weight [V, H] bf16 (H, V and the strides multiples of 8, 16-byte aligned), labels [N], names [N, K] int32 (K <= 256),
 // teacher [N, K] fp32, rest [N] fp32 or null, row_scale [N] or null (then `scale` alone).  Scratch: sorted [N, K] int32, partial
@@ -289,25 +293,26 @@ int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* la
   return static_cast<int>(cudaGetLastError());
 }
 
-// glp [N] fp32 and no_label [N] int32: what apb_lmhead_dlogits takes in place of the log-prob's upstream gradient and the labels.
-int apb_distill_rows(const float* g_value, const float* g_lp, const float* others, int N, float* glp, int* no_label, cudaStream_t stream) {
+// d(logits) [N, V] bf16 (row stride ldd) of the rows of a forward pass: the coefficients of their probabilities, the product whose epilogue
+// writes probability times coefficient, then the named tokens' places and the label's.  g_value, g_lp, g_ent [N] fp32: upstream gradients
+// (null: none); the others as kept by the forward pass.  Scratch: [2 N] words of 32 bits.
+int apb_lmhead_distill_dlogits(const void* hidden, const void* weight, const int* names, const int* labels, const float* row_scale,
+                               const float* logit, const float* named_grad, const float* others, const float* lse, const float* ent,
+                               const float* g_value, const float* g_lp, const float* g_ent, float* scratch, void* dlogits, int N, int V, int H,
+                               int K, long long ldh, long long ldw, long long ldd, float scale, cudaStream_t stream) {
   using namespace apb;
   if (N <= 0) return 0;
-  if (!g_value || !others || !glp || !no_label) return kBadArgument;
-  distill_rows_kernel<<<(N + 255) / 256, 256, 0, stream>>>(g_value, g_lp, others, N, glp, no_label);
-  return static_cast<int>(cudaGetLastError());
-}
-
-// The named tokens' places and the label's of d [N, V] bf16 (row stride ldd); arguments as kept by the forward pass.
-int apb_distill_places(const int* names, const int* labels, const float* logit, const float* named_grad, const float* others, const float* lse,
-                       const float* ent, const float* g_value, const float* g_lp, const float* g_ent, const float* row_scale, float scale,
-                       int K, int V, int N, void* d, long long ldd, cudaStream_t stream) {
-  using namespace apb;
-  if (N <= 0) return 0;
-  if (!labels || !logit || !others || !lse || !ent || !g_value || !d || K < 0 || K > kMostNamed || (K > 0 && (!names || !named_grad)))
+  if (!hidden || !weight || !labels || !logit || !others || !lse || !ent || !scratch || !dlogits || K < 0 || K > kMostNamed ||
+      (K > 0 && (!names || !named_grad)) || V <= 0 || H <= 0 || (ldd % 8))
     return kBadArgument;
+  int* no_label = reinterpret_cast<int*>(scratch + N);
+  distill_rows_kernel<<<(N + 255) / 256, 256, 0, stream>>>(g_value, g_lp, others, N, scratch, no_label);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const int rc = apb_lmhead_dlogits(hidden, weight, no_label, row_scale, lse, ent, scratch, g_ent, dlogits, N, V, H, ldh, ldw, ldd, scale, stream);
+  if (rc) return rc;
   distill_places_kernel<<<(N + 7) / 8, 256, 0, stream>>>(names, labels, logit, named_grad, others, lse, ent, g_value, g_lp, g_ent, row_scale,
-                                                         scale, K, V, N, static_cast<__nv_bfloat16*>(d), ldd);
+                                                         scale, K, V, N, static_cast<__nv_bfloat16*>(dlogits), ldd);
   return static_cast<int>(cudaGetLastError());
 }
 }

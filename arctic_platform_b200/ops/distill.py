@@ -31,9 +31,7 @@ def _fn(name: str):
         c, fns = ctypes, {}
         vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
         fns["fwd"] = _lib.declare("apb_lmhead_distill_fwd", [vp] * 16 + [i, i, i, i, ll, ll, f, f, vp])
-        fns["rows"] = _lib.declare("apb_distill_rows", [vp, vp, vp, i, vp, vp, vp])
-        fns["places"] = _lib.declare("apb_distill_places", [vp] * 11 + [f, i, i, i, vp, ll, vp])
-        fns["dlogits"] = _lib.declare("apb_lmhead_dlogits", [vp] * 9 + [i, i, i, ll, ll, ll, f, vp])
+        fns["dlogits"] = _lib.declare("apb_lmhead_distill_dlogits", [vp] * 15 + [i, i, i, i, ll, ll, ll, f, vp])
         _FN.update(fns)              # in one step: another thread may be looking
     return _FN[name]
 
@@ -82,21 +80,32 @@ def distill_ref(hidden, weight, labels, teacher_ids, teacher_logprobs, teacher_r
     return value, logprob, entropy
 
 
+def _split_pays(n: int, H: int, pairs: int) -> bool:
+    """Whether a product ``[n, H]`` over the vocabulary is cut into parts of it that add up in fp32: where its tiles of 256 x 256 leave much of
+    their last wave of CTA pairs idle (4096 x 2560: 160 tiles, 2.2 waves, 2.6 ms; in six parts 2.0 ms)."""
+    tiles = -(-n // 256) * -(-H // 256)
+    return tiles < 0.85 * pairs * -(-tiles // pairs)
+
+
 class _LmHeadDistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ids, teacher, rest, inv_temp_t, inv_temp_s, reverse, with_entropy, bwd_chunk):
         N, H = hidden.shape
         V, K = weight.shape[0], ids.shape[1]
-        f32 = dict(device=hidden.device, dtype=torch.float32)
-        partial = torch.empty((N, (V + 127) // 128, 4), **f32)
-        in_order = torch.empty((N, K), device=hidden.device, dtype=torch.int32)
-        logit, named = torch.empty((N, K + 1), **f32), torch.empty((N, K), **f32)
-        value, lp, ent, lse, others = torch.empty((5, N), **f32).unbind(0)
-        _lib.check(_fn("fwd")(_lib.ptr(hidden), _lib.ptr(weight), _lib.ptr(labels), _lib.ptr(ids), _lib.ptr(teacher), _lib.ptr(rest),
-                              _lib.ptr(inv_temp_t), _lib.ptr(partial), _lib.ptr(in_order), _lib.ptr(logit), _lib.ptr(value), _lib.ptr(lp),
-                              _lib.ptr(ent), _lib.ptr(lse), _lib.ptr(others), _lib.ptr(named), N, V, H, K, hidden.stride(0), weight.stride(0),
-                              inv_temp_s, reverse, _lib.stream_ptr()), "apb_lmhead_distill_fwd")
-        ctx.save_for_backward(hidden, weight, labels, ids, inv_temp_t, logit, named, others, lse, ent)
+        dev, f32 = hidden.device, torch.float32
+        partial = torch.empty((N, (V + 127) // 128, 4), device=dev, dtype=f32)
+        in_order = torch.empty((N, K), device=dev, dtype=torch.int32)
+        value, lp, ent = (torch.empty(N, device=dev, dtype=f32) for _ in range(3))
+        # what the backward pass takes up again: logits of the named tokens and the label, gradients of the named ones, two numbers a row
+        logit, named = torch.empty((N, K + 1), device=dev, dtype=f32), torch.empty((N, K), device=dev, dtype=f32)
+        rows = torch.empty((2, N), device=dev, dtype=f32)
+        lse = rows.data_ptr()
+        opt = lambda t: None if t is None else t.data_ptr()                                  # noqa: E731
+        _lib.check(_fn("fwd")(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), ids.data_ptr(), teacher.data_ptr(), opt(rest),
+                              opt(inv_temp_t), partial.data_ptr(), in_order.data_ptr(), logit.data_ptr(), value.data_ptr(), lp.data_ptr(),
+                              ent.data_ptr(), lse, lse + 4 * N, named.data_ptr(), N, V, H, K, hidden.stride(0), weight.stride(0), inv_temp_s,
+                              reverse, _lib.stream_ptr()), "apb_lmhead_distill_fwd")
+        ctx.save_for_backward(hidden, weight, labels, ids, inv_temp_t, logit, named, rows, ent)
         ctx.inv_temp_s, ctx.with_entropy, ctx.bwd_chunk = inv_temp_s, with_entropy, bwd_chunk
         ctx.set_materialize_grads(False)
         return value, lp, (ent if with_entropy else lp.new_zeros(0))
@@ -104,51 +113,47 @@ class _LmHeadDistillFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_value, g_lp, g_ent):
-        hidden, weight, labels, ids, it, logit, named, others, lse, ent = ctx.saved_tensors
+        hidden, weight, labels, ids, it, logit, named, rows, ent = ctx.saved_tensors
         N, H = hidden.shape
         V, K = weight.shape[0], ids.shape[1]
         dev = hidden.device
-        with torch.cuda.device(dev):
-            whole = lambda g: None if g is None else g.float().contiguous()                  # noqa: E731
-            g_value = torch.zeros(N, device=dev) if g_value is None else whole(g_value)
-            g_lp, g_ent = whole(g_lp), whole(g_ent) if ctx.with_entropy else None
-            glp = torch.empty(N, device=dev, dtype=torch.float32)
-            no_label = torch.empty(N, device=dev, dtype=torch.int32)
-            _lib.check(_fn("rows")(_lib.ptr(g_value), _lib.ptr(g_lp), _lib.ptr(others), N, _lib.ptr(glp), _lib.ptr(no_label),
-                                   _lib.stream_ptr()), "apb_distill_rows")
-            d_hidden = torch.empty((N, H), device=dev, dtype=hidden.dtype)
-            acc = getattr(weight, "grad_f32", None)
-            chunk = ctx.bwd_chunk
-            if chunk is None:
-                chunk = _bwd_rows(N, V, memory_budget.spare_bytes(dev, _BWD_BUDGET) if N > _BWD_ROWS else 0)
-            want_h, want_w = ctx.needs_input_grad[:2]
-            dw32 = None if not want_w else acc if acc is not None else torch.zeros((V, H), device=dev, dtype=torch.float32)
-            buf_rows = min(chunk, N) if ctx.bwd_chunk or N <= _BWD_ROWS else -(-chunk // _BWD_ROWS) * _BWD_ROWS
-            buf = torch.empty((buf_rows, V), device=dev, dtype=torch.bfloat16)
-            for s in range(0, N, chunk):
-                n = min(chunk, N - s)
-                rows = slice(s, s + n)
-                part = lambda t: _lib.ptr(None if t is None else t[rows])                     # noqa: E731
-                h, dl = hidden[rows], buf[:n]
-                _lib.check(_fn("dlogits")(_lib.ptr(h), _lib.ptr(weight), part(no_label), part(it), part(lse), part(ent), part(glp),
-                                          part(g_ent), _lib.ptr(dl), n, V, H, h.stride(0), weight.stride(0), dl.stride(0), ctx.inv_temp_s,
-                                          _lib.stream_ptr()), "apb_lmhead_dlogits")
-                _lib.check(_fn("places")(part(ids), part(labels), part(logit), part(named), part(others), part(lse), part(ent),
-                                         part(g_value), part(g_lp), part(g_ent), part(it), ctx.inv_temp_s, K, V, n, _lib.ptr(dl),
-                                         dl.stride(0), _lib.stream_ptr()), "apb_distill_places")
-                if not want_h:
-                    pass
-                elif -(-n // 256) * -(-H // 256) < torch.cuda.get_device_properties(dev).multi_processor_count // 2:
-                    # fewer tiles than CTA pairs: the vocabulary is cut into parts that add up in fp32, as in lm_head_logprobs
+        want_h, want_w = ctx.needs_input_grad[:2]
+        whole = lambda g: None if g is None else g.to(torch.float32).contiguous()            # noqa: E731
+        g_value, g_lp, g_ent = whole(g_value), whole(g_lp), whole(g_ent) if ctx.with_entropy else None
+        at = lambda t, s, size: None if t is None else t.data_ptr() + s * size               # noqa: E731
+        chunk = ctx.bwd_chunk
+        if chunk is None:
+            chunk = _bwd_rows(N, V, memory_budget.spare_bytes(dev, _BWD_BUDGET) if N > _BWD_ROWS else 0)
+        buf_rows = min(chunk, N) if ctx.bwd_chunk or N <= _BWD_ROWS else -(-chunk // _BWD_ROWS) * _BWD_ROWS
+        buf = torch.empty((buf_rows, V), device=dev, dtype=torch.bfloat16)
+        scratch = torch.empty(2 * min(chunk, N), device=dev, dtype=torch.float32)
+        d_hidden = torch.empty((N, H), device=dev, dtype=hidden.dtype) if want_h else None
+        acc = getattr(weight, "grad_f32", None) if want_w else None
+        # one chunk: the weight's gradient leaves its product in its own type; several add up in fp32
+        dw = None if not want_w or acc is not None else torch.empty((V, H), device=dev, dtype=weight.dtype) if chunk >= N else \
+            torch.zeros((V, H), device=dev, dtype=torch.float32)
+        pairs = torch.cuda.get_device_properties(dev).multi_processor_count // 2
+        lse = rows.data_ptr()
+        for s in range(0, N, chunk):
+            n = min(chunk, N - s)
+            h, dl = hidden[s:s + n], buf[:n]
+            _lib.check(_fn("dlogits")(h.data_ptr(), weight.data_ptr(), at(ids, s, 4 * K), at(labels, s, 4), at(it, s, 4),
+                                      at(logit, s, 4 * K + 4), at(named, s, 4 * K), lse + 4 * (N + s), lse + 4 * s, at(ent, s, 4),
+                                      at(g_value, s, 4), at(g_lp, s, 4), at(g_ent, s, 4), scratch.data_ptr(), dl.data_ptr(), n, V, H, K,
+                                      hidden.stride(0), weight.stride(0), V, ctx.inv_temp_s, _lib.stream_ptr()), "apb_lmhead_distill_dlogits")
+            if want_h:
+                if _split_pays(n, H, pairs):
                     total = torch.zeros((n, H), device=dev, dtype=torch.float32)
                     gemm.gemm_raw(dl, weight, total, M=n, N=H, K=V, b_mn=True, epi=gemm.EPI_F32_ACCUM)
-                    d_hidden[rows].copy_(total)
+                    d_hidden[s:s + n].copy_(total)
                 else:
-                    gemm.matmul_nn(dl, weight, out=d_hidden[rows])
-                if want_w:
-                    gemm.matmul_tn(dl, h, out=dw32, accumulate=True)
-            dw = None if acc is not None or not want_w else dw32.to(weight.dtype)
-        return d_hidden if want_h else None, dw, None, None, None, None, None, None, None, None, None
+                    gemm.matmul_nn(dl, weight, out=d_hidden[s:s + n])
+            if want_w:
+                into = acc if acc is not None else dw
+                gemm.matmul_tn(dl, h, out=into, accumulate=into.dtype == torch.float32)
+        if dw is not None and dw.dtype != weight.dtype:
+            dw = dw.to(weight.dtype)
+        return d_hidden, dw, None, None, None, None, None, None, None, None, None
 
 
 def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, teacher_ids: torch.Tensor,
@@ -191,16 +196,20 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
         # connected to its inputs, so that a shard without rows still has a gradient of zeros
         z = (hidden.sum() + weight[:0].sum()) * 0.0 + hidden.new_zeros(0, dtype=torch.float32)
         return z, z, (z if with_entropy else None)
-    with torch.cuda.device(hidden.device):
-        row16 = lambda t: t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 else t.contiguous()   # noqa: E731
-        whole = lambda t, dtype: t.detach().to(dtype).contiguous()                           # noqa: E731
-        it_t = whole(inv_temperature, torch.float32) if torch.is_tensor(inv_temperature) else None
-        if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.data_ptr() % 16:
-            raise ValueError("weight must have whole rows on 16-byte boundaries")
-        if teacher_ids.dtype == torch.int64:         # before 32 bits cut them
-            teacher_ids = torch.where((teacher_ids < 0) | (teacher_ids >= V), -1, teacher_ids)
-        value, lp, ent = _LmHeadDistillFn.apply(
-            row16(hidden), weight, whole(labels, torch.int32), whole(teacher_ids, torch.int32), whole(teacher_logprobs, torch.float32),
-            None if teacher_rest is None else whole(teacher_rest, torch.float32), it_t, 1.0 if it_t is not None else float(inv_temperature),
-            float(reverse), with_entropy, bwd_chunk)
+    if hidden.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(hidden.device):
+            return lm_head_distill(hidden, weight, labels, teacher_ids, teacher_logprobs, teacher_rest, inv_temperature, reverse, with_entropy,
+                                   bwd_chunk)
+    if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.data_ptr() % 16:
+        raise ValueError("weight must have whole rows on 16-byte boundaries")
+    if hidden.stride(1) != 1 or hidden.stride(0) % 8 or hidden.data_ptr() % 16:
+        hidden = hidden.contiguous()
+    whole = lambda t, dtype: t.detach().to(dtype).contiguous()                               # noqa: E731
+    if teacher_ids.dtype == torch.int64:         # before 32 bits cut them
+        teacher_ids = torch.where((teacher_ids < 0) | (teacher_ids >= V), -1, teacher_ids)
+    it_t = whole(inv_temperature, torch.float32) if torch.is_tensor(inv_temperature) else None
+    value, lp, ent = _LmHeadDistillFn.apply(
+        hidden, weight, whole(labels, torch.int32), whole(teacher_ids, torch.int32), whole(teacher_logprobs, torch.float32),
+        None if teacher_rest is None else whole(teacher_rest, torch.float32), it_t, 1.0 if it_t is not None else float(inv_temperature),
+        float(reverse), with_entropy, bwd_chunk)
     return value, lp, (ent if with_entropy else None)
