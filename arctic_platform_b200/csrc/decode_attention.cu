@@ -478,7 +478,8 @@ decode_cascade_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_co
         if (ok && live) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) tmem_ld_32x32(t_s + half * 64 + c * 32, sc[c]);
-          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 2; ++c) tmem_ld_wait(sc[c]);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -505,7 +506,7 @@ decode_cascade_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_co
                 for (int c = 0; c < 2; ++c) {
                   uint32_t r[32];
                   tmem_ld_32x32(t_o + c * 32, r);
-                  tmem_ld_wait();
+                  tmem_ld_wait(r);
 #pragma unroll
                   for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
                   tmem_st_32x32(t_o + c * 32, r);
@@ -549,7 +550,7 @@ decode_cascade_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_co
           for (int c = 0; c < 2; ++c) {
             uint32_t r[32];
             tmem_ld_32x32(t_o + c * 32, r);
-            tmem_ld_wait();
+            tmem_ld_wait(r);
             float4* dst = reinterpret_cast<float4*>(stage + row * kDaOutStride + half * 64 + c * 32);
 #pragma unroll
             for (int i = 0; i < 8; ++i)

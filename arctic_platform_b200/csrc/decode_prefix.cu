@@ -226,7 +226,8 @@ decode_prefix_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       float mx = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + c * 32, sc[c]);
-      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_wait(sc[c]);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -248,7 +249,7 @@ decode_prefix_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
           for (int c = 0; c < D / 32; ++c) {
             uint32_t r[32];
             tmem_ld_32x32(t_o + c * 32, r);
-            tmem_ld_wait();
+            tmem_ld_wait(r);
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
             tmem_st_32x32(t_o + c * 32, r);
@@ -289,7 +290,7 @@ decode_prefix_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         for (int c = 0; c < D / 32; ++c) {
           uint32_t r[32];
           tmem_ld_32x32(t_o + c * 32, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
 #pragma unroll
           for (int i = 0; i < 32; ++i) o_acc[c * 32 + i] = __uint_as_float(r[i]);
         }
