@@ -74,7 +74,7 @@ def _compile_one(src: Path, verbose: bool) -> Path:
 
 # what serving any stateful architecture needs: the status word, the GEMMs, the kernels of a ragged batch; each names the
 # sources of its own layers in models/registry.py
-SERVE_STEMS = ("status", "gemm_tcgen05", "gemm_tcgen05_2cta", "gemm_simt", "serve_layers")
+SERVE_STEMS = ("status", "gemm_tcgen05", "gemm_tcgen05_2cta", "gemm_simt", "serve_layers", "top_logprobs")
 
 
 def serve_lib(architecture: str) -> Path:

@@ -38,8 +38,9 @@ struct DrawArgs {
   const float* min_p;
   float temperature_all, top_p_all, min_p_all;
   int top_k_all;
-  const void* u;              // [B] fp32 or fp64; null: a hash of (seed, step, row)
-  const int* step;
+  const void* u;              // [B] fp32 or fp64; null: noise of every token by a hash of (seed, step, row, token)
+  const int* step;            // on the device, with `seed_dev` too: a captured launch sees new values
+  const int* seed_dev;        // or null: `seed`
   uint32_t seed;
   int u64;
   int V, parts, per, room;    // per: elements of a part; room: of a lane's list
@@ -156,7 +157,7 @@ struct DrawShared {
   unsigned long long weight[kDrawFew];
   double warp_mass[2][kDrawWarps], sub[kDrawWarps], before;
   unsigned long long scan[kDrawWarps], above;
-  float warp_f[2][kDrawWarps];
+  float warp_f[2][kDrawWarps], warp_key[kDrawWarps];
   int warp_i[kDrawWarps];
   int list_n[2], limb[2], warp_n[kDrawWarps], chosen, owner;
 };
@@ -301,25 +302,25 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int ele
       bool in[kDrawGroup];
 #pragma unroll
       for (int j = 0; j < kDrawGroup; ++j) in[j] = in_chosen(l[j], c[j]) && l[j] == l[j];
-      if (!MASS) {
+      if constexpr (!MASS) {
 #pragma unroll
         for (int j = 0; j < kDrawGroup; ++j)
           if (in[j]) atomicAdd(&h[0][c[j]], 1u);
-        return;
-      }
-      unsigned long long w[kDrawGroup];
+      } else {
+        unsigned long long w[kDrawGroup];
 #pragma unroll
-      for (int j = 0; j < kDrawGroup; ++j) w[j] = r.units(l[j]);       // at most 2^45: 3 limbs of 16 bits, 4 of 13
+        for (int j = 0; j < kDrawGroup; ++j) w[j] = r.units(l[j]);       // at most 2^45: 3 limbs of 16 bits, 4 of 13
 #pragma unroll
-      for (int j = 0; j < kDrawGroup; ++j) {
-        if (!in[j]) continue;
-        const uint32_t mask = (1u << limb) - 1u;
-        atomicAdd(&h[0][c[j]], static_cast<uint32_t>(w[j]) & mask);
-        atomicAdd(&h[1][c[j]], static_cast<uint32_t>(w[j] >> limb) & mask);
-        const uint32_t rest = static_cast<uint32_t>(w[j] >> (2 * limb));         // most have no more
-        if (rest) {
-          atomicAdd(&h[2][c[j]], rest & mask);
-          if (rest >> limb) atomicAdd(&h[3][c[j]], rest >> limb);
+        for (int j = 0; j < kDrawGroup; ++j) {
+          if (!in[j]) continue;
+          const uint32_t mask = (1u << limb) - 1u;
+          atomicAdd(&h[0][c[j]], static_cast<uint32_t>(w[j]) & mask);
+          atomicAdd(&h[1][c[j]], static_cast<uint32_t>(w[j] >> limb) & mask);
+          const uint32_t rest = static_cast<uint32_t>(w[j] >> (2 * limb));         // most have no more
+          if (rest) {
+            atomicAdd(&h[2][c[j]], rest & mask);
+            if (rest >> limb) atomicAdd(&h[3][c[j]], rest >> limb);
+          }
         }
       }
     });
@@ -418,7 +419,8 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int ele
   return -INFINITY;
 }
 
-template <typename T, bool KEPT>
+// GIVEN: by a given number, else by noise
+template <typename T, bool KEPT, bool GIVEN>
 __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a) {
   pdl_entry();
   extern __shared__ __align__(16) unsigned char draw_smem[];
@@ -644,126 +646,181 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
     if (lane == 0) sh.warp_mass[slot][warp] = s0;
   }
 
-  // masses of what stays
-  if (by_rank || by_share || by_mass) {
-    if (!by_mass) weigh(threshold, slot ^= 1);
-    factor = 1.0;
+  if constexpr (!GIVEN) {
+    // The largest of l / T and a noise of each token's own, numbers and rounding as in decode.cu's draws: a restriction changes what is drawn only
+    // where it leaves that token out, and logits that differ in their last bits seldom change it.
+    const uint32_t step = a.step ? static_cast<uint32_t>(*a.step) : 0u, seed = a.seed_dev ? static_cast<uint32_t>(*a.seed_dev) : a.seed;
+    const uint32_t base = draw_hash(seed ^ (step * 0x9E3779B9u)) ^ draw_hash(static_cast<uint32_t>(b) * 0x85ebca6bU + 1u);
+    float best = -INFINITY;
+    int best_i = 0x7fffffff;
+    const int hi = r.to(warp);
+#pragma unroll 4
+    for (int i = r.from(warp) + lane; i < hi; i += 32) {
+      const float l = r.at(i);
+      if (!(l >= threshold)) continue;
+      const uint32_t h = draw_hash(base + static_cast<uint32_t>(begin + i) * 0x9E3779B9u);
+      const float x = (static_cast<float>(h >> 8) + 0.5f) * (1.f / 16777216.f);
+      const float key = l * inv_t - __logf(-__logf(x));
+      if (key > best) {
+        best = key;
+        best_i = begin + i;
+      }
+    }
+    auto join = [&]() {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float key = __shfl_xor_sync(0xffffffffu, best, o);
+        const int i = __shfl_xor_sync(0xffffffffu, best_i, o);
+        if (key > best || (key == best && i < best_i)) {
+          best = key;
+          best_i = i;
+        }
+      }
+    };
+    join();
+    if (lane == 0) {
+      sh.warp_key[warp] = best;
+      sh.warp_i[warp] = best_i;
+    }
     row_sync(a.parts);
-  }
-  if (warp == 0) {
-    // the ranges of up to 8 parts, some a lane; a target that roundings put behind the last of their sums lies in the last that has mass
-    double v[kDrawRanges], total = 0.0;
-    const int q = lane / 4;
-#pragma unroll
-    for (int j = 0; j < kDrawRanges; ++j)        // relative to the largest's
-      v[j] = q < a.parts ? __longlong_as_double(ld_cluster_u64(map_to_cta(smem_u32(&sh.warp_mass[slot][lane % 4 * kDrawRanges + j]), q))) * factor : 0.0;
-#pragma unroll
-    for (int j = 0; j < kDrawRanges; ++j) total += v[j];
-    const double upto = warp_scan_f64(total, lane);
-    double u;
-    if (a.u == nullptr) {
-      const uint32_t step = a.step ? static_cast<uint32_t>(*a.step) : 0u;
-      const uint32_t base = draw_hash(a.seed ^ (step * 0x9E3779B9u)) ^ draw_hash(static_cast<uint32_t>(b) * 0x85ebca6bU + 1u);
-      u = (static_cast<double>(draw_hash(base + 0x9E3779B9u)) + static_cast<double>(draw_hash(base ^ 0x85ebca6bU)) * 0x1p-32) * 0x1p-32;
-    } else {
-      u = a.u64 ? static_cast<const double*>(a.u)[b] : static_cast<double>(static_cast<const float*>(a.u)[b]);
-    }
-    // 1 and above, and what is not a number, stand for the largest number below 1
-    u = u < 1.0 ? fmax(u, 0.0) : 1.0 - 0x1p-52;
-    const double target = u * __shfl_sync(0xffffffffu, upto, 31);
-    // a range of less than 2^-80 has only elements that a mass is not formed of (below e^-70 of the largest), or none
-    const unsigned behind = __ballot_sync(0xffffffffu, total > 0x1p-80 && target < upto), some = __ballot_sync(0xffffffffu, total > 0x1p-80);
-    const int owner = behind ? __ffs(behind) - 1 : 31 - __clz(some);
-    double before = __shfl_up_sync(0xffffffffu, upto, 1);
-    if (lane == 0) before = 0.0;
-    if (lane == owner) {
-      int range = 0;
-      double begins = before;
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < kDrawRanges; ++j) {
-        if (!found && v[j] > 0x1p-80) {
-          range = j;
-          begins = before;
+    if (part == 0 && warp == 0) {
+      best = -INFINITY;
+      best_i = 0x7fffffff;
+      for (int p = 0; p < a.parts; ++p) {
+        if (lane >= kDrawWarps) break;
+        const float key = ld_cluster_f32(map_to_cta(smem_u32(&sh.warp_key[lane]), p));
+        const int i = static_cast<int>(ld_cluster_u32(map_to_cta(smem_u32(&sh.warp_i[lane]), p)));
+        if (key > best || (key == best && i < best_i)) {
+          best = key;
+          best_i = i;
         }
-        before += v[j];
-        found = found || (v[j] > 0x1p-80 && target < before);
       }
-      sh.owner = lane * kDrawRanges + range;
-      sh.before = target - begins;            // within the range
-    }
-  }
-  __syncthreads();
-  if (sh.owner / kDrawWarps == part) {
-    // the range again, a run to each warp; then the run element by element
-    const double target = sh.before;
-    const int lo = r.from(sh.owner % kDrawWarps), hi = r.to(sh.owner % kDrawWarps), run = (hi - lo + kDrawWarps - 1) / kDrawWarps;
-    const int r0 = min(lo + warp * run, hi), r1 = min(r0 + run, hi);
-    // of a run up to 256 elements stay in registers: their loads go out together, and the search takes them from there
-    constexpr int kHeld = 8;
-    float l[kHeld];
-    double w[kHeld], s = 0.0;
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) l[j] = r0 + 32 * j + lane < r1 ? r.at(r0 + 32 * j + lane) : -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      w[j] = r0 + 32 * j < r1 && l[j] >= threshold ? r.mass(l[j]) : 0.0;
-      s += w[j];
-    }
-    for (int i = r0 + 32 * kHeld + lane; i < r1; i += 32) {
-      const float x = r.at(i);
-      if (x >= threshold) s += r.mass(x);
-    }
-    s = warp_sum_f64(s);
-    if (lane == 0) sh.sub[warp] = s;
-    __syncthreads();
-    const double mass = lane < kDrawWarps ? sh.sub[lane] : 0.0, upto = warp_scan_f64(mass, lane);
-    const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0), behind = __ballot_sync(0xffffffffu, mass > 0.0 && target < upto);
-    const int at = behind ? __ffs(behind) - 1 : 31 - __clz(some);
-    double before = __shfl_sync(0xffffffffu, upto - mass, at);
-    if (warp == at) {
-      int drawn = -1;                         // the first behind which the target does not lie, or the last with any mass
-      auto search = [&](int i0, double x) {
-        const double upto_x = before + warp_scan_f64(x, lane);
-        const unsigned held = __ballot_sync(0xffffffffu, x > 0.0), hit = __ballot_sync(0xffffffffu, x > 0.0 && target < upto_x);
-        if (hit) {
-          drawn = i0 + __ffs(hit) - 1;
-          return true;
-        }
-        if (held) drawn = i0 + 31 - __clz(held);
-        before = __shfl_sync(0xffffffffu, upto_x, 31);
-        return false;
-      };
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < kHeld; ++j)
-        if (!found && r0 + 32 * j < r1) found = search(r0 + 32 * j, w[j]);
-      for (int i0 = r0 + 32 * kHeld; i0 < r1 && !found; i0 += 32) {
-        const float x = i0 + lane < r1 ? r.at(i0 + lane) : -INFINITY;
-        found = search(i0, i0 + lane < r1 && x >= threshold ? r.mass(x) : 0.0);
-      }
+      __syncwarp();
+      join();
       if (lane == 0) {
-        const float x = r.at(drawn);
-        a.tokens[b] = begin + drawn;
-        a.logprobs[b] = static_cast<float>((static_cast<double>(x) - static_cast<double>(m)) / static_cast<double>(t) - log(all_mass));
+        // the largest always stays, so there is one; its key can be -inf only where T is so small that l / T is
+        const int i = best_i < a.V ? best_i : 0;
+        const float l = r.seen(draw_logit(static_cast<const T*>(a.logits)[b * a.ld + i]));
+        a.tokens[b] = i;
+        a.logprobs[b] = static_cast<float>((static_cast<double>(l) - static_cast<double>(m)) / static_cast<double>(t) - log(all_mass));
       }
     }
+    row_sync(a.parts);
+  } else {
+    // masses of what stays
+    if (by_rank || by_share || by_mass) {
+      if (!by_mass) weigh(threshold, slot ^= 1);
+      factor = 1.0;
+      row_sync(a.parts);
+    }
+    if (warp == 0) {
+      // the ranges of up to 8 parts, some a lane; a target that roundings put behind the last of their sums lies in the last that has mass
+      double v[kDrawRanges], total = 0.0;
+      const int q = lane / 4;
+#pragma unroll
+      for (int j = 0; j < kDrawRanges; ++j)        // relative to the largest's
+        v[j] = q < a.parts ? __longlong_as_double(ld_cluster_u64(map_to_cta(smem_u32(&sh.warp_mass[slot][lane % 4 * kDrawRanges + j]), q))) * factor : 0.0;
+#pragma unroll
+      for (int j = 0; j < kDrawRanges; ++j) total += v[j];
+      const double upto = warp_scan_f64(total, lane);
+      double u = a.u64 ? static_cast<const double*>(a.u)[b] : static_cast<double>(static_cast<const float*>(a.u)[b]);
+      // 1 and above, and what is not a number, stand for the largest number below 1
+      u = u < 1.0 ? fmax(u, 0.0) : 1.0 - 0x1p-52;
+      const double target = u * __shfl_sync(0xffffffffu, upto, 31);
+      // a range of less than 2^-80 has only elements that a mass is not formed of (below e^-70 of the largest), or none
+      const unsigned behind = __ballot_sync(0xffffffffu, total > 0x1p-80 && target < upto), some = __ballot_sync(0xffffffffu, total > 0x1p-80);
+      const int owner = behind ? __ffs(behind) - 1 : 31 - __clz(some);
+      double before = __shfl_up_sync(0xffffffffu, upto, 1);
+      if (lane == 0) before = 0.0;
+      if (lane == owner) {
+        int range = 0;
+        double begins = before;
+        bool found = false;
+#pragma unroll
+        for (int j = 0; j < kDrawRanges; ++j) {
+          if (!found && v[j] > 0x1p-80) {
+            range = j;
+            begins = before;
+          }
+          before += v[j];
+          found = found || (v[j] > 0x1p-80 && target < before);
+        }
+        sh.owner = lane * kDrawRanges + range;
+        sh.before = target - begins;            // within the range
+      }
+    }
+    __syncthreads();
+    if (sh.owner / kDrawWarps == part) {
+      // the range again, a run to each warp; then the run element by element
+      const double target = sh.before;
+      const int lo = r.from(sh.owner % kDrawWarps), hi = r.to(sh.owner % kDrawWarps), run = (hi - lo + kDrawWarps - 1) / kDrawWarps;
+      const int r0 = min(lo + warp * run, hi), r1 = min(r0 + run, hi);
+      // of a run up to 256 elements stay in registers: their loads go out together, and the search takes them from there
+      constexpr int kHeld = 8;
+      float l[kHeld];
+      double w[kHeld], s = 0.0;
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) l[j] = r0 + 32 * j + lane < r1 ? r.at(r0 + 32 * j + lane) : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) {
+        w[j] = r0 + 32 * j < r1 && l[j] >= threshold ? r.mass(l[j]) : 0.0;
+        s += w[j];
+      }
+      for (int i = r0 + 32 * kHeld + lane; i < r1; i += 32) {
+        const float x = r.at(i);
+        if (x >= threshold) s += r.mass(x);
+      }
+      s = warp_sum_f64(s);
+      if (lane == 0) sh.sub[warp] = s;
+      __syncthreads();
+      const double mass = lane < kDrawWarps ? sh.sub[lane] : 0.0, upto = warp_scan_f64(mass, lane);
+      const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0), behind = __ballot_sync(0xffffffffu, mass > 0.0 && target < upto);
+      const int at = behind ? __ffs(behind) - 1 : 31 - __clz(some);
+      double before = __shfl_sync(0xffffffffu, upto - mass, at);
+      if (warp == at) {
+        int drawn = -1;                         // the first behind which the target does not lie, or the last with any mass
+        auto search = [&](int i0, double x) {
+          const double upto_x = before + warp_scan_f64(x, lane);
+          const unsigned held = __ballot_sync(0xffffffffu, x > 0.0), hit = __ballot_sync(0xffffffffu, x > 0.0 && target < upto_x);
+          if (hit) {
+            drawn = i0 + __ffs(hit) - 1;
+            return true;
+          }
+          if (held) drawn = i0 + 31 - __clz(held);
+          before = __shfl_sync(0xffffffffu, upto_x, 31);
+          return false;
+        };
+        bool found = false;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+          if (!found && r0 + 32 * j < r1) found = search(r0 + 32 * j, w[j]);
+        for (int i0 = r0 + 32 * kHeld; i0 < r1 && !found; i0 += 32) {
+          const float x = i0 + lane < r1 ? r.at(i0 + lane) : -INFINITY;
+          found = search(i0, i0 + lane < r1 && x >= threshold ? r.mass(x) : 0.0);
+        }
+        if (lane == 0) {
+          const float x = r.at(drawn);
+          a.tokens[b] = begin + drawn;
+          a.logprobs[b] = static_cast<float>((static_cast<double>(x) - static_cast<double>(m)) / static_cast<double>(t) - log(all_mass));
+        }
+      }
+    }
+    row_sync(a.parts);                          // nobody leaves while its shared memory may be read
   }
-  row_sync(a.parts);                          // nobody leaves while its shared memory may be read
 }
 
-template <typename T, bool KEPT>
+template <typename T, bool KEPT, bool GIVEN>
 static int launch_draw_as(const DrawArgs& a, int B, cudaStream_t s) {
   static int allowed[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!allowed[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(draw_kernel<T, KEPT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(draw_kernel<T, KEPT, GIVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                kDrawShared + kDrawBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
     allowed[dev & 63] = 1;
   }
-  return static_cast<int>(launch_kernel_clusters(draw_kernel<T, KEPT>, dim3(static_cast<unsigned>(B) * a.parts), dim3(kDrawThreads),
+  return static_cast<int>(launch_kernel_clusters(draw_kernel<T, KEPT, GIVEN>, dim3(static_cast<unsigned>(B) * a.parts), dim3(kDrawThreads),
                                                  kDrawShared + kDrawBytes, a.parts, s, a));
 }
 
@@ -776,7 +833,8 @@ static int launch_draw(DrawArgs a, int B, cudaStream_t s) {
   a.per = ((a.V + parts - 1) / parts + 7) / 8 * 8;
   const bool kept = a.per <= kDrawKept;
   a.room = (kDrawBytes / 4 - (kept ? a.per + 4 : 0)) / kDrawThreads;
-  return kept ? launch_draw_as<T, true>(a, B, s) : launch_draw_as<T, false>(a, B, s);
+  if (!a.u) return kept ? launch_draw_as<T, true, false>(a, B, s) : launch_draw_as<T, false, false>(a, B, s);
+  return kept ? launch_draw_as<T, true, true>(a, B, s) : launch_draw_as<T, false, true>(a, B, s);
 }
 
 }  // namespace apb
@@ -785,15 +843,16 @@ extern "C" {
 
 // logits [B, V], row stride ld: type 0 fp32, 1 bf16, 2 fp16.  Of each setting a tensor [B] (fp32, top_k int32) or null and one number
 // for all rows: temperature (<= 0: the first of the largest logits), top_k (<= 0: off), top_p (>= 1: off), min_p (<= 0: off).  u [B] in
-// [0, 1): fp32, or fp64 with u64; null: a hash of seed, *step (null: 0) and the row.  tokens [B] int32, logprobs [B] fp32.  V up to 393216.
+// [0, 1): fp32, or fp64 with u64; null: the largest of logit / T and noise of each token's own, a hash of *seed_dev (null: seed), *step (null:
+// 0), the row and the token.  tokens [B] int32, logprobs [B] fp32.  V up to 393216.
 int apb_draw(const void* logits, int type, long long ld, const float* temperature, float temperature_all, const int* top_k, int top_k_all,
-             const float* top_p, float top_p_all, const float* min_p, float min_p_all, const void* u, int u64, unsigned seed, const int* step,
-             int B, int V, int* tokens, float* logprobs, cudaStream_t s) {
+             const float* top_p, float top_p_all, const float* min_p, float min_p_all, const void* u, int u64, unsigned seed,
+             const int* seed_dev, const int* step, int B, int V, int* tokens, float* logprobs, cudaStream_t s) {
   using namespace apb;
   if (B <= 0) return 0;
   if (!logits || !tokens || !logprobs || V < 1 || V > kDrawMost || type < 0 || type > 2) return kBadArgument;
   DrawArgs a{logits, ld, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all,
-             u, step, static_cast<uint32_t>(seed), u64, V, 1, 0, 0, tokens, logprobs};
+             u, step, seed_dev, static_cast<uint32_t>(seed), u64, V, 1, 0, 0, tokens, logprobs};
   if (type == 0) return launch_draw<float>(a, B, s);
   if (type == 1) return launch_draw<__nv_bfloat16>(a, B, s);
   return launch_draw<__half>(a, B, s);

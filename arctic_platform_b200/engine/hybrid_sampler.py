@@ -26,7 +26,7 @@ import torch.nn.functional as F
 from ..models.decoder import _qknorm_partial_rope, gate_up_act
 from ..ops import gemm, norm
 from ..ops.attention import AttnLayout
-from .reference_sampler import EXTRA_KEYS, LogitsProcessor, ReferenceSampler, filter_logits
+from .reference_sampler import EXTRA_KEYS, LogitsProcessor, ReferenceSampler, filter_logits, shaping_of
 from .sampler import SamplingParams
 
 
@@ -170,7 +170,7 @@ class HybridSampler(ReferenceSampler):
     def generate(self, prompts: Sequence[Sequence[int]], sampling_params=None) -> List[dict]:
         sp = sampling_params if isinstance(sampling_params, SamplingParams) else \
             SamplingParams.from_dict(sampling_params, supported=EXTRA_KEYS)
-        self._raw_params = sampling_params if isinstance(sampling_params, dict) else None
+        self._raw_params = shaping_of(sampling_params)
         if self._asleep:
             raise RuntimeError("sampler is asleep; call wake() first")
         if sp.seed is not None:

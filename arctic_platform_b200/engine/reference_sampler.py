@@ -34,6 +34,13 @@ def filter_logits(logits: torch.Tensor, top_k: int, top_p: float) -> torch.Tenso
 EXTRA_KEYS = ("repetition_penalty", "presence_penalty", "frequency_penalty", "min_p", "min_tokens", "logit_bias")
 
 
+def shaping_of(sampling_params) -> Optional[dict]:
+    """What :class:`LogitsProcessor` takes of the parameters of a call: a dict's keys, the ``min_p`` of :class:`SamplingParams`."""
+    if isinstance(sampling_params, SamplingParams):
+        return {"min_p": sampling_params.min_p}
+    return sampling_params if isinstance(sampling_params, dict) else None
+
+
 class LogitsProcessor:
     """Distribution shaping that the tensor-op samplers implement beyond temperature / top-k / top-p, in the order
     vLLM applies it: ``logit_bias``, repetition penalty (prompt and output tokens: positive logits divided, negative
@@ -102,7 +109,7 @@ class ReferenceSampler:
         stops = set(int(t) for t in sp.stop_token_ids)
         if self.eos is not None and not sp.ignore_eos:
             stops.add(int(self.eos))
-        shaper = LogitsProcessor(sampling_params if isinstance(sampling_params, dict) else None, sorted(stops))
+        shaper = LogitsProcessor(shaping_of(sampling_params), sorted(stops))
         results: List[dict] = []
         for pi, prompt in enumerate(prompts):
             if len(prompt) == 0:

@@ -37,7 +37,7 @@ import torch
 
 from ..models.config import DecoderConfig
 from ..models.decoder import DecoderLM
-from ..ops import _lib, gemm, kv_fp8, norm
+from ..ops import _lib, gemm, kv_fp8, norm, sampling
 from ..ops.attention import AttnLayout, attention_fwd_cuda
 from ..utils.transfer_stats import to_device, to_host
 
@@ -62,13 +62,14 @@ class SamplingParams:
     ignore_eos: bool = False
     logprobs: Optional[int] = None
     seed: Optional[int] = None
+    min_p: float = 0.0          # tokens below this share of the most likely one's probability are dropped (0: none)
 
     @staticmethod
     def from_dict(d: Optional[dict], supported: Tuple[str, ...] = ()) -> "SamplingParams":
         """``supported`` names extra keys the calling engine implements itself (they are then not reported)."""
         d = dict(d or {})
         sp = SamplingParams()
-        for k in ("n", "temperature", "max_tokens", "top_p", "top_k", "ignore_eos", "logprobs", "seed"):
+        for k in ("n", "temperature", "max_tokens", "top_p", "top_k", "ignore_eos", "logprobs", "seed", "min_p"):
             if k in d and d[k] is not None:
                 setattr(sp, k, d[k])
         if d.get("stop_token_ids"):
@@ -379,6 +380,9 @@ class SamplerEngine:
         self.d_topp = torch.ones(B, device=dev, dtype=torch.float32)
         self.d_thr = torch.zeros(B, device=dev, dtype=torch.float32)
         self._filter_on = False
+        self.d_minp = torch.zeros(B, device=dev, dtype=torch.float32)
+        self.d_seed = torch.zeros(1, **i32)
+        self._min_p_on = False
         self.splits = 4
         self.n_groups = B            # rows in use in the node tables (a power-of-two bucket bounds the prefix grid)
         f32 = dict(device=dev, dtype=torch.float32)
@@ -615,7 +619,10 @@ class SamplerEngine:
         prev_chain = _fn("chain")(1)
         try:
             logits = self._decode_logits(B)
-            if self._filter_on:
+            if self._min_p_on:
+                sampling.draw_raw(logits, None, self.d_temp, self.d_topk, self.d_topp, self.d_minp, self.d_new_tok, self.d_new_lp,
+                                  self.d_seed, self.d_step)
+            elif self._filter_on:
                 _lib.check(_fn("sample_f")(_lib.ptr(logits), logits.stride(0), _lib.ptr(self.d_temp), B, c.vocab_size,
                                            ctypes.c_uint(self.seed & 0xFFFFFFFF), _lib.ptr(self.d_step),
                                            _lib.ptr(self.d_topk), _lib.ptr(self.d_topp), _lib.ptr(self.d_thr),
@@ -780,7 +787,7 @@ class SamplerEngine:
                 self._decode_step(B)
             return
         nodes = self._group_bucket() if self._cascade_on() else 0
-        key = (B, nodes, self.n_levels, self._filter_on, nodes == 0 or self._one_launch, self._longest)
+        key = (B, nodes, self.n_levels, self._filter_on, self._min_p_on, nodes == 0 or self._one_launch, self._longest)
         g = self._graphs.get(key)
         if g is None:
             # the first steps run eagerly (kernel attribute set-up, device binding, allocator warm-up)
@@ -803,7 +810,8 @@ class SamplerEngine:
     def generate(self, prompts: Sequence[Sequence[int]], sampling_params=None) -> List[dict]:
         """Generates ``n`` samples per prompt.  Returns one record per sample, prompt-major:
         ``{"token_ids", "logprobs", "finish_reason", "prompt_len", "prompt_index", "text"}``."""
-        sp = sampling_params if isinstance(sampling_params, SamplingParams) else SamplingParams.from_dict(sampling_params)
+        sp = sampling_params if isinstance(sampling_params, SamplingParams) else \
+            SamplingParams.from_dict(sampling_params, supported=("min_p",))
         if self._asleep:
             raise RuntimeError("sampler is asleep; call wake() first")
         if self.fp8 and self._fp8_stale:
@@ -811,6 +819,8 @@ class SamplerEngine:
         self._filter_on = bool((sp.top_k is not None and sp.top_k > 0) or sp.top_p < 1.0)
         self.d_topk.fill_(int(sp.top_k) if sp.top_k and sp.top_k > 0 else 0)
         self.d_topp.fill_(float(sp.top_p))
+        self._min_p_on = sp.min_p is not None and float(sp.min_p) > 0.0
+        self.d_minp.fill_(float(sp.min_p or 0.0))
         if getattr(self, "d_arrived", None) is not None:
             self.d_arrived.zero_()         # a call that an error ended may have left arrivals behind
         self._own[:] = 0
@@ -837,6 +847,7 @@ class SamplerEngine:
         if sp.seed is not None:
             self.seed = int(sp.seed)
             self.d_step.zero_()            # a seeded call restarts the random stream
+        self.d_seed.fill_((self.seed + (1 << 31)) % (1 << 32) - (1 << 31))
         results: List[Optional[dict]] = [None] * (len(prompts_np) * sp.n)
         # work queue: runs of prompts that start with the same (page-aligned) header; a run is admitted as a whole --
         # its header is prefilled and stored once, every prompt's n rollouts form one prompt node below it
@@ -1125,7 +1136,10 @@ class SamplerEngine:
             tok0 = torch.empty(n, device=self.device, dtype=torch.int32)
             lp0 = torch.empty(n, device=self.device, dtype=torch.float32)
             seed0 = ctypes.c_uint((self.seed * 2654435761 + 12345) & 0xFFFFFFFF)
-            if self._filter_on:       # the first token obeys the same top-k / top-p cut-off as the decode steps
+            if self._min_p_on:
+                sampling.draw_raw(logits, None, temp, int(sp.top_k or 0), float(sp.top_p), float(sp.min_p), tok0, lp0,
+                                  self.seed * 2654435761 + 12345, self.d_step)
+            elif self._filter_on:       # the first token obeys the same top-k / top-p cut-off as the decode steps
                 topk0 = torch.full((n,), int(sp.top_k) if sp.top_k and sp.top_k > 0 else 0, device=self.device, dtype=torch.int32)
                 topp0 = torch.full((n,), float(sp.top_p), device=self.device, dtype=torch.float32)
                 thr0 = torch.empty(n, device=self.device, dtype=torch.float32)

@@ -34,7 +34,7 @@ import torch
 from ..models.config import DecoderConfig
 from ..models.decoder import DecoderLM
 from ..ops.attention import AttnLayout
-from .reference_sampler import EXTRA_KEYS, LogitsProcessor, ReferenceSampler, filter_logits
+from .reference_sampler import EXTRA_KEYS, LogitsProcessor, ReferenceSampler, filter_logits, shaping_of
 from .sampler import SamplingParams
 
 
@@ -82,7 +82,7 @@ class SpeculativeSampler(ReferenceSampler):
     def generate(self, prompts: Sequence[Sequence[int]], sampling_params=None) -> List[dict]:
         sp = sampling_params if isinstance(sampling_params, SamplingParams) else \
             SamplingParams.from_dict(sampling_params, supported=EXTRA_KEYS)
-        if LogitsProcessor(sampling_params if isinstance(sampling_params, dict) else None).active:
+        if LogitsProcessor(shaping_of(sampling_params)).active:
             return super().generate(prompts, sampling_params)      # history-dependent shaping: plain decoding
         if self._asleep:
             raise RuntimeError("sampler is asleep; call wake() first")

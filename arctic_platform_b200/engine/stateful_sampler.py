@@ -30,6 +30,7 @@ import numpy as np
 import torch
 
 from ..models import registry
+from ..ops.logprob import best_tokens
 from ..ops.serving import PAGE, StepBatch, StepEntry
 from ..utils.transfer_stats import to_device
 from .sampler import SamplerEngine, _Seq
@@ -259,12 +260,12 @@ class StatefulSampler(SamplerEngine):
                     z = self.step([(slot, part, want)])
                     if not want:
                         continue
+                    if top_k > 1:
+                        v, i = best_tokens(z, int(top_k))
+                        top += [dict(zip(ii, vv)) for ii, vv in zip(i.tolist(), v.tolist())]
                     z = torch.log_softmax(z, -1)
                     nxt = torch.tensor([seq[at + w + 1] for w in want], device=z.device)
                     lp += z.gather(1, nxt[:, None])[:, 0].tolist()
-                    if top_k > 1:
-                        v, i = torch.topk(z, int(top_k), dim=-1)
-                        top += [dict(zip(ii, vv)) for ii, vv in zip(i.tolist(), v.tolist())]
             finally:
                 self.close_sequence(slot)
             rows.append(lp)

@@ -566,6 +566,7 @@ class EngineWorker:
         most likely tokens with their log-probs (``{"log_probs": rows, "top_log_probs": [[{token: lp}]]}``), which
         the reference takes from its sampler's ``prompt_logprobs`` (arctic_platform/common/http_server.py:949)."""
         from ..models.decoder import token_logprobs
+        from ..ops.logprob import best_tokens
         from ..rl.zorro_train.layout import build_packed_batch
         model = self._target_model()
         if self.sampler is not None and getattr(self.sampler, "_asleep", False):
@@ -600,8 +601,7 @@ class EngineWorker:
         top_lp = torch.empty((N, k), dtype=torch.float32, device=h.device)
         top_id = torch.empty((N, k), dtype=torch.int64, device=h.device)
         for r0 in range(0, N, 2048):
-            z = torch.log_softmax((h[r0:r0 + 2048].float() @ W.float().t()), -1)
-            top_lp[r0:r0 + 2048], top_id[r0:r0 + 2048] = torch.topk(z, k, dim=-1)
+            top_lp[r0:r0 + 2048], top_id[r0:r0 + 2048] = best_tokens(h[r0:r0 + 2048].float() @ W.float().t(), k)
         model.train(was_training)
         R_ = pk.response_length
         lp_grid = torch.zeros((len(prompts) * R_, k), dtype=torch.float32)

@@ -358,14 +358,31 @@ def token_logprobs(model: DecoderLM, packed, inv_temperature=1.0, with_entropy: 
     restricts the distribution of the constrained rows to their legal tokens."""
     from ..ops.logprob import lm_head_logprobs
 
-    if routed_experts is not None:          # [B, S, L_moe, k] aligned with the input grid -> packed token order
-        routed_experts = packed.gather_inputs(routed_experts)
-    hidden = model.forward_hidden(packed.input_ids, packed.positions, packed.layout, routed_experts)
-    pred = rows.gather_rows(hidden, packed.pred_index)
+    pred = prediction_rows(model, packed, routed_experts)
     if action_masks is not None:
         from ..utils.action_masks import masked_logprobs
         return masked_logprobs(pred, model.output_weight, packed.labels, action_masks, inv_temperature, with_entropy)
     return lm_head_logprobs(pred, model.output_weight, packed.labels, inv_temperature, with_entropy)
+
+
+def prediction_rows(model: DecoderLM, packed, routed_experts=None) -> torch.Tensor:
+    """Final hidden states ``[N, H]`` of the rows that predict ``packed.labels``."""
+    if routed_experts is not None:          # [B, S, L_moe, k] aligned with the input grid -> packed token order
+        routed_experts = packed.gather_inputs(routed_experts)
+    hidden = model.forward_hidden(packed.input_ids, packed.positions, packed.layout, routed_experts)
+    return rows.gather_rows(hidden, packed.pred_index)
+
+
+@torch.no_grad()
+def top_token_logprobs(model: DecoderLM, pred: torch.Tensor, k: int, inv_temperature: float = 1.0, chunk: int = 2048):
+    """The ``k`` most likely tokens at prediction rows ``pred [N, H]``: log-probabilities ``[N, k]``, ids ``[N, k]`` int32 and the log of
+    the others' mass ``[N]``.  Logits are formed ``chunk`` rows at a time."""
+    from ..ops.logprob import top_logprobs
+    parts = [top_logprobs(model.logits(pred[s:s + chunk]), k, inv_temperature) for s in range(0, pred.shape[0], chunk)]
+    if not parts:
+        z = pred.new_zeros((0, k), dtype=torch.float32)
+        return z, z.to(torch.int32), z.new_zeros(0)
+    return tuple(torch.cat(x) for x in zip(*parts))
 
 
 # ----------------------------------------------------------------------------- selective checkpointing, per block

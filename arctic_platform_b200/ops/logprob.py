@@ -237,3 +237,12 @@ def top_logprobs(logits: torch.Tensor, k: int, inv_temperature=1.0) -> Tuple[tor
                          1.0 if per_row is not None else float(inv_temperature), N, V, k, lp.data_ptr(), ids.data_ptr(), rest.data_ptr(),
                          _lib.stream_ptr()), "apb_top_logprobs")
     return lp, ids, rest
+
+
+def best_tokens(logits: torch.Tensor, k: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Log-probabilities and indices ``[N, k]`` of the most likely tokens of fp32 ``logits [N, V]``, for any ``k`` up to V
+    (:func:`top_logprobs` where it has a kernel for it)."""
+    if logits.is_cuda and 1 <= k <= min(MOST_TOP, logits.shape[-1]):
+        lp, ids, _ = top_logprobs(logits, k)
+        return lp, ids
+    return torch.topk(torch.log_softmax(logits, -1), k, dim=-1)

@@ -29,19 +29,21 @@ def _fn():
     if _FN is None:
         c = ctypes
         vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
-        _FN = _lib.declare("apb_draw", [vp, i, ll, vp, f, vp, i, vp, f, vp, f, vp, i, c.c_uint, vp, i, i, vp, vp, vp])
+        _FN = _lib.declare("apb_draw", [vp, i, ll, vp, f, vp, i, vp, f, vp, f, vp, i, c.c_uint, vp, vp, i, i, vp, vp, vp])
     return _FN
 
 
 def draw_raw(logits: torch.Tensor, uniforms: Optional[torch.Tensor], temperature, top_k, top_p, min_p, tokens: torch.Tensor,
-             logprobs: torch.Tensor, seed: int = 0, step: Optional[torch.Tensor] = None) -> None:
+             logprobs: torch.Tensor, seed: Union[int, torch.Tensor] = 0, step: Optional[torch.Tensor] = None) -> None:
     """The launch behind :func:`sample` on checked arguments of the current device: each setting a number or a contiguous tensor ``[B]``
-    (fp32, ``top_k`` int32).  Without ``uniforms`` the numbers are a hash of ``seed``, ``step`` (one int32 on the device, read by the kernel, so
-    that a captured graph sees new values) and the row."""
+    (fp32, ``top_k`` int32).  Without ``uniforms`` the token is the largest of ``l / T`` and Gumbel noise by a hash of
+    ``seed``, ``step``, the row and the token, the noise of the rollout engine's other draws; seed and step on the device (one int32 each)
+    are read by the kernel, so that a captured graph sees new values."""
     both = lambda x, off: (None, x) if not torch.is_tensor(x) else (x.data_ptr(), off)          # noqa: E731
     _lib.check(_fn()(logits.data_ptr(), _TYPES[logits.dtype], logits.stride(0), *both(temperature, 1.0), *both(top_k, 0), *both(top_p, 1.0),
                      *both(min_p, 0.0), None if uniforms is None else uniforms.data_ptr(),
-                     uniforms is not None and uniforms.dtype is torch.float64, ctypes.c_uint(seed & 0xFFFFFFFF),
+                     uniforms is not None and uniforms.dtype is torch.float64,
+                     ctypes.c_uint(0 if torch.is_tensor(seed) else seed & 0xFFFFFFFF), seed.data_ptr() if torch.is_tensor(seed) else None,
                      None if step is None else step.data_ptr(), logits.shape[0], logits.shape[1], tokens.data_ptr(), logprobs.data_ptr(),
                      _lib.stream_ptr()), "apb_draw")
 

@@ -11,6 +11,7 @@ server can form global token means (see ``common/utils/metrics.py``).
   (arctic_platform/integrations/verl/grpo_loss.py:415-522).
 * ``grpo``      -- decoupled-PPO variant with a proximal policy, behaviour-importance cap and the same
   aggregation modes (arctic_platform/rl/processors/grpo.py:195-394).
+* ``distill``   -- divergence from a teacher's most likely tokens (``ops/distill.py``), the same aggregation modes.
 * ``sft`` / ``sft_ce`` -- next-token cross entropy with global-token normalisation
   (arctic_platform/sft/processor.py:95-292).
 """
@@ -251,6 +252,45 @@ def grpo_loss(model_outputs: dict, batch: dict, meta: dict, config: dict, device
                "actor/behav_imp_weight.sum": vals[5], "actor/behav_imp_weight.tokens": n,
                "actor/pg_clipfrac_lower.sum": vals[6], "actor/pg_clipfrac_lower.tokens": n,
                "actor/entropy.sum": vals[7], "actor/entropy.tokens": n}
+    return loss, metrics
+
+
+@register_loss_fn("distill")
+def distill_loss(model_outputs: dict, batch: dict, meta: dict, config: dict, device) -> Tuple[torch.Tensor, dict]:
+    """Divergence of the student from a teacher at the loss positions, aggregated by [``loss_agg_mode``] (token-mean unless given).
+
+    The batch carries the teacher's most likely tokens ``teacher_top_ids [B, R, K]`` (-1: none) with their log-probabilities
+    ``teacher_top_logprobs`` and, optionally, the log of the mass of all others, ``teacher_rest [B, R]``: what a forward pass with
+    ``meta['top_logprobs']`` answers as ``top_ids``, ``top_log_probs`` and ``top_rest``.  [``reverse``]: 0 is KL(teacher, student), 1
+    KL(student, teacher), numbers between weigh both.  [``ce_coeff``] adds the cross entropy of the batch's own tokens, [``entropy_coeff``]
+    takes the entropy off as in the policy losses."""
+    cfg = {**(meta.get("actor_config") or {}), **(config or {})}
+    if "divergence" not in model_outputs:
+        raise NotImplementedError("distill needs a pass that compares with the batch's teacher (loss_fn 'distill' by its own name)")
+    packed, _take, mask, seq_ids = _token_views(model_outputs, batch, device)
+    info = _global_info(meta, model_outputs)
+    info.update(seq_ids=seq_ids, num_seqs=packed.batch_size)
+    agg_mode = cfg.get("loss_agg_mode", "token-mean")
+    value = torch.where(mask, model_outputs["divergence"], 0.0)          # positions without loss may have a teacher of zeros
+    loss = agg_loss(value, mask, agg_mode, **info)
+    mf = mask.float()
+    sums = [mf.sum(), value.sum().detach()]
+    ce_coeff, entropy_coeff = float(cfg.get("ce_coeff", 0.0) or 0.0), float(cfg.get("entropy_coeff", 0.0) or 0.0)
+    lp, entropy = model_outputs["logprobs"], model_outputs.get("entropy")
+    if ce_coeff:
+        loss = loss - ce_coeff * agg_loss(torch.where(mask, lp, 0.0), mask, agg_mode, **info)
+    sums.append(-(torch.where(mask, lp, 0.0)).sum().detach())
+    if entropy is not None:
+        if entropy_coeff:
+            loss = loss - entropy_coeff * agg_loss(torch.where(mask, entropy, 0.0), mask, agg_mode, **info)
+        sums.append(torch.where(mask, entropy, 0.0).sum().detach())
+    vals = to_host(torch.stack(sums)).tolist()
+    ntok = vals[0]
+    metrics = {"distill/divergence.sum": vals[1], "distill/divergence.tokens": ntok, "distill/cross_entropy.sum": vals[2],
+               "distill/cross_entropy.tokens": ntok,
+               "loss.sum": vals[1] + ce_coeff * vals[2] - (entropy_coeff * vals[3] if entropy is not None else 0.0), "loss.tokens": ntok}
+    if entropy is not None:
+        metrics["actor/entropy_loss.sum"], metrics["actor/entropy_loss.tokens"] = vals[3], ntok
     return loss, metrics
 
 

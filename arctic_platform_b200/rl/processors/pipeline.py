@@ -19,7 +19,7 @@ import torch
 from ...utils import sft_profile
 from ...utils.transfer_stats import to_device, to_host
 from ...common.registry import LOSS_FNS, POST_PROCESSORS, register_post_processor, resolve_fn
-from ...models.decoder import token_logprobs
+from ...models.decoder import prediction_rows, token_logprobs, top_token_logprobs
 from ..zorro_train.layout import PackedBatch, build_packed_batch, build_plain_packed
 from . import losses as _losses  # noqa: F401  (registers the built-in losses)
 from .padding import *  # noqa: F401,F403  (padded grid <-> packed row helpers, importable from here as well)
@@ -50,6 +50,38 @@ def _entropy(model_outputs, batch, meta, config, device):
 def _temperature(model_outputs, batch, meta, config, device):
     """Temperature is folded into the lm-head epilogue (``meta['temperature']``)."""
     return model_outputs
+
+
+@register_post_processor("compute_top_logprobs")
+def _top_logprobs(model_outputs, batch, meta, config, device):
+    """The pass's most likely tokens (``meta['top_logprobs']`` of them, 64 unless it says otherwise) are formed beside its log-probs."""
+    return model_outputs
+
+
+def _top_wanted(meta: dict, processing: dict) -> int:
+    """Most likely tokens per position that the call asks for (0: none)."""
+    k = meta.get("top_logprobs")
+    if k is None and "compute_top_logprobs" in (processing.get("post") or []):
+        k = 64
+    k = int(k or 0)
+    if k < 0:
+        raise ValueError(f"meta['top_logprobs'] = {k}")
+    return k
+
+
+def teacher_of(batch: Dict[str, Any], packed, device):
+    """The teacher's numbers at the predictions of ``packed``: ``teacher_top_ids`` and ``teacher_top_logprobs`` ``[B, R, K]`` and, where the
+    batch has it, ``teacher_rest`` ``[B, R]`` of the response grid."""
+    missing = [k for k in ("teacher_top_ids", "teacher_top_logprobs") if batch.get(k) is None]
+    if missing:
+        raise KeyError(f"distill needs batch[{missing[0]!r}]")
+    ids, lq, rest = (batch.get(k) for k in ("teacher_top_ids", "teacher_top_logprobs", "teacher_rest"))
+    grid = (packed.batch_size, packed.response_length)
+    if ids.dim() != 3 or tuple(ids.shape[:2]) != grid or lq.shape != ids.shape or (rest is not None and tuple(rest.shape) != grid):
+        raise ValueError(f"teacher_top_ids {list(ids.shape)}, teacher_top_logprobs {list(lq.shape)} and teacher_rest "
+                         f"{None if rest is None else list(rest.shape)} must be [{grid[0]}, {grid[1]}, K] twice and [{grid[0]}, {grid[1]}]")
+    take = lambda t: packed.gather_from_grid(to_device(t, device))                          # noqa: E731
+    return take(ids), take(lq).float(), None if rest is None else take(rest).float()
 
 
 def response_length_of(batch: dict, meta: dict) -> int:
@@ -125,6 +157,11 @@ def run_pipeline(engine, batch: Dict[str, torch.Tensor], meta: Optional[dict] = 
     actor = meta.get("actor_config", {}) or {}
     want_entropy = bool(actor.get("entropy_coeff", 0.0)) or bool(meta.get("compute_entropy", not backward))
     temperature = float(meta.get("temperature", 1.0) or 1.0)
+    n_top, distill, kw = _top_wanted(meta, processing), loss_name == "distill", processing.get("loss_kwargs") or {}
+    want_entropy = want_entropy or (distill and bool(kw.get("entropy_coeff")))
+    if (n_top or distill) and (getattr(model, "sp_group", None) is not None or batch.get("action_mask_tokens") is not None):
+        raise NotImplementedError("most likely tokens and distillation are not available together with sequence parallelism or action masks")
+    top = divergence = None
     model.train(backward)
     ctx = torch.enable_grad() if backward else torch.no_grad()
     with ctx:
@@ -134,9 +171,21 @@ def run_pipeline(engine, batch: Dict[str, torch.Tensor], meta: Optional[dict] = 
             if sp_group is None:
                 # rollout routing replay: the experts the sampler chose, per input token and MoE layer
                 routed = batch.get("routed_experts") if packed.src_index is not None else None
-                lp, ent = token_logprobs(model, packed, 1.0 / temperature, with_entropy=want_entropy,
-                                         action_masks=action_masks_of(batch, packed),
-                                         routed_experts=None if routed is None else to_device(routed, device))
+                if n_top or distill:
+                    pred = prediction_rows(model, packed, None if routed is None else to_device(routed, device))
+                    if n_top:
+                        top = top_token_logprobs(model, pred, n_top, 1.0 / temperature)
+                if distill:
+                    from ...ops.distill import lm_head_distill
+                    divergence, lp, ent = lm_head_distill(pred, model.output_weight, packed.labels, *teacher_of(batch, packed, device),
+                                                          1.0 / temperature, float(kw.get("reverse", 0.0)), want_entropy)
+                elif n_top:
+                    from ...ops.logprob import lm_head_logprobs
+                    lp, ent = lm_head_logprobs(pred, model.output_weight, packed.labels, 1.0 / temperature, want_entropy)
+                else:
+                    lp, ent = token_logprobs(model, packed, 1.0 / temperature, with_entropy=want_entropy,
+                                             action_masks=action_masks_of(batch, packed),
+                                             routed_experts=None if routed is None else to_device(routed, device))
             else:
                 lp, ent, owned = _sp_logprobs(model, packed, sp_group, 1.0 / temperature, want_entropy, batch)
                 # every rank of the sequence-parallel group holds the same batch and scores its own rows; the loss
@@ -144,6 +193,8 @@ def run_pipeline(engine, batch: Dict[str, torch.Tensor], meta: Optional[dict] = 
                 import torch.distributed as dist
                 meta["dp_size"] = int(meta.get("dp_size", 1) or 1) * dist.get_world_size(sp_group)
         outputs: Dict[str, Any] = {"logprobs": lp, "entropy": ent, "packed": packed}
+        if divergence is not None:
+            outputs["divergence"] = divergence
         if owned is not None:
             outputs["owned"] = owned
         for name in processing.get("post") or []:
@@ -153,7 +204,7 @@ def run_pipeline(engine, batch: Dict[str, torch.Tensor], meta: Optional[dict] = 
         if loss_name:
             loss_fn = resolve_fn(loss_name, LOSS_FNS)
             with sft_profile.timed("loss"):
-                loss, metrics = loss_fn(outputs, batch, meta, processing.get("loss_kwargs") or {}, device)
+                loss, metrics = loss_fn(outputs, batch, meta, kw, device)
         if backward:
             if loss is None:
                 raise ValueError("backward needs a loss_fn")
@@ -175,5 +226,10 @@ def run_pipeline(engine, batch: Dict[str, torch.Tensor], meta: Optional[dict] = 
         out_batch = {"log_probs": to_host(packed.scatter_to_grid(lp_out))}
         if ent_out is not None:
             out_batch["entropy"] = to_host(packed.scatter_to_grid(ent_out))
+        if top is not None:                       # what a distilling pass takes as teacher_top_logprobs, teacher_top_ids, teacher_rest
+            for name, t, fill in (("top_log_probs", top[0], 0.0), ("top_ids", top[1], -1), ("top_rest", top[2], 0.0)):
+                out_batch[name] = to_host(packed.scatter_to_grid(t, fill))
+        if divergence is not None:
+            out_batch["divergence"] = to_host(packed.scatter_to_grid(divergence.detach()))
         result["batch"] = out_batch
     return result

@@ -73,14 +73,14 @@ class PackedBatch:
         return self
 
     def scatter_to_grid(self, values: torch.Tensor, fill: float = 0.0) -> torch.Tensor:
-        """Per-token values ``[N]`` -> padded ``[B, R]`` response grid."""
-        grid = values.new_full((self.batch_size * self.response_length,), fill)
+        """Per-token values ``[N, ...]`` -> padded ``[B, R, ...]`` response grid."""
+        grid = values.new_full((self.batch_size * self.response_length,) + tuple(values.shape[1:]), fill)
         grid[self.out_index.to(values.device)] = values
-        return grid.view(self.batch_size, self.response_length)
+        return grid.view((self.batch_size, self.response_length) + tuple(values.shape[1:]))
 
     def gather_from_grid(self, grid: torch.Tensor) -> torch.Tensor:
-        """Padded ``[B, R]`` grid -> per-token ``[N]`` in the order of ``labels``."""
-        return grid.reshape(-1)[self.out_index.to(grid.device)]
+        """Padded ``[B, R, ...]`` grid -> per-token ``[N, ...]`` in the order of ``labels``."""
+        return grid.reshape((-1,) + tuple(grid.shape[2:]))[self.out_index.to(grid.device)]
 
     @property
     def redundancy(self) -> float:

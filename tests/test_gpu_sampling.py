@@ -172,6 +172,31 @@ def test_drawn_numbers_of_the_device():
     assert float((a == c).float().mean()) < 0.05
 
 
+@pytest.mark.parametrize("B,V", [(1, 151936), (5, 4001), (130, 32000)])
+def test_noise_is_that_of_the_engines_other_draws(B, V):
+    """Without restrictions the tokens of the rollout engine's kernel; with them, where that token stays, the same one."""
+    import ctypes
+    from arctic_platform_b200.engine.sampler import _fn
+    from arctic_platform_b200.ops import _lib
+    z, _ = make(B, V, seed=11)
+    T = torch.full((B,), 0.8, device="cuda")
+    step = torch.full((1,), 7, device="cuda", dtype=torch.int32)
+    seed = torch.full((1,), 99, device="cuda", dtype=torch.int32)
+    new = lambda: (torch.empty(B, device="cuda", dtype=torch.int32), torch.empty(B, device="cuda"))      # noqa: E731
+    want, got, held = new(), new(), new()
+    _lib.check(_fn("sample")(_lib.ptr(z), z.stride(0), _lib.ptr(T), B, V, ctypes.c_uint(99), _lib.ptr(step), _lib.ptr(want[0]), _lib.ptr(want[1]),
+                             _lib.stream_ptr()), "sample")
+    sampling.draw_raw(z, None, T, 0, 1.0, 0.0, *got, seed=seed, step=step)
+    torch.testing.assert_close(got[0], want[0], rtol=0, atol=0)
+    torch.testing.assert_close(got[1], want[1], rtol=RTOL, atol=2 * ATOL)
+    sampling.draw_raw(z, None, T, 0, 1.0, 0.05, *held, seed=99, step=step)
+    x = z.double() / 0.8
+    stays = (x - x.amax(-1, keepdim=True)).gather(1, want[0].long()[:, None])[:, 0] >= torch.log(torch.tensor(0.05)).double()
+    assert bool((held[0] == want[0])[stays].all()) and bool((held[0] != want[0])[~stays].all())
+    kept = (x - x.amax(-1, keepdim=True)).gather(1, held[0].long()[:, None])[:, 0]
+    assert bool((kept >= torch.log(torch.tensor(0.05)).double()).all())
+
+
 def test_refusals():
     z, u = make(4, 50)
     for bad in ((z[0], u), (z.double(), u), (z, u[:3]), (z, u.half()), (z, u.cpu()), (z, u, torch.ones(3, device="cuda")),
