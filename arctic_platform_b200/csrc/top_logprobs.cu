@@ -2,12 +2,14 @@
 // the mass of all other tokens.
 //
 // Mathematics.  One pass.  A candidate is a logit's order and its index in one 64-bit number, larger for larger logits and, of equal ones, for
-// the lower index, so that the k largest numbers are the answer.  A buffer takes what is above a number that k candidates are known to reach
-// (first the k-th largest of the threads' largest ones, then the k-th of the buffer whenever it is sorted); what falls out of the
-// buffer, or never was above that number, can no longer be among the k and adds exp(l) to the sum of the others.  That sum is therefore
-// formed from them alone: one minus the named tokens' share would keep nothing of it where they hold all but a little.
+// the lower index, so that the k largest numbers are the answer.  A buffer takes what reaches a bound that k candidates are known to reach: at
+// first k of the threads' largest ones, later k of the buffer, whenever it has grown; what falls out of the buffer, or never reached the
+// bound, can no longer be among the k and adds exp(l) to the sum of the others.  That sum is therefore formed from them alone: one minus
+// the named tokens' share would keep nothing of it where they hold all but a little.  A bound is found bit by bit, by counting what
+// reaches it, and only until few more than k do (2000 cycles; sorting the buffer of 1024 instead took 17000, and 0.69 ms the pass over 2048
+// rows of 151936 where HBM wants 0.19).
 //
-// Layout.  One CTA walks a row, or each CTA of a cluster a part of it where rows are few, and the first one sorts what the others kept.
+// Layout.  One CTA walks a row, or each CTA of a cluster a part of it where rows are few, and the first one sorts what all have kept.
 #include "common.cuh"
 #include "host_utils.cuh"
 
@@ -38,6 +40,13 @@ __device__ __forceinline__ unsigned long long top_candidate(float z, int i) {
   return static_cast<unsigned long long>(top_key(z)) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
 }
 
+// 2^((z - ref) scale2), z <= ref: the difference first, as a product of a large logit would lose the digits that tell it from its neighbours.
+__device__ __forceinline__ float top_mass(float z, float ref, float scale2) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((z - ref) * scale2));
+  return z == ref ? 1.f : y;
+}
+
 // The first `size` (a power of 2 from 64 on) entries of the buffer in falling order (all threads).  Pairs at most 32 apart lie in 64 entries
 // that one warp walks: between those steps the warp alone waits.
 __device__ void top_sort(unsigned long long* buf, int size) {
@@ -60,18 +69,24 @@ __device__ void top_sort(unsigned long long* buf, int size) {
   __syncthreads();
 }
 
-// 2^((z - ref) scale2), z <= ref: the difference first, as a product of a large logit would lose the digits that tell it from its neighbours.
-__device__ __forceinline__ float top_mass(float z, float ref, float scale2) { return z == ref ? 1.f : exp2f((z - ref) * scale2); }
-
-// Sum of the others' masses against a reference that moves up: the value of `least`, which none of them is above.
-struct TopSum {
-  float scale2, ref = -INFINITY, s = 0.f;
-  __device__ __forceinline__ void add(float z) { s += top_mass(z, ref, scale2); }
-  __device__ __forceinline__ void move(float to) {           // to >= ref
-    s = s == 0.f ? 0.f : s * top_mass(ref, to, scale2);
-    ref = to;
+// A number that at least `want` of the CTA's candidates reach (E of a thread, 0: none), the largest one with so many unless no more than
+// `enough` reach a smaller one already.
+template <int E>
+__device__ unsigned long long top_bound(const unsigned long long (&c)[E], int want, int enough) {
+  unsigned long long x = 0;
+#pragma unroll 1
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long t = x | 1ull << bit;
+    int reach = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) reach += __syncthreads_count(c[e] >= t);
+    if (reach >= want) {
+      x = t;
+      if (reach <= enough) break;
+    }
   }
-};
+  return x;
+}
 
 template <typename T, int ROOM>
 __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
@@ -80,7 +95,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   __shared__ float warp_s[kTopThreads / 32], part_ref, part_s, shared_log;
   __shared__ int held, part_held;
   constexpr int kVec = 16 / sizeof(T);
-  constexpr int kAtOnce = 8;              // elements of a thread between two looks at the buffer
+  constexpr int kAtOnce = 16;             // elements of a thread between two looks at the buffer
   constexpr int kWords = kAtOnce / kVec;
   constexpr int kWarps = kTopThreads / 32;
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
@@ -88,48 +103,68 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   const int begin = min(part * a.per, a.V), n = min(a.V - begin, a.per), k = a.k;
   const T* src = static_cast<const T*>(a.logits) + row * a.ld + begin;
   const float scale2 = a.scale * (a.row_scale ? a.row_scale[row] : 1.f) * kTopLog2e;
-  TopSum sum{scale2};
-  unsigned long long least = 0;           // candidates above this may be among the k: at least k are, or the buffer has taken all
-  float least_z = -INFINITY;
-  int least_i = 0x7fffffff;
-  const int crowd = max(ROOM / 2, 2 * k); // held entries from which on sorting pays: a higher `least`
+  constexpr int kOwn = ROOM / kTopThreads;              // candidates of the buffer that a thread looks at
+  float sum = 0.f, ref = -INFINITY;                     // of the others' masses against `ref`, which none of them is above
+  float bound_z = -INFINITY;                            // candidates reach the bound with more than this, or with as much and no higher index
+  int bound_i = 0x7fffffff;
+  unsigned long long bound = 0;
+  const int crowd = max(ROOM / 2, k + ROOM / 4);        // held entries from which on a new bound pays
+  const int loose = k + k / 4;                          // candidates that a bound may leave before the last
   if (tid == 0) held = 0;
   __syncthreads();
 
-  auto set_least = [&](unsigned long long c) {
-    least = c;
-    least_z = c ? top_value(c) : -INFINITY;
-    least_i = c ? static_cast<int>(0xffffffffu - static_cast<uint32_t>(c)) : 0x7fffffff;
-    sum.move(least_z);
+  auto set_bound = [&](unsigned long long x) {
+    const uint32_t key = static_cast<uint32_t>(x >> 32), low = static_cast<uint32_t>(x);
+    if (x <= bound || key < 0x007fffffu) return;        // below -inf: all reach it
+    bound = x;
+    bound_z = key == 0x7fffffffu ? 0.f : top_unkey(key);            // the place of -0, which no candidate has
+    bound_i = key == 0x7fffffffu || low < 0x80000000u ? 0x7fffffff : static_cast<int>(0xffffffffu - low);
+    sum = sum == 0.f ? 0.f : sum * top_mass(ref, bound_z, scale2);
+    ref = bound_z;
   };
-  // candidate(z, at) > least without forming it (-inf included: nothing is below it, and indices are below least_i before it is set)
-  auto above = [&](float z, int at) { return z > least_z || (z == least_z && at < least_i); };
-  auto sort_size = [](int have) { return have <= 64 ? 64 : 1 << (32 - __clz(have - 1)); };
-  // sorts, keeps the k largest and counts the others into the sum
-  auto squeeze = [&](int have) {
-    const int size = sort_size(have);
-    for (int i = have + tid; i < size; i += kTopThreads) buf[i] = 0;
-    top_sort(buf, size);
-    if (have >= k) set_least(buf[k - 1]);
-    for (int i = k + tid; i < have; i += kTopThreads)
-      if (top_value(buf[i]) > -INFINITY) sum.add(top_value(buf[i]));
-    __syncthreads();
-    if (tid == 0) held = min(have, k);
+  auto reaches = [&](float z, int at) { return z > bound_z || (z == bound_z && at <= bound_i); };
+  // a new bound, which at least k of the `have` entries of the buffer reach, as `enough` says; what does not goes into the sum
+  auto squeeze = [&](int have, int enough) {
+    unsigned long long c[kOwn];
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) c[e] = tid + e * kTopThreads < have ? buf[tid + e * kTopThreads] : 0;
+    if (have > k) {
+      const unsigned long long x = top_bound(c, k, enough);
+      if (tid == 0) held = 0;
+      __syncthreads();
+      set_bound(x);
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) {
+        if (c[e] >= x && c[e] != 0) buf[atomicAdd(&held, 1)] = c[e];
+        else if (c[e] != 0 && top_value(c[e]) > -INFINITY) sum += top_mass(top_value(c[e]), ref, scale2);
+      }
+    } else if (tid == 0) {
+      held = have;
+    }
     __syncthreads();
   };
-  // the elements of one step: what is not above `least` into the sum, the others into the buffer
+  // the elements of one step: what does not reach the bound into the sum, the others into the buffer
   auto take = [&](const float (&z)[kAtOnce], int at0, uint32_t there) {
-    uint32_t waiting = 0;
     auto at = [&](int j) { return at0 + (j / kVec) * kTopThreads * kVec + j % kVec; };
-    auto sieve = [&](uint32_t in) {
+    bool maybe = false;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) maybe |= z[j] >= bound_z;
+    uint32_t waiting = 0;
+    if (maybe) {
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (((there >> j) & 1u) && reaches(z[j], at(j))) waiting |= 1u << j;
+    }
+    auto add = [&](uint32_t in) {
+      float s[2] = {0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j) {
-        const bool on = (in >> j) & 1u, up = on && above(z[j], at(j));
-        if (up) waiting |= 1u << j;
-        if (on && !up && z[j] > -INFINITY) sum.add(z[j]);
+        const float y = top_mass(z[j], ref, scale2);
+        s[j & 1] += ((in >> j) & 1u) && z[j] > -INFINITY ? y : 0.f;
       }
+      sum += s[0] + s[1];
     };
-    sieve(there);
+    add(there & ~waiting);
     for (;;) {
       uint32_t left = 0;
       bool full = false;
@@ -148,9 +183,12 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
       if (!__syncthreads_or(left != 0 || full)) break;
       const int have = min(held, ROOM);
       __syncthreads();
-      squeeze(have);
+      squeeze(have, loose);
       if (!__syncthreads_or(left != 0)) break;
-      sieve(left);
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (((left >> j) & 1u) && reaches(z[j], at(j))) waiting |= 1u << j;
+      add(left & ~waiting);
     }
   };
   auto number = [](T x) {
@@ -183,17 +221,14 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     fetch(next, w0 + kWords * kTopThreads);
     const int at0 = begin + head + (w0 + tid) * kVec;
     if (w0 == 0 && k <= kTopThreads && words > kTopThreads) {
-      // k threads' largest elements: so many candidates reach the k-th of them.  Every thread has at least its first word.
-      unsigned long long best = 0;
+      // k threads' largest elements: so many candidates reach the bound.  Every thread has at least its first word.
+      unsigned long long best[1] = {0};
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j) {
         const unsigned long long c = top_candidate(z[j], at0 + (j / kVec) * kTopThreads * kVec + j % kVec);
-        if (((there >> j) & 1u) && c > best) best = c;
+        if (((there >> j) & 1u) && c > best[0]) best[0] = c;
       }
-      buf[tid] = best;
-      top_sort(buf, kTopThreads);
-      set_least(buf[k - 1] - 1);
-      __syncthreads();
+      set_bound(top_bound(best, k, loose));
     }
     take(z, at0, there);
   }
@@ -206,15 +241,16 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     if (i < n) z[0] = number(src[i]);
     take(z, begin + i, i < n ? 1u : 0u);
   }
+  const int sorted = max(64, 1 << (32 - __clz(k - 1 | 1)));         // entries that are sorted in the end: a power of 2, at least k
   {
     const int have = min(held, ROOM);
     __syncthreads();
-    squeeze(have);
+    squeeze(have, a.parts > 1 ? ROOM / a.parts : sorted);
   }
 
-  // the sum over the CTA; the reference is the same in all threads
-  auto join = [&]() {
-    float s = warp_sum(sum.s);
+  // a sum over the CTA
+  auto join = [&](float s) {
+    s = warp_sum(s);
     if (lane == 0) warp_s[warp] = s;
     __syncthreads();
     s = 0.f;
@@ -222,16 +258,26 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     __syncthreads();
     return s;
   };
-  float others = join();
+  // in order; what is behind the k goes to the others, against the k-th, which no reference is above
+  auto finish = [&](int have) {
+    for (int i = have + tid; i < sorted; i += kTopThreads) buf[i] = 0;
+    top_sort(buf, sorted);
+    const float last = top_value(buf[k - 1]);
+    sum = sum == 0.f ? 0.f : sum * top_mass(ref, last, scale2);
+    ref = last;
+    for (int i = k + tid; i < sorted; i += kTopThreads)
+      if (buf[i] != 0 && top_value(buf[i]) > -INFINITY) sum += top_mass(top_value(buf[i]), ref, scale2);
+  };
+  int have = held;
   if (a.parts > 1) {
+    const float s = join(sum);
     if (tid == 0) {
-      part_ref = sum.ref;
-      part_s = others;
-      part_held = held;
+      part_ref = ref;
+      part_s = s;
+      part_held = have;
     }
     cluster_sync_all();
     if (part == 0) {
-      int have = held;
       for (int p = 1; p < a.parts; ++p) {
         int other;
         asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(other) : "r"(map_to_cta(smem_u32(&part_held), p)) : "memory");
@@ -240,28 +286,32 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
           asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(c) : "r"(map_to_cta(smem_u32(&buf[i]), p)) : "memory");
           buf[have + i] = c;
         }
-        have += other;                    // parts * k <= ROOM
+        have += other;                    // each has at most ROOM / parts
       }
-      sum.s = 0.f;
+      sum = 0.f;
       __syncthreads();
-      squeeze(have);                      // at least k are there: none of the parts' references is above the new one
-      others = join();
-      for (int p = 0; p < a.parts; ++p) {
-        const float ref = ld_cluster_f32(map_to_cta(smem_u32(&part_ref), p)), s = ld_cluster_f32(map_to_cta(smem_u32(&part_s), p));
-        if (s > 0.f) others += s * top_mass(ref, sum.ref, scale2);
-      }
+      squeeze(have, sorted);
+      finish(held);
+      if (tid == 0)
+        for (int p = 0; p < a.parts; ++p) {
+          const float r = ld_cluster_f32(map_to_cta(smem_u32(&part_ref), p)), t = ld_cluster_f32(map_to_cta(smem_u32(&part_s), p));
+          if (t > 0.f) sum += t * top_mass(r, ref, scale2);
+        }
     }
     cluster_sync_all();                   // nobody leaves while its buffer may be read
     if (part != 0) return;
+  } else {
+    finish(have);
   }
+  float others = join(sum);
 
   // denominator: the others and the k
   const float top = top_value(buf[0]);
   const float scale = a.scale * (a.row_scale ? a.row_scale[row] : 1.f);
   float log_others = -INFINITY;           // against `top`
   if (others > 1e-25f) {
-    log_others = (sum.ref == top ? 0.f : (sum.ref - top) * scale) + logf(others);
-  } else if (k < a.V && least_z > -INFINITY) {
+    log_others = (ref == top ? 0.f : (ref - top) * scale) + logf(others);
+  } else if (k < a.V && top_value(buf[k - 1]) > -INFINITY) {
     // all of them so far below the k-th (57 nats) that their masses against it are lost: the row again, against their largest
     const T* all = static_cast<const T*>(a.logits) + row * a.ld;
     const unsigned long long last = buf[k - 1];
@@ -275,18 +325,17 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     __syncthreads();
     for (int w = 0; w < kWarps; ++w) most = fmaxf(most, warp_s[w]);
     __syncthreads();
-    sum.s = 0.f;
+    sum = 0.f;
     for (int i = tid; i < a.V; i += kTopThreads) {
       const float z = number(all[i]);
-      if (z > -INFINITY && top_candidate(z, i) < last) sum.s += top_mass(z, most, scale2);
+      if (z > -INFINITY && top_candidate(z, i) < last) sum += top_mass(z, most, scale2);
     }
-    others = join();
+    others = join(sum);
     if (others > 0.f) log_others = (most - top) * scale + logf(others);
   }
   float named = 0.f;
   for (int i = tid; i < k; i += kTopThreads) named += top_mass(top_value(buf[i]), top, scale2);
-  sum.s = named;
-  named = join();
+  named = join(named);
   if (tid == 0) {
     others = expf(log_others);
     const float log_all = logf(named + others);
