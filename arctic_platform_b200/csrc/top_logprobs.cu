@@ -41,18 +41,51 @@ __device__ __forceinline__ unsigned long long top_candidate(float z, int i) {
 }
 
 // 2^((z - ref) scale2), z <= ref: the difference first, as a product of a large logit would lose the digits that tell it from its neighbours.
-__device__ __forceinline__ float top_mass(float z, float ref, float scale2) {
+__device__ __forceinline__ float top_power(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((z - ref) * scale2));
-  return z == ref ? 1.f : y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float top_mass(float z, float ref, float scale2) { return z == ref ? 1.f : top_power((z - ref) * scale2); }
+
+// 64 entries of a warp, a: those of lane, b: those 32 behind; steps of a bitonic network over runs of `run` that begin `stride` apart, for entries
+// whose place is base + lane and base + 32 + lane.
+__device__ __forceinline__ void top_steps(unsigned long long& a, unsigned long long& b, int base, int run, int stride) {
+  const int lane = threadIdx.x & 31;
+  if (stride == 32) {
+    if ((a < b) == (((base + lane) & run) == 0)) {
+      const unsigned long long t = a;
+      a = b;
+      b = t;
+    }
+    stride = 16;
+  }
+  for (; stride > 0; stride >>= 1) {
+    const unsigned long long c = __shfl_xor_sync(0xffffffffu, a, stride), d = __shfl_xor_sync(0xffffffffu, b, stride);
+    const bool first = (lane & stride) == 0;
+    const bool larger_a = first == (((base + lane) & run) == 0), larger_b = first == (((base + 32 + lane) & run) == 0);
+    a = (a < c) == larger_a ? c : a;
+    b = (b < d) == larger_b ? d : b;
+  }
+}
+__device__ __forceinline__ void top_sort_64(unsigned long long& a, unsigned long long& b, int base) {
+  for (int run = 2; run <= 64; run <<= 1) top_steps(a, b, base, run, run >> 1);
 }
 
-// The first `size` (a power of 2 from 64 on) entries of the buffer in falling order (all threads).  Pairs at most 32 apart lie in 64 entries
-// that one warp walks: between those steps the warp alone waits.
+// The first `size` (a power of 2 from 64 on) entries of the buffer in falling order (all threads).  Entries at most 32 apart meet in a warp's
+// registers, those further apart in shared memory.
 __device__ void top_sort(unsigned long long* buf, int size) {
+  const int lane = threadIdx.x & 31;
   __syncthreads();
-  for (int run = 2; run <= size; run <<= 1)
-    for (int stride = run >> 1; stride > 0; stride >>= 1) {
+  for (int base = (threadIdx.x >> 5) * 64; base < size; base += 2 * kTopThreads) {
+    unsigned long long a = buf[base + lane], b = buf[base + 32 + lane];
+    top_sort_64(a, b, base);
+    buf[base + lane] = a;
+    buf[base + 32 + lane] = b;
+  }
+  __syncthreads();
+  for (int run = 128; run <= size; run <<= 1) {
+    for (int stride = run >> 1; stride >= 64; stride >>= 1) {
       for (int t = threadIdx.x; t < size / 2; t += kTopThreads) {
         const int i = 2 * t - (t & (stride - 1)), j = i + stride;
         const unsigned long long a = buf[i], b = buf[j];
@@ -61,21 +94,64 @@ __device__ void top_sort(unsigned long long* buf, int size) {
           buf[j] = a;
         }
       }
-      // the next step's pairs: of half the distance, or the widest of the next run
-      const int next = stride > 1 ? stride >> 1 : run;
-      if (stride > 32 || next > 32) __syncthreads();
-      else __syncwarp();
+      __syncthreads();
     }
+    for (int base = (threadIdx.x >> 5) * 64; base < size; base += 2 * kTopThreads) {
+      unsigned long long a = buf[base + lane], b = buf[base + 32 + lane];
+      top_steps(a, b, base, run, 32);
+      buf[base + lane] = a;
+      buf[base + 32 + lane] = b;
+    }
+    __syncthreads();
+  }
+}
+
+// A number that at least `want` candidates reach, two of each thread (0: none), by their warps: each warp's share-th largest one, the least of
+// these.  0 where a warp has too few.  About twice `want` reach it if they lie in any order.
+__device__ unsigned long long top_rough_bound(unsigned long long a, unsigned long long b, int want, unsigned long long* ends) {
+  constexpr int kWarps = kTopThreads / 32;
+  const int share = (want + kWarps - 1) / kWarps - 1;       // index of it
+  if (share >= 64) return 0;
+  top_sort_64(a, b, 0);
+  const unsigned long long low = __shfl_sync(0xffffffffu, share < 32 ? a : b, share & 31);
+  if ((threadIdx.x & 31) == 0) ends[threadIdx.x >> 5] = low;
   __syncthreads();
+  unsigned long long x = ends[0];
+  for (int w = 1; w < kWarps; ++w) x = ends[w] < x ? ends[w] : x;
+  return x;
 }
 
 // A number that at least `want` of the CTA's candidates reach (E of a thread, 0: none), the largest one with so many unless no more than
 // `enough` reach a smaller one already.
 template <int E>
-__device__ unsigned long long top_bound(const unsigned long long (&c)[E], int want, int enough) {
-  unsigned long long x = 0;
+__device__ unsigned long long top_bound(const unsigned long long (&c)[E], int want, int enough, unsigned long long (&ends)[2][kTopThreads / 32]) {
+  // the bits that all have in common need no counting
+  unsigned long long lo = ~0ull, hi = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (c[e] != 0) {
+      lo = c[e] < lo ? c[e] : lo;
+      hi = c[e] > hi ? c[e] : hi;
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long a = __shfl_xor_sync(0xffffffffu, lo, o), b = __shfl_xor_sync(0xffffffffu, hi, o);
+    lo = a < lo ? a : lo;
+    hi = b > hi ? b : hi;
+  }
+  if ((threadIdx.x & 31) == 0) {
+    ends[0][threadIdx.x >> 5] = lo;
+    ends[1][threadIdx.x >> 5] = hi;
+  }
+  __syncthreads();
+  for (int w = 0; w < kTopThreads / 32; ++w) {
+    lo = ends[0][w] < lo ? ends[0][w] : lo;
+    hi = ends[1][w] > hi ? ends[1][w] : hi;
+  }
+  const int from = 63 - __clzll(static_cast<long long>(lo ^ hi));           // the highest bit in which they differ, -1: none
+  unsigned long long x = from < 0 ? lo : from == 63 ? 0ull : hi >> (from + 1) << (from + 1);
 #pragma unroll 1
-  for (int bit = 63; bit >= 0; --bit) {
+  for (int bit = from; bit >= 0; --bit) {
     const unsigned long long t = x | 1ull << bit;
     int reach = 0;
 #pragma unroll
@@ -94,6 +170,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   __shared__ unsigned long long buf[ROOM];
   __shared__ float warp_s[kTopThreads / 32], part_ref, part_s, shared_log;
   __shared__ int held, part_held;
+  __shared__ unsigned long long ends[2][kTopThreads / 32];
   constexpr int kVec = 16 / sizeof(T);
   constexpr int kAtOnce = 16;             // elements of a thread between two looks at the buffer
   constexpr int kWords = kAtOnce / kVec;
@@ -109,7 +186,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   int bound_i = 0x7fffffff;
   unsigned long long bound = 0;
   const int crowd = max(ROOM / 2, k + ROOM / 4);        // held entries from which on a new bound pays
-  const int loose = k + k / 4;                          // candidates that a bound may leave before the last
+  const int loose = k + k / 4 + 8;                      // candidates that a bound may leave before the last
   if (tid == 0) held = 0;
   __syncthreads();
 
@@ -124,12 +201,21 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   };
   auto reaches = [&](float z, int at) { return z > bound_z || (z == bound_z && at <= bound_i); };
   // a new bound, which at least k of the `have` entries of the buffer reach, as `enough` says; what does not goes into the sum
-  auto squeeze = [&](int have, int enough) {
+  auto squeeze = [&](int have, int enough, bool last) {
     unsigned long long c[kOwn];
 #pragma unroll
     for (int e = 0; e < kOwn; ++e) c[e] = tid + e * kTopThreads < have ? buf[tid + e * kTopThreads] : 0;
     if (have > k) {
-      const unsigned long long x = top_bound(c, k, enough);
+      // roughly first, if that leaves few enough
+      unsigned long long x = 0;
+      if (kOwn == 2 && !last) {
+        x = top_rough_bound(c[0], c[1], k, ends[0]);
+        int reach = 0;
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) reach += __syncthreads_count(c[e] != 0 && c[e] >= x);
+        if (reach > crowd - ROOM / 8) x = 0;
+      }
+      if (x == 0) x = top_bound(c, k, enough, ends);
       if (tid == 0) held = 0;
       __syncthreads();
       set_bound(x);
@@ -143,28 +229,28 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     }
     __syncthreads();
   };
-  // the elements of one step: what does not reach the bound into the sum, the others into the buffer
-  auto take = [&](const float (&z)[kAtOnce], int at0, uint32_t there) {
+  auto clean = [](float f) { return f == f ? f + 0.f : -INFINITY; };     // no number: the least likely; -0 is as large as 0
+  // the elements of one step, as they are: what does not reach the bound into the sum, the others into the buffer
+  auto take = [&](float (&z)[kAtOnce], int at0, uint32_t there) {
     auto at = [&](int j) { return at0 + (j / kVec) * kTopThreads * kVec + j % kVec; };
-    bool maybe = false;
+    float most = z[0];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) maybe |= z[j] >= bound_z;
+    for (int j = 1; j < kAtOnce; ++j) most = fmaxf(most, z[j]);
+    // what is below the bound goes into the sum; no number is below it, places without an element hold -inf
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const float y = top_power((z[j] - ref) * scale2);
+      s[j & 3] += z[j] < bound_z ? y : 0.f;
+    }
+    sum += (s[0] + s[1]) + (s[2] + s[3]);
     uint32_t waiting = 0;
-    if (maybe) {
+    if (most >= bound_z || bound_z == -INFINITY) {
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j)
-        if (((there >> j) & 1u) && reaches(z[j], at(j))) waiting |= 1u << j;
+        if (!(z[j] < bound_z)) waiting |= 1u << j;
+      waiting &= there;
     }
-    auto add = [&](uint32_t in) {
-      float s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const float y = top_mass(z[j], ref, scale2);
-        s[j & 1] += ((in >> j) & 1u) && z[j] > -INFINITY ? y : 0.f;
-      }
-      sum += s[0] + s[1];
-    };
-    add(there & ~waiting);
     for (;;) {
       uint32_t left = 0;
       bool full = false;
@@ -175,6 +261,11 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
 #pragma unroll
         for (int i = 1; i < kAtOnce; ++i)
           if (i == j) zj = z[i];
+        zj = clean(zj);
+        if (!reaches(zj, at(j))) {
+          if (zj > -INFINITY) sum += top_mass(zj, ref, scale2);
+          continue;
+        }
         const int slot = atomicAdd(&held, 1);
         if (slot < ROOM) buf[slot] = top_candidate(zj, at(j));
         else left |= 1u << j;
@@ -183,18 +274,12 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
       if (!__syncthreads_or(left != 0 || full)) break;
       const int have = min(held, ROOM);
       __syncthreads();
-      squeeze(have, loose);
+      squeeze(have, loose, false);
       if (!__syncthreads_or(left != 0)) break;
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j)
-        if (((left >> j) & 1u) && reaches(z[j], at(j))) waiting |= 1u << j;
-      add(left & ~waiting);
+      waiting = left;
     }
   };
-  auto number = [](T x) {
-    const float f = static_cast<float>(x);
-    return f == f ? f + 0.f : -INFINITY;  // what is not a number is the least likely; -0 is as large as 0
-  };
+  auto number = [&](T x) { return clean(static_cast<float>(x)); };
 
   const int ahead = static_cast<int>((-(reinterpret_cast<uintptr_t>(src)) & 15) / sizeof(T));
   const int head = min(ahead, n), words = (n - head) / kVec, tail = head + words * kVec;
@@ -215,20 +300,25 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     for (int q = 0; q < kWords; ++q) {
       const T* x = reinterpret_cast<const T*>(&next[q]);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) z[q * kVec + j] = number(x[j]);
-      if (w0 + q * kTopThreads + tid < words) there |= ((1u << kVec) - 1u) << (q * kVec);
+      for (int j = 0; j < kVec; ++j) z[q * kVec + j] = static_cast<float>(x[j]);
+      if (w0 + q * kTopThreads + tid < words) {
+        there |= ((1u << kVec) - 1u) << (q * kVec);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) z[q * kVec + j] = -INFINITY;
+      }
     }
     fetch(next, w0 + kWords * kTopThreads);
     const int at0 = begin + head + (w0 + tid) * kVec;
     if (w0 == 0 && k <= kTopThreads && words > kTopThreads) {
-      // k threads' largest elements: so many candidates reach the bound.  Every thread has at least its first word.
-      unsigned long long best[1] = {0};
+      // of the threads' largest elements k reach the bound.  Every thread has at least its first word.
+      unsigned long long best = 0;
 #pragma unroll
       for (int j = 0; j < kAtOnce; ++j) {
-        const unsigned long long c = top_candidate(z[j], at0 + (j / kVec) * kTopThreads * kVec + j % kVec);
-        if (((there >> j) & 1u) && c > best[0]) best[0] = c;
+        const unsigned long long c = top_candidate(clean(z[j]), at0 + (j / kVec) * kTopThreads * kVec + j % kVec);
+        if (((there >> j) & 1u) && c > best) best = c;
       }
-      set_bound(top_bound(best, k, loose));
+      set_bound(top_rough_bound(best, 0, k, ends[0]));
     }
     take(z, at0, there);
   }
@@ -236,16 +326,16 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     // in front of the first and behind the last whole word: at most 14 elements
     float z[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) z[j] = 0.f;
+    for (int j = 0; j < kAtOnce; ++j) z[j] = -INFINITY;
     const int i = tid < head ? tid : tail + tid - head;
-    if (i < n) z[0] = number(src[i]);
+    if (i < n) z[0] = static_cast<float>(src[i]);
     take(z, begin + i, i < n ? 1u : 0u);
   }
   const int sorted = max(64, 1 << (32 - __clz(k - 1 | 1)));         // entries that are sorted in the end: a power of 2, at least k
   {
     const int have = min(held, ROOM);
     __syncthreads();
-    squeeze(have, a.parts > 1 ? ROOM / a.parts : sorted);
+    squeeze(have, a.parts > 1 ? ROOM / a.parts : sorted, true);
   }
 
   // a sum over the CTA
@@ -290,12 +380,12 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
       }
       sum = 0.f;
       __syncthreads();
-      squeeze(have, sorted);
+      squeeze(have, sorted, true);
       finish(held);
       if (tid == 0)
         for (int p = 0; p < a.parts; ++p) {
           const float r = ld_cluster_f32(map_to_cta(smem_u32(&part_ref), p)), t = ld_cluster_f32(map_to_cta(smem_u32(&part_s), p));
-          if (t > 0.f) sum += t * top_mass(r, ref, scale2);
+          if (!(t <= 0.f)) sum += t * top_mass(r, ref, scale2);
         }
     }
     cluster_sync_all();                   // nobody leaves while its buffer may be read
@@ -312,7 +402,8 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   if (others > 1e-25f) {
     log_others = (ref == top ? 0.f : (ref - top) * scale) + logf(others);
   } else if (k < a.V && top_value(buf[k - 1]) > -INFINITY) {
-    // all of them so far below the k-th (57 nats) that their masses against it are lost: the row again, against their largest
+    // all of them so far below the k-th (57 nats) that their masses against it are lost, or among them what is no number: the row again, against
+    // their largest
     const T* all = static_cast<const T*>(a.logits) + row * a.ld;
     const unsigned long long last = buf[k - 1];
     float most = -INFINITY;
