@@ -15,7 +15,6 @@
 
 namespace apb {
 
-constexpr int kTopThreads = 512;
 constexpr int kTopMost = 1024;            // k
 constexpr float kTopLog2e = 1.44269504088896340736f;
 
@@ -74,10 +73,11 @@ __device__ __forceinline__ void top_sort_64(unsigned long long& a, unsigned long
 
 // The first `size` (a power of 2 from 64 on) entries of the buffer in falling order (all threads).  Entries at most 32 apart meet in a warp's
 // registers, those further apart in shared memory.
+template <int THREADS>
 __device__ void top_sort(unsigned long long* buf, int size) {
   const int lane = threadIdx.x & 31;
   __syncthreads();
-  for (int base = (threadIdx.x >> 5) * 64; base < size; base += 2 * kTopThreads) {
+  for (int base = (threadIdx.x >> 5) * 64; base < size; base += 2 * THREADS) {
     unsigned long long a = buf[base + lane], b = buf[base + 32 + lane];
     top_sort_64(a, b, base);
     buf[base + lane] = a;
@@ -86,7 +86,7 @@ __device__ void top_sort(unsigned long long* buf, int size) {
   __syncthreads();
   for (int run = 128; run <= size; run <<= 1) {
     for (int stride = run >> 1; stride >= 64; stride >>= 1) {
-      for (int t = threadIdx.x; t < size / 2; t += kTopThreads) {
+      for (int t = threadIdx.x; t < size / 2; t += THREADS) {
         const int i = 2 * t - (t & (stride - 1)), j = i + stride;
         const unsigned long long a = buf[i], b = buf[j];
         if ((a < b) == ((i & run) == 0)) {
@@ -96,7 +96,7 @@ __device__ void top_sort(unsigned long long* buf, int size) {
       }
       __syncthreads();
     }
-    for (int base = (threadIdx.x >> 5) * 64; base < size; base += 2 * kTopThreads) {
+    for (int base = (threadIdx.x >> 5) * 64; base < size; base += 2 * THREADS) {
       unsigned long long a = buf[base + lane], b = buf[base + 32 + lane];
       top_steps(a, b, base, run, 32);
       buf[base + lane] = a;
@@ -106,15 +106,35 @@ __device__ void top_sort(unsigned long long* buf, int size) {
   }
 }
 
-// A number that at least `want` candidates reach, two of each thread (0: none), by their warps: each warp's share-th largest one, the least of
-// these.  0 where a warp has too few.  About twice `want` reach it if they lie in any order.
-__device__ unsigned long long top_rough_bound(unsigned long long a, unsigned long long b, int want, unsigned long long* ends) {
-  constexpr int kWarps = kTopThreads / 32;
-  const int share = (want + kWarps - 1) / kWarps - 1;       // index of it
-  if (share >= 64) return 0;
-  top_sort_64(a, b, 0);
-  const unsigned long long low = __shfl_sync(0xffffffffu, share < 32 ? a : b, share & 31);
-  if ((threadIdx.x & 31) == 0) ends[threadIdx.x >> 5] = low;
+// A number that at least `want` candidates reach, of each thread one or two (TWO) by their orders' keys (0: none): each warp's share-th largest, the
+// least of these.  0 where a warp has too few.  About twice `want` reach it if they lie in any order.
+template <int THREADS, bool TWO>
+__device__ unsigned long long top_rough_bound(uint32_t a, uint32_t b, int want, unsigned long long* ends) {
+  constexpr int kWarps = THREADS / 32;
+  const int lane = threadIdx.x & 31, share = (want + kWarps - 1) / kWarps - 1;         // index of it
+  if (share >= (TWO ? 64 : 32)) return 0;
+#pragma unroll
+  for (int run = 2; run <= (TWO ? 64 : 32); run <<= 1) {
+    if (TWO && run == 64) {
+      const uint32_t t = max(a, b);
+      b = min(a, b);
+      a = t;
+    }
+#pragma unroll
+    for (int stride = run == 64 ? 16 : run >> 1; stride > 0; stride >>= 1) {
+      const uint32_t c = __shfl_xor_sync(0xffffffffu, a, stride);
+      const bool first = (lane & stride) == 0;
+      const bool falls = run == 32 || run == 64 || (lane & run) == 0;         // of 64 the first 32 fall, the others rise until they meet
+      a = first == falls ? max(a, c) : min(a, c);
+      if (TWO) {
+        const uint32_t d = __shfl_xor_sync(0xffffffffu, b, stride);
+        const bool falls_b = run == 64 || (run == 32 ? false : (lane & run) == 0);
+        b = first == falls_b ? max(b, d) : min(b, d);
+      }
+    }
+  }
+  const uint32_t low = __shfl_sync(0xffffffffu, share < 32 ? a : b, share & 31);
+  if (lane == 0) ends[threadIdx.x >> 5] = static_cast<unsigned long long>(low) << 32;
   __syncthreads();
   unsigned long long x = ends[0];
   for (int w = 1; w < kWarps; ++w) x = ends[w] < x ? ends[w] : x;
@@ -123,8 +143,8 @@ __device__ unsigned long long top_rough_bound(unsigned long long a, unsigned lon
 
 // A number that at least `want` of the CTA's candidates reach (E of a thread, 0: none), the largest one with so many unless no more than
 // `enough` reach a smaller one already.
-template <int E>
-__device__ unsigned long long top_bound(const unsigned long long (&c)[E], int want, int enough, unsigned long long (&ends)[2][kTopThreads / 32]) {
+template <int THREADS, int E>
+__device__ unsigned long long top_bound(const unsigned long long (&c)[E], int want, int enough, unsigned long long (&ends)[2][THREADS / 32]) {
   // the bits that all have in common need no counting
   unsigned long long lo = ~0ull, hi = 0;
 #pragma unroll
@@ -144,7 +164,7 @@ __device__ unsigned long long top_bound(const unsigned long long (&c)[E], int wa
     ends[1][threadIdx.x >> 5] = hi;
   }
   __syncthreads();
-  for (int w = 0; w < kTopThreads / 32; ++w) {
+  for (int w = 0; w < THREADS / 32; ++w) {
     lo = ends[0][w] < lo ? ends[0][w] : lo;
     hi = ends[1][w] > hi ? ends[1][w] : hi;
   }
@@ -164,23 +184,23 @@ __device__ unsigned long long top_bound(const unsigned long long (&c)[E], int wa
   return x;
 }
 
-template <typename T, int ROOM>
-__global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
+template <typename T, int ROOM, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_kernel(const TopArgs a) {
   pdl_entry();
   __shared__ unsigned long long buf[ROOM];
-  __shared__ float warp_s[kTopThreads / 32], part_ref, part_s, shared_log;
+  __shared__ float warp_s[THREADS / 32], part_ref, part_s, shared_log;
   __shared__ int held, part_held;
-  __shared__ unsigned long long ends[2][kTopThreads / 32];
+  __shared__ unsigned long long ends[2][THREADS / 32];
   constexpr int kVec = 16 / sizeof(T);
   constexpr int kAtOnce = 16;             // elements of a thread between two looks at the buffer
   constexpr int kWords = kAtOnce / kVec;
-  constexpr int kWarps = kTopThreads / 32;
+  constexpr int kWarps = THREADS / 32;
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int begin = min(part * a.per, a.V), n = min(a.V - begin, a.per), k = a.k;
   const T* src = static_cast<const T*>(a.logits) + row * a.ld + begin;
   const float scale2 = a.scale * (a.row_scale ? a.row_scale[row] : 1.f) * kTopLog2e;
-  constexpr int kOwn = ROOM / kTopThreads;              // candidates of the buffer that a thread looks at
+  constexpr int kOwn = ROOM / THREADS;              // candidates of the buffer that a thread looks at
   float sum = 0.f, ref = -INFINITY;                     // of the others' masses against `ref`, which none of them is above
   float bound_z = -INFINITY;                            // candidates reach the bound with more than this, or with as much and no higher index
   int bound_i = 0x7fffffff;
@@ -204,18 +224,18 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   auto squeeze = [&](int have, int enough, bool last) {
     unsigned long long c[kOwn];
 #pragma unroll
-    for (int e = 0; e < kOwn; ++e) c[e] = tid + e * kTopThreads < have ? buf[tid + e * kTopThreads] : 0;
+    for (int e = 0; e < kOwn; ++e) c[e] = tid + e * THREADS < have ? buf[tid + e * THREADS] : 0;
     if (have > k) {
       // roughly first, if that leaves few enough
       unsigned long long x = 0;
       if (kOwn == 2 && !last) {
-        x = top_rough_bound(c[0], c[1], k, ends[0]);
+        x = top_rough_bound<THREADS, true>(static_cast<uint32_t>(c[0] >> 32), static_cast<uint32_t>(c[1] >> 32), k, ends[0]);
         int reach = 0;
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) reach += __syncthreads_count(c[e] != 0 && c[e] >= x);
         if (reach > crowd - ROOM / 8) x = 0;
       }
-      if (x == 0) x = top_bound(c, k, enough, ends);
+      if (x == 0) x = top_bound<THREADS>(c, k, enough, ends);
       if (tid == 0) held = 0;
       __syncthreads();
       set_bound(x);
@@ -232,7 +252,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   auto clean = [](float f) { return f == f ? f + 0.f : -INFINITY; };     // no number: the least likely; -0 is as large as 0
   // the elements of one step, as they are: what does not reach the bound into the sum, the others into the buffer
   auto take = [&](float (&z)[kAtOnce], int at0, uint32_t there) {
-    auto at = [&](int j) { return at0 + (j / kVec) * kTopThreads * kVec + j % kVec; };
+    auto at = [&](int j) { return at0 + (j / kVec) * THREADS * kVec + j % kVec; };
     float most = z[0];
 #pragma unroll
     for (int j = 1; j < kAtOnce; ++j) most = fmaxf(most, z[j]);
@@ -287,13 +307,13 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   auto fetch = [&](uint4 (&raw)[kWords], int w0) {
 #pragma unroll
     for (int q = 0; q < kWords; ++q) {
-      const int w = w0 + q * kTopThreads + tid;
+      const int w = w0 + q * THREADS + tid;
       raw[q] = w < words ? __ldcs(s4 + w) : make_uint4(0, 0, 0, 0);
     }
   };
   uint4 next[kWords];
   fetch(next, 0);
-  for (int w0 = 0; w0 < words; w0 += kWords * kTopThreads) {
+  for (int w0 = 0; w0 < words; w0 += kWords * THREADS) {
     float z[kAtOnce];
     uint32_t there = 0;
 #pragma unroll
@@ -301,24 +321,22 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
       const T* x = reinterpret_cast<const T*>(&next[q]);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) z[q * kVec + j] = static_cast<float>(x[j]);
-      if (w0 + q * kTopThreads + tid < words) {
+      if (w0 + q * THREADS + tid < words) {
         there |= ((1u << kVec) - 1u) << (q * kVec);
       } else {
 #pragma unroll
         for (int j = 0; j < kVec; ++j) z[q * kVec + j] = -INFINITY;
       }
     }
-    fetch(next, w0 + kWords * kTopThreads);
+    fetch(next, w0 + kWords * THREADS);
     const int at0 = begin + head + (w0 + tid) * kVec;
-    if (w0 == 0 && k <= kTopThreads && words > kTopThreads) {
+    if (w0 == 0 && k <= THREADS && words > THREADS) {
       // of the threads' largest elements k reach the bound.  Every thread has at least its first word.
-      unsigned long long best = 0;
+      uint32_t best = 0;
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const unsigned long long c = top_candidate(clean(z[j]), at0 + (j / kVec) * kTopThreads * kVec + j % kVec);
-        if (((there >> j) & 1u) && c > best) best = c;
-      }
-      set_bound(top_rough_bound(best, 0, k, ends[0]));
+      for (int j = 0; j < kAtOnce; ++j)
+        if ((there >> j) & 1u) best = max(best, top_key(clean(z[j])));
+      set_bound(top_rough_bound<THREADS, false>(best, 0, k, ends[0]));
     }
     take(z, at0, there);
   }
@@ -350,12 +368,12 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
   };
   // in order; what is behind the k goes to the others, against the k-th, which no reference is above
   auto finish = [&](int have) {
-    for (int i = have + tid; i < sorted; i += kTopThreads) buf[i] = 0;
-    top_sort(buf, sorted);
+    for (int i = have + tid; i < sorted; i += THREADS) buf[i] = 0;
+    top_sort<THREADS>(buf, sorted);
     const float last = top_value(buf[k - 1]);
     sum = sum == 0.f ? 0.f : sum * top_mass(ref, last, scale2);
     ref = last;
-    for (int i = k + tid; i < sorted; i += kTopThreads)
+    for (int i = k + tid; i < sorted; i += THREADS)
       if (buf[i] != 0 && top_value(buf[i]) > -INFINITY) sum += top_mass(top_value(buf[i]), ref, scale2);
   };
   int have = held;
@@ -371,7 +389,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
       for (int p = 1; p < a.parts; ++p) {
         int other;
         asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(other) : "r"(map_to_cta(smem_u32(&part_held), p)) : "memory");
-        for (int i = tid; i < other; i += kTopThreads) {
+        for (int i = tid; i < other; i += THREADS) {
           unsigned long long c;
           asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(c) : "r"(map_to_cta(smem_u32(&buf[i]), p)) : "memory");
           buf[have + i] = c;
@@ -407,7 +425,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     const T* all = static_cast<const T*>(a.logits) + row * a.ld;
     const unsigned long long last = buf[k - 1];
     float most = -INFINITY;
-    for (int i = tid; i < a.V; i += kTopThreads) {
+    for (int i = tid; i < a.V; i += THREADS) {
       const float z = number(all[i]);
       if (top_candidate(z, i) < last) most = fmaxf(most, z);
     }
@@ -417,7 +435,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     for (int w = 0; w < kWarps; ++w) most = fmaxf(most, warp_s[w]);
     __syncthreads();
     sum = 0.f;
-    for (int i = tid; i < a.V; i += kTopThreads) {
+    for (int i = tid; i < a.V; i += THREADS) {
       const float z = number(all[i]);
       if (z > -INFINITY && top_candidate(z, i) < last) sum += top_mass(z, most, scale2);
     }
@@ -425,7 +443,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     if (others > 0.f) log_others = (most - top) * scale + logf(others);
   }
   float named = 0.f;
-  for (int i = tid; i < k; i += kTopThreads) named += top_mass(top_value(buf[i]), top, scale2);
+  for (int i = tid; i < k; i += THREADS) named += top_mass(top_value(buf[i]), top, scale2);
   named = join(named);
   if (tid == 0) {
     others = expf(log_others);
@@ -435,26 +453,30 @@ __global__ void __launch_bounds__(kTopThreads, 2) top_kernel(const TopArgs a) {
     a.rest[row] = top == -INFINITY ? -INFINITY : named < others ? log1pf(-named / (named + others)) : log_others - log_all;
   }
   __syncthreads();
-  for (int i = tid; i < k; i += kTopThreads) {
+  for (int i = tid; i < k; i += THREADS) {
     const float z = top_value(buf[i]);
     a.ids[static_cast<long long>(row) * k + i] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(buf[i]));
     a.logprobs[static_cast<long long>(row) * k + i] = top == -INFINITY ? -INFINITY : (z == top ? 0.f : (z - top) * scale) - shared_log;
   }
 }
 
-template <typename T, int ROOM>
-static int launch_top(TopArgs a, int N, cudaStream_t s) {
-  // parts of a row where the GPU has room for more CTAs than rows (two a SM), as long as their candidates fit the first one's buffer
+template <typename T, int ROOM, int THREADS>
+static int launch_top_as(TopArgs a, int N, cudaStream_t s) {
+  // parts of a row where the GPU has room for more CTAs than rows, as long as their candidates fit the first one's buffer
   int parts = 1;
-  while (parts < 8 && static_cast<long long>(N) * parts * 2 <= 2 * sm_count() && a.V / parts > 8192 && 2 * parts * a.k <= ROOM) parts *= 2;
+  while (parts < 8 && static_cast<long long>(N) * parts * 2 <= 1024 / THREADS * sm_count() && a.V / parts > 16 * THREADS && 2 * parts * a.k <= ROOM)
+    parts *= 2;
   a.parts = parts;
   a.per = ((a.V + parts - 1) / parts + 7) / 8 * 8;
-  return static_cast<int>(launch_kernel_clusters(top_kernel<T, ROOM>, dim3(static_cast<unsigned>(N) * parts), dim3(kTopThreads), 0, parts, s, a));
+  return static_cast<int>(launch_kernel_clusters(top_kernel<T, ROOM, THREADS>, dim3(static_cast<unsigned>(N) * parts), dim3(THREADS), 0, parts, s, a));
 }
 
 template <typename T>
-static int launch_top_of(const TopArgs& a, int N, cudaStream_t s) {
-  return a.k <= 256 ? launch_top<T, 1024>(a, N, s) : launch_top<T, 2048>(a, N, s);
+static int launch_top(const TopArgs& a, int N, cudaStream_t s) {
+  // 256 threads, four CTAs an SM, wait for one another less (2048 rows of 151936, k = 64: 345 us, 435 with 512); from about 100 on their
+  // buffer is filled too often (256 rows of 248320, k = 128: 112 us against 106)
+  if (a.k <= 96) return launch_top_as<T, 512, 256>(a, N, s);
+  return a.k <= 256 ? launch_top_as<T, 1024, 512>(a, N, s) : launch_top_as<T, 2048, 512>(a, N, s);
 }
 
 }  // namespace apb
@@ -469,8 +491,8 @@ int apb_top_logprobs(const void* logits, int type, long long ld, const float* ro
   if (N <= 0) return 0;
   if (!logits || !logprobs || !ids || !rest || V < 1 || k < 1 || k > V || k > kTopMost || type < 0 || type > 2) return kBadArgument;
   TopArgs a{logits, ld, row_scale, scale, V, k, 1, 0, logprobs, ids, rest};
-  if (type == 0) return launch_top_of<float>(a, N, s);
-  if (type == 1) return launch_top_of<__nv_bfloat16>(a, N, s);
-  return launch_top_of<__half>(a, N, s);
+  if (type == 0) return launch_top<float>(a, N, s);
+  if (type == 1) return launch_top<__nv_bfloat16>(a, N, s);
+  return launch_top<__half>(a, N, s);
 }
 }
