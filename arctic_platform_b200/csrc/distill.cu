@@ -13,13 +13,18 @@
 //   named    one CTA per row: the row's names in rising order for the product's epilogue; logits of the named tokens and the label as
 //            dot products in fp32.  An entry below 0 or beyond the vocabulary names nothing, a token named again counts once, by
 //            its first entry.
-//   product  CTA pairs (gemm_tcgen05_2cta.cu), records of every 128 columns without the named ones
+//   product  CTA pairs (gemm_tcgen05_2cta.cu), records of every 128 columns without the named ones and, where there is room, their exponentials
 //   combine  one warp per row: statistics, value, log-prob and entropy of the label's distribution, c and the named places' gradients
-//   rows     the coefficient of p that the backward product takes; places  the named places and the label's over its output
+//   rows     the coefficient of p in the backward pass; spread  the kept exponentials times it (or the product again); places  the named places
+//            and the label's over that
 //
-// Why the named logits are dot products of their own instead of columns taken out of the product's tiles: the tensor cores round their
-// running sums toward zero, 1e-6 of a logit at 2560 terms, all to one side; here a lane adds every 256th term and the warp joins.  The named
-// tokens carry nearly all of the mass, so values and log-probs are off by a quarter of what they were with all logits from the tiles.
+// Why the named logits are dot products of their own instead of columns taken out of the product's tiles: the named tokens carry nearly all of
+// the mass and of the gradient, and a tensor core's running sum of all H terms is less exact than fp32 sums of a 32nd of them that a warp joins.
+// It costs a read of K rows of the weight for every row (4096 rows with 64 names, H = 2560: 0.23 ms of 8.3).
+//
+// Time of a whole pass and its gradients at 4096 x 151936 x 2560: 8.3 ms, of which the product 2.17 (with the exponentials kept), spread 0.42,
+// d_hidden 2.12 and d_weight 2.25 (cuBLAS's sustained rate gives 2.25 for each); 10.0 with the logits formed again.  At H = 1024, 549 rows
+// 0.79 ms (0.93).
 #include "common.cuh"
 #include "gemm_common.cuh"
 #include "host_utils.cuh"
@@ -41,11 +46,12 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
   return s;
 }
 
-// names [N, K] as given; sorted [N, K]; logit [N, K + 1]: of every entry (-inf where it names nothing), then of the label.
+// names [N, K] as given; sorted [N, K] and where every 128 columns of the vocabulary have theirs in it (the product's named_at); logit [N, K + 1]:
+// of every entry (-inf where it names nothing), then of the label.
 __global__ void __launch_bounds__(256)
 distill_named_kernel(const __nv_bfloat16* __restrict__ hidden, long long ldh, const __nv_bfloat16* __restrict__ weight, long long ldw,
                      const int* __restrict__ names, const int* __restrict__ labels, const float* __restrict__ row_scale, float scale, int K,
-                     int V, int H, int* __restrict__ sorted, float* __restrict__ logit) {
+                     int V, int H, int* __restrict__ sorted, uint16_t* __restrict__ named_at, float* __restrict__ logit) {
   __shared__ int name[kMostNamed];
   __shared__ int kept[kMostNamed];
   const long long row = blockIdx.x;
@@ -67,6 +73,19 @@ distill_named_kernel(const __nv_bfloat16* __restrict__ hidden, long long ldh, co
     int rank = 0;
     for (int j = 0; j < K; ++j) rank += kept[j] < id || (kept[j] == id && j < tid);
     sorted[row * K + rank] = id;
+    name[rank] = id;
+  }
+  __syncthreads();
+  const int tiles = K > 0 ? (V + 127) / 128 : 0;
+  for (int t = tid; t < tiles; t += 256) {
+    int lo = 0, hi = K;                  // first entry of this tile or behind it
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (name[mid] < t * 128) lo = mid + 1;
+      else hi = mid;
+    }
+    while (hi < K && name[hi] < V && name[hi] >> 7 == t) ++hi;
+    named_at[row * tiles + t] = static_cast<uint16_t>(hi > lo ? lo | (hi - lo) << 8 : 0);     // K <= 256, at most 128 in a tile
   }
   const float rs = scale * (row_scale ? row_scale[row] : 1.f);
   const uint4* h = reinterpret_cast<const uint4*>(hidden + row * ldh);
@@ -102,6 +121,8 @@ struct DistillRows {
 // x * y, 0 where x is: a class without mass adds nothing, whatever its logarithm is
 __device__ __forceinline__ float mass_times(float x, float y) { return x > 0.f ? x * y : 0.f; }
 
+constexpr int kRecords = 8;      // of a lane in flight (549 rows of 1187 records: 8 us, 27 with one)
+
 __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows a) {
   const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (row >= a.N) return;
@@ -109,12 +130,23 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows 
   const float* zk = a.logit + static_cast<long long>(row) * (a.K + 1);
   const float* lq = a.teacher + static_cast<long long>(row) * a.K;
   float m = -INFINITY, s = 0.f, e = 0.f;                // of the tokens not named
-  for (int t = lane; t < a.tiles; t += 32) {
-    const float4 v = pr[t];
-    const float mn = fmaxf(m, v.x);
-    const float c0 = m == -INFINITY ? 0.f : __expf(m - mn), c1 = v.x == -INFINITY ? 0.f : __expf(v.x - mn);
-    s = s * c0 + v.y * c1;
-    e = e * c0 + v.z * c1;
+  for (int t0 = lane; t0 < a.tiles; t0 += 32 * kRecords) {
+    float4 v[kRecords];
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < kRecords; ++i) {
+      v[i] = t0 + 32 * i < a.tiles ? pr[t0 + 32 * i] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      mn = fmaxf(mn, v[i].x);
+    }
+    const float c0 = m == -INFINITY ? 0.f : __expf(m - mn);
+    s *= c0;
+    e *= c0;
+#pragma unroll
+    for (int i = 0; i < kRecords; ++i) {
+      const float c = v[i].x == -INFINITY ? 0.f : __expf(v[i].x - mn);
+      s = fmaf(v[i].y, c, s);
+      e = fmaf(v[i].z, c, e);
+    }
     m = mn;
   }
 #pragma unroll
@@ -208,6 +240,38 @@ distill_rows_kernel(const float* __restrict__ g_value, const float* __restrict__
   no_label[i] = -1;
 }
 
+// d(logits) of the tokens not named from what the forward product kept of them, exp(z - m) of every 128 columns' largest m in bf16: times
+// exp(m - lse) and the row's coefficient.  One CTA per row, 16 bytes a thread; bound by memory (4096 x 151936: 2.5 GB, 0.4 ms, where forming the
+// logits again takes 2.1).  The named places hold zeros.  A value is rounded twice, by 2^-8 at most each time; the named tokens, which
+// carry nearly all of a row's gradient, and the label are written from fp32 behind this.
+__global__ void __launch_bounds__(256)
+distill_spread_kernel(const uint4* __restrict__ kept, const float4* __restrict__ partial, const float* __restrict__ glp,
+                      const float* __restrict__ lse, const float* __restrict__ row_scale, float scale, int V, uint4* __restrict__ d) {
+  const long long row = blockIdx.x;
+  const int units = V / 8, tiles = (V + 127) / 128;
+  const float c = -glp[row] * scale * (row_scale ? row_scale[row] : 1.f), l = lse[row];
+#pragma unroll 4
+  for (int u = threadIdx.x; u < units; u += 256) {
+    const uint4 x = __ldcs(kept + row * units + u);
+    const float m = partial[row * tiles + u / 16].x, f = m == -INFINITY ? 0.f : c * __expf(m - l);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      o[i] = pack_bf16x2(v.x * f, v.y * f);
+    }
+    d[row * units + u] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+__global__ void __launch_bounds__(256) distill_round_kernel(const float4* __restrict__ x, uint2* __restrict__ y, long long n) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const float4 v = x[i];
+    y[i] = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  }
+}
+
 // One warp per row: the places of the named tokens, and the label's, in d(logits) [N, V] bf16.
 __global__ void __launch_bounds__(256)
 distill_places_kernel(const int* __restrict__ names, const int* __restrict__ labels, const float* __restrict__ logit,
@@ -250,13 +314,17 @@ extern "C" {
 int apb_lmhead_dlogits(const void* hidden, const void* weight, const int* labels, const float* row_scale, const float* lse, const float* ent,
                        const float* g_lp, const float* g_ent, void* dlogits, int M, int V, int H, long long ldh, long long ldw, long long ldd,
                        float scale, cudaStream_t stream);
+int apb_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc, int a_mn, int b_mn,
+                  int epi, int splits, float alpha, const void* bias, void* C2, long long ldc2, const void* tile_map, int num_map_tiles,
+                  long long b_rows, int bn, int max_ctas, cudaStream_t stream);
 
 // hidden [N, H] and weight [V, H] bf16 (H, V and the strides multiples of 8, 16-byte aligned), labels [N], names [N, K] int32 (K <= 256),
-// teacher [N, K] fp32, rest [N] fp32 or null, row_scale [N] or null (then `scale` alone).  Scratch: sorted [N, K] int32, partial
-// [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1], named_grad [N, K], others, lse, ent [N].
+// teacher [N, K] fp32, rest [N] fp32 or null, row_scale [N] or null (then `scale` alone).  Scratch: sorted [N, K] int32 and
+// behind it [N][ceil(V / 128)] uint16, partial [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1], named_grad [N, K], others, lse, ent [N] and, if not
+// null, kept [N, V] bf16 (then partial too).
 int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* labels, const int* names, const float* teacher,
                            const float* rest, const float* row_scale, float* partial, int* sorted, float* logit, float* value, float* lp,
-                           float* ent, float* lse, float* others, float* named_grad, int N, int V, int H, int K, long long ldh,
+                           float* ent, float* lse, float* others, float* named_grad, void* kept, int N, int V, int H, int K, long long ldh,
                            long long ldw, float scale, float mix, cudaStream_t stream) {
   using namespace apb;
   if (N <= 0) return 0;
@@ -265,7 +333,8 @@ int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* la
       ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15))
     return kBadArgument;
   distill_named_kernel<<<N, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(hidden), ldh, static_cast<const __nv_bfloat16*>(weight),
-                                              ldw, names, labels, row_scale, scale, K, V, H, sorted, logit);
+                                              ldw, names, labels, row_scale, scale, K, V, H, sorted,
+                                              reinterpret_cast<uint16_t*>(sorted + static_cast<long long>(N) * K), logit);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
   CUtensorMap ta, tb;
@@ -278,11 +347,14 @@ int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* la
   p.N = V;
   p.K = H;
   p.epi = kEpiRestPartial;
+  p.C = kept;
+  p.ldc = V;
   p.splits = 1;
   p.alpha = scale;
   p.row_scale = row_scale;
   p.partial = partial;
   p.named = sorted;
+  p.named_at = reinterpret_cast<const uint16_t*>(sorted + static_cast<long long>(N) * K);
   p.n_named = K;
   p.status = status_device_ptr();
   rc = launch_gemm_pair(ta, tb, p, stream);
@@ -293,26 +365,52 @@ int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* la
   return static_cast<int>(cudaGetLastError());
 }
 
-// d(logits) [N, V] bf16 (row stride ldd) of the rows of a forward pass: the coefficients of their probabilities, the product whose epilogue
-// writes probability times coefficient, then the named tokens' places and the label's.  g_value, g_lp, g_ent [N] fp32: upstream gradients
-// (null: none); the others as kept by the forward pass.  Scratch: [2 N] words of 32 bits.
-int apb_lmhead_distill_dlogits(const void* hidden, const void* weight, const int* names, const int* labels, const float* row_scale,
-                               const float* logit, const float* named_grad, const float* others, const float* lse, const float* ent,
-                               const float* g_value, const float* g_lp, const float* g_ent, float* scratch, void* dlogits, int N, int V, int H,
-                               int K, long long ldh, long long ldw, long long ldd, float scale, cudaStream_t stream) {
+// The backward pass of N rows of a forward pass: d(logits) [N, V] bf16, of it d_hidden [N, H] bf16 and d_weight [V, H] (bf16, or fp32 that is
+// added to), either may be null.  d(logits): the coefficients of the probabilities; probability times coefficient, from what the forward
+// pass kept or, without it or with g_ent, by the product again; the named tokens' places and the label's.  g_value, g_lp, g_ent [N] fp32:
+// upstream gradients (null: none); the others as kept by the forward pass.  Scratch: scratch [2 N] words of 32 bits; total [N, H] fp32 or null:
+// then d_hidden's product is cut along the vocabulary.
+int apb_lmhead_distill_bwd(const void* hidden, const void* weight, const int* names, const int* labels, const float* row_scale,
+                           const float* logit, const float* named_grad, const float* others, const float* lse, const float* ent,
+                           const float* g_value, const float* g_lp, const float* g_ent, const void* kept, const float* partial, float* scratch,
+                           void* dlogits, void* d_hidden, float* total, void* d_weight, int weight_f32, int N, int V, int H, int K,
+                           long long ldh, long long ldw, float scale, cudaStream_t stream) {
   using namespace apb;
   if (N <= 0) return 0;
   if (!hidden || !weight || !labels || !logit || !others || !lse || !ent || !scratch || !dlogits || K < 0 || K > kMostNamed ||
-      (K > 0 && (!names || !named_grad)) || V <= 0 || H <= 0 || (ldd % 8))
+      (K > 0 && (!names || !named_grad)) || V <= 0 || H <= 0 || (V % 8) || (H % 8) || (kept && !partial))
     return kBadArgument;
   int* no_label = reinterpret_cast<int*>(scratch + N);
   distill_rows_kernel<<<(N + 255) / 256, 256, 0, stream>>>(g_value, g_lp, others, N, scratch, no_label);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
-  const int rc = apb_lmhead_dlogits(hidden, weight, no_label, row_scale, lse, ent, scratch, g_ent, dlogits, N, V, H, ldh, ldw, ldd, scale, stream);
+  int rc = 0;
+  if (kept && !g_ent) {
+    distill_spread_kernel<<<N, 256, 0, stream>>>(static_cast<const uint4*>(kept), reinterpret_cast<const float4*>(partial), scratch, lse, row_scale,
+                                                 scale, V, static_cast<uint4*>(dlogits));
+    rc = static_cast<int>(cudaGetLastError());
+  } else {
+    rc = apb_lmhead_dlogits(hidden, weight, no_label, row_scale, lse, ent, scratch, g_ent, dlogits, N, V, H, ldh, ldw, V, scale, stream);
+  }
   if (rc) return rc;
   distill_places_kernel<<<(N + 7) / 8, 256, 0, stream>>>(names, labels, logit, named_grad, others, lse, ent, g_value, g_lp, g_ent, row_scale,
-                                                         scale, K, V, N, static_cast<__nv_bfloat16*>(dlogits), ldd);
-  return static_cast<int>(cudaGetLastError());
+                                                         scale, K, V, N, static_cast<__nv_bfloat16*>(dlogits), V);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (d_hidden && total) {
+    e = cudaMemsetAsync(total, 0, sizeof(float) * N * H, stream);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    rc = apb_gemm_bf16(dlogits, weight, total, N, H, V, V, ldw, H, 0, 1, kEpiF32Accum, 1, 1.f, nullptr, nullptr, 0, nullptr, 0, 0, 0, 0, stream);
+    if (rc) return rc;
+    const long long n = static_cast<long long>(N) * H / 4, grid = (n + 255) / 256, cap = 8ll * sm_count();
+    distill_round_kernel<<<static_cast<int>(grid < cap ? grid : cap), 256, 0, stream>>>(reinterpret_cast<const float4*>(total),
+                                                                                       static_cast<uint2*>(d_hidden), n);
+    rc = static_cast<int>(cudaGetLastError());
+  } else if (d_hidden) {
+    rc = apb_gemm_bf16(dlogits, weight, d_hidden, N, H, V, V, ldw, H, 0, 1, kEpiBf16, 1, 1.f, nullptr, nullptr, 0, nullptr, 0, 0, 0, 0, stream);
+  }
+  if (rc || !d_weight) return rc;
+  return apb_gemm_bf16(dlogits, hidden, d_weight, V, H, N, V, ldh, H, 1, 1, weight_f32 ? kEpiF32Accum : kEpiBf16, 1, 1.f, nullptr, nullptr, 0,
+                       nullptr, 0, 0, 0, 0, stream);
 }
 }

@@ -20,7 +20,8 @@ enum GemmEpilogue : int {
   kEpiGeGLU = 9,       // as kEpiSwiGLU with the tanh form of GELU as the activation of the gate
   kEpiClampGLU = 10,   // as kEpiSwiGLU: g = min(gate, limit), u = clamp(up, -limit, limit), g sigmoid(1.702 g) (u + 1)
   kEpiSigmoidGate = 11,    // C(bf16) = acc * sigmoid(gate), gate (bf16) laid out like C
-  kEpiRestPartial = 12,    // as kEpiLogprobPartial over the columns that the row does not name (CTA pairs only; no label)
+  kEpiRestPartial = 12,    // as kEpiLogprobPartial over the columns that the row does not name (CTA pairs only; no label); C(bf16) = their
+                           // exp(z - max of the record), 0 for the others, if C != null
 };
 
 __host__ __device__ inline bool is_glu_epilogue(int epi) {
@@ -68,6 +69,7 @@ struct GemmParams {
   const float* row_glp;    // [M] upstream gradient of the log-prob
   const float* row_gent;   // [M] upstream gradient of the entropy, or null
   const int* named;        // kEpiRestPartial: [M][n_named] columns that a row names, rising, INT_MAX behind the last
+  const uint16_t* named_at; // [M][ceil(N / 128)] of every 128 columns: its first entry of that list, and 256 times how many it has
   int n_named;
   // peer-aware modes
   void* c_peers[8];        // per-rank output base pointers (symmetric buffers)
@@ -243,49 +245,35 @@ __device__ __forceinline__ void lmhead_partial_128(const GemmParams& p, int row,
 }
 
 // One record (max, sum exp, sum exp * z, 0) of a row's 128 columns from `n0` on without those that the row names: the sum of the
-// others is formed from them alone, as one minus the named ones' share would keep nothing of it where they hold all but a little.  Where
-// the named columns fall is found by a search in the row's rising list (its 7 loads and the 128 masked columns hide behind the main loop,
-// which the epilogue of another accumulator always overlaps: the lm-head product of 4096 x 151936 x 2560 takes as long as without).
-__device__ __forceinline__ void lmhead_rest_128(const GemmParams& p, int row, bool row_ok, const uint32_t (&acc)[4][32], int n0) {
-  const float rs = p.alpha * ((p.row_scale && row_ok) ? p.row_scale[row] : 1.f);
-  const int cols = p.N - n0;
+// others is formed from them alone, as one minus the named ones' share would keep nothing of it where they hold all but a little.
+struct LmheadRest {
   uint32_t out[4];                       // bit j of word c: column 32 c + j is left out
+  float rs;
+  // Which columns are named, from the row's table and, where it has some here, its list.  Before the accumulator is waited for: loads one behind
+  // another take long while the products' operands come in.  (549 x 151936 x 1024 with the exponentials kept: 0.34 ms, with a search in the
+  // list instead of the table 0.37.  At K = 2560 the products hide either.)
+  __device__ __forceinline__ void find(const GemmParams& p, int row, bool row_ok, int n0) {
+    rs = p.alpha * ((p.row_scale && row_ok) ? p.row_scale[row] : 1.f);
+    const int cols = p.N - n0;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int n = cols - 32 * c;
-    out[c] = n >= 32 ? 0u : n <= 0 ? ~0u : ~0u << n;
-  }
-  if (row_ok && p.n_named > 0) {
-    const int* list = p.named + static_cast<long long>(row) * p.n_named;
-    int lo = 0, hi = p.n_named;          // first entry that is not below n0
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (list[mid] < n0) lo = mid + 1;
-      else hi = mid;
+    for (int c = 0; c < 4; ++c) {
+      const int n = cols - 32 * c;
+      out[c] = n >= 32 ? 0u : n <= 0 ? ~0u : ~0u << n;
     }
-    for (; lo < p.n_named; ++lo) {
-      const int j = list[lo] - n0;       // n0 >= 0: no overflow
-      if (j >= 128) break;
+    if (!row_ok || p.n_named <= 0 || cols <= 0) return;
+    const uint32_t at = p.named_at[static_cast<long long>(row) * ((p.N + 127) / 128) + n0 / 128];
+    const int lo = at & 255, hi = lo + (at >> 8);
+    if (lo == hi) return;
+    const int* list = p.named + static_cast<long long>(row) * p.n_named;
+    for (int i = lo; i < hi; ++i) {
+      const int j = list[i] - n0;        // 0 .. 127
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         if (j >> 5 == c) out[c] |= 1u << (j & 31);
     }
   }
-  float m = -INFINITY, s = 0.f, e = 0.f;
-#pragma unroll
-  for (int j = 0; j < 128; ++j)
-    if (!((out[j / 32] >> (j % 32)) & 1u)) m = fmaxf(m, __uint_as_float(acc[j / 32][j % 32]) * rs);
-#pragma unroll
-  for (int j = 0; j < 128; ++j) {
-    const bool in = !((out[j / 32] >> (j % 32)) & 1u);
-    const float z = __uint_as_float(acc[j / 32][j % 32]) * rs;
-    const float x = in ? __expf(z - m) : 0.f;
-    s += x;
-    e += in ? x * z : 0.f;
-  }
-  if (row_ok)
-    *(reinterpret_cast<float4*>(p.partial) + static_cast<long long>(row) * ((p.N + 127) / 128) + n0 / 128) = make_float4(m, s, e, 0.f);
-}
+  __device__ __forceinline__ bool in(int j) const { return !((out[j / 32] >> (j % 32)) & 1u); }
+};
 
 // What d loss / d logits of a row needs besides the logit.
 struct LmheadRow {

@@ -74,13 +74,37 @@ enum PairEpi : int { kPairBf16, kPairF32, kPairSwiGLU, kPairGeGLU, kPairClampGLU
 // output are clipped by the tensor maps; a box that would begin outside is not sent.
 template <int EPI>
 __device__ __forceinline__ void pair_epilogue(const GemmParams& p, const CUtensorMap& tma_c, const CUtensorMap& tma_c2,
-                                              const StagedBox& out, int row0, int nb, const uint32_t (&acc)[4][32]) {
+                                              const StagedBox& out, int row0, int nb, const uint32_t (&acc)[4][32], const LmheadRest& rest) {
   const int row = row0 + out.lane;
   const bool row_ok = row < p.M;
   if constexpr (EPI == kPairPartial) {
     lmhead_partial_128(p, row, row_ok, acc, nb);
   } else if constexpr (EPI == kPairRest) {
-    lmhead_rest_128(p, row, row_ok, acc, nb);
+    float m = -INFINITY, s = 0.f, e = 0.f;
+#pragma unroll
+    for (int j = 0; j < 128; ++j)
+      if (rest.in(j)) m = fmaxf(m, __uint_as_float(acc[j / 32][j % 32]) * rest.rs);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const bool keep = p.C != nullptr && nb + c * 64 < p.N;
+      if (keep) out.begin();
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int i = c * 64 + u * 8 + j;
+          const float z = __uint_as_float(acc[i / 32][i % 32]) * rest.rs;
+          x[j] = rest.in(i) ? __expf(z - m) : 0.f;
+          s += x[j];
+          e += rest.in(i) ? x[j] * z : 0.f;
+        }
+        if (keep) out.put(u, make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])));
+      }
+      if (keep) out.send(&tma_c, nb + c * 64, row0, false);
+    }
+    if (row_ok)
+      *(reinterpret_cast<float4*>(p.partial) + static_cast<long long>(row) * ((p.N + 127) / 128) + nb / 128) = make_float4(m, s, e, 0.f);
   } else if constexpr (EPI == kPairF32) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -374,6 +398,8 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       const int halves = halves_of(n0);
       for (int h = 0; h < halves; ++h) {
         const int slot = NT == 512 ? h : (it & 1);
+        LmheadRest rest;
+        if constexpr (EPI == kPairRest) rest.find(p, row0 + lane, row0 + lane < p.M, n0 + h * 256 + part * 128);
         ok = mbar_wait(&tfull_bar[slot], used[slot] & 1, p.status, kTimeoutTmemFull);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -391,7 +417,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[slot]), 0));
         const int nb = n0 + h * 256 + part * 128;
-        if (row0 < p.M && nb < p.N) pair_epilogue<EPI>(p, tma_c, tma_c2, out, row0, nb, acc);
+        if (row0 < p.M && nb < p.N) pair_epilogue<EPI>(p, tma_c, tma_c2, out, row0, nb, acc, rest);
       }
     }
     if (lane == 0) tma_out_wait_all();

@@ -7,8 +7,8 @@ these classes, q the teacher's masses and p the student's, the divergence is ``(
 ``teacher_rest`` both sums run over the named tokens alone (p stays normalised over the whole vocabulary).
 
 On CUDA the vocabulary product runs on tcgen05 CTA pairs with an epilogue that reduces every 128 columns to records without the named
-tokens, whose logits are fp32 dot products (``csrc/distill.cu``); the backward pass forms d(logits) in bf16 a chunk of rows at a time and feeds
-two products, as :func:`~.logprob.lm_head_logprobs` does.  CPU tensors use the fp32 expression below (the oracle of the GPU tests).
+tokens, whose logits are fp32 dot products (``csrc/distill.cu``); the backward pass forms d(logits) in bf16 a chunk of rows at a time, from the
+exponentials that the forward pass kept or from the logits once more, and feeds two products.  CPU tensors use the fp32 expression below (the oracle of the GPU tests).
 """
 from __future__ import annotations
 
@@ -17,7 +17,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from . import _lib, gemm
+from . import _lib
 from .logprob import _BWD_BUDGET, _BWD_ROWS, _bwd_rows
 from ..utils import memory_budget
 
@@ -30,8 +30,8 @@ def _fn(name: str):
     if not _FN:
         c, fns = ctypes, {}
         vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
-        fns["fwd"] = _lib.declare("apb_lmhead_distill_fwd", [vp] * 16 + [i, i, i, i, ll, ll, f, f, vp])
-        fns["dlogits"] = _lib.declare("apb_lmhead_distill_dlogits", [vp] * 15 + [i, i, i, i, ll, ll, ll, f, vp])
+        fns["fwd"] = _lib.declare("apb_lmhead_distill_fwd", [vp] * 17 + [i, i, i, i, ll, ll, f, f, vp])
+        fns["bwd"] = _lib.declare("apb_lmhead_distill_bwd", [vp] * 20 + [i, i, i, i, i, ll, ll, f, vp])
         _FN.update(fns)              # in one step: another thread may be looking
     return _FN[name]
 
@@ -82,9 +82,19 @@ def distill_ref(hidden, weight, labels, teacher_ids, teacher_logprobs, teacher_r
 
 def _split_pays(n: int, H: int, pairs: int) -> bool:
     """Whether a product ``[n, H]`` over the vocabulary is cut into parts of it that add up in fp32: where its tiles of 256 x 256 leave much of
-    their last wave of CTA pairs idle (4096 x 2560: 160 tiles, 2.2 waves, 2.6 ms; in six parts 2.0 ms)."""
+    their last wave of CTA pairs idle (4096 x 2560: 160 tiles, 2.2 waves, 2.6 ms; in six parts 2.1 ms)."""
     tiles = -(-n // 256) * -(-H // 256)
     return tiles < 0.85 * pairs * -(-tiles // pairs)
+
+
+_KEEP_FROM = 1 << 26      # probabilities from which on keeping them pays: below, looking for the memory takes as long as forming them again
+
+
+def _keep_pays(N: int, V: int, device) -> bool:
+    """Whether the forward pass keeps the exponentials of its logits in bf16 for the backward pass, which then need not form the logits again
+    (a quarter of its products): where the device has room for them and for the gradient beside."""
+    size = 2 * N * V
+    return N * V >= _KEEP_FROM and size <= _BWD_BUDGET // 2 and memory_budget.spare_bytes(device, 3 * size) >= 3 * size
 
 
 class _LmHeadDistillFn(torch.autograd.Function):
@@ -94,18 +104,20 @@ class _LmHeadDistillFn(torch.autograd.Function):
         V, K = weight.shape[0], ids.shape[1]
         dev, f32 = hidden.device, torch.float32
         partial = torch.empty((N, (V + 127) // 128, 4), device=dev, dtype=f32)
-        in_order = torch.empty((N, K), device=dev, dtype=torch.int32)
+        in_order = torch.empty(N * K + (N * partial.shape[1] + 1) // 2, device=dev, dtype=torch.int32)
         value, lp, ent = (torch.empty(N, device=dev, dtype=f32) for _ in range(3))
-        # what the backward pass takes up again: logits of the named tokens and the label, gradients of the named ones, two numbers a row
+        # what the backward pass takes up again: logits of the named tokens and the label, gradients of the named ones, two numbers a row and
+        # the exponentials of the others
         logit, named = torch.empty((N, K + 1), device=dev, dtype=f32), torch.empty((N, K), device=dev, dtype=f32)
         rows = torch.empty((2, N), device=dev, dtype=f32)
         lse = rows.data_ptr()
+        kept = torch.empty((N, V), device=dev, dtype=torch.bfloat16) if any(ctx.needs_input_grad[:2]) and _keep_pays(N, V, dev) else None
         opt = lambda t: None if t is None else t.data_ptr()                                  # noqa: E731
         _lib.check(_fn("fwd")(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), ids.data_ptr(), teacher.data_ptr(), opt(rest),
                               opt(inv_temp_t), partial.data_ptr(), in_order.data_ptr(), logit.data_ptr(), value.data_ptr(), lp.data_ptr(),
-                              ent.data_ptr(), lse, lse + 4 * N, named.data_ptr(), N, V, H, K, hidden.stride(0), weight.stride(0), inv_temp_s,
-                              reverse, _lib.stream_ptr()), "apb_lmhead_distill_fwd")
-        ctx.save_for_backward(hidden, weight, labels, ids, inv_temp_t, logit, named, rows, ent)
+                              ent.data_ptr(), lse, lse + 4 * N, named.data_ptr(), opt(kept), N, V, H, K, hidden.stride(0), weight.stride(0),
+                              inv_temp_s, reverse, _lib.stream_ptr()), "apb_lmhead_distill_fwd")
+        ctx.save_for_backward(hidden, weight, labels, ids, inv_temp_t, logit, named, rows, ent, kept, None if kept is None else partial)
         ctx.inv_temp_s, ctx.with_entropy, ctx.bwd_chunk = inv_temp_s, with_entropy, bwd_chunk
         ctx.set_materialize_grads(False)
         return value, lp, (ent if with_entropy else lp.new_zeros(0))
@@ -113,7 +125,7 @@ class _LmHeadDistillFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_value, g_lp, g_ent):
-        hidden, weight, labels, ids, it, logit, named, rows, ent = ctx.saved_tensors
+        hidden, weight, labels, ids, it, logit, named, rows, ent, kept, partial = ctx.saved_tensors
         N, H = hidden.shape
         V, K = weight.shape[0], ids.shape[1]
         dev = hidden.device
@@ -133,24 +145,17 @@ class _LmHeadDistillFn(torch.autograd.Function):
         dw = None if not want_w or acc is not None else torch.empty((V, H), device=dev, dtype=weight.dtype) if chunk >= N else \
             torch.zeros((V, H), device=dev, dtype=torch.float32)
         pairs = torch.cuda.get_device_properties(dev).multi_processor_count // 2
-        lse = rows.data_ptr()
+        total = torch.empty((min(chunk, N), H), device=dev, dtype=torch.float32) if want_h and _split_pays(min(chunk, N), H, pairs) else None
+        into = acc if acc is not None else dw
+        lse, tiles = rows.data_ptr(), (V + 127) // 128
         for s in range(0, N, chunk):
             n = min(chunk, N - s)
-            h, dl = hidden[s:s + n], buf[:n]
-            _lib.check(_fn("dlogits")(h.data_ptr(), weight.data_ptr(), at(ids, s, 4 * K), at(labels, s, 4), at(it, s, 4),
-                                      at(logit, s, 4 * K + 4), at(named, s, 4 * K), lse + 4 * (N + s), lse + 4 * s, at(ent, s, 4),
-                                      at(g_value, s, 4), at(g_lp, s, 4), at(g_ent, s, 4), scratch.data_ptr(), dl.data_ptr(), n, V, H, K,
-                                      hidden.stride(0), weight.stride(0), V, ctx.inv_temp_s, _lib.stream_ptr()), "apb_lmhead_distill_dlogits")
-            if want_h:
-                if _split_pays(n, H, pairs):
-                    total = torch.zeros((n, H), device=dev, dtype=torch.float32)
-                    gemm.gemm_raw(dl, weight, total, M=n, N=H, K=V, b_mn=True, epi=gemm.EPI_F32_ACCUM)
-                    d_hidden[s:s + n].copy_(total)
-                else:
-                    gemm.matmul_nn(dl, weight, out=d_hidden[s:s + n])
-            if want_w:
-                into = acc if acc is not None else dw
-                gemm.matmul_tn(dl, h, out=into, accumulate=into.dtype == torch.float32)
+            _lib.check(_fn("bwd")(at(hidden, s, 2 * hidden.stride(0)), weight.data_ptr(), at(ids, s, 4 * K), at(labels, s, 4), at(it, s, 4),
+                                  at(logit, s, 4 * K + 4), at(named, s, 4 * K), lse + 4 * (N + s), lse + 4 * s, at(ent, s, 4),
+                                  at(g_value, s, 4), at(g_lp, s, 4), at(g_ent, s, 4), at(kept, s, 2 * V), at(partial, s, 16 * tiles),
+                                  scratch.data_ptr(), buf.data_ptr(), at(d_hidden, s, 2 * H), at(total, 0, 4), at(into, 0, 4),
+                                  into is not None and into.dtype == torch.float32, n, V, H, K, hidden.stride(0), weight.stride(0),
+                                  ctx.inv_temp_s, _lib.stream_ptr()), "apb_lmhead_distill_bwd")
         if dw is not None and dw.dtype != weight.dtype:
             dw = dw.to(weight.dtype)
         return d_hidden, dw, None, None, None, None, None, None, None, None, None

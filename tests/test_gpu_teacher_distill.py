@@ -34,7 +34,7 @@ def gradients(h, w, labels, ids, lq, rest, it, reverse, ups, entropy=True):
     return out, d @ w.double(), d.t() @ h.double(), d.abs() @ w.double().abs(), d.abs().t() @ h.double().abs()
 
 
-def check(N, V, H, K, with_rest, reverse, it=1.0, entropy=True, ups=None, chunk=None, data=None, seed=0):
+def check(N, V, H, K, with_rest, reverse, it=1.0, entropy=True, ups=None, chunk=None, data=None, seed=0, roundings=1):
     h, w, labels, ids, lq, rest = data or make(N, V, H, K, seed)
     rest = rest if with_rest else None
     g = torch.Generator(device="cuda").manual_seed(seed + 1)
@@ -53,7 +53,7 @@ def check(N, V, H, K, with_rest, reverse, it=1.0, entropy=True, ups=None, chunk=
     grads = torch.autograd.grad([o for o, u in zip(got, ups) if u is not None], (hl, wl), [u for u in ups if u is not None])
     for a, b, s in zip(grads, (dh, dw), (sh, sw)):
         off = (a.double() - b).abs()
-        assert bool((off <= (2.0 ** -8 + 4 * ERR * max(scale, 1)) * s + 2.0 ** -8 * b.abs() + 1e-12).all()), float((off / s.clamp_min(1e-9)).max())
+        assert bool((off <= (roundings * 2.0 ** -8 + 4 * ERR * max(scale, 1)) * s + 2.0 ** -8 * b.abs() + 1e-12).all()), float((off / s.clamp_min(1e-9)).max())
     return got, grads
 
 
@@ -61,6 +61,34 @@ def check(N, V, H, K, with_rest, reverse, it=1.0, entropy=True, ups=None, chunk=
 @pytest.mark.parametrize("with_rest,reverse", [(False, 0.0), (True, 0.0), (True, 1.0), (False, 1.0), (True, 0.4)])
 def test_values_and_gradients(N, V, H, K, with_rest, reverse):
     check(N, V, H, min(K, V), with_rest, reverse, seed=N)
+
+
+@pytest.mark.parametrize("N,V,H,K", [(1, 8, 8, 1), (5, 136, 64, 8), (129, 2008, 128, 64), (300, 520, 72, 256), (260, 4096, 256, 3), (700, 392, 64, 5)])
+@pytest.mark.parametrize("reverse", [0.0, 0.4])
+def test_exponentials_kept_for_the_backward_pass(N, V, H, K, reverse, monkeypatch):
+    """A probability is rounded to bf16 once more (and by the square of a rounding, which 2^-8 of its 4 ERR covers)."""
+    monkeypatch.setattr(distill, "_keep_pays", lambda *a: True)
+    one = torch.linspace(-1, 1, N, device="cuda")
+    more = {"roundings": 2, "seed": N}
+    check(N, V, H, min(K, V), True, reverse, ups=[one, one.flip(0), None], **more)
+    check(N, V, H, min(K, V), True, reverse, it=torch.linspace(0.3, 1.5, N, device="cuda"), ups=[one, None, None], chunk=256, **more)
+    check(N, V, H, min(K, V), True, reverse, **more)           # an entropy's gradient too: formed from the logits again
+
+
+def test_kept_exponentials_serve_two_backward_passes_and_one_is_chosen_by_size(monkeypatch):
+    h, w, labels, ids, lq, rest = make(512, 131072, 64, 8, 11)         # from 2^26 on they are kept
+    hl, wl = h.requires_grad_(True), w.requires_grad_(True)
+    value = distill.lm_head_distill(hl, wl, labels, ids, lq, rest, reverse=0.5)[0].sum()
+    kept = [t for t in value.grad_fn.next_functions[0][0].saved_tensors if t is not None and t.shape == (512, 131072)]
+    assert len(kept) == 1 and kept[0].dtype == torch.bfloat16
+    a = torch.autograd.grad(value, (hl, wl), retain_graph=True)
+    b = torch.autograd.grad(value, (hl, wl))
+    assert torch.equal(a[1], b[1])
+    torch.testing.assert_close(a[0], b[0], rtol=2.0 ** -7, atol=1e-6)    # parts of the vocabulary add up in any order
+    monkeypatch.setattr(distill, "_keep_pays", lambda *a: False)
+    c = torch.autograd.grad(distill.lm_head_distill(hl, wl, labels, ids, lq, rest, reverse=0.5)[0].sum(), (hl, wl))
+    for x, y in zip(a, c):
+        assert float((x.double() - y.double()).norm() / y.double().norm()) < 2.0 ** -7     # each once or twice off by 2^-8 and 2^-9 on average
 
 
 def test_temperatures_and_no_entropy():
