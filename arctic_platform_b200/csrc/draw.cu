@@ -3,8 +3,8 @@
 //
 // Mathematics.  Every restriction keeps the logits from a threshold on, so a row comes down to one threshold: the top_k-th largest
 // logit; the least logit with exp((l - max) / T) >= min_p; the least logit of which the strictly larger ones hold less than top_p of what
-// stayed so far.  Masses and their sums are 64-bit numbers: fp32 ones put one draw of some hundred, from flat rows of 151936, on the
-// neighbour's side of a border.  Nothing is added by floating atomics, so that the same numbers give the same token every time.
+// stayed so far.  Masses and their sums are 64-bit numbers: an fp32 running sum is off by 2^-24 of itself at best, a hundredth of
+// one token's mass in a flat row of 151936, which would put one draw of a hundred on the neighbour's side of a border.  Nothing is added by floating atomics, so that the same numbers give the same token every time.
 //
 // Layout.  One CTA of 32 warps a row, or a cluster of 2, 4 or 8 where the rows leave SMs idle.  One walk reads a part from global memory, finds the
 // largest logit and adds up the masses (of exp(l / T) itself: 64-bit numbers have the range, so nothing waits for the largest); a warp has a
@@ -127,8 +127,8 @@ __device__ __forceinline__ void row_sync(int parts) {       // the CTAs of a row
 // exp2(x / 64) of a 64-bit number, x from -2^16 to 2^16: x split into a whole number, whose power is a table's and an exponent, and a rest of at
 // most 1/2, whose power is its series to the third term (the fourth is below 4e-11 of the result).  The high word of a table's entry is less by
 // its index at the place from which the shifted whole number carries into the exponent, so that one addition sets both.  7 operations in 64
-// bits with the addition of the result to a sum.  The table has a copy for every two lanes: 1024 entries and a term less, one copy, cost
-// 6 passes through shared memory a load where this has 2 (the walk of a row of 151936 by one CTA 21 us).
+// bits with the addition of the result to a sum.  The table has a copy for every two lanes: a load takes 2 passes through shared
+// memory, where one table of 1024 entries and a series shorter by a term takes 6 and no less time in all.
 struct DrawPower {
   double y, power;                        // the result is their product
 };
@@ -534,9 +534,9 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
   r.m = m;
   r.cut = m - 70.f * t;
   const int k = a.top_k ? a.top_k[b] : a.top_k_all;
-  const float mp = fminf(a.min_p ? a.min_p[b] : a.min_p_all, 1.f);
+  const float least_share = a.min_p ? a.min_p[b] : a.min_p_all, mp = fminf(least_share, 1.f);
   const float p = a.top_p ? a.top_p[b] : a.top_p_all;
-  const bool by_rank = k > 0 && k < a.V, by_share = mp > 0.f, by_mass = p < 1.f;
+  const bool by_rank = k > 0 && k < a.V, by_share = least_share > 0.f, by_mass = p < 1.f;
   // exp((l - m) / T) of this warp's elements >= bound
   auto weigh = [&](float bound, int slot) {
     double s0 = 0.0;

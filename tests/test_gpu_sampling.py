@@ -51,6 +51,17 @@ def test_types_and_strides(dtype, spare):
     same(wide[:, 1:], u, 0.8, 30, 0.9)                        # rows that begin off the 16-byte boundaries
 
 
+def test_settings_that_are_not_numbers_are_off_and_expanded_rows():
+    z, u = make(6, 5003, seed=9)
+    nan = float("nan")
+    for s in ((1.0, 0, 1.0, nan), (1.0, 0, nan, 0.0), (0.8, 20, nan, nan), (0.8, 20, 0.9, torch.full((6,), nan, device="cuda"))):
+        same(z, u, *s)
+    a = sampling.sample(z, u, 0.8, 20)
+    b = sampling.sample(z, u, 0.8, 20, nan, nan)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    same(z[:1].expand(6, 5003), u, 0.8, 0, 0.9)
+
+
 def test_settings_of_their_own_for_each_row():
     B, V = 48, 5003
     z, u = make(B, V, seed=5)
