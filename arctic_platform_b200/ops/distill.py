@@ -205,9 +205,9 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
         with torch.cuda.device(hidden.device):
             return lm_head_distill(hidden, weight, labels, teacher_ids, teacher_logprobs, teacher_rest, inv_temperature, reverse, with_entropy,
                                    bwd_chunk)
-    if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.data_ptr() % 16:
+    if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.stride(0) < H or weight.data_ptr() % 16:
         raise ValueError("weight must have whole rows on 16-byte boundaries")
-    if hidden.stride(1) != 1 or hidden.stride(0) % 8 or hidden.data_ptr() % 16:
+    if hidden.stride(1) != 1 or hidden.stride(0) % 8 or hidden.stride(0) < H or hidden.data_ptr() % 16:     # expanded rows too
         hidden = hidden.contiguous()
     whole = lambda t, dtype: t.detach().to(dtype).contiguous()                               # noqa: E731
     if teacher_ids.dtype == torch.int64:         # before 32 bits cut them

@@ -209,6 +209,81 @@ def test_strides_streams_and_a_captured_forward():
     assert torch.equal(got, want)
 
 
+def test_expanded_rows_and_overlapping_ones():
+    h, w, labels, ids, lq, rest = make(9, 256, 64, 6, 12)
+    one = h[:1].expand(9, 64)
+    assert one.stride(0) == 0
+    want = distill.lm_head_distill(one.contiguous(), w, labels, ids, lq, rest)[0]
+    hl = h[:1].detach().requires_grad_(True)
+    got = distill.lm_head_distill(hl.expand(9, 64), w, labels, ids, lq, rest)[0]
+    assert torch.equal(got, want)
+    (d,) = torch.autograd.grad(got.sum(), hl)
+    each = [torch.autograd.grad(distill.lm_head_distill(x, w, labels[i:i + 1], ids[i:i + 1], lq[i:i + 1], rest[i:i + 1])[0].sum(), x)[0]
+            for i in range(9) for x in [h[:1].detach().requires_grad_(True)]]
+    many = torch.stack(each).double()
+    # nine gradients in bf16 each (2^-8 twice: d(logits) and the row) add up in bf16
+    assert bool(((d.double() - many.sum(0)).abs() <= 12 * 2.0 ** -8 * many.abs().sum(0) + 1e-2 * many.abs().amax()).all())
+    again = lq[:1].expand(9, 6)
+    a = distill.lm_head_distill(h, w, labels, ids[:1].expand(9, 6), again, rest[:1].expand(9))[0]
+    b = distill.lm_head_distill(h, w, labels, ids[:1].expand(9, 6).contiguous(), again.contiguous(), rest[:1].expand(9).contiguous())[0]
+    assert torch.equal(a, b)
+    with pytest.raises(ValueError):
+        distill.lm_head_distill(h, w[:1].expand(256, 64), labels, ids, lq, rest)
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_a_captured_forward_and_backward_pass(keep, monkeypatch):
+    monkeypatch.setattr(distill, "_keep_pays", lambda *a: keep)
+    h, w, labels, ids, lq, rest = make(300, 520, 64, 7, 13)
+    lab32, up = labels.to(torch.int32), torch.linspace(-1, 1, 300, device="cuda")
+
+    def run(hl, wl):
+        value, lp, _ = distill.lm_head_distill(hl, wl, lab32, ids, lq, rest, reverse=0.5)
+        return torch.autograd.grad([value, lp], (hl, wl), [up, up])
+
+    want = run(h.clone().requires_grad_(True), w.clone().requires_grad_(True))
+    hl, wl = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(hl, wl)
+    for _ in range(2):
+        for g in got:
+            g.zero_()
+        graph.replay()
+        assert torch.equal(got[1], want[1])
+        torch.testing.assert_close(got[0], want[0], rtol=2.0 ** -7, atol=1e-6)     # parts of the vocabulary add up in any order
+    with torch.no_grad():
+        hl.copy_(h.flip(0))
+    graph.replay()
+    new = run(h.flip(0).clone().requires_grad_(True), w.clone().requires_grad_(True))
+    assert torch.equal(got[1], new[1]) and not torch.equal(got[1], want[1])
+
+
+def test_two_passes_on_two_streams_at_once():
+    data = [make(200, 1000, 128, 9, s) for s in (14, 15)]
+
+    def run(d):
+        h, w, labels, ids, lq, rest = d
+        hl, wl = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        return torch.autograd.grad(distill.lm_head_distill(hl, wl, labels, ids, lq, rest, reverse=0.3)[0].sum(), (hl, wl))
+
+    want = [run(d) for d in data]
+    sides = [torch.cuda.Stream() for _ in data]
+    got = [[], []]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for i, d in enumerate(data):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(run(d))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert torch.equal(g[1], want[i][1])
+            torch.testing.assert_close(g[0], want[i][0], rtol=2.0 ** -7, atol=1e-5)
+
+
 def test_refusals():
     h, w, labels, ids, lq, rest = make(8, 64, 64, 4, 9)
     f = distill.lm_head_distill
