@@ -178,7 +178,7 @@ def run_pipeline(engine, batch: Dict[str, torch.Tensor], meta: Optional[dict] = 
                 if distill:
                     from ...ops.distill import lm_head_distill
                     divergence, lp, ent = lm_head_distill(pred, model.output_weight, packed.labels, *teacher_of(batch, packed, device),
-                                                          1.0 / temperature, float(kw.get("reverse", 0.0)), want_entropy)
+                                                          1.0 / temperature, float({**actor, **kw}.get("reverse") or 0.0), want_entropy)
                 elif n_top:
                     from ...ops.logprob import lm_head_logprobs
                     lp, ent = lm_head_logprobs(pred, model.output_weight, packed.labels, 1.0 / temperature, want_entropy)

@@ -95,6 +95,10 @@ def test_a_student_that_is_its_own_teacher_has_nothing_to_learn():
     assert abs(r["avg_loss"]) < 1e-5 and float(r["batch"]["divergence"].abs().max()) < 1e-4
     other = worker("log_prob", 6).forward_no_grad(batch, {"temperature": 0.8}, {"loss_fn": "distill"})
     assert other["avg_loss"] > 1e-3
+    # options stand in the call's own arguments or, as those of the policy losses, in the actor's
+    actor, call = (worker("log_prob", 6).forward_no_grad(batch, {"temperature": 0.8, **m}, {"loss_fn": "distill", "loss_kwargs": k})["avg_loss"]
+                   for m, k in (({"actor_config": {"reverse": 1.0}}, {}), ({}, {"reverse": 1.0})))
+    assert actor == pytest.approx(call) and actor != pytest.approx(other["avg_loss"])
 
 
 def test_micro_batches_add_up_and_refusals():
