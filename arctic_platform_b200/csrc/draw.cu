@@ -10,7 +10,7 @@
 // largest logit and adds up the masses (of exp(l / T) itself: 64-bit numbers have the range, so nothing waits for the largest); a warp has a
 // contiguous range, so that a draw from the whole distribution is then a search in 32 sums, in the 32 of that range and in some
 // hundred elements.  A part that fits shared memory is kept there for further walks, a longer one is read again from L2.  A threshold is found
-// by histograms that the CTAs of a cluster read from one another.
+// by histograms that the CTAs of a cluster read from one another; where one CTA has a long row, only of what lies near it, as a sample tells.
 #include "common.cuh"
 #include "host_utils.cuh"
 
@@ -256,16 +256,18 @@ struct DrawRow {
     return s[0] + s[1];
   }
   // the same in whole units of 2^-45
-  __device__ __forceinline__ unsigned long long units(float l) const {
-    return static_cast<unsigned long long>(__double_as_longlong(fma(mass(l), 0x1p45, 4503599627370496.0))) - 0x4330000000000000ull;
+  __device__ __forceinline__ unsigned long long units_of(double mass) const {
+    return static_cast<unsigned long long>(__double_as_longlong(fma(mass, 0x1p45, 4503599627370496.0))) - 0x4330000000000000ull;
   }
+  __device__ __forceinline__ unsigned long long units(float l) const { return units_of(mass(l)); }
 };
 
 // The threshold of a restriction on the elements that each(f) gives f, a warp's share to each warp (all that can matter of them): the least logit of
-// which the strictly larger ones count (MASS: weigh) less than `target`.  The same in every CTA of the row.  At most one call by count and one
-// by mass.
+// which the strictly larger ones count (MASS: weigh) less than `target`, `above` of which lies in elements that are not given; none that is
+// given lies above `top`.  NaN if there is none.  The same in every CTA of the row.
 template <bool MASS, typename Row, typename Each>
-__device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int elements, float per_class, unsigned long long target) {
+__device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int elements, float per_class, unsigned long long target,
+                                float top, unsigned long long above) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // Sums of limbs over `elements` elements of this CTA have to fit 32 bits: additions of 32 bits are carried out by shared memory, those of 64
   // are a loop of comparisons.
@@ -273,14 +275,13 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int ele
   if (tid == 0) sh.limb[MASS] = limb;
   // Classes of a level: 2048 equal steps down from the largest logit (the last takes what is left), 2048 steps of that class, then the bytes
   // of the logits' order, the highest first.
-  unsigned long long above = 0;             // of the elements in higher classes
   uint32_t prefix = 0;
   int first = 0, second = 0;
   for (int level = 0; level < 6; ++level) {
     const int shift = 40 - 8 * level;       // level 2: the highest byte
     // whether an element belongs to the classes chosen so far; its class of this level
     auto in_chosen = [&](float l, int& c) {
-      const float x = l == r.m ? 0.f : (r.m - l) * per_class;
+      const float x = l == top ? 0.f : (top - l) * per_class;
       c = static_cast<int>(fminf(x, kDrawClasses - 1.f));
       if (level == 0) return true;
       if (c != first) return false;
@@ -296,6 +297,7 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int ele
     for (int q = 0; q < (MASS ? 4 : 1); ++q)
 #pragma unroll
       for (int i = 0; i < kDrawPer; ++i) h[q][tid + i * kDrawThreads] = 0;
+    if (tid == 0) sh.chosen = -1;
     __syncthreads();
     each([&](const float (&l)[kDrawGroup]) {
       int c[kDrawGroup];
@@ -362,8 +364,12 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int ele
       }
     }
     __syncthreads();
-    above = sh.above;
     const int chosen = sh.chosen;
+    if (chosen < 0) {
+      row_sync(r.parts);
+      return NAN;
+    }
+    above = sh.above;
     if (level == 5) {                         // all bytes: one value
       row_sync(r.parts);
       return draw_unkey(prefix << 8 | (255u - chosen));
@@ -419,6 +425,78 @@ __device__ float draw_threshold(const Row& r, DrawShared& sh, Each each, int ele
   return -INFINITY;
 }
 
+// A sample of a row, 32 words of every 256: where what it weighs from below comes to 0.8 and to 1.25 of `left`, the mass that a nucleus leaves
+// out (but 16 of the sample above the first).  The nucleus' border lies between, but for bad luck, which draw_threshold sees.  Classes are
+// those of draw_threshold from `m` down to `widest`.  One CTA a row.
+template <typename Row>
+__device__ void draw_bracket(const Row& r, DrawShared& sh, double left, float inv_t, float threshold, float per_class, float widest, float& lower,
+                             float& upper) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+#pragma unroll
+  for (int i = 0; i < kDrawPer; ++i) sh.hist[0][tid + i * kDrawThreads] = sh.hist[1][tid + i * kDrawThreads] = 0;
+  if (tid == 0) sh.chosen = kDrawClasses - 1;
+  __syncthreads();
+  // 2^20 stand for `left`; no more than 2^16 for one, so that an eighth of the largest row adds up in 32 bits
+  static_assert((kDrawMost / 8 + 8192) * 65537ll < 1ll << 32, "weights of a sample");
+  const float lift = static_cast<float>(log(8 * 0x1p20 / left));
+  uint32_t last = 0, lasts = 0;               // of the last class, which has most
+  for (int w = warp * 256 + lane; w < r.words; w += kDrawWarps * 256) {
+    float x[Row::kVec];
+    r.word(w, x);
+#pragma unroll
+    for (int j = 0; j < Row::kVec; ++j) {
+      const float l = x[j];
+      const int c = static_cast<int>(fminf((r.m - l) * per_class, kDrawClasses - 1.f));
+      const uint32_t weight = l >= threshold ? static_cast<uint32_t>(fminf(__expf((l - r.m) * inv_t + lift), 65536.f) + 0.5f) : 0u;
+      if (c < kDrawClasses - 1) {
+        if (l >= threshold) {
+          atomicAdd(&sh.hist[0][c], weight);
+          atomicAdd(&sh.hist[1][c], 1u);
+        }
+      } else {
+        last += weight;
+        lasts += l >= threshold;
+      }
+    }
+  }
+  last = __reduce_add_sync(0xffffffffu, last);
+  lasts = __reduce_add_sync(0xffffffffu, lasts);
+  if (lane == 0) {
+    atomicAdd(&sh.hist[0][kDrawClasses - 1], last);
+    atomicAdd(&sh.hist[1][kDrawClasses - 1], lasts);
+  }
+  __syncthreads();
+  constexpr unsigned long long kWeight = (1ull << 40) - 1;      // the weight; above it the number
+  unsigned long long v[kDrawPer], own = 0;
+#pragma unroll
+  for (int i = 0; i < kDrawPer; ++i) {
+    v[i] = sh.hist[0][kDrawPer * tid + i] | static_cast<unsigned long long>(sh.hist[1][kDrawPer * tid + i]) << 40;
+    own += v[i];
+  }
+  const unsigned long long upto = warp_scan_u64(own, lane);
+  if (lane == 31) sh.scan[warp] = upto;
+  __syncthreads();
+  unsigned long long before = upto - own, all = 0;
+  for (int w = 0; w < kDrawWarps; ++w) {
+    if (w < warp) before += sh.scan[w];
+    all += sh.scan[w];
+  }
+  auto below = [&](unsigned long long x) { return static_cast<uint32_t>((all & kWeight) - (x & kWeight)); };
+  auto low = [&](unsigned long long x) { return below(x) <= 838861u && (x >> 40) >= 16; };
+  auto high = [&](unsigned long long x) { return below(x) >= 1310720u; };
+#pragma unroll
+  for (int i = 0; i < kDrawPer; ++i) {
+    const unsigned long long x = before + v[i];
+    const bool first = kDrawPer * tid + i == 0;
+    if (low(x) && (first || !low(before))) sh.chosen = kDrawPer * tid + i;
+    if (!high(x) && (first || high(before))) sh.owner = kDrawPer * tid + i;       // one there always is: nothing lies below the last
+    before = x;
+  }
+  __syncthreads();
+  lower = sh.chosen == kDrawClasses - 1 ? widest : fmaxf(widest, r.m - (sh.chosen + 1) / per_class);
+  upper = sh.owner == 0 ? INFINITY : r.m - sh.owner / per_class;
+}
+
 // GIVEN: by a given number, else by noise
 template <typename T, bool KEPT, bool GIVEN>
 __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a) {
@@ -440,6 +518,8 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
   r.flat = false;
   r.z = draw_buffer + (4 - r.head % 4) % 4;           // words of the row on words of the buffer
   float* const heavy = draw_buffer + (KEPT ? a.per + 4 : 0) + warp * 32 * a.room;
+  const float p = a.top_p ? a.top_p[b] : a.top_p_all;
+  const bool by_mass = p < 1.f;
 
   for (int i = tid; i < 1024; i += kDrawThreads) {
     const double e = exp2((i >> 4) / 64.0);
@@ -535,8 +615,7 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
   r.cut = m - 70.f * t;
   const int k = a.top_k ? a.top_k[b] : a.top_k_all;
   const float least_share = a.min_p ? a.min_p[b] : a.min_p_all, mp = fminf(least_share, 1.f);
-  const float p = a.top_p ? a.top_p[b] : a.top_p_all;
-  const bool by_rank = k > 0 && k < a.V, by_share = least_share > 0.f, by_mass = p < 1.f;
+  const bool by_rank = k > 0 && k < a.V, by_share = least_share > 0.f;
   // exp((l - m) / T) of this warp's elements >= bound
   auto weigh = [&](float bound, int slot) {
     double s0 = 0.0;
@@ -576,7 +655,7 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
   // what stays: logits >= threshold
   float threshold = -INFINITY;
   if (by_rank)
-    threshold = draw_threshold<false>(r, sh, [&](auto f) { r.walk(warp, lane, NAN, f); }, n, 64.f * inv_t, static_cast<unsigned long long>(k));
+    threshold = draw_threshold<false>(r, sh, [&](auto f) { r.walk(warp, lane, NAN, f); }, n, 64.f * inv_t, static_cast<unsigned long long>(k), m, 0ull);
   if (by_share) {
     // the least fp32 number l with (l - m) / T >= log(min_p), in 64 bits; from a rounded guess it is a step or two
     const double need = log(static_cast<double>(mp)) * static_cast<double>(t);
@@ -605,42 +684,85 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
       const double under = log(least * 0x1p-45) - 1e-5;
       reach = fmaxf(reach, static_cast<float>(static_cast<double>(m) + static_cast<double>(t) * under) - 1e-6f * fabsf(m));
     }
-    // each lane's, in a column of its own of the warp's list
-    int have = 0;
-    r.walk(warp, lane, NAN, [&](const float (&l)[kDrawGroup]) {
-#pragma unroll
-      for (int j = 0; j < kDrawGroup; ++j)
-        if (l[j] >= reach) {
-          if (have < a.room) heavy[have * 32 + lane] = l[j];
-          ++have;
-        }
-    });
-    const int most = __reduce_max_sync(0xffffffffu, have), together = __reduce_add_sync(0xffffffffu, have);
-    if (lane == 0) sh.warp_n[warp] = together;
-    __syncthreads();
-    const int elements = __reduce_add_sync(0xffffffffu, lane < kDrawWarps ? sh.warp_n[lane] : 0);
-    const bool listed = most <= a.room;       // else the warp's range takes the list's place
-    auto each = [&](auto f) {
-      if (!listed) {
-        r.walk(warp, lane, NAN, [&](float (&l)[kDrawGroup]) {
-#pragma unroll
-          for (int j = 0; j < kDrawGroup; ++j) l[j] = l[j] >= reach ? l[j] : NAN;
-          f(l);
-        });
-        return;
-      }
-#pragma unroll 1
-      for (int i = 0; i < most; i += kDrawGroup) {
-        float l[kDrawGroup];
-#pragma unroll
-        for (int j = 0; j < kDrawGroup; ++j) l[j] = i + j < have ? heavy[(i + j) * 32 + lane] : NAN;
-        f(l);
-      }
-    };
-    const float per_class = reach > -INFINITY && reach < m ? fminf((kDrawClasses - 0.1f) / (m - reach), 1e30f) : 64.f * inv_t;
-    threshold = fmaxf(threshold, draw_threshold<true>(r, sh, each, elements, per_class, target));
+    const bool ranged = reach > -INFINITY && reach < m;
+    const float widest = reach, per_class = ranged ? fminf((kDrawClasses - 0.1f) / (m - reach), 1e30f) : 64.f * inv_t;
+    // Of a long row a sample says roughly where the border is: only what lies near it is then sorted, what lies above is added up, and nothing else
+    // is listed.  (128 rows of 151936, top_p = 0.95: 104 us, 182 with everything above `widest` sorted.)  Should the border lie elsewhere, it
+    // is sought once more without.
+    float upper = INFINITY;
+    bool narrow = !KEPT && a.parts == 1 && !redo && ranged && least > 0.0;
+    if (narrow) draw_bracket(r, sh, total - share, inv_t, threshold, per_class, widest, reach, upper);
     double s0 = 0.0;
-    each([&](const float (&l)[kDrawGroup]) { s0 += r.masses(l, threshold); });
+    float border;
+#pragma unroll 1
+    for (;;) {
+      // each lane's, in a column of its own of the warp's list: from the front those up to `upper`, from the back those above
+      const int nowhere = (a.room - 1) * 32 + lane;      // the column's last place takes what is not listed: a store less to decide about
+      int front = lane, back = nowhere - 32;
+      r.walk(warp, lane, NAN, [&](const float (&l)[kDrawGroup]) {
+#pragma unroll
+        for (int j = 0; j < kDrawGroup; ++j) {       // no branches (170 us with them): nearly every warp has some of both kinds
+          const int in = l[j] >= reach, is_high = l[j] >= upper;
+          heavy[front > back || !in ? nowhere : is_high ? back : front] = l[j];
+          back -= is_high * 32;
+          front += (in - is_high) * 32;
+        }
+      });
+      const int have = front / 32, high = (nowhere - 32 - back) / 32;
+      const int most = __reduce_max_sync(0xffffffffu, have), together = __reduce_add_sync(0xffffffffu, have);
+      const bool listed = __reduce_max_sync(0xffffffffu, have + high) < a.room;       // else the warp's range takes the list's place
+      if (lane == 0) sh.warp_n[warp] = together;
+      const bool full = __syncthreads_or(!listed);
+      const int elements = __reduce_add_sync(0xffffffffu, lane < kDrawWarps ? sh.warp_n[lane] : 0);
+      auto each = [&](auto f) {
+        if (!listed) {
+          r.walk(warp, lane, NAN, [&](float (&l)[kDrawGroup]) {
+#pragma unroll
+            for (int j = 0; j < kDrawGroup; ++j) l[j] = l[j] >= reach ? l[j] : NAN;
+            f(l);
+          });
+          return;
+        }
+#pragma unroll 1
+        for (int i = 0; i < most; i += kDrawGroup) {
+          float l[kDrawGroup];
+#pragma unroll
+          for (int j = 0; j < kDrawGroup; ++j) l[j] = i + j < have ? heavy[(i + j) * 32 + lane] : NAN;
+          f(l);
+        }
+      };
+      s0 = 0.0;
+      unsigned long long above = 0;
+      if (narrow && !full) {
+#pragma unroll 1
+        for (int i = 0; i < high; i += kDrawGroup) {
+          double s[2] = {0.0, 0.0};
+#pragma unroll
+          for (int j = 0; j < kDrawGroup; ++j) {
+            const double q = r.mass(i + j < high ? heavy[nowhere - 32 * (1 + i + j)] : NAN);
+            s[j & 1] += q;
+            above += r.units_of(q);
+          }
+          s0 += s[0] + s[1];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+        if (lane == 0) sh.scan[warp] = above;
+        __syncthreads();
+        above = 0;
+        for (int w = 0; w < kDrawWarps; ++w) above += sh.scan[w];
+      }
+      border = narrow && full ? NAN : draw_threshold<true>(r, sh, each, elements, per_class, target, upper < m ? upper : m, above);
+      if (!narrow && !(border == border)) border = reach;
+      if (border == border) {
+        each([&](const float (&l)[kDrawGroup]) { s0 += r.masses(l, border); });
+        break;
+      }
+      narrow = false;
+      reach = widest;
+      upper = INFINITY;
+    }
+    threshold = fmaxf(threshold, border);
     s0 = warp_sum_f64(s0);
     slot ^= 1;
     if (lane == 0) sh.warp_mass[slot][warp] = s0;

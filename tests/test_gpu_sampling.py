@@ -62,6 +62,36 @@ def test_settings_that_are_not_numbers_are_off_and_expanded_rows():
     same(z[:1].expand(6, 5003), u, 0.8, 0, 0.9)
 
 
+@pytest.mark.parametrize("V,dtype", [(24601, torch.float32), (40003, torch.bfloat16), (151936, torch.float32)])
+@pytest.mark.parametrize("top_p", [1e-6, 0.3, 0.9, 0.95, 0.9999])
+def test_nuclei_of_long_rows_that_have_a_cta_each(V, dtype, top_p):
+    """Rows of which a sample says roughly where the nucleus ends: usual ones, sharp and flat ones, and such that the sample misleads."""
+    B = 80                                                     # more than half the SMs: no clusters
+    z, u = make(B, V, dtype, seed=V)
+    same(z, u, 0.7, 0, top_p)
+    z = z.clone()
+    z[0] = 1.0                                                 # all equal
+    z[1, 1:] = -float("inf")
+    z[2] = torch.where(torch.arange(V, device="cuda") % 2 == 0, 0.0, 3.0)
+    z[3] *= 30
+    z[4] *= 0.01
+    z[5] = float("nan")
+    z[6, ::3] = float("nan")
+    z[7, V // 2:] = -float("inf")
+    z[8] = torch.arange(V, device="cuda") / V                  # rising
+    z[9, 17] = 1e30
+    z[10, 17] = float("inf")
+    z[11] = -1e30
+    every = torch.arange(V, device="cuda") // (128 if dtype == torch.float32 else 256) % 8
+    for i in range(8):                                         # one run of eight unlike the others: a sample of those sees another row
+        z[12 + i] = torch.where(every == i, z[12 + i] - 6, z[12 + i])
+        z[20 + i] = torch.where(every == i, z[20 + i] + 4, z[20 + i])
+    z[28:40] = z[28:40].round()                                # many equal ones
+    same(z, u, 0.7, 0, top_p)
+    same(z, u, 1.3, 3000, top_p, 1e-4)
+    same(z, u, torch.linspace(0.2, 3.0, B, device="cuda"), 0, top_p, 1e-3)
+
+
 def test_settings_of_their_own_for_each_row():
     B, V = 48, 5003
     z, u = make(B, V, seed=5)
