@@ -320,8 +320,8 @@ int apb_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, lo
 
 // hidden [N, H] and weight [V, H] bf16 (H, V and the strides multiples of 8, 16-byte aligned), labels [N], names [N, K] int32 (K <= 256),
 // teacher [N, K] fp32, rest [N] fp32 or null, row_scale [N] or null (then `scale` alone).  Scratch: sorted [N, K] int32 and
-// behind it [N][ceil(V / 128)] uint16, partial [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1], named_grad [N, K], others, lse, ent [N] and, if not
-// null, kept [N, V] bf16 (then partial too).
+// behind it [N][ceil(V / 128)] uint16, partial [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1],
+// named_grad [N, K], others, lse, ent [N] and, if not null, kept [N, V] bf16 (then partial too).
 int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* labels, const int* names, const float* teacher,
                            const float* rest, const float* row_scale, float* partial, int* sorted, float* logit, float* value, float* lp,
                            float* ent, float* lse, float* others, float* named_grad, void* kept, int N, int V, int H, int K, long long ldh,

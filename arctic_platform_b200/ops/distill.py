@@ -8,7 +8,8 @@ these classes, q the teacher's masses and p the student's, the divergence is ``(
 
 On CUDA the vocabulary product runs on tcgen05 CTA pairs with an epilogue that reduces every 128 columns to records without the named
 tokens, whose logits are fp32 dot products (``csrc/distill.cu``); the backward pass forms d(logits) in bf16 a chunk of rows at a time, from the
-exponentials that the forward pass kept or from the logits once more, and feeds two products.  CPU tensors use the fp32 expression below (the oracle of the GPU tests).
+exponentials that the forward pass kept or from the logits once more, and feeds two products.  CPU tensors use the
+fp32 expression below (the oracle of the GPU tests).
 """
 from __future__ import annotations
 

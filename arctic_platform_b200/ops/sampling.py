@@ -8,7 +8,8 @@
   times all of it; at ``T <= 0`` the first of the largest logits, whatever the other settings are;
 * its log-probability is that of ``softmax(l / T)`` without restrictions (of ``softmax(l)`` at ``T <= 0``), as a policy's gradient wants it.
 
-The order of the restrictions is that of ``engine/reference_sampler.py``.  Masses are 64-bit numbers.  CUDA tensors run ``csrc/draw.cu``, CPU tensors the expression below (the oracle of the GPU tests).
+The order of the restrictions is that of ``engine/reference_sampler.py``.  Masses are 64-bit numbers.  CUDA tensors run ``csrc/draw.cu``,
+CPU tensors the expression below (the oracle of the GPU tests).
 """
 from __future__ import annotations
 
