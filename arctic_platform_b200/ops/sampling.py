@@ -104,18 +104,19 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Setting = 
     B, V = logits.shape
     if uniforms.dtype not in (torch.float32, torch.float64) or uniforms.shape != (B,):
         raise ValueError(f"uniforms must be fp32 or fp64 [{B}], got {uniforms.dtype} {list(uniforms.shape)}")
+    on = logits.device
     for name, x in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
         if torch.is_tensor(x):
-            if x.shape != (B,) or x.device != logits.device:
-                raise ValueError(f"{name} must be a number or [{B}] on {logits.device}, got {list(x.shape)} on {x.device}")
-            if x.is_floating_point() == (name == "top_k") or x.dtype == torch.bool or x.is_complex():
+            if x.shape != (B,) or x.device != on:
+                raise ValueError(f"{name} must be a number or [{B}] on {on}, got {list(x.shape)} on {x.device}")
+            if x.is_floating_point() == (name == "top_k") or x.dtype is torch.bool or x.is_complex():
                 raise ValueError(f"{name} cannot be {x.dtype}")
-    if uniforms.device != logits.device:
+    if uniforms.device != on:
         raise ValueError(f"uniforms live on {uniforms.device}, logits on {logits.device}")
     if out is not None:
         for name, t, dtype in (("out[0]", out[0], torch.int32), ("out[1]", out[1], torch.float32)):
-            if t.shape != (B,) or t.dtype != dtype or not t.is_contiguous() or t.device != logits.device:
-                raise ValueError(f"{name} must be contiguous {dtype} [{B}] on {logits.device}, got {t.dtype} {list(t.shape)} on {t.device}")
+            if t.shape != (B,) or t.dtype != dtype or not t.is_contiguous() or t.device != on:
+                raise ValueError(f"{name} must be contiguous {dtype} [{B}] on {on}, got {t.dtype} {list(t.shape)} on {t.device}")
     if not logits.is_cuda:
         tokens, logprobs = sample_ref(logits, uniforms, temperature, top_k, top_p, min_p)
         if out is None:
@@ -130,12 +131,13 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Setting = 
             return sample(logits, uniforms, temperature, top_k, top_p, min_p, out)
     if logits.stride(1) != 1:
         logits = logits.contiguous()
-    number = lambda x: x.to(torch.float32).contiguous() if torch.is_tensor(x) else float(x)      # noqa: E731
+    # the usual types pass as they are: a conversion that converts nothing still costs the host a microsecond
+    whole = lambda x, dtype: x if x.dtype is dtype and x.is_contiguous() else x.to(dtype).contiguous()      # noqa: E731
+    number = lambda x: whole(x, torch.float32) if torch.is_tensor(x) else float(x)                            # noqa: E731
     if torch.is_tensor(top_k):
-        top_k = (top_k.clamp(0, V) if top_k.dtype == torch.int64 else top_k).to(torch.int32).contiguous()
+        top_k = whole(top_k.clamp(0, V) if top_k.dtype is torch.int64 else top_k, torch.int32)
     else:
         top_k = max(0, min(int(top_k), V))
-    tokens, logprobs = out if out is not None else (torch.empty(B, device=logits.device, dtype=torch.int32),
-                                                     torch.empty(B, device=logits.device, dtype=torch.float32))
-    draw_raw(logits, uniforms.contiguous(), number(temperature), top_k, number(top_p), number(min_p), tokens, logprobs)
+    tokens, logprobs = out if out is not None else (torch.empty(B, device=on, dtype=torch.int32), torch.empty(B, device=on, dtype=torch.float32))
+    draw_raw(logits, uniforms if uniforms.is_contiguous() else uniforms.contiguous(), number(temperature), top_k, number(top_p), number(min_p), tokens, logprobs)
     return tokens, logprobs
