@@ -14,6 +14,7 @@ fp32 expression below (the oracle of the GPU tests).
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -98,40 +99,46 @@ def _keep_pays(N: int, V: int, device) -> bool:
     return N * V >= _KEEP_FROM and size <= _BWD_BUDGET // 2 and memory_budget.spare_bytes(device, 3 * size) >= 3 * size
 
 
+@functools.lru_cache(maxsize=None)
+def _pairs(device) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count // 2
+
+
 class _LmHeadDistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ids, teacher, rest, inv_temp_t, inv_temp_s, reverse, with_entropy, bwd_chunk):
         N, H = hidden.shape
         V, K = weight.shape[0], ids.shape[1]
         dev, f32 = hidden.device, torch.float32
-        partial = torch.empty((N, (V + 127) // 128, 4), device=dev, dtype=f32)
-        in_order = torch.empty(N * K + (N * partial.shape[1] + 1) // 2, device=dev, dtype=torch.int32)
+        tiles = (V + 127) // 128
+        partial = torch.empty((N, tiles, 4), device=dev, dtype=f32)
+        in_order = torch.empty(N * K + (N * tiles + 1) // 2, device=dev, dtype=torch.int32)
         value, lp, ent = (torch.empty(N, device=dev, dtype=f32) for _ in range(3))
-        # what the backward pass takes up again: logits of the named tokens and the label, gradients of the named ones, two numbers a row and
-        # the exponentials of the others
-        logit, named = torch.empty((N, K + 1), device=dev, dtype=f32), torch.empty((N, K), device=dev, dtype=f32)
-        rows = torch.empty((2, N), device=dev, dtype=f32)
+        # what the backward pass takes up again: log-sum-exp and coefficient of the others of every row, logits [N, K + 1] of the named tokens and
+        # the label, gradients [N, K] of the named ones (one block: an allocation costs the host 3 us) and the exponentials of the others
+        rows = torch.empty(N * (2 * K + 3), device=dev, dtype=f32)
         lse = rows.data_ptr()
+        others, logit, named = lse + 4 * N, lse + 8 * N, lse + 4 * N * (K + 3)
         kept = torch.empty((N, V), device=dev, dtype=torch.bfloat16) if any(ctx.needs_input_grad[:2]) and _keep_pays(N, V, dev) else None
         opt = lambda t: None if t is None else t.data_ptr()                                  # noqa: E731
         _lib.check(_fn("fwd")(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), ids.data_ptr(), teacher.data_ptr(), opt(rest),
-                              opt(inv_temp_t), partial.data_ptr(), in_order.data_ptr(), logit.data_ptr(), value.data_ptr(), lp.data_ptr(),
-                              ent.data_ptr(), lse, lse + 4 * N, named.data_ptr(), opt(kept), N, V, H, K, hidden.stride(0), weight.stride(0),
+                              opt(inv_temp_t), partial.data_ptr(), in_order.data_ptr(), logit, value.data_ptr(), lp.data_ptr(),
+                              ent.data_ptr(), lse, others, named, opt(kept), N, V, H, K, hidden.stride(0), weight.stride(0),
                               inv_temp_s, reverse, _lib.stream_ptr()), "apb_lmhead_distill_fwd")
-        ctx.save_for_backward(hidden, weight, labels, ids, inv_temp_t, logit, named, rows, ent, kept, None if kept is None else partial)
+        ctx.save_for_backward(hidden, weight, labels, ids, inv_temp_t, rows, ent, kept, None if kept is None else partial)
         ctx.inv_temp_s, ctx.with_entropy, ctx.bwd_chunk = inv_temp_s, with_entropy, bwd_chunk
         ctx.set_materialize_grads(False)
-        return value, lp, (ent if with_entropy else lp.new_zeros(0))
+        return value, lp, (ent if with_entropy else None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_value, g_lp, g_ent):
-        hidden, weight, labels, ids, it, logit, named, rows, ent, kept, partial = ctx.saved_tensors
+        hidden, weight, labels, ids, it, rows, ent, kept, partial = ctx.saved_tensors
         N, H = hidden.shape
         V, K = weight.shape[0], ids.shape[1]
         dev = hidden.device
         want_h, want_w = ctx.needs_input_grad[:2]
-        whole = lambda g: None if g is None else g.to(torch.float32).contiguous()            # noqa: E731
+        whole = lambda g: g if g is None or g.dtype is torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()  # noqa: E731
         g_value, g_lp, g_ent = whole(g_value), whole(g_lp), whole(g_ent) if ctx.with_entropy else None
         at = lambda t, s, size: None if t is None else t.data_ptr() + s * size               # noqa: E731
         chunk = ctx.bwd_chunk
@@ -145,14 +152,15 @@ class _LmHeadDistillFn(torch.autograd.Function):
         # one chunk: the weight's gradient leaves its product in its own type; several add up in fp32
         dw = None if not want_w or acc is not None else torch.empty((V, H), device=dev, dtype=weight.dtype) if chunk >= N else \
             torch.zeros((V, H), device=dev, dtype=torch.float32)
-        pairs = torch.cuda.get_device_properties(dev).multi_processor_count // 2
+        pairs = _pairs(dev)
         total = torch.empty((min(chunk, N), H), device=dev, dtype=torch.float32) if want_h and _split_pays(min(chunk, N), H, pairs) else None
         into = acc if acc is not None else dw
         lse, tiles = rows.data_ptr(), (V + 127) // 128
+        others, logit, named = lse + 4 * N, lse + 8 * N, lse + 4 * N * (K + 3)
         for s in range(0, N, chunk):
             n = min(chunk, N - s)
             _lib.check(_fn("bwd")(at(hidden, s, 2 * hidden.stride(0)), weight.data_ptr(), at(ids, s, 4 * K), at(labels, s, 4), at(it, s, 4),
-                                  at(logit, s, 4 * K + 4), at(named, s, 4 * K), lse + 4 * (N + s), lse + 4 * s, at(ent, s, 4),
+                                  logit + 4 * s * (K + 1), named + 4 * s * K, others + 4 * s, lse + 4 * s, at(ent, s, 4),
                                   at(g_value, s, 4), at(g_lp, s, 4), at(g_ent, s, 4), at(kept, s, 2 * V), at(partial, s, 16 * tiles),
                                   scratch.data_ptr(), buf.data_ptr(), at(d_hidden, s, 2 * H), at(total, 0, 4), at(into, 0, 4),
                                   into is not None and into.dtype == torch.float32, n, V, H, K, hidden.stride(0), weight.stride(0),
@@ -210,12 +218,11 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
         raise ValueError("weight must have whole rows on 16-byte boundaries")
     if hidden.stride(1) != 1 or hidden.stride(0) % 8 or hidden.stride(0) < H or hidden.data_ptr() % 16:     # expanded rows too
         hidden = hidden.contiguous()
-    whole = lambda t, dtype: t.detach().to(dtype).contiguous()                               # noqa: E731
+    whole = lambda t, dtype: t if t.dtype is dtype and t.is_contiguous() and not t.requires_grad else t.detach().to(dtype).contiguous()  # noqa: E731
     if teacher_ids.dtype == torch.int64:         # before 32 bits cut them
         teacher_ids = torch.where((teacher_ids < 0) | (teacher_ids >= V), -1, teacher_ids)
     it_t = whole(inv_temperature, torch.float32) if torch.is_tensor(inv_temperature) else None
-    value, lp, ent = _LmHeadDistillFn.apply(
+    return _LmHeadDistillFn.apply(
         hidden, weight, whole(labels, torch.int32), whole(teacher_ids, torch.int32), whole(teacher_logprobs, torch.float32),
         None if teacher_rest is None else whole(teacher_rest, torch.float32), it_t, 1.0 if it_t is not None else float(inv_temperature),
         float(reverse), with_entropy, bwd_chunk)
-    return value, lp, (ent if with_entropy else None)
