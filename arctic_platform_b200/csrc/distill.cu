@@ -22,6 +22,9 @@
 // the mass and of the gradient, and a tensor core's running sum of all H terms is less exact than fp32 sums of a 32nd of them that a warp joins.
 // It costs a read of K rows of the weight for every row (4096 rows with 64 names, H = 2560: 0.23 ms of 8.3).
 //
+// d(logits) is rounded to bf16, the type in which the tensor cores take it with a bf16 weight: an entry is off by 2^-8 of itself at most, and a
+// gradient in norm by 2.1 to 2.9e-3 where its own rounding to bf16 makes 1.7e-3.
+//
 // Time of a whole pass and its gradients at 4096 x 151936 x 2560: 8.3 ms, of which the product 2.17 (with the exponentials kept), spread 0.42,
 // d_hidden 2.12 and d_weight 2.25 (cuBLAS's sustained rate gives 2.25 for each); 10.0 with the logits formed again.  At H = 1024, 549 rows
 // 0.79 ms (0.93).
