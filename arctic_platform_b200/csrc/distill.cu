@@ -11,7 +11,7 @@
 // (and the label's) are put over it afterwards.
 //
 //   named    one CTA per row: the row's names in rising order for the product's epilogue; logits of the named tokens and the label as
-//            dot products in fp32.  An entry below 0 or beyond the vocabulary names nothing, a token named again counts once, by
+//            dot products.  An entry below 0 or beyond the vocabulary names nothing, a token named again counts once, by
 //            its first entry.
 //   product  CTA pairs (gemm_tcgen05_2cta.cu), records of every 128 columns without the named ones and, where there is room, their exponentials
 //   combine  one warp per row: statistics, value, log-prob and entropy of the label's distribution, c and the named places' gradients
@@ -19,7 +19,7 @@
 //            and the label's over that
 //
 // Why the named logits are dot products of their own instead of columns taken out of the product's tiles: the named tokens carry nearly all of
-// the mass and of the gradient, and a tensor core's running sum of all H terms is less exact than fp32 sums of a 32nd of them that a warp joins.
+// the mass and of the gradient, and a tensor core's running sum of all H terms is less exact than 64-bit sums of eight products each.
 // It costs a read of K rows of the weight for every row (4096 rows with 64 names, H = 2560: 0.23 ms of 8.3).
 //
 // d(logits) is rounded to bf16, the type in which the tensor cores take it with a bf16 weight: an entry is off by 2^-8 of itself at most, and a
@@ -37,6 +37,11 @@ namespace apb {
 constexpr int kMostNamed = 256;
 constexpr int kNoName = 0x7fffffff;
 
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 __device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
   const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -54,7 +59,7 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
 __global__ void __launch_bounds__(256)
 distill_named_kernel(const __nv_bfloat16* __restrict__ hidden, long long ldh, const __nv_bfloat16* __restrict__ weight, long long ldw,
                      const int* __restrict__ names, const int* __restrict__ labels, const float* __restrict__ row_scale, float scale, int K,
-                     int V, int H, int* __restrict__ sorted, uint16_t* __restrict__ named_at, float* __restrict__ logit) {
+                     int V, int H, int* __restrict__ sorted, uint16_t* __restrict__ named_at, double* __restrict__ logit) {
   __shared__ int name[kMostNamed];
   __shared__ int kept[kMostNamed];
   const long long row = blockIdx.x;
@@ -95,20 +100,20 @@ distill_named_kernel(const __nv_bfloat16* __restrict__ hidden, long long ldh, co
   const int chunks = H / 8;
   for (int k = warp; k <= K; k += 8) {
     const int id = k < K ? kept[k] : labels[row];
-    float s = 0.f;
+    double s = 0.0;                        // products of two bf16 numbers are exact in fp32, eight of them add up there
     const bool there = id >= 0 && id < V;
     if (there) {
       const uint4* w = reinterpret_cast<const uint4*>(weight + static_cast<long long>(id) * ldw);
-      for (int c = lane; c < chunks; c += 32) s = dot8(h[c], w[c], s);
-      s = warp_sum(s);
+      for (int c = lane; c < chunks; c += 32) s += static_cast<double>(dot8(h[c], w[c], 0.f));
+      s = warp_sum_f64(s);
     }
-    if (lane == 0) logit[row * (K + 1) + k] = there ? s * rs : -INFINITY;
+    if (lane == 0) logit[row * (K + 1) + k] = there ? s * static_cast<double>(rs) : -INFINITY;
   }
 }
 
 struct DistillRows {
   const float4* partial;     // [N][tiles] records of the columns not named
-  const float* logit;        // [N, K + 1]
+  const double* logit;       // [N, K + 1]
   const float* teacher;      // [N, K] log-probabilities
   const float* rest;         // [N] log of the others' mass, or null
   float* value;              // [N]
@@ -121,8 +126,11 @@ struct DistillRows {
   float mix;
 };
 
+// Logits of the named tokens, the log-sum-exp and the value's terms are 64-bit numbers here: a divergence is a small difference of
+// log-probabilities, themselves differences of numbers around 16, and in fp32 was off by up to 1e-5 of itself where rows are few.
 // x * y, 0 where x is: a class without mass adds nothing, whatever its logarithm is
 __device__ __forceinline__ float mass_times(float x, float y) { return x > 0.f ? x * y : 0.f; }
+__device__ __forceinline__ double mass_times(double x, double y) { return x > 0.0 ? x * y : 0.0; }
 
 constexpr int kRecords = 8;      // of a lane in flight (549 rows of 1187 records: 8 us, 27 with one)
 
@@ -130,7 +138,7 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows 
   const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (row >= a.N) return;
   const float4* pr = a.partial + static_cast<long long>(row) * a.tiles;
-  const float* zk = a.logit + static_cast<long long>(row) * (a.K + 1);
+  const double* zk = a.logit + static_cast<long long>(row) * (a.K + 1);
   const float* lq = a.teacher + static_cast<long long>(row) * a.K;
   float m = -INFINITY, s = 0.f, e = 0.f;                // of the tokens not named
   for (int t0 = lane; t0 < a.tiles; t0 += 32 * kRecords) {
@@ -162,51 +170,54 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows 
     m = mn;
   }
   float top = m;
-  for (int k = lane; k < a.K; k += 32) top = fmaxf(top, zk[k]);
+  for (int k = lane; k < a.K; k += 32) top = fmaxf(top, static_cast<float>(zk[k]));
   top = warp_max(top);
-  float st = 0.f, et = 0.f;
+  double st = 0.0, et = 0.0;
   for (int k = lane; k < a.K; k += 32) {
-    const float z = zk[k];
+    const double z = zk[k];
     if (z == -INFINITY) continue;
-    const float x = expf(z - top);
+    const double x = exp(z - top);
     st += x;
     et += x * z;
   }
-  st = warp_sum(st);
-  et = warp_sum(et);
-  const float shift = m == -INFINITY ? 0.f : expf(m - top);
-  const float sum = st + s * shift;
-  const float lse = top + logf(sum);
-  const float ent = lse - (et + e * shift) / sum;
+  st = warp_sum_f64(st);
+  et = warp_sum_f64(et);
+  const double shift = m == -INFINITY ? 0.0 : exp(static_cast<double>(m) - top);
+  const double sum = st + s * shift;
+  const double lse = top + log(sum);
+  const float ent = static_cast<float>(lse - (et + e * shift) / sum);
   // classes
   const bool bucket = a.rest != nullptr;
-  const float lpr = s > 0.f ? m + logf(s) - lse : -INFINITY, pr_ = expf(lpr);
+  const double rest_lp = s > 0.f ? m + log(static_cast<double>(s)) - lse : -INFINITY, rest_p = exp(rest_lp);
+  const float lpr = static_cast<float>(rest_lp), pr_ = expf(lpr);
   const float lqr = bucket ? a.rest[row] : -INFINITY, qr = expf(lqr);
-  float F = 0.f, R = 0.f, Q = 0.f, E = 0.f;
+  double F = 0.0, R = 0.0;
+  float Q = 0.f, E = 0.f;
   for (int k = lane; k < a.K; k += 32) {
-    const float z = zk[k];
+    const double z = zk[k];
     if (z == -INFINITY) continue;
-    const float lp = z - lse, l = lq[k], q = expf(l);
-    F += mass_times(q, l - lp);
+    const double lp = z - lse, l = lq[k];
+    const float q = expf(lq[k]);
+    F += mass_times(static_cast<double>(q), l - lp);
     Q += q;
     if (a.mix != 0.f) {
-      const float p = expf(lp);
+      const double p = exp(lp);
       R += mass_times(p, lp - l);
-      E += mass_times(p, lp - l + 1.f);
+      E += static_cast<float>(mass_times(p, lp - l + 1.0));
     }
   }
-  F = warp_sum(F);
+  F = warp_sum_f64(F);
   Q = warp_sum(Q);
-  R = warp_sum(R);
+  R = warp_sum_f64(R);
   E = warp_sum(E);
   float c = 0.f;
   if (bucket) {
-    F += mass_times(qr, lqr - lpr);
+    F += mass_times(static_cast<double>(qr), lqr - rest_lp);
     Q += qr;
     // below the least normal number (87 below the largest logit) the others' probabilities are zeros to the product's epilogue as well
     c = pr_ >= 1.18e-38f ? -(1.f - a.mix) * (qr / pr_) : 0.f;
     if (a.mix != 0.f) {
-      R += mass_times(pr_, lpr - lqr);
+      R += mass_times(rest_p, rest_lp - lqr);
       E += mass_times(pr_, lpr - lqr + 1.f);
       if (pr_ > 0.f) c += a.mix * (lpr - lqr + 1.f);
     }
@@ -214,20 +225,20 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows 
   c += (1.f - a.mix) * Q;
   if (a.mix != 0.f) c -= a.mix * E;
   for (int k = lane; k < a.K; k += 32) {
-    const float z = zk[k];
+    const double z = zk[k];
     float g = 0.f;
     if (z != -INFINITY) {
-      const float lp = z - lse, p = expf(lp), l = lq[k];
+      const float lp = static_cast<float>(z - lse), p = expf(lp), l = lq[k];
       g = (1.f - a.mix) * (p * Q - expf(l));
       if (a.mix != 0.f) g += a.mix * mass_times(p, lp - l + 1.f - E);
     }
     a.named_grad[static_cast<long long>(row) * a.K + k] = g;
   }
   if (lane == 0) {
-    a.value[row] = a.mix == 0.f ? F : (1.f - a.mix) * F + a.mix * R;
-    a.lp[row] = zk[a.K] - lse;
+    a.value[row] = static_cast<float>(a.mix == 0.f ? F : (1.f - a.mix) * F + a.mix * R);
+    a.lp[row] = static_cast<float>(zk[a.K] - lse);
     a.ent[row] = ent;
-    a.lse[row] = lse;
+    a.lse[row] = static_cast<float>(lse);
     a.others[row] = c;
   }
 }
@@ -277,14 +288,14 @@ __global__ void __launch_bounds__(256) distill_round_kernel(const float4* __rest
 
 // One warp per row: the places of the named tokens, and the label's, in d(logits) [N, V] bf16.
 __global__ void __launch_bounds__(256)
-distill_places_kernel(const int* __restrict__ names, const int* __restrict__ labels, const float* __restrict__ logit,
+distill_places_kernel(const int* __restrict__ names, const int* __restrict__ labels, const double* __restrict__ logit,
                       const float* __restrict__ named_grad, const float* __restrict__ others, const float* __restrict__ lse,
                       const float* __restrict__ ent, const float* __restrict__ g_value, const float* __restrict__ g_lp,
                       const float* __restrict__ g_ent, const float* __restrict__ row_scale, float scale, int K, int V, int N,
                       __nv_bfloat16* __restrict__ d, long long ldd) {
   const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (row >= N) return;
-  const float* zk = logit + static_cast<long long>(row) * (K + 1);
+  const double* zk = logit + static_cast<long long>(row) * (K + 1);
   const int label = labels[row];
   const float rs = scale * (row_scale ? row_scale[row] : 1.f);
   const float gv = g_value ? g_value[row] : 0.f, gl = g_lp ? g_lp[row] : 0.f, ge = g_ent ? g_ent[row] : 0.f, l = lse[row], en = ent[row];
@@ -293,7 +304,7 @@ distill_places_kernel(const int* __restrict__ names, const int* __restrict__ lab
   for (int k = lane; k < K; k += 32) {
     if (zk[k] == -INFINITY) continue;
     const int id = names[static_cast<long long>(row) * K + k];
-    const float lp = zk[k] - l, p = expf(lp);
+    const float lp = static_cast<float>(zk[k] - l), p = expf(lp);
     float g = (gv == 0.f ? 0.f : gv * named_grad[static_cast<long long>(row) * K + k]) - gl * p - ge * mass_times(p, lp + en);
     if (id == label) {
       g += gl;
@@ -303,7 +314,7 @@ distill_places_kernel(const int* __restrict__ names, const int* __restrict__ lab
   }
   label_named = __any_sync(0xffffffffu, label_named);
   if (lane == 0 && !label_named && label >= 0 && label < V) {
-    const float lp = zk[K] - l, p = expf(lp);
+    const float lp = static_cast<float>(zk[K] - l), p = expf(lp);
     to[label] = __float2bfloat16_rn(((gv == 0.f ? 0.f : gv * others[row] * p) - gl * p - ge * mass_times(p, lp + en) + gl) * rs);
   }
 }
@@ -323,10 +334,10 @@ int apb_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, lo
 
 // hidden [N, H] and weight [V, H] bf16 (H, V and the strides multiples of 8, 16-byte aligned), labels [N], names [N, K] int32 (K <= 256),
 // teacher [N, K] fp32, rest [N] fp32 or null, row_scale [N] or null (then `scale` alone).  Scratch: sorted [N, K] int32 and
-// behind it [N][ceil(V / 128)] uint16, partial [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1],
+// behind it [N][ceil(V / 128)] uint16, partial [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1] fp64,
 // named_grad [N, K], others, lse, ent [N] and, if not null, kept [N, V] bf16 (then partial too).
 int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* labels, const int* names, const float* teacher,
-                           const float* rest, const float* row_scale, float* partial, int* sorted, float* logit, float* value, float* lp,
+                           const float* rest, const float* row_scale, float* partial, int* sorted, double* logit, float* value, float* lp,
                            float* ent, float* lse, float* others, float* named_grad, void* kept, int N, int V, int H, int K, long long ldh,
                            long long ldw, float scale, float mix, cudaStream_t stream) {
   using namespace apb;
@@ -374,7 +385,7 @@ int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* la
 // upstream gradients (null: none); the others as kept by the forward pass.  Scratch: scratch [2 N] words of 32 bits; total [N, H] fp32 or null:
 // then d_hidden's product is cut along the vocabulary.
 int apb_lmhead_distill_bwd(const void* hidden, const void* weight, const int* names, const int* labels, const float* row_scale,
-                           const float* logit, const float* named_grad, const float* others, const float* lse, const float* ent,
+                           const double* logit, const float* named_grad, const float* others, const float* lse, const float* ent,
                            const float* g_value, const float* g_lp, const float* g_ent, const void* kept, const float* partial, float* scratch,
                            void* dlogits, void* d_hidden, float* total, void* d_weight, int weight_f32, int N, int V, int H, int K,
                            long long ldh, long long ldw, float scale, cudaStream_t stream) {

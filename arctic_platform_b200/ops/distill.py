@@ -7,7 +7,7 @@ these classes, q the teacher's masses and p the student's, the divergence is ``(
 ``teacher_rest`` both sums run over the named tokens alone (p stays normalised over the whole vocabulary).
 
 On CUDA the vocabulary product runs on tcgen05 CTA pairs with an epilogue that reduces every 128 columns to records without the named
-tokens, whose logits are fp32 dot products (``csrc/distill.cu``); the backward pass forms d(logits) in bf16 a chunk of rows at a time, from the
+tokens, whose logits are dot products of their own (``csrc/distill.cu``); the backward pass forms d(logits) in bf16 a chunk of rows at a time, from the
 exponentials that the forward pass kept or from the logits once more, and feeds two products.  CPU tensors use the
 fp32 expression below (the oracle of the GPU tests).
 """
@@ -114,11 +114,12 @@ class _LmHeadDistillFn(torch.autograd.Function):
         partial = torch.empty((N, tiles, 4), device=dev, dtype=f32)
         in_order = torch.empty(N * K + (N * tiles + 1) // 2, device=dev, dtype=torch.int32)
         value, lp, ent = (torch.empty(N, device=dev, dtype=f32) for _ in range(3))
-        # what the backward pass takes up again: log-sum-exp and coefficient of the others of every row, logits [N, K + 1] of the named tokens and
-        # the label, gradients [N, K] of the named ones (one block: an allocation costs the host 3 us) and the exponentials of the others
-        rows = torch.empty(N * (2 * K + 3), device=dev, dtype=f32)
-        lse = rows.data_ptr()
-        others, logit, named = lse + 4 * N, lse + 8 * N, lse + 4 * N * (K + 3)
+        # what the backward pass takes up again: logits [N, K + 1] of the named tokens and the label in 64 bits, log-sum-exp and coefficient of the
+        # others of every row, gradients [N, K] of the named ones (one block: an allocation costs the host 3 us) and the others' exponentials
+        rows = torch.empty(N * (3 * K + 4), device=dev, dtype=f32)
+        logit = rows.data_ptr()
+        lse = logit + 8 * N * (K + 1)
+        others, named = lse + 4 * N, lse + 8 * N
         kept = torch.empty((N, V), device=dev, dtype=torch.bfloat16) if any(ctx.needs_input_grad[:2]) and _keep_pays(N, V, dev) else None
         opt = lambda t: None if t is None else t.data_ptr()                                  # noqa: E731
         _lib.check(_fn("fwd")(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), ids.data_ptr(), teacher.data_ptr(), opt(rest),
@@ -155,12 +156,13 @@ class _LmHeadDistillFn(torch.autograd.Function):
         pairs = _pairs(dev)
         total = torch.empty((min(chunk, N), H), device=dev, dtype=torch.float32) if want_h and _split_pays(min(chunk, N), H, pairs) else None
         into = acc if acc is not None else dw
-        lse, tiles = rows.data_ptr(), (V + 127) // 128
-        others, logit, named = lse + 4 * N, lse + 8 * N, lse + 4 * N * (K + 3)
+        logit, tiles = rows.data_ptr(), (V + 127) // 128
+        lse = logit + 8 * N * (K + 1)
+        others, named = lse + 4 * N, lse + 8 * N
         for s in range(0, N, chunk):
             n = min(chunk, N - s)
             _lib.check(_fn("bwd")(at(hidden, s, 2 * hidden.stride(0)), weight.data_ptr(), at(ids, s, 4 * K), at(labels, s, 4), at(it, s, 4),
-                                  logit + 4 * s * (K + 1), named + 4 * s * K, others + 4 * s, lse + 4 * s, at(ent, s, 4),
+                                  logit + 8 * s * (K + 1), named + 4 * s * K, others + 4 * s, lse + 4 * s, at(ent, s, 4),
                                   at(g_value, s, 4), at(g_lp, s, 4), at(g_ent, s, 4), at(kept, s, 2 * V), at(partial, s, 16 * tiles),
                                   scratch.data_ptr(), buf.data_ptr(), at(d_hidden, s, 2 * H), at(total, 0, 4), at(into, 0, 4),
                                   into is not None and into.dtype == torch.float32, n, V, H, K, hidden.stride(0), weight.stride(0),
