@@ -7,6 +7,7 @@
 // KV cache layout: [num_pages, Hkv, 16, D] bf16 -- the 16 tokens of one (page, head)
 // are one contiguous 4 KB tile (D = 128).
 #include "common.cuh"
+#include "draw_noise.cuh"
 #include "host_utils.cuh"
 #include "paged_mma.cuh"
 
@@ -650,14 +651,6 @@ __global__ void __launch_bounds__(256) decode_advance_kernel(const DecodeAdvance
 }
 
 // ---------------------------------------------------------------------------- sampling
-__device__ __forceinline__ uint32_t hash_u32(uint32_t x) {
-  x ^= x >> 16;
-  x *= 0x7feb352dU;
-  x ^= x >> 15;
-  x *= 0x846ca68bU;
-  x ^= x >> 16;
-  return x;
-}
 // Order-preserving map float -> uint32 (larger float = larger key) and back.
 __device__ __forceinline__ uint32_t float_key(float z) {
   const uint32_t u = __float_as_uint(z);
@@ -845,8 +838,7 @@ sample_kernel(const float* __restrict__ logits, long long ldl, const float* __re
   const float* row = logits + b * ldl;
   const float cut = (thr && !greedy) ? thr[b] : -INFINITY;
   SampleRec r{-INFINITY, 0.f, -INFINITY, 0.f, 0};
-  // one hash per element: the per-(seed, step, row) part is mixed once, the column enters by a Weyl step
-  const uint32_t base = hash_u32(seed ^ (step * 0x9E3779B9u)) ^ hash_u32(static_cast<uint32_t>(b) * 0x85ebca6bU + 1u);
+  const uint32_t base = noise_base(seed, step, b);
   auto consider = [&](float raw, int i) {
     const float z = raw * invT;
     // running softmax statistics with ONE exponential per element (the rescaling branch is taken only when a new
@@ -859,13 +851,7 @@ sample_kernel(const float* __restrict__ logits, long long ldl, const float* __re
     }
     float key = z;
     if (!greedy) {
-      if (z >= cut) {
-        const uint32_t h = hash_u32(base + static_cast<uint32_t>(i) * 0x9E3779B9u);
-        const float u = (static_cast<float>(h >> 8) + 0.5f) * (1.f / 16777216.f);
-        key = z - __logf(-__logf(u));
-      } else {
-        key = -INFINITY;  // outside the top-k / top-p set
-      }
+      key = z >= cut ? z + draw_noise(base, i) : -INFINITY;      // -inf: outside the top-k / top-p set
     }
     if (key > r.best) {
       r.best = key;

@@ -17,6 +17,7 @@
 // quarters of it), with a nucleus of 0.95 104 us (chains of short steps of one CTA behind two walks), one row of 151936 in a cluster of 8
 // 19 us (latency).
 #include "common.cuh"
+#include "draw_noise.cuh"
 #include "host_utils.cuh"
 
 namespace apb {
@@ -58,14 +59,6 @@ __device__ __forceinline__ uint32_t draw_key(float z) {      // larger logit, la
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float draw_unkey(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
-__device__ __forceinline__ uint32_t draw_hash(uint32_t x) {
-  x ^= x >> 16;
-  x *= 0x7feb352dU;
-  x ^= x >> 15;
-  x *= 0x846ca68bU;
-  x ^= x >> 16;
-  return x;
-}
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -778,7 +771,7 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
     // The largest of l / T and a noise of each token's own, numbers and rounding as in decode.cu's draws: a restriction changes what is drawn only
     // where it leaves that token out, and logits that differ in their last bits seldom change it.
     const uint32_t step = a.step ? static_cast<uint32_t>(*a.step) : 0u, seed = a.seed_dev ? static_cast<uint32_t>(*a.seed_dev) : a.seed;
-    const uint32_t base = draw_hash(seed ^ (step * 0x9E3779B9u)) ^ draw_hash(static_cast<uint32_t>(b) * 0x85ebca6bU + 1u);
+    const uint32_t base = noise_base(seed, step, b);
     float best = -INFINITY;
     int best_i = 0x7fffffff;
     const int hi = r.to(warp);
@@ -786,9 +779,7 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
     for (int i = r.from(warp) + lane; i < hi; i += 32) {
       const float l = r.at(i);
       if (!(l >= threshold)) continue;
-      const uint32_t h = draw_hash(base + static_cast<uint32_t>(begin + i) * 0x9E3779B9u);
-      const float x = (static_cast<float>(h >> 8) + 0.5f) * (1.f / 16777216.f);
-      const float key = l * inv_t - __logf(-__logf(x));
+      const float key = l * inv_t + draw_noise(base, begin + i);
       if (key > best) {
         best = key;
         best_i = begin + i;
