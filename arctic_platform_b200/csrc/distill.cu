@@ -119,15 +119,17 @@ struct DistillRows {
   float* value;              // [N]
   float* lp;
   float* ent;
-  float* lse;
+  double* lse;
+  float* ref;                // the same in fp32
   float* others;             // c: d value / d z of a token not named is this times its probability
   float* named_grad;         // [N, K] d value / d z of the named ones
   int tiles, K, N;
   float mix;
 };
 
-// Logits of the named tokens, the log-sum-exp and the value's terms are 64-bit numbers here: a divergence is a small difference of
-// log-probabilities, themselves differences of numbers around 16, and in fp32 was off by up to 1e-5 of itself where rows are few.
+// Logits of the named tokens, the log-sum-exp and the terms of the value and of its gradient are 64-bit numbers here.  A divergence is a small
+// difference of log-probabilities, themselves differences of numbers around 16, and in fp32 was off by up to 1e-5 of itself where rows are
+// few.  The terms of a gradient cancel where a student is sure or near its teacher: in fp32 they left 1e-7 times the upstream gradient.
 // x * y, 0 where x is: a class without mass adds nothing, whatever its logarithm is
 __device__ __forceinline__ float mass_times(float x, float y) { return x > 0.f ? x * y : 0.f; }
 __device__ __forceinline__ double mass_times(double x, double y) { return x > 0.0 ? x * y : 0.0; }
@@ -188,58 +190,57 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows 
   const float ent = static_cast<float>(lse - (et + e * shift) / sum);
   // classes
   const bool bucket = a.rest != nullptr;
+  const double mix = a.mix, one_way = 1.0 - mix;
   const double rest_lp = s > 0.f ? m + log(static_cast<double>(s)) - lse : -INFINITY, rest_p = exp(rest_lp);
-  const float lpr = static_cast<float>(rest_lp), pr_ = expf(lpr);
-  const float lqr = bucket ? a.rest[row] : -INFINITY, qr = expf(lqr);
-  double F = 0.0, R = 0.0;
-  float Q = 0.f, E = 0.f;
+  const double lqr = bucket ? a.rest[row] : -INFINITY, qr = exp(lqr);
+  double F = 0.0, R = 0.0, Q = 0.0, E = 0.0;
   for (int k = lane; k < a.K; k += 32) {
     const double z = zk[k];
     if (z == -INFINITY) continue;
-    const double lp = z - lse, l = lq[k];
-    const float q = expf(lq[k]);
-    F += mass_times(static_cast<double>(q), l - lp);
+    const double lp = z - lse, l = lq[k], q = exp(l);
+    F += mass_times(q, l - lp);
     Q += q;
     if (a.mix != 0.f) {
       const double p = exp(lp);
       R += mass_times(p, lp - l);
-      E += static_cast<float>(mass_times(p, lp - l + 1.0));
+      E += mass_times(p, lp - l + 1.0);
     }
   }
   F = warp_sum_f64(F);
-  Q = warp_sum(Q);
+  Q = warp_sum_f64(Q);
   R = warp_sum_f64(R);
-  E = warp_sum(E);
-  float c = 0.f;
+  E = warp_sum_f64(E);
+  double c = 0.0;
   if (bucket) {
-    F += mass_times(static_cast<double>(qr), lqr - rest_lp);
+    F += mass_times(qr, lqr - rest_lp);
     Q += qr;
     // below the least normal number (87 below the largest logit) the others' probabilities are zeros to the product's epilogue as well
-    c = pr_ >= 1.18e-38f ? -(1.f - a.mix) * (qr / pr_) : 0.f;
+    c = rest_p >= 1.18e-38 ? -one_way * (qr / rest_p) : 0.0;
     if (a.mix != 0.f) {
       R += mass_times(rest_p, rest_lp - lqr);
-      E += mass_times(pr_, lpr - lqr + 1.f);
-      if (pr_ > 0.f) c += a.mix * (lpr - lqr + 1.f);
+      E += mass_times(rest_p, rest_lp - lqr + 1.0);
+      if (rest_p > 0.0) c += mix * (rest_lp - lqr + 1.0);
     }
   }
-  c += (1.f - a.mix) * Q;
-  if (a.mix != 0.f) c -= a.mix * E;
+  c += one_way * Q;
+  if (a.mix != 0.f) c -= mix * E;
   for (int k = lane; k < a.K; k += 32) {
     const double z = zk[k];
-    float g = 0.f;
+    double g = 0.0;
     if (z != -INFINITY) {
-      const float lp = static_cast<float>(z - lse), p = expf(lp), l = lq[k];
-      g = (1.f - a.mix) * (p * Q - expf(l));
-      if (a.mix != 0.f) g += a.mix * mass_times(p, lp - l + 1.f - E);
+      const double lp = z - lse, p = exp(lp), l = lq[k];
+      g = one_way * (p * Q - exp(l));
+      if (a.mix != 0.f) g += mix * mass_times(p, lp - l + 1.0 - E);
     }
-    a.named_grad[static_cast<long long>(row) * a.K + k] = g;
+    a.named_grad[static_cast<long long>(row) * a.K + k] = static_cast<float>(g);
   }
   if (lane == 0) {
-    a.value[row] = static_cast<float>(a.mix == 0.f ? F : (1.f - a.mix) * F + a.mix * R);
+    a.value[row] = static_cast<float>(a.mix == 0.f ? F : one_way * F + mix * R);
     a.lp[row] = static_cast<float>(zk[a.K] - lse);
     a.ent[row] = ent;
-    a.lse[row] = static_cast<float>(lse);
-    a.others[row] = c;
+    a.lse[row] = lse;
+    a.ref[row] = static_cast<float>(lse);
+    a.others[row] = static_cast<float>(c);
   }
 }
 
@@ -255,15 +256,15 @@ distill_rows_kernel(const float* __restrict__ g_value, const float* __restrict__
 }
 
 // d(logits) of the tokens not named from what the forward product kept of them, exp(z - m) of every 128 columns' largest m in bf16: times
-// exp(m - lse) and the row's coefficient.  One CTA per row, 16 bytes a thread; bound by memory (4096 x 151936: 2.5 GB, 0.4 ms, where forming the
+// exp(m - ref) and the row's coefficient.  One CTA per row, 16 bytes a thread; bound by memory (4096 x 151936: 2.5 GB, 0.4 ms, where forming the
 // logits again takes 2.1).  The named places hold zeros.  A value is rounded twice, by 2^-8 at most each time; the named tokens, which
 // carry nearly all of a row's gradient, and the label are written from fp32 behind this.
 __global__ void __launch_bounds__(256)
 distill_spread_kernel(const uint4* __restrict__ kept, const float4* __restrict__ partial, const float* __restrict__ glp,
-                      const float* __restrict__ lse, const float* __restrict__ row_scale, float scale, int V, uint4* __restrict__ d) {
+                      const float* __restrict__ ref, const float* __restrict__ row_scale, float scale, int V, uint4* __restrict__ d) {
   const long long row = blockIdx.x;
   const int units = V / 8, tiles = (V + 127) / 128;
-  const float c = -glp[row] * scale * (row_scale ? row_scale[row] : 1.f), l = lse[row];
+  const float c = -glp[row] * scale * (row_scale ? row_scale[row] : 1.f), l = ref[row];
 #pragma unroll 4
   for (int u = threadIdx.x; u < units; u += 256) {
     const uint4 x = __ldcs(kept + row * units + u);
@@ -286,10 +287,11 @@ __global__ void __launch_bounds__(256) distill_round_kernel(const float4* __rest
   }
 }
 
-// One warp per row: the places of the named tokens, and the label's, in d(logits) [N, V] bf16.
+// One warp per row: the places of the named tokens, and the label's, in d(logits) [N, V] bf16.  Log-probabilities come from the 64-bit
+// log-sum-exp, and the label's 1 - p from its own: where a student is sure of a token, 1 - p of an fp32 log-sum-exp around 50 is off by 2e-6.
 __global__ void __launch_bounds__(256)
 distill_places_kernel(const int* __restrict__ names, const int* __restrict__ labels, const double* __restrict__ logit,
-                      const float* __restrict__ named_grad, const float* __restrict__ others, const float* __restrict__ lse,
+                      const float* __restrict__ named_grad, const float* __restrict__ others, const double* __restrict__ lse,
                       const float* __restrict__ ent, const float* __restrict__ g_value, const float* __restrict__ g_lp,
                       const float* __restrict__ g_ent, const float* __restrict__ row_scale, float scale, int K, int V, int N,
                       __nv_bfloat16* __restrict__ d, long long ldd) {
@@ -298,24 +300,22 @@ distill_places_kernel(const int* __restrict__ names, const int* __restrict__ lab
   const double* zk = logit + static_cast<long long>(row) * (K + 1);
   const int label = labels[row];
   const float rs = scale * (row_scale ? row_scale[row] : 1.f);
-  const float gv = g_value ? g_value[row] : 0.f, gl = g_lp ? g_lp[row] : 0.f, ge = g_ent ? g_ent[row] : 0.f, l = lse[row], en = ent[row];
+  const float gv = g_value ? g_value[row] : 0.f, gl = g_lp ? g_lp[row] : 0.f, ge = g_ent ? g_ent[row] : 0.f, en = ent[row];
+  const double l = lse[row];
   __nv_bfloat16* to = d + row * ldd;
   bool label_named = false;
   for (int k = lane; k < K; k += 32) {
     if (zk[k] == -INFINITY) continue;
     const int id = names[static_cast<long long>(row) * K + k];
     const float lp = static_cast<float>(zk[k] - l), p = expf(lp);
-    float g = (gv == 0.f ? 0.f : gv * named_grad[static_cast<long long>(row) * K + k]) - gl * p - ge * mass_times(p, lp + en);
-    if (id == label) {
-      g += gl;
-      label_named = true;
-    }
-    to[id] = __float2bfloat16_rn(g * rs);
+    const float g = (gv == 0.f ? 0.f : gv * named_grad[static_cast<long long>(row) * K + k]) - ge * mass_times(p, lp + en);
+    if (id == label) label_named = true;
+    to[id] = __float2bfloat16_rn((g - gl * (id == label ? expm1f(lp) : p)) * rs);
   }
   label_named = __any_sync(0xffffffffu, label_named);
   if (lane == 0 && !label_named && label >= 0 && label < V) {
     const float lp = static_cast<float>(zk[K] - l), p = expf(lp);
-    to[label] = __float2bfloat16_rn(((gv == 0.f ? 0.f : gv * others[row] * p) - gl * p - ge * mass_times(p, lp + en) + gl) * rs);
+    to[label] = __float2bfloat16_rn(((gv == 0.f ? 0.f : gv * others[row] * p) - gl * expm1f(lp) - ge * mass_times(p, lp + en)) * rs);
   }
 }
 
@@ -334,15 +334,15 @@ int apb_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, lo
 
 // hidden [N, H] and weight [V, H] bf16 (H, V and the strides multiples of 8, 16-byte aligned), labels [N], names [N, K] int32 (K <= 256),
 // teacher [N, K] fp32, rest [N] fp32 or null, row_scale [N] or null (then `scale` alone).  Scratch: sorted [N, K] int32 and
-// behind it [N][ceil(V / 128)] uint16, partial [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1] fp64,
-// named_grad [N, K], others, lse, ent [N] and, if not null, kept [N, V] bf16 (then partial too).
+// behind it [N][ceil(V / 128)] uint16, partial [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1] and
+// lse [N] fp64, named_grad [N, K], others, ref (lse in fp32), ent [N] and, if not null, kept [N, V] bf16 (then partial too).
 int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* labels, const int* names, const float* teacher,
                            const float* rest, const float* row_scale, float* partial, int* sorted, double* logit, float* value, float* lp,
-                           float* ent, float* lse, float* others, float* named_grad, void* kept, int N, int V, int H, int K, long long ldh,
+                           float* ent, double* lse, float* ref, float* others, float* named_grad, void* kept, int N, int V, int H, int K, long long ldh,
                            long long ldw, float scale, float mix, cudaStream_t stream) {
   using namespace apb;
   if (N <= 0) return 0;
-  if (!hidden || !weight || !labels || !partial || !value || !lp || !ent || !lse || !others || !logit || K < 0 || K > kMostNamed ||
+  if (!hidden || !weight || !labels || !partial || !value || !lp || !ent || !lse || !ref || !others || !logit || K < 0 || K > kMostNamed ||
       (K > 0 && (!names || !teacher || !sorted || !named_grad)) || V <= 0 || H <= 0 || (H % 8) || (V % 8) || (ldh % 8) || (ldw % 8) ||
       ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15))
     return kBadArgument;
@@ -373,7 +373,7 @@ int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* la
   p.status = status_device_ptr();
   rc = launch_gemm_pair(ta, tb, p, stream);
   if (rc) return rc;
-  DistillRows a{reinterpret_cast<const float4*>(partial), logit, teacher, rest, value, lp, ent, lse, others, named_grad, (V + 127) / 128, K, N,
+  DistillRows a{reinterpret_cast<const float4*>(partial), logit, teacher, rest, value, lp, ent, lse, ref, others, named_grad, (V + 127) / 128, K, N,
                 mix};
   distill_combine_kernel<<<(N + 7) / 8, 256, 0, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
@@ -385,13 +385,13 @@ int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* la
 // upstream gradients (null: none); the others as kept by the forward pass.  Scratch: scratch [2 N] words of 32 bits; total [N, H] fp32 or null:
 // then d_hidden's product is cut along the vocabulary.
 int apb_lmhead_distill_bwd(const void* hidden, const void* weight, const int* names, const int* labels, const float* row_scale,
-                           const double* logit, const float* named_grad, const float* others, const float* lse, const float* ent,
+                           const double* logit, const float* named_grad, const float* others, const double* lse, const float* ref, const float* ent,
                            const float* g_value, const float* g_lp, const float* g_ent, const void* kept, const float* partial, float* scratch,
                            void* dlogits, void* d_hidden, float* total, void* d_weight, int weight_f32, int N, int V, int H, int K,
                            long long ldh, long long ldw, float scale, cudaStream_t stream) {
   using namespace apb;
   if (N <= 0) return 0;
-  if (!hidden || !weight || !labels || !logit || !others || !lse || !ent || !scratch || !dlogits || K < 0 || K > kMostNamed ||
+  if (!hidden || !weight || !labels || !logit || !others || !lse || !ref || !ent || !scratch || !dlogits || K < 0 || K > kMostNamed ||
       (K > 0 && (!names || !named_grad)) || V <= 0 || H <= 0 || (V % 8) || (H % 8) || (kept && !partial))
     return kBadArgument;
   int* no_label = reinterpret_cast<int*>(scratch + N);
@@ -400,11 +400,11 @@ int apb_lmhead_distill_bwd(const void* hidden, const void* weight, const int* na
   if (e != cudaSuccess) return static_cast<int>(e);
   int rc = 0;
   if (kept && !g_ent) {
-    distill_spread_kernel<<<N, 256, 0, stream>>>(static_cast<const uint4*>(kept), reinterpret_cast<const float4*>(partial), scratch, lse, row_scale,
+    distill_spread_kernel<<<N, 256, 0, stream>>>(static_cast<const uint4*>(kept), reinterpret_cast<const float4*>(partial), scratch, ref, row_scale,
                                                  scale, V, static_cast<uint4*>(dlogits));
     rc = static_cast<int>(cudaGetLastError());
   } else {
-    rc = apb_lmhead_dlogits(hidden, weight, no_label, row_scale, lse, ent, scratch, g_ent, dlogits, N, V, H, ldh, ldw, V, scale, stream);
+    rc = apb_lmhead_dlogits(hidden, weight, no_label, row_scale, ref, ent, scratch, g_ent, dlogits, N, V, H, ldh, ldw, V, scale, stream);
   }
   if (rc) return rc;
   distill_places_kernel<<<(N + 7) / 8, 256, 0, stream>>>(names, labels, logit, named_grad, others, lse, ent, g_value, g_lp, g_ent, row_scale,

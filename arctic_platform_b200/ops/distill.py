@@ -32,8 +32,8 @@ def _fn(name: str):
     if not _FN:
         c, fns = ctypes, {}
         vp, i, ll, f = c.c_void_p, c.c_int, c.c_longlong, c.c_float
-        fns["fwd"] = _lib.declare("apb_lmhead_distill_fwd", [vp] * 17 + [i, i, i, i, ll, ll, f, f, vp])
-        fns["bwd"] = _lib.declare("apb_lmhead_distill_bwd", [vp] * 20 + [i, i, i, i, i, ll, ll, f, vp])
+        fns["fwd"] = _lib.declare("apb_lmhead_distill_fwd", [vp] * 18 + [i, i, i, i, ll, ll, f, f, vp])
+        fns["bwd"] = _lib.declare("apb_lmhead_distill_bwd", [vp] * 21 + [i, i, i, i, i, ll, ll, f, vp])
         _FN.update(fns)              # in one step: another thread may be looking
     return _FN[name]
 
@@ -104,6 +104,14 @@ def _pairs(device) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count // 2
 
 
+def _row_places(rows: torch.Tensor, N: int, K: int) -> Tuple[int, int, int, int, int]:
+    """Addresses of logits ``[N, K + 1]`` and log-sum-exp ``[N]`` (fp64), of that in fp32, the others' coefficients ``[N]`` and the named gradients
+    ``[N, K]`` in the block that a forward pass keeps."""
+    logit = rows.data_ptr()
+    lse = logit + 8 * N * (K + 1)
+    return logit, lse, lse + 8 * N, lse + 12 * N, lse + 16 * N
+
+
 class _LmHeadDistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ids, teacher, rest, inv_temp_t, inv_temp_s, reverse, with_entropy, bwd_chunk):
@@ -114,17 +122,16 @@ class _LmHeadDistillFn(torch.autograd.Function):
         partial = torch.empty((N, tiles, 4), device=dev, dtype=f32)
         in_order = torch.empty(N * K + (N * tiles + 1) // 2, device=dev, dtype=torch.int32)
         value, lp, ent = (torch.empty(N, device=dev, dtype=f32) for _ in range(3))
-        # what the backward pass takes up again: logits [N, K + 1] of the named tokens and the label in 64 bits, log-sum-exp and coefficient of the
-        # others of every row, gradients [N, K] of the named ones (one block: an allocation costs the host 3 us) and the others' exponentials
-        rows = torch.empty(N * (3 * K + 4), device=dev, dtype=f32)
-        logit = rows.data_ptr()
-        lse = logit + 8 * N * (K + 1)
-        others, named = lse + 4 * N, lse + 8 * N
+        # what the backward pass takes up again: logits [N, K + 1] of the named tokens and the label and log-sum-exp [N] in 64 bits, that in 32,
+        # coefficient of the others of every row, gradients [N, K] of the named ones (one block: an allocation costs the host 3 us) and the
+        # others' exponentials
+        rows = torch.empty(N * (3 * K + 6), device=dev, dtype=f32)
+        logit, lse, ref, others, named = _row_places(rows, N, K)
         kept = torch.empty((N, V), device=dev, dtype=torch.bfloat16) if any(ctx.needs_input_grad[:2]) and _keep_pays(N, V, dev) else None
         opt = lambda t: None if t is None else t.data_ptr()                                  # noqa: E731
         _lib.check(_fn("fwd")(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), ids.data_ptr(), teacher.data_ptr(), opt(rest),
                               opt(inv_temp_t), partial.data_ptr(), in_order.data_ptr(), logit, value.data_ptr(), lp.data_ptr(),
-                              ent.data_ptr(), lse, others, named, opt(kept), N, V, H, K, hidden.stride(0), weight.stride(0),
+                              ent.data_ptr(), lse, ref, others, named, opt(kept), N, V, H, K, hidden.stride(0), weight.stride(0),
                               inv_temp_s, reverse, _lib.stream_ptr()), "apb_lmhead_distill_fwd")
         ctx.save_for_backward(hidden, weight, labels, ids, inv_temp_t, rows, ent, kept, None if kept is None else partial)
         ctx.inv_temp_s, ctx.with_entropy, ctx.bwd_chunk = inv_temp_s, with_entropy, bwd_chunk
@@ -156,14 +163,13 @@ class _LmHeadDistillFn(torch.autograd.Function):
         pairs = _pairs(dev)
         total = torch.empty((min(chunk, N), H), device=dev, dtype=torch.float32) if want_h and _split_pays(min(chunk, N), H, pairs) else None
         into = acc if acc is not None else dw
-        logit, tiles = rows.data_ptr(), (V + 127) // 128
-        lse = logit + 8 * N * (K + 1)
-        others, named = lse + 4 * N, lse + 8 * N
+        logit, lse, ref, others, named = _row_places(rows, N, K)
+        tiles = (V + 127) // 128
         for s in range(0, N, chunk):
             n = min(chunk, N - s)
             _lib.check(_fn("bwd")(at(hidden, s, 2 * hidden.stride(0)), weight.data_ptr(), at(ids, s, 4 * K), at(labels, s, 4), at(it, s, 4),
-                                  logit + 8 * s * (K + 1), named + 4 * s * K, others + 4 * s, lse + 4 * s, at(ent, s, 4),
-                                  at(g_value, s, 4), at(g_lp, s, 4), at(g_ent, s, 4), at(kept, s, 2 * V), at(partial, s, 16 * tiles),
+                                  logit + 8 * s * (K + 1), named + 4 * s * K, others + 4 * s, lse + 8 * s, ref + 4 * s,
+                                  at(ent, s, 4), at(g_value, s, 4), at(g_lp, s, 4), at(g_ent, s, 4), at(kept, s, 2 * V), at(partial, s, 16 * tiles),
                                   scratch.data_ptr(), buf.data_ptr(), at(d_hidden, s, 2 * H), at(total, 0, 4), at(into, 0, 4),
                                   into is not None and into.dtype == torch.float32, n, V, H, K, hidden.stride(0), weight.stride(0),
                                   ctx.inv_temp_s, _lib.stream_ptr()), "apb_lmhead_distill_bwd")
