@@ -8,7 +8,8 @@
 //                   = p_v c,  c = (1 - mix) (Q - qr / pr) + mix (lpr - lqr + 1 - E)  for any other (without the class of the others
 //                                                                                  qr / pr = 0 and lpr - lqr + 1 = 0).
 // So the rows' gradient is dense only as a multiple of p, which is what the log-prob head's backward epilogue writes; the K named places
-// (and the label's) are put over it afterwards.
+// (and the label's) are put over it afterwards.  Where pr is so small that p_v leaves fp32's range it is a multiple of p_v / pr instead, a softmax
+// of the others alone.
 //
 //   named    one CTA per row: the row's names in rising order for the product's epilogue; logits of the named tokens and the label as
 //            dot products.  An entry below 0 or beyond the vocabulary names nothing, a token named again counts once, by
@@ -120,8 +121,8 @@ struct DistillRows {
   float* lp;
   float* ent;
   double* lse;
-  float* ref;                // the same in fp32
-  float* others;             // c: d value / d z of a token not named is this times its probability
+  float* ref;                // d value / d z_v of a token not named is others exp(z_v - ref); lse in fp32, or that of the others alone
+  float* others;
   float* named_grad;         // [N, K] d value / d z of the named ones
   int tiles, K, N;
   float mix;
@@ -133,6 +134,10 @@ struct DistillRows {
 // x * y, 0 where x is: a class without mass adds nothing, whatever its logarithm is
 __device__ __forceinline__ float mass_times(float x, float y) { return x > 0.f ? x * y : 0.f; }
 __device__ __forceinline__ double mass_times(double x, double y) { return x > 0.0 ? x * y : 0.0; }
+
+// Where the log of the others' mass is below this their probabilities come near the end of fp32's range (2^-126, 87 below the largest), but not the
+// gradient that the teacher's mass of them asks for: it is formed from their shares of their own sum.
+constexpr double kLeastRest = -69.0;
 
 constexpr int kRecords = 8;      // of a lane in flight (549 rows of 1187 records: 8 us, 27 with one)
 
@@ -210,12 +215,12 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows 
   Q = warp_sum_f64(Q);
   R = warp_sum_f64(R);
   E = warp_sum_f64(E);
+  const bool far = bucket && s > 0.f && rest_lp < kLeastRest;
   double c = 0.0;
   if (bucket) {
     F += mass_times(qr, lqr - rest_lp);
     Q += qr;
-    // below the least normal number (87 below the largest logit) the others' probabilities are zeros to the product's epilogue as well
-    c = rest_p >= 1.18e-38 ? -one_way * (qr / rest_p) : 0.0;
+    if (!far && s > 0.f) c = -one_way * (qr / rest_p);
     if (a.mix != 0.f) {
       R += mass_times(rest_p, rest_lp - lqr);
       E += mass_times(rest_p, rest_lp - lqr + 1.0);
@@ -224,6 +229,7 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows 
   }
   c += one_way * Q;
   if (a.mix != 0.f) c -= mix * E;
+  if (far) c = mass_times(rest_p, c) - one_way * qr;           // c pr, without the quotient
   for (int k = lane; k < a.K; k += 32) {
     const double z = zk[k];
     double g = 0.0;
@@ -239,20 +245,23 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const DistillRows 
     a.lp[row] = static_cast<float>(zk[a.K] - lse);
     a.ent[row] = ent;
     a.lse[row] = lse;
-    a.ref[row] = static_cast<float>(lse);
+    a.ref[row] = static_cast<float>(far ? lse + rest_lp : lse);
     a.others[row] = static_cast<float>(c);
   }
 }
 
-// The upstream gradient of a log-prob that would give every token not named what it gets: minus the coefficient of its probability.
+// The upstream gradient of a log-prob that would give every token not named what it gets: minus the coefficient of exp(z - ref).  Where ref is not
+// the log-sum-exp, the others' probabilities add up to less than e^-69, and the entropy's gradient of them, below 100 times that, is left out.
 __global__ void __launch_bounds__(256)
-distill_rows_kernel(const float* __restrict__ g_value, const float* __restrict__ g_lp, const float* __restrict__ others, int N,
-                    float* __restrict__ out, int* __restrict__ no_label) {
+distill_rows_kernel(const float* __restrict__ g_value, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
+                    const float* __restrict__ others, const double* __restrict__ lse, const float* __restrict__ ref, int N,
+                    float* __restrict__ out, int* __restrict__ no_label, float* __restrict__ out_ent) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= N) return;
-  const float g = g_value ? g_value[i] : 0.f;
-  out[i] = (g_lp ? g_lp[i] : 0.f) - (g == 0.f ? 0.f : g * others[i]);
+  const float g = g_value ? g_value[i] : 0.f, gl = g_lp ? g_lp[i] : 0.f, l = static_cast<float>(lse[i]), r = ref[i];
+  out[i] = (r == l ? gl : gl * expf(r - l)) - (g == 0.f ? 0.f : g * others[i]);
   no_label[i] = -1;
+  if (g_ent) out_ent[i] = r == l ? g_ent[i] : 0.f;
 }
 
 // d(logits) of the tokens not named from what the forward product kept of them, exp(z - m) of every 128 columns' largest m in bf16: times
@@ -292,7 +301,7 @@ __global__ void __launch_bounds__(256) distill_round_kernel(const float4* __rest
 __global__ void __launch_bounds__(256)
 distill_places_kernel(const int* __restrict__ names, const int* __restrict__ labels, const double* __restrict__ logit,
                       const float* __restrict__ named_grad, const float* __restrict__ others, const double* __restrict__ lse,
-                      const float* __restrict__ ent, const float* __restrict__ g_value, const float* __restrict__ g_lp,
+                      const float* __restrict__ ref, const float* __restrict__ ent, const float* __restrict__ g_value, const float* __restrict__ g_lp,
                       const float* __restrict__ g_ent, const float* __restrict__ row_scale, float scale, int K, int V, int N,
                       __nv_bfloat16* __restrict__ d, long long ldd) {
   const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
@@ -315,7 +324,8 @@ distill_places_kernel(const int* __restrict__ names, const int* __restrict__ lab
   label_named = __any_sync(0xffffffffu, label_named);
   if (lane == 0 && !label_named && label >= 0 && label < V) {
     const float lp = static_cast<float>(zk[K] - l), p = expf(lp);
-    to[label] = __float2bfloat16_rn(((gv == 0.f ? 0.f : gv * others[row] * p) - gl * expm1f(lp) - ge * mass_times(p, lp + en)) * rs);
+    const float share = expf(static_cast<float>(zk[K] - ref[row]));
+    to[label] = __float2bfloat16_rn(((gv == 0.f ? 0.f : gv * others[row] * share) - gl * expm1f(lp) - ge * mass_times(p, lp + en)) * rs);
   }
 }
 
@@ -335,7 +345,7 @@ int apb_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, lo
 // hidden [N, H] and weight [V, H] bf16 (H, V and the strides multiples of 8, 16-byte aligned), labels [N], names [N, K] int32 (K <= 256),
 // teacher [N, K] fp32, rest [N] fp32 or null, row_scale [N] or null (then `scale` alone).  Scratch: sorted [N, K] int32 and
 // behind it [N][ceil(V / 128)] uint16, partial [N][ceil(V / 128)][4] fp32.  Kept for the backward pass: logit [N, K + 1] and
-// lse [N] fp64, named_grad [N, K], others, ref (lse in fp32), ent [N] and, if not null, kept [N, V] bf16 (then partial too).
+// lse [N] fp64, named_grad [N, K], others, ref, ent [N] and, if not null, kept [N, V] bf16 (then partial too).
 int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* labels, const int* names, const float* teacher,
                            const float* rest, const float* row_scale, float* partial, int* sorted, double* logit, float* value, float* lp,
                            float* ent, double* lse, float* ref, float* others, float* named_grad, void* kept, int N, int V, int H, int K, long long ldh,
@@ -382,7 +392,7 @@ int apb_lmhead_distill_fwd(const void* hidden, const void* weight, const int* la
 // The backward pass of N rows of a forward pass: d(logits) [N, V] bf16, of it d_hidden [N, H] bf16 and d_weight [V, H] (bf16, or fp32 that is
 // added to), either may be null.  d(logits): the coefficients of the probabilities; probability times coefficient, from what the forward
 // pass kept or, without it or with g_ent, by the product again; the named tokens' places and the label's.  g_value, g_lp, g_ent [N] fp32:
-// upstream gradients (null: none); the others as kept by the forward pass.  Scratch: scratch [2 N] words of 32 bits; total [N, H] fp32 or null:
+// upstream gradients (null: none); the others as kept by the forward pass.  Scratch: scratch [3 N] words of 32 bits; total [N, H] fp32 or null:
 // then d_hidden's product is cut along the vocabulary.
 int apb_lmhead_distill_bwd(const void* hidden, const void* weight, const int* names, const int* labels, const float* row_scale,
                            const double* logit, const float* named_grad, const float* others, const double* lse, const float* ref, const float* ent,
@@ -395,7 +405,8 @@ int apb_lmhead_distill_bwd(const void* hidden, const void* weight, const int* na
       (K > 0 && (!names || !named_grad)) || V <= 0 || H <= 0 || (V % 8) || (H % 8) || (kept && !partial))
     return kBadArgument;
   int* no_label = reinterpret_cast<int*>(scratch + N);
-  distill_rows_kernel<<<(N + 255) / 256, 256, 0, stream>>>(g_value, g_lp, others, N, scratch, no_label);
+  float* ent_rows = scratch + 2ll * N;
+  distill_rows_kernel<<<(N + 255) / 256, 256, 0, stream>>>(g_value, g_lp, g_ent, others, lse, ref, N, scratch, no_label, ent_rows);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
   int rc = 0;
@@ -404,10 +415,10 @@ int apb_lmhead_distill_bwd(const void* hidden, const void* weight, const int* na
                                                  scale, V, static_cast<uint4*>(dlogits));
     rc = static_cast<int>(cudaGetLastError());
   } else {
-    rc = apb_lmhead_dlogits(hidden, weight, no_label, row_scale, ref, ent, scratch, g_ent, dlogits, N, V, H, ldh, ldw, V, scale, stream);
+    rc = apb_lmhead_dlogits(hidden, weight, no_label, row_scale, ref, ent, scratch, g_ent ? ent_rows : nullptr, dlogits, N, V, H, ldh, ldw, V, scale, stream);
   }
   if (rc) return rc;
-  distill_places_kernel<<<(N + 7) / 8, 256, 0, stream>>>(names, labels, logit, named_grad, others, lse, ent, g_value, g_lp, g_ent, row_scale,
+  distill_places_kernel<<<(N + 7) / 8, 256, 0, stream>>>(names, labels, logit, named_grad, others, lse, ref, ent, g_value, g_lp, g_ent, row_scale,
                                                          scale, K, V, N, static_cast<__nv_bfloat16*>(dlogits), V);
   e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);

@@ -105,8 +105,8 @@ def _pairs(device) -> int:
 
 
 def _row_places(rows: torch.Tensor, N: int, K: int) -> Tuple[int, int, int, int, int]:
-    """Addresses of logits ``[N, K + 1]`` and log-sum-exp ``[N]`` (fp64), of that in fp32, the others' coefficients ``[N]`` and the named gradients
-    ``[N, K]`` in the block that a forward pass keeps."""
+    """Addresses of logits ``[N, K + 1]`` and log-sum-exp ``[N]`` (fp64), the others' references and coefficients ``[N]`` and the named
+    gradients ``[N, K]`` in the block that a forward pass keeps."""
     logit = rows.data_ptr()
     lse = logit + 8 * N * (K + 1)
     return logit, lse, lse + 8 * N, lse + 12 * N, lse + 16 * N
@@ -122,7 +122,7 @@ class _LmHeadDistillFn(torch.autograd.Function):
         partial = torch.empty((N, tiles, 4), device=dev, dtype=f32)
         in_order = torch.empty(N * K + (N * tiles + 1) // 2, device=dev, dtype=torch.int32)
         value, lp, ent = (torch.empty(N, device=dev, dtype=f32) for _ in range(3))
-        # what the backward pass takes up again: logits [N, K + 1] of the named tokens and the label and log-sum-exp [N] in 64 bits, that in 32,
+        # what the backward pass takes up again: logits [N, K + 1] of the named tokens and the label and log-sum-exp [N] in 64 bits, reference and
         # coefficient of the others of every row, gradients [N, K] of the named ones (one block: an allocation costs the host 3 us) and the
         # others' exponentials
         rows = torch.empty(N * (3 * K + 6), device=dev, dtype=f32)
@@ -154,7 +154,7 @@ class _LmHeadDistillFn(torch.autograd.Function):
             chunk = _bwd_rows(N, V, memory_budget.spare_bytes(dev, _BWD_BUDGET) if N > _BWD_ROWS else 0)
         buf_rows = min(chunk, N) if ctx.bwd_chunk or N <= _BWD_ROWS else -(-chunk // _BWD_ROWS) * _BWD_ROWS
         buf = torch.empty((buf_rows, V), device=dev, dtype=torch.bfloat16)
-        scratch = torch.empty(2 * min(chunk, N), device=dev, dtype=torch.float32)
+        scratch = torch.empty(3 * min(chunk, N), device=dev, dtype=torch.float32)
         d_hidden = torch.empty((N, H), device=dev, dtype=hidden.dtype) if want_h else None
         acc = getattr(weight, "grad_f32", None) if want_w else None
         # one chunk: the weight's gradient leaves its product in its own type; several add up in fp32
