@@ -114,7 +114,7 @@ def _row_places(rows: torch.Tensor, N: int, K: int) -> Tuple[int, int, int, int,
 
 class _LmHeadDistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, labels, ids, teacher, rest, inv_temp_t, inv_temp_s, reverse, with_entropy, bwd_chunk):
+    def forward(ctx, hidden, weight, labels, ids, teacher, rest, inv_temp_t, inv_temp_s, reverse, with_entropy, bwd_chunk, grads):
         N, H = hidden.shape
         V, K = weight.shape[0], ids.shape[1]
         dev, f32 = hidden.device, torch.float32
@@ -127,7 +127,8 @@ class _LmHeadDistillFn(torch.autograd.Function):
         # others' exponentials
         rows = torch.empty(N * (3 * K + 6), device=dev, dtype=f32)
         logit, lse, ref, others, named = _row_places(rows, N, K)
-        kept = torch.empty((N, V), device=dev, dtype=torch.bfloat16) if any(ctx.needs_input_grad[:2]) and _keep_pays(N, V, dev) else None
+        keep = grads and any(ctx.needs_input_grad[:2]) and _keep_pays(N, V, dev)
+        kept = torch.empty((N, V), device=dev, dtype=torch.bfloat16) if keep else None
         opt = lambda t: None if t is None else t.data_ptr()                                  # noqa: E731
         _lib.check(_fn("fwd")(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), ids.data_ptr(), teacher.data_ptr(), opt(rest),
                               opt(inv_temp_t), partial.data_ptr(), in_order.data_ptr(), logit, value.data_ptr(), lp.data_ptr(),
@@ -175,7 +176,7 @@ class _LmHeadDistillFn(torch.autograd.Function):
                                   ctx.inv_temp_s, _lib.stream_ptr()), "apb_lmhead_distill_bwd")
         if dw is not None and dw.dtype != weight.dtype:
             dw = dw.to(weight.dtype)
-        return d_hidden, dw, None, None, None, None, None, None, None, None, None
+        return (d_hidden, dw) + (None,) * 10
 
 
 def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, teacher_ids: torch.Tensor,
@@ -233,4 +234,4 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     return _LmHeadDistillFn.apply(
         hidden, weight, whole(labels, torch.int32), whole(teacher_ids, torch.int32), whole(teacher_logprobs, torch.float32),
         None if teacher_rest is None else whole(teacher_rest, torch.float32), it_t, 1.0 if it_t is not None else float(inv_temperature),
-        float(reverse), with_entropy, bwd_chunk)
+        float(reverse), with_entropy, bwd_chunk, torch.is_grad_enabled())      # which is off within the function, whatever its inputs need
