@@ -94,7 +94,8 @@ _KEEP_FROM = 1 << 26      # probabilities from which on keeping them pays: below
 
 def _keep_pays(N: int, V: int, device) -> bool:
     """Whether the forward pass keeps the exponentials of its logits in bf16 for the backward pass, which then need not form the logits again
-    (a quarter of its products): where the device has room for them and for the gradient beside."""
+    (a quarter of its products): where the device has room for them and for the gradient beside.  Kept ones are rounded to bf16 once more, so that
+    the last bits of a gradient depend on it."""
     size = 2 * N * V
     return N * V >= _KEEP_FROM and size <= _BWD_BUDGET // 2 and memory_budget.spare_bytes(device, 3 * size) >= 3 * size
 
@@ -127,7 +128,9 @@ class _LmHeadDistillFn(torch.autograd.Function):
         # others' exponentials
         rows = torch.empty(N * (3 * K + 6), device=dev, dtype=f32)
         logit, lse, ref, others, named = _row_places(rows, N, K)
-        keep = grads and any(ctx.needs_input_grad[:2]) and _keep_pays(N, V, dev)
+        # not by what memory happens to be free where the caller bounds it, or wants the same bits each time
+        may = bwd_chunk is None and not torch.are_deterministic_algorithms_enabled()
+        keep = grads and may and any(ctx.needs_input_grad[:2]) and _keep_pays(N, V, dev)
         kept = torch.empty((N, V), device=dev, dtype=torch.bfloat16) if keep else None
         opt = lambda t: None if t is None else t.data_ptr()                                  # noqa: E731
         _lib.check(_fn("fwd")(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), ids.data_ptr(), teacher.data_ptr(), opt(rest),
@@ -152,7 +155,8 @@ class _LmHeadDistillFn(torch.autograd.Function):
         at = lambda t, s, size: None if t is None else t.data_ptr() + s * size               # noqa: E731
         chunk = ctx.bwd_chunk
         if chunk is None:
-            chunk = _bwd_rows(N, V, memory_budget.spare_bytes(dev, _BWD_BUDGET) if N > _BWD_ROWS else 0)
+            fixed = N <= _BWD_ROWS or torch.are_deterministic_algorithms_enabled()
+            chunk = _bwd_rows(N, V, 0 if fixed else memory_budget.spare_bytes(dev, _BWD_BUDGET))
         buf_rows = min(chunk, N) if ctx.bwd_chunk or N <= _BWD_ROWS else -(-chunk // _BWD_ROWS) * _BWD_ROWS
         buf = torch.empty((buf_rows, V), device=dev, dtype=torch.bfloat16)
         scratch = torch.empty(3 * min(chunk, N), device=dev, dtype=torch.float32)
@@ -190,7 +194,12 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     An entry of ``teacher_ids`` outside the vocabulary (-1 by custom) names nothing; a token named again in a row counts once, by its
     first entry.  A row that names nothing has divergence 0 without ``teacher_rest``.  A class that the teacher gives no mass (a
     log-probability of ``-inf``) makes the reverse divergence infinite.  ``inv_temperature`` is a float or a per-row tensor ``[N]``.
-    On CUDA: bf16 hidden states and weights, H and V multiples of 8, K at most 256."""
+    On CUDA: bf16 hidden states and weights, H and V multiples of 8, K at most 256.
+
+    ``bwd_chunk``: rows of d(logits) that the backward pass forms at a time.  Without it the backward pass takes more memory where the device has
+    it to spare: the probabilities of the forward pass, rounded to bf16 (2 N V bytes, from 2^26 of them on), and more rows at a time.  With it, or under
+    ``torch.use_deterministic_algorithms``, what is computed does not depend on that.  d(logits) is a bf16 tensor either way, so that a gradient
+    is off by 2.3 to 2.5e-3 of its norm, 1.7e-3 of it its own rounding."""
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"hidden {list(hidden.shape)} and weight {list(weight.shape)} must be [N, H] and [V, H]")
     N, H = hidden.shape
