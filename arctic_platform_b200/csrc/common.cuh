@@ -334,8 +334,9 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// The same for one load's registers; nothing that reads them can move in front of it.
+// Waits for this warp's loads from tensor memory.  The registers of a load are named, so that nothing that reads them can move in front of it: to the
+// compiler they hold their values from the load on, and arithmetic on registers is not kept behind a statement that does not name them.  After
+// several loads each one's registers are named.
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),

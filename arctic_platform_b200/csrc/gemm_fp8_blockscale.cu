@@ -126,7 +126,7 @@ gemm_fp8_bs_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_const
       for (int c = 0; c < 4; ++c) {
         uint32_t v[32];
         tmem_ld_32x32(tmem_base + lane_off + buf * 128 + c * 32, v);
-        tmem_ld_wait();
+        tmem_ld_wait(v);
 #pragma unroll
         for (int i = 0; i < 32; ++i) acc[c * 32 + i] += __uint_as_float(v[i]) * sc;
       }

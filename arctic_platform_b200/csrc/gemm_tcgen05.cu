@@ -319,7 +319,8 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tma_a, const CUtens
         uint32_t acc[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32(taddr + c * 32, acc[c]);
-        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait(acc[c]);
         lmhead_partial_128(p, row, row_ok, acc, n0);
         tc_fence_before();
         __syncwarp();
@@ -334,7 +335,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tma_a, const CUtens
           if (col0 >= p.N) break;
           uint32_t r[32];
           tmem_ld_32x32(taddr + c * 32, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           if (!row_ok) continue;
           __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.C) + static_cast<long long>(row) * p.ldc + col0;
 #pragma unroll
@@ -362,14 +363,14 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tma_a, const CUtens
         if (BN % 32 != 0 && ncols == 16) {
           uint32_t h[16];
           tmem_ld_32x16(taddr + c * 32, h);
-          tmem_ld_wait();
+          tmem_ld_wait(h);
 #pragma unroll
           for (int j = 0; j < 16; ++j) r[j] = h[j];
 #pragma unroll
           for (int j = 16; j < 32; ++j) r[j] = 0u;
         } else {
           tmem_ld_32x32(taddr + c * 32, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
         }
         // a box of 32 x 32 per warp; columns that it holds beyond the tile's are added as zeros.  Rows: it belongs to the tile as a
         // whole, or the map ends with the tile's rows; a box that would reach into another group's rows goes the other way.

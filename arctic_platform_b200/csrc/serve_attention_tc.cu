@@ -205,7 +205,7 @@ sigmoid_attn_tc_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_c
         for (int c = 0; c < kStcKeys / 32; ++c) {
           uint32_t r[32], pk[16];
           tmem_ld_32x32(t_s + c * 32, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             // sigmoid(z) = 1 / (1 + 2^(-z log2 e)); one reciprocal serves two weights (exponents are capped so that
@@ -234,7 +234,7 @@ sigmoid_attn_tc_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_c
         for (int c = 0; c < p.E; c += 32) {
           uint32_t r[32];
           tmem_ld_32x32(t_o + c, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
           if (row < q_valid) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)

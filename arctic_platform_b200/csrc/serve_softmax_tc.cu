@@ -260,11 +260,11 @@ softmax_attn_tc_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_c
         if (c < p.E) {
           uint32_t r[32];
           tmem_ld_32x32(tmem_base + lane_off + 256 + c, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[n][i] = __uint_as_float(r[i]) * i0;
           tmem_ld_32x32(tmem_base + lane_off + 384 + c, r);
-          tmem_ld_wait();
+          tmem_ld_wait(r);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             o[n][i] = c + i < p.E ? o[n][i] - __uint_as_float(r[i]) * i1 : 0.f;
