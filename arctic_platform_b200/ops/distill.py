@@ -234,8 +234,9 @@ def lm_head_distill(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
                                    bwd_chunk)
     if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.stride(0) < H or weight.data_ptr() % 16:
         raise ValueError("weight must have whole rows on 16-byte boundaries")
-    if hidden.stride(1) != 1 or hidden.stride(0) % 8 or hidden.stride(0) < H or hidden.data_ptr() % 16:     # expanded rows too
-        hidden = hidden.contiguous()
+    # expanded rows too; contiguous() would leave dense rows off their boundary, and a single row of any stride, as they are
+    if hidden.stride(1) != 1 or hidden.stride(0) % 8 or hidden.stride(0) < H or hidden.data_ptr() % 16:
+        hidden = hidden.clone(memory_format=torch.contiguous_format)
     whole = lambda t, dtype: t if t.dtype is dtype and t.is_contiguous() and not t.requires_grad else t.detach().to(dtype).contiguous()  # noqa: E731
     if teacher_ids.dtype == torch.int64:         # before 32 bits cut them
         teacher_ids = torch.where((teacher_ids < 0) | (teacher_ids >= V), -1, teacher_ids)
