@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
   if (r.flat) m = 0.f;
   const float inv_t = 1.f / t;
   r.m = m;
-  r.cut = m - 70.f * t;
+  r.cut = m - 693.f * t;                      // 2^-1000 of the largest's mass, as far as a table and 64 bits reach
   const int k = a.top_k ? a.top_k[b] : a.top_k_all;
   const float least_share = a.min_p ? a.min_p[b] : a.min_p_all, mp = fminf(least_share, 1.f);
   const bool by_rank = k > 0 && k < a.V, by_share = least_share > 0.f;
@@ -826,8 +826,13 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
     }
     row_sync(a.parts);
   } else {
-    // masses of what stays
-    if (by_rank || by_share || by_mass) {
+    double u = a.u64 ? static_cast<const double*>(a.u)[b] : static_cast<double>(static_cast<const float*>(a.u)[b]);
+    // 1 and above, and what is not a number, stand for the largest number below 1
+    u = u < 1.0 ? fmax(u, 0.0) : 1.0 - 0x1p-52;
+    // Masses of what stays.  The first walk's sums hold 2^-1000 for every element below that, which is next to nothing beside any u but those next
+    // to 0 (torch.rand gives 0 once in 2^24): these want to know which ranges have any mass.
+    const bool restricted = by_rank || by_share || by_mass, weighed = restricted || redo || u < 0x1p-60;
+    if (restricted || (weighed && !redo)) {
       if (!by_mass) weigh(threshold, slot ^= 1);
       factor = 1.0;
       row_sync(a.parts);
@@ -842,12 +847,10 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
 #pragma unroll
       for (int j = 0; j < kDrawRanges; ++j) total += v[j];
       const double upto = warp_scan_f64(total, lane);
-      double u = a.u64 ? static_cast<const double*>(a.u)[b] : static_cast<double>(static_cast<const float*>(a.u)[b]);
-      // 1 and above, and what is not a number, stand for the largest number below 1
-      u = u < 1.0 ? fmax(u, 0.0) : 1.0 - 0x1p-52;
       const double target = u * __shfl_sync(0xffffffffu, upto, 31);
-      // a range of less than 2^-80 has only elements that a mass is not formed of (below e^-70 of the largest), or none
-      const unsigned behind = __ballot_sync(0xffffffffu, total > 0x1p-80 && target < upto), some = __ballot_sync(0xffffffffu, total > 0x1p-80);
+      // a range of the first walk's with less than 2^-80 may have none: its sum is what its elements' places are worth
+      const double none = weighed ? 0.0 : 0x1p-80;
+      const unsigned behind = __ballot_sync(0xffffffffu, total > none && target < upto), some = __ballot_sync(0xffffffffu, total > none);
       const int owner = behind ? __ffs(behind) - 1 : 31 - __clz(some);
       double before = __shfl_up_sync(0xffffffffu, upto, 1);
       if (lane == 0) before = 0.0;
@@ -857,12 +860,12 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
         bool found = false;
 #pragma unroll
         for (int j = 0; j < kDrawRanges; ++j) {
-          if (!found && v[j] > 0x1p-80) {
+          if (!found && v[j] > none) {
             range = j;
             begins = before;
           }
           before += v[j];
-          found = found || (v[j] > 0x1p-80 && target < before);
+          found = found || (v[j] > none && target < before);
         }
         sh.owner = lane * kDrawRanges + range;
         sh.before = target - begins;            // within the range

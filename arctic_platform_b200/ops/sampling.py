@@ -5,7 +5,8 @@
 * the tokens stay whose logit is at least the ``top_k``-th largest, those with ``exp((l - max) / T) >= min_p``, and of what is left those of
   which the strictly larger ones hold less than ``top_p`` of its mass (equal logits stay or go together, the largest always stay);
 * the token is the first one, in the order of the vocabulary, up to which, itself included, the mass of what stayed is above ``u``
-  times all of it; at ``T <= 0`` the first of the largest logits, whatever the other settings are;
+  times all of it (a mass below e^-693 of the largest one's counts as none); at ``T <= 0`` the first of the largest logits, whatever the
+  other settings are;
 * its log-probability is that of ``softmax(l / T)`` without restrictions (of ``softmax(l)`` at ``T <= 0``), as a policy's gradient wants it.
 
 The order of the restrictions is that of ``engine/reference_sampler.py``.  Masses are 64-bit numbers.  CUDA tensors run ``csrc/draw.cu``,
@@ -65,7 +66,7 @@ def sample_ref(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
     T = torch.where(greedy, 1.0, T)
     most = z.amax(-1, keepdim=True)
     x = torch.where(z == most, 0.0, (z - torch.where(torch.isinf(most) & (most < 0), 0.0, most)) / T)
-    full = x.exp()
+    full = torch.where(x < -693.0, 0.0, x.exp())
     order = torch.sort(z, dim=-1, descending=True).values
     kth = order.gather(1, torch.where((k > 0) & (k < V), k, V) - 1)
     keep = (z >= kth) & ((m <= 0) | torch.isnan(m) | (x >= torch.log(m.clamp_max(1.0))))
