@@ -15,7 +15,7 @@
 //            dot products.  An entry below 0 or beyond the vocabulary names nothing, a token named again counts once, by
 //            its first entry.
 //   product  CTA pairs (gemm_tcgen05_2cta.cu), records of every 128 columns without the named ones and, where there is room, their exponentials
-//   combine  one warp per row: statistics, value, log-prob and entropy of the label's distribution, c and the named places' gradients
+//   combine  one warp per row: statistics, value, log-prob and entropy of the label's distribution, c and the named places' gradients, in 64 bits
 //   rows     the coefficient of p in the backward pass; spread  the kept exponentials times it (or the product again); places  the named places
 //            and the label's over that
 //
@@ -24,7 +24,9 @@
 // It costs a read of K rows of the weight for every row (4096 rows with 64 names, H = 2560: 0.23 ms of 8.3).
 //
 // d(logits) is rounded to bf16, the type in which the tensor cores take it with a bf16 weight: an entry is off by 2^-8 of itself at most, and a
-// gradient in norm by 2.1 to 2.9e-3 where its own rounding to bf16 makes 1.7e-3.
+// gradient in norm by 2.3 to 2.5e-3 where its own rounding to bf16 makes 1.7e-3.  That is one more rounding of the named entries, which hold
+// nearly all of it; that of the kept exponentials does not show in three digits.  A second product for what the rounding leaves would take another
+// 4.4 of 8.3 ms.
 //
 // Time of a whole pass and its gradients at 4096 x 151936 x 2560: 8.3 ms, of which the product 2.17 (with the exponentials kept), spread 0.42,
 // d_hidden 2.12 and d_weight 2.25 (cuBLAS's sustained rate gives 2.25 for each); 10.0 with the logits formed again.  At H = 1024, 549 rows

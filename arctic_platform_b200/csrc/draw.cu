@@ -686,8 +686,9 @@ __global__ void __launch_bounds__(kDrawThreads, 1) draw_kernel(const DrawArgs a)
     const bool ranged = reach > -INFINITY && reach < m;
     const float widest = reach, per_class = ranged ? fminf((kDrawClasses - 0.1f) / (m - reach), 1e30f) : 64.f * inv_t;
     // Of a long row a sample says roughly where the border is: only what lies near it is then sorted, what lies above is added up, and nothing else
-    // is listed.  (128 rows of 151936, top_p = 0.95: 104 us, 182 with everything above `widest` sorted.)  Should the border lie elsewhere, it
-    // is sought once more without.
+    // is listed.  (128 rows of 151936, top_p = 0.95: 103 us, 182 with everything above `widest` sorted.)  Should the border lie elsewhere, it
+    // is sought once more without, as it is where the lists do not hold what lies above: 44032 of 151936 logits, which the nuclei of flat rows
+    // exceed (T = 1, top_p 0.95: 242 us; T = 1.3: 316; in 16 bits 507 and 323).
     float upper = INFINITY;
     bool narrow = !KEPT && a.parts == 1 && !redo && ranged && least > 0.0;
     if (narrow) draw_bracket(r, sh, total - share, inv_t, threshold, per_class, widest, reach, upper);

@@ -476,8 +476,9 @@ static int launch_top_as(TopArgs a, int N, cudaStream_t s) {
 
 template <typename T>
 static int launch_top(const TopArgs& a, int N, cudaStream_t s) {
-  // 256 threads, four CTAs an SM, wait for one another less (2048 rows of 151936, k = 64: 345 us, 435 with 512); from about 100 on their
-  // buffer is filled too often (256 rows of 248320, k = 128: 112 us against 100)
+  // 256 threads, four CTAs an SM, wait for one another less, but their buffer is filled more often.  Where both break even goes with the rows: near
+  // k = 220 for 2048 rows of 151936 (k = 64 / 96 / 128 / 192: 344 / 364 / 390 / 469 us, 412 / 422 / 446 / 475 with 512), 160 for 333 and 200 for
+  // 1024 of 32000, but below 48 for 256 long rows in 16 bits (248320, k = 64 / 96 / 128 / 192: 97 / 99 / 113 / 131 us, 93 / 90 / 101 / 101)
   if (a.k <= 96) return launch_top_as<T, 512, 256>(a, N, s);
   return a.k <= 256 ? launch_top_as<T, 1024, 512>(a, N, s) : launch_top_as<T, 2048, 512>(a, N, s);
 }

@@ -89,7 +89,9 @@ def _split_pays(n: int, H: int, pairs: int) -> bool:
     return tiles < 0.85 * pairs * -(-tiles // pairs)
 
 
-_KEEP_FROM = 1 << 26      # probabilities from which on keeping them pays: below, looking for the memory takes as long as forming them again
+# Probabilities from which on keeping them pays.  With the memory at hand it saves 20 us of 360 at 1e7 of them, 56 of 703 to 222 of 2186 at 6e7
+# (H = 1024 and 2560), and costs 22 of 205 at 1e6; but where the allocator has not enough, asking the driver takes 150 us to 2 ms.
+_KEEP_FROM = 1 << 26
 
 
 def _keep_pays(N: int, V: int, device) -> bool:
